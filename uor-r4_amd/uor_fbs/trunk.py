@@ -1,0 +1,390 @@
+"""The float trunk's operators on the GPU (include/uor_trunk.h): the selective state space scan and
+its short causal convolution (packed sequences, their gradients, single tokens over device slots),
+and the norms before and after a block fused with its gate and residual scale (and their gradients).
+
+Every function takes and returns torch tensors on one HIP device, runs on torch's current stream and
+waits for nothing. Activations are bfloat16 or float32; parameters, the scan's states and the
+parameters' gradients are float32. Rows are packed: ``offsets`` (int32, one more than there are
+sequences, ascending, on the device) says where each sequence's rows begin; without it all rows are
+one sequence. Where the inner axes of a tensor are not dense it is copied first. Errors raise
+``TrunkError``; there is no fallback: a missing library or device raises.
+
+``*_backward`` computes the gradients from the call's own inputs; nothing is kept between calls.
+Results are the same each time, bit for bit.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import os
+from typing import NamedTuple, Optional
+
+import torch
+
+PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+LIB_PATH = os.path.join(PKG, "lib", "libuor_trunk_hip.so")
+SYMBOLS = ("uor_trunk_abi_version", "uor_trunk_last_error", "uor_trunk_sizeof_scan", "uor_trunk_sizeof_conv",
+           "uor_trunk_sizeof_norms", "uor_trunk_scan_workspace_bytes", "uor_trunk_scan_async",
+           "uor_trunk_scan_backward_workspace_bytes", "uor_trunk_scan_backward_async", "uor_trunk_scan_step_async",
+           "uor_trunk_conv_async", "uor_trunk_conv_backward_workspace_bytes", "uor_trunk_conv_backward_async",
+           "uor_trunk_conv_step_async", "uor_trunk_norms_async", "uor_trunk_norms_backward_workspace_bytes",
+           "uor_trunk_norms_backward_async")
+ABI_VERSION = 1
+DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+MAX_DIM = MAX_STATE = 128
+MAX_TAPS = 4
+MAX_WIDTH = 8192
+
+P, I64, U32, F32 = C.c_void_p, C.c_int64, C.c_uint32, C.c_float
+
+
+class TrunkError(ValueError):
+    pass
+
+
+class CScan(C.Structure):
+    _fields_ = ([("device", C.c_int32)] + [(n, U32) for n in ("dtype", "tokens", "seqs", "heads", "groups", "dim", "state",
+                                                              "slots", "reserved")]
+                + [(n, I64) for n in ("x_stride", "dt_stride", "b_stride", "c_stride", "y_stride")]
+                + [(n, P) for n in ("x", "dt", "B", "C", "A", "D", "dt_bias", "offsets", "initial", "y", "final", "index",
+                                    "states", "dy", "dfinal", "dx", "ddt", "dB", "dC", "dA", "dD", "ddt_bias", "dinitial")])
+
+
+class CConv(C.Structure):
+    _fields_ = ([("device", C.c_int32)] + [(n, U32) for n in ("dtype", "tokens", "seqs", "channels", "taps", "slots", "silu")]
+                + [(n, I64) for n in ("x_stride", "y_stride")]
+                + [(n, P) for n in ("x", "weight", "bias", "offsets", "initial", "y", "final", "index", "states", "dy",
+                                    "dfinal", "dx", "dinitial", "dweight", "dbias")])
+
+
+class CNorms(C.Structure):
+    _fields_ = ([("device", C.c_int32)] + [(n, U32) for n in ("dtype", "rows", "width")] + [("eps", F32), ("reserved", U32)]
+                + [(n, I64) for n in ("residual_stride", "out_stride", "gate_stride")]
+                + [(n, P) for n in ("residual", "out", "gate", "post", "scale", "pre", "residual_out", "normed",
+                                    "dresidual_out", "dnormed", "dresidual", "dout", "dgate", "dpost", "dscale", "dpre")])
+
+
+class ScanGrads(NamedTuple):
+    dx: torch.Tensor
+    ddt: torch.Tensor
+    dA: torch.Tensor
+    dB: torch.Tensor
+    dC: torch.Tensor
+    dD: Optional[torch.Tensor]
+    ddt_bias: Optional[torch.Tensor]
+    dinitial: Optional[torch.Tensor]
+
+
+class ConvGrads(NamedTuple):
+    dx: torch.Tensor
+    dweight: torch.Tensor
+    dbias: Optional[torch.Tensor]
+    dinitial: Optional[torch.Tensor]
+
+
+class NormGrads(NamedTuple):
+    dresidual: Optional[torch.Tensor]
+    dout: Optional[torch.Tensor]
+    dgate: Optional[torch.Tensor]
+    dpost: Optional[torch.Tensor]
+    dscale: Optional[torch.Tensor]
+    dpre: Optional[torch.Tensor]
+
+
+_lib = None
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        if not os.path.exists(LIB_PATH):
+            raise TrunkError(f"{LIB_PATH} is not built (make -C uor-r4_amd/csrc)")
+        L = C.CDLL(LIB_PATH)
+        L.uor_trunk_abi_version.restype = U32
+        L.uor_trunk_last_error.restype = C.c_char_p
+        for name, struct in (("scan", CScan), ("conv", CConv), ("norms", CNorms)):
+            size = getattr(L, f"uor_trunk_sizeof_{name}")
+            size.restype = C.c_uint64
+            if size() != C.sizeof(struct) or L.uor_trunk_abi_version() != ABI_VERSION:
+                raise TrunkError(f"{LIB_PATH} is of another version: build it again")
+            forms = {"scan": ("", "_backward", "_step"), "conv": ("", "_backward", "_step"), "norms": ("", "_backward")}[name]
+            for form in forms:
+                call = getattr(L, f"uor_trunk_{name}{form}_async")
+                needs = form == "_backward" or (name == "scan" and form == "")
+                call.argtypes = [C.POINTER(struct)] + ([P, C.c_uint64] if needs else []) + [P]
+                if needs:
+                    f = getattr(L, f"uor_trunk_{name}{form}_workspace_bytes")
+                    f.argtypes, f.restype = [C.POINTER(struct)], C.c_uint64
+        _lib = L
+    return _lib
+
+
+def _call(name, args, device, workspace=False):
+    L = lib()
+    extra, keep = (), None
+    if workspace:
+        n = getattr(L, f"uor_trunk_{name}_workspace_bytes")(C.byref(args))
+        keep = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        extra = (None if keep is None else keep.data_ptr(), n)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    code = getattr(L, f"uor_trunk_{name}_async")(C.byref(args), *extra, stream)
+    if code:
+        raise TrunkError(f"uor_trunk_{name} status {code}: {L.uor_trunk_last_error().decode()}")
+
+
+def _want(ok, text):
+    if not ok:
+        raise TrunkError(text)
+
+
+def _rows(name, t, dtype, *shape):
+    """t with dense inner axes, and the values between its rows (None: None, 0)."""
+    if t is None:
+        return None, 0
+    _want(isinstance(t, torch.Tensor), f"{name} is no tensor")
+    _want(t.dtype == dtype, f"{name} is {t.dtype}, not {dtype}")
+    _want(tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    inner, dense = 1, True
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        dense = dense and (size == 1 or stride == inner)
+        inner *= size
+    if t.shape[0] <= 1:
+        return (t if dense else t.contiguous()), inner
+    if not dense or t.stride(0) < inner:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _dense(name, t, dtype, *shape):
+    t, _ = _rows(name, t, dtype, *shape)
+    return None if t is None else t.contiguous()
+
+
+def _one_device(*tensors):
+    """The tensors' device: one HIP device for all of them."""
+    devices = {t.device for t in tensors if t is not None}
+    _want(len(devices) == 1, f"the tensors are on different devices: {sorted(map(str, devices))}")
+    device = devices.pop()
+    _want(device.type == "cuda", f"the tensors are on {device}: a HIP device is wanted")
+    return device
+
+
+def _offsets(offsets, tokens):
+    if offsets is None:
+        return None, 1
+    _want(offsets.dim() == 1 and offsets.numel() >= 2, "offsets has one place more than there are sequences, two at least")
+    _want(offsets.dtype in (torch.int32, torch.int64), f"offsets is {offsets.dtype}, not int32")
+    return offsets.int().contiguous(), offsets.numel() - 1
+
+
+def _index(slots, rows, states):
+    if slots is None:
+        _want(states >= rows, f"{rows} rows for {states} states")
+        return None
+    _want(slots.dtype in (torch.int32, torch.int64), f"slots is {slots.dtype}, not int32")
+    _want(tuple(slots.shape) == (rows,), f"slots has shape {tuple(slots.shape)}, not {(rows,)}")
+    return slots.int().contiguous()
+
+
+_NOTHING = 16  # the address of a tensor of no values: it is there, and nothing of it is read
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr() or _NOTHING
+
+
+def _dtype(t, name):
+    _want(isinstance(t, torch.Tensor) and t.dtype in DTYPES, f"{name} is no tensor of bfloat16 or float32")
+    return t.dtype
+
+
+# ---------------------------------------------------------------------------------------------
+# The scan.
+
+
+def _scan_args(x, dt, A, B, Cm, D, dt_bias, offsets, initial, step=False):
+    dtype = _dtype(x, "x")
+    _want(x.dim() == 3, "x has the axes row, head and value")
+    _want(isinstance(B, torch.Tensor) and B.dim() == 3, "B has the axes row, group and state")
+    tokens, heads, dim = x.shape
+    groups, state = B.shape[1:]
+    _want(groups >= 1 and heads >= 1 and heads % groups == 0, f"{heads} heads are not whole groups of {groups}")
+    _want(1 <= dim <= MAX_DIM and 1 <= state <= MAX_STATE, f"dim {dim} or state {state} outside 1..128")
+    off, seqs = (None, tokens) if step else _offsets(offsets, tokens)
+    x, xs = _rows("x", x, dtype, tokens, heads, dim)
+    dt, ds = _rows("dt", dt, dtype, tokens, heads)
+    B, bs = _rows("B", B, dtype, tokens, groups, state)
+    Cm, cs = _rows("C", Cm, dtype, tokens, groups, state)
+    f32 = torch.float32
+    _want(A is not None, "A is no tensor")
+    A, D, dt_bias = _dense("A", A, f32, heads), _dense("D", D, f32, heads), _dense("dt_bias", dt_bias, f32, heads)
+    initial = _dense("initial", initial, f32, seqs, heads, dim, state)
+    keep = (x, dt, A, B, Cm, D, dt_bias, off, initial)
+    a = CScan(dtype=DTYPES[dtype], tokens=tokens, seqs=seqs, heads=heads, groups=groups, dim=dim, state=state,
+              x_stride=xs, dt_stride=ds, b_stride=bs, c_stride=cs, y_stride=heads * dim, x=_ptr(x), dt=_ptr(dt), B=_ptr(B),
+              C=_ptr(Cm), A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias), offsets=_ptr(off), initial=_ptr(initial))
+    return a, keep
+
+
+def scan(x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, initial=None):
+    """(y, final): the scan of x (rows, heads, dim) with dt (rows, heads), A (heads), B and C (rows,
+    groups, state), the skip D and the steps' bias (heads), from the states ``initial`` (sequences,
+    heads, dim, state; zeros without). ``final`` are the states after each sequence's last row."""
+    a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, offsets, initial)
+    device = _one_device(*keep)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    final = torch.empty((a.seqs, a.heads, a.dim, a.state), dtype=torch.float32, device=device)
+    a.device, a.y, a.final = device.index, _ptr(y), _ptr(final)
+    _call("scan", a, device, workspace=True)
+    return y, final
+
+
+def scan_backward(dy, x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, initial=None, dfinal=None):
+    """The gradients of ``scan`` at its inputs from those of its outputs; ``dfinal`` None: zeros.
+    dD, ddt_bias and dinitial are None where the input is."""
+    a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, offsets, initial)
+    dy, a.y_stride = _rows("dy", dy, x.dtype, *x.shape)
+    _want(dy is not None, "dy is no tensor")
+    f32 = torch.float32
+    dfinal = _dense("dfinal", dfinal, f32, a.seqs, a.heads, a.dim, a.state)
+    device = _one_device(dy, dfinal, *keep)
+    make = lambda like, dtype=None: None if like is None else torch.empty(like.shape, dtype=dtype or like.dtype, device=device)  # noqa: E731
+    got = ScanGrads(make(x), make(dt), make(A), make(B), make(C), make(D), make(dt_bias), make(initial))
+    a.device, a.dy, a.dfinal = device.index, _ptr(dy), _ptr(dfinal)
+    a.dx, a.ddt, a.dA, a.dB, a.dC, a.dD, a.ddt_bias, a.dinitial = map(_ptr, got)
+    _call("scan_backward", a, device, workspace=True)
+    return got
+
+
+def scan_step(x, dt, A, B, C, states, *, slots=None, D=None, dt_bias=None):
+    """y (rows, heads, dim): one token a session. ``states`` (slots, heads, dim, state) float32 is
+    updated in place; ``slots`` (int32) says which state each row has, no two alike. A row whose slot
+    is outside the states is skipped and its y is 0."""
+    a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, None, None, step=True)
+    _want(isinstance(states, torch.Tensor) and states.dtype == torch.float32 and states.is_contiguous()
+          and tuple(states.shape[1:]) == (a.heads, a.dim, a.state) and states.dim() == 4,
+          f"states is no dense float32 tensor of (slots, {a.heads}, {a.dim}, {a.state})")
+    index = _index(slots, a.tokens, states.shape[0])
+    device = _one_device(states, index, *keep)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    a.device, a.y, a.index, a.states, a.slots = device.index, _ptr(y), _ptr(index), _ptr(states), states.shape[0]
+    _call("scan_step", a, device)
+    return y
+
+
+# ---------------------------------------------------------------------------------------------
+# The convolution.
+
+
+def _conv_args(x, weight, bias, offsets, initial, silu, step=False):
+    dtype = _dtype(x, "x")
+    _want(x.dim() == 2, "x has the axes row and channel")
+    _want(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight has the axes channel and tap")
+    tokens, channels = x.shape
+    taps = weight.shape[1]
+    _want(channels >= 1 and 1 <= taps <= MAX_TAPS, f"{taps} taps outside 1..{MAX_TAPS}, or no channels")
+    off, seqs = (None, tokens) if step else _offsets(offsets, tokens)
+    x, xs = _rows("x", x, dtype, tokens, channels)
+    weight = _dense("weight", weight, torch.float32, channels, taps)
+    bias = _dense("bias", bias, torch.float32, channels)
+    initial = _dense("initial", initial, dtype, seqs, taps - 1, channels)
+    a = CConv(dtype=DTYPES[dtype], tokens=tokens, seqs=seqs, channels=channels, taps=taps, silu=int(bool(silu)), x_stride=xs,
+              y_stride=channels, x=_ptr(x), weight=_ptr(weight), bias=_ptr(bias), offsets=_ptr(off), initial=_ptr(initial))
+    return a, (x, weight, bias, off, initial)
+
+
+def conv(x, weight, bias=None, *, offsets=None, initial=None, silu=True):
+    """(y, final): y_t = silu(bias + sum_k weight[:, k] x_(t - taps + 1 + k)) over each sequence's own
+    rows of x (rows, channels), the rows before it from ``initial`` (sequences, taps - 1, channels;
+    zeros without). ``final`` are each sequence's last taps - 1 rows, the next call's ``initial``."""
+    a, keep = _conv_args(x, weight, bias, offsets, initial, silu)
+    device = _one_device(*keep)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    final = torch.empty((a.seqs, a.taps - 1, a.channels), dtype=x.dtype, device=device)
+    a.device, a.y, a.final = device.index, _ptr(y), _ptr(final)
+    _call("conv", a, device)
+    return y, final
+
+
+def conv_backward(dy, x, weight, bias=None, *, offsets=None, initial=None, dfinal=None, silu=True):
+    """The gradients of ``conv`` at its inputs; dbias and dinitial are None where the input is."""
+    a, keep = _conv_args(x, weight, bias, offsets, initial, silu)
+    dy, a.y_stride = _rows("dy", dy, x.dtype, *x.shape)
+    _want(dy is not None, "dy is no tensor")
+    dfinal = _dense("dfinal", dfinal, x.dtype, a.seqs, a.taps - 1, a.channels)
+    device = _one_device(dy, dfinal, *keep)
+    make = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=device)  # noqa: E731
+    got = ConvGrads(make(x), make(weight), make(bias), make(initial))
+    a.device, a.dy, a.dfinal = device.index, _ptr(dy), _ptr(dfinal)
+    a.dx, a.dweight, a.dbias, a.dinitial = (_ptr(t) for t in got)
+    _call("conv_backward", a, device, workspace=True)
+    return got
+
+
+def conv_step(x, weight, states, bias=None, *, slots=None, silu=True):
+    """y (rows, channels): one token a session; ``states`` (slots, taps - 1, channels) of x's type is
+    updated in place, ``slots`` as in ``scan_step``."""
+    a, keep = _conv_args(x, weight, bias, None, None, silu, step=True)
+    _want(isinstance(states, torch.Tensor) and states.dtype == x.dtype and states.is_contiguous() and states.dim() == 3
+          and tuple(states.shape[1:]) == (a.taps - 1, a.channels),
+          f"states is no dense {x.dtype} tensor of (slots, {a.taps - 1}, {a.channels})")
+    index = _index(slots, a.tokens, states.shape[0])
+    device = _one_device(states, index, *keep)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    a.device, a.y, a.index, a.states, a.slots = device.index, _ptr(y), _ptr(index), _ptr(states), states.shape[0]
+    _call("conv_step", a, device)
+    return y
+
+
+# ---------------------------------------------------------------------------------------------
+# The norms.
+
+
+def _norms_args(residual, out, gate, post, scale, pre, eps):
+    first = residual if residual is not None else out
+    dtype = _dtype(first, "residual" if residual is not None else "out")
+    _want(first.dim() == 2, "rows have the axes row and value")
+    _want(out is not None or (gate is None and post is None and scale is None), "a gate, post or scale without a block's output")
+    _want(out is not None or pre is not None, "nothing to compute: neither a block's output nor pre")
+    rows, width = first.shape
+    _want(1 <= width <= MAX_WIDTH, f"width {width} outside 1..{MAX_WIDTH}")
+    _want(eps >= 0, "eps is negative")
+    residual, rs = _rows("residual", residual, dtype, rows, width)
+    out, os_ = _rows("out", out, dtype, rows, width)
+    gate, gs = _rows("gate", gate, dtype, rows, width)
+    post, scale, pre = (_dense(n, t, torch.float32, width) for n, t in (("post", post), ("scale", scale), ("pre", pre)))
+    a = CNorms(dtype=DTYPES[dtype], rows=rows, width=width, eps=eps, residual_stride=rs, out_stride=os_, gate_stride=gs,
+               residual=_ptr(residual), out=_ptr(out), gate=_ptr(gate), post=_ptr(post), scale=_ptr(scale), pre=_ptr(pre))
+    return a, dtype, (residual, out, gate, post, scale, pre)
+
+
+def norms(residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps=1e-6):
+    """(residual', normed) between two blocks: v = out silu(gate), residual' = residual + scale
+    rms(v) post, normed = rms(residual') pre, with rows of (rows, width). Without ``out`` the residual
+    is only normed (residual' is the residual itself); without ``residual`` residual' is the normed
+    block alone; without ``pre`` normed is None. ``gate``, ``post`` and ``scale`` are 1 without."""
+    a, dtype, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
+    device = _one_device(*keep)
+    make = lambda: torch.empty((a.rows, a.width), dtype=dtype, device=device)  # noqa: E731
+    residual_out = residual if out is None else make()
+    normed = None if pre is None else make()
+    a.device, a.normed = device.index, _ptr(normed)
+    a.residual_out = None if out is None else _ptr(residual_out)
+    _call("norms", a, device)
+    return residual_out, normed
+
+
+def norms_backward(dresidual_out, dnormed, residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps=1e-6):
+    """The gradients of ``norms`` at its inputs, None where there is none; either of the outputs'
+    gradients may be None for zeros."""
+    a, dtype, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
+    _want(dnormed is None or pre is not None, "dnormed without pre")
+    dresidual_out = _dense("dresidual_out", dresidual_out, dtype, a.rows, a.width)
+    dnormed = _dense("dnormed", dnormed, dtype, a.rows, a.width)
+    device = _one_device(dresidual_out, dnormed, *keep)
+    make = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=device)  # noqa: E731
+    got = NormGrads(*map(make, (residual, out, gate, post, scale, pre)))
+    a.device, a.dresidual_out, a.dnormed = device.index, _ptr(dresidual_out), _ptr(dnormed)
+    a.dresidual, a.dout, a.dgate, a.dpost, a.dscale, a.dpre = map(_ptr, got)
+    _call("norms_backward", a, device, workspace=True)
+    return got
