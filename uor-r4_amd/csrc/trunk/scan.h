@@ -95,7 +95,8 @@ struct Scan {
   float *final;
   float *starts;         // [pieces][heads][dim][state]: where a piece begins, if sequences are cut; or NULL
   double *totals;        // [pieces][heads]: log2 of a piece's whole decay
-  bool x_wide, b_wide, c_wide, y_wide;
+  uint32_t part;         // values of dim of a wavefront
+  bool x_wide, b_wide, c_wide, y_wide, state_wide;
 };
 
 // Pieces are dealt to the eight XCDs in turn, and a piece's heads run on one of them, next to each
@@ -243,7 +244,7 @@ __device__ __forceinline__ void advance(f32x4 (&h)[NT * PW / 4], const Own<NT, P
 
 int check_scan(const uor_trunk_scan_args *s, bool step);
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
-uint32_t piece_rows(uint32_t tokens, uint32_t heads);
+uint32_t piece_rows(uint32_t tokens, uint32_t heads, uint32_t most);
 inline uint32_t tiles_of(uint32_t dim) { return (dim + 63) / 64; }
 
 }  // namespace trunk

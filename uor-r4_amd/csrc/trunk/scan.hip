@@ -1,208 +1,261 @@
 // scan.hip - the selective state space scan over packed sequences: outputs and final states.
 //
-// One block takes one head of one piece of a sequence, chunk after chunk, with the head's state in
-// registers (its transpose as result tiles: rows of the state's axis, a column a value of x) and a
-// copy of it as operand parts in LDS. A wavefront owns 16 rows of the chunk for y and a part of the
-// state's tiles for the update. The scores C_t . B_s are computed with s along the tile's rows, so
-// that a lane's results are, once scaled, its operand of the next product over s.
+// One wavefront takes one head of one piece of a sequence (or 32 or 64 of its values), chunk after
+// chunk, with the state in registers: as columns of values of x, so that pairs of its tiles are the
+// operand of the product with C as they lie. The scores C_t . B_s are computed with s along the
+// tile's rows, so that a lane's results are, once scaled, its operand of the next product over s. The
+// blocks' wavefronts are heads of one group and share B and C; x is each wavefront's own.
 //
 // Rows are bound by time, not by products: a sequence of many rows and few heads would run on few
 // blocks. Such sequences are cut into pieces: a first launch gives every piece its end state from
 // zeros, a second joins them along the sequence, and the main launch runs all pieces at once.
-#include "scan.h"
+#include "wave.h"
 
 namespace trunk {
 
-// The parts of the state as an operand, [part][16 PW][16 NT].
-template <class T, int NT, int PW>
-__device__ __forceinline__ void publish(T *to, const f32x4 (&h)[NT * PW / 4], const Own<NT, PW> &own) {
-  const int lane = threadIdx.x & 63, q = lane >> 4;
-#pragma unroll
-  for (int i = 0; i < NT * PW / 4; i++) {
-    T *row = to + (own.p * 16 + (lane & 15)) * pitch<T>(16 * NT) + (own.n + i) * 16 + 4 * q;
-    if constexpr (Mma<T>::kParts == 1) {
-      *(f32x4 *)row = h[i];
-    } else {
-      bf16x4 hi, lo;
-#pragma unroll
-      for (int r = 0; r < 4; r++) hi[r] = (bf16)h[i][r];
-#pragma unroll
-      for (int r = 0; r < 4; r++) lo[r] = (bf16)(h[i][r] - (float)hi[r]);
-      *(bf16x4 *)row = hi;
-      *(bf16x4 *)(row + 16 * PW * pitch<T>(16 * NT)) = lo;
+// The values of x that are infinite or no number, times their weights, onto y of their rows and of
+// those after them: a row a lane. Rounding y before it changes nothing, as no such sum is finite.
+template <class T, int NP, int PP>
+__device__ __forceinline__ void add_odd(T *y, int64_t y_stride, uint32_t first, uint32_t end, uint32_t dim, uint32_t state, const T *sB,
+                                     const T *sC, const T *sX, const Steps &s, float skip) {
+  __threadfence_block();  // y has been written by other lanes
+  const uint32_t t = threadIdx.x & 63;
+  if (first + t >= end) return;
+  T *row = y + (int64_t)(first + t) * y_stride;
+  for (uint32_t from = 0; from <= t; from++) {
+    float weight = 0.0f;
+    bool known = false;
+    for (uint32_t p = 0; p < dim; p++) {
+      const float v = (float)sX[from * PP + p];
+      if (finite(v)) continue;
+      if (!known) {
+        for (uint32_t n = 0; n < state; n++) weight += (float)sC[t * NP + n] * (float)sB[from * NP + n];
+        weight *= from < t ? exp2_((s.hi[t] - s.hi[from]) + (s.lo[t] - s.lo[from])) * s.step[from] : s.step[from];
+        if (from == t) weight += skip;
+        known = true;
+      }
+      row[p] = (T)((float)row[p] + weight * v);
     }
   }
 }
 
-template <class T, int NT, int PW>
-__global__ __launch_bounds__(kThreads) void scan_rows(Scan a) {
-  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kLp = pitch<T>(kChunk);
-  __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sBt[kN * kLp], sXt[kP * kLp], sH[Mma<T>::kParts * kP * kNp];
-  __shared__ Decays d;
-  __shared__ int odd;
+template <class T, int NT, int PW, int W>
+__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
+  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP), kThreads_ = 64 * W;
+  __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sXs[W][kChunk * kPp];
+  __shared__ Steps steps[W];
 
-  uint32_t number, head;
-  place_of(blockIdx.x, a.heads * a.tiles, number, head);
-  const uint32_t p0 = head % a.tiles * kP;
-  head /= a.tiles;
+  const Unit unit = unit_of<W>(a, kP);
   Piece at;
-  if (number >= a.pieces || !piece(a.rows, number, a.size, at)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
-  const uint32_t group = head / (a.heads / a.groups);
-  const T *x = (const T *)a.x + head * a.dim + p0, *dt = (const T *)a.dt + head;
-  const T *B = (const T *)a.B + group * a.state, *C = (const T *)a.C + group * a.state;
-  T *y = (T *)a.y + head * a.dim + p0;
-  const uint32_t dim = a.dim - p0 < (uint32_t)kP ? a.dim - p0 : kP;
+  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at)) return;
+  const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
+  const uint32_t head = unit.head;
+  const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head;
+  const T *B = (const T *)a.B + unit.group * a.state, *C = (const T *)a.C + unit.group * a.state;
+  T *y = (T *)a.y + head * a.dim + unit.p0, *sX = sXs[wave];
+  Steps &s = steps[wave];
+  const uint32_t dim = a.dim - unit.p0 < (uint32_t)kP ? a.dim - unit.p0 : kP;
   const float A = a.A[head], skip = a.D ? a.D[head] : 0.0f, bias = a.bias ? a.bias[head] : 0.0f;
-  const uint64_t whole = (uint64_t)a.dim * a.state;
-  const Own<NT, PW> own;
-  f32x4 h[NT * PW / 4];
-  load_state<NT, PW>(h, own,
-                     a.starts ? a.starts + ((uint64_t)number * a.heads + head) * whole
-                              : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole : nullptr,
-                     p0, a.dim, a.state);
+  const uint64_t whole = (uint64_t)a.dim * a.state, part = (uint64_t)unit.p0 * a.state;
+  f32x4 h[NT][PW];
+  get_state<NT, PW>(h,
+                    a.starts ? a.starts + ((uint64_t)unit.piece * a.heads + head) * whole + part
+                             : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + part : nullptr,
+                    dim, a.state, a.state_wide);
+
+  // A chunk's rows are fetched into registers while the state goes past the chunk before.
+  Load<T, kN, kThreads_> nextB, nextC;
+  Load<T, kP, 64> nextX;
+  float raw = 0.0f;
+  const auto fetch = [&](uint32_t first) {
+    const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
+    const int lane = anew(lane0), thread = wave * 64 + lane;
+    nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
+    nextC.get(thread, C, a.c_stride, first, end, a.state, a.c_wide);
+    nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
+    if (first + lane < end) raw = (float)dt[(int64_t)(first + lane) * a.dt_stride];
+  };
+  if (at.first < at.end) fetch(at.first);
 
   for (uint32_t first = at.first; first < at.end; first += kChunk) {
     const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
+    const int lane = anew(lane0), thread = wave * 64 + lane, q = lane >> 4, i16 = lane & 15;
     __syncthreads();  // the chunk before has been read
-    if (threadIdx.x == 0) odd = 0;
+    nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+    nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
+    const bool odd = __any(nextX.put(lane, sX, a.x_stride, dim, a.x_wide));
+    const Decay d = steps_of(lane, s, raw, first + lane < end, A, bias);
     __syncthreads();
-    stage<T, kN>(sB, sBt, B, a.b_stride, first, end, a.state, a.b_wide);
-    stage<T, kN>(sC, (T *)nullptr, C, a.c_stride, first, end, a.state, a.c_wide);
-    if (stage<T, kP>((T *)nullptr, sXt, x, a.x_stride, first, end, dim, a.x_wide)) odd = 1;
-    publish<T, NT, PW>(sH, h, own);
-    if (wave == 0) decays(d, dt, a.dt_stride, first, end, A, bias);
-    __syncthreads();
+    if (unit.idle) {
+      if (end < at.end) fetch(end);
+      continue;
+    }
 
-    // y's rows of this wavefront, transposed: what comes from the state before the chunk.
-    const int t = wave * 16 + i16;
-    f32x4 acc[PW];
+    // y, transposed: what comes from the state before the chunk.
+    f32x4 acc[4][PW];
 #pragma unroll
-    for (int i = 0; i < PW; i++) acc[i] = f32x4{0, 0, 0, 0};
+    for (int tile = 0; tile < 4; tile++)
 #pragma unroll
-    for (int k = 0; k < kN; k += 32) {
-      const V8<T> c = operand(sC + t * kNp, k + 8 * q);
+      for (int i = 0; i < PW; i++) acc[tile][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < PW; i++)
+    for (int k = 0; k < NT / 2; k++) {
+      V8<T> c[4];
 #pragma unroll
-        for (int part = Mma<T>::kParts - 1; part >= 0; part--)
-          acc[i] = Mma<T>::mul(operand(sH + (part * kP + i * 16 + i16) * kNp, k + 8 * q), c, acc[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < PW; i++) acc[i] *= d.from[t];
-    // What comes from the chunk's own rows, two tiles of 16 at a time.
-    const float hi = d.hi[t], lo = d.lo[t];
-#pragma unroll
-    for (int pair = 0; pair < 2; pair++) {
-      if (2 * pair > wave) break;
-      f32x8 m;
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int s0 = (2 * pair + half) * 16;
-        f32x4 score = {0, 0, 0, 0};
-        if (2 * pair + half <= wave) {
-#pragma unroll
-          for (int k = 0; k < kN; k += 32)
-            score = Mma<T>::mul(operand(sB + (s0 + i16) * kNp, k + 8 * q), operand(sC + t * kNp, k + 8 * q), score);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int s = s0 + 4 * q + r;
-          const float decay = exp2_((hi - d.hi[s]) + (lo - d.lo[s])) * d.step[s];
-          m[4 * half + r] = s < t ? score[r] * decay : s == t ? score[r] * d.step[s] + skip : 0.0f;
-        }
-      }
-      const auto w = Mma<T>::split(m);
-      if (odd == 0) {
-#pragma unroll
-        for (int i = 0; i < PW; i++)
-          acc[i] = Mma<T>::mul(operand_tiles(sXt + (i * 16 + i16) * kLp, pair * 32 + 4 * q), w, acc[i]);
-      } else {
-        // Some x of the chunk is infinite or no number: its products with the zeros above the
-        // diagonal would reach rows before it. Such values are left out of the product, and added to
-        // the rows from their own on one by one.
-#pragma unroll
-        for (int i = 0; i < PW; i++) {
-          V8<T> v = operand_tiles(sXt + (i * 16 + i16) * kLp, pair * 32 + 4 * q);
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[e] = finite((float)v[e]) ? v[e] : (T)0.0f;
-          acc[i] = Mma<T>::mul(v, w, acc[i]);
-        }
-#pragma unroll 1
-        for (int s = pair * 32; s < pair * 32 + 32; s++) {
-          const int from = ((s & 15) >> 2) * 16 + i16, at = (s & 16 ? 4 : 0) + (s & 3);
-          float mine = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; e++) mine = e == at ? __shfl(m[e], from) : mine;
-          if (s > t) continue;
-#pragma unroll
-          for (int i = 0; i < PW; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const float v = (float)sXt[(i * 16 + 4 * q + r) * kLp + s];
-              if (!finite(v)) acc[i][r] += mine * v;
-            }
-        }
-      }
-    }
-    if (first + t < end) {
-      T *row = y + (int64_t)(first + t) * a.y_stride;
+      for (int tile = 0; tile < 4; tile++) c[tile] = operand(sC + (tile * 16 + i16) * kNp, 32 * k + 8 * q);
 #pragma unroll
       for (int i = 0; i < PW; i++) {
-        const uint32_t p = i * 16 + 4 * q;
-        V4<T> v;
+        const auto hs = Mma<T>::split(__builtin_shufflevector(h[2 * k][i], h[2 * k + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = (T)acc[i][r];
-        if (a.y_wide && p + 4 <= dim) {
-          *(V4<T> *)(row + p) = v;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (p + r < dim) row[p + r] = v[r];
-        }
+        for (int tile = 0; tile < 4; tile++) acc[tile][i] = Mma<T>::mul(hs, c[tile], acc[tile][i]);
       }
     }
-    advance<T, NT, PW>(h, own, sXt, sBt, d.to, d.whole);
+    __builtin_amdgcn_sched_barrier(0);
+    V8<T> xs[2][PW];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sX, 32 * k, i);
+    // Some x of the chunk is infinite or no number: its products with the zeros above the diagonal
+    // would reach rows before it. Such values are left out of the products, and added afterwards.
+    if (odd) {
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < PW; i++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) xs[k][i][e] = finite((float)xs[k][i][e]) ? xs[k][i][e] : (T)0.0f;
+    }
+
+    // And what comes from the chunk's own rows, 16 at a time.
+#pragma unroll
+    for (int tile = 0; tile < 4; tile++) {
+      const int t = tile * 16 + i16;
+      __builtin_amdgcn_sched_barrier(0);  // tiles taken together would not fit the registers
+      if (first + tile * 16 >= end) break;
+      V8<T> c[NT / 2];
+#pragma unroll
+      for (int k = 0; k < NT / 2; k++) c[k] = operand(sC + t * kNp, 32 * k + 8 * q);
+      const float u = s.u[t];
+      const auto score = [&](int other) {
+        f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < NT / 2; k++) v = Mma<T>::mul(operand(sB + (other * 16 + i16) * kNp, 32 * k + 8 * q), c[k], v);
+        return v;
+      };
+      const auto before = [&](int other) {  // a tile before this one: its rows' weight at this one's start
+        const float c = other + 1 == tile ? 1.0f : tile == 2 ? d.c20 : other == 0 ? d.c30 : d.c31;
+        return score(other) * (*(const f32x4 *)(s.v + other * 16 + 4 * q) * c);
+      };
+#pragma unroll
+      for (int i = 0; i < PW; i++) acc[tile][i] *= tile < 2 ? d.from[tile] * u : d.from[tile];
+      const auto add = [&](int pair, f32x8 m) {
+        const auto w = Mma<T>::split(m);
+#pragma unroll
+        for (int i = 0; i < PW; i++) acc[tile][i] = Mma<T>::mul(xs[pair][i], w, acc[tile][i]);
+      };
+      if (tile >= 2) {
+        add(0, __builtin_shufflevector(before(0), before(1), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int i = 0; i < PW; i++) acc[tile][i] *= u;
+      }
+      // The tile's own rows, and the tile before it in the same pair.
+      f32x4 own = score(tile);
+      const f32x4 step = *(const f32x4 *)(s.step + tile * 16 + 4 * q), hi = *(const f32x4 *)(s.hi + tile * 16 + 4 * q),
+                  lo = *(const f32x4 *)(s.lo + tile * 16 + 4 * q);
+      const float hi_t = s.hi[t], lo_t = s.lo[t];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int other = 4 * q + r;
+        const float decay = exp2_((hi_t - hi[r]) + (lo_t - lo[r])) * step[r];
+        own[r] = keep(own[r] * decay, other < i16) + keep(own[r] * step[r] + skip, other == i16);
+      }
+      if (tile & 1) add(tile >> 1, __builtin_shufflevector(before(tile - 1) * u, own, 0, 1, 2, 3, 4, 5, 6, 7));
+      else add(tile >> 1, __builtin_shufflevector(own, f32x4{0, 0, 0, 0}, 0, 1, 2, 3, 4, 5, 6, 7));
+      if (a.y_wide) {  // rows past the last and columns past dim are dropped
+        const uint32_t pitch = (uint32_t)a.y_stride * sizeof(T);
+        const auto to = __builtin_amdgcn_make_buffer_rsrc((void *)(y + (int64_t)first * a.y_stride), 0,
+                                                          (int)((end - first - 1) * pitch + dim * (uint32_t)sizeof(T)), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PW; i += 2) {
+          const uint32_t p = place(i, 4 * q);
+          store_eight<T>(to, t * pitch + p * (uint32_t)sizeof(T), p, dim, __builtin_shufflevector(acc[tile][i], acc[tile][i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      } else if (first + t < end) {
+        T *row = y + (int64_t)(first + t) * a.y_stride;
+#pragma unroll
+        for (int i = 0; i < PW; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (place(i, 4 * q + r) < (int)dim) row[place(i, 4 * q + r)] = (T)acc[tile][i][r];
+      }
+    }
+    if (odd) {
+      add_odd<T, kNp, kPp>(y, a.y_stride, first, end, dim, a.state, sB, sC, sX, s, skip);
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sX, 32 * k, i);
+    }
+    if (end < at.end) fetch(end);  // now that y's registers are free
+    advance<T, NT, PW>(lane, h, xs, sB, s.v, d.to, d.whole);
   }
-  if (a.final && at.end == at.stop)
-    store_state<NT, PW>(h, own, a.final + ((uint64_t)at.seq * a.heads + head) * whole, p0, a.dim, a.state);
+  if (a.final && at.end == at.stop && !unit.idle)
+    put_state<NT, PW>(h, a.final + ((uint64_t)at.seq * a.heads + head) * whole + part, dim, a.state, a.state_wide);
 }
 
 // A piece's end state from zeros and its whole decay; a sequence's last piece needs neither.
-template <class T, int NT, int PW>
-__global__ __launch_bounds__(kThreads) void scan_ends(Scan a) {
-  constexpr int kN = 16 * NT, kP = 16 * PW, kLp = pitch<T>(kChunk);
-  __shared__ __align__(16) T sBt[kN * kLp], sXt[kP * kLp];
-  __shared__ Decays d;
-  uint32_t number, head;
-  place_of(blockIdx.x, a.heads * a.tiles, number, head);
-  const uint32_t p0 = head % a.tiles * kP;
-  head /= a.tiles;
+template <class T, int NT, int PW, int W>
+__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
+  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP), kThreads_ = 64 * W;
+  __shared__ __align__(16) T sB[kChunk * kNp], sXs[W][kChunk * kPp];
+  __shared__ Steps steps[W];
+  const Unit unit = unit_of<W>(a, kP);
   Piece at;
-  if (number >= a.pieces || !piece(a.rows, number, a.size, at) || at.end == at.stop) return;
-  const int wave = threadIdx.x >> 6;
-  const uint32_t group = head / (a.heads / a.groups);
-  const T *x = (const T *)a.x + head * a.dim + p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + group * a.state;
-  const uint32_t dim = a.dim - p0 < (uint32_t)kP ? a.dim - p0 : kP;
+  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at) || at.end == at.stop) return;
+  const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
+  const uint32_t head = unit.head;
+  const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + unit.group * a.state;
+  const uint32_t dim = a.dim - unit.p0 < (uint32_t)kP ? a.dim - unit.p0 : kP;
   const float A = a.A[head], bias = a.bias ? a.bias[head] : 0.0f;
-  const Own<NT, PW> own;
-  f32x4 h[NT * PW / 4];
+  f32x4 h[NT][PW];
 #pragma unroll
-  for (int i = 0; i < NT * PW / 4; i++) h[i] = f32x4{0, 0, 0, 0};
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int i = 0; i < PW; i++) h[n][i] = f32x4{0, 0, 0, 0};
   double total = 0.0;
+  Load<T, kN, kThreads_> nextB;
+  Load<T, kP, 64> nextX;
+  float raw = 0.0f;
+  const auto fetch = [&](uint32_t first) {
+    const int lane = anew(lane0), thread = wave * 64 + lane;
+    const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
+    nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
+    nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
+    if (first + lane < end) raw = (float)dt[(int64_t)(first + lane) * a.dt_stride];
+  };
+  if (at.first < at.end) fetch(at.first);
   for (uint32_t first = at.first; first < at.end; first += kChunk) {
     const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
+    const int lane = anew(lane0), thread = wave * 64 + lane;
     __syncthreads();
-    stage<T, kN>((T *)nullptr, sBt, B, a.b_stride, first, end, a.state, a.b_wide);
-    stage<T, kP>((T *)nullptr, sXt, x, a.x_stride, first, end, dim, a.x_wide);
-    if (wave == 0) decays(d, dt, a.dt_stride, first, end, A, bias);
+    nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+    nextX.put(lane, sXs[wave], a.x_stride, dim, a.x_wide);
+    const Decay d = steps_of(lane, steps[wave], raw, first + lane < end, A, bias);
     __syncthreads();
-    advance<T, NT, PW>(h, own, sXt, sBt, d.to, d.whole);
+    if (end < at.end) fetch(end);
+    if (unit.idle) continue;
+    V8<T> xs[2][PW];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sXs[wave], 32 * k, i);
+    advance<T, NT, PW>(lane, h, xs, sB, steps[wave].v, d.to, d.whole);
     total += d.total;
   }
-  const uint64_t slot = (uint64_t)number * a.heads + head;
-  store_state<NT, PW>(h, own, a.starts + slot * a.dim * a.state, p0, a.dim, a.state);
-  if (threadIdx.x == 0 && p0 == 0) a.totals[slot] = total;
+  if (unit.idle) return;
+  const uint64_t slot = (uint64_t)unit.piece * a.heads + head;
+  put_state<NT, PW>(h, a.starts + slot * a.dim * a.state + (uint64_t)unit.p0 * a.state, dim, a.state, a.state_wide);
+  if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
 }
 
 // The pieces' end states into their start states, along each sequence.
@@ -230,8 +283,8 @@ __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
 
 // How many rows a piece has: sequences are cut where heads alone would leave the card idle. The
 // grid then has about 1,024 blocks; pieces under 256 rows cost more to join than they gain.
-uint32_t piece_rows(uint32_t tokens, uint32_t heads) {
-  const uint64_t want = ((uint64_t)tokens * heads + 1023) / 1024;
+uint32_t piece_rows(uint32_t tokens, uint32_t heads, uint32_t most) {
+  const uint64_t want = ((uint64_t)tokens * heads + most - 1) / most;
   const uint64_t size = (want < 256 ? 256 : want) + kChunk - 1;
   const uint64_t rows = size / kChunk * kChunk;
   return rows < tokens ? (uint32_t)rows : (tokens + kChunk) / kChunk * kChunk;
@@ -239,26 +292,36 @@ uint32_t piece_rows(uint32_t tokens, uint32_t heads) {
 
 namespace {
 
-template <class T, int NT, int PW>
-int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
-  const uint32_t blocks = grid_of(a.pieces, a.heads * a.tiles);
+template <class T, int NT, int PW, int W>
+int launch(Scan a, uint32_t seqs, hipStream_t stream) {
+  const uint32_t units = a.heads / a.groups * a.tiles, blocks = grid_of(a.pieces, a.groups * ((units + W - 1) / W));
   if (a.starts) {
-    hipLaunchKernelGGL((scan_ends<T, NT, PW>), dim3(blocks), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((scan_ends<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
     const uint32_t parts = (a.dim * a.state + kThreads - 1) / kThreads;
     hipLaunchKernelGGL(scan_join, dim3(seqs * a.heads, parts), dim3(kThreads), 0, stream, a);
   }
-  hipLaunchKernelGGL((scan_rows<T, NT, PW>), dim3(blocks), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
   return launched();
+}
+template <class T, int NT, int PW>
+int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
+  const uint32_t units = a.heads / a.groups * a.tiles;
+  return units == 1 ? launch<T, NT, PW, 1>(a, seqs, stream) : units == 2 ? launch<T, NT, PW, 2>(a, seqs, stream) : launch<T, NT, PW, 4>(a, seqs, stream);
 }
 template <class T, int NT>
 int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
-  return a.dim <= 32 ? launch<T, NT, 2>(a, seqs, stream) : launch<T, NT, 4>(a, seqs, stream);
+  if constexpr (sizeof(T) == 2 && NT < 8)
+    if (a.part == 64) return launch<T, NT, 4>(a, seqs, stream);
+  return launch<T, NT, 2>(a, seqs, stream);
 }
 template <class T>
 int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
   return a.state <= 32 ? launch<T, 2>(a, seqs, stream) : a.state <= 64 ? launch<T, 4>(a, seqs, stream) : launch<T, 8>(a, seqs, stream);
 }
 
+// The values of dim that a wavefront holds the state of: as many as its registers have room for.
+uint32_t part_of(const uor_trunk_scan_args *s) { return s->dtype == UOR_TRUNK_BF16 && s->state <= 64 && s->dim > 32 ? 64 : 32; }
+uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->heads * ((s->dim + part_of(s) - 1) / part_of(s)), 4096); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
 }
@@ -286,7 +349,9 @@ int check_scan(const uor_trunk_scan_args *s, bool step) {
 // A call's arguments as the kernels take them, cut into pieces of `size` rows.
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size) {
   const uint32_t bytes = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
-  const auto wide = [&](const void *p, int64_t stride, uint32_t part) { return aligned16(p, stride, bytes) && part * bytes % 16 == 0; };
+  const auto wide = [&](const void *p, int64_t stride, uint32_t part) {
+    return aligned16(p, stride, bytes) && part * bytes % 16 == 0 && stride < (1 << 22);  // a chunk's rows within 2^31 bytes
+  };
   Scan a{};
   a.rows = Rows{s->offsets, s->tokens, s->seqs};
   a.heads = s->heads, a.groups = s->groups, a.dim = s->dim, a.state = s->state;
@@ -296,6 +361,7 @@ Scan scan_of(const uor_trunk_scan_args *s, uint32_t size) {
   a.initial = s->initial, a.y = s->y, a.final = s->final;
   a.x_wide = wide(s->x, s->x_stride, s->dim), a.b_wide = wide(s->B, s->b_stride, s->state), a.c_wide = wide(s->C, s->c_stride, s->state);
   a.y_wide = wide(s->y, s->y_stride, s->dim);
+  a.state_wide = s->state % 4 == 0 && aligned16(s->initial, 0, 4) && aligned16(s->final, 0, 4);
   return a;
 }
 
@@ -311,7 +377,7 @@ extern "C" uint64_t uor_trunk_sizeof_norms(void) { return sizeof(uor_trunk_norms
 
 extern "C" uint64_t uor_trunk_scan_workspace_bytes(const uor_trunk_scan_args *s) {
   if (check_scan(s, false)) return 0;
-  const uint32_t size = piece_rows(s->tokens, s->heads * tiles_of(s->dim));
+  const uint32_t size = rows_of(s);
   if (size >= s->tokens) return 0;
   const uint64_t n = pieces(s->tokens, s->seqs, size);
   return starts_bytes(n, s) + n * s->heads * sizeof(double);
@@ -323,7 +389,8 @@ extern "C" int uor_trunk_scan_async(const uor_trunk_scan_args *s, void *workspac
   const uint64_t want = uor_trunk_scan_workspace_bytes(s);
   if (want && (!workspace || bytes < want || (uintptr_t)workspace % 16))
     return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)want);
-  Scan a = scan_of(s, piece_rows(s->tokens, s->heads * tiles_of(s->dim)));
+  Scan a = scan_of(s, rows_of(s));
+  a.part = part_of(s), a.tiles = (s->dim + a.part - 1) / a.part;
   if (want) {
     a.starts = (float *)workspace;
     a.totals = (double *)((char *)workspace + starts_bytes(a.pieces, s));

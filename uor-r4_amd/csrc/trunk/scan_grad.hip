@@ -442,7 +442,7 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
   const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups;
   const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128, p16 = s->dim <= 32 ? 32 : 64;
-  p.size = piece_rows(s->tokens, s->heads * tiles);
+  p.size = piece_rows(s->tokens, s->heads * tiles, 1024);
   p.pieces = pieces(s->tokens, s->seqs, p.size);
   p.chunks = pieces(s->tokens, s->seqs, kChunk);
   // Blocks of a group share its heads where the chunks alone do not fill the card.
