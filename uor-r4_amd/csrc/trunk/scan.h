@@ -25,6 +25,22 @@ constexpr int kThreads = 256; // four wavefronts
 // Split is an operand that was computed in 32 bits. With bf16 it is the sum of two bf16 parts,
 // 2^-18 of a value off at most: one part alone would add an error of the size of y's own rounding
 // to y, and states and their sums are held to 32 bits' worth.
+//
+// v rounded to bf16, and v then what the rounding left of it. Two values at a time, as they are
+// rounded by one instruction and lie in one register.
+__device__ __forceinline__ bf16x8 round8(f32x8 &v) {
+  using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+  u32x4 out;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const bf16x2 two = {(bf16)v[2 * e], (bf16)v[2 * e + 1]};
+    out[e] = __builtin_bit_cast(uint32_t, two);
+    asm("" : "+v"(out[e]));  // else each value is rounded once more by itself
+    v[2 * e] -= __builtin_bit_cast(float, out[e] << 16);
+    v[2 * e + 1] -= __builtin_bit_cast(float, out[e] & 0xffff0000u);
+  }
+  return __builtin_bit_cast(bf16x8, out);
+}
 template <class T>
 struct Mma;
 template <>
@@ -35,10 +51,8 @@ struct Mma<bf16> {
   static constexpr int kParts = 2;
   static __device__ __forceinline__ Split split(f32x8 v) {
     Split s;
-#pragma unroll
-    for (int e = 0; e < 8; e++) s.hi[e] = (bf16)v[e];
-#pragma unroll
-    for (int e = 0; e < 8; e++) s.lo[e] = (bf16)(v[e] - (float)s.hi[e]);
+    s.hi = round8(v);
+    s.lo = round8(v);
     return s;
   }
   static __device__ __forceinline__ f32x4 mul(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -244,7 +258,8 @@ __device__ __forceinline__ void advance(f32x4 (&h)[NT * PW / 4], const Own<NT, P
 
 int check_scan(const uor_trunk_scan_args *s, bool step);
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
-uint32_t piece_rows(uint32_t tokens, uint32_t heads, uint32_t most);
+dim3 join_of(const Scan &a, uint32_t seqs);
+uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units);
 inline uint32_t tiles_of(uint32_t dim) { return (dim + 63) / 64; }
 
 }  // namespace trunk

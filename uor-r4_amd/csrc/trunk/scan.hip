@@ -59,8 +59,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
   const uint64_t whole = (uint64_t)a.dim * a.state, part = (uint64_t)unit.p0 * a.state;
   f32x4 h[NT][PW];
   get_state<NT, PW>(h,
-                    a.starts ? a.starts + ((uint64_t)unit.piece * a.heads + head) * whole + part
-                             : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + part : nullptr,
+                    at.number ? a.starts + ((uint64_t)unit.piece * a.heads + head) * whole + part
+                              : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + part : nullptr,
                     dim, a.state, a.state_wide);
 
   // A chunk's rows are fetched into registers while the state goes past the chunk before.
@@ -73,9 +73,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
     nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
     nextC.get(thread, C, a.c_stride, first, end, a.state, a.c_wide);
     nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
-    if (first + lane < end) raw = (float)dt[(int64_t)(first + lane) * a.dt_stride];
+    raw = first + lane < end ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
   };
-  if (at.first < at.end) fetch(at.first);
+  fetch(at.first);  // past the last chunk nothing is read: rows that are always fetched need no register before
 
   for (uint32_t first = at.first; first < at.end; first += kChunk) {
     const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
     const Decay d = steps_of(lane, s, raw, first + lane < end, A, bias);
     __syncthreads();
     if (unit.idle) {
-      if (end < at.end) fetch(end);
+      fetch(end);
       continue;
     }
 
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
 #pragma unroll
         for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sX, 32 * k, i);
     }
-    if (end < at.end) fetch(end);  // now that y's registers are free
+    fetch(end);  // now that y's registers are free
     advance<T, NT, PW>(lane, h, xs, sB, s.v, d.to, d.whole);
   }
   if (a.final && at.end == at.stop && !unit.idle)
@@ -231,9 +231,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
     const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
     nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
     nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
-    if (first + lane < end) raw = (float)dt[(int64_t)(first + lane) * a.dt_stride];
+    raw = first + lane < end ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
   };
-  if (at.first < at.end) fetch(at.first);
+  fetch(at.first);  // past the last chunk nothing is read: rows that are always fetched need no register before
   for (uint32_t first = at.first; first < at.end; first += kChunk) {
     const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
     const int lane = anew(lane0), thread = wave * 64 + lane;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
     nextX.put(lane, sXs[wave], a.x_stride, dim, a.x_wide);
     const Decay d = steps_of(lane, steps[wave], raw, first + lane < end, A, bias);
     __syncthreads();
-    if (end < at.end) fetch(end);
+    fetch(end);
     if (unit.idle) continue;
     V8<T> xs[2][PW];
 #pragma unroll
@@ -258,36 +258,56 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
   if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
 }
 
-// The pieces' end states into their start states, along each sequence.
+constexpr uint32_t kAhead = 8;
+
+// The pieces' end states into their start states, along each sequence that has more than one.
 __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
   const uint32_t seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
   uint32_t start, end;
   a.rows.of(seq, start, end);
   const uint32_t n = end > start ? (end - start - 1) / a.size + 1 : 1;
-  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state;
+  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
+  if (n == 1) return;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float h = a.initial ? a.initial[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
-    for (uint32_t j = 0; j < n; j++) {
-      const uint64_t slot = (base + j) * a.heads + head;
-      float *at = a.starts + slot * whole + e;
-      if (j + 1 == n) {
-        *at = h;
-        break;
+    float *at = a.starts + (base * a.heads + head) * whole + e;
+    const double *totals = a.totals + base * a.heads + head;
+    float own[kAhead], decay[kAhead];  // of the next pieces: what is read does not wait for the sums
+    const auto read = [&](uint32_t j) {
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; k++) {
+        const uint32_t piece = j + k + 1 < n ? j + k : 0;
+        own[k] = at[piece * step];
+        decay[k] = (float)totals[(uint64_t)piece * a.heads];
       }
-      const float own = *at;
-      *at = h;
-      h = exp2_((float)a.totals[slot]) * h + own;
+    };
+    for (uint32_t j = 0; j < n; j += kAhead) {
+      read(j);
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; k++) {
+        if (j + k >= n) break;
+        if (j + k) at[(j + k) * step] = h;
+        h = exp2_(decay[k]) * h + own[k];
+      }
     }
   }
 }
 
-// How many rows a piece has: sequences are cut where heads alone would leave the card idle. The
-// grid then has about 1,024 blocks; pieces under 256 rows cost more to join than they gain.
-uint32_t piece_rows(uint32_t tokens, uint32_t heads, uint32_t most) {
-  const uint64_t want = ((uint64_t)tokens * heads + most - 1) / most;
+// How many rows a piece has: sequences are cut where they alone would leave the card idle. The grid
+// then has about 4,096 wavefronts, two for each place; pieces under 256 rows cost more to join than
+// they gain. Where there are sequences for every place only those are cut that would still run when
+// the others have long ended.
+uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units) {
+  const uint64_t even = ((uint64_t)tokens * units + 4095) / 4096, want = (uint64_t)seqs * units < 2048 ? even : 4 * even;
   const uint64_t size = (want < 256 ? 256 : want) + kChunk - 1;
   const uint64_t rows = size / kChunk * kChunk;
   return rows < tokens ? (uint32_t)rows : (tokens + kChunk) / kChunk * kChunk;
+}
+
+// A thread for each value where there are few states, fewer where most sequences will not be cut.
+dim3 join_of(const Scan &a, uint32_t seqs) {
+  const uint32_t states = seqs * a.heads, most = (a.dim * a.state + kThreads - 1) / kThreads, even = 2048 / states + 1;
+  return dim3(states, most < even ? most : even);
 }
 
 namespace {
@@ -297,8 +317,7 @@ int launch(Scan a, uint32_t seqs, hipStream_t stream) {
   const uint32_t units = a.heads / a.groups * a.tiles, blocks = grid_of(a.pieces, a.groups * ((units + W - 1) / W));
   if (a.starts) {
     hipLaunchKernelGGL((scan_ends<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
-    const uint32_t parts = (a.dim * a.state + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(scan_join, dim3(seqs * a.heads, parts), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(scan_join, join_of(a, seqs), dim3(kThreads), 0, stream, a);
   }
   hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
   return launched();
@@ -320,8 +339,8 @@ int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
 }
 
 // The values of dim that a wavefront holds the state of: as many as its registers have room for.
-uint32_t part_of(const uor_trunk_scan_args *s) { return s->dtype == UOR_TRUNK_BF16 && s->state <= 64 && s->dim > 32 ? 64 : 32; }
-uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->heads * ((s->dim + part_of(s) - 1) / part_of(s)), 4096); }
+uint32_t part_of(const uor_trunk_scan_args *s) { return 32; }
+uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + part_of(s) - 1) / part_of(s))); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
 }

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void grad_states(Grad k) {
   f32x4 h[kTiles];
   const float *from = BACK ? k.dfinal : a.initial;
   const uint64_t slot = (uint64_t)number * a.heads + head;
-  load_state<NT, PW>(h, own, !STORE ? nullptr : a.starts ? a.starts + slot * whole : from ? from + ((uint64_t)at.seq * a.heads + head) * whole : nullptr,
+  load_state<NT, PW>(h, own, !STORE ? nullptr : a.starts && (BACK || at.number) ? a.starts + slot * whole : from ? from + ((uint64_t)at.seq * a.heads + head) * whole : nullptr,
                      p0, a.dim, a.state);
   const uint32_t chunks = (at.end - at.first + kChunk - 1) / kChunk;
   const uint64_t base = at.start / kChunk + at.seq + (at.first - at.start) / kChunk;
@@ -442,7 +442,7 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
   const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups;
   const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128, p16 = s->dim <= 32 ? 32 : 64;
-  p.size = piece_rows(s->tokens, s->heads * tiles, 1024);
+  p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles);
   p.pieces = pieces(s->tokens, s->seqs, p.size);
   p.chunks = pieces(s->tokens, s->seqs, kChunk);
   // Blocks of a group share its heads where the chunks alone do not fill the card.
@@ -471,7 +471,7 @@ template <class T, int NT, int PW>
 int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
   const Scan &a = k.s;
   const dim3 block(kThreads), sweep(grid_of(a.pieces, a.heads * a.tiles));
-  const dim3 join(seqs * a.heads, (a.dim * a.state + kThreads - 1) / kThreads);
+  const dim3 join = join_of(a, seqs);
   if (a.starts) {
     hipLaunchKernelGGL((grad_states<T, NT, PW, false, false>), sweep, block, 0, stream, k);
     hipLaunchKernelGGL(scan_join, join, block, 0, stream, a);

@@ -39,8 +39,30 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
-// log(1 + e^v) without overflow; its derivative is sigmoid(v).
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) + (v != v ? v : 0.0f); }
+// e^v of v <= 0, to 2^-22 of it: what the rounding of v log2(e) leaves goes into the result.
+__device__ __forceinline__ float exp_down(float v) {
+  v = fmaxf(v, -120.0f);
+  const float t = v * kLog2e, left = fmaf(v, 1.92596299e-8f, fmaf(v, kLog2e, -t));
+  const float e = exp2_(t);
+  return fmaf(e, left * 0.693147181f, e);
+}
+// log(1 + e^v) without overflow; its derivative is sigmoid(v). With e = e^-|v|, log(1 + e) is
+// 2 artanh(z) of z = e / (2 + e) <= 1/3, whose series is z + z^3 / 3 + ... + z^15 / 15 to 2^-25 of it.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = exp_down(-fabsf(v)), d = 2.0f + e;
+  float r = __builtin_amdgcn_rcpf(d);
+  r = fmaf(r, fmaf(-d, r, 1.0f), r);
+  const float z = e * r, s = z * z;
+  float p = 1.0f / 15.0f;
+  p = fmaf(p, s, 1.0f / 13.0f);
+  p = fmaf(p, s, 1.0f / 11.0f);
+  p = fmaf(p, s, 1.0f / 9.0f);
+  p = fmaf(p, s, 1.0f / 7.0f);
+  p = fmaf(p, s, 1.0f / 5.0f);
+  p = fmaf(p, s, 1.0f / 3.0f);
+  p = fmaf(p * s, z, z);
+  return fmaxf(v, 0.0f) + 2.0f * p + (v != v ? v : 0.0f);
+}
 
 // The packed rows of a call. Offsets are clamped to the rows that there are, and a sequence's end
 // to its start, so a table of any content stays inside the arrays.

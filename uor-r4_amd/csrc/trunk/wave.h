@@ -31,13 +31,9 @@ struct Fine<bf16> {
   bf16x8 hi, mid, lo;
   static __device__ __forceinline__ Fine of(f32x8 v) {
     Fine s;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      s.hi[e] = (bf16)v[e];
-      const float left = v[e] - (float)s.hi[e];
-      s.mid[e] = (bf16)left;
-      s.lo[e] = (bf16)(left - (float)s.mid[e]);
-    }
+    s.hi = round8(v);
+    s.mid = round8(v);
+    s.lo = round8(v);
     return s;
   }
 };
@@ -119,12 +115,12 @@ struct Load {
   V8<T> v[kN];
   const T *at;
   uint32_t rows;
-  __device__ __forceinline__ void get(int thread, const T *base, int64_t stride, uint32_t first, uint32_t end, uint32_t cols, bool wide) {
+  __device__ __forceinline__ void get(uint32_t thread, const T *base, int64_t stride, uint32_t first, uint32_t end, uint32_t cols, bool wide) {
     at = base + (int64_t)first * stride;
     rows = end - first;
-    if (!wide) return;
-    // Reads past the buffer's end give zeros: rows past the chunk's last, and columns sent there.
-    const uint32_t pitch = (uint32_t)stride * sizeof(T), bytes = (rows - 1) * pitch + cols * (uint32_t)sizeof(T);
+    // Reads past the buffer's end give zeros: rows past the chunk's last, columns sent there, and
+    // all that this form cannot read.
+    const uint32_t pitch = (uint32_t)stride * sizeof(T), bytes = wide && rows ? (rows - 1) * pitch + cols * (uint32_t)sizeof(T) : 0;
     const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)at, 0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kN; i++) {
@@ -133,19 +129,21 @@ struct Load {
     }
   }
   // Whether some value is infinite or no number.
-  __device__ __forceinline__ bool put(int thread, T *to, int64_t stride, uint32_t cols, bool wide) const {
+  __device__ __forceinline__ bool put(uint32_t thread, T *to, int64_t stride, uint32_t cols, bool wide) const {
     bool odd = false;
     if (wide) {
 #pragma unroll
       for (int i = 0; i < kN; i++) {
-        const int job = i * THREADS + thread;
+        const uint32_t job = i * THREADS + thread;
         *(V8<T> *)(to + job / (COLS / 8) * kPitch + job % (COLS / 8) * 8) = v[i];
       }
       if constexpr (sizeof(T) == 2) {  // the largest exponent of all
+        using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
         using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
         u16x8 most = 0;
 #pragma unroll
-        for (int i = 0; i < kN; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8, v[i]) & (uint16_t)0x7fff);
+        for (int i = 0; i < kN; i++)
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8, __builtin_bit_cast(u32x4, v[i]) & 0x7fff7fffu));
         odd = __builtin_reduce_max(most) >= 0x7f80;
       } else {
 #pragma unroll
@@ -155,7 +153,7 @@ struct Load {
       }
     } else {
 #pragma unroll 1
-      for (int job = thread; job < kChunk * COLS; job += THREADS) {
+      for (uint32_t job = thread; job < kChunk * COLS; job += THREADS) {
         const uint32_t row = job / COLS, col = job % COLS;
         const T one = row < rows && col < cols ? at[(int64_t)row * stride + col] : (T)0.0f;
         to[row * kPitch + col] = one;
