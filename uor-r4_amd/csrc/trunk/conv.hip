@@ -5,9 +5,15 @@
 // channels (16 bytes of bf16) and the rows before it in registers.
 #include "trunk.h"
 
+#include <type_traits>
+
 namespace trunk {
 
-constexpr uint32_t kRun = 32;  // rows of a thread's run: the rows before it are read twice
+// Rows of a thread's run: the rows before it are read twice, and a gradient computes those after it
+// twice. Shorter runs fill the card sooner.
+constexpr uint32_t kRun = 16, kGradRun = 32;
+constexpr int kBatch = 4;  // rows that are read together
+constexpr uint32_t kGradThreads = 512;
 
 struct Conv {
   Rows rows;
@@ -21,30 +27,67 @@ struct Conv {
   void *states;
   const void *dy, *dfinal;
   void *dx, *dinitial;
-  float *parts;      // [workers][TAPS + 1][channels]: sums of a worker's runs
-  uint32_t workers;
-  bool x_wide, y_wide, state_wide, silu;
+  float *parts;      // [blocks][TAPS + 1][channels]: sums of a block's runs
+  uint32_t workers;  // lines of the grid
+  bool silu;
 };
 
-template <class T>
-__device__ __forceinline__ void store8(T *row, uint32_t col, uint32_t cols, bool wide, f32x8 v) {
-  const V8<T> o = __builtin_convertvector(v, V8<T>);
-  if (wide && col + 8 <= cols) {
-    *(V8<T> *)(row + col) = o;
-    return;
+// A thread's E channels of a row: eight, or in a gradient, which holds more of them, four. WIDE: all
+// rows are whole pieces of eight channels, aligned to 16 bytes.
+template <class T, int E>
+using Raw = __attribute__((ext_vector_type(E))) T;
+template <int E>
+using Some = __attribute__((ext_vector_type(E))) float;
+
+template <class T, bool WIDE, int E>
+__device__ __forceinline__ void store_some(T *row, uint32_t col, uint32_t cols, Some<E> v) {
+  const Raw<T, E> o = __builtin_convertvector(v, Raw<T, E>);
+  if constexpr (WIDE) {
+    *(Raw<T, E> *)(row + col) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (col + e < cols) row[col + e] = o[e];
   }
-#pragma unroll
-  for (int e = 0; e < 8; e++)
-    if (col + e < cols) row[col + e] = o[e];
 }
-template <class T>
-__device__ __forceinline__ f32x8 row8(const void *base, int64_t at, uint32_t col, uint32_t cols, bool wide) {
-  return __builtin_convertvector(load8((const T *)base + at, true, col, cols, wide), f32x8);
-}
-template <int TAPS>
-__device__ __forceinline__ void taps_of(const Conv &a, uint32_t c, f32x8 (&w)[TAPS], f32x8 &bias) {
+template <class T, bool WIDE, int E>
+__device__ __forceinline__ Raw<T, E> raw_some(const void *base, int64_t at, uint32_t col, uint32_t cols) {
+  const T *row = (const T *)base + at;
+  if constexpr (WIDE) return *(const Raw<T, E> *)(row + col);
+  Raw<T, E> v;
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
+  for (int e = 0; e < E; e++) v[e] = col + e < cols ? row[col + e] : (T)0.0f;
+  return v;
+}
+template <class T, bool WIDE, int E>
+__device__ __forceinline__ Some<E> row_some(const void *base, int64_t at, uint32_t col, uint32_t cols) {
+  return __builtin_convertvector(raw_some<T, WIDE, E>(base, at, col, cols), Some<E>);
+}
+// A block's threads: `lines` runs by the channels' pieces of E, or one run by THREADS of them.
+struct Lane {
+  uint32_t line, run, c;
+};
+template <int E, uint32_t THREADS>
+__host__ __device__ __forceinline__ uint32_t lines_of(uint32_t channels) {
+  const uint32_t groups = (channels + E - 1) / E;
+  return groups > THREADS ? 1 : THREADS / groups;
+}
+template <int E, uint32_t THREADS>
+__host__ __device__ __forceinline__ uint32_t parts_of(uint32_t channels) {
+  return ((channels + E - 1) / E + THREADS - 1) / THREADS;
+}
+template <int E, uint32_t THREADS>
+__device__ __forceinline__ bool lane_of(const Conv &a, Lane &l) {
+  const uint32_t groups = (a.channels + E - 1) / E, parts = parts_of<E, THREADS>(a.channels), lines = lines_of<E, THREADS>(a.channels);
+  const uint32_t thread = blockIdx.x % parts * THREADS + threadIdx.x;
+  l.line = parts > 1 ? 0 : thread / groups, l.run = blockIdx.x / parts * lines + l.line;
+  l.c = (parts > 1 ? thread : thread % groups) * E;
+  return l.line < lines && l.c < a.channels;
+}
+template <int TAPS, int E>
+__device__ __forceinline__ void taps_of(const Conv &a, uint32_t c, Some<E> (&w)[TAPS], Some<E> &bias) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
     const bool there = c + e < a.channels;
 #pragma unroll
     for (int k = 0; k < TAPS; k++) w[k][e] = there ? a.weight[(c + e) * TAPS + k] : 0.0f;
@@ -52,146 +95,202 @@ __device__ __forceinline__ void taps_of(const Conv &a, uint32_t c, f32x8 (&w)[TA
   }
 }
 // Row `first - TAPS + 1 + k` of the sequence for each k < TAPS - 1: its own, or one before it.
-template <class T, int TAPS>
-__device__ __forceinline__ void rows_before(const Conv &a, const Piece &at, uint32_t c, f32x8 *window) {
+template <class T, int TAPS, bool WIDE, int E>
+__device__ __forceinline__ void rows_before(const Conv &a, const Piece &at, uint32_t c, Some<E> *window) {
 #pragma unroll
   for (int k = 0; k < TAPS - 1; k++) {
     const int64_t row = (int64_t)at.first - (TAPS - 1) + k, back = row - at.start;
-    window[k] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (back >= 0) window[k] = row8<T>(a.x, row * a.x_stride, c, a.channels, a.x_wide);
+    window[k] = Some<E>(0.0f);
+    if (back >= 0) window[k] = row_some<T, WIDE, E>(a.x, row * a.x_stride, c, a.channels);
     else if (a.initial)
-      window[k] = row8<T>(a.initial, ((int64_t)at.seq * (TAPS - 1) + (TAPS - 1) + back) * a.channels, c, a.channels, a.state_wide);
+      window[k] = row_some<T, WIDE, E>(a.initial, ((int64_t)at.seq * (TAPS - 1) + (TAPS - 1) + back) * a.channels, c, a.channels);
   }
 }
-template <int TAPS>
-__device__ __forceinline__ f32x8 weighted(const f32x8 *window, const f32x8 &x, const f32x8 (&w)[TAPS], const f32x8 &bias) {
-  f32x8 v = bias;
+// bias + sum of w[k] rows[k]: the rows before the one that is last.
+template <int TAPS, int E>
+__device__ __forceinline__ Some<E> weighted(const Some<E> *rows, const Some<E> (&w)[TAPS], const Some<E> &bias) {
+  Some<E> v = bias;
 #pragma unroll
-  for (int k = 0; k < TAPS - 1; k++) v += window[k] * w[k];
-  return v + x * w[TAPS - 1];
+  for (int k = 0; k < TAPS; k++) v = __builtin_elementwise_fma(rows[k], w[k], v);  // one rounding in every form
+  return v;
 }
-template <int TAPS>
-__device__ __forceinline__ void shift(f32x8 *window, const f32x8 &x) {
+template <int E>
+__device__ __forceinline__ Some<E> silu(Some<E> v) {
 #pragma unroll
-  for (int k = 0; k + 2 < TAPS; k++) window[k] = window[k + 1];
-  if (TAPS > 1) window[TAPS - 2] = x;
+  for (int e = 0; e < E; e++) v[e] *= sigmoid(v[e]);
+  return v;
 }
 
-template <class T, int TAPS>
-__global__ __launch_bounds__(256) void conv_rows(Conv a) {
-  const uint32_t groups = (a.channels + 7) / 8;
-  const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint32_t number = (uint32_t)(id / groups), c = (uint32_t)(id % groups) * 8;
+template <class T, int TAPS, bool WIDE>
+__global__ __launch_bounds__(256, 4) void conv_rows(Conv a) {
+  constexpr int E = 8, kPast = TAPS - 1;
+  Lane l;
   Piece at;
-  if (number >= a.pieces || !piece(a.rows, number, kRun, at)) return;
-  f32x8 w[TAPS], bias, window[TAPS];
-  taps_of<TAPS>(a, c, w, bias);
-  rows_before<T, TAPS>(a, at, c, window);
-#pragma unroll 4
-  for (uint32_t t = at.first; t < at.end; t++) {
-    const f32x8 x = row8<T>(a.x, t * a.x_stride, c, a.channels, a.x_wide);
-    f32x8 v = weighted<TAPS>(window, x, w, bias);
-    shift<TAPS>(window, x);
-    if (a.silu) {
+  if (!lane_of<E, 256>(a, l) || l.run >= a.pieces || !piece(a.rows, l.run, kRun, at)) return;
+  const uint32_t c = l.c;
+  Some<E> w[TAPS], bias, rows[kPast + kBatch];
+  taps_of<TAPS, E>(a, c, w, bias);
+  rows_before<T, TAPS, WIDE, E>(a, at, c, rows);
+  uint32_t left = 0;  // rows of the last batch
+  for (uint32_t first = at.first; first < at.end; first += kBatch) {
+    left = min(at.end - first, (uint32_t)kBatch);
+    const T *x = (const T *)a.x + (int64_t)first * a.x_stride;
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] *= sigmoid(v[e]);
+    for (int k = 0; k < kBatch; k++) {
+      rows[kPast + k] = row_some<T, WIDE, E>(x, 0, c, a.channels);
+      x += first + k + 1 < at.end ? a.x_stride : 0;  // rows past the last are read as the last
     }
-    store8((T *)a.y + t * a.y_stride, c, a.channels, a.y_wide, v);
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      Some<E> v = weighted<TAPS, E>(rows + k, w, bias);
+      if (a.silu) v = silu<E>(v);
+      if (k < (int)left) store_some<T, WIDE, E>((T *)a.y + (first + k) * a.y_stride, c, a.channels, v);
+    }
+    if (first + kBatch < at.end) {
+#pragma unroll
+      for (int k = 0; k < kPast; k++) rows[k] = rows[kBatch + k];
+    }
   }
   if (a.final && at.end == at.stop) {
 #pragma unroll
-    for (int k = 0; k < TAPS - 1; k++)
-      store8((T *)a.final + ((int64_t)at.seq * (TAPS - 1) + k) * a.channels, c, a.channels, a.state_wide, window[k]);
+    for (int k = 0; k < kPast; k++) {
+      Some<E> v = rows[k];
+#pragma unroll
+      for (int n = 1; n <= kBatch; n++) v = left == (uint32_t)n ? rows[k + n] : v;
+      store_some<T, WIDE, E>((T *)a.final + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
+    }
   }
 }
 
 // dx of a row needs the gradients before the activation of the TAPS - 1 rows after it: a run goes
 // that far past its end, and dx follows TAPS - 1 rows behind. The parameters' sums take a run's own
-// rows; a worker's runs are fixed, so that its sums have one order.
-template <class T, int TAPS>
-__global__ __launch_bounds__(256) void conv_grad_rows(Conv a) {
-  const uint32_t groups = (a.channels + 7) / 8;
-  const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint32_t worker = (uint32_t)(id / groups), c = (uint32_t)(id % groups) * 8;
-  if (worker >= a.workers) return;
-  f32x8 w[TAPS], bias, sums[TAPS + 1];
-  taps_of<TAPS>(a, c, w, bias);
+// rows; a line's runs are fixed, and a block's lines are joined in their order, so that all sums
+// have one order.
+template <class T, int TAPS, bool WIDE>
+__global__ __launch_bounds__(kGradThreads, 3) void conv_grad_rows(Conv a) {
+  constexpr int E = 4, kPast = TAPS - 1;
+  __shared__ float joined[kGradThreads * E];
+  Lane l;
+  const bool there = lane_of<E, kGradThreads>(a, l);
+  const uint32_t c = l.c;
+  Some<E> sums[TAPS + 1];
 #pragma unroll
-  for (int k = 0; k <= TAPS; k++) sums[k] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-  for (uint32_t number = worker; number < a.pieces; number += a.workers) {
-    Piece at;
-    if (!piece(a.rows, number, kRun, at)) continue;
-    f32x8 window[TAPS], d[TAPS];  // the rows before t; the gradients at rows t - TAPS + 1 .. t
-    rows_before<T, TAPS>(a, at, c, window);
+  for (int k = 0; k <= TAPS; k++) sums[k] = Some<E>(0.0f);
+  if (there) {
+    Some<E> w[TAPS], bias;
+    taps_of<TAPS, E>(a, c, w, bias);
+    for (uint32_t number = l.run; number < a.pieces; number += a.workers) {
+      Piece at;
+      if (!piece(a.rows, number, kGradRun, at)) continue;
+      // rows[kPast + k] and d[kPast + k]: of row first + k, and before them those of the rows before.
+      Some<E> rows[kPast + kBatch], d[kPast + kBatch];
+      rows_before<T, TAPS, WIDE, E>(a, at, c, rows);
 #pragma unroll
-    for (int k = 0; k < TAPS; k++) d[k] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    // A sequence's first run emits the rows before the sequence too.
-    const int64_t emit = at.number ? at.first : (int64_t)at.start - (TAPS - 1);
-#pragma unroll 2
-    for (int64_t t = at.first; t < (int64_t)at.end + TAPS - 1; t++) {
+      for (int k = 0; k < kPast; k++) d[k] = Some<E>(0.0f);
+      // A sequence's first run emits the rows before the sequence too.
+      const int64_t emit = at.number ? at.first : (int64_t)at.start - kPast;
+      const uint32_t last = at.end + kPast;  // a run of no rows still has the rows before
+      Raw<T, E> xs[kBatch], gs[kBatch], next_x[kBatch], next_g[kBatch];
+      const auto fetch = [&](uint32_t first) {  // a batch ahead; rows past the last are read as the last, and not used
+        const uint32_t most = at.stop - 1, from = min(first, most);
+        const T *x = (const T *)a.x + (int64_t)from * a.x_stride, *g = (const T *)a.dy + (int64_t)from * a.y_stride;
 #pragma unroll
-      for (int k = 0; k + 1 < TAPS; k++) d[k] = d[k + 1];
-      d[TAPS - 1] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (t < at.stop) {
-        const f32x8 x = row8<T>(a.x, t * a.x_stride, c, a.channels, a.x_wide);
-        f32x8 g = row8<T>(a.dy, t * a.y_stride, c, a.channels, a.y_wide);
-        if (a.silu) {
-          const f32x8 v = weighted<TAPS>(window, x, w, bias);
+        for (int k = 0; k < kBatch; k++) {
+          next_x[k] = raw_some<T, WIDE, E>(x, 0, c, a.channels);
+          next_g[k] = raw_some<T, WIDE, E>(g, 0, c, a.channels);
+          const bool more = first + k < most;
+          x += more ? a.x_stride : 0;
+          g += more ? a.y_stride : 0;
+        }
+      };
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float s = sigmoid(v[e]);
-            g[e] *= s * (1.0f + v[e] * (1.0f - s));
+      for (int k = 0; k < kBatch; k++) next_x[k] = next_g[k] = Raw<T, E>((T)0.0f);
+      if (at.start != at.stop) fetch(at.first);
+      // A batch of rows. EDGE: some may be past the run's last, or before the first that it emits;
+      // where none is, nothing is asked row by row, and stores are not waited for.
+      const auto batch = [&](uint32_t first, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) xs[k] = next_x[k], gs[k] = next_g[k];
+        if (at.start != at.stop) fetch(first + kBatch);
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) {
+          const uint32_t t = first + b;
+          rows[kPast + b] = __builtin_convertvector(xs[b], Some<E>);
+          Some<E> g = __builtin_convertvector(gs[b], Some<E>);
+          if (a.silu) {
+            const Some<E> v = weighted<TAPS, E>(rows + b, w, bias);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+              const float s = sigmoid(v[e]);
+              g[e] *= s * fmaf(v[e], 1.0f - s, 1.0f);
+            }
           }
-        }
-        d[TAPS - 1] = g;
-        if (t < at.end) {
+          if (EDGE && t >= at.stop) g = Some<E>(0.0f);  // whatever the rows before are
+          d[kPast + b] = g;
+          if (!EDGE || t < at.end) {
 #pragma unroll
-          for (int k = 0; k < TAPS - 1; k++) sums[k] += g * window[k];
-          sums[TAPS - 1] += g * x;
-          sums[TAPS] += g;
-        }
-        shift<TAPS>(window, x);
-      }
-      const int64_t row = t - (TAPS - 1);
-      if (row < emit) continue;
-      f32x8 v = d[0] * w[TAPS - 1];
+            for (int k = 0; k < TAPS; k++) sums[k] = __builtin_elementwise_fma(g, rows[b + k], sums[k]);
+            sums[TAPS] += g;
+          }
+          const int64_t row = (int64_t)t - kPast;
+          if (EDGE && (row < emit || t >= last)) continue;
+          Some<E> v = d[b] * w[kPast];
 #pragma unroll
-      for (int k = 1; k < TAPS; k++) v += d[k] * w[TAPS - 1 - k];
-      const int64_t last = row - ((int64_t)at.stop - (TAPS - 1));  // its place among the sequence's last rows
-      if (a.dfinal && last >= 0)
-        v += row8<T>(a.dfinal, ((int64_t)at.seq * (TAPS - 1) + last) * a.channels, c, a.channels, a.state_wide);
-      if (row >= (int64_t)at.start) {
-        store8((T *)a.dx + row * a.channels, c, a.channels, a.state_wide, v);
-      } else if (a.dinitial) {
-        const int64_t k = row - at.start + TAPS - 1;
-        store8((T *)a.dinitial + ((int64_t)at.seq * (TAPS - 1) + k) * a.channels, c, a.channels, a.state_wide, v);
-      }
+          for (int k = 1; k < TAPS; k++) v = __builtin_elementwise_fma(d[b + k], w[kPast - k], v);
+          if (EDGE) {
+            const int64_t back = row - ((int64_t)at.stop - kPast);  // its place among the sequence's last rows
+            if (a.dfinal && back >= 0) v += row_some<T, WIDE, E>(a.dfinal, ((int64_t)at.seq * kPast + back) * a.channels, c, a.channels);
+            if (row < (int64_t)at.start) {
+              const int64_t k = row - at.start + kPast;
+              if (a.dinitial) store_some<T, WIDE, E>((T *)a.dinitial + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
+              continue;
+            }
+          }
+          store_some<T, WIDE, E>((T *)a.dx + row * a.channels, c, a.channels, v);
+        }
+#pragma unroll
+        for (int k = 0; k < kPast; k++) rows[k] = rows[kBatch + k], d[k] = d[kBatch + k];
+      };
+      // The rows that no batch of the middle may reach past: the run's end, and before the sequence's
+      // last rows, which have gradients of their own.
+      const int64_t middle = min((int64_t)at.end, (int64_t)at.stop - 1);
+      uint32_t first = at.first;
+      if (first < last) batch(first, std::true_type{}), first += kBatch;
+      for (; first + kBatch <= middle; first += kBatch) batch(first, std::false_type{});
+      for (; first < last; first += kBatch) batch(first, std::true_type{});
     }
   }
+  // The block's lines side by side.
+  const uint32_t parts = parts_of<E, kGradThreads>(a.channels), lines = lines_of<E, kGradThreads>(a.channels);
+  const uint32_t groups = (a.channels + E - 1) / E, block = blockIdx.x / parts, c0 = blockIdx.x % parts * kGradThreads * E;
+  const uint32_t width = parts > 1 ? kGradThreads * E : groups * E;
 #pragma unroll
-  for (int k = 0; k <= TAPS; k++)
-    store8(a.parts + ((uint64_t)worker * (TAPS + 1) + k) * a.channels, c, a.channels, a.channels % 4 == 0, sums[k]);
+  for (int k = 0; k <= TAPS; k++) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++) joined[threadIdx.x * E + e] = sums[k][e];
+    __syncthreads();
+    for (uint32_t at = threadIdx.x; at < width && c0 + at < a.channels; at += kGradThreads) {
+      float v = 0.0f;
+      for (uint32_t line = 0; line < lines; line++) v += joined[line * groups * E + at];
+      a.parts[((uint64_t)block * (TAPS + 1) + k) * a.channels + c0 + at] = v;
+    }
+  }
 }
 
-// The workers' sums, one block 64 sums: four threads a sum, each a quarter of the workers.
-__global__ __launch_bounds__(256) void conv_grad_sums(const float *parts, uint32_t workers, uint32_t channels, uint32_t taps,
-                                                      float *dweight, float *dbias) {
-  __shared__ float part[4][64];
-  const uint32_t at = blockIdx.x * 64 + threadIdx.x % 64, n = (taps + 1) * channels, quarter = threadIdx.x / 64;
-  float v = 0.0f;
-  if (at < n)
-    for (uint32_t w = quarter; w < workers; w += 4) v += parts[(uint64_t)w * n + at];
-  part[quarter][threadIdx.x % 64] = v;
-  __syncthreads();
-  if (quarter || at >= n) return;
-  v = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-  const uint32_t k = at / channels, c = at % channels;
-  if (k < taps) dweight[c * taps + k] = v;
-  else if (dbias) dbias[c] = v;
+__global__ __launch_bounds__(1024) void conv_grad_sums(const float *parts, uint32_t blocks, uint32_t channels, uint32_t taps,
+                                                       float *dweight, float *dbias) {
+  sum_columns(parts, blocks, (taps + 1) * channels, [&](uint32_t at, float v) {
+    const uint32_t k = at / channels, c = at % channels;
+    if (k < taps) dweight[c * taps + k] = v;
+    else if (dbias) dbias[c] = v;
+  });
 }
 
-template <class T, int TAPS>
+template <class T, int TAPS, bool WIDE>
 __global__ __launch_bounds__(256) void conv_step(Conv a) {
+  constexpr int E = 8;
   const uint32_t groups = (a.channels + 7) / 8;
   const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t row = (uint32_t)(id / groups), c = (uint32_t)(id % groups) * 8;
@@ -199,24 +298,20 @@ __global__ __launch_bounds__(256) void conv_step(Conv a) {
   const int64_t slot = a.index ? a.index[row] : (int64_t)row;
   T *y = (T *)a.y + row * a.y_stride;
   if (slot < 0 || slot >= a.slots) {
-    store8(y, c, a.channels, a.y_wide, f32x8{0, 0, 0, 0, 0, 0, 0, 0});
+    store_some<T, WIDE, E>(y, c, a.channels, Some<E>(0.0f));
     return;
   }
-  f32x8 w[TAPS], bias, window[TAPS];
+  Some<E> w[TAPS], bias, rows[TAPS];
   T *state = (T *)a.states + slot * (TAPS - 1) * a.channels;
 #pragma unroll
-  for (int k = 0; k < TAPS - 1; k++) window[k] = row8<T>(state, (int64_t)k * a.channels, c, a.channels, a.state_wide);
-  const f32x8 x = row8<T>(a.x, row * a.x_stride, c, a.channels, a.x_wide);
-  taps_of<TAPS>(a, c, w, bias);
-  f32x8 v = weighted<TAPS>(window, x, w, bias);
-  shift<TAPS>(window, x);
-  if (a.silu) {
+  for (int k = 0; k < TAPS - 1; k++) rows[k] = row_some<T, WIDE, E>(state, (int64_t)k * a.channels, c, a.channels);
+  rows[TAPS - 1] = row_some<T, WIDE, E>(a.x, row * a.x_stride, c, a.channels);
+  taps_of<TAPS, E>(a, c, w, bias);
+  Some<E> v = weighted<TAPS, E>(rows, w, bias);
+  if (a.silu) v = silu<E>(v);
+  store_some<T, WIDE, E>(y, c, a.channels, v);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= sigmoid(v[e]);
-  }
-  store8(y, c, a.channels, a.y_wide, v);
-#pragma unroll
-  for (int k = 0; k < TAPS - 1; k++) store8(state, k * a.channels + c, (k + 1) * a.channels, a.state_wide, window[k]);
+  for (int k = 0; k < TAPS - 1; k++) store_some<T, WIDE, E>(state + k * a.channels, c, a.channels, rows[k + 1]);
 }
 
 namespace {
@@ -234,62 +329,70 @@ int check_conv(const uor_trunk_conv_args *s, bool step) {
   if (((uint64_t)s->tokens + s->seqs) * ((s->channels + 7) / 8) / 32 > 0x3fffffffu) return fail(-1, "too many rows and channels for one call");
   return 0;
 }
-Conv conv_of(const uor_trunk_conv_args *s) {
-  const uint32_t bytes = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
-  const auto wide = [&](const void *p, int64_t stride) { return aligned16(p, stride, bytes); };
+Conv conv_of(const uor_trunk_conv_args *s, uint32_t run) {
   Conv a{};
   a.rows = Rows{s->offsets, s->tokens, s->seqs};
-  a.channels = s->channels, a.pieces = pieces(s->tokens, s->seqs, kRun), a.slots = s->slots;
+  a.channels = s->channels, a.pieces = pieces(s->tokens, s->seqs, run), a.slots = s->slots;
   a.x_stride = s->x_stride, a.y_stride = s->y_stride;
   a.x = s->x, a.weight = s->weight, a.bias = s->bias, a.initial = s->initial, a.y = s->y, a.final = s->final;
   a.index = s->index, a.states = s->states, a.dy = s->dy, a.dfinal = s->dfinal, a.dx = s->dx, a.dinitial = s->dinitial;
   a.silu = s->silu != 0;
-  a.x_wide = wide(s->x, s->x_stride), a.y_wide = wide(s->y ? s->y : s->dy, s->y_stride);
-  a.state_wide = wide(s->initial, s->channels) && wide(s->final, s->channels) && wide(s->states, s->channels) &&
-                 wide(s->dfinal, s->channels) && wide(s->dinitial, s->channels) && wide(s->dx, s->channels);
   return a;
 }
-// Workers of a gradient: enough threads for the card, and at least four runs each where there are so many.
-uint32_t workers_of(uint32_t count, uint32_t channels) {
-  const uint32_t groups = (channels + 7) / 8, most = (1u << 18) / groups + 1, few = (count + 3) / 4;
-  return few < most ? few : most;
+bool wide_of(const uor_trunk_conv_args *s) {
+  const uint32_t bytes = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
+  if (s->channels % 8) return false;
+  const auto wide = [&](const void *p, int64_t stride) { return aligned16(p, stride, bytes); };
+  return wide(s->x, s->x_stride) && wide(s->y, s->y_stride) && wide(s->dy, s->y_stride) && wide(s->initial, 0) && wide(s->final, 0) &&
+         wide(s->states, 0) && wide(s->dfinal, 0) && wide(s->dinitial, 0) && wide(s->dx, 0);
 }
-template <template <class, int> class F, class... V>
-int by_taps(const uor_trunk_conv_args *s, V... v) {
-  if (s->dtype == UOR_TRUNK_BF16)
-    switch (s->taps) {
-      case 1: return F<bf16, 1>::run(v...);
-      case 2: return F<bf16, 2>::run(v...);
-      case 3: return F<bf16, 3>::run(v...);
-      default: return F<bf16, 4>::run(v...);
-    }
-  switch (s->taps) {
-    case 1: return F<float, 1>::run(v...);
-    case 2: return F<float, 2>::run(v...);
-    case 3: return F<float, 3>::run(v...);
-    default: return F<float, 4>::run(v...);
+// The blocks of `runs` runs, and of a gradient: two for each compute unit, each line with four runs
+// at least where there are so many.
+uint32_t blocks_of(uint32_t runs, uint32_t channels) {
+  const uint32_t lines = lines_of<8, 256>(channels);
+  return (runs + lines - 1) / lines * parts_of<8, 256>(channels);
+}
+uint32_t grad_blocks_of(uint32_t runs, uint32_t channels) {
+  const uint32_t lines = lines_of<4, kGradThreads>(channels), parts = parts_of<4, kGradThreads>(channels);
+  const uint32_t few = (runs + 4 * lines - 1) / (4 * lines), most = (768 + parts - 1) / parts;
+  return few < 1 ? 1 : few < most ? few : most;
+}
+template <template <class, int, bool> class F, class T, bool WIDE, class... V>
+int by_taps(uint32_t taps, V... v) {
+  switch (taps) {
+    case 1: return F<T, 1, WIDE>::run(v...);
+    case 2: return F<T, 2, WIDE>::run(v...);
+    case 3: return F<T, 3, WIDE>::run(v...);
+    default: return F<T, 4, WIDE>::run(v...);
   }
 }
-uint32_t blocks_of(uint64_t rows, uint32_t channels) { return (uint32_t)((rows * ((channels + 7) / 8) + 255) / 256); }
-template <class T, int TAPS>
+template <template <class, int, bool> class F, class... V>
+int by_form(const uor_trunk_conv_args *s, V... v) {
+  const bool wide = wide_of(s);
+  if (s->dtype == UOR_TRUNK_BF16) return wide ? by_taps<F, bf16, true>(s->taps, v...) : by_taps<F, bf16, false>(s->taps, v...);
+  return wide ? by_taps<F, float, true>(s->taps, v...) : by_taps<F, float, false>(s->taps, v...);
+}
+template <class T, int TAPS, bool WIDE>
 struct RowsCall {
   static int run(Conv a, hipStream_t stream) {
-    hipLaunchKernelGGL((conv_rows<T, TAPS>), dim3(blocks_of(a.pieces, a.channels)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((conv_rows<T, TAPS, WIDE>), dim3(blocks_of(a.pieces, a.channels)), dim3(256), 0, stream, a);
     return launched();
   }
 };
-template <class T, int TAPS>
+template <class T, int TAPS, bool WIDE>
 struct StepCall {
   static int run(Conv a, hipStream_t stream) {
-    hipLaunchKernelGGL((conv_step<T, TAPS>), dim3(blocks_of(a.rows.tokens, a.channels)), dim3(256), 0, stream, a);
+    const uint64_t threads = (uint64_t)a.rows.tokens * ((a.channels + 7) / 8);
+    hipLaunchKernelGGL((conv_step<T, TAPS, WIDE>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, a);
     return launched();
   }
 };
-template <class T, int TAPS>
+template <class T, int TAPS, bool WIDE>
 struct GradCall {
-  static int run(Conv a, float *dweight, float *dbias, hipStream_t stream) {
-    hipLaunchKernelGGL((conv_grad_rows<T, TAPS>), dim3(blocks_of(a.workers, a.channels)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(conv_grad_sums, dim3((a.channels * (TAPS + 1) + 63) / 64), dim3(256), 0, stream, a.parts, a.workers,
+  static int run(Conv a, uint32_t blocks, float *dweight, float *dbias, hipStream_t stream) {
+    const uint32_t parts = parts_of<4, kGradThreads>(a.channels);
+    hipLaunchKernelGGL((conv_grad_rows<T, TAPS, WIDE>), dim3(blocks * parts), dim3(kGradThreads), 0, stream, a);
+    hipLaunchKernelGGL(conv_grad_sums, dim3((a.channels * (TAPS + 1) + 63) / 64), dim3(1024), 0, stream, a.parts, blocks,
                        a.channels, (uint32_t)TAPS, dweight, dbias);
     return launched();
   }
@@ -305,7 +408,7 @@ extern "C" int uor_trunk_conv_async(const uor_trunk_conv_args *s, void *stream) 
   if (s->tokens && !s->y) return fail(-1, "null y");
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return by_taps<RowsCall>(s, conv_of(s), (hipStream_t)stream);
+  return by_form<RowsCall>(s, conv_of(s, kRun), (hipStream_t)stream);
 }
 
 extern "C" int uor_trunk_conv_step_async(const uor_trunk_conv_args *s, void *stream) {
@@ -315,12 +418,12 @@ extern "C" int uor_trunk_conv_step_async(const uor_trunk_conv_args *s, void *str
   if (!s->index && s->slots < s->tokens) return fail(-1, "%u rows for %u states", s->tokens, s->slots);
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return by_taps<StepCall>(s, conv_of(s), (hipStream_t)stream);
+  return by_form<StepCall>(s, conv_of(s, kRun), (hipStream_t)stream);
 }
 
 extern "C" uint64_t uor_trunk_conv_backward_workspace_bytes(const uor_trunk_conv_args *s) {
   if (check_conv(s, false)) return 0;
-  return (uint64_t)workers_of(pieces(s->tokens, s->seqs, kRun), s->channels) * (s->taps + 1) * s->channels * sizeof(float);
+  return (uint64_t)grad_blocks_of(pieces(s->tokens, s->seqs, kGradRun), s->channels) * (s->taps + 1) * s->channels * sizeof(float);
 }
 
 extern "C" int uor_trunk_conv_backward_async(const uor_trunk_conv_args *s, void *workspace, uint64_t bytes, void *stream) {
@@ -329,10 +432,11 @@ extern "C" int uor_trunk_conv_backward_async(const uor_trunk_conv_args *s, void 
   const uint64_t want = uor_trunk_conv_backward_workspace_bytes(s);
   if (!workspace || bytes < want || (uintptr_t)workspace % 16)
     return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)want);
-  Conv a = conv_of(s);
-  a.workers = workers_of(a.pieces, s->channels);
+  Conv a = conv_of(s, kGradRun);
+  const uint32_t blocks = grad_blocks_of(a.pieces, s->channels);
+  a.workers = blocks * lines_of<4, kGradThreads>(s->channels);
   a.parts = (float *)workspace;
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return by_taps<GradCall>(s, a, s->dweight, s->dbias, (hipStream_t)stream);
+  return by_form<GradCall>(s, a, blocks, s->dweight, s->dbias, (hipStream_t)stream);
 }

@@ -236,20 +236,12 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
   }
 }
 
-// The blocks' sums: 64 sums a block, four threads a sum, each a quarter of the blocks.
-__global__ __launch_bounds__(256) void norms_grad_sums(const float *parts, uint32_t workers, uint32_t width, float *dpost,
-                                                       float *dscale, float *dpre) {
-  __shared__ float part[4][64];
-  const uint32_t at = blockIdx.x * 64 + threadIdx.x % 64, n = 3 * width, quarter = threadIdx.x / 64;
-  float v = 0.0f;
-  if (at < n)
-    for (uint32_t w = quarter; w < workers; w += 4) v += parts[(uint64_t)w * n + at];
-  part[quarter][threadIdx.x % 64] = v;
-  __syncthreads();
-  if (quarter || at >= n) return;
-  v = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-  float *to = at < width ? dpost : at < 2 * width ? dscale : dpre;
-  if (to) to[at % width] = v;
+__global__ __launch_bounds__(1024) void norms_grad_sums(const float *parts, uint32_t workers, uint32_t width, float *dpost,
+                                                        float *dscale, float *dpre) {
+  sum_columns(parts, workers, 3 * width, [&](uint32_t at, float v) {
+    float *to = at < width ? dpost : at < 2 * width ? dscale : dpre;
+    if (to) to[at % width] = v;
+  });
 }
 
 namespace {
@@ -356,7 +348,7 @@ extern "C" int uor_trunk_norms_backward_async(const uor_trunk_norms_args *s, voi
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
   if (const int e = s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(a, true, (hipStream_t)stream) : launch<float>(a, true, (hipStream_t)stream)) return e;
-  hipLaunchKernelGGL(norms_grad_sums, dim3((3 * s->width + 63) / 64), dim3(256), 0, (hipStream_t)stream, a.parts, a.workers, s->width,
+  hipLaunchKernelGGL(norms_grad_sums, dim3((3 * s->width + 63) / 64), dim3(1024), 0, (hipStream_t)stream, a.parts, a.workers, s->width,
                      s->dpost, s->dscale, s->dpre);
   return launched();
 }

@@ -339,7 +339,7 @@ int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
 }
 
 // The values of dim that a wavefront holds the state of: as many as its registers have room for.
-uint32_t part_of(const uor_trunk_scan_args *s) { return 32; }
+uint32_t part_of(const uor_trunk_scan_args *) { return 32; }
 uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + part_of(s) - 1) / part_of(s))); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;

@@ -38,7 +38,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// 1 / (1 + e^-v): the exponent's rounding, |v| 2^-24 of e^-v, is at most 2^-25 of v sigmoid(v).
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp2_(-kLog2e * v)); }
 // e^v of v <= 0, to 2^-22 of it: what the rounding of v log2(e) leaves goes into the result.
 __device__ __forceinline__ float exp_down(float v) {
   v = fmaxf(v, -120.0f);
@@ -120,6 +121,23 @@ __device__ __forceinline__ V8<T> load8(const T *row, bool there, uint32_t col, u
   for (int e = 0; e < 8; e++)
     if (col + e < cols) v[e] = row[col + e];
   return v;
+}
+
+// The sums of the columns of parts[rows][n], each given to put(column, sum), in one order: a block
+// of 1,024 threads takes 64 columns, 16 threads a column.
+template <class F>
+__device__ __forceinline__ void sum_columns(const float *parts, uint32_t rows, uint32_t n, F put) {
+  __shared__ float part[16][64];
+  const uint32_t at = blockIdx.x * 64 + threadIdx.x % 64, share = threadIdx.x / 64;
+  float v = 0.0f;
+  if (at < n)
+#pragma unroll 8
+    for (uint32_t r = share; r < rows; r += 16) v += parts[(uint64_t)r * n + at];
+  part[share][threadIdx.x % 64] = v;
+  __syncthreads();
+  if (share || at >= n) return;
+  for (int k = 1; k < 16; k++) v += part[k][threadIdx.x];
+  put(at, v);
 }
 
 // Host side: the last error's text, and a call's device.
