@@ -260,6 +260,10 @@ int check_scan(const uor_trunk_scan_args *s, bool step);
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
 dim3 join_of(const Scan &a, uint32_t seqs);
 uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units);
-inline uint32_t tiles_of(uint32_t dim) { return (dim + 63) / 64; }
+// Whether rows whose heads or groups are `part` values can be read 16 bytes at a time, and a chunk of
+// them by offsets of 32 bits.
+inline bool wide_rows(const void *p, int64_t stride, uint32_t part, uint32_t bytes) {
+  return aligned16(p, stride, bytes) && part * bytes % 16 == 0 && stride < (1 << 22);
+}
 
 }  // namespace trunk

@@ -203,63 +203,6 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
     put_state<NT, PW>(h, a.final + ((uint64_t)at.seq * a.heads + head) * whole + part, dim, a.state, a.state_wide);
 }
 
-// A piece's end state from zeros and its whole decay; a sequence's last piece needs neither.
-template <class T, int NT, int PW, int W>
-__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
-  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP), kThreads_ = 64 * W;
-  __shared__ __align__(16) T sB[kChunk * kNp], sXs[W][kChunk * kPp];
-  __shared__ Steps steps[W];
-  const Unit unit = unit_of<W>(a, kP);
-  Piece at;
-  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at) || at.end == at.stop) return;
-  const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
-  const uint32_t head = unit.head;
-  const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + unit.group * a.state;
-  const uint32_t dim = a.dim - unit.p0 < (uint32_t)kP ? a.dim - unit.p0 : kP;
-  const float A = a.A[head], bias = a.bias ? a.bias[head] : 0.0f;
-  f32x4 h[NT][PW];
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int i = 0; i < PW; i++) h[n][i] = f32x4{0, 0, 0, 0};
-  double total = 0.0;
-  Load<T, kN, kThreads_> nextB;
-  Load<T, kP, 64> nextX;
-  float raw = 0.0f;
-  const auto fetch = [&](uint32_t first) {
-    const int lane = anew(lane0), thread = wave * 64 + lane;
-    const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
-    nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
-    nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
-    raw = first + lane < end ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
-  };
-  fetch(at.first);  // past the last chunk nothing is read: rows that are always fetched need no register before
-  for (uint32_t first = at.first; first < at.end; first += kChunk) {
-    const uint32_t end = at.end - first > kChunk ? first + kChunk : at.end;
-    const int lane = anew(lane0), thread = wave * 64 + lane;
-    __syncthreads();
-    nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
-    nextX.put(lane, sXs[wave], a.x_stride, dim, a.x_wide);
-    const Decay d = steps_of(lane, steps[wave], raw, first + lane < end, A, bias);
-    __syncthreads();
-    fetch(end);
-    if (unit.idle) continue;
-    V8<T> xs[2][PW];
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-#pragma unroll
-      for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sXs[wave], 32 * k, i);
-    advance<T, NT, PW>(lane, h, xs, sB, steps[wave].v, d.to, d.whole);
-    total += d.total;
-  }
-  if (unit.idle) return;
-  const uint64_t slot = (uint64_t)unit.piece * a.heads + head;
-  put_state<NT, PW>(h, a.starts + slot * a.dim * a.state + (uint64_t)unit.p0 * a.state, dim, a.state, a.state_wide);
-  if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
-}
-
-constexpr uint32_t kAhead = 8;
-
 // The pieces' end states into their start states, along each sequence that has more than one.
 __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
   const uint32_t seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
@@ -316,7 +259,7 @@ template <class T, int NT, int PW, int W>
 int launch(Scan a, uint32_t seqs, hipStream_t stream) {
   const uint32_t units = a.heads / a.groups * a.tiles, blocks = grid_of(a.pieces, a.groups * ((units + W - 1) / W));
   if (a.starts) {
-    hipLaunchKernelGGL((scan_ends<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((scan_ends<T, NT, PW, W, false>), dim3(blocks), dim3(64 * W), 0, stream, a);
     hipLaunchKernelGGL(scan_join, join_of(a, seqs), dim3(kThreads), 0, stream, a);
   }
   hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
@@ -368,13 +311,11 @@ int check_scan(const uor_trunk_scan_args *s, bool step) {
 // A call's arguments as the kernels take them, cut into pieces of `size` rows.
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size) {
   const uint32_t bytes = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
-  const auto wide = [&](const void *p, int64_t stride, uint32_t part) {
-    return aligned16(p, stride, bytes) && part * bytes % 16 == 0 && stride < (1 << 22);  // a chunk's rows within 2^31 bytes
-  };
+  const auto wide = [&](const void *p, int64_t stride, uint32_t part) { return wide_rows(p, stride, part, bytes); };
   Scan a{};
   a.rows = Rows{s->offsets, s->tokens, s->seqs};
   a.heads = s->heads, a.groups = s->groups, a.dim = s->dim, a.state = s->state;
-  a.size = size, a.pieces = pieces(s->tokens, s->seqs, size), a.tiles = tiles_of(s->dim);
+  a.size = size, a.pieces = pieces(s->tokens, s->seqs, size), a.tiles = (s->dim + 31) / 32;
   a.x_stride = s->x_stride, a.dt_stride = s->dt_stride, a.b_stride = s->b_stride, a.c_stride = s->c_stride, a.y_stride = s->y_stride;
   a.x = s->x, a.dt = s->dt, a.B = s->B, a.C = s->C, a.A = s->A, a.D = s->D, a.bias = s->dt_bias;
   a.initial = s->initial, a.y = s->y, a.final = s->final;

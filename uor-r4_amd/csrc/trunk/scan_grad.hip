@@ -8,369 +8,554 @@
 //   dC_t = e^(l_t) h^T dy_t + sum_(s <= t) W_ts e_ts D_s B_s,
 //   g'   = e^(l_end) g + sum_t e^(l_t) dy_t (x) C_t   for the chunk before.
 //
-// W_ts e_ts D_s is summed over a group's heads before its two products with B and C. With
-// E_ts = W_ts S_ts e_ts D_s, q_t = e^(l_t) C_t . h^T dy_t and r_s = D_s e^(l_end - l_s) B_s . g^T x_s,
-// the gradient at the logarithm of row u's decay is
+// The gradient at the logarithm of row u's decay is
 //
-//   da_u = e^(l_end) <g, h> + sum_(t >= u) q_t + sum_(s < u) r_s + sum_(t >= u, s < u) E_ts,
+//   da_u = e^(l_end) <g, h> + sum_(s < u) r_s + sum_(t >= u) C_t . dC_t - sum_(s >= u) D_s x_s . i_s,
 //
-// whose last sum is the sum over t >= u of E's row t less its column t. At the step itself it is
-// (r_u + column u of E) / D_u + A da_u, where what D_u divides is summed without it.
+// with r_s = D_s x_s . (what g gives dx_s) and i_s what the chunk's own rows give it: C_t . dC_t is what
+// row t has from the state and from all rows up to it, of which those from u on are taken off again.
+// At the step itself it is x_u . (dx_u - skip dy_u) / D_u + A da_u, where what D_u divides is summed
+// without it.
 //
-// First all chunks' h and g are written by two launches that go along the sequences and back (cut
-// into pieces where those are long, as in the scan); then every chunk of every group is a block.
-#include "scan.h"
+// A block takes one group of one piece of a sequence, a wavefront one of its heads (or 32 of a head's
+// values), with g in registers. It goes along the piece once for h, and writes the states before its
+// chunks down but for the last, which it still holds; then back, chunk after chunk. Both states are
+// wanted in two layouts: h is summed as columns of the state's axis, and g, held as columns of x's
+// values, is turned by products with parts of the unit matrix, which are exact. dB and dC are summed
+// over the block's wavefronts through LDS, in their order. Long sequences are cut into pieces as in
+// the scan; one launch more gives every piece's gradient at its start.
+#include "wave.h"
 
 namespace trunk {
 
 struct Grad {
-  Scan s;               // pieces of the sweeps; s.starts as there, for the sweep that runs
+  Scan s;               // s.tiles: parts of dim, rounded up to a power of two
   const void *dy;
   const float *dfinal;
-  uint32_t chunks;      // places of chunks
-  uint32_t parts;       // blocks that share a group's heads
-  float *h, *g, *gt;    // [chunks][heads * tiles][16 NT x 16 PW]: h and gt by rows of state, g by rows of dim
-  float *sums;          // [chunks][heads][3]: dA, dD, ddt_bias
-  float *dBparts, *dCparts;  // [parts][tokens][groups][state], with more than one part
+  uint32_t subs, parts; // a group's wavefronts are taken in so many turns, shared by so many blocks
+  float *h;             // [tokens / 64 + 1][heads * tiles][NT * 2][64][4]: states before chunks
+  float *g_starts;      // like s.starts: the gradients at the pieces' ends
+  double *sums;         // [pieces][heads][3]: dA, dD, ddt_bias
+  float *dBparts, *dCparts;  // [parts][tokens][groups][state], with more than one turn
   void *dx, *ddt, *dB, *dC;
   float *dA, *dD, *dbias, *dinitial;
-  bool dy_wide, dx_wide;
+  bool dy_wide, dx_wide, shared_wide;
 };
 
-// The states along a piece: forward from its start, or back from its end (x then is dy, B is C).
-// STORE: every chunk's is written; otherwise only the piece's last, for the join.
-template <class T, int NT, int PW, bool BACK, bool STORE>
-__global__ __launch_bounds__(kThreads) void grad_states(Grad k) {
-  constexpr int kN = 16 * NT, kP = 16 * PW, kLp = pitch<T>(kChunk), kTiles = NT * PW / 4;
-  __shared__ __align__(16) T sBt[kN * kLp], sXt[kP * kLp];
-  __shared__ Decays d;
-  const Scan &a = k.s;
-  uint32_t number, place;
-  place_of(blockIdx.x, a.heads * a.tiles, number, place);
-  const uint32_t tile = place % a.tiles, head = place / a.tiles, p0 = tile * kP;
-  Piece at;
-  if (number >= a.pieces || !piece(a.rows, number, a.size, at)) return;
-  // The sequence's last piece this way has nothing after it to start.
-  const bool last = BACK ? at.first == at.start : at.end == at.stop;
-  if (!STORE && last) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
-  const uint32_t group = head / (a.heads / a.groups);
-  const T *x = (const T *)(BACK ? k.dy : a.x) + head * a.dim + p0, *dt = (const T *)a.dt + head;
-  const T *B = (const T *)(BACK ? a.C : a.B) + group * a.state;
-  const int64_t x_stride = BACK ? a.y_stride : a.x_stride, b_stride = BACK ? a.c_stride : a.b_stride;
-  const bool x_wide = BACK ? k.dy_wide : a.x_wide, b_wide = BACK ? a.c_wide : a.b_wide;
-  const uint32_t dim = a.dim - p0 < (uint32_t)kP ? a.dim - p0 : kP;
-  const float A = a.A[head], bias = a.bias ? a.bias[head] : 0.0f;
-  const uint64_t whole = (uint64_t)a.dim * a.state;
-  const Own<NT, PW> own;
-  f32x4 h[kTiles];
-  const float *from = BACK ? k.dfinal : a.initial;
-  const uint64_t slot = (uint64_t)number * a.heads + head;
-  load_state<NT, PW>(h, own, !STORE ? nullptr : a.starts && (BACK || at.number) ? a.starts + slot * whole : from ? from + ((uint64_t)at.seq * a.heads + head) * whole : nullptr,
-                     p0, a.dim, a.state);
-  const uint32_t chunks = (at.end - at.first + kChunk - 1) / kChunk;
-  const uint64_t base = at.start / kChunk + at.seq + (at.first - at.start) / kChunk;
-  double total = 0.0;
-  for (uint32_t i = 0; i < chunks; i++) {
-    const uint32_t j = BACK ? chunks - 1 - i : i;
-    const uint32_t first = at.first + j * kChunk, end = at.end - first > kChunk ? first + kChunk : at.end;
-    if constexpr (STORE) {
-      const bool zeros = !from && (BACK ? end == at.stop : first == at.start);  // never read
-      if (!zeros) {
-        const uint64_t to = ((base + j) * a.heads * a.tiles + place) * (kN * kP);
+// The 32 x 16 part `which` of the unit matrix as an operand.
+template <class T>
+__device__ __forceinline__ V8<T> ones(int lane, int which) {
+  V8<T> v;
 #pragma unroll
-        for (int e = 0; e < kTiles; e++) {
-          const int n = (own.n + e) * 16 + 4 * q, p = own.p * 16 + i16;
-          float *turned = (BACK ? k.gt : k.h) + to;
+  for (int e = 0; e < 8; e++) v[e] = (T)(e >> 2 == which && 4 * (lane >> 4) + (e & 3) == (lane & 15) ? 1.0f : 0.0f);
+  return v;
+}
+// The turned parts: two operands of a row's 32 places each, as one of the places' rows `which`.
+__device__ __forceinline__ bf16x8 turn(bf16x8 a, bf16x8 b, bf16x8 unit) {
+  const f32x4 zero = {0, 0, 0, 0};
+  const f32x4 x = Mma<bf16>::mul(a, unit, zero), y = Mma<bf16>::mul(b, unit, zero);
+  return __builtin_convertvector(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), bf16x8);
+}
+__device__ __forceinline__ Fine<bf16> turn(const Fine<bf16> &a, const Fine<bf16> &b, bf16x8 unit) {
+  return {turn(a.hi, b.hi, unit), turn(a.mid, b.mid, unit), turn(a.lo, b.lo, unit)};
+}
+__device__ __forceinline__ Fine<float> turn(const Fine<float> &a, const Fine<float> &b, f32x8 unit) {
+  const f32x4 zero = {0, 0, 0, 0};
+  return {__builtin_shufflevector(Mma<float>::mul(a.v, unit, zero), Mma<float>::mul(b.v, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+__device__ __forceinline__ f32x8 whole_of(const Fine<bf16> &a) {
+  return __builtin_convertvector(a.hi, f32x8) + (__builtin_convertvector(a.mid, f32x8) + __builtin_convertvector(a.lo, f32x8));
+}
+__device__ __forceinline__ f32x8 whole_of(const Fine<float> &a) { return a.v; }
+
+__device__ __forceinline__ float dot(f32x8 a, f32x8 b) {
+  float v = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 4; r++) turned[(n + r) * kP + p] = h[e][r];
-          if (BACK) *(f32x4 *)(k.g + to + p * kN + n) = h[e];
-        }
-      }
-      // The state after the sequence's last chunk this way is read by no chunk.
-      if (last && i + 1 == chunks && !(BACK && k.dinitial)) break;
-    }
-    __syncthreads();
-    stage<T, kN>((T *)nullptr, sBt, B, b_stride, first, end, a.state, b_wide);
-    stage<T, kP>((T *)nullptr, sXt, x, x_stride, first, end, dim, x_wide);
-    if (wave == 0) decays(d, dt, a.dt_stride, first, end, A, bias);
-    __syncthreads();
-    advance<T, NT, PW>(h, own, sXt, sBt, BACK ? d.from : d.to, d.whole);
-    total += d.total;
-  }
-  if constexpr (STORE) {
-    if (BACK && k.dinitial && last)
-      store_state<NT, PW>(h, own, k.dinitial + ((uint64_t)at.seq * a.heads + head) * whole, p0, a.dim, a.state);
-  } else {
-    store_state<NT, PW>(h, own, a.starts + slot * whole, p0, a.dim, a.state);
-    if (threadIdx.x == 0 && p0 == 0) a.totals[slot] = total;
-  }
+  for (int e = 0; e < 8; e++) v = fmaf(a[e], b[e], v);
+  return v;
+}
+// The sum of a column's four lanes.
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
 }
 
-template <class T, int NT, int PW>
-__global__ __launch_bounds__(kThreads) void grad_rows(Grad k) {
-  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP), kLp = pitch<T>(kChunk);
-  constexpr int kZp = kChunk + 4;
-  // W summed over heads is handed over where x and dy were.
-  constexpr int kRowsBytes = 2 * kChunk * kPp * (int)sizeof(T), kZBytes = kChunk * kZp * 4;
-  __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sYt[kP * kLp];
-  __shared__ __align__(16) char sRows[kRowsBytes > kZBytes ? kRowsBytes : kZBytes];
-  __shared__ Decays d;
-  __shared__ float sQ[kChunk], sR[kChunk], sCol[kChunk], sDirect[kChunk], sRow[4][kChunk], sBase[4], sDiag[4];
-  T *sX = (T *)sRows, *sY = sX + kChunk * kPp;
-  float *sZ = (float *)sRows;
-  const Scan &a = k.s;
-  uint32_t number, place;
-  place_of(blockIdx.x, a.groups * k.parts, number, place);
-  Piece at;
-  if (number >= k.chunks || !piece(a.rows, number, kChunk, at) || at.first == at.end) return;
-  const uint32_t group = place / k.parts, part = place % k.parts, share = a.heads / a.groups;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i16 = lane & 15;
-  const bool has_h = a.initial || at.first != at.start, has_g = k.dfinal || at.end != at.stop;
-  const int mine = wave * 16 + i16;  // this lane's column: its row s, and its row t
-  const uint32_t row = at.first + mine;
-
-  stage<T, kN>(sB, (T *)nullptr, (const T *)a.B + group * a.state, a.b_stride, at.first, at.end, a.state, a.b_wide);
-  stage<T, kN>(sC, (T *)nullptr, (const T *)a.C + group * a.state, a.c_stride, at.first, at.end, a.state, a.c_wide);
-  __syncthreads();
-  f32x4 S[4], Z[4], accB[NT], accC[NT];
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    S[t] = Z[t] = f32x4{0, 0, 0, 0};
-    if (t < wave) continue;
-#pragma unroll
-    for (int n = 0; n < kN; n += 32)
-      S[t] = Mma<T>::mul(operand(sC + (t * 16 + i16) * kNp, n + 8 * q), operand(sB + mine * kNp, n + 8 * q), S[t]);
-  }
-#pragma unroll
-  for (int n = 0; n < NT; n++) accB[n] = accC[n] = f32x4{0, 0, 0, 0};
-
-  for (uint32_t head = group * share + share * part / k.parts; head < group * share + share * (part + 1) / k.parts; head++) {
-    const float A = a.A[head], bias = a.bias ? a.bias[head] : 0.0f, skip = a.D ? a.D[head] : 0.0f;
-    double da = 0.0;             // of row `lane`, on the first wavefront
-    float direct = 0.0f, diag = 0.0f;
-    for (uint32_t tile = 0; tile < a.tiles; tile++) {
-      const uint32_t p0 = tile * kP, dim = a.dim - p0 < (uint32_t)kP ? a.dim - p0 : kP;
-      __syncthreads();
-      stage<T, kP>(sX, (T *)nullptr, (const T *)a.x + head * a.dim + p0, a.x_stride, at.first, at.end, dim, a.x_wide);
-      stage<T, kP>(sY, sYt, (const T *)k.dy + head * a.dim + p0, a.y_stride, at.first, at.end, dim, k.dy_wide);
-      if (wave == 0 && tile == 0) decays(d, (const T *)a.dt + head, a.dt_stride, at.first, at.end, A, bias);
-      __syncthreads();
-      const uint64_t held = ((uint64_t)number * a.heads * a.tiles + head * a.tiles + tile) * (kN * kP);
-      const float step = d.step[mine], tail = d.tail[mine], from = d.from[mine], hi = d.hi[mine], lo = d.lo[mine];
-
-      // dx: what comes through the state after the chunk.
-      f32x4 dx[PW];
-#pragma unroll
-      for (int i = 0; i < PW; i++) dx[i] = f32x4{0, 0, 0, 0};
-      if (has_g) {
-#pragma unroll
-        for (int n = 0; n < kN; n += 32) {
-          const V8<T> b = operand(sB + mine * kNp, n + 8 * q);
-#pragma unroll
-          for (int i = 0; i < PW; i++)
-            dx[i] = Mma<T>::mul(Mma<T>::split(*(const f32x8 *)(k.g + held + (i * 16 + i16) * kN + n + 8 * q)), b, dx[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < PW; i++) dx[i] *= tail;
-      }
-      // W, and through it the chunk's own part of dx and of the sums.
-      float col = 0.0f, own = 0.0f;
-      f32x4 M[4];
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        M[t] = f32x4{0, 0, 0, 0};
-        if (t < wave) continue;
-        f32x4 w = {0, 0, 0, 0};
-#pragma unroll
-        for (int p = 0; p < kP; p += 32)
-          w = Mma<T>::mul(operand(sY + (t * 16 + i16) * kPp, p + 8 * q), operand(sX + mine * kPp, p + 8 * q), w);
-        float rows[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int tt = t * 16 + 4 * q + r;
-          const float e = tt > mine ? exp2_((d.hi[tt] - hi) + (d.lo[tt] - lo)) : 1.0f;
-          const float z = tt >= mine ? w[r] * e : 0.0f;
-          M[t][r] = tt >= mine ? S[t][r] * e : 0.0f;
-          Z[t][r] += z * step;
-          const float both = tt >= mine ? z * S[t][r] : 0.0f;
-          own += tt == mine ? both : 0.0f;
-          diag += tt == mine ? w[r] : 0.0f;
-          const float off = tt > mine ? both : 0.0f;
-          col += off;
-          rows[r] = off * step;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-#pragma unroll
-          for (int m = 1; m < 16; m <<= 1) rows[r] += __shfl_xor(rows[r], m);
-          if (i16 == 0) sRow[wave][t * 16 + 4 * q + r] = rows[r];
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 4; t++)
-        if (t < wave && lane < 16) sRow[wave][t * 16 + lane] = 0.0f;
-#pragma unroll
-      for (int pair = 0; pair < 2; pair++) {
-        if (2 * pair + 1 < wave) continue;
-        const auto m = Mma<T>::split(__builtin_shufflevector(M[2 * pair], M[2 * pair + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int i = 0; i < PW; i++) dx[i] = Mma<T>::mul(operand_tiles(sYt + (i * 16 + i16) * kLp, pair * 32 + 4 * q), m, dx[i]);
-      }
-      if (row < at.end) {
-        T *to = (T *)k.dx + ((uint64_t)row * a.heads + head) * a.dim + p0;
-#pragma unroll
-        for (int i = 0; i < PW; i++) {
-          const uint32_t p = i * 16 + 4 * q;
-          const V4<T> y = *(const V4<T> *)(sY + mine * kPp + p);
-          V4<T> v;
-#pragma unroll
-          for (int r = 0; r < 4; r++) v[r] = (T)(step * dx[i][r] + skip * (float)y[r]);
-          if (k.dx_wide && p + 4 <= dim) {
-            *(V4<T> *)(to + p) = v;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-              if (p + r < dim) to[p + r] = v[r];
-          }
-        }
-      }
-      // dB and dC: what comes through the states.
-      float through = 0.0f, into = 0.0f, inner = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        f32x4 vb = {0, 0, 0, 0}, vc = {0, 0, 0, 0};
-#pragma unroll
-        for (int p = 0; p < kP; p += 32) {
-          const uint64_t place8 = held + (n * 16 + i16) * kP + p + 8 * q;
-          f32x8 g, h;
-          if (has_g) {
-            g = *(const f32x8 *)(k.gt + place8);
-            vb = Mma<T>::mul(Mma<T>::split(g), operand(sX + mine * kPp, p + 8 * q), vb);
-          }
-          if (has_h) {
-            h = *(const f32x8 *)(k.h + place8);
-            vc = Mma<T>::mul(Mma<T>::split(h), operand(sY + mine * kPp, p + 8 * q), vc);
-          }
-          if (has_g && has_h && n % 4 == wave) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) inner += g[e] * h[e];
-          }
-        }
-        vb *= tail;
-        vc *= from;
-        const V4<T> b = *(const V4<T> *)(sB + mine * kNp + n * 16 + 4 * q), c = *(const V4<T> *)(sC + mine * kNp + n * 16 + 4 * q);
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          into += vb[r] * (float)b[r];
-          through += vc[r] * (float)c[r];
-        }
-        accB[n] += vb * step;
-        accC[n] += vc;
-      }
-      // A column's sums over its four lanes, and the wavefront's part of <g, h>.
-#pragma unroll
-      for (int m = 16; m < 64; m <<= 1) {
-        into += __shfl_xor(into, m);
-        through += __shfl_xor(through, m);
-        col += __shfl_xor(col, m);
-        own += __shfl_xor(own, m);
-      }
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) inner += __shfl_xor(inner, m);
-      if (q == 0) {
-        sQ[mine] = through;
-        sR[mine] = into;
-        sCol[mine] = col;
-        sDirect[mine] = into + col + own;
-      }
-      if (lane == 0) sBase[wave] = inner;
-      __syncthreads();
-      if (wave == 0) {
-        // da of row u = lane: sums over t >= u less those over s >= u, as one sum from the end, and the
-        // r of the rows before.
-        const float at_step = d.step[lane];
-        const double r = (double)(sR[lane] * at_step);
-        double later = (double)sQ[lane] + ((double)((sRow[0][lane] + sRow[1][lane]) + (sRow[2][lane] + sRow[3][lane])) - (double)(sCol[lane] * at_step));
-        double before = r;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const double l = __shfl_down(later, m), b = __shfl_up(before, m);
-          if (lane + m < 64) later += l;
-          if (lane >= m) before += b;
-        }
-        const double base = (double)d.whole * (double)((sBase[0] + sBase[1]) + (sBase[2] + sBase[3]));
-        da += later + (before - r) + base;
-        direct += sDirect[lane];
-      }
-    }
-    // The head's parameters and its steps.
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) diag += __shfl_xor(diag, m);
-    if (lane == 0) sDiag[wave] = diag;
-    __syncthreads();
-    if (wave == 0) {
-      float dstep = 0.0f, dA = 0.0f;
-      if (at.first + lane < at.end) {
-        const float raw = (float)((const T *)a.dt)[(int64_t)(at.first + lane) * a.dt_stride + head] + bias;
-        dstep = (direct + A * (float)da) * sigmoid(raw);
-        dA = d.step[lane] * (float)da;
-        ((T *)k.ddt)[(uint64_t)(at.first + lane) * a.heads + head] = (T)dstep;
-      }
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        dstep += __shfl_xor(dstep, m);
-        dA += __shfl_xor(dA, m);
-      }
-      if (lane == 0) {
-        float *to = k.sums + ((uint64_t)number * a.heads + head) * 3;
-        to[0] = dA;
-        to[1] = (sDiag[0] + sDiag[1]) + (sDiag[2] + sDiag[3]);
-        to[2] = dstep;
-      }
-    }
-  }
-
-  // The chunk's own part of dB and dC, of all heads at once.
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < 4; t++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) sZ[(t * 16 + 4 * q + r) * kZp + mine] = Z[t][r];
-  __syncthreads();
-#pragma unroll
-  for (int pair = 0; pair < 2; pair++) {
-    const auto zb = Mma<T>::split(__builtin_shufflevector(Z[2 * pair], Z[2 * pair + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-    const auto zc = Mma<T>::split(*(const f32x8 *)(sZ + mine * kZp + pair * 32 + 8 * q));
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      V8<T> c, b;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        c[e] = sC[(pair * 32 + (e >> 2) * 16 + 4 * q + (e & 3)) * kNp + n * 16 + i16];
-        b[e] = sB[(pair * 32 + 8 * q + e) * kNp + n * 16 + i16];
-      }
-      accB[n] = Mma<T>::mul(c, zb, accB[n]);
-      accC[n] = Mma<T>::mul(b, zc, accC[n]);
-    }
-  }
-  if (row >= at.end) return;
-  const uint64_t to = ((uint64_t)row * a.groups + group) * a.state;
+// h as columns of the state's axis: h[n][i] holds rows place(i, 4 q + r) of dim, column place(n, lane % 16).
+template <int NT>
+__device__ __forceinline__ void get_turned(int lane, f32x4 (&h)[NT][2], const float *at, uint32_t dim, uint32_t state) {
+  const int q = lane >> 4, i16 = lane & 15;
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const uint32_t c = n * 16 + 4 * q + r;
-      if (c >= a.state) continue;
-      if (k.parts == 1) {
-        ((T *)k.dB)[to + c] = (T)accB[n][r];
-        ((T *)k.dC)[to + c] = (T)accC[n][r];
-      } else {
-        const uint64_t plane = (uint64_t)part * a.rows.tokens * a.groups * a.state;
-        k.dBparts[plane + to + c] = accB[n][r];
-        k.dCparts[plane + to + c] = accC[n][r];
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t p = place(i, 4 * q + r), c = place(n, i16);
+        h[n][i][r] = at && p < dim && c < state ? at[(uint64_t)p * state + c] : 0.0f;
+      }
+}
+// advance, for a state that lies so.
+template <class T, int NT>
+__device__ __forceinline__ void advance_turned(int lane, f32x4 (&h)[NT][2], const T *sX, const T *sB, const float *rows, const float (&to)[4],
+                                               float whole) {
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) h[n][i] *= whole;
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const f32x8 weight = weights(lane, rows, 32 * k, to[2 * k], to[2 * k + 1]);
+    Fine<T> w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) w[i] = Fine<T>::of(widen<T>(column<T, pitch<T>(32)>(lane, sX, 32 * k, i)) * weight);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const V8<T> b = column<T, pitch<T>(16 * NT)>(lane, sB, 32 * k, n);
+#pragma unroll
+      for (int i = 0; i < 2; i++) h[n][i] = mul(w[i], b, h[n][i]);
+    }
+  }
+}
+
+// Wavefronts that a SIMD is to hold: with states of more than 64 a wavefront needs all its registers.
+template <int NT, int W>
+constexpr int kHeld = NT > 4 || W == 1 ? 1 : 2;
+
+template <class T, int NT, int W>
+__global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
+  constexpr int kN = 16 * NT, kP = 32, kNp = pitch<T>(kN), kPp = pitch<T>(kP), G = NT < 4 ? NT : 4;
+  __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sYs[W][kChunk * kPp];
+  __shared__ __align__(16) float sRed[W][G * 2 * 256];
+  __shared__ GradSteps steps[W];
+  __shared__ float sTurn[W][3][kChunk];  // C_t . dC_t, x_s . (what g gives dx_s), x_s . (all of dx_s)
+  __shared__ float sDa[W][kChunk], sDirect[W][kChunk], sDiag[W];
+  const Scan &a = k.s;
+  const uint32_t share = a.heads / a.groups, units = share * a.tiles;
+  uint32_t number, block;
+  place_of(blockIdx.x, a.groups * k.parts, number, block);
+  Piece at;
+  if (number >= a.pieces || !piece(a.rows, number, a.size, at)) return;
+  const uint32_t group = block / k.parts, part = block % k.parts;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
+  const T *B = (const T *)a.B + group * a.state, *C = (const T *)a.C + group * a.state;
+  const uint64_t whole = (uint64_t)a.dim * a.state;
+  const uint32_t chunks = (at.end - at.first + kChunk - 1) / kChunk;
+  T *sY = sYs[wave];
+  GradSteps &s = steps[wave];
+  const uint32_t sub0 = k.subs * part / k.parts, sub1 = k.subs * (part + 1) / k.parts;
+
+#pragma unroll 1
+  for (uint32_t sub = sub0; sub < sub1; sub++) {
+    uint32_t unit = sub * W + wave;
+    bool idle = unit >= units;
+    if (idle) unit = 0;
+    const uint32_t head = group * share + unit / a.tiles, tile = unit % a.tiles, p0 = tile * kP;
+    idle = idle || p0 >= a.dim;
+    const uint32_t dim = idle ? 0 : a.dim - p0 < (uint32_t)kP ? a.dim - p0 : kP;
+    const T *x = (const T *)a.x + head * a.dim + p0, *dy = (const T *)k.dy + head * a.dim + p0, *dt = (const T *)a.dt + head;
+    const float A = a.A[head], skip = a.D ? a.D[head] : 0.0f, bias = a.bias ? a.bias[head] : 0.0f;
+    const uint64_t cell = (uint64_t)p0 * a.state;
+    const float *start = at.number ? a.starts + ((uint64_t)number * a.heads + head) * whole + cell
+                                   : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + cell : nullptr;
+    const float *finish = at.end != at.stop ? k.g_starts + ((uint64_t)number * a.heads + head) * whole + cell
+                                            : k.dfinal ? k.dfinal + ((uint64_t)at.seq * a.heads + head) * whole + cell : nullptr;
+    // Where the state before the piece's j-th chunk is kept.
+    const auto kept = [&](uint32_t j) {
+      return k.h + (((uint64_t)(at.first / kChunk + j) * a.heads + head) * a.tiles + tile) * (NT * 2 * 256);
+    };
+
+    // Along the piece, but for its last chunk.
+    f32x4 h[NT][2];
+    get_turned<NT>(lane0, h, idle ? nullptr : start, dim, a.state);
+    {
+      Load<T, kN, 64 * W> nextB;
+      Load<T, kP, 64> nextX;
+      float raw = 0.0f;
+      const auto fetch = [&](uint32_t j) {
+        const uint32_t first = at.first + j * kChunk, rows = j + 1 < chunks ? kChunk : 0;
+        const int lane = anew(lane0), thread = wave * 64 + lane;
+        nextB.get(thread, B, a.b_stride, first, first + rows, a.state, a.b_wide);
+        nextX.get(lane, x, a.x_stride, first, first + rows, dim, a.x_wide && dim);
+        raw = rows ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
+      };
+      fetch(0);
+#pragma unroll 1
+      for (uint32_t j = 0; j + 1 < chunks; j++) {
+        const int lane = anew(lane0), thread = wave * 64 + lane;
+        __syncthreads();
+        nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+        nextX.put(lane, sY, a.x_stride, dim, a.x_wide && dim);
+        const Decay d = steps_of(lane, s, raw, true, A, bias);
+        __syncthreads();
+        fetch(j + 1);
+        if (idle) continue;
+        advance_turned<T, NT>(lane, h, sY, sB, s.v, d.to, d.whole);
+        if (j + 2 < chunks) {
+          float *to = kept(j + 1) + lane * 4;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) *(f32x4 *)(to + (n * 2 + i) * 256) = h[n][i];
+        }
       }
     }
+
+    // And back.
+    f32x4 g[NT][2];
+    get_state<NT, 2>(g, idle ? nullptr : finish, dim, a.state, a.state_wide);
+    double sumA = 0.0, sumD = 0.0, sumBias = 0.0;
+    Load<T, kN, 64 * W> nextB, nextC;
+    Load<T, kP, 64> nextY;
+    float raw = 0.0f;
+    const auto fetch = [&](uint32_t j) {  // none where j is past the first chunk
+      const bool more = j < chunks;
+      const uint32_t first = more ? at.first + j * kChunk : at.first;
+      const uint32_t end = !more ? first : at.end - first > kChunk ? first + kChunk : at.end;
+      const int lane = anew(lane0), thread = wave * 64 + lane;
+      nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
+      nextC.get(thread, C, a.c_stride, first, end, a.state, a.c_wide);
+      nextY.get(lane, dy, a.y_stride, first, end, dim, k.dy_wide && dim);
+      raw = first + lane < end ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
+    };
+    fetch(chunks - 1);
+#pragma unroll 1
+    for (uint32_t j = chunks; j-- > 0;) {
+      const uint32_t first = at.first + j * kChunk, end = at.end - first > kChunk ? first + kChunk : at.end;
+      const int lane = anew(lane0), thread = wave * 64 + lane, q = lane >> 4, i16 = lane & 15;
+      const bool has_h = start || j, has_g = finish || j + 1 < chunks, more = end - first > 32;
+      __syncthreads();
+      nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+      nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
+      nextY.put(lane, sY, a.y_stride, dim, k.dy_wide && dim);
+      const float raw_now = raw;
+      const Decay d = steps_of(lane, s, raw, first + lane < end, A, bias);
+      V8<T> X[4];  // x's rows, as operands over dim
+      {
+        const uint32_t pitch = (uint32_t)a.x_stride * sizeof(T);
+        const T *rows = x + (int64_t)first * a.x_stride;
+        const uint32_t bytes = a.x_wide && dim ? (end - first - 1) * pitch + dim * (uint32_t)sizeof(T) : 0;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)rows, 0, (int)bytes, 0x00020000);
+#pragma unroll
+        for (int t = 0; t < 4; t++) X[t] = load_eight<T>(from, (t * 16 + i16) * pitch + 8 * q * (uint32_t)sizeof(T), 8 * q, dim);
+        if (!a.x_wide) {
+#pragma unroll
+          for (int t = 0; t < 4; t++)
+            X[t] = load8(rows + (int64_t)(t * 16 + i16) * a.x_stride, first + t * 16 + i16 < end, 8 * q, dim, false);
+        }
+      }
+      if (!idle && j + 1 < chunks) {
+        if (j) {
+          const float *from = kept(j) + lane * 4;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) h[n][i] = *(const f32x4 *)(from + (n * 2 + i) * 256);
+        } else {
+          get_turned<NT>(lane, h, start, dim, a.state);
+        }
+      }
+      __syncthreads();
+
+      // dx, and g turned: what comes through the state after the chunk.
+      f32x4 dx[4][2];
+      typename Mma<T>::Split gt[NT];
+      float inner = 0.0f, diag = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; t++) dx[t][0] = dx[t][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < NT; n++) gt[n] = Mma<T>::split(f32x8{0, 0, 0, 0, 0, 0, 0, 0});
+      if (!idle && has_g) {
+#pragma unroll
+        for (int kk = 0; kk < NT / 2; kk++) {
+          Fine<T> gp[2];
+#pragma unroll
+          for (int i = 0; i < 2; i++) gp[i] = Fine<T>::of(__builtin_shufflevector(g[2 * kk][i], g[2 * kk + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            const V8<T> b = operand(sB + (t * 16 + i16) * kNp, 32 * kk + 8 * q);
+#pragma unroll
+            for (int i = 0; i < 2; i++) dx[t][i] = mul(gp[i], b, dx[t][i]);
+          }
+#pragma unroll
+          for (int w = 0; w < 2; w++) {
+            const int n = 2 * kk + w;
+            const f32x8 turned = whole_of(turn(gp[0], gp[1], ones<T>(lane, w)));
+            inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
+            gt[n] = Mma<T>::split(turned);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const float tail = s.w[t * 16 + i16] * d.to[t];
+#pragma unroll
+          for (int i = 0; i < 2; i++) dx[t][i] *= tail;
+        }
+      }
+      if (!idle) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const float into = column_sum(dot(widen<T>(X[t]), __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7)));
+          if (q == 0) sTurn[wave][1][t * 16 + i16] = into;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      f32x4 accB[2][NT], accC[2][NT];
+      // What comes through the states, of two tiles of rows.
+      const auto begin_B = [&](int pair) {
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const int t = 2 * pair + w;
+          const float weight = s.v[t * 16 + i16] * d.to[t];
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            accB[w][n] = f32x4{0, 0, 0, 0};
+            if (!idle && has_g) accB[w][n] = Mma<T>::mul(gt[n], X[t], accB[w][n]) * weight;
+          }
+        }
+      };
+      const auto begin_C = [&](int pair) {
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+          for (int n = 0; n < NT; n++) accC[w][n] = f32x4{0, 0, 0, 0};
+        if (idle || !has_h) return;
+        V8<T> y[2];
+        float weight[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const int t = 2 * pair + w;
+          y[w] = operand(sY + (t * 16 + i16) * kPp, 8 * q);
+          weight[w] = s.u[t * 16 + i16] * d.from[t];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const auto hp = Fine<T>::of(__builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int w = 0; w < 2; w++) accC[w][n] = mul(hp, y[w], accC[w][n]) * weight[w];
+        }
+      };
+      // The chunk's own rows: rows s of pair sp with rows t of pair tp.
+      const auto rows_with = [&](int sp, int tp) {
+        if (idle) return;
+        Fine<T> Z[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const int ss = 2 * sp + w, mine = ss * 16 + i16;
+          const float step = s.step[mine], to_end = s.w[mine], hi_s = s.hi[mine], lo_s = s.lo[mine];
+          V8<T> b[NT / 2];
+#pragma unroll
+          for (int kk = 0; kk < NT / 2; kk++) b[kk] = operand(sB + mine * kNp, 32 * kk + 8 * q);
+          f32x4 M[2], z[2];
+#pragma unroll
+          for (int v = 0; v < 2; v++) {
+            const int tt = 2 * tp + v;
+            M[v] = z[v] = f32x4{0, 0, 0, 0};
+            if (tt < ss) continue;
+            f32x4 S = {0, 0, 0, 0};
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; kk++) S = Mma<T>::mul(operand(sC + (tt * 16 + i16) * kNp, 32 * kk + 8 * q), b[kk], S);
+            const f32x4 Wt = Mma<T>::mul(operand(sY + (tt * 16 + i16) * kPp, 8 * q), X[ss], f32x4{0, 0, 0, 0});
+            if (tt > ss) {
+              const float c = tt == ss + 1 ? 1.0f : tt == 2 ? d.c20 : ss == 0 ? d.c30 : d.c31;
+              const f32x4 e = *(const f32x4 *)(s.u + tt * 16 + 4 * q) * (c * to_end);
+              M[v] = S * e;
+              z[v] = Wt * e * step;
+            } else {
+              const f32x4 hi = *(const f32x4 *)(s.hi + tt * 16 + 4 * q), lo = *(const f32x4 *)(s.lo + tt * 16 + 4 * q);
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const int row = 4 * q + r;
+                const float e = exp2_((hi[r] - hi_s) + (lo[r] - lo_s));
+                M[v][r] = keep(S[r] * e, row > i16) + keep(S[r], row == i16);
+                z[v][r] = (keep(Wt[r] * e, row > i16) + keep(Wt[r], row == i16)) * step;
+                diag += keep(Wt[r], row == i16);
+              }
+            }
+          }
+          const auto m = Fine<T>::of(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int i = 0; i < 2; i++) dx[ss][i] = mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[ss][i]);
+          Z[w] = Fine<T>::of(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
+#pragma unroll
+          for (int w = 0; w < 2; w++) accB[w][n] = mul(c, Z[w], accB[w][n]);
+        }
+        Fine<T> Zt[2];
+#pragma unroll
+        for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
+#pragma unroll
+          for (int v = 0; v < 2; v++) accC[v][n] = mul(b, Zt[v], accC[v][n]);
+        }
+      };
+      // The sums over the block's wavefronts, of two tiles of rows, and out: turns after the first add
+      // to what the turn before wrote, by the same threads.
+      const auto reduce = [&](const f32x4 (&acc)[2][NT], int pair, T *out, float *between) {
+#pragma unroll
+        for (int n0 = 0; n0 < NT; n0 += G) {
+#pragma unroll
+          for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int n = 0; n < G; n++) *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = acc[w][n0 + n];
+          __syncthreads();
+          for (uint32_t item = thread; item < G * 64; item += 64 * W) {
+            const uint32_t of = item & 63, w = item >> 6 & 1, n = item >> 7 << 1;
+            f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+              lo += *(const f32x4 *)(sRed[i] + ((w * G + n) * 64 + of) * 4);
+              hi += *(const f32x4 *)(sRed[i] + ((w * G + n + 1) * 64 + of) * 4);
+            }
+            const uint32_t row = first + (2 * pair + w) * 16 + (of & 15), col = (n0 + n) * 16 + 8 * (of >> 4);
+            if (row >= end || col >= a.state) continue;
+            f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const uint64_t to = ((uint64_t)row * a.groups + group) * a.state + col;
+            if (k.subs > 1) {
+              float *mid = between + (uint64_t)part * a.rows.tokens * a.groups * a.state + to;
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (col + e < a.state) {
+                  if (sub > sub0) v[e] += mid[e];
+                  if (sub + 1 < sub1 || k.parts > 1) mid[e] = v[e];
+                }
+              if (sub + 1 < sub1 || k.parts > 1) continue;
+            }
+            const V8<T> o = __builtin_convertvector(v, V8<T>);
+            if (k.shared_wide) {
+              *(V8<T> *)(out + to) = o;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (col + e < a.state) out[to + e] = o[e];
+            }
+          }
+          __syncthreads();
+        }
+      };
+      const auto finish_C = [&](int pair) {
+        if (!idle) {
+#pragma unroll
+          for (int w = 0; w < 2; w++) {
+            const int t = (2 * pair + w) * 16 + i16;
+            float through = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; kk++)
+              through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
+                             __builtin_shufflevector(accC[w][2 * kk], accC[w][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+            through = column_sum(through);
+            if (q == 0) sTurn[wave][0][t] = through;
+          }
+        }
+        reduce(accC, pair, (T *)k.dC, k.dCparts);
+      };
+      const auto finish_x = [&](int pair) {
+        if (idle) return;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const int t = 2 * pair + w, mine = t * 16 + i16;
+          const f32x8 all = __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const float direct = column_sum(dot(widen<T>(X[t]), all));
+          if (q == 0) sTurn[wave][2][mine] = direct;
+          if (first + mine >= end) continue;
+          const f32x8 v = all * s.step[mine] + widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
+          const V8<T> o = __builtin_convertvector(v, V8<T>);
+          T *to = (T *)k.dx + ((uint64_t)(first + mine) * a.heads + head) * a.dim + p0 + 8 * q;
+          if (k.dx_wide && 8 * q + 8 <= (int)dim) {
+            *(V8<T> *)to = o;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (8 * q + e < (int)dim) to[e] = o[e];
+          }
+        }
+      };
+      begin_C(0);
+      begin_B(0);
+      rows_with(0, 0);
+      finish_C(0);
+      if (more) {
+        begin_C(1);
+        rows_with(0, 1);
+      }
+      finish_x(0);
+      reduce(accB, 0, (T *)k.dB, k.dBparts);
+      if (more) {
+        begin_B(1);
+        rows_with(1, 1);
+        finish_C(1);
+        finish_x(1);
+        reduce(accB, 1, (T *)k.dB, k.dBparts);
+      }
+
+      // A row a lane: the gradients at its decay and its step, of all the head's wavefronts.
+      if (!idle) {
+        const bool there = first + lane < end && (more || lane < 32);
+        const float step = s.step[lane];
+        const float r = there ? sTurn[wave][1][lane] * step : 0.0f, own = there ? sTurn[wave][2][lane] - sTurn[wave][1][lane] : 0.0f;
+        const double later = there ? (double)sTurn[wave][0][lane] - (double)(own * step) : 0.0;
+        const double before = running_sum((double)r), through = running_sum(later);
+        const double base = has_g ? (double)d.whole * (double)wave_sum(inner) : 0.0;
+        sDa[wave][lane] = (float)(base + (before - (double)r) + (lane_of(through, 63) - (through - later)));
+        sDirect[wave][lane] = there ? sTurn[wave][2][lane] : 0.0f;
+        const float all = wave_sum(diag);
+        if (lane == 0) sDiag[wave] = all;
+      } else {
+        sDa[wave][lane] = sDirect[wave][lane] = 0.0f;
+        if (lane == 0) sDiag[wave] = 0.0f;
+      }
+      __syncthreads();
+      if (!idle && tile == 0) {
+        float da = 0.0f, direct = 0.0f, all = 0.0f;
+        for (uint32_t i = 0; i < a.tiles; i++) {
+          da += sDa[wave + i][lane];
+          direct += sDirect[wave + i][lane];
+          all += sDiag[wave + i];
+        }
+        if (lane == 0) sumD += (double)all;
+        if (first + lane < end) {
+          const float dstep = (direct + A * da) * sigmoid(raw_now + bias);
+          sumA += (double)(s.step[lane] * da);
+          sumBias += (double)dstep;
+          ((T *)k.ddt)[(uint64_t)(first + lane) * a.heads + head] = (T)dstep;
+        }
+      }
+      fetch(j - 1);
+      if (!idle && (j || (!at.number && k.dinitial))) {
+        V8<T> ys[2][2];
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) ys[kk][i] = column<T, kPp>(lane, sY, 32 * kk, i);
+        advance<T, NT, 2>(lane, g, ys, sC, s.u, d.from, d.whole);
+      }
+    }
+    if (idle) continue;
+    if (!at.number && k.dinitial)
+      put_state<NT, 2>(g, k.dinitial + ((uint64_t)at.seq * a.heads + head) * whole + cell, dim, a.state, a.state_wide);
+    if (tile == 0) {
+      sumA = wave_sum(sumA), sumD = wave_sum(sumD), sumBias = wave_sum(sumBias);
+      if (lane0 == 0) {
+        double *to = k.sums + ((uint64_t)number * a.heads + head) * 3;
+        to[0] = sumA, to[1] = sumD, to[2] = sumBias;
+      }
+    }
+  }
 }
 
 // The parts' sums of dB and dC, in their order.
@@ -387,19 +572,19 @@ __global__ __launch_bounds__(256) void grad_parts(Grad k) {
   ((T *)k.dC)[at] = (T)c;
 }
 
-// The chunks' sums of the parameters' gradients, a block a head. Places of chunks that no sequence
-// has hold nothing, and are left out as they were in grad_rows.
-__global__ __launch_bounds__(256) void grad_sums(Grad k) {
-  __shared__ double part[3][256];
+// The pieces' sums of the parameters' gradients, a block a head. Places of pieces that no sequence has
+// hold nothing, and are left out.
+__global__ __launch_bounds__(1024) void grad_sums(Grad k) {
+  __shared__ double part[3][1024];
   const uint32_t head = blockIdx.x;
   double v[3] = {0.0, 0.0, 0.0};
-  for (uint32_t c = threadIdx.x; c < k.chunks; c += 256) {
+  for (uint32_t c = threadIdx.x; c < k.s.pieces; c += 1024) {
     Piece at;
-    if (!piece(k.s.rows, c, kChunk, at) || at.first == at.end) continue;
-    for (int i = 0; i < 3; i++) v[i] += (double)k.sums[((uint64_t)c * k.s.heads + head) * 3 + i];
+    if (!piece(k.s.rows, c, k.s.size, at)) continue;
+    for (int i = 0; i < 3; i++) v[i] += k.sums[((uint64_t)c * k.s.heads + head) * 3 + i];
   }
   for (int i = 0; i < 3; i++) part[i][threadIdx.x] = v[i];
-  for (int m = 128; m; m >>= 1) {
+  for (int m = 512; m; m >>= 1) {
     __syncthreads();
     if ((int)threadIdx.x < m)
       for (int i = 0; i < 3; i++) part[i][threadIdx.x] += part[i][threadIdx.x + m];
@@ -410,22 +595,34 @@ __global__ __launch_bounds__(256) void grad_sums(Grad k) {
   if (k.dbias) k.dbias[head] = (float)part[2][0];
 }
 
-// The pieces' end states into their start states, from each sequence's end.
+// The gradients at the pieces' starts, of their own y, into those at their ends, from each cut
+// sequence's end.
 __global__ __launch_bounds__(kThreads) void grad_join(Grad k) {
   const Scan &a = k.s;
   const uint32_t seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
   uint32_t start, end;
   a.rows.of(seq, start, end);
   const uint32_t n = end > start ? (end - start - 1) / a.size + 1 : 1;
-  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state;
+  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
+  if (n == 1) return;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float g = k.dfinal ? k.dfinal[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
-    for (uint32_t j = n; j-- > 0;) {
-      const uint64_t slot = (base + j) * a.heads + head;
-      float *at = a.starts + slot * whole + e;
-      const float own = j ? *at : 0.0f, decay = j ? exp2_((float)a.totals[slot]) : 0.0f;
-      *at = g;
-      g = decay * g + own;
+    float *at = k.g_starts + (base * a.heads + head) * whole + e;
+    const double *totals = a.totals + base * a.heads + head;
+    for (uint32_t j = 0; j < n; j += kAhead) {  // from the end
+      float own[kAhead], decay[kAhead];
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; i++) {
+        const uint32_t piece = j + i + 1 < n ? n - 1 - j - i : n - 1;
+        own[i] = at[piece * step];
+        decay[i] = (float)totals[(uint64_t)piece * a.heads];
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; i++) {
+        if (j + i >= n) break;
+        if (j + i) at[(n - 1 - j - i) * step] = g;
+        g = exp2_(decay[i]) * g + own[i];
+      }
     }
   }
 }
@@ -433,22 +630,28 @@ __global__ __launch_bounds__(kThreads) void scan_join(Scan a);
 
 namespace {
 
+uint32_t tiles_of(uint32_t dim) { return dim <= 32 ? 1 : dim <= 64 ? 2 : 4; }
+
 // Where a gradient's scratch memory begins, and how much there is.
 struct Plan {
-  uint32_t size, pieces, chunks, parts;
-  uint64_t cut, totals, h, g, gt, sums, dB, dC, bytes;
+  uint32_t size, pieces, waves, subs, parts;
+  uint64_t cut, back, totals, h, sums, dB, dC, bytes;
 };
 Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
-  const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups;
-  const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128, p16 = s->dim <= 32 ? 32 : 64;
+  const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups, units = share * tiles;
+  const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128;
   p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles);
   p.pieces = pieces(s->tokens, s->seqs, p.size);
-  p.chunks = pieces(s->tokens, s->seqs, kChunk);
-  // Blocks of a group share its heads where the chunks alone do not fill the card.
-  const uint64_t blocks = (uint64_t)p.chunks * s->groups;
+  // As many wavefronts to a block as its LDS has room for, whole heads each turn.
+  const uint32_t most = s->dtype == UOR_TRUNK_BF16 && s->state <= 64 ? 8 : 4;
+  p.waves = 1;
+  while (p.waves < units && p.waves < most) p.waves *= 2;
+  p.subs = (units + p.waves - 1) / p.waves;
+  // Blocks of a group share its turns where the pieces alone do not fill the card.
+  const uint64_t blocks = (uint64_t)p.pieces * s->groups;
   p.parts = blocks >= 512 ? 1 : (uint32_t)((511 + blocks) / blocks);
-  if (p.parts > share) p.parts = share;
+  if (p.parts > p.subs) p.parts = p.subs;
   uint64_t at = 0;
   const auto take = [&](uint64_t bytes) {
     const uint64_t begin = at;
@@ -456,47 +659,53 @@ Plan plan_of(const uor_trunk_scan_args *s) {
     return begin;
   };
   const bool cut = p.size < s->tokens;
-  p.cut = take(cut ? (uint64_t)p.pieces * s->heads * s->dim * s->state * 4 : 0);
+  const uint64_t starts = cut ? (uint64_t)p.pieces * s->heads * s->dim * s->state * 4 : 0;
+  p.cut = take(starts), p.back = take(starts);
   p.totals = take(cut ? (uint64_t)p.pieces * s->heads * 8 : 0);
-  const uint64_t states = (uint64_t)p.chunks * s->heads * tiles * n16 * p16 * 4;
-  p.h = take(states), p.g = take(states), p.gt = take(states);
-  p.sums = take((uint64_t)p.chunks * s->heads * 3 * 4);
-  const uint64_t rows = p.parts > 1 ? (uint64_t)p.parts * s->tokens * s->groups * s->state * 4 : 0;
+  // States are kept of chunks that have one before them and one after them in their piece.
+  p.h = take(p.size > 2 * kChunk && s->tokens > 2 * kChunk ? ((uint64_t)s->tokens / kChunk + 1) * s->heads * tiles * n16 * 32 * 4 : 0);
+  p.sums = take((uint64_t)p.pieces * s->heads * 3 * 8);
+  const uint64_t rows = p.subs > 1 ? (uint64_t)p.parts * s->tokens * s->groups * s->state * 4 : 0;
   p.dB = take(rows), p.dC = take(rows);
   p.bytes = at;
   return p;
 }
 
-template <class T, int NT, int PW>
+template <class T, int NT, int W>
 int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
   const Scan &a = k.s;
-  const dim3 block(kThreads), sweep(grid_of(a.pieces, a.heads * a.tiles));
-  const dim3 join = join_of(a, seqs);
   if (a.starts) {
-    hipLaunchKernelGGL((grad_states<T, NT, PW, false, false>), sweep, block, 0, stream, k);
-    hipLaunchKernelGGL(scan_join, join, block, 0, stream, a);
+    constexpr int E = W < 4 ? W : 4;
+    Scan s = a;
+    s.tiles = (a.dim + 31) / 32;
+    const uint32_t units = a.heads / a.groups * s.tiles;
+    const dim3 grid(grid_of(a.pieces, a.groups * ((units + E - 1) / E))), join = join_of(a, seqs);
+    hipLaunchKernelGGL((scan_ends<T, NT, 2, E, false>), grid, dim3(64 * E), 0, stream, s);
+    hipLaunchKernelGGL(scan_join, join, dim3(kThreads), 0, stream, s);
+    s.x = k.dy, s.x_stride = a.y_stride, s.x_wide = k.dy_wide;
+    s.B = a.C, s.b_stride = a.c_stride, s.b_wide = a.c_wide;
+    s.starts = k.g_starts;
+    hipLaunchKernelGGL((scan_ends<T, NT, 2, E, true>), grid, dim3(64 * E), 0, stream, s);
+    hipLaunchKernelGGL(grad_join, join, dim3(kThreads), 0, stream, k);
   }
-  hipLaunchKernelGGL((grad_states<T, NT, PW, false, true>), sweep, block, 0, stream, k);
-  if (a.starts) {
-    hipLaunchKernelGGL((grad_states<T, NT, PW, true, false>), sweep, block, 0, stream, k);
-    hipLaunchKernelGGL(grad_join, join, block, 0, stream, k);
-  }
-  hipLaunchKernelGGL((grad_states<T, NT, PW, true, true>), sweep, block, 0, stream, k);
-  hipLaunchKernelGGL((grad_rows<T, NT, PW>), dim3(grid_of(k.chunks, a.groups * k.parts)), block, 0, stream, k);
+  hipLaunchKernelGGL((grad_rows<T, NT, W>), dim3(grid_of(a.pieces, a.groups * k.parts)), dim3(64 * W), 0, stream, k);
   if (k.parts > 1 && a.rows.tokens) {
     const uint64_t n = (uint64_t)a.rows.tokens * a.groups * a.state;
     hipLaunchKernelGGL(grad_parts<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, stream, k);
   }
-  hipLaunchKernelGGL(grad_sums, dim3(a.heads), dim3(256), 0, stream, k);
+  hipLaunchKernelGGL(grad_sums, dim3(a.heads), dim3(1024), 0, stream, k);
   return launched();
 }
 template <class T, int NT>
-int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
-  return k.s.dim <= 32 ? launch<T, NT, 2>(k, seqs, stream) : launch<T, NT, 4>(k, seqs, stream);
+int launch(const Grad &k, uint32_t waves, uint32_t seqs, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && NT < 8)
+    if (waves == 8) return launch<T, NT, 8>(k, seqs, stream);
+  return waves == 1 ? launch<T, NT, 1>(k, seqs, stream) : waves == 2 ? launch<T, NT, 2>(k, seqs, stream) : launch<T, NT, 4>(k, seqs, stream);
 }
 template <class T>
-int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
-  return k.s.state <= 32 ? launch<T, 2>(k, seqs, stream) : k.s.state <= 64 ? launch<T, 4>(k, seqs, stream) : launch<T, 8>(k, seqs, stream);
+int launch(const Grad &k, uint32_t waves, uint32_t seqs, hipStream_t stream) {
+  return k.s.state <= 32 ? launch<T, 2>(k, waves, seqs, stream)
+                         : k.s.state <= 64 ? launch<T, 4>(k, waves, seqs, stream) : launch<T, 8>(k, waves, seqs, stream);
 }
 
 }  // namespace
@@ -516,22 +725,26 @@ extern "C" int uor_trunk_scan_backward_async(const uor_trunk_scan_args *s, void 
   if (!workspace || bytes < p.bytes || (uintptr_t)workspace % 16)
     return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)p.bytes);
   const uint32_t tiles = tiles_of(s->dim);
-  if (((uint64_t)p.chunks + kXcds) * s->heads * tiles > 0x7fffffffu) return fail(-1, "too many rows and heads for one call");
+  if (((uint64_t)p.pieces + kXcds) * s->heads * tiles > 0x7fffffffu) return fail(-1, "too many rows and heads for one call");
   const uint32_t size = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
   char *base = (char *)workspace;
   Grad k{};
   k.s = scan_of(s, p.size);
+  k.s.tiles = tiles;
   if (p.size < s->tokens) {
     k.s.starts = (float *)(base + p.cut);
+    k.g_starts = (float *)(base + p.back);
     k.s.totals = (double *)(base + p.totals);
   }
-  k.dy = s->dy, k.dfinal = s->dfinal, k.chunks = p.chunks, k.parts = p.parts;
-  k.h = (float *)(base + p.h), k.g = (float *)(base + p.g), k.gt = (float *)(base + p.gt), k.sums = (float *)(base + p.sums);
+  k.s.state_wide = s->state % 4 == 0 && aligned16(s->initial, 0, 4) && aligned16(s->dfinal, 0, 4) && aligned16(s->dinitial, 0, 4);
+  k.dy = s->dy, k.dfinal = s->dfinal, k.subs = p.subs, k.parts = p.parts;
+  k.h = (float *)(base + p.h), k.sums = (double *)(base + p.sums);
   k.dBparts = (float *)(base + p.dB), k.dCparts = (float *)(base + p.dC);
   k.dx = s->dx, k.ddt = s->ddt, k.dB = s->dB, k.dC = s->dC, k.dA = s->dA, k.dD = s->dD, k.dbias = s->ddt_bias, k.dinitial = s->dinitial;
-  k.dy_wide = aligned16(s->dy, s->y_stride, size) && s->dim * size % 16 == 0;
+  k.dy_wide = wide_rows(s->dy, s->y_stride, s->dim, size);
   k.dx_wide = aligned16(s->dx, 0, size) && s->dim * size % 16 == 0;
+  k.shared_wide = aligned16(s->dB, 0, size) && aligned16(s->dC, 0, size) && s->state % 8 == 0;
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(k, s->seqs, (hipStream_t)stream) : launch<float>(k, s->seqs, (hipStream_t)stream);
+  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(k, p.waves, s->seqs, (hipStream_t)stream) : launch<float>(k, p.waves, s->seqs, (hipStream_t)stream);
 }

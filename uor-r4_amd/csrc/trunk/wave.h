@@ -45,7 +45,11 @@ struct Fine<float> {
 __device__ __forceinline__ f32x4 mul(bf16x8 a, const Fine<bf16> &b, f32x4 c) {
   return Mma<bf16>::mul(a, b.hi, Mma<bf16>::mul(a, b.mid, Mma<bf16>::mul(a, b.lo, c)));
 }
+__device__ __forceinline__ f32x4 mul(const Fine<bf16> &a, bf16x8 b, f32x4 c) {
+  return Mma<bf16>::mul(a.hi, b, Mma<bf16>::mul(a.mid, b, Mma<bf16>::mul(a.lo, b, c)));
+}
 __device__ __forceinline__ f32x4 mul(f32x8 a, const Fine<float> &b, f32x4 c) { return Mma<float>::mul(a, b.v, c); }
+__device__ __forceinline__ f32x4 mul(const Fine<float> &a, f32x8 b, f32x4 c) { return Mma<float>::mul(a.v, b, c); }
 
 // A lane's number, anew: what a loop computes from it is computed again each time, and does not stand
 // in registers, of which these kernels have none to spare.
@@ -111,7 +115,7 @@ __device__ __forceinline__ float keep(float v, bool wanted) {
 // registers long before they are put down; others are read when they are.
 template <class T, int COLS, int THREADS>
 struct Load {
-  static constexpr int kN = kChunk * (COLS / 8) / THREADS, kPitch = pitch<T>(COLS);
+  static constexpr int kJobs = kChunk * (COLS / 8), kN = (kJobs + THREADS - 1) / THREADS, kPitch = pitch<T>(COLS);
   V8<T> v[kN];
   const T *at;
   uint32_t rows;
@@ -124,7 +128,7 @@ struct Load {
     const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)at, 0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kN; i++) {
-      const uint32_t job = i * THREADS + thread, col = job % (COLS / 8) * 8;
+      const uint32_t job = i * THREADS + thread, col = job % (COLS / 8) * 8;  // a job too many is a row too many
       v[i] = load_eight<T>(from, job / (COLS / 8) * pitch + col * (uint32_t)sizeof(T), col, cols);
     }
   }
@@ -135,7 +139,7 @@ struct Load {
 #pragma unroll
       for (int i = 0; i < kN; i++) {
         const uint32_t job = i * THREADS + thread;
-        *(V8<T> *)(to + job / (COLS / 8) * kPitch + job % (COLS / 8) * 8) = v[i];
+        if (kJobs % THREADS == 0 || job < kJobs) *(V8<T> *)(to + job / (COLS / 8) * kPitch + job % (COLS / 8) * 8) = v[i];
       }
       if constexpr (sizeof(T) == 2) {  // the largest exponent of all
         using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
@@ -197,6 +201,9 @@ struct Steps {
   float u[kChunk];     // e^(l_t - r_i), from the start of the row's tile i
   float v[kChunk];     // D_t e^(r_(i+1) - l_t), to its end
 };
+struct GradSteps : Steps {
+  float w[kChunk];  // e^(r_(i+1) - l_t)
+};
 struct Decay {
   float to[4];     // from a tile's end to the chunk's
   float from[4];   // from the chunk's start to a tile's
@@ -204,7 +211,8 @@ struct Decay {
   float c20, c30, c31;  // from the end of tile 0 to tile 2's start, ...
   double total;
 };
-__device__ __forceinline__ Decay steps_of(int lane, Steps &s, float raw, bool there, float A, float bias) {
+template <class S>
+__device__ __forceinline__ Decay steps_of(int lane, S &s, float raw, bool there, float A, float bias) {
   const float step = there ? softplus(raw + bias) : 0.0f;
   const double l = running_sum(there ? (double)step * (double)A * 1.4426950408889634 : 0.0);
   const double r1 = lane_of(l, 15), r2 = lane_of(l, 31), r3 = lane_of(l, 47), r4 = lane_of(l, 63);
@@ -214,7 +222,9 @@ __device__ __forceinline__ Decay steps_of(int lane, Steps &s, float raw, bool th
   s.lo[lane] = hi - hi == 0.0f ? (float)(l - (double)hi) : 0.0f;
   s.step[lane] = step;
   s.u[lane] = between(l, start);
-  s.v[lane] = step * between(end, l);
+  const float w = between(end, l);
+  s.v[lane] = step * w;
+  if constexpr (sizeof(S) > sizeof(Steps)) s.w[lane] = w;
   Decay d;
   d.to[0] = between(r4, r1), d.to[1] = between(r4, r2), d.to[2] = between(r4, r3), d.to[3] = 1.0f;
   d.from[0] = 1.0f, d.from[1] = exp2_((float)r1), d.from[2] = exp2_((float)r2), d.from[3] = exp2_((float)r3);
@@ -318,5 +328,66 @@ __device__ __forceinline__ Unit unit_of(const Scan &a, uint32_t parts) {
   u.p0 = unit % a.tiles * parts;
   return u;
 }
+
+// A piece's end state from zeros and its whole decay; a sequence's last piece needs neither. BACK: the
+// gradient at the state before a piece from that of y alone, with dy for x and C for B, along the
+// piece from its end: the sum of e^(l_t) dy_t (x) C_t.
+template <class T, int NT, int PW, int W, bool BACK>
+__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
+  constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP);
+  __shared__ __align__(16) T sB[kChunk * kNp], sXs[W][kChunk * kPp];
+  __shared__ Steps steps[W];
+  const Unit unit = unit_of<W>(a, kP);
+  Piece at;
+  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at) || (BACK ? at.first == at.start : at.end == at.stop)) return;
+  const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
+  const uint32_t head = unit.head;
+  const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + unit.group * a.state;
+  const uint32_t dim = a.dim - unit.p0 < (uint32_t)kP ? a.dim - unit.p0 : kP;
+  const float A = a.A[head], bias = a.bias ? a.bias[head] : 0.0f;
+  f32x4 h[NT][PW];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int i = 0; i < PW; i++) h[n][i] = f32x4{0, 0, 0, 0};
+  double total = 0.0;
+  Load<T, kN, 64 * W> nextB;
+  Load<T, kP, 64> nextX;
+  float raw = 0.0f;
+  const uint32_t chunks = (at.end - at.first + kChunk - 1) / kChunk;
+  const auto fetch = [&](uint32_t i) {  // the i-th chunk on the way, none past the last
+    const uint32_t first = i < chunks ? at.first + (BACK ? chunks - 1 - i : i) * kChunk : at.first;
+    const uint32_t end = i < chunks ? (at.end - first > kChunk ? first + kChunk : at.end) : first;
+    const int lane = anew(lane0), thread = wave * 64 + lane;
+    nextB.get(thread, B, a.b_stride, first, end, a.state, a.b_wide);
+    nextX.get(lane, x, a.x_stride, first, end, dim, a.x_wide);
+    raw = first + lane < end ? (float)dt[(int64_t)(first + lane) * a.dt_stride] : 0.0f;
+  };
+  fetch(0);
+  for (uint32_t i = 0; i < chunks; i++) {
+    const uint32_t first = at.first + (BACK ? chunks - 1 - i : i) * kChunk, end = at.end - first > kChunk ? first + kChunk : at.end;
+    const int lane = anew(lane0), thread = wave * 64 + lane;
+    __syncthreads();
+    nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+    nextX.put(lane, sXs[wave], a.x_stride, dim, a.x_wide);
+    const Decay d = steps_of(lane, steps[wave], raw, first + lane < end, A, bias);
+    __syncthreads();
+    fetch(i + 1);
+    if (unit.idle) continue;
+    V8<T> xs[2][PW];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int i = 0; i < PW; i++) xs[k][i] = column<T, kPp>(lane, sXs[wave], 32 * k, i);
+    advance<T, NT, PW>(lane, h, xs, sB, BACK ? steps[wave].u : steps[wave].v, BACK ? d.from : d.to, d.whole);
+    total += d.total;
+  }
+  if (unit.idle) return;
+  const uint64_t slot = (uint64_t)unit.piece * a.heads + head;
+  put_state<NT, PW>(h, a.starts + slot * a.dim * a.state + (uint64_t)unit.p0 * a.state, dim, a.state, a.state_wide);
+  if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
+}
+
+constexpr uint32_t kAhead = 8;  // pieces that a join reads before it sums them
 
 }  // namespace trunk
