@@ -100,7 +100,8 @@ struct Scan {
   Rows rows;
   uint32_t heads, groups, dim, state;
   uint32_t size, pieces;  // rows of a piece, and how many pieces the grid has
-  uint32_t tiles;         // blocks of a head: parts of dim
+  uint32_t later;         // places of pieces after a sequence's first
+  uint32_t tiles;         // a head's parts of dim
   int64_t x_stride, dt_stride, b_stride, c_stride, y_stride;
   const void *x, *dt, *B, *C;
   const float *A, *D, *bias;
@@ -109,7 +110,6 @@ struct Scan {
   float *final;
   float *starts;         // [pieces][heads][dim][state]: where a piece begins, if sequences are cut; or NULL
   double *totals;        // [pieces][heads]: log2 of a piece's whole decay
-  uint32_t part;         // values of dim of a wavefront
   bool x_wide, b_wide, c_wide, y_wide, state_wide;
 };
 
@@ -258,7 +258,23 @@ __device__ __forceinline__ void advance(f32x4 (&h)[NT * PW / 4], const Own<NT, P
 
 int check_scan(const uor_trunk_scan_args *s, bool step);
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
-dim3 join_of(const Scan &a, uint32_t seqs);
+// A join's blocks: by sequences, or by the places of later pieces, where there are fewer.
+__host__ __device__ inline uint32_t join_places(const Scan &a) { return a.rows.seqs < a.later ? a.rows.seqs : a.later; }
+// The sequence of a join's block, and how many pieces it has.
+__device__ __forceinline__ bool joined(const Scan &a, uint32_t i, uint32_t &seq, uint32_t &n) {
+  if (a.rows.seqs < a.later) {
+    uint32_t start, end;
+    a.rows.of(i, start, end);
+    seq = i, n = end > start ? (end - start - 1) / a.size + 1 : 1;
+    return n > 1;
+  }
+  uint32_t which;
+  return later_piece(a.rows, i, a.size, seq, which, n) && !which;
+}
+inline dim3 join_of(const Scan &a) {
+  const uint32_t states = join_places(a) * a.heads, most = (a.dim * a.state + kThreads - 1) / kThreads, even = 4096 / states + 1;
+  return dim3(states, most < even ? most : even);
+}
 uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units);
 // Whether rows whose heads or groups are `part` values can be read 16 bytes at a time, and a chunk of
 // them by offsets of 32 bits.

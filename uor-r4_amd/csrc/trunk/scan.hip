@@ -205,12 +205,10 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
 
 // The pieces' end states into their start states, along each sequence that has more than one.
 __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
-  const uint32_t seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  uint32_t start, end;
-  a.rows.of(seq, start, end);
-  const uint32_t n = end > start ? (end - start - 1) / a.size + 1 : 1;
-  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
-  if (n == 1) return;
+  const uint32_t head = blockIdx.x % a.heads;
+  uint32_t seq, n;
+  if (!joined(a, blockIdx.x / a.heads, seq, n)) return;
+  const uint64_t base = a.rows.at(seq) / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float h = a.initial ? a.initial[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = a.starts + (base * a.heads + head) * whole + e;
@@ -247,43 +245,29 @@ uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units) {
   return rows < tokens ? (uint32_t)rows : (tokens + kChunk) / kChunk * kChunk;
 }
 
-// A thread for each value where there are few states, fewer where most sequences will not be cut.
-dim3 join_of(const Scan &a, uint32_t seqs) {
-  const uint32_t states = seqs * a.heads, most = (a.dim * a.state + kThreads - 1) / kThreads, even = 2048 / states + 1;
-  return dim3(states, most < even ? most : even);
-}
-
 namespace {
 
 template <class T, int NT, int PW, int W>
-int launch(Scan a, uint32_t seqs, hipStream_t stream) {
-  const uint32_t units = a.heads / a.groups * a.tiles, blocks = grid_of(a.pieces, a.groups * ((units + W - 1) / W));
+int launch(const Scan &a, hipStream_t stream) {
+  const uint32_t units = a.heads / a.groups * a.tiles, blocks = a.groups * ((units + W - 1) / W);
   if (a.starts) {
-    hipLaunchKernelGGL((scan_ends<T, NT, PW, W, false>), dim3(blocks), dim3(64 * W), 0, stream, a);
-    hipLaunchKernelGGL(scan_join, join_of(a, seqs), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((scan_ends<T, NT, PW, W, false>), dim3(grid_of(a.later, blocks)), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL(scan_join, join_of(a), dim3(kThreads), 0, stream, a);
   }
-  hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(blocks), dim3(64 * W), 0, stream, a);
+  hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(grid_of(a.pieces, blocks)), dim3(64 * W), 0, stream, a);
   return launched();
 }
 template <class T, int NT, int PW>
-int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
+int launch(const Scan &a, hipStream_t stream) {
   const uint32_t units = a.heads / a.groups * a.tiles;
-  return units == 1 ? launch<T, NT, PW, 1>(a, seqs, stream) : units == 2 ? launch<T, NT, PW, 2>(a, seqs, stream) : launch<T, NT, PW, 4>(a, seqs, stream);
-}
-template <class T, int NT>
-int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2 && NT < 8)
-    if (a.part == 64) return launch<T, NT, 4>(a, seqs, stream);
-  return launch<T, NT, 2>(a, seqs, stream);
+  return units == 1 ? launch<T, NT, PW, 1>(a, stream) : units == 2 ? launch<T, NT, PW, 2>(a, stream) : launch<T, NT, PW, 4>(a, stream);
 }
 template <class T>
-int launch(const Scan &a, uint32_t seqs, hipStream_t stream) {
-  return a.state <= 32 ? launch<T, 2>(a, seqs, stream) : a.state <= 64 ? launch<T, 4>(a, seqs, stream) : launch<T, 8>(a, seqs, stream);
+int launch(const Scan &a, hipStream_t stream) {
+  return a.state <= 32 ? launch<T, 2, 2>(a, stream) : a.state <= 64 ? launch<T, 4, 2>(a, stream) : launch<T, 8, 2>(a, stream);
 }
 
-// The values of dim that a wavefront holds the state of: as many as its registers have room for.
-uint32_t part_of(const uor_trunk_scan_args *) { return 32; }
-uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + part_of(s) - 1) / part_of(s))); }
+uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32)); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
 }
@@ -315,7 +299,7 @@ Scan scan_of(const uor_trunk_scan_args *s, uint32_t size) {
   Scan a{};
   a.rows = Rows{s->offsets, s->tokens, s->seqs};
   a.heads = s->heads, a.groups = s->groups, a.dim = s->dim, a.state = s->state;
-  a.size = size, a.pieces = pieces(s->tokens, s->seqs, size), a.tiles = (s->dim + 31) / 32;
+  a.size = size, a.pieces = pieces(s->tokens, s->seqs, size), a.later = s->tokens / size + 1, a.tiles = (s->dim + 31) / 32;
   a.x_stride = s->x_stride, a.dt_stride = s->dt_stride, a.b_stride = s->b_stride, a.c_stride = s->c_stride, a.y_stride = s->y_stride;
   a.x = s->x, a.dt = s->dt, a.B = s->B, a.C = s->C, a.A = s->A, a.D = s->D, a.bias = s->dt_bias;
   a.initial = s->initial, a.y = s->y, a.final = s->final;
@@ -350,7 +334,6 @@ extern "C" int uor_trunk_scan_async(const uor_trunk_scan_args *s, void *workspac
   if (want && (!workspace || bytes < want || (uintptr_t)workspace % 16))
     return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)want);
   Scan a = scan_of(s, rows_of(s));
-  a.part = part_of(s), a.tiles = (s->dim + a.part - 1) / a.part;
   if (want) {
     a.starts = (float *)workspace;
     a.totals = (double *)((char *)workspace + starts_bytes(a.pieces, s));
@@ -358,5 +341,5 @@ extern "C" int uor_trunk_scan_async(const uor_trunk_scan_args *s, void *workspac
   if ((uint64_t)(a.pieces + kXcds) * a.heads * a.tiles > 0x7fffffffu) return fail(-1, "too many sequences and heads for one call");
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(a, s->seqs, (hipStream_t)stream) : launch<float>(a, s->seqs, (hipStream_t)stream);
+  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(a, (hipStream_t)stream) : launch<float>(a, (hipStream_t)stream);
 }

@@ -8,14 +8,15 @@
 //   dC_t = e^(l_t) h^T dy_t + sum_(s <= t) W_ts e_ts D_s B_s,
 //   g'   = e^(l_end) g + sum_t e^(l_t) dy_t (x) C_t   for the chunk before.
 //
-// The gradient at the logarithm of row u's decay is
+// With E_ts = W_ts S_ts e_ts D_s, q_t = e^(l_t) C_t . h^T dy_t and r_s = D_s e^(l_end - l_s) x_s . g B_s, the
+// gradient at the logarithm of row u's decay is
 //
-//   da_u = e^(l_end) <g, h> + sum_(s < u) r_s + sum_(t >= u) C_t . dC_t - sum_(s >= u) D_s x_s . i_s,
+//   da_u = e^(l_end) <g, h> + sum_(t >= u) q_t + sum_(s < u) r_s + sum_(t >= u, s < u) E_ts,
 //
-// with r_s = D_s x_s . (what g gives dx_s) and i_s what the chunk's own rows give it: C_t . dC_t is what
-// row t has from the state and from all rows up to it, of which those from u on are taken off again.
-// At the step itself it is x_u . (dx_u - skip dy_u) / D_u + A da_u, where what D_u divides is summed
-// without it.
+// whose last sum is taken tile by tile: rows' sums over the tiles before u's, columns' over those
+// after it, and within u's own tile its rows' running sums. (The sum over t >= u of E's row t less its
+// column t is the same, but what cancels there is many times what is left.) At the step itself the
+// gradient is (r_u + column u of E) / D_u + A da_u, where what D_u divides is summed without it.
 //
 // A block takes one group of one piece of a sequence, a wavefront one of its heads (or 32 of a head's
 // values), with g in registers. It goes along the piece once for h, and writes the states before its
@@ -56,23 +57,33 @@ __device__ __forceinline__ bf16x8 turn(bf16x8 a, bf16x8 b, bf16x8 unit) {
   const f32x4 x = Mma<bf16>::mul(a, unit, zero), y = Mma<bf16>::mul(b, unit, zero);
   return __builtin_convertvector(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), bf16x8);
 }
+__device__ __forceinline__ Mma<bf16>::Split turn(const Mma<bf16>::Split &a, const Mma<bf16>::Split &b, bf16x8 unit) {
+  return {turn(a.hi, b.hi, unit), turn(a.lo, b.lo, unit)};
+}
+__device__ __forceinline__ f32x8 turn(f32x8 a, f32x8 b, f32x8 unit) {
+  const f32x4 zero = {0, 0, 0, 0};
+  return __builtin_shufflevector(Mma<float>::mul(a, unit, zero), Mma<float>::mul(b, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7);
+}
 __device__ __forceinline__ Fine<bf16> turn(const Fine<bf16> &a, const Fine<bf16> &b, bf16x8 unit) {
   return {turn(a.hi, b.hi, unit), turn(a.mid, b.mid, unit), turn(a.lo, b.lo, unit)};
 }
-__device__ __forceinline__ Fine<float> turn(const Fine<float> &a, const Fine<float> &b, f32x8 unit) {
-  const f32x4 zero = {0, 0, 0, 0};
-  return {__builtin_shufflevector(Mma<float>::mul(a.v, unit, zero), Mma<float>::mul(b.v, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7)};
-}
+__device__ __forceinline__ Fine<float> turn(const Fine<float> &a, const Fine<float> &b, f32x8 unit) { return {turn(a.v, b.v, unit)}; }
 __device__ __forceinline__ f32x8 whole_of(const Fine<bf16> &a) {
   return __builtin_convertvector(a.hi, f32x8) + (__builtin_convertvector(a.mid, f32x8) + __builtin_convertvector(a.lo, f32x8));
 }
 __device__ __forceinline__ f32x8 whole_of(const Fine<float> &a) { return a.v; }
 
 __device__ __forceinline__ float dot(f32x8 a, f32x8 b) {
-  float v = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; e++) v = fmaf(a[e], b[e], v);
-  return v;
+  const f32x4 v = __builtin_shufflevector(a, a, 0, 1, 2, 3) * __builtin_shufflevector(b, b, 0, 1, 2, 3) +
+                  __builtin_shufflevector(a, a, 4, 5, 6, 7) * __builtin_shufflevector(b, b, 4, 5, 6, 7);
+  return (v[0] + v[1]) + (v[2] + v[3]);
+}
+// The sum of a row's 16 lanes, to all of them: from 8, 4, 2 and 1 lanes on, around the row.
+__device__ __forceinline__ float row_sum(float v) {
+  v += moved<0x128>(v);
+  v += moved<0x124>(v);
+  v += moved<0x122>(v);
+  return v + moved<0x121>(v);
 }
 // The sum of a column's four lanes.
 __device__ __forceinline__ float column_sum(float v) {
@@ -95,13 +106,16 @@ template <int NT>
 __device__ __forceinline__ void get_turned(int lane, f32x4 (&h)[NT][2], const float *at, uint32_t dim, uint32_t state) {
   const int q = lane >> 4, i16 = lane & 15;
 #pragma unroll
+  for (int n = 0; n < NT; n++) h[n][0] = h[n][1] = f32x4{0, 0, 0, 0};
+  if (!at) return;
+#pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const uint32_t p = place(i, 4 * q + r), c = place(n, i16);
-        h[n][i][r] = at && p < dim && c < state ? at[(uint64_t)p * state + c] : 0.0f;
+        h[n][i][r] = p < dim && c < state ? at[(uint64_t)p * state + c] : 0.0f;
       }
 }
 // advance, for a state that lies so.
@@ -137,7 +151,9 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sYs[W][kChunk * kPp];
   __shared__ __align__(16) float sRed[W][G * 2 * 256];
   __shared__ GradSteps steps[W];
-  __shared__ float sTurn[W][3][kChunk];  // C_t . dC_t, x_s . (what g gives dx_s), x_s . (all of dx_s)
+  // q and r / D without their decays; of E its tiles' own part of da, the rows' sums over the tiles
+  // before, the columns' over those after / D, and the columns' whole sums / D.
+  __shared__ float sSum[W][6][kChunk];
   __shared__ float sDa[W][kChunk], sDirect[W][kChunk], sDiag[W];
   const Scan &a = k.s;
   const uint32_t share = a.heads / a.groups, units = share * a.tiles;
@@ -290,22 +306,17 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
           for (int w = 0; w < 2; w++) {
             const int n = 2 * kk + w;
             const f32x8 turned = whole_of(turn(gp[0], gp[1], ones<T>(lane, w)));
-            inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
+            if (has_h) inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
             gt[n] = Mma<T>::split(turned);
           }
         }
 #pragma unroll
         for (int t = 0; t < 4; t++) {
+          const float into = column_sum(dot(widen<T>(X[t]), __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7)));
+          if (q == 0) sSum[wave][1][t * 16 + i16] = into;
           const float tail = s.w[t * 16 + i16] * d.to[t];
 #pragma unroll
           for (int i = 0; i < 2; i++) dx[t][i] *= tail;
-        }
-      }
-      if (!idle) {
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const float into = column_sum(dot(widen<T>(X[t]), __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7)));
-          if (q == 0) sTurn[wave][1][t * 16 + i16] = into;
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -342,13 +353,30 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         for (int n = 0; n < NT; n++) {
           const auto hp = Fine<T>::of(__builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-          for (int w = 0; w < 2; w++) accC[w][n] = mul(hp, y[w], accC[w][n]) * weight[w];
+          for (int w = 0; w < 2; w++) accC[w][n] = mul(hp, y[w], accC[w][n]);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const int t = (2 * pair + w) * 16 + i16;
+          float through = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < NT / 2; kk++)
+            through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
+                           __builtin_shufflevector(accC[w][2 * kk], accC[w][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+          through = column_sum(through);
+          if (q == 0) sSum[wave][0][t] = through;
+#pragma unroll
+          for (int n = 0; n < NT; n++) accC[w][n] *= weight[w];
         }
       };
+      // A lane's parts of E's columns, below and in their own tile, and of its parts on both sides of
+      // the second and of the third tile.
+      float col[4] = {0, 0, 0, 0}, own[4] = {0, 0, 0, 0}, around[2] = {0, 0};
       // The chunk's own rows: rows s of pair sp with rows t of pair tp.
       const auto rows_with = [&](int sp, int tp) {
         if (idle) return;
-        Fine<T> Z[2];
+        typename Mma<T>::Split Z[2];
+        float rows[2][4] = {};  // a lane's part of E's rows
 #pragma unroll
         for (int w = 0; w < 2; w++) {
           const int ss = 2 * sp + w, mine = ss * 16 + i16;
@@ -370,39 +398,66 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               const float c = tt == ss + 1 ? 1.0f : tt == 2 ? d.c20 : ss == 0 ? d.c30 : d.c31;
               const f32x4 e = *(const f32x4 *)(s.u + tt * 16 + 4 * q) * (c * to_end);
               M[v] = S * e;
-              z[v] = Wt * e * step;
+              z[v] = Wt * e;
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const float both = z[v][r] * S[r], e_ts = both * step;
+                col[ss] += both;
+                rows[v][r] += e_ts;
+                if (tt >= 2 && ss == 0) around[0] += e_ts;
+                if (tt == 3 && ss <= 1) around[1] += e_ts;
+              }
             } else {
               const f32x4 hi = *(const f32x4 *)(s.hi + tt * 16 + 4 * q), lo = *(const f32x4 *)(s.lo + tt * 16 + 4 * q);
+              float inside = 0.0f;
 #pragma unroll
               for (int r = 0; r < 4; r++) {
                 const int row = 4 * q + r;
-                const float e = exp2_((hi[r] - hi_s) + (lo[r] - lo_s));
+                const float e = exp2_((hi[r] - hi_s) + (lo[r] - lo_s)), at_s = keep(Wt[r], row == i16);
+                const float below = keep(Wt[r] * e, row > i16);
                 M[v][r] = keep(S[r] * e, row > i16) + keep(S[r], row == i16);
-                z[v][r] = (keep(Wt[r] * e, row > i16) + keep(Wt[r], row == i16)) * step;
-                diag += keep(Wt[r], row == i16);
+                z[v][r] = below + at_s;
+                const float both = keep(below * S[r], row > i16);
+                own[ss] += both + keep(at_s * S[r], row == i16);
+                diag += at_s;
+                inside += keep(running_sum16(moved<0x111>(both * step)), row >= i16);
               }
+              inside = column_sum(inside);
+              if (q == 0) sSum[wave][2][mine] = inside;
             }
+            z[v] *= step;
           }
-          const auto m = Fine<T>::of(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          const auto m = Mma<T>::split(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-          for (int i = 0; i < 2; i++) dx[ss][i] = mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[ss][i]);
-          Z[w] = Fine<T>::of(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          for (int i = 0; i < 2; i++) dx[ss][i] = Mma<T>::mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[ss][i]);
+          Z[w] = Mma<T>::split(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int v = 0; v < 2; v++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float sum = row_sum(rows[v][r]);
+            float *to = &sSum[wave][3][(2 * tp + v) * 16 + 4 * q + r];
+            if (i16 == 0) *to = sp == tp && tp ? *to + sum : sum;  // (0, 1) comes before (1, 1)
+          }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
 #pragma unroll
-          for (int w = 0; w < 2; w++) accB[w][n] = mul(c, Z[w], accB[w][n]);
+          for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(c, Z[w], accB[w][n]);
         }
-        Fine<T> Zt[2];
+        __builtin_amdgcn_sched_barrier(0);
+        typename Mma<T>::Split Zt[2];
 #pragma unroll
         for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
 #pragma unroll
-          for (int v = 0; v < 2; v++) accC[v][n] = mul(b, Zt[v], accC[v][n]);
+          for (int v = 0; v < 2; v++) accC[v][n] = Mma<T>::mul(b, Zt[v], accC[v][n]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       };
       // The sums over the block's wavefronts, of two tiles of rows, and out: turns after the first add
       // to what the turn before wrote, by the same threads.
@@ -448,30 +503,14 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
           __syncthreads();
         }
       };
-      const auto finish_C = [&](int pair) {
-        if (!idle) {
-#pragma unroll
-          for (int w = 0; w < 2; w++) {
-            const int t = (2 * pair + w) * 16 + i16;
-            float through = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < NT / 2; kk++)
-              through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
-                             __builtin_shufflevector(accC[w][2 * kk], accC[w][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-            through = column_sum(through);
-            if (q == 0) sTurn[wave][0][t] = through;
-          }
-        }
-        reduce(accC, pair, (T *)k.dC, k.dCparts);
-      };
       const auto finish_x = [&](int pair) {
         if (idle) return;
 #pragma unroll
         for (int w = 0; w < 2; w++) {
           const int t = 2 * pair + w, mine = t * 16 + i16;
           const f32x8 all = __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          const float direct = column_sum(dot(widen<T>(X[t]), all));
-          if (q == 0) sTurn[wave][2][mine] = direct;
+          const float below = column_sum(col[t]), at_s = column_sum(own[t]);
+          if (q == 0) sSum[wave][4][mine] = below, sSum[wave][5][mine] = below + at_s;
           if (first + mine >= end) continue;
           const f32x8 v = all * s.step[mine] + widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
           const V8<T> o = __builtin_convertvector(v, V8<T>);
@@ -488,7 +527,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
       begin_C(0);
       begin_B(0);
       rows_with(0, 0);
-      finish_C(0);
+      reduce(accC, 0, (T *)k.dC, k.dCparts);
       if (more) {
         begin_C(1);
         rows_with(0, 1);
@@ -498,7 +537,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
       if (more) {
         begin_B(1);
         rows_with(1, 1);
-        finish_C(1);
+        reduce(accC, 1, (T *)k.dC, k.dCparts);
         finish_x(1);
         reduce(accB, 1, (T *)k.dB, k.dBparts);
       }
@@ -507,12 +546,20 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
       if (!idle) {
         const bool there = first + lane < end && (more || lane < 32);
         const float step = s.step[lane];
-        const float r = there ? sTurn[wave][1][lane] * step : 0.0f, own = there ? sTurn[wave][2][lane] - sTurn[wave][1][lane] : 0.0f;
-        const double later = there ? (double)sTurn[wave][0][lane] - (double)(own * step) : 0.0;
-        const double before = running_sum((double)r), through = running_sum(later);
-        const double base = has_g ? (double)d.whole * (double)wave_sum(inner) : 0.0;
-        sDa[wave][lane] = (float)(base + (before - (double)r) + (lane_of(through, 63) - (through - later)));
-        sDirect[wave][lane] = there ? sTurn[wave][2][lane] : 0.0f;
+        const float(&sum)[6][kChunk] = sSum[wave];
+        // Their decays' errors would be common to all rows that the sums reach.
+        const double l = s.l[lane], r = there && has_g ? (double)sum[1][lane] * power64(d.total - l) : 0.0;
+        const double into = r * (double)step, before = running_sum(into);
+        const double q_t = there && has_h ? (double)sum[0][lane] * power64(l) : 0.0, through = running_sum(q_t);
+        const double base = has_g && has_h ? power64(d.total) * (double)wave_sum(inner) : 0.0;
+        const double row = there ? (double)sum[3][lane] : 0.0, rows_to = running_sum16(row);
+        const double col_s = there ? (double)(sum[4][lane] * step) : 0.0, cols_to = running_sum16(col_s);
+        const float second = wave_sum(around[0]), third = wave_sum(around[1]);
+        double inside = there ? (double)sum[2][lane] : 0.0;
+        inside += (__shfl(rows_to, lane | 15) - (rows_to - row)) + (cols_to - col_s);
+        inside += (double)(lane >> 4 == 1 ? second : lane >> 4 == 2 ? third : 0.0f);
+        sDa[wave][lane] = (float)(base + (before - into) + (lane_of(through, 63) - (through - q_t)) + inside);
+        sDirect[wave][lane] = there ? (float)r + sum[5][lane] : 0.0f;
         const float all = wave_sum(diag);
         if (lane == 0) sDiag[wave] = all;
       } else {
@@ -599,12 +646,10 @@ __global__ __launch_bounds__(1024) void grad_sums(Grad k) {
 // sequence's end.
 __global__ __launch_bounds__(kThreads) void grad_join(Grad k) {
   const Scan &a = k.s;
-  const uint32_t seq = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  uint32_t start, end;
-  a.rows.of(seq, start, end);
-  const uint32_t n = end > start ? (end - start - 1) / a.size + 1 : 1;
-  const uint64_t base = start / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
-  if (n == 1) return;
+  const uint32_t head = blockIdx.x % a.heads;
+  uint32_t seq, n;
+  if (!joined(a, blockIdx.x / a.heads, seq, n)) return;
+  const uint64_t base = a.rows.at(seq) / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float g = k.dfinal ? k.dfinal[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = k.g_starts + (base * a.heads + head) * whole + e;
@@ -672,14 +717,14 @@ Plan plan_of(const uor_trunk_scan_args *s) {
 }
 
 template <class T, int NT, int W>
-int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
+int launch(const Grad &k, hipStream_t stream) {
   const Scan &a = k.s;
   if (a.starts) {
     constexpr int E = W < 4 ? W : 4;
     Scan s = a;
     s.tiles = (a.dim + 31) / 32;
     const uint32_t units = a.heads / a.groups * s.tiles;
-    const dim3 grid(grid_of(a.pieces, a.groups * ((units + E - 1) / E))), join = join_of(a, seqs);
+    const dim3 grid(grid_of(a.later, a.groups * ((units + E - 1) / E))), join = join_of(a);
     hipLaunchKernelGGL((scan_ends<T, NT, 2, E, false>), grid, dim3(64 * E), 0, stream, s);
     hipLaunchKernelGGL(scan_join, join, dim3(kThreads), 0, stream, s);
     s.x = k.dy, s.x_stride = a.y_stride, s.x_wide = k.dy_wide;
@@ -697,15 +742,15 @@ int launch(const Grad &k, uint32_t seqs, hipStream_t stream) {
   return launched();
 }
 template <class T, int NT>
-int launch(const Grad &k, uint32_t waves, uint32_t seqs, hipStream_t stream) {
+int launch(const Grad &k, uint32_t waves, hipStream_t stream) {
   if constexpr (sizeof(T) == 2 && NT < 8)
-    if (waves == 8) return launch<T, NT, 8>(k, seqs, stream);
-  return waves == 1 ? launch<T, NT, 1>(k, seqs, stream) : waves == 2 ? launch<T, NT, 2>(k, seqs, stream) : launch<T, NT, 4>(k, seqs, stream);
+    if (waves == 8) return launch<T, NT, 8>(k, stream);
+  return waves == 1 ? launch<T, NT, 1>(k, stream) : waves == 2 ? launch<T, NT, 2>(k, stream) : launch<T, NT, 4>(k, stream);
 }
 template <class T>
-int launch(const Grad &k, uint32_t waves, uint32_t seqs, hipStream_t stream) {
-  return k.s.state <= 32 ? launch<T, 2>(k, waves, seqs, stream)
-                         : k.s.state <= 64 ? launch<T, 4>(k, waves, seqs, stream) : launch<T, 8>(k, waves, seqs, stream);
+int launch(const Grad &k, uint32_t waves, hipStream_t stream) {
+  return k.s.state <= 32 ? launch<T, 2>(k, waves, stream)
+                         : k.s.state <= 64 ? launch<T, 4>(k, waves, stream) : launch<T, 8>(k, waves, stream);
 }
 
 }  // namespace
@@ -746,5 +791,5 @@ extern "C" int uor_trunk_scan_backward_async(const uor_trunk_scan_args *s, void 
   k.shared_wide = aligned16(s->dB, 0, size) && aligned16(s->dC, 0, size) && s->state % 8 == 0;
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
-  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(k, p.waves, s->seqs, (hipStream_t)stream) : launch<float>(k, p.waves, s->seqs, (hipStream_t)stream);
+  return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(k, p.waves, (hipStream_t)stream) : launch<float>(k, p.waves, (hipStream_t)stream);
 }

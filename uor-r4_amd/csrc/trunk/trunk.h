@@ -109,6 +109,34 @@ __device__ __forceinline__ bool piece(const Rows &rows, uint32_t i, uint32_t siz
   return true;
 }
 
+// The i-th of the places that pieces after a sequence's first have, of which there are `size`-long
+// stretches of rows: sequence s has them from offsets[s] / size on. Where several sequences begin in
+// one stretch only the last can have any. `which` is the piece's number less one, `count` how many
+// pieces its sequence has.
+__device__ __forceinline__ bool later_piece(const Rows &rows, uint32_t i, uint32_t size, uint32_t &seq, uint32_t &which, uint32_t &count) {
+  uint32_t lo = 0, hi = rows.seqs;  // the last sequence that begins in the i-th stretch or before
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (rows.at(mid) / size <= i) lo = mid;
+    else hi = mid;
+  }
+  uint32_t start, stop;
+  rows.of(lo, start, stop);
+  if (start / size > i || stop == start) return false;
+  seq = lo;
+  which = i - start / size;
+  count = (stop - start - 1) / size + 1;
+  return which + 1 < count;
+}
+__device__ __forceinline__ Piece piece_of(const Rows &rows, uint32_t seq, uint32_t number, uint32_t size) {
+  Piece p;
+  rows.of(seq, p.start, p.stop);
+  p.seq = seq, p.number = number;
+  p.first = p.start + number * size;
+  p.end = p.stop - p.first > size ? p.first + size : p.stop;
+  return p;
+}
+
 // Up to eight values of a row from `col` on, zeros past `cols` or without a row.
 template <class T>
 __device__ __forceinline__ V8<T> load8(const T *row, bool there, uint32_t col, uint32_t cols, bool wide) {

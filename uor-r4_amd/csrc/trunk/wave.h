@@ -168,30 +168,48 @@ struct Load {
   }
 };
 
-// The sum over lanes 0 .. this one.
+// v of the lane that a data movement between lanes names, 0 where it names none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The sum over the lanes of its 16 up to this one, and over lanes 0 .. this one.
+template <class F>
+__device__ __forceinline__ F running_sum16(F v) {
+  v += moved<0x111>(v);  // from 1, 2, 4 and 8 lanes before
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  return v + moved<0x118>(v);
+}
 __device__ __forceinline__ double running_sum(double v) {
-#define TRUNK_STEP(CTRL, ROWS)                                                                                                 \
-  {                                                                                                                            \
-    const uint64_t bits = __builtin_bit_cast(uint64_t, v);                                                                     \
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, ROWS, 0xf, false);                           \
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CTRL, ROWS, 0xf, false);                   \
-    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                                  \
-  }
-  TRUNK_STEP(0x111, 0xf)  // from 1, 2, 4 and 8 lanes before, in each 16
-  TRUNK_STEP(0x112, 0xf)
-  TRUNK_STEP(0x114, 0xf)
-  TRUNK_STEP(0x118, 0xf)
-  TRUNK_STEP(0x142, 0xa)  // the first 16's sum to the second, the third's to the fourth
-  TRUNK_STEP(0x143, 0xc)  // the first half's to the second
-#undef TRUNK_STEP
-  return v;
+  v = running_sum16(v);
+  v += moved<0x142, 0xa>(v);         // the first 16's sum to the second, the third's to the fourth
+  return v + moved<0x143, 0xc>(v);  // the first half's to the second
 }
 __device__ __forceinline__ double lane_of(double v, int lane) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, v);
   const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ float between(double later, double before) { return exp2_((float)(later - before)); }
+// 2^v: what v's rounding to 32 bits leaves goes into the result, as these factors are common to whole
+// rows and states and their errors do not cancel in sums.
+__device__ __forceinline__ float power(double v) {
+  const float hi = (float)v, e = exp2_(hi), left = hi - hi == 0.0f ? (float)(v - (double)hi) : 0.0f;
+  return fmaf(e, left * 0.693147181f, e);
+}
+// The same with no more than the exponential's own error, for sums over many rows.
+__device__ __forceinline__ double power64(double v) {
+  const float hi = (float)v;
+  return (double)exp2_(hi) * (1.0 + (hi - hi == 0.0f ? (v - (double)hi) * 0.6931471805599453 : 0.0));
+}
+__device__ __forceinline__ float between(double later, double before) { return power(later - before); }
 
 // What a wavefront knows of its chunk's steps. The logarithms (base 2) are sums in 64 bits; l_t is
 // kept as a float and the float that is left of it, so that l_t - l_s has the error of its own size.
@@ -202,7 +220,8 @@ struct Steps {
   float v[kChunk];     // D_t e^(r_(i+1) - l_t), to its end
 };
 struct GradSteps : Steps {
-  float w[kChunk];  // e^(r_(i+1) - l_t)
+  double l[kChunk];  // the logarithms themselves
+  float w[kChunk];   // e^(r_(i+1) - l_t)
 };
 struct Decay {
   float to[4];     // from a tile's end to the chunk's
@@ -224,11 +243,11 @@ __device__ __forceinline__ Decay steps_of(int lane, S &s, float raw, bool there,
   s.u[lane] = between(l, start);
   const float w = between(end, l);
   s.v[lane] = step * w;
-  if constexpr (sizeof(S) > sizeof(Steps)) s.w[lane] = w;
+  if constexpr (sizeof(S) > sizeof(Steps)) s.w[lane] = w, s.l[lane] = l;
   Decay d;
   d.to[0] = between(r4, r1), d.to[1] = between(r4, r2), d.to[2] = between(r4, r3), d.to[3] = 1.0f;
-  d.from[0] = 1.0f, d.from[1] = exp2_((float)r1), d.from[2] = exp2_((float)r2), d.from[3] = exp2_((float)r3);
-  d.whole = exp2_((float)r4);
+  d.from[0] = 1.0f, d.from[1] = power(r1), d.from[2] = power(r2), d.from[3] = power(r3);
+  d.whole = power(r4);
   d.c20 = between(r2, r1), d.c30 = between(r3, r1), d.c31 = between(r3, r2);
   d.total = r4;
   return d;
@@ -239,13 +258,17 @@ template <int NT, int PW>
 __device__ __forceinline__ void get_state(f32x4 (&h)[NT][PW], const float *at, uint32_t dim, uint32_t state, bool wide) {
   const int lane = threadIdx.x & 63, q = lane >> 4, i16 = lane & 15;
 #pragma unroll
+  for (int i = 0; i < PW; i++)
+#pragma unroll
+    for (int n = 0; n < NT; n++) h[n][i] = f32x4{0, 0, 0, 0};
+  if (!at) return;
+#pragma unroll
   for (int i = 0; i < PW; i++) {
     const uint32_t p = place(i, i16);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const uint32_t first = place(n, 4 * q);
-      h[n][i] = f32x4{0, 0, 0, 0};
-      if (!at || p >= dim) continue;
+      if (p >= dim) continue;
       const float *from = at + (uint64_t)p * state + first;
       if (wide) {
         if (first < state) h[n][i] = *(const f32x4 *)from;
@@ -338,8 +361,10 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
   __shared__ __align__(16) T sB[kChunk * kNp], sXs[W][kChunk * kPp];
   __shared__ Steps steps[W];
   const Unit unit = unit_of<W>(a, kP);
-  Piece at;
-  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at) || (BACK ? at.first == at.start : at.end == at.stop)) return;
+  uint32_t seq, which, count;
+  if (unit.piece >= a.later || !later_piece(a.rows, unit.piece, a.size, seq, which, count)) return;
+  const Piece at = piece_of(a.rows, seq, BACK ? which + 1 : which, a.size);
+  const uint32_t number = at.start / a.size + seq + at.number;  // its place among all pieces
   const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
   const uint32_t head = unit.head;
   const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + unit.group * a.state;
@@ -383,7 +408,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
     total += d.total;
   }
   if (unit.idle) return;
-  const uint64_t slot = (uint64_t)unit.piece * a.heads + head;
+  const uint64_t slot = (uint64_t)number * a.heads + head;
   put_state<NT, PW>(h, a.starts + slot * a.dim * a.state + (uint64_t)unit.p0 * a.state, dim, a.state, a.state_wide);
   if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
 }
