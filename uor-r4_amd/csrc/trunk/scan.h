@@ -269,7 +269,7 @@ __device__ __forceinline__ bool joined(const Scan &a, uint32_t i, uint32_t &seq,
     return n > 1;
   }
   uint32_t which;
-  return later_piece(a.rows, i, a.size, seq, which, n) && !which;
+  return later_piece<true>(a.rows, i, a.size, seq, which, n) && !which;
 }
 inline dim3 join_of(const Scan &a) {
   const uint32_t states = join_places(a) * a.heads, most = (a.dim * a.state + kThreads - 1) / kThreads, even = 4096 / states + 1;

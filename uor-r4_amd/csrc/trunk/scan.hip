@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
 
   const Unit unit = unit_of<W>(a, kP);
   Piece at;
-  if (unit.piece >= a.pieces || !piece(a.rows, unit.piece, a.size, at)) return;
+  if (unit.piece >= a.pieces || !wave_piece(a.rows, unit.piece, a.size, at)) return;
   const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
   const uint32_t head = unit.head;
   const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head;

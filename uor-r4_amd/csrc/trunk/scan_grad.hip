@@ -40,7 +40,7 @@ struct Grad {
   float *dBparts, *dCparts;  // [parts][tokens][groups][state], with more than one turn
   void *dx, *ddt, *dB, *dC;
   float *dA, *dD, *dbias, *dinitial;
-  bool dy_wide, dx_wide, shared_wide;
+  bool dy_wide, dx_wide, shared_wide, mid_wide;
 };
 
 // The 32 x 16 part `which` of the unit matrix as an operand.
@@ -64,15 +64,6 @@ __device__ __forceinline__ f32x8 turn(f32x8 a, f32x8 b, f32x8 unit) {
   const f32x4 zero = {0, 0, 0, 0};
   return __builtin_shufflevector(Mma<float>::mul(a, unit, zero), Mma<float>::mul(b, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ __forceinline__ Fine<bf16> turn(const Fine<bf16> &a, const Fine<bf16> &b, bf16x8 unit) {
-  return {turn(a.hi, b.hi, unit), turn(a.mid, b.mid, unit), turn(a.lo, b.lo, unit)};
-}
-__device__ __forceinline__ Fine<float> turn(const Fine<float> &a, const Fine<float> &b, f32x8 unit) { return {turn(a.v, b.v, unit)}; }
-__device__ __forceinline__ f32x8 whole_of(const Fine<bf16> &a) {
-  return __builtin_convertvector(a.hi, f32x8) + (__builtin_convertvector(a.mid, f32x8) + __builtin_convertvector(a.lo, f32x8));
-}
-__device__ __forceinline__ f32x8 whole_of(const Fine<float> &a) { return a.v; }
-
 __device__ __forceinline__ float dot(f32x8 a, f32x8 b) {
   const f32x4 v = __builtin_shufflevector(a, a, 0, 1, 2, 3) * __builtin_shufflevector(b, b, 0, 1, 2, 3) +
                   __builtin_shufflevector(a, a, 4, 5, 6, 7) * __builtin_shufflevector(b, b, 4, 5, 6, 7);
@@ -160,7 +151,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   uint32_t number, block;
   place_of(blockIdx.x, a.groups * k.parts, number, block);
   Piece at;
-  if (number >= a.pieces || !piece(a.rows, number, a.size, at)) return;
+  if (number >= a.pieces || !wave_piece(a.rows, number, a.size, at)) return;
   const uint32_t group = block / k.parts, part = block % k.parts;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
   const T *B = (const T *)a.B + group * a.state, *C = (const T *)a.C + group * a.state;
@@ -230,6 +221,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
     f32x4 g[NT][2];
     get_state<NT, 2>(g, idle ? nullptr : finish, dim, a.state, a.state_wide);
     double sumA = 0.0, sumD = 0.0, sumBias = 0.0;
+    const bool x_wide = a.x_wide && dim;
     Load<T, kN, 64 * W> nextB, nextC;
     Load<T, kP, 64> nextY;
     float raw = 0.0f;
@@ -247,302 +239,302 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
 #pragma unroll 1
     for (uint32_t j = chunks; j-- > 0;) {
       const uint32_t first = at.first + j * kChunk, end = at.end - first > kChunk ? first + kChunk : at.end;
-      const int lane = anew(lane0), thread = wave * 64 + lane, q = lane >> 4, i16 = lane & 15;
       const bool has_h = start || j, has_g = finish || j + 1 < chunks, more = end - first > 32;
       __syncthreads();
-      nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
-      nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
-      nextY.put(lane, sY, a.y_stride, dim, k.dy_wide && dim);
       const float raw_now = raw;
-      const Decay d = steps_of(lane, s, raw, first + lane < end, A, bias);
-      V8<T> X[4];  // x's rows, as operands over dim
+      Decay d;
       {
-        const uint32_t pitch = (uint32_t)a.x_stride * sizeof(T);
-        const T *rows = x + (int64_t)first * a.x_stride;
-        const uint32_t bytes = a.x_wide && dim ? (end - first - 1) * pitch + dim * (uint32_t)sizeof(T) : 0;
-        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)rows, 0, (int)bytes, 0x00020000);
+        const int lane = anew(lane0), thread = wave * 64 + lane;
+        nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
+        nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
+        nextY.put(lane, sY, a.y_stride, dim, k.dy_wide && dim);
+        d = steps_of(lane, s, raw, first + lane < end, A, bias);
+        if (!idle && j + 1 < chunks) {
+          if (j) {
+            const float *from = kept(j) + lane * 4;
 #pragma unroll
-        for (int t = 0; t < 4; t++) X[t] = load_eight<T>(from, (t * 16 + i16) * pitch + 8 * q * (uint32_t)sizeof(T), 8 * q, dim);
-        if (!a.x_wide) {
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int t = 0; t < 4; t++)
-            X[t] = load8(rows + (int64_t)(t * 16 + i16) * a.x_stride, first + t * 16 + i16 < end, 8 * q, dim, false);
-        }
-      }
-      if (!idle && j + 1 < chunks) {
-        if (j) {
-          const float *from = kept(j) + lane * 4;
-#pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) h[n][i] = *(const f32x4 *)(from + (n * 2 + i) * 256);
-        } else {
-          get_turned<NT>(lane, h, start, dim, a.state);
+              for (int i = 0; i < 2; i++) h[n][i] = *(const f32x4 *)(from + (n * 2 + i) * 256);
+          } else {
+            get_turned<NT>(lane, h, start, dim, a.state);
+          }
         }
       }
       __syncthreads();
 
-      // dx, and g turned: what comes through the state after the chunk.
-      f32x4 dx[4][2];
-      typename Mma<T>::Split gt[NT];
-      float inner = 0.0f, diag = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 4; t++) dx[t][0] = dx[t][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int n = 0; n < NT; n++) gt[n] = Mma<T>::split(f32x8{0, 0, 0, 0, 0, 0, 0, 0});
-      if (!idle && has_g) {
-#pragma unroll
-        for (int kk = 0; kk < NT / 2; kk++) {
-          Fine<T> gp[2];
-#pragma unroll
-          for (int i = 0; i < 2; i++) gp[i] = Fine<T>::of(__builtin_shufflevector(g[2 * kk][i], g[2 * kk + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int t = 0; t < 4; t++) {
-            const V8<T> b = operand(sB + (t * 16 + i16) * kNp, 32 * kk + 8 * q);
-#pragma unroll
-            for (int i = 0; i < 2; i++) dx[t][i] = mul(gp[i], b, dx[t][i]);
-          }
+      // Rows s by pairs of tiles, and for each the rows t of the pair after and of its own: (1, 1),
+      // (0, 1), (0, 0). accB and dx are the rows s', accC the rows t's. One copy of the code serves all
+      // three, as with one each the loop would not stay in the instruction cache.
+      f32x4 accB[2][NT], accC[2][NT], dx[2][2];
+      V8<T> X[2];  // x's rows s, as operands over dim
+      // A lane's parts of E's columns below and in their own tile, and of its parts on both sides of
+      // the second and of the third tile.
+      float inner = 0.0f, diag = 0.0f, col[2], own[2], around[2] = {0, 0};
+#pragma unroll 1
+      for (int step_ = more ? 0 : 2; step_ < 3; step_++) {
+        const int sp = step_ == 0, tp = step_ < 2;
+        const int lane = anew(lane0), q = lane >> 4, i16 = lane & 15, s0 = 32 * sp + i16, t0 = 32 * tp + i16;
+        if (step_ != 2 || !more) {
+          // What comes through the state after the chunk: dx, and with g turned dB.
+          col[0] = col[1] = own[0] = own[1] = 0.0f;
 #pragma unroll
           for (int w = 0; w < 2; w++) {
-            const int n = 2 * kk + w;
-            const f32x8 turned = whole_of(turn(gp[0], gp[1], ones<T>(lane, w)));
-            if (has_h) inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
-            gt[n] = Mma<T>::split(turned);
+            dx[w][0] = dx[w][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < NT; n++) accB[w][n] = f32x4{0, 0, 0, 0};
           }
-        }
+          if (x_wide) {
+            const uint32_t pitch = (uint32_t)a.x_stride * sizeof(T), bytes = (end - first - 1) * pitch + dim * (uint32_t)sizeof(T);
+            const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(x + (int64_t)first * a.x_stride), 0, (int)bytes, 0x00020000);
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const float into = column_sum(dot(widen<T>(X[t]), __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7)));
-          if (q == 0) sSum[wave][1][t * 16 + i16] = into;
-          const float tail = s.w[t * 16 + i16] * d.to[t];
-#pragma unroll
-          for (int i = 0; i < 2; i++) dx[t][i] *= tail;
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-
-      f32x4 accB[2][NT], accC[2][NT];
-      // What comes through the states, of two tiles of rows.
-      const auto begin_B = [&](int pair) {
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const int t = 2 * pair + w;
-          const float weight = s.v[t * 16 + i16] * d.to[t];
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            accB[w][n] = f32x4{0, 0, 0, 0};
-            if (!idle && has_g) accB[w][n] = Mma<T>::mul(gt[n], X[t], accB[w][n]) * weight;
-          }
-        }
-      };
-      const auto begin_C = [&](int pair) {
-#pragma unroll
-        for (int w = 0; w < 2; w++)
-#pragma unroll
-          for (int n = 0; n < NT; n++) accC[w][n] = f32x4{0, 0, 0, 0};
-        if (idle || !has_h) return;
-        V8<T> y[2];
-        float weight[2];
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const int t = 2 * pair + w;
-          y[w] = operand(sY + (t * 16 + i16) * kPp, 8 * q);
-          weight[w] = s.u[t * 16 + i16] * d.from[t];
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const auto hp = Fine<T>::of(__builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int w = 0; w < 2; w++) accC[w][n] = mul(hp, y[w], accC[w][n]);
-        }
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const int t = (2 * pair + w) * 16 + i16;
-          float through = 0.0f;
-#pragma unroll
-          for (int kk = 0; kk < NT / 2; kk++)
-            through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
-                           __builtin_shufflevector(accC[w][2 * kk], accC[w][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-          through = column_sum(through);
-          if (q == 0) sSum[wave][0][t] = through;
-#pragma unroll
-          for (int n = 0; n < NT; n++) accC[w][n] *= weight[w];
-        }
-      };
-      // A lane's parts of E's columns, below and in their own tile, and of its parts on both sides of
-      // the second and of the third tile.
-      float col[4] = {0, 0, 0, 0}, own[4] = {0, 0, 0, 0}, around[2] = {0, 0};
-      // The chunk's own rows: rows s of pair sp with rows t of pair tp.
-      const auto rows_with = [&](int sp, int tp) {
-        if (idle) return;
-        typename Mma<T>::Split Z[2];
-        float rows[2][4] = {};  // a lane's part of E's rows
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const int ss = 2 * sp + w, mine = ss * 16 + i16;
-          const float step = s.step[mine], to_end = s.w[mine], hi_s = s.hi[mine], lo_s = s.lo[mine];
-          V8<T> b[NT / 2];
-#pragma unroll
-          for (int kk = 0; kk < NT / 2; kk++) b[kk] = operand(sB + mine * kNp, 32 * kk + 8 * q);
-          f32x4 M[2], z[2];
-#pragma unroll
-          for (int v = 0; v < 2; v++) {
-            const int tt = 2 * tp + v;
-            M[v] = z[v] = f32x4{0, 0, 0, 0};
-            if (tt < ss) continue;
-            f32x4 S = {0, 0, 0, 0};
-#pragma unroll
-            for (int kk = 0; kk < NT / 2; kk++) S = Mma<T>::mul(operand(sC + (tt * 16 + i16) * kNp, 32 * kk + 8 * q), b[kk], S);
-            const f32x4 Wt = Mma<T>::mul(operand(sY + (tt * 16 + i16) * kPp, 8 * q), X[ss], f32x4{0, 0, 0, 0});
-            if (tt > ss) {
-              const float c = tt == ss + 1 ? 1.0f : tt == 2 ? d.c20 : ss == 0 ? d.c30 : d.c31;
-              const f32x4 e = *(const f32x4 *)(s.u + tt * 16 + 4 * q) * (c * to_end);
-              M[v] = S * e;
-              z[v] = Wt * e;
-#pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const float both = z[v][r] * S[r], e_ts = both * step;
-                col[ss] += both;
-                rows[v][r] += e_ts;
-                if (tt >= 2 && ss == 0) around[0] += e_ts;
-                if (tt == 3 && ss <= 1) around[1] += e_ts;
-              }
-            } else {
-              const f32x4 hi = *(const f32x4 *)(s.hi + tt * 16 + 4 * q), lo = *(const f32x4 *)(s.lo + tt * 16 + 4 * q);
-              float inside = 0.0f;
-#pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const int row = 4 * q + r;
-                const float e = exp2_((hi[r] - hi_s) + (lo[r] - lo_s)), at_s = keep(Wt[r], row == i16);
-                const float below = keep(Wt[r] * e, row > i16);
-                M[v][r] = keep(S[r] * e, row > i16) + keep(S[r], row == i16);
-                z[v][r] = below + at_s;
-                const float both = keep(below * S[r], row > i16);
-                own[ss] += both + keep(at_s * S[r], row == i16);
-                diag += at_s;
-                inside += keep(running_sum16(moved<0x111>(both * step)), row >= i16);
-              }
-              inside = column_sum(inside);
-              if (q == 0) sSum[wave][2][mine] = inside;
+            for (int w = 0; w < 2; w++) X[w] = load_eight<T>(from, (s0 + 16 * w) * pitch + 8 * q * (uint32_t)sizeof(T), 8 * q, dim);
+          } else {
+            T *rows = (T *)sRed[wave];
+#pragma unroll 1
+            for (uint32_t e = lane; e < 32 * kP; e += 64) {
+              const uint32_t row = first + 32 * sp + e / kP, c = e % kP;
+              rows[e] = row < end && c < dim ? x[(int64_t)row * a.x_stride + c] : (T)0.0f;
             }
-            z[v] *= step;
-          }
-          const auto m = Mma<T>::split(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-          for (int i = 0; i < 2; i++) dx[ss][i] = Mma<T>::mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[ss][i]);
-          Z[w] = Mma<T>::split(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int w = 0; w < 2; w++) X[w] = operand(rows + (w * 16 + i16) * kP, 8 * q);
+          }
+          if (!idle && has_g) {
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; kk++) {
+              Fine<T> gp[2];
+#pragma unroll
+              for (int i = 0; i < 2; i++) gp[i] = Fine<T>::of(__builtin_shufflevector(g[2 * kk][i], g[2 * kk + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+              for (int w = 0; w < 2; w++) {
+                const V8<T> b = operand(sB + (s0 + 16 * w) * kNp, 32 * kk + 8 * q);
+#pragma unroll
+                for (int i = 0; i < 2; i++) dx[w][i] = mul(gp[i], b, dx[w][i]);
+              }
+#pragma unroll
+              for (int half = 0; half < 2; half++) {
+                const int n = 2 * kk + half;
+                const V8<T> unit_part = ones<T>(lane, half);
+                const f32x4 zero = {0, 0, 0, 0};  // the parts' sum is the value itself
+                const f32x8 turned = __builtin_shufflevector(mul(gp[0], unit_part, zero), mul(gp[1], unit_part, zero), 0, 1, 2, 3, 4, 5, 6, 7);
+                if (has_h && (step_ == 0 || !more)) inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
+                const auto gt = Mma<T>::split(turned);
+#pragma unroll
+                for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(gt, X[w], accB[w][n]);
+              }
+            }
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+              const float into = column_sum(dot(widen<T>(X[w]), __builtin_shufflevector(dx[w][0], dx[w][1], 0, 1, 2, 3, 4, 5, 6, 7)));
+              if (q == 0) sSum[wave][1][s0 + 16 * w] = into;
+              const float tail = s.w[s0 + 16 * w] * s.to[2 * sp + w], weight = s.v[s0 + 16 * w] * s.to[2 * sp + w];
+#pragma unroll
+              for (int i = 0; i < 2; i++) dx[w][i] *= tail;
+#pragma unroll
+              for (int n = 0; n < NT; n++) accB[w][n] *= weight;
+            }
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (step_ != 1) {
+          // What comes through the state before the chunk: dC.
 #pragma unroll
-        for (int v = 0; v < 2; v++)
+          for (int v = 0; v < 2; v++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float sum = row_sum(rows[v][r]);
-            float *to = &sSum[wave][3][(2 * tp + v) * 16 + 4 * q + r];
-            if (i16 == 0) *to = sp == tp && tp ? *to + sum : sum;  // (0, 1) comes before (1, 1)
+            for (int n = 0; n < NT; n++) accC[v][n] = f32x4{0, 0, 0, 0};
+          if (!idle && has_h) {
+            V8<T> y[2];
+#pragma unroll
+            for (int v = 0; v < 2; v++) y[v] = operand(sY + (t0 + 16 * v) * kPp, 8 * q);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              const auto hp = Fine<T>::of(__builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+              for (int v = 0; v < 2; v++) accC[v][n] = mul(hp, y[v], accC[v][n]);
+            }
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+              const int t = t0 + 16 * v;
+              float through = 0.0f;
+#pragma unroll
+              for (int kk = 0; kk < NT / 2; kk++)
+                through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
+                               __builtin_shufflevector(accC[v][2 * kk], accC[v][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+              through = column_sum(through);
+              if (q == 0) sSum[wave][0][t] = through;
+              const float weight = s.u[t] * s.from[2 * tp + v];
+#pragma unroll
+              for (int n = 0; n < NT; n++) accC[v][n] *= weight;
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (!idle) {
+          // What comes from the chunk's own rows.
+          typename Mma<T>::Split Z[2];
+          float rows[2][4] = {};  // a lane's part of E's rows, over the tiles before theirs
+#pragma unroll
+          for (int w = 0; w < 2; w++) {
+            const int mine = s0 + 16 * w;
+            const float step = s.step[mine], to_end = s.w[mine];
+            V8<T> b[NT / 2];
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; kk++) b[kk] = operand(sB + mine * kNp, 32 * kk + 8 * q);
+            f32x4 M[2], z[2];
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+              M[v] = z[v] = f32x4{0, 0, 0, 0};
+              if (v < w && sp == tp) continue;
+              f32x4 S = {0, 0, 0, 0};
+#pragma unroll
+              for (int kk = 0; kk < NT / 2; kk++) S = Mma<T>::mul(operand(sC + (t0 + 16 * v) * kNp, 32 * kk + 8 * q), b[kk], S);
+              const f32x4 Wt = Mma<T>::mul(operand(sY + (t0 + 16 * v) * kPp, 8 * q), X[w], f32x4{0, 0, 0, 0});
+              const int t4 = 32 * tp + 16 * v + 4 * q;
+              if (v > w || sp != tp) {
+                // Tiles 2 and 1 are next to each other, and so are those of one pair.
+                const float c = sp == tp || (v == 0 && w == 1) ? 1.0f : s.c[v ? 1 + w : 0];
+                const f32x4 e = *(const f32x4 *)(s.u + t4) * (c * to_end);
+                M[v] = S * e;
+                z[v] = Wt * e;
+                float all = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                  const float both = z[v][r] * S[r], e_ts = both * step;
+                  col[w] += both;
+                  rows[v][r] += e_ts;
+                  all += e_ts;
+                }
+                if (sp != tp && w == 0) around[0] += all;
+                if (sp != tp && v == 1) around[1] += all;
+              } else {
+                const float hi_s = s.hi[mine], lo_s = s.lo[mine];
+                const f32x4 hi = *(const f32x4 *)(s.hi + t4), lo = *(const f32x4 *)(s.lo + t4);
+                float inside = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                  const int row = 4 * q + r;
+                  const float e = exp2_((hi[r] - hi_s) + (lo[r] - lo_s)), at_s = keep(Wt[r], row == i16);
+                  const float below = keep(Wt[r] * e, row > i16);
+                  M[v][r] = keep(S[r] * e, row > i16) + keep(S[r], row == i16);
+                  z[v][r] = below + at_s;
+                  const float both = keep(below * S[r], row > i16);
+                  own[w] += both + keep(at_s * S[r], row == i16);
+                  diag += at_s;
+                  inside += keep(running_sum16(moved<0x111>(both * step)), row >= i16);
+                }
+                inside = column_sum(inside);
+                if (q == 0) sSum[wave][2][mine] = inside;
+              }
+              z[v] *= step;
+            }
+            const auto m = Mma<T>::split(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int i = 0; i < 2; i++) dx[w][i] = Mma<T>::mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[w][i]);
+            Z[w] = Mma<T>::split(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
+          for (int v = 0; v < 2; v++)
 #pragma unroll
-          for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(c, Z[w], accB[w][n]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        typename Mma<T>::Split Zt[2];
-#pragma unroll
-        for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
-#pragma unroll
-          for (int v = 0; v < 2; v++) accC[v][n] = Mma<T>::mul(b, Zt[v], accC[v][n]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      // The sums over the block's wavefronts, of two tiles of rows, and out: turns after the first add
-      // to what the turn before wrote, by the same threads.
-      const auto reduce = [&](const f32x4 (&acc)[2][NT], int pair, T *out, float *between) {
-#pragma unroll
-        for (int n0 = 0; n0 < NT; n0 += G) {
-#pragma unroll
-          for (int w = 0; w < 2; w++)
-#pragma unroll
-            for (int n = 0; n < G; n++) *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = acc[w][n0 + n];
-          __syncthreads();
-          for (uint32_t item = thread; item < G * 64; item += 64 * W) {
-            const uint32_t of = item & 63, w = item >> 6 & 1, n = item >> 7 << 1;
-            f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < W; i++) {
-              lo += *(const f32x4 *)(sRed[i] + ((w * G + n) * 64 + of) * 4);
-              hi += *(const f32x4 *)(sRed[i] + ((w * G + n + 1) * 64 + of) * 4);
+            for (int r = 0; r < 4; r++) {
+              const float sum = row_sum(rows[v][r]);
+              float *to = &sSum[wave][3][32 * tp + 16 * v + 4 * q + r];
+              if (i16 == 0) *to = sp == tp ? sum : *to + sum;  // (1, 1) comes before (0, 1)
             }
-            const uint32_t row = first + (2 * pair + w) * 16 + (of & 15), col = (n0 + n) * 16 + 8 * (of >> 4);
-            if (row >= end || col >= a.state) continue;
-            f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            const uint64_t to = ((uint64_t)row * a.groups + group) * a.state + col;
-            if (k.subs > 1) {
-              float *mid = between + (uint64_t)part * a.rows.tokens * a.groups * a.state + to;
 #pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (col + e < a.state) {
-                  if (sub > sub0) v[e] += mid[e];
-                  if (sub + 1 < sub1 || k.parts > 1) mid[e] = v[e];
-                }
-              if (sub + 1 < sub1 || k.parts > 1) continue;
-            }
+          for (int n = 0; n < NT; n++) {
+            const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
+#pragma unroll
+            for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(c, Z[w], accB[w][n]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          typename Mma<T>::Split Zt[2];
+#pragma unroll
+          for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
+#pragma unroll
+            for (int v = 0; v < 2; v++) accC[v][n] = Mma<T>::mul(b, Zt[v], accC[v][n]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (!idle && step_ != 1) {
+#pragma unroll
+          for (int w = 0; w < 2; w++) {
+            const int mine = s0 + 16 * w;
+            const float below = column_sum(col[w]), in = column_sum(own[w]);
+            if (q == 0) sSum[wave][4][mine] = below, sSum[wave][5][mine] = below + in;
+            if (first + mine >= end) continue;
+            const f32x8 v = __builtin_shufflevector(dx[w][0], dx[w][1], 0, 1, 2, 3, 4, 5, 6, 7) * s.step[mine] +
+                            widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
             const V8<T> o = __builtin_convertvector(v, V8<T>);
-            if (k.shared_wide) {
-              *(V8<T> *)(out + to) = o;
+            T *to = (T *)k.dx + ((uint64_t)(first + mine) * a.heads + head) * a.dim + p0 + 8 * q;
+            if (k.dx_wide) {  // whole pieces of eight values, or four of 32 bits
+              if (8 * q + 8 <= (int)dim) *(V8<T> *)to = o;
+              else if (8 * q < (int)dim) *(V4<T> *)to = __builtin_shufflevector(o, o, 0, 1, 2, 3);
             } else {
 #pragma unroll
               for (int e = 0; e < 8; e++)
-                if (col + e < a.state) out[to + e] = o[e];
+                if (8 * q + e < (int)dim) to[e] = o[e];
             }
           }
-          __syncthreads();
         }
-      };
-      const auto finish_x = [&](int pair) {
-        if (idle) return;
+
+        // dB's and dC's sums over the block's wavefronts, of two tiles of rows, and out: turns after the
+        // first add to what the turn before wrote, by the same threads.
+#pragma unroll 1
+        for (int which = step_ == 0; which < 2; which++) {  // dC after (0, 1) and (0, 0), dB after (1, 1) and (0, 0)
+          if (which && step_ == 1) break;
+          const int pair = which ? sp : tp;
+          T *out = (T *)(which ? k.dB : k.dC);
+          float *mid = (which ? k.dBparts : k.dCparts) + (uint64_t)part * a.rows.tokens * a.groups * a.state;
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const int t = 2 * pair + w, mine = t * 16 + i16;
-          const f32x8 all = __builtin_shufflevector(dx[t][0], dx[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          const float below = column_sum(col[t]), at_s = column_sum(own[t]);
-          if (q == 0) sSum[wave][4][mine] = below, sSum[wave][5][mine] = below + at_s;
-          if (first + mine >= end) continue;
-          const f32x8 v = all * s.step[mine] + widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
-          const V8<T> o = __builtin_convertvector(v, V8<T>);
-          T *to = (T *)k.dx + ((uint64_t)(first + mine) * a.heads + head) * a.dim + p0 + 8 * q;
-          if (k.dx_wide && 8 * q + 8 <= (int)dim) {
-            *(V8<T> *)to = o;
-          } else {
+          for (int n0 = 0; n0 < NT; n0 += G) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-              if (8 * q + e < (int)dim) to[e] = o[e];
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+              for (int n = 0; n < G; n++)
+                *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = which ? accB[w][n0 + n] : accC[w][n0 + n];
+            __syncthreads();
+#pragma unroll
+            for (uint32_t item = wave * 64 + lane; item < G * 128; item += 64 * W) {
+              const uint32_t of = item & 63, w = item >> 6 & 1, n = item >> 7;
+              const uint32_t row = first + (2 * pair + w) * 16 + (of & 15), c = place(n0 + n, 4 * (of >> 4));
+              const bool there = row < end && c < a.state;
+              const uint64_t to = ((uint64_t)row * a.groups + group) * a.state + c;
+              const bool adds = sub > sub0, keeps = sub + 1 < sub1 || k.parts > 1;
+              f32x4 v = {0, 0, 0, 0};
+              if (there && adds) {
+                if (k.mid_wide) {
+                  v = *(const f32x4 *)(mid + to);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 4; e++) v[e] = c + e < a.state ? mid[to + e] : 0.0f;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < W; i++) v += *(const f32x4 *)(sRed[i] + ((w * G + n) * 64 + of) * 4);
+              if (!there) continue;
+              const V4<T> o = __builtin_convertvector(v, V4<T>);
+              if (k.mid_wide && keeps) *(f32x4 *)(mid + to) = v;
+              else if (k.shared_wide && !keeps) *(V4<T> *)(out + to) = o;
+              else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  if (c + e >= a.state) break;
+                  if (keeps) mid[to + e] = v[e];
+                  else out[to + e] = o[e];
+                }
+              }
+            }
+            __syncthreads();
           }
         }
-      };
-      begin_C(0);
-      begin_B(0);
-      rows_with(0, 0);
-      reduce(accC, 0, (T *)k.dC, k.dCparts);
-      if (more) {
-        begin_C(1);
-        rows_with(0, 1);
-      }
-      finish_x(0);
-      reduce(accB, 0, (T *)k.dB, k.dBparts);
-      if (more) {
-        begin_B(1);
-        rows_with(1, 1);
-        reduce(accC, 1, (T *)k.dC, k.dCparts);
-        finish_x(1);
-        reduce(accB, 1, (T *)k.dB, k.dBparts);
       }
 
       // A row a lane: the gradients at its decay and its step, of all the head's wavefronts.
+      const int lane = anew(lane0);
       if (!idle) {
         const bool there = first + lane < end && (more || lane < 32);
         const float step = s.step[lane];
@@ -619,16 +611,18 @@ __global__ __launch_bounds__(256) void grad_parts(Grad k) {
   ((T *)k.dC)[at] = (T)c;
 }
 
-// The pieces' sums of the parameters' gradients, a block a head. Places of pieces that no sequence has
-// hold nothing, and are left out.
+// The pieces' sums of the parameters' gradients, a block a head.
 __global__ __launch_bounds__(1024) void grad_sums(Grad k) {
   __shared__ double part[3][1024];
   const uint32_t head = blockIdx.x;
   double v[3] = {0.0, 0.0, 0.0};
-  for (uint32_t c = threadIdx.x; c < k.s.pieces; c += 1024) {
-    Piece at;
-    if (!piece(k.s.rows, c, k.s.size, at)) continue;
-    for (int i = 0; i < 3; i++) v[i] += k.sums[((uint64_t)c * k.s.heads + head) * 3 + i];
+  for (uint32_t seq = threadIdx.x; seq < k.s.rows.seqs; seq += 1024) {
+    uint32_t start, stop;
+    k.s.rows.of(seq, start, stop);
+    const uint32_t n = stop > start ? (stop - start - 1) / k.s.size + 1 : 1;
+    const double *from = k.sums + ((uint64_t)(start / k.s.size + seq) * k.s.heads + head) * 3;
+    for (uint32_t j = 0; j < n; j++)
+      for (int i = 0; i < 3; i++) v[i] += from[(uint64_t)j * k.s.heads * 3 + i];
   }
   for (int i = 0; i < 3; i++) part[i][threadIdx.x] = v[i];
   for (int m = 512; m; m >>= 1) {
@@ -788,7 +782,8 @@ extern "C" int uor_trunk_scan_backward_async(const uor_trunk_scan_args *s, void 
   k.dx = s->dx, k.ddt = s->ddt, k.dB = s->dB, k.dC = s->dC, k.dA = s->dA, k.dD = s->dD, k.dbias = s->ddt_bias, k.dinitial = s->dinitial;
   k.dy_wide = wide_rows(s->dy, s->y_stride, s->dim, size);
   k.dx_wide = aligned16(s->dx, 0, size) && s->dim * size % 16 == 0;
-  k.shared_wide = aligned16(s->dB, 0, size) && aligned16(s->dC, 0, size) && s->state % 8 == 0;
+  k.shared_wide = aligned16(s->dB, 0, size) && aligned16(s->dC, 0, size) && s->state % 4 == 0;
+  k.mid_wide = s->state % 4 == 0;
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
   return s->dtype == UOR_TRUNK_BF16 ? launch<bf16>(k, p.waves, (hipStream_t)stream) : launch<float>(k, p.waves, (hipStream_t)stream);

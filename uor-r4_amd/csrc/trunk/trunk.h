@@ -90,13 +90,28 @@ struct Piece {
   uint32_t start, stop;  // its sequence's rows
 };
 __host__ __device__ __forceinline__ uint32_t pieces(uint32_t tokens, uint32_t seqs, uint32_t size) { return tokens / size + seqs; }
-__device__ __forceinline__ bool piece(const Rows &rows, uint32_t i, uint32_t size, Piece &p) {
-  uint32_t lo = 0, hi = rows.seqs;  // the last sequence whose pieces begin at or before i
+// The last sequence that begins at or before some place, the first if none does. WAVE: the lanes of a
+// wavefront ask for the same, and look at 64 sequences at a time: what each look waits for is a read.
+template <bool WAVE, class F>
+__device__ __forceinline__ uint32_t last_before(uint32_t seqs, F begins_before) {
+  uint32_t lo = 0, hi = seqs;
   while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (rows.at(mid) / size + mid <= i) lo = mid;
-    else hi = mid;
+    if constexpr (WAVE) {
+      const uint32_t step = (hi - lo + 63) / 64, mid = lo + (threadIdx.x & 63) * step;
+      const uint64_t ahead = __ballot(mid < hi && begins_before(mid));
+      lo += ahead ? (63 - __builtin_clzll(ahead)) * step : 0;
+      hi = hi - lo > step ? lo + step : hi;
+    } else {
+      const uint32_t mid = (lo + hi) / 2;
+      if (begins_before(mid)) lo = mid;
+      else hi = mid;
+    }
   }
+  return lo;
+}
+template <bool WAVE = false>
+__device__ __forceinline__ bool piece(const Rows &rows, uint32_t i, uint32_t size, Piece &p) {
+  const uint32_t lo = last_before<WAVE>(rows.seqs, [&](uint32_t s) { return rows.at(s) / size + s <= i; });
   const uint32_t base = rows.at(lo) / size + lo;
   if (base > i) return false;  // only where the offsets do not ascend
   rows.of(lo, p.start, p.stop);
@@ -109,17 +124,16 @@ __device__ __forceinline__ bool piece(const Rows &rows, uint32_t i, uint32_t siz
   return true;
 }
 
+__device__ __forceinline__ bool wave_piece(const Rows &rows, uint32_t i, uint32_t size, Piece &p) { return piece<true>(rows, i, size, p); }
+
 // The i-th of the places that pieces after a sequence's first have, of which there are `size`-long
 // stretches of rows: sequence s has them from offsets[s] / size on. Where several sequences begin in
 // one stretch only the last can have any. `which` is the piece's number less one, `count` how many
 // pieces its sequence has.
+template <bool WAVE>
 __device__ __forceinline__ bool later_piece(const Rows &rows, uint32_t i, uint32_t size, uint32_t &seq, uint32_t &which, uint32_t &count) {
-  uint32_t lo = 0, hi = rows.seqs;  // the last sequence that begins in the i-th stretch or before
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (rows.at(mid) / size <= i) lo = mid;
-    else hi = mid;
-  }
+  // The last sequence that begins in the i-th stretch or before.
+  const uint32_t lo = last_before<WAVE>(rows.seqs, [&](uint32_t s) { return rows.at(s) / size <= i; });
   uint32_t start, stop;
   rows.of(lo, start, stop);
   if (start / size > i || stop == start) return false;

@@ -221,6 +221,7 @@ struct Steps {
 };
 struct GradSteps : Steps {
   double l[kChunk];  // the logarithms themselves
+  float to[4], from[4], c[3];  // as Decay's, for code that does not know which tiles it takes
   float w[kChunk];   // e^(r_(i+1) - l_t)
 };
 struct Decay {
@@ -250,6 +251,13 @@ __device__ __forceinline__ Decay steps_of(int lane, S &s, float raw, bool there,
   d.whole = power(r4);
   d.c20 = between(r2, r1), d.c30 = between(r3, r1), d.c31 = between(r3, r2);
   d.total = r4;
+  if constexpr (sizeof(S) > sizeof(Steps)) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) s.to[i] = d.to[i], s.from[i] = d.from[i];
+      s.c[0] = d.c20, s.c[1] = d.c30, s.c[2] = d.c31;
+    }
+  }
   return d;
 }
 
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
   __shared__ Steps steps[W];
   const Unit unit = unit_of<W>(a, kP);
   uint32_t seq, which, count;
-  if (unit.piece >= a.later || !later_piece(a.rows, unit.piece, a.size, seq, which, count)) return;
+  if (unit.piece >= a.later || !later_piece<true>(a.rows, unit.piece, a.size, seq, which, count)) return;
   const Piece at = piece_of(a.rows, seq, BACK ? which + 1 : which, a.size);
   const uint32_t number = at.start / a.size + seq + at.number;  // its place among all pieces
   const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
