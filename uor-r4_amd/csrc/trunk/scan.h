@@ -275,7 +275,7 @@ inline dim3 join_of(const Scan &a) {
   const uint32_t states = join_places(a) * a.heads, most = (a.dim * a.state + kThreads - 1) / kThreads, even = 4096 / states + 1;
   return dim3(states, most < even ? most : even);
 }
-uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units);
+uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units, uint32_t least);
 // Whether rows whose heads or groups are `part` values can be read 16 bytes at a time, and a chunk of
 // them by offsets of 32 bits.
 inline bool wide_rows(const void *p, int64_t stride, uint32_t part, uint32_t bytes) {

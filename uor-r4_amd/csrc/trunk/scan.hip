@@ -235,12 +235,12 @@ __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
 }
 
 // How many rows a piece has: sequences are cut where they alone would leave the card idle. The grid
-// then has about 4,096 wavefronts, two for each place; pieces under 256 rows cost more to join than
-// they gain. Where there are sequences for every place only those are cut that would still run when
-// the others have long ended.
-uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units) {
+// then has about 4,096 wavefronts, two for each place; pieces under `least` rows cost more to join
+// than they gain. Where there are sequences for every place only those are cut that would still run
+// when the others have long ended.
+uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units, uint32_t least) {
   const uint64_t even = ((uint64_t)tokens * units + 4095) / 4096, want = (uint64_t)seqs * units < 2048 ? even : 4 * even;
-  const uint64_t size = (want < 256 ? 256 : want) + kChunk - 1;
+  const uint64_t size = (want < least ? least : want) + kChunk - 1;
   const uint64_t rows = size / kChunk * kChunk;
   return rows < tokens ? (uint32_t)rows : (tokens + kChunk) / kChunk * kChunk;
 }
@@ -267,7 +267,7 @@ int launch(const Scan &a, hipStream_t stream) {
   return a.state <= 32 ? launch<T, 2, 2>(a, stream) : a.state <= 64 ? launch<T, 4, 2>(a, stream) : launch<T, 8, 2>(a, stream);
 }
 
-uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32)); }
+uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32), 256); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
 }

@@ -132,13 +132,20 @@ __device__ __forceinline__ void advance_turned(int lane, f32x4 (&h)[NT][2], cons
   }
 }
 
+// What a loop computes from these values is computed again each time (see anew).
+template <int NT>
+__device__ __forceinline__ void hold(f32x4 (&h)[NT][2]) {
+#pragma unroll
+  for (int n = 0; n < NT; n++) asm volatile("" : "+v"(h[n][0]), "+v"(h[n][1]));
+}
+
 // Wavefronts that a SIMD is to hold: with states of more than 64 a wavefront needs all its registers.
 template <int NT, int W>
 constexpr int kHeld = NT > 4 || W == 1 ? 1 : 2;
 
 template <class T, int NT, int W>
 __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
-  constexpr int kN = 16 * NT, kP = 32, kNp = pitch<T>(kN), kPp = pitch<T>(kP), G = NT < 4 ? NT : 4;
+  constexpr int kN = 16 * NT, kP = 32, kNp = pitch<T>(kN), kPp = pitch<T>(kP), G = 2;
   __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sYs[W][kChunk * kPp];
   __shared__ __align__(16) float sRed[W][G * 2 * 256];
   __shared__ GradSteps steps[W];
@@ -300,6 +307,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             for (int w = 0; w < 2; w++) X[w] = operand(rows + (w * 16 + i16) * kP, 8 * q);
           }
           if (!idle && has_g) {
+            hold(g);
 #pragma unroll
             for (int kk = 0; kk < NT / 2; kk++) {
               Fine<T> gp[2];
@@ -322,6 +330,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
 #pragma unroll
                 for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(gt, X[w], accB[w][n]);
               }
+              __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int w = 0; w < 2; w++) {
@@ -343,6 +352,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
 #pragma unroll
             for (int n = 0; n < NT; n++) accC[v][n] = f32x4{0, 0, 0, 0};
           if (!idle && has_h) {
+            hold(h);
             V8<T> y[2];
 #pragma unroll
             for (int v = 0; v < 2; v++) y[v] = operand(sY + (t0 + 16 * v) * kPp, 8 * q);
@@ -495,7 +505,8 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             for (int w = 0; w < 2; w++)
 #pragma unroll
               for (int n = 0; n < G; n++)
-                *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = which ? accB[w][n0 + n] : accC[w][n0 + n];
+                if (which) *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = accB[w][n0 + n];
+                else *(f32x4 *)(sRed[wave] + ((w * G + n) * 64 + lane) * 4) = accC[w][n0 + n];
             __syncthreads();
 #pragma unroll
             for (uint32_t item = wave * 64 + lane; item < G * 128; item += 64 * W) {
@@ -680,10 +691,10 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
   const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups, units = share * tiles;
   const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128;
-  p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles);
+  p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles, 128);
   p.pieces = pieces(s->tokens, s->seqs, p.size);
   // As many wavefronts to a block as its LDS has room for, whole heads each turn.
-  const uint32_t most = s->dtype == UOR_TRUNK_BF16 && s->state <= 64 ? 8 : 4;
+  const uint32_t most = 4;
   p.waves = 1;
   while (p.waves < units && p.waves < most) p.waves *= 2;
   p.subs = (units + p.waves - 1) / p.waves;
@@ -737,8 +748,6 @@ int launch(const Grad &k, hipStream_t stream) {
 }
 template <class T, int NT>
 int launch(const Grad &k, uint32_t waves, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2 && NT < 8)
-    if (waves == 8) return launch<T, NT, 8>(k, stream);
   return waves == 1 ? launch<T, NT, 1>(k, stream) : waves == 2 ? launch<T, NT, 2>(k, stream) : launch<T, NT, 4>(k, stream);
 }
 template <class T>
