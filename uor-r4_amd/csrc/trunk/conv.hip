@@ -12,7 +12,7 @@ namespace trunk {
 // Rows of a thread's run: the rows before it are read twice, and a gradient computes those after it
 // twice. Shorter runs fill the card sooner.
 constexpr uint32_t kRun = 16, kGradRun = 32;
-constexpr int kBatch = 4;  // rows that are read together
+constexpr int kBatch = 4, kRowBatch = 8;  // rows that are read together, in a gradient and without
 constexpr uint32_t kGradThreads = 512;
 
 struct Conv {
@@ -122,33 +122,33 @@ __device__ __forceinline__ Some<E> silu(Some<E> v) {
 }
 
 template <class T, int TAPS, bool WIDE>
-__global__ __launch_bounds__(256, 4) void conv_rows(Conv a) {
+__global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
   constexpr int E = 8, kPast = TAPS - 1;
   Lane l;
   Piece at;
   if (!lane_of<E, 256>(a, l) || l.run >= a.pieces || !piece(a.rows, l.run, kRun, at)) return;
   const uint32_t c = l.c;
-  Some<E> w[TAPS], bias, rows[kPast + kBatch];
+  Some<E> w[TAPS], bias, rows[kPast + kRowBatch];
   taps_of<TAPS, E>(a, c, w, bias);
   rows_before<T, TAPS, WIDE, E>(a, at, c, rows);
   uint32_t left = 0;  // rows of the last batch
-  for (uint32_t first = at.first; first < at.end; first += kBatch) {
-    left = min(at.end - first, (uint32_t)kBatch);
+  for (uint32_t first = at.first; first < at.end; first += kRowBatch) {
+    left = min(at.end - first, (uint32_t)kRowBatch);
     const T *x = (const T *)a.x + (int64_t)first * a.x_stride;
 #pragma unroll
-    for (int k = 0; k < kBatch; k++) {
+    for (int k = 0; k < kRowBatch; k++) {
       rows[kPast + k] = row_some<T, WIDE, E>(x, 0, c, a.channels);
       x += first + k + 1 < at.end ? a.x_stride : 0;  // rows past the last are read as the last
     }
 #pragma unroll
-    for (int k = 0; k < kBatch; k++) {
+    for (int k = 0; k < kRowBatch; k++) {
       Some<E> v = weighted<TAPS, E>(rows + k, w, bias);
       if (a.silu) v = silu<E>(v);
       if (k < (int)left) store_some<T, WIDE, E>((T *)a.y + (first + k) * a.y_stride, c, a.channels, v);
     }
-    if (first + kBatch < at.end) {
+    if (first + kRowBatch < at.end) {
 #pragma unroll
-      for (int k = 0; k < kPast; k++) rows[k] = rows[kBatch + k];
+      for (int k = 0; k < kPast; k++) rows[k] = rows[kRowBatch + k];
     }
   }
   if (a.final && at.end == at.stop) {
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 4) void conv_rows(Conv a) {
     for (int k = 0; k < kPast; k++) {
       Some<E> v = rows[k];
 #pragma unroll
-      for (int n = 1; n <= kBatch; n++) v = left == (uint32_t)n ? rows[k + n] : v;
+      for (int n = 1; n <= kRowBatch; n++) v = left == (uint32_t)n ? rows[k + n] : v;
       store_some<T, WIDE, E>((T *)a.final + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
     }
   }

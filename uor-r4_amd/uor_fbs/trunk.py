@@ -92,6 +92,7 @@ class NormGrads(NamedTuple):
 
 
 _lib = None
+_calls = {}  # name: (the call, its workspace's size or None)
 
 
 def lib():
@@ -109,81 +110,100 @@ def lib():
                 raise TrunkError(f"{LIB_PATH} is of another version: build it again")
             forms = {"scan": ("", "_backward", "_step"), "conv": ("", "_backward", "_step"), "norms": ("", "_backward")}[name]
             for form in forms:
-                call = getattr(L, f"uor_trunk_{name}{form}_async")
+                call, bytes_of = getattr(L, f"uor_trunk_{name}{form}_async"), None
                 needs = form == "_backward" or (name == "scan" and form == "")
                 call.argtypes = [C.POINTER(struct)] + ([P, C.c_uint64] if needs else []) + [P]
                 if needs:
-                    f = getattr(L, f"uor_trunk_{name}{form}_workspace_bytes")
-                    f.argtypes, f.restype = [C.POINTER(struct)], C.c_uint64
+                    bytes_of = getattr(L, f"uor_trunk_{name}{form}_workspace_bytes")
+                    bytes_of.argtypes, bytes_of.restype = [C.POINTER(struct)], C.c_uint64
+                _calls[name + form] = call, bytes_of
         _lib = L
     return _lib
 
 
-def _call(name, args, device, workspace=False):
-    L = lib()
-    extra, keep = (), None
-    if workspace:
-        n = getattr(L, f"uor_trunk_{name}_workspace_bytes")(C.byref(args))
-        keep = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        extra = (None if keep is None else keep.data_ptr(), n)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    code = getattr(L, f"uor_trunk_{name}_async")(C.byref(args), *extra, stream)
+def _call(name, args, index):
+    """The library's call on the current stream of device `index`."""
+    L = _lib or lib()
+    call, bytes_of = _calls[name]
+    args.device, ref, stream = index, C.byref(args), torch._C._cuda_getCurrentRawStream(index)
+    if bytes_of is None:
+        code = call(ref, stream)
+    else:
+        n = bytes_of(ref)
+        keep = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", index)) if n else None
+        code = call(ref, None if keep is None else keep.data_ptr(), n, stream)
     if code:
         raise TrunkError(f"uor_trunk_{name} status {code}: {L.uor_trunk_last_error().decode()}")
 
 
-def _want(ok, text):
+def _want(ok, text, *values):
     if not ok:
-        raise TrunkError(text)
+        raise TrunkError(text.format(*values))
 
 
-def _rows(name, t, dtype, *shape):
-    """t with dense inner axes, and the values between its rows (None: None, 0)."""
+def _check(name, t, dtype, shape):
+    _want(isinstance(t, torch.Tensor), "{} is no tensor", name)
+    _want(t.dtype == dtype, "{} is {}, not {}", name, t.dtype, dtype)
+    _want(t.shape == shape, "{} has shape {}, not {}", name, tuple(t.shape), shape)
+
+
+def _rows(name, t, dtype, shape, inner):
+    """t with dense inner axes of `inner` values, and the values between its rows (None: None, 0)."""
     if t is None:
         return None, 0
-    _want(isinstance(t, torch.Tensor), f"{name} is no tensor")
-    _want(t.dtype == dtype, f"{name} is {t.dtype}, not {dtype}")
-    _want(tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    inner, dense = 1, True
+    _check(name, t, dtype, shape)
+    if t.is_contiguous():
+        return t, inner
+    size_so_far = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        dense = dense and (size == 1 or stride == inner)
-        inner *= size
-    if t.shape[0] <= 1:
-        return (t if dense else t.contiguous()), inner
-    if not dense or t.stride(0) < inner:
-        t = t.contiguous()
-    return t, t.stride(0)
+        if size != 1 and stride != size_so_far:
+            return t.contiguous(), inner
+        size_so_far *= size
+    if t.shape[0] > 1 and t.stride(0) < inner:
+        return t.contiguous(), inner
+    return t, (t.stride(0) if t.shape[0] > 1 else inner)
 
 
-def _dense(name, t, dtype, *shape):
-    t, _ = _rows(name, t, dtype, *shape)
-    return None if t is None else t.contiguous()
+def _dense(name, t, dtype, shape):
+    if t is None:
+        return None
+    _check(name, t, dtype, shape)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _one_device(*tensors):
-    """The tensors' device: one HIP device for all of them."""
-    devices = {t.device for t in tensors if t is not None}
-    _want(len(devices) == 1, f"the tensors are on different devices: {sorted(map(str, devices))}")
-    device = devices.pop()
-    _want(device.type == "cuda", f"the tensors are on {device}: a HIP device is wanted")
-    return device
+    """The index of the tensors' device: one HIP device for all of them."""
+    index = None
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()
+            if index is None:
+                index = at
+            elif at != index:
+                raise TrunkError("the tensors are on different devices: {}".format(sorted({str(t.device) for t in tensors if t is not None})))
+    _want(index is not None and index >= 0, "the tensors are on cpu: a HIP device is wanted")
+    return index
 
 
 def _offsets(offsets, tokens):
     if offsets is None:
         return None, 1
     _want(offsets.dim() == 1 and offsets.numel() >= 2, "offsets has one place more than there are sequences, two at least")
-    _want(offsets.dtype in (torch.int32, torch.int64), f"offsets is {offsets.dtype}, not int32")
-    return offsets.int().contiguous(), offsets.numel() - 1
+    return _int32("offsets", offsets), offsets.numel() - 1
+
+
+def _int32(name, t):
+    _want(t.dtype in (torch.int32, torch.int64), "{} is {}, not int32", name, t.dtype)
+    t = t if t.dtype == torch.int32 else t.int()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _index(slots, rows, states):
     if slots is None:
-        _want(states >= rows, f"{rows} rows for {states} states")
+        _want(states >= rows, "{} rows for {} states", rows, states)
         return None
-    _want(slots.dtype in (torch.int32, torch.int64), f"slots is {slots.dtype}, not int32")
-    _want(tuple(slots.shape) == (rows,), f"slots has shape {tuple(slots.shape)}, not {(rows,)}")
-    return slots.int().contiguous()
+    _want(slots.shape == (rows,), "slots has shape {}, not {}", tuple(slots.shape), (rows,))
+    return _int32("slots", slots)
 
 
 _NOTHING = 16  # the address of a tensor of no values: it is there, and nothing of it is read
@@ -194,8 +214,13 @@ def _ptr(t):
 
 
 def _dtype(t, name):
-    _want(isinstance(t, torch.Tensor) and t.dtype in DTYPES, f"{name} is no tensor of bfloat16 or float32")
+    _want(isinstance(t, torch.Tensor) and t.dtype in DTYPES, "{} is no tensor of bfloat16 or float32", name)
     return t.dtype
+
+
+def _make(like):
+    """A dense tensor of the same type, shape and device (None: None)."""
+    return None if like is None else torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -207,23 +232,21 @@ def _scan_args(x, dt, A, B, Cm, D, dt_bias, offsets, initial, step=False):
     _want(x.dim() == 3, "x has the axes row, head and value")
     _want(isinstance(B, torch.Tensor) and B.dim() == 3, "B has the axes row, group and state")
     tokens, heads, dim = x.shape
-    groups, state = B.shape[1:]
-    _want(groups >= 1 and heads >= 1 and heads % groups == 0, f"{heads} heads are not whole groups of {groups}")
-    _want(1 <= dim <= MAX_DIM and 1 <= state <= MAX_STATE, f"dim {dim} or state {state} outside 1..128")
+    _, groups, state = B.shape
+    _want(groups >= 1 and heads >= 1 and heads % groups == 0, "{} heads are not whole groups of {}", heads, groups)
+    _want(1 <= dim <= MAX_DIM and 1 <= state <= MAX_STATE, "dim {} or state {} outside 1..128", dim, state)
     off, seqs = (None, tokens) if step else _offsets(offsets, tokens)
-    x, xs = _rows("x", x, dtype, tokens, heads, dim)
-    dt, ds = _rows("dt", dt, dtype, tokens, heads)
-    B, bs = _rows("B", B, dtype, tokens, groups, state)
-    Cm, cs = _rows("C", Cm, dtype, tokens, groups, state)
+    x, xs = _rows("x", x, dtype, (tokens, heads, dim), heads * dim)
+    dt, ds = _rows("dt", dt, dtype, (tokens, heads), heads)
+    B, bs = _rows("B", B, dtype, (tokens, groups, state), groups * state)
+    Cm, cs = _rows("C", Cm, dtype, (tokens, groups, state), groups * state)
     f32 = torch.float32
     _want(A is not None, "A is no tensor")
-    A, D, dt_bias = _dense("A", A, f32, heads), _dense("D", D, f32, heads), _dense("dt_bias", dt_bias, f32, heads)
-    initial = _dense("initial", initial, f32, seqs, heads, dim, state)
-    keep = (x, dt, A, B, Cm, D, dt_bias, off, initial)
-    a = CScan(dtype=DTYPES[dtype], tokens=tokens, seqs=seqs, heads=heads, groups=groups, dim=dim, state=state,
-              x_stride=xs, dt_stride=ds, b_stride=bs, c_stride=cs, y_stride=heads * dim, x=_ptr(x), dt=_ptr(dt), B=_ptr(B),
-              C=_ptr(Cm), A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias), offsets=_ptr(off), initial=_ptr(initial))
-    return a, keep
+    A, D, dt_bias = _dense("A", A, f32, (heads,)), _dense("D", D, f32, (heads,)), _dense("dt_bias", dt_bias, f32, (heads,))
+    initial = _dense("initial", initial, f32, (seqs, heads, dim, state))
+    a = CScan(0, DTYPES[dtype], tokens, seqs, heads, groups, dim, state, 0, 0, xs, ds, bs, cs, heads * dim, _ptr(x), _ptr(dt),
+              _ptr(B), _ptr(Cm), _ptr(A), _ptr(D), _ptr(dt_bias), _ptr(off), _ptr(initial))
+    return a, (x, dt, A, B, Cm, D, dt_bias, off, initial)
 
 
 def scan(x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, initial=None):
@@ -231,11 +254,10 @@ def scan(x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, initial=None):
     groups, state), the skip D and the steps' bias (heads), from the states ``initial`` (sequences,
     heads, dim, state; zeros without). ``final`` are the states after each sequence's last row."""
     a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, offsets, initial)
-    device = _one_device(*keep)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    final = torch.empty((a.seqs, a.heads, a.dim, a.state), dtype=torch.float32, device=device)
-    a.device, a.y, a.final = device.index, _ptr(y), _ptr(final)
-    _call("scan", a, device, workspace=True)
+    index = _one_device(*keep)
+    y, final = _make(x), torch.empty((a.seqs, a.heads, a.dim, a.state), dtype=torch.float32, device=x.device)
+    a.y, a.final = _ptr(y), _ptr(final)
+    _call("scan", a, index)
     return y, final
 
 
@@ -243,16 +265,14 @@ def scan_backward(dy, x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, ini
     """The gradients of ``scan`` at its inputs from those of its outputs; ``dfinal`` None: zeros.
     dD, ddt_bias and dinitial are None where the input is."""
     a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, offsets, initial)
-    dy, a.y_stride = _rows("dy", dy, x.dtype, *x.shape)
     _want(dy is not None, "dy is no tensor")
-    f32 = torch.float32
-    dfinal = _dense("dfinal", dfinal, f32, a.seqs, a.heads, a.dim, a.state)
-    device = _one_device(dy, dfinal, *keep)
-    make = lambda like, dtype=None: None if like is None else torch.empty(like.shape, dtype=dtype or like.dtype, device=device)  # noqa: E731
-    got = ScanGrads(make(x), make(dt), make(A), make(B), make(C), make(D), make(dt_bias), make(initial))
-    a.device, a.dy, a.dfinal = device.index, _ptr(dy), _ptr(dfinal)
+    dy, a.y_stride = _rows("dy", dy, x.dtype, x.shape, a.heads * a.dim)
+    dfinal = _dense("dfinal", dfinal, torch.float32, (a.seqs, a.heads, a.dim, a.state))
+    index = _one_device(dy, dfinal, *keep)
+    got = ScanGrads(*map(_make, (x, dt, A, B, C, D, dt_bias, initial)))
+    a.dy, a.dfinal = _ptr(dy), _ptr(dfinal)
     a.dx, a.ddt, a.dA, a.dB, a.dC, a.dD, a.ddt_bias, a.dinitial = map(_ptr, got)
-    _call("scan_backward", a, device, workspace=True)
+    _call("scan_backward", a, index)
     return got
 
 
@@ -261,14 +281,14 @@ def scan_step(x, dt, A, B, C, states, *, slots=None, D=None, dt_bias=None):
     updated in place; ``slots`` (int32) says which state each row has, no two alike. A row whose slot
     is outside the states is skipped and its y is 0."""
     a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, None, None, step=True)
-    _want(isinstance(states, torch.Tensor) and states.dtype == torch.float32 and states.is_contiguous()
-          and tuple(states.shape[1:]) == (a.heads, a.dim, a.state) and states.dim() == 4,
-          f"states is no dense float32 tensor of (slots, {a.heads}, {a.dim}, {a.state})")
-    index = _index(slots, a.tokens, states.shape[0])
-    device = _one_device(states, index, *keep)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    a.device, a.y, a.index, a.states, a.slots = device.index, _ptr(y), _ptr(index), _ptr(states), states.shape[0]
-    _call("scan_step", a, device)
+    inner = (a.heads, a.dim, a.state)
+    _want(isinstance(states, torch.Tensor) and states.dtype == torch.float32 and states.dim() == 4 and states.shape[1:] == inner
+          and states.is_contiguous(), "states is no dense float32 tensor of (slots, {}, {}, {})", *inner)
+    slots = _index(slots, a.tokens, states.shape[0])
+    index = _one_device(states, slots, *keep)
+    y = _make(x)
+    a.y, a.index, a.states, a.slots = _ptr(y), _ptr(slots), _ptr(states), states.shape[0]
+    _call("scan_step", a, index)
     return y
 
 
@@ -282,14 +302,14 @@ def _conv_args(x, weight, bias, offsets, initial, silu, step=False):
     _want(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight has the axes channel and tap")
     tokens, channels = x.shape
     taps = weight.shape[1]
-    _want(channels >= 1 and 1 <= taps <= MAX_TAPS, f"{taps} taps outside 1..{MAX_TAPS}, or no channels")
+    _want(channels >= 1 and 1 <= taps <= MAX_TAPS, "{} taps outside 1..{}, or no channels", taps, MAX_TAPS)
     off, seqs = (None, tokens) if step else _offsets(offsets, tokens)
-    x, xs = _rows("x", x, dtype, tokens, channels)
-    weight = _dense("weight", weight, torch.float32, channels, taps)
-    bias = _dense("bias", bias, torch.float32, channels)
-    initial = _dense("initial", initial, dtype, seqs, taps - 1, channels)
-    a = CConv(dtype=DTYPES[dtype], tokens=tokens, seqs=seqs, channels=channels, taps=taps, silu=int(bool(silu)), x_stride=xs,
-              y_stride=channels, x=_ptr(x), weight=_ptr(weight), bias=_ptr(bias), offsets=_ptr(off), initial=_ptr(initial))
+    x, xs = _rows("x", x, dtype, (tokens, channels), channels)
+    weight = _dense("weight", weight, torch.float32, (channels, taps))
+    bias = _dense("bias", bias, torch.float32, (channels,))
+    initial = _dense("initial", initial, dtype, (seqs, taps - 1, channels))
+    a = CConv(0, DTYPES[dtype], tokens, seqs, channels, taps, 0, 1 if silu else 0, xs, channels, _ptr(x), _ptr(weight), _ptr(bias),
+              _ptr(off), _ptr(initial))
     return a, (x, weight, bias, off, initial)
 
 
@@ -298,26 +318,24 @@ def conv(x, weight, bias=None, *, offsets=None, initial=None, silu=True):
     rows of x (rows, channels), the rows before it from ``initial`` (sequences, taps - 1, channels;
     zeros without). ``final`` are each sequence's last taps - 1 rows, the next call's ``initial``."""
     a, keep = _conv_args(x, weight, bias, offsets, initial, silu)
-    device = _one_device(*keep)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    final = torch.empty((a.seqs, a.taps - 1, a.channels), dtype=x.dtype, device=device)
-    a.device, a.y, a.final = device.index, _ptr(y), _ptr(final)
-    _call("conv", a, device)
+    index = _one_device(*keep)
+    y, final = _make(x), torch.empty((a.seqs, a.taps - 1, a.channels), dtype=x.dtype, device=x.device)
+    a.y, a.final = _ptr(y), _ptr(final)
+    _call("conv", a, index)
     return y, final
 
 
 def conv_backward(dy, x, weight, bias=None, *, offsets=None, initial=None, dfinal=None, silu=True):
     """The gradients of ``conv`` at its inputs; dbias and dinitial are None where the input is."""
     a, keep = _conv_args(x, weight, bias, offsets, initial, silu)
-    dy, a.y_stride = _rows("dy", dy, x.dtype, *x.shape)
     _want(dy is not None, "dy is no tensor")
-    dfinal = _dense("dfinal", dfinal, x.dtype, a.seqs, a.taps - 1, a.channels)
-    device = _one_device(dy, dfinal, *keep)
-    make = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=device)  # noqa: E731
-    got = ConvGrads(make(x), make(weight), make(bias), make(initial))
-    a.device, a.dy, a.dfinal = device.index, _ptr(dy), _ptr(dfinal)
-    a.dx, a.dweight, a.dbias, a.dinitial = (_ptr(t) for t in got)
-    _call("conv_backward", a, device, workspace=True)
+    dy, a.y_stride = _rows("dy", dy, x.dtype, x.shape, a.channels)
+    dfinal = _dense("dfinal", dfinal, x.dtype, (a.seqs, a.taps - 1, a.channels))
+    index = _one_device(dy, dfinal, *keep)
+    got = ConvGrads(*map(_make, (x, weight, bias, initial)))
+    a.dy, a.dfinal = _ptr(dy), _ptr(dfinal)
+    a.dx, a.dweight, a.dbias, a.dinitial = map(_ptr, got)
+    _call("conv_backward", a, index)
     return got
 
 
@@ -325,14 +343,14 @@ def conv_step(x, weight, states, bias=None, *, slots=None, silu=True):
     """y (rows, channels): one token a session; ``states`` (slots, taps - 1, channels) of x's type is
     updated in place, ``slots`` as in ``scan_step``."""
     a, keep = _conv_args(x, weight, bias, None, None, silu, step=True)
-    _want(isinstance(states, torch.Tensor) and states.dtype == x.dtype and states.is_contiguous() and states.dim() == 3
-          and tuple(states.shape[1:]) == (a.taps - 1, a.channels),
-          f"states is no dense {x.dtype} tensor of (slots, {a.taps - 1}, {a.channels})")
-    index = _index(slots, a.tokens, states.shape[0])
-    device = _one_device(states, index, *keep)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    a.device, a.y, a.index, a.states, a.slots = device.index, _ptr(y), _ptr(index), _ptr(states), states.shape[0]
-    _call("conv_step", a, device)
+    inner = (a.taps - 1, a.channels)
+    _want(isinstance(states, torch.Tensor) and states.dtype == x.dtype and states.dim() == 3 and states.shape[1:] == inner
+          and states.is_contiguous(), "states is no dense {} tensor of (slots, {}, {})", x.dtype, *inner)
+    slots = _index(slots, a.tokens, states.shape[0])
+    index = _one_device(states, slots, *keep)
+    y = _make(x)
+    a.y, a.index, a.states, a.slots = _ptr(y), _ptr(slots), _ptr(states), states.shape[0]
+    _call("conv_step", a, index)
     return y
 
 
@@ -346,16 +364,16 @@ def _norms_args(residual, out, gate, post, scale, pre, eps):
     _want(first.dim() == 2, "rows have the axes row and value")
     _want(out is not None or (gate is None and post is None and scale is None), "a gate, post or scale without a block's output")
     _want(out is not None or pre is not None, "nothing to compute: neither a block's output nor pre")
-    rows, width = first.shape
-    _want(1 <= width <= MAX_WIDTH, f"width {width} outside 1..{MAX_WIDTH}")
+    rows, width = shape = first.shape
+    _want(1 <= width <= MAX_WIDTH, "width {} outside 1..{}", width, MAX_WIDTH)
     _want(eps >= 0, "eps is negative")
-    residual, rs = _rows("residual", residual, dtype, rows, width)
-    out, os_ = _rows("out", out, dtype, rows, width)
-    gate, gs = _rows("gate", gate, dtype, rows, width)
-    post, scale, pre = (_dense(n, t, torch.float32, width) for n, t in (("post", post), ("scale", scale), ("pre", pre)))
-    a = CNorms(dtype=DTYPES[dtype], rows=rows, width=width, eps=eps, residual_stride=rs, out_stride=os_, gate_stride=gs,
-               residual=_ptr(residual), out=_ptr(out), gate=_ptr(gate), post=_ptr(post), scale=_ptr(scale), pre=_ptr(pre))
-    return a, dtype, (residual, out, gate, post, scale, pre)
+    residual, rs = _rows("residual", residual, dtype, shape, width)
+    out, os_ = _rows("out", out, dtype, shape, width)
+    gate, gs = _rows("gate", gate, dtype, shape, width)
+    post, scale, pre = (_dense(n, t, torch.float32, (width,)) for n, t in (("post", post), ("scale", scale), ("pre", pre)))
+    a = CNorms(0, DTYPES[dtype], rows, width, eps, 0, rs, os_, gs, _ptr(residual), _ptr(out), _ptr(gate), _ptr(post), _ptr(scale),
+               _ptr(pre))
+    return a, first, (residual, out, gate, post, scale, pre)
 
 
 def norms(residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps=1e-6):
@@ -363,28 +381,26 @@ def norms(residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps
     rms(v) post, normed = rms(residual') pre, with rows of (rows, width). Without ``out`` the residual
     is only normed (residual' is the residual itself); without ``residual`` residual' is the normed
     block alone; without ``pre`` normed is None. ``gate``, ``post`` and ``scale`` are 1 without."""
-    a, dtype, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
-    device = _one_device(*keep)
-    make = lambda: torch.empty((a.rows, a.width), dtype=dtype, device=device)  # noqa: E731
-    residual_out = residual if out is None else make()
-    normed = None if pre is None else make()
-    a.device, a.normed = device.index, _ptr(normed)
+    a, first, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
+    index = _one_device(*keep)
+    residual_out = residual if out is None else _make(first)
+    normed = None if pre is None else _make(first)
+    a.normed = _ptr(normed)
     a.residual_out = None if out is None else _ptr(residual_out)
-    _call("norms", a, device)
+    _call("norms", a, index)
     return residual_out, normed
 
 
 def norms_backward(dresidual_out, dnormed, residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps=1e-6):
     """The gradients of ``norms`` at its inputs, None where there is none; either of the outputs'
     gradients may be None for zeros."""
-    a, dtype, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
+    a, first, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
     _want(dnormed is None or pre is not None, "dnormed without pre")
-    dresidual_out = _dense("dresidual_out", dresidual_out, dtype, a.rows, a.width)
-    dnormed = _dense("dnormed", dnormed, dtype, a.rows, a.width)
-    device = _one_device(dresidual_out, dnormed, *keep)
-    make = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=device)  # noqa: E731
-    got = NormGrads(*map(make, (residual, out, gate, post, scale, pre)))
-    a.device, a.dresidual_out, a.dnormed = device.index, _ptr(dresidual_out), _ptr(dnormed)
+    dresidual_out = _dense("dresidual_out", dresidual_out, first.dtype, first.shape)
+    dnormed = _dense("dnormed", dnormed, first.dtype, first.shape)
+    index = _one_device(dresidual_out, dnormed, *keep)
+    got = NormGrads(*map(_make, (residual, out, gate, post, scale, pre)))
+    a.dresidual_out, a.dnormed = _ptr(dresidual_out), _ptr(dnormed)
     a.dresidual, a.dout, a.dgate, a.dpost, a.dscale, a.dpre = map(_ptr, got)
-    _call("norms_backward", a, device, workspace=True)
+    _call("norms_backward", a, index)
     return got
