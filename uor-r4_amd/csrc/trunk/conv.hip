@@ -40,24 +40,19 @@ template <int E>
 using Some = __attribute__((ext_vector_type(E))) float;
 
 template <class T, bool WIDE, int E>
-__device__ __forceinline__ void store_some(T *row, uint32_t col, uint32_t cols, Some<E> v) {
+__device__ __forceinline__ void put_some(T *row, uint32_t col, uint32_t cols, Some<E> v) {
   const Raw<T, E> o = __builtin_convertvector(v, Raw<T, E>);
   if constexpr (WIDE) {
     *(Raw<T, E> *)(row + col) = o;
   } else {
-#pragma unroll
-    for (int e = 0; e < E; e++)
-      if (col + e < cols) row[col + e] = o[e];
+    store_some<T, E>(row, col, cols, o);
   }
 }
 template <class T, bool WIDE, int E>
 __device__ __forceinline__ Raw<T, E> raw_some(const void *base, int64_t at, uint32_t col, uint32_t cols) {
   const T *row = (const T *)base + at;
   if constexpr (WIDE) return *(const Raw<T, E> *)(row + col);
-  Raw<T, E> v;
-#pragma unroll
-  for (int e = 0; e < E; e++) v[e] = col + e < cols ? row[col + e] : (T)0.0f;
-  return v;
+  else return load_some<T, E>(row, true, col, cols);
 }
 template <class T, bool WIDE, int E>
 __device__ __forceinline__ Some<E> row_some(const void *base, int64_t at, uint32_t col, uint32_t cols) {
@@ -144,7 +139,7 @@ __global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
     for (int k = 0; k < kRowBatch; k++) {
       Some<E> v = weighted<TAPS, E>(rows + k, w, bias);
       if (a.silu) v = silu<E>(v);
-      if (k < (int)left) store_some<T, WIDE, E>((T *)a.y + (first + k) * a.y_stride, c, a.channels, v);
+      if (k < (int)left) put_some<T, WIDE, E>((T *)a.y + (first + k) * a.y_stride, c, a.channels, v);
     }
     if (first + kRowBatch < at.end) {
 #pragma unroll
@@ -157,7 +152,7 @@ __global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
       Some<E> v = rows[k];
 #pragma unroll
       for (int n = 1; n <= kRowBatch; n++) v = left == (uint32_t)n ? rows[k + n] : v;
-      store_some<T, WIDE, E>((T *)a.final + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
+      put_some<T, WIDE, E>((T *)a.final + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
     }
   }
 }
@@ -243,11 +238,11 @@ __global__ __launch_bounds__(kGradThreads, 3) void conv_grad_rows(Conv a) {
             if (a.dfinal && back >= 0) v += row_some<T, WIDE, E>(a.dfinal, ((int64_t)at.seq * kPast + back) * a.channels, c, a.channels);
             if (row < (int64_t)at.start) {
               const int64_t k = row - at.start + kPast;
-              if (a.dinitial) store_some<T, WIDE, E>((T *)a.dinitial + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
+              if (a.dinitial) put_some<T, WIDE, E>((T *)a.dinitial + ((int64_t)at.seq * kPast + k) * a.channels, c, a.channels, v);
               continue;
             }
           }
-          store_some<T, WIDE, E>((T *)a.dx + row * a.channels, c, a.channels, v);
+          put_some<T, WIDE, E>((T *)a.dx + row * a.channels, c, a.channels, v);
         }
 #pragma unroll
         for (int k = 0; k < kPast; k++) rows[k] = rows[kBatch + k], d[k] = d[kBatch + k];
@@ -298,7 +293,7 @@ __global__ __launch_bounds__(256) void conv_step(Conv a) {
   const int64_t slot = a.index ? a.index[row] : (int64_t)row;
   T *y = (T *)a.y + row * a.y_stride;
   if (slot < 0 || slot >= a.slots) {
-    store_some<T, WIDE, E>(y, c, a.channels, Some<E>(0.0f));
+    put_some<T, WIDE, E>(y, c, a.channels, Some<E>(0.0f));
     return;
   }
   Some<E> w[TAPS], bias, rows[TAPS];
@@ -309,9 +304,9 @@ __global__ __launch_bounds__(256) void conv_step(Conv a) {
   taps_of<TAPS, E>(a, c, w, bias);
   Some<E> v = weighted<TAPS, E>(rows, w, bias);
   if (a.silu) v = silu<E>(v);
-  store_some<T, WIDE, E>(y, c, a.channels, v);
+  put_some<T, WIDE, E>(y, c, a.channels, v);
 #pragma unroll
-  for (int k = 0; k < TAPS - 1; k++) store_some<T, WIDE, E>(state + k * a.channels, c, a.channels, rows[k + 1]);
+  for (int k = 0; k < TAPS - 1; k++) put_some<T, WIDE, E>(state + k * a.channels, c, a.channels, rows[k + 1]);
 }
 
 namespace {
@@ -346,15 +341,14 @@ bool wide_of(const uor_trunk_conv_args *s) {
   return wide(s->x, s->x_stride) && wide(s->y, s->y_stride) && wide(s->dy, s->y_stride) && wide(s->initial, 0) && wide(s->final, 0) &&
          wide(s->states, 0) && wide(s->dfinal, 0) && wide(s->dinitial, 0) && wide(s->dx, 0);
 }
-// The blocks of `runs` runs, and of a gradient: two for each compute unit, each line with four runs
-// at least where there are so many.
+// The blocks of `runs` runs, and of a gradient: three for each compute unit at most.
 uint32_t blocks_of(uint32_t runs, uint32_t channels) {
   const uint32_t lines = lines_of<8, 256>(channels);
   return (runs + lines - 1) / lines * parts_of<8, 256>(channels);
 }
 uint32_t grad_blocks_of(uint32_t runs, uint32_t channels) {
   const uint32_t lines = lines_of<4, kGradThreads>(channels), parts = parts_of<4, kGradThreads>(channels);
-  const uint32_t few = (runs + 4 * lines - 1) / (4 * lines), most = (768 + parts - 1) / parts;
+  const uint32_t few = (runs + lines - 1) / lines, most = (768 + parts - 1) / parts;
   return few < 1 ? 1 : few < most ? few : most;
 }
 template <template <class, int, bool> class F, class T, bool WIDE, class... V>

@@ -20,7 +20,6 @@ struct Norms {
   const void *dresidual_out, *dnormed;
   void *dresidual, *dout, *dgate;
   float *parts;  // [workers][3][width]: a block's sums of dpost, dscale, dpre
-  bool residual_wide, out_wide, gate_wide, wide;  // wide: the dense rows
 };
 
 // The sum over a row's lanes, to all of them; `scratch` where a row has more than a wavefront.
@@ -48,20 +47,12 @@ __device__ __forceinline__ f32x8 param8(const float *p, uint32_t col, uint32_t c
   return v;
 }
 template <class T>
-__device__ __forceinline__ f32x8 values(const void *base, int64_t at, bool there, uint32_t col, uint32_t cols, bool wide) {
-  return __builtin_convertvector(load8((const T *)base + at, there && base, col, cols, wide), f32x8);
+__device__ __forceinline__ f32x8 values(const void *base, int64_t at, bool there, uint32_t col, uint32_t cols) {
+  return __builtin_convertvector((load_some<T, 8>((const T *)base + at, there && base, col, cols)), f32x8);
 }
 template <class T>
-__device__ __forceinline__ void put(void *base, int64_t at, uint32_t col, uint32_t cols, bool wide, f32x8 v) {
-  T *row = (T *)base + at;
-  const V8<T> o = __builtin_convertvector(v, V8<T>);
-  if (wide && col + 8 <= cols) {
-    *(V8<T> *)(row + col) = o;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; e++)
-    if (col + e < cols) row[col + e] = o[e];
+__device__ __forceinline__ void put(void *base, int64_t at, uint32_t col, uint32_t cols, f32x8 v) {
+  store_some<T, 8>((T *)base + at, col, cols, __builtin_convertvector(v, V8<T>));
 }
 
 // Threads of a block: rows of up to a wavefront share 256, longer ones have a block.
@@ -86,10 +77,10 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_rows(Norms a) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const uint32_t c = (i * LANES + lane) * 8;
-      r[i] = values<T>(a.residual, row * a.residual_stride, there, c, a.width, a.residual_wide);
-      v[i] = values<T>(a.out, row * a.out_stride, there, c, a.width, a.out_wide);
+      r[i] = values<T>(a.residual, row * a.residual_stride, there, c, a.width);
+      v[i] = values<T>(a.out, row * a.out_stride, there, c, a.width);
       if (a.gate) {
-        const f32x8 z = values<T>(a.gate, row * a.gate_stride, there, c, a.width, a.gate_wide);
+        const f32x8 z = values<T>(a.gate, row * a.gate_stride, there, c, a.width);
 #pragma unroll
         for (int e = 0; e < 8; e++) v[i][e] *= z[e] * sigmoid(z[e]);
       }
@@ -103,7 +94,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_rows(Norms a) {
       for (int i = 0; i < V; i++) {
         const uint32_t c = (i * LANES + lane) * 8;
         r[i] += scale[i] * (v[i] * inverse * post[i]);
-        if (there) put<T>(a.residual_out, row * a.width, c, a.width, a.wide, r[i]);
+        if (there) put<T>(a.residual_out, row * a.width, c, a.width, r[i]);
       }
     }
     if (a.pre) {
@@ -114,7 +105,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_rows(Norms a) {
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const uint32_t c = (i * LANES + lane) * 8;
-        if (there) put<T>(a.normed, row * a.width, c, a.width, a.wide, r[i] * inverse * pre[i]);
+        if (there) put<T>(a.normed, row * a.width, c, a.width, r[i] * inverse * pre[i]);
       }
     }
   }
@@ -145,10 +136,10 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const uint32_t c = (i * LANES + lane) * 8;
-      r[i] = values<T>(a.residual, row * a.residual_stride, there, c, a.width, a.residual_wide);
-      u[i] = values<T>(a.out, row * a.out_stride, there, c, a.width, a.out_wide);
-      z[i] = values<T>(a.gate, row * a.gate_stride, there, c, a.width, a.gate_wide);
-      d[i] = values<T>(a.dresidual_out, row * a.width, there, c, a.width, a.wide);
+      r[i] = values<T>(a.residual, row * a.residual_stride, there, c, a.width);
+      u[i] = values<T>(a.out, row * a.out_stride, there, c, a.width);
+      z[i] = values<T>(a.gate, row * a.gate_stride, there, c, a.width);
+      d[i] = values<T>(a.dresidual_out, row * a.width, there, c, a.width);
       v[i] = u[i];
       if (a.gate) {
 #pragma unroll
@@ -169,7 +160,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const uint32_t c = (i * LANES + lane) * 8;
-        e[i] = values<T>(a.dnormed, row * a.width, there, c, a.width, a.wide);
+        e[i] = values<T>(a.dnormed, row * a.width, there, c, a.width);
         sum += total(r[i] * r[i]);
         with += total(e[i] * pre[i] * r[i]);
       }
@@ -184,7 +175,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const uint32_t c = (i * LANES + lane) * 8;
-      if (there && a.dresidual) put<T>(a.dresidual, row * a.width, c, a.width, a.wide, d[i]);
+      if (there && a.dresidual) put<T>(a.dresidual, row * a.width, c, a.width, d[i]);
     }
     if (!a.out) continue;
     float with = 0.0f;
@@ -211,9 +202,9 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
           dz[e] = dv[e] * u[i][e] * s * (1.0f + z[i][e] * (1.0f - s));
           dv[e] *= z[i][e] * s;
         }
-        if (there) put<T>(a.dgate, row * a.width, c, a.width, a.wide, dz);
+        if (there) put<T>(a.dgate, row * a.width, c, a.width, dz);
       }
-      if (there) put<T>(a.dout, row * a.width, c, a.width, a.wide, dv);
+      if (there) put<T>(a.dout, row * a.width, c, a.width, dv);
     }
   }
   // The sums of the block's rows side by side, in the order of its lanes.
@@ -298,19 +289,12 @@ int check_norms(const uor_trunk_norms_args *s) {
   return 0;
 }
 Norms norms_of(const uor_trunk_norms_args *s) {
-  const uint32_t bytes = s->dtype == UOR_TRUNK_BF16 ? 2 : 4;
   Norms a{};
   a.rows = s->rows, a.width = s->width, a.eps = s->eps, a.share = 1.0f / (float)s->width;
   a.residual_stride = s->residual_stride, a.out_stride = s->out_stride, a.gate_stride = s->gate_stride;
   a.residual = s->residual, a.out = s->out, a.gate = s->gate, a.post = s->post, a.scale = s->scale, a.pre = s->pre;
   a.residual_out = s->residual_out, a.normed = s->normed, a.dresidual_out = s->dresidual_out, a.dnormed = s->dnormed;
   a.dresidual = s->dresidual, a.dout = s->dout, a.dgate = s->dgate;
-  a.residual_wide = aligned16(s->residual, s->residual_stride, bytes), a.out_wide = aligned16(s->out, s->out_stride, bytes);
-  a.gate_wide = aligned16(s->gate, s->gate_stride, bytes);
-  a.wide = true;
-  for (const void *p : {(const void *)s->residual_out, (const void *)s->normed, s->dresidual_out, s->dnormed,
-                        (const void *)s->dresidual, (const void *)s->dout, (const void *)s->dgate})
-    a.wide = a.wide && aligned16(p, s->width, bytes);
   return a;
 }
 

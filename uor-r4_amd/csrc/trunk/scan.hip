@@ -267,7 +267,7 @@ int launch(const Scan &a, hipStream_t stream) {
   return a.state <= 32 ? launch<T, 2, 2>(a, stream) : a.state <= 64 ? launch<T, 4, 2>(a, stream) : launch<T, 8, 2>(a, stream);
 }
 
-uint32_t rows_of(const uor_trunk_scan_args *s) { return piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32), 512); }
+uint32_t rows_of(const uor_trunk_scan_args *s) { return s->tokens <= 512 ? 512 + kChunk : piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32), 128); }
 uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
   return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
 }

@@ -299,9 +299,9 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
           } else {
             T *rows = (T *)sRed[wave];
 #pragma unroll 1
-            for (uint32_t e = lane; e < 32 * kP; e += 64) {
-              const uint32_t row = first + 32 * sp + e / kP, c = e % kP;
-              rows[e] = row < end && c < dim ? x[(int64_t)row * a.x_stride + c] : (T)0.0f;
+            for (uint32_t e = lane * 8; e < 32 * kP; e += 512) {
+              const uint32_t row = first + 32 * sp + e / kP;
+              *(V8<T> *)(rows + e) = load_some<T, 8>(x + (int64_t)row * a.x_stride, row < end, e % kP, dim);
             }
 #pragma unroll
             for (int w = 0; w < 2; w++) X[w] = operand(rows + (w * 16 + i16) * kP, 8 * q);
@@ -691,7 +691,7 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
   const uint32_t tiles = tiles_of(s->dim), share = s->heads / s->groups, units = share * tiles;
   const uint64_t n16 = s->state <= 32 ? 32 : s->state <= 64 ? 64 : 128;
-  p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles, 128);
+  p.size = piece_rows(s->tokens, s->seqs, s->heads * tiles, 64);
   p.pieces = pieces(s->tokens, s->seqs, p.size);
   // As many wavefronts to a block as its LDS has room for, whole heads each turn.
   const uint32_t most = 4;

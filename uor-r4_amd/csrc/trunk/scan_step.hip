@@ -47,9 +47,7 @@ __global__ __launch_bounds__(256) void scan_step(Step a) {
     if (a.wide) {
       if (n < a.state) h = *(const f32x4 *)at;
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (n + e < a.state) h[e] = at[e];
+      h = load_some<float, 4>(at - n, true, n, a.state);
     }
     const float v = (float)x[p], in = step * v;
     float sum = 0.0f;
@@ -61,9 +59,7 @@ __global__ __launch_bounds__(256) void scan_step(Step a) {
     if (a.wide) {
       if (n < a.state) *(f32x4 *)at = h;
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (n + e < a.state) at[e] = h[e];
+      store_some<float, 4>(at - n, n, a.state, h);
     }
 #pragma unroll
     for (int k = 1; k < LN; k <<= 1) sum += __shfl_xor(sum, k);

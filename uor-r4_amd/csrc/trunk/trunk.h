@@ -151,18 +151,43 @@ __device__ __forceinline__ Piece piece_of(const Rows &rows, uint32_t seq, uint32
   return p;
 }
 
-// Up to eight values of a row from `col` on, zeros past `cols` or without a row.
-template <class T>
-__device__ __forceinline__ V8<T> load8(const T *row, bool there, uint32_t col, uint32_t cols, bool wide) {
-  V8<T> v;
+// N values next to each other, of which no more is known than that each is aligned: memory is read and
+// written 16 bytes at a time at any address.
+template <class T, int N>
+struct Loose {
+  using Values = __attribute__((ext_vector_type(N))) T;
+  typedef Values At __attribute__((aligned(sizeof(T))));
+};
+template <class T, int N>
+__device__ __forceinline__ typename Loose<T, N>::Values loose(const T *at) {
+  return *(const typename Loose<T, N>::At *)at;
+}
+template <class T, int N>
+__device__ __forceinline__ void loose(T *at, typename Loose<T, N>::Values v) {
+  *(typename Loose<T, N>::At *)at = v;
+}
+// N values of a row from `col` on, zeros past `cols` or without a row.
+template <class T, int N>
+__device__ __forceinline__ typename Loose<T, N>::Values load_some(const T *row, bool there, uint32_t col, uint32_t cols) {
+  typename Loose<T, N>::Values v;
 #pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = (T)0.0f;
+  for (int e = 0; e < N; e++) v[e] = (T)0.0f;
   if (!there || col >= cols) return v;
-  if (wide && col + 8 <= cols) return *(const V8<T> *)(row + col);
+  if (col + N <= cols) return loose<T, N>(row + col);
 #pragma unroll
-  for (int e = 0; e < 8; e++)
+  for (int e = 0; e < N; e++)
     if (col + e < cols) v[e] = row[col + e];
   return v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_some(T *row, uint32_t col, uint32_t cols, typename Loose<T, N>::Values v) {
+  if (col + N <= cols) {
+    loose<T, N>(row + col, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; e++)
+    if (col + e < cols) row[col + e] = v[e];
 }
 
 // The sums of the columns of parts[rows][n], each given to put(column, sum), in one order: a block

@@ -157,11 +157,12 @@ struct Load {
       }
     } else {
 #pragma unroll 1
-      for (uint32_t job = thread; job < kChunk * COLS; job += THREADS) {
-        const uint32_t row = job / COLS, col = job % COLS;
-        const T one = row < rows && col < cols ? at[(int64_t)row * stride + col] : (T)0.0f;
-        to[row * kPitch + col] = one;
-        odd |= !finite((float)one);
+      for (uint32_t job = thread; job < kJobs; job += THREADS) {
+        const uint32_t row = job / (COLS / 8), col = job % (COLS / 8) * 8;
+        const V8<T> some = load_some<T, 8>(at + (int64_t)row * stride, row < rows, col, cols);
+        *(V8<T> *)(to + row * kPitch + col) = some;
+#pragma unroll
+        for (int e = 0; e < 8; e++) odd |= !finite((float)some[e]);
       }
     }
     return odd;
