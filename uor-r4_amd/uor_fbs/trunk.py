@@ -91,6 +91,8 @@ class NormGrads(NamedTuple):
     dpre: Optional[torch.Tensor]
 
 
+_Tensor = torch.Tensor
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # none without a HIP device to call it for
 _lib = None
 _calls = {}  # name: (the call, its workspace's size or None)
 
@@ -125,7 +127,7 @@ def _call(name, args, index):
     """The library's call on the current stream of device `index`."""
     L = _lib or lib()
     call, bytes_of = _calls[name]
-    args.device, ref, stream = index, C.byref(args), torch._C._cuda_getCurrentRawStream(index)
+    args.device, ref, stream = index, C.byref(args), _raw_stream(index)
     if bytes_of is None:
         code = call(ref, stream)
     else:
@@ -151,7 +153,8 @@ def _rows(name, t, dtype, shape, inner):
     """t with dense inner axes of `inner` values, and the values between its rows (None: None, 0)."""
     if t is None:
         return None, 0
-    _check(name, t, dtype, shape)
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.shape == shape):
+        _check(name, t, dtype, shape)
     if t.is_contiguous():
         return t, inner
     size_so_far = 1
@@ -167,7 +170,8 @@ def _rows(name, t, dtype, shape, inner):
 def _dense(name, t, dtype, shape):
     if t is None:
         return None
-    _check(name, t, dtype, shape)
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.shape == shape):
+        _check(name, t, dtype, shape)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -220,7 +224,9 @@ def _dtype(t, name):
 
 def _make(like):
     """A dense tensor of the same type, shape and device (None: None)."""
-    return None if like is None else torch.empty_like(like, memory_format=torch.contiguous_format)
+    if like is None:
+        return None
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 # ---------------------------------------------------------------------------------------------
