@@ -462,6 +462,24 @@ def test_scan_of_many_short_sequences(state, dtype):
     check_scan_backward(x, m, dtype)
 
 
+def test_scan_of_many_rows_in_order_of_length(dtype):
+    """Calls large enough to go through their sequences by length give what smaller ones give."""
+    lengths = [(i * 37) % 161 for i in range(450)]
+    x, m = scan_case(dtype, lengths, 16, 2, 32, 16, seed=4)
+    assert sum(lengths) >= 32768
+    dy = m(*x["x"].shape)
+    (y, final), grads = trunk.scan(**x), trunk.scan_backward(dy, **x)
+    cuts = [0, 200, 450]
+    for a, b in zip(cuts, cuts[1:]):
+        rows = slice(sum(lengths[:a]), sum(lengths[:b]))
+        part = {**x, **{k: x[k][rows] for k in ("x", "dt", "B", "C")}, "offsets": oracle.offsets_of(lengths[a:b]).cuda()}
+        y2, final2 = trunk.scan(**part)
+        assert torch.equal(y[rows], y2) and torch.equal(final[a:b], final2)
+        some = trunk.scan_backward(dy[rows], **part)
+        for name in ("dx", "ddt", "dB", "dC"):
+            assert torch.equal(getattr(grads, name)[rows], getattr(some, name)), name
+
+
 def test_scan_of_thousands_of_sequences(dtype):
     x, _ = scan_case(dtype, [1] * 5000, 1, 1, 4, 3, initial=True, seed=3)
     check_scan(x, dtype)

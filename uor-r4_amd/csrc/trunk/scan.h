@@ -95,6 +95,7 @@ struct Scan {
   float *final;
   float *starts;         // [pieces][heads][dim][state]: where a piece begins, if sequences are cut; or NULL
   double *totals;        // [pieces][heads]: log2 of a piece's whole decay
+  uint32_t *order;       // the pieces, longest first: how many, and from the third on sequence and number; or NULL
   bool x_wide, b_wide, c_wide, y_wide, state_wide;
 };
 
@@ -110,6 +111,17 @@ __device__ __forceinline__ void place_of(uint32_t block, uint32_t heads, uint32_
 
 int check_scan(const uor_trunk_scan_args *s, bool step);
 Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
+// The block's piece, in the pieces' order or the call's; `number` is then its place among all pieces.
+__device__ __forceinline__ bool next_piece(const Scan &a, uint32_t &number, Piece &at) {
+  if (number >= a.pieces) return false;
+  if (!a.order) return wave_piece(a.rows, number, a.size, at);
+  if (number >= a.order[0]) return false;
+  const uint32_t *place = a.order + 2 + 2 * number;
+  at = piece_of(a.rows, place[0], place[1], a.size);
+  number = at.start / a.size + at.seq + at.number;
+  return true;
+}
+
 // A join's blocks: by sequences, or by the places of later pieces, where there are fewer.
 __host__ __device__ inline uint32_t join_places(const Scan &a) { return a.rows.seqs < a.later ? a.rows.seqs : a.later; }
 // The sequence of a join's block, and how many pieces it has.

@@ -7,9 +7,10 @@
 // wavefronts are of one group and share B and C; x is each wavefront's own.
 //
 // Rows are bound by instructions and by time, not by bytes or products: 300 bf16 prompts of up to 509,
-// 8 heads of 64 by a state of 64, take 116 us, of which their bytes would take 41, the vector
-// instructions 48 and the products 16. Two pairs of tiles of x a wavefront compute scores and decays
-// once for both, but leave half the wavefronts, two a SIMD instead of three: 130 us against 112.
+// 8 heads of 64 by a state of 64, take 82 us (91 with the launches around), of which their bytes would
+// take 41, the vector instructions 48 and the products 16. Two pairs of tiles of x a wavefront compute
+// scores and decays once for both, but leave half the wavefronts, two a SIMD instead of three: 130 us
+// against 112, before the longest went first.
 //
 // A sequence of many rows and few heads would run on few wavefronts. Such sequences are cut into
 // pieces: a first launch gives every piece its end state from zeros, a second joins them along the
@@ -51,9 +52,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
   __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sXs[W][kChunk * kPp];
   __shared__ Steps steps[W];
 
-  const Unit unit = unit_of<W>(a, kP);
+  Unit unit = unit_of<W>(a, kP);
   Piece at;
-  if (unit.piece >= a.pieces || !wave_piece(a.rows, unit.piece, a.size, at)) return;
+  if (!next_piece(a, unit.piece, at)) return;
   const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
   const uint32_t head = unit.head;
   const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head;
@@ -240,6 +241,48 @@ __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
   }
 }
 
+// The pieces by their chunks, the longest first, so that none begins when the others end: 300 prompts of
+// up to 509 take 116 us in their own order and 82 in this, and 5 for the order. Which of two alike comes
+// first may differ from call to call; no result depends on it.
+__global__ __launch_bounds__(1024) void scan_order(Scan a) {
+  constexpr uint32_t kBuckets = 64;
+  __shared__ uint32_t next[kBuckets + 1];
+  for (uint32_t b = threadIdx.x; b <= kBuckets; b += 1024) next[b] = 0;
+  __syncthreads();
+  const auto bucket = [](uint32_t rows) {
+    const uint32_t chunks = (rows + kChunk - 1) / kChunk;
+    return kBuckets - (chunks < kBuckets ? chunks : kBuckets);
+  };
+  const auto each = [&](auto put) {
+    for (uint32_t seq = threadIdx.x; seq < a.rows.seqs; seq += 1024) {
+      uint32_t start, stop;
+      a.rows.of(seq, start, stop);
+      const uint32_t n = stop > start ? (stop - start - 1) / a.size + 1 : 1;
+      if (n > 1) put(seq, 0, n - 1, bucket(a.size));
+      put(seq, n - 1, 1, bucket(stop - start - (n - 1) * a.size));
+    }
+  };
+  each([&](uint32_t, uint32_t, uint32_t count, uint32_t b) { atomicAdd(&next[b], count); });
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t sum = 0;
+    for (uint32_t b = 0; b <= kBuckets; b++) {
+      const uint32_t here = next[b];
+      next[b] = sum;
+      sum += here;
+    }
+    a.order[0] = sum < a.pieces ? sum : a.pieces;  // more only where the offsets do not ascend
+  }
+  __syncthreads();
+  each([&](uint32_t seq, uint32_t number, uint32_t count, uint32_t b) {
+    const uint32_t at = atomicAdd(&next[b], count);
+    for (uint32_t i = 0; i < count && at + i < a.pieces; i++) {
+      a.order[2 + 2 * (at + i)] = seq;
+      a.order[3 + 2 * (at + i)] = number + i;
+    }
+  });
+}
+
 // How many rows a piece has: sequences are cut where they alone would leave the card idle. The grid
 // then has about 4,096 wavefronts, two for each place; pieces under `least` rows cost more to join
 // than they gain: one head over 9 prompts of 2,580 rows takes 122 us in pieces of 512 and 47 in pieces of
@@ -261,6 +304,7 @@ int launch(const Scan &a, hipStream_t stream) {
     hipLaunchKernelGGL((scan_ends<T, NT, PW, W, false>), dim3(grid_of(a.later, blocks)), dim3(64 * W), 0, stream, a);
     hipLaunchKernelGGL(scan_join, join_of(a), dim3(kThreads), 0, stream, a);
   }
+  if (a.order) hipLaunchKernelGGL(scan_order, dim3(1), dim3(1024), 0, stream, a);
   hipLaunchKernelGGL((scan_rows<T, NT, PW, W>), dim3(grid_of(a.pieces, blocks)), dim3(64 * W), 0, stream, a);
   return launched();
 }
@@ -278,8 +322,29 @@ int launch(const Scan &a, hipStream_t stream) {
 uint32_t rows_of(const uor_trunk_scan_args *s) {
   return s->tokens <= 512 ? 512 + kChunk : piece_rows(s->tokens, s->seqs, s->heads * ((s->dim + 31) / 32), 128);
 }
-uint64_t starts_bytes(uint64_t pieces, const uor_trunk_scan_args *s) {
-  return (pieces * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
+// Where a call's scratch memory begins, and how much there is.
+struct Plan {
+  uint32_t size;
+  bool cut, ordered;
+  uint64_t totals, order, bytes;
+};
+Plan plan_of(const uor_trunk_scan_args *s) {
+  Plan p{};
+  p.size = rows_of(s);
+  p.cut = p.size < s->tokens;
+  const uint64_t n = pieces(s->tokens, s->seqs, p.size), waves = n * s->heads * ((s->dim + 31) / 32);
+  // One launch more, where more wavefronts are wanted than the card holds and each has long to go; the
+  // launch looks at 1,024 sequences at a time.
+  p.ordered = s->seqs > 1 && s->seqs <= 8192 && waves > 3072 && s->tokens >= 32768;
+  if (p.cut) {
+    p.totals = (n * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
+    p.bytes = p.totals + n * s->heads * sizeof(double);
+  }
+  if (p.ordered) {
+    p.order = (p.bytes + 15) / 16 * 16;
+    p.bytes = p.order + (n + 1) * 8;
+  }
+  return p;
 }
 
 }  // namespace
@@ -329,25 +394,20 @@ extern "C" uint64_t uor_trunk_sizeof_scan(void) { return sizeof(uor_trunk_scan_a
 extern "C" uint64_t uor_trunk_sizeof_conv(void) { return sizeof(uor_trunk_conv_args); }
 extern "C" uint64_t uor_trunk_sizeof_norms(void) { return sizeof(uor_trunk_norms_args); }
 
-extern "C" uint64_t uor_trunk_scan_workspace_bytes(const uor_trunk_scan_args *s) {
-  if (check_scan(s, false)) return 0;
-  const uint32_t size = rows_of(s);
-  if (size >= s->tokens) return 0;
-  const uint64_t n = pieces(s->tokens, s->seqs, size);
-  return starts_bytes(n, s) + n * s->heads * sizeof(double);
-}
+extern "C" uint64_t uor_trunk_scan_workspace_bytes(const uor_trunk_scan_args *s) { return check_scan(s, false) ? 0 : plan_of(s).bytes; }
 
 extern "C" int uor_trunk_scan_async(const uor_trunk_scan_args *s, void *workspace, uint64_t bytes, void *stream) {
   if (const int e = check_scan(s, false)) return e;
   if (s->tokens && !s->y) return fail(-1, "null y");
-  const uint64_t want = uor_trunk_scan_workspace_bytes(s);
-  if (want && (!workspace || bytes < want || (uintptr_t)workspace % 16))
-    return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)want);
-  Scan a = scan_of(s, rows_of(s));
-  if (want) {
+  const Plan p = plan_of(s);
+  if (p.bytes && (!workspace || bytes < p.bytes || (uintptr_t)workspace % 16))
+    return fail(-1, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)p.bytes);
+  Scan a = scan_of(s, p.size);
+  if (p.cut) {
     a.starts = (float *)workspace;
-    a.totals = (double *)((char *)workspace + starts_bytes(a.pieces, s));
+    a.totals = (double *)((char *)workspace + p.totals);
   }
+  if (p.ordered) a.order = (uint32_t *)((char *)workspace + p.order);
   if ((uint64_t)(a.pieces + kXcds) * a.heads * a.tiles > 0x7fffffffu) return fail(-1, "too many sequences and heads for one call");
   const OnDevice on(s->device);
   if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);

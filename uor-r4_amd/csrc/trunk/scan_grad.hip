@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   uint32_t number, block;
   place_of(blockIdx.x, a.groups * k.parts, number, block);
   Piece at;
-  if (number >= a.pieces || !wave_piece(a.rows, number, a.size, at)) return;
+  if (!next_piece(a, number, at)) return;
   const uint32_t group = block / k.parts, part = block % k.parts;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
   const T *B = (const T *)a.B + group * a.state, *C = (const T *)a.C + group * a.state;
@@ -682,6 +682,7 @@ __global__ __launch_bounds__(kThreads) void grad_join(Grad k) {
   }
 }
 __global__ __launch_bounds__(kThreads) void scan_join(Scan a);
+__global__ __launch_bounds__(1024) void scan_order(Scan a);
 
 namespace {
 
@@ -690,7 +691,8 @@ uint32_t tiles_of(uint32_t dim) { return dim <= 32 ? 1 : dim <= 64 ? 2 : 4; }
 // Where a gradient's scratch memory begins, and how much there is.
 struct Plan {
   uint32_t size, pieces, waves, subs, parts;
-  uint64_t cut, back, totals, h, sums, dB, dC, bytes;
+  bool ordered;
+  uint64_t cut, back, totals, order, h, sums, dB, dC, bytes;
 };
 Plan plan_of(const uor_trunk_scan_args *s) {
   Plan p{};
@@ -716,6 +718,9 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   const bool cut = p.size < s->tokens;
   const uint64_t starts = cut ? (uint64_t)p.pieces * s->heads * s->dim * s->state * 4 : 0;
   p.cut = take(starts), p.back = take(starts);
+  // As in the scan; two wavefronts a SIMD, and each chunk takes several times as long.
+  p.ordered = s->seqs > 1 && s->seqs <= 8192 && (uint64_t)p.pieces * s->groups * p.parts * p.waves > 2048 && s->tokens >= 16384;
+  p.order = take(p.ordered ? ((uint64_t)p.pieces + 1) * 8 : 0);
   p.totals = take(cut ? (uint64_t)p.pieces * s->heads * 8 : 0);
   // States are kept of chunks that have one before them and one after them in their piece.
   p.h = take(p.size > 2 * kChunk && s->tokens > 2 * kChunk ? ((uint64_t)s->tokens / kChunk + 1) * s->heads * tiles * n16 * 32 * 4 : 0);
@@ -743,6 +748,7 @@ int launch(const Grad &k, hipStream_t stream) {
     hipLaunchKernelGGL((scan_ends<T, NT, 2, E, true>), grid, dim3(64 * E), 0, stream, s);
     hipLaunchKernelGGL(grad_join, join, dim3(kThreads), 0, stream, k);
   }
+  if (a.order) hipLaunchKernelGGL(scan_order, dim3(1), dim3(1024), 0, stream, a);
   hipLaunchKernelGGL((grad_rows<T, NT, W>), dim3(grid_of(a.pieces, a.groups * k.parts)), dim3(64 * W), 0, stream, k);
   if (k.parts > 1 && a.rows.tokens) {
     const uint64_t n = (uint64_t)a.rows.tokens * a.groups * a.state;
@@ -789,6 +795,7 @@ extern "C" int uor_trunk_scan_backward_async(const uor_trunk_scan_args *s, void 
     k.g_starts = (float *)(base + p.back);
     k.s.totals = (double *)(base + p.totals);
   }
+  if (p.ordered) k.s.order = (uint32_t *)(base + p.order);
   k.s.state_wide = s->state % 4 == 0 && aligned16(s->initial, 0, 4) && aligned16(s->dfinal, 0, 4) && aligned16(s->dinitial, 0, 4);
   k.dy = s->dy, k.dfinal = s->dfinal, k.subs = p.subs, k.parts = p.parts;
   k.h = (float *)(base + p.h), k.sums = (double *)(base + p.sums);
