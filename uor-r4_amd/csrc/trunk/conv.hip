@@ -83,15 +83,17 @@ __device__ __forceinline__ bool lane_of(const Conv &a, Lane &l) {
   l.c = (parts > 1 ? thread : thread % groups) * E;
   return l.line < lines && l.c < a.channels;
 }
-template <int TAPS, int E>
+template <int TAPS, bool WIDE, int E>
 __device__ __forceinline__ void taps_of(const Conv &a, uint32_t c, Some<E> (&w)[TAPS], Some<E> &bias) {
+  // A channel's taps are next to each other; whole pieces ask for no channel that is not there.
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const bool there = c + e < a.channels;
+    Some<TAPS> taps = 0.0f;
+    if (WIDE || c + e < a.channels) taps = loose<float, TAPS>(a.weight + (uint64_t)(c + e) * TAPS);
 #pragma unroll
-    for (int k = 0; k < TAPS; k++) w[k][e] = there ? a.weight[(c + e) * TAPS + k] : 0.0f;
-    bias[e] = there && a.bias ? a.bias[c + e] : 0.0f;
+    for (int k = 0; k < TAPS; k++) w[k][e] = taps[k];
   }
+  bias = a.bias ? load_some<float, E>(a.bias, true, c, a.channels) : Some<E>(0.0f);
 }
 // Row `first - TAPS + 1 + k` of the sequence for each k < TAPS - 1: its own, or one before it.
 template <class T, int TAPS, bool WIDE, int E>
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
   if (!lane_of<E, 256>(a, l) || l.run >= a.pieces || !piece(a.rows, l.run, kRun, at)) return;
   const uint32_t c = l.c;
   Some<E> w[TAPS], bias, rows[kPast + kRowBatch];
-  taps_of<TAPS, E>(a, c, w, bias);
+  taps_of<TAPS, WIDE, E>(a, c, w, bias);
   rows_before<T, TAPS, WIDE, E>(a, at, c, rows);
   uint32_t left = 0;  // rows of the last batch
   for (uint32_t first = at.first; first < at.end; first += kRowBatch) {
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kGradThreads, 3) void conv_grad_rows(Conv a) {
   for (int k = 0; k <= TAPS; k++) sums[k] = Some<E>(0.0f);
   if (there) {
     Some<E> w[TAPS], bias;
-    taps_of<TAPS, E>(a, c, w, bias);
+    taps_of<TAPS, WIDE, E>(a, c, w, bias);
     for (uint32_t number = l.run; number < a.pieces; number += a.workers) {
       Piece at;
       if (!piece(a.rows, number, kGradRun, at)) continue;
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(256) void conv_step(Conv a) {
 #pragma unroll
   for (int k = 0; k < TAPS - 1; k++) rows[k] = row_some<T, WIDE, E>(state, (int64_t)k * a.channels, c, a.channels);
   rows[TAPS - 1] = row_some<T, WIDE, E>(a.x, row * a.x_stride, c, a.channels);
-  taps_of<TAPS, E>(a, c, w, bias);
+  taps_of<TAPS, WIDE, E>(a, c, w, bias);
   Some<E> v = weighted<TAPS, E>(rows, w, bias);
   if (a.silu) v = silu<E>(v);
   put_some<T, WIDE, E>(y, c, a.channels, v);
