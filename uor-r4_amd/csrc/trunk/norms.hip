@@ -41,12 +41,9 @@ __device__ __forceinline__ float row_sum(float v, float *scratch) {
 }
 __device__ __forceinline__ f32x8 eight(float v) { return f32x8{v, v, v, v, v, v, v, v}; }
 __device__ __forceinline__ float total(f32x8 v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
-// A parameter's eight values, `other` without one.
+// A parameter's eight values, `other` without one; what is past the last column meets only zeros.
 __device__ __forceinline__ f32x8 param8(const float *p, uint32_t col, uint32_t cols, float other) {
-  f32x8 v;
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = col + e < cols ? (p ? p[col + e] : other) : 0.0f;
-  return v;
+  return p ? load_some<float, 8>(p, true, col, cols) : eight(other);
 }
 template <class T>
 __device__ __forceinline__ f32x8 values(const void *base, int64_t at, bool there, uint32_t col, uint32_t cols) {
