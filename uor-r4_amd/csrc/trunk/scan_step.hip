@@ -2,7 +2,8 @@
 //
 // One block takes one head of one session. Bound by the state, read and written once: LN lanes hold
 // a row of it, four values each, with their four of B and C in registers, and y is their sum. 1,024
-// sessions of 8 heads of 64 by 64, 268 MB of states read and written: 67 us, 4.0 TB/s.
+// sessions of 8 heads of 64 by 64, 268 MB of states read and written: 57 us, 4.7 TB/s; with B and C
+// read a value at a time 67.
 #include "scan.h"
 
 namespace trunk {
@@ -35,12 +36,8 @@ __global__ __launch_bounds__(256) void scan_step(Step a) {
   const T *B = (const T *)a.B + row * a.b_stride + group * a.state, *C = (const T *)a.C + row * a.c_stride + group * a.state;
   const float step = softplus((float)((const T *)a.dt)[row * a.dt_stride + head] + (a.bias ? a.bias[head] : 0.0f));
   const float decay = exp2_(step * a.A[head] * kLog2e), skip = a.D ? a.D[head] : 0.0f;
-  f32x4 b, c;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    b[e] = n + e < a.state ? (float)B[n + e] : 0.0f;
-    c[e] = n + e < a.state ? (float)C[n + e] : 0.0f;
-  }
+  const f32x4 b = __builtin_convertvector((load_some<T, 4>(B, true, n, a.state)), f32x4);
+  const f32x4 c = __builtin_convertvector((load_some<T, 4>(C, true, n, a.state)), f32x4);
   float *states = a.states + ((uint64_t)slot * a.heads + head) * a.dim * a.state;
   for (uint32_t p = pr; p < a.dim; p += kRows) {
     float *at = states + (uint64_t)p * a.state + n;
