@@ -3,10 +3,10 @@
 //
 // Bound by its rows, read once and written once. A thread walks down a run of rows with eight
 // channels (16 bytes of bf16) and the rows before it in registers; a batch of rows is read before the
-// first is used. 300 bf16 prompts of up to 509 by 640 channels: 64 us, 3.0 TB/s; a row at a time 103.
+// first is used. 300 bf16 prompts of up to 509 by 640 channels: 52 us, 3.7 TB/s; a row at a time 103.
 // The gradient holds sums, gradients and rows of four channels, three wavefronts a SIMD; it reads a
 // batch ahead, and rows in a run's middle ask nothing row by row, so that no store is waited for:
-// 2,048 sequences of 128 take 307 us, 3.3 TB/s; with eight channels 390, without the middle 354.
+// 2,048 sequences of 128 take 306 us, 3.3 TB/s; with eight channels 390, without the middle 354.
 #include "trunk.h"
 
 #include <type_traits>
