@@ -6,7 +6,8 @@
 // first is used. 300 bf16 prompts of up to 509 by 640 channels: 52 us, 3.7 TB/s; a row at a time 103.
 // The gradient holds sums, gradients and rows of four channels, three wavefronts a SIMD; it reads a
 // batch ahead, and rows in a run's middle ask nothing row by row, so that no store is waited for:
-// 2,048 sequences of 128 take 306 us, 3.3 TB/s; with eight channels 390, without the middle 354.
+// 2,048 sequences of 128 take 258 us, 3.9 TB/s; with eight channels, in blocks of 512 threads, 390
+// where four took 307, without the middle 354.
 #include "trunk.h"
 
 #include <type_traits>
@@ -17,7 +18,10 @@ namespace trunk {
 // twice. Shorter runs fill the card sooner.
 constexpr uint32_t kRun = 16, kGradRun = 32;
 constexpr int kBatch = 4, kRowBatch = 8;  // rows that are read together, in a gradient and without
-constexpr uint32_t kGradThreads = 512;
+// A gradient's registers leave a SIMD three wavefronts, twelve a compute unit: one block of 768 threads,
+// and no more blocks than compute units, so that all begin at once: 258 us; 768 blocks 279, 512 threads
+// (one block still) 299, 384 (two, a sixth of the lanes idle) 379, 1,024 (128 registers a thread) 387.
+constexpr uint32_t kGradThreads = 768, kMostGradBlocks = 256;
 
 struct Conv {
   Rows rows;
@@ -347,14 +351,14 @@ bool wide_of(const uor_trunk_conv_args *s) {
   return wide(s->x, s->x_stride) && wide(s->y, s->y_stride) && wide(s->dy, s->y_stride) && wide(s->initial, 0) && wide(s->final, 0) &&
          wide(s->states, 0) && wide(s->dfinal, 0) && wide(s->dinitial, 0) && wide(s->dx, 0);
 }
-// The blocks of `runs` runs, and of a gradient: three for each compute unit at most.
+// The blocks of `runs` runs, and of a gradient: one for each compute unit at most.
 uint32_t blocks_of(uint32_t runs, uint32_t channels) {
   const uint32_t lines = lines_of<8, 256>(channels);
   return (runs + lines - 1) / lines * parts_of<8, 256>(channels);
 }
 uint32_t grad_blocks_of(uint32_t runs, uint32_t channels) {
   const uint32_t lines = lines_of<4, kGradThreads>(channels), parts = parts_of<4, kGradThreads>(channels);
-  const uint32_t few = (runs + lines - 1) / lines, most = (768 + parts - 1) / parts;
+  const uint32_t few = (runs + lines - 1) / lines, most = (kMostGradBlocks + parts - 1) / parts;
   return few < 1 ? 1 : few < most ? few : most;
 }
 template <template <class, int, bool> class F, class T, bool WIDE, class... V>
