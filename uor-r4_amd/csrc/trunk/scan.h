@@ -12,10 +12,6 @@ constexpr int kThreads = 256; // four wavefronts
 // places 8 (lane / 16) .. + 7, or for an operand built from two result tiles places 4 (lane / 16)
 // .. + 3 of the first and of the second: any order of the places is right if both operands have
 // the same. A lane's four results are rows 4 (lane / 16) + r of column lane % 16.
-//
-// Split is an operand that was computed in 32 bits. With bf16 it is the sum of two bf16 parts,
-// 2^-18 of a value off at most: one part alone would add an error of the size of y's own rounding
-// to y, and states and their sums are held to 32 bits' worth.
 
 // v rounded to bf16, and v then what the rounding left of it. Two values at a time, as they are
 // rounded by one instruction and lie in one register.
@@ -36,27 +32,12 @@ template <class T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-  struct Split {
-    bf16x8 hi, lo;
-  };
-  static constexpr int kParts = 2;
-  static __device__ __forceinline__ Split split(f32x8 v) {
-    Split s;
-    s.hi = round8(v);
-    s.lo = round8(v);
-    return s;
-  }
   static __device__ __forceinline__ f32x4 mul(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x4 mul(bf16x8 a, const Split &b, f32x4 c) { return mul(a, b.hi, mul(a, b.lo, c)); }
-  static __device__ __forceinline__ f32x4 mul(const Split &a, bf16x8 b, f32x4 c) { return mul(a.hi, b, mul(a.lo, b, c)); }
 };
 template <>
 struct Mma<float> {
-  using Split = f32x8;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ Split split(f32x8 v) { return v; }
   static __device__ __forceinline__ f32x4 mul(f32x8 a, f32x8 b, f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);

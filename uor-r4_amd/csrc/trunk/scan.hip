@@ -111,9 +111,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
       for (int tile = 0; tile < 4; tile++) c[tile] = operand(sC + (tile * 16 + i16) * kNp, 32 * k + 8 * q);
 #pragma unroll
       for (int i = 0; i < PW; i++) {
-        const auto hs = Mma<T>::split(__builtin_shufflevector(h[2 * k][i], h[2 * k + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
+        const auto hs = Fine<T>::of(__builtin_shufflevector(h[2 * k][i], h[2 * k + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int tile = 0; tile < 4; tile++) acc[tile][i] = Mma<T>::mul(hs, c[tile], acc[tile][i]);
+        for (int tile = 0; tile < 4; tile++) acc[tile][i] = mul(hs, c[tile], acc[tile][i]);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -156,9 +156,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
 #pragma unroll
       for (int i = 0; i < PW; i++) acc[tile][i] *= tile < 2 ? d.from[tile] * u : d.from[tile];
       const auto add = [&](int pair, f32x8 m) {
-        const auto w = Mma<T>::split(m);
+        const auto w = Fine<T>::of(m);
 #pragma unroll
-        for (int i = 0; i < PW; i++) acc[tile][i] = Mma<T>::mul(xs[pair][i], w, acc[tile][i]);
+        for (int i = 0; i < PW; i++) acc[tile][i] = mul(xs[pair][i], w, acc[tile][i]);
       };
       if (tile >= 2) {
         add(0, __builtin_shufflevector(before(0), before(1), 0, 1, 2, 3, 4, 5, 6, 7));

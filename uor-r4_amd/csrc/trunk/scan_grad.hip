@@ -62,12 +62,12 @@ __device__ __forceinline__ bf16x8 turn(bf16x8 a, bf16x8 b, bf16x8 unit) {
   const f32x4 x = Mma<bf16>::mul(a, unit, zero), y = Mma<bf16>::mul(b, unit, zero);
   return __builtin_convertvector(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), bf16x8);
 }
-__device__ __forceinline__ Mma<bf16>::Split turn(const Mma<bf16>::Split &a, const Mma<bf16>::Split &b, bf16x8 unit) {
-  return {turn(a.hi, b.hi, unit), turn(a.lo, b.lo, unit)};
+__device__ __forceinline__ Fine<bf16> turn(const Fine<bf16> &a, const Fine<bf16> &b, bf16x8 unit) {
+  return {turn(a.hi, b.hi, unit), turn(a.mid, b.mid, unit), turn(a.lo, b.lo, unit)};
 }
-__device__ __forceinline__ f32x8 turn(f32x8 a, f32x8 b, f32x8 unit) {
+__device__ __forceinline__ Fine<float> turn(const Fine<float> &a, const Fine<float> &b, f32x8 unit) {
   const f32x4 zero = {0, 0, 0, 0};
-  return __builtin_shufflevector(Mma<float>::mul(a, unit, zero), Mma<float>::mul(b, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7);
+  return {__builtin_shufflevector(Mma<float>::mul(a.v, unit, zero), Mma<float>::mul(b.v, unit, zero), 0, 1, 2, 3, 4, 5, 6, 7)};
 }
 __device__ __forceinline__ float dot(f32x8 a, f32x8 b) {
   const f32x4 v = __builtin_shufflevector(a, a, 0, 1, 2, 3) * __builtin_shufflevector(b, b, 0, 1, 2, 3) +
@@ -331,9 +331,9 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
                 const f32x4 zero = {0, 0, 0, 0};  // the parts' sum is the value itself
                 const f32x8 turned = __builtin_shufflevector(mul(gp[0], unit_part, zero), mul(gp[1], unit_part, zero), 0, 1, 2, 3, 4, 5, 6, 7);
                 if (has_h && (step_ == 0 || !more)) inner += dot(turned, __builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
-                const auto gt = Mma<T>::split(turned);
+                const auto gt = Fine<T>::of(turned);
 #pragma unroll
-                for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(gt, X[w], accB[w][n]);
+                for (int w = 0; w < 2; w++) accB[w][n] = mul(gt, X[w], accB[w][n]);
               }
               __builtin_amdgcn_sched_barrier(0);
             }
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         }
         if (!idle) {
           // What comes from the chunk's own rows.
-          typename Mma<T>::Split Z[2];
+          Fine<T> Z[2];
           float rows[2][4] = {};  // a lane's part of E's rows, over the tiles before theirs
 #pragma unroll
           for (int w = 0; w < 2; w++) {
@@ -442,10 +442,10 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               }
               z[v] *= step;
             }
-            const auto m = Mma<T>::split(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            const auto m = Fine<T>::of(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (int i = 0; i < 2; i++) dx[w][i] = Mma<T>::mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[w][i]);
-            Z[w] = Mma<T>::split(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int i = 0; i < 2; i++) dx[w][i] = mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[w][i]);
+            Z[w] = Fine<T>::of(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
             __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
@@ -460,17 +460,17 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
           for (int n = 0; n < NT; n++) {
             const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
 #pragma unroll
-            for (int w = 0; w < 2; w++) accB[w][n] = Mma<T>::mul(c, Z[w], accB[w][n]);
+            for (int w = 0; w < 2; w++) accB[w][n] = mul(c, Z[w], accB[w][n]);
           }
           __builtin_amdgcn_sched_barrier(0);
-          typename Mma<T>::Split Zt[2];
+          Fine<T> Zt[2];
 #pragma unroll
           for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
 #pragma unroll
           for (int n = 0; n < NT; n++) {
             const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
 #pragma unroll
-            for (int v = 0; v < 2; v++) accC[v][n] = Mma<T>::mul(b, Zt[v], accC[v][n]);
+            for (int v = 0; v < 2; v++) accC[v][n] = mul(b, Zt[v], accC[v][n]);
           }
           __builtin_amdgcn_sched_barrier(0);
         }

@@ -23,7 +23,11 @@ namespace trunk {
 // are then 16 or 32 bytes of memory, and in this order the operand of the next product.
 __device__ __forceinline__ int place(int tile, int row) { return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3); }
 
-// A bf16 operand in three parts, 2^-25 of a value off at most: what a state is summed from.
+// An operand that was computed in 32 bits. With bf16 it goes in as the sum of three bf16 parts, 2^-25 of
+// a value off at most, so that the products are those of 32 bits. With two parts, 2^-18 off, one bf16
+// output in a thousand rounded the other way than 32-bit sums do, and states were four times further from
+// 64 bits than such sums are; 300 bf16 prompts of up to 509 took 92 us where they take 98, gradients of
+// 2,048 sequences of 128 1,000 where they take 1,075.
 template <class T>
 struct Fine;
 template <>
@@ -318,8 +322,7 @@ __device__ __forceinline__ f32x8 weights(int lane, const float *rows, int row0, 
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// h' = e^(l_end) h + the sum over the chunk's rows of their weight, column of x and row of B: in three
-// parts, so that the sums of a state are as good as in 32 bits.
+// h' = e^(l_end) h + the sum over the chunk's rows of their weight, column of x and row of B.
 template <class T, int NT, int PW>
 __device__ __forceinline__ void advance(int lane, f32x4 (&h)[NT][PW], const V8<T> (&xs)[2][PW], const T *sB, const float *rows, const float (&to)[4], float whole) {
 #pragma unroll
