@@ -1,0 +1,83 @@
+"""GPU tests of the float trunk's operators (uor_fbs.trunk) at the edges of what a call may hold: rows that
+no sequence owns, offsets of any content, far slots, pieces of several chunks, values that are not finite. Tolerances are
+those of the operators' own tests."""
+
+import pytest
+import torch
+
+import trunk_cases as oracle
+from test_hip_trunk import CONV_UNIT, check_scan, check_scan_backward, conv_case, dtype, near, scan_case, trunk  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def stale(monkeypatch):
+    """Memory that a call takes holds NaN, as it may after other work."""
+    def filled(make):
+        def made(*args, **kw):
+            t = make(*args, **kw)
+            if t.is_cuda and t.numel():
+                t.view(torch.uint8).fill_(255)
+            return t
+        return made
+
+    monkeypatch.setattr(torch, "empty", filled(torch.empty))
+    monkeypatch.setattr(torch, "empty_like", filled(torch.empty_like))
+
+
+# ---------------------------------------------------------------------------------------------
+# Rows that no sequence owns.
+
+
+def without_ends(x, lengths):
+    """The case with its first and last sequence's rows left to nobody."""
+    x = {**x, "offsets": oracle.offsets_of(lengths)[1:-1].contiguous().cuda()}
+    if x["initial"] is not None:
+        x["initial"] = x["initial"][1:-1].contiguous()
+    return x
+
+
+PADDED = [
+    # lengths, heads, groups, dim, state; the first and the last are nobody's
+    ([3, 37, 0, 26, 14], 2, 1, 32, 16),
+    ([70, 20, 5, 90], 8, 1, 32, 20),       # a group's heads in two blocks
+    ([9, 1100, 130, 700], 2, 1, 16, 16),   # cut into pieces
+    ([5, 0, 0, 0, 200], 3, 3, 65, 33),     # nothing owned at all
+]
+
+
+@pytest.mark.parametrize("shape", PADDED, ids=str)
+def test_rows_of_no_sequence_are_zeros(shape, dtype, stale):
+    x, m = scan_case(dtype, *shape, initial=True, seed=12)
+    x = without_ends(x, shape[0])
+    a, b = int(x["offsets"][0]), int(x["offsets"][-1])
+    x["x"][:a], x["x"][b:] = 0, 0  # the oracle's dD takes in all rows
+    check_scan(x, dtype)
+    check_scan_backward(x, m, dtype)
+    dy = m(*x["x"].shape)
+    want = (*trunk.scan(**x), *trunk.scan_backward(dy, **x))
+    assert not any(t[:a].any() or t[b:].any() for t in (want[0], *(want[2 + i] for i in (0, 1, 3, 4))))
+    for t in (dy, *(x[k] for k in ("x", "dt", "B", "C"))):
+        t[:a], t[b:] = float("nan"), float("nan")
+    for one, two in zip(want, (*trunk.scan(**x), *trunk.scan_backward(dy, **x))):
+        assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("lengths,channels", [([3, 40, 0, 1, 33, 50], 24), ([30, 0, 64], 13), ([1, 700, 900], 8)], ids=str)
+def test_rows_of_no_sequence_are_zeros_in_the_convolution(lengths, channels, dtype, stale):
+    x, m = conv_case(dtype, lengths, channels, 4, True, seed=3)
+    x = without_ends(x, lengths)
+    y, final = trunk.conv(**x)
+    want, last, size = oracle.conv(**x)
+    near("y", y, want, size * 1.1, dtype, CONV_UNIT)
+    assert torch.equal(final.cpu().double(), last)
+    dy, dfinal = m(*y.shape), m(*final.shape)
+    got = trunk.conv_backward(dy, **x, dfinal=dfinal)
+    grads, sizes = oracle.conv_backward(dy, **x, dfinal=dfinal)
+    for name in trunk.ConvGrads._fields:
+        near(name, getattr(got, name), grads[name], sizes[name], torch.float32 if name in ("dweight", "dbias") else dtype,
+             CONV_UNIT + (sum(lengths) * 2.0 ** -24 if name in ("dweight", "dbias") else 0))
+    a, b = int(x["offsets"][0]), int(x["offsets"][-1])
+    for t in (y, got.dx):
+        assert not t[:a].any() and not t[b:].any()

@@ -129,6 +129,7 @@ __device__ __forceinline__ Some<E> silu(Some<E> v) {
 template <class T, int TAPS, bool WIDE>
 __global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
   constexpr int E = 8, kPast = TAPS - 1;
+  clear_unowned(a.rows, (T *)a.y, a.y_stride, a.channels);
   Lane l;
   Piece at;
   if (!lane_of<E, 256>(a, l) || l.run >= a.pieces || !piece(a.rows, l.run, kRun, at)) return;
@@ -175,6 +176,7 @@ template <class T, int TAPS, bool WIDE>
 __global__ __launch_bounds__(kGradThreads, 3) void conv_grad_rows(Conv a) {
   constexpr int E = 4, kPast = TAPS - 1;
   __shared__ float joined[kGradThreads * E];
+  clear_unowned(a.rows, (T *)a.dx, a.channels, a.channels);
   Lane l;
   const bool there = lane_of<E, kGradThreads>(a, l);
   const uint32_t c = l.c;

@@ -52,6 +52,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
   __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sXs[W][kChunk * kPp];
   __shared__ Steps steps[W];
 
+  clear_unowned(a.rows, (T *)a.y, a.y_stride, a.heads * a.dim);
   Unit unit = unit_of<W>(a, kP);
   Piece at;
   if (!next_piece(a, unit.piece, at)) return;

@@ -160,6 +160,10 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   __shared__ float sDa[W][kChunk], sDirect[W][kChunk], sDiag[W];
   const Scan &a = k.s;
   const uint32_t share = a.heads / a.groups, units = share * a.tiles;
+  clear_unowned(a.rows, (T *)k.dx, (int64_t)a.heads * a.dim, a.heads * a.dim);
+  clear_unowned(a.rows, (T *)k.ddt, a.heads, a.heads);
+  clear_unowned(a.rows, (T *)k.dB, (int64_t)a.groups * a.state, a.groups * a.state);
+  clear_unowned(a.rows, (T *)k.dC, (int64_t)a.groups * a.state, a.groups * a.state);
   uint32_t number, block;
   place_of(blockIdx.x, a.groups * k.parts, number, block);
   Piece at;
@@ -618,6 +622,10 @@ template <class T>
 __global__ __launch_bounds__(256) void grad_parts(Grad k) {
   const uint64_t n = (uint64_t)k.s.rows.tokens * k.s.groups * k.s.state, at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= n) return;
+  uint32_t first, end;
+  k.s.rows.owned(first, end);
+  const uint32_t row = (uint32_t)(at / (k.s.groups * k.s.state));
+  if (row < first || row >= end) return;  // cleared, and there are no parts
   float b = 0.0f, c = 0.0f;
   for (uint32_t p = 0; p < k.parts; p++) {
     b += k.dBparts[p * n + at];

@@ -79,7 +79,20 @@ struct Rows {
     start = at(s);
     end = max(at(s + 1), start);
   }
+  // The rows that some sequence may own, of offsets that ascend.
+  __device__ __forceinline__ void owned(uint32_t &first, uint32_t &end) const {
+    first = at(0);
+    end = max(at(seqs), first);
+  }
 };
+// Zeros in the rows of `cols` values that no sequence owns: the blocks of a grid share them.
+template <class T>
+__device__ __forceinline__ void clear_unowned(const Rows &rows, T *to, int64_t stride, uint32_t cols) {
+  uint32_t first, end;
+  rows.owned(first, end);
+  for (uint64_t i = blockIdx.x; i < rows.tokens - (end - first); i += gridDim.x)
+    for (uint32_t c = threadIdx.x; c < cols; c += blockDim.x) to[(int64_t)(i < first ? i : i + (end - first)) * stride + c] = (T)0.0f;
+}
 
 // Pieces of `size` rows: sequence s owns the pieces from offsets[s] / size + s on. Those places
 // do not overlap, as ceil(length / size) pieces fit below the next sequence's, and all lie below

@@ -6,7 +6,8 @@ Every function takes and returns torch tensors on one HIP device, runs on torch'
 waits for nothing. Activations are bfloat16 or float32; parameters, the scan's states and the
 parameters' gradients are float32. Rows are packed: ``offsets`` (int32, one more than there are
 sequences, ascending, on the device) says where each sequence's rows begin; without it all rows are
-one sequence. Where the inner axes of a tensor are not dense it is copied first. Errors raise
+one sequence. Rows before the first offset and from the last one on are no sequence's: what is
+returned is 0 there, and nothing else depends on them. Where the inner axes of a tensor are not dense it is copied first. Errors raise
 ``TrunkError``; there is no fallback: a missing library or device raises.
 
 ``*_backward`` computes the gradients from the call's own inputs; nothing is kept between calls.
