@@ -81,3 +81,37 @@ def test_rows_of_no_sequence_are_zeros_in_the_convolution(lengths, channels, dty
     a, b = int(x["offsets"][0]), int(x["offsets"][-1])
     for t in (y, got.dx):
         assert not t[:a].any() and not t[b:].any()
+
+
+# ---------------------------------------------------------------------------------------------
+# Places.
+
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 1, 1 << 31, -(1 << 32) + 1, 1 << 62])
+def test_slots_past_32_bits_are_skipped(far, dtype):
+    x, m = scan_case(dtype, [3], 2, 1, 16, 16)
+    states = m.f32(4, 2, 16, 16)
+    kept = states.clone()
+    slots = torch.tensor([3, far, 2]).cuda()
+    y = trunk.scan_step(**{k: x[k] for k in ("x", "dt", "A", "B", "C")}, states=states, slots=slots)
+    assert not y[1].any() and y[0].any() and y[2].any()
+    assert torch.equal(states[:2], kept[:2]) and not torch.equal(states[2:], kept[2:])
+    c, m = conv_case(dtype, [3], 8, 4, False)
+    held = m(4, 3, 8)
+    kept = held.clone()
+    y = trunk.conv_step(c["x"], c["weight"], held, slots=slots)
+    assert not y[1].any() and torch.equal(held[:2], kept[:2]) and not torch.equal(held[2:], kept[2:])
+
+
+def test_offsets_past_32_bits_are_the_nearest_inside(dtype):
+    x, m = scan_case(dtype, [40, 60], 2, 1, 32, 32)
+    dy = m(*x["x"].shape)
+    want = (*trunk.scan(**x), *trunk.scan_backward(dy, **x)[:7])
+    x["offsets"] = torch.tensor([-(1 << 32) + 7, 40, (1 << 32) + 50]).cuda()
+    for a, b in zip(want, (*trunk.scan(**x), *trunk.scan_backward(dy, **x)[:7])):
+        assert torch.equal(a, b)
+    c, _ = conv_case(dtype, [40, 60], 16, 4, False)
+    want = trunk.conv(**c)
+    c["offsets"] = x["offsets"]
+    for a, b in zip(want, trunk.conv(**c)):
+        assert torch.equal(a, b)

@@ -204,3 +204,11 @@ def test_c_entries_refuse_before_they_reach_a_device():
 
 def test_the_struct_sizes_are_the_librarys():
     assert (C.sizeof(trunk.CScan), C.sizeof(trunk.CConv), C.sizeof(trunk.CNorms)) == (40 + 5 * 8 + 23 * 8, 32 + 2 * 8 + 15 * 8, 24 + 3 * 8 + 16 * 8)
+
+
+def test_places_of_64_bits_stay_where_they_are_or_outside():
+    """Slots and offsets may be int64; those past 32 bits become none that there is."""
+    wide = torch.tensor([0, 5, -1, 1 << 31, 1 << 32, (1 << 32) + 5, -(1 << 32), 1 << 62])
+    got = trunk._int32("slots", wide)
+    most = 2 ** 31 - 1
+    assert got.dtype == torch.int32 and got.tolist() == [0, 5, -1, most, most, most, -1, most]

@@ -199,7 +199,7 @@ def _offsets(offsets, tokens):
 
 def _int32(name, t):
     _want(t.dtype in (torch.int32, torch.int64), "{} is {}, not int32", name, t.dtype)
-    t = t if t.dtype == torch.int32 else t.int()
+    t = t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).int()  # what is outside stays outside
     return t if t.is_contiguous() else t.contiguous()
 
 
