@@ -212,3 +212,15 @@ def test_places_of_64_bits_stay_where_they_are_or_outside():
     got = trunk._int32("slots", wide)
     most = 2 ** 31 - 1
     assert got.dtype == torch.int32 and got.tolist() == [0, 5, -1, most, most, most, -1, most]
+
+
+def test_places_that_are_no_tensors_are_refused():
+    x, w = bf16(6, 10), f32(10, 4)
+    for call in (lambda: trunk.scan(**scan_inputs(offsets=[0, 5])), lambda: trunk.conv(x, w, offsets=[0, 6]),
+                 lambda: trunk.conv_backward(x, x, w, offsets=(0, 6))):
+        with pytest.raises(trunk.TrunkError, match="offsets is no tensor"):
+            call()
+    for call in (lambda: trunk.scan_step(**scan_inputs(), states=f32(6, 4, 8, 6), slots=[0, 1, 2, 3, 4]),
+                 lambda: trunk.conv_step(x, w, bf16(6, 3, 10), slots=list(range(6)))):
+        with pytest.raises(trunk.TrunkError, match="slots is no tensor"):
+            call()

@@ -193,6 +193,7 @@ def _one_device(*tensors):
 def _offsets(offsets, tokens):
     if offsets is None:
         return None, 1
+    _want(isinstance(offsets, torch.Tensor), "offsets is no tensor")
     _want(offsets.dim() == 1 and offsets.numel() >= 2, "offsets has one place more than there are sequences, two at least")
     return _int32("offsets", offsets), offsets.numel() - 1
 
@@ -207,6 +208,7 @@ def _index(slots, rows, states):
     if slots is None:
         _want(states >= rows, "{} rows for {} states", rows, states)
         return None
+    _want(isinstance(slots, torch.Tensor), "slots is no tensor")
     _want(slots.shape == (rows,), "slots has shape {}, not {}", tuple(slots.shape), (rows,))
     return _int32("slots", slots)
 
