@@ -115,3 +115,24 @@ def test_offsets_past_32_bits_are_the_nearest_inside(dtype):
     c["offsets"] = x["offsets"]
     for a, b in zip(want, trunk.conv(**c)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("stride", [0, 8, -64])
+def test_one_row_has_no_stride(stride, dtype):
+    """From C: the strides of a call of one row are not looked at."""
+    x, m = scan_case(dtype, [1], 2, 1, 64, 64, initial=True)
+    dy, df = m(*x["x"].shape), m.f32(1, 2, 64, 64)
+    y, final = trunk.scan(**x)
+    grads = trunk.scan_backward(dy, **x, dfinal=df)
+    a, keep = trunk._scan_args(*(x[k] for k in ("x", "dt", "A", "B", "C", "D", "dt_bias", "offsets", "initial")))
+    a.x_stride = a.dt_stride = a.b_stride = a.c_stride = a.y_stride = stride
+    y2, final2 = torch.empty_like(y), torch.empty_like(final)
+    a.y, a.final = y2.data_ptr(), final2.data_ptr()
+    trunk._call("scan", a, 0)
+    assert torch.equal(y, y2) and torch.equal(final, final2)
+    got = trunk.ScanGrads(*(torch.empty_like(g) for g in grads))
+    a.dy, a.dfinal = dy.data_ptr(), df.data_ptr()
+    a.dx, a.ddt, a.dA, a.dB, a.dC, a.dD, a.ddt_bias, a.dinitial = (g.data_ptr() for g in got)
+    trunk._call("scan_backward", a, 0)
+    for one, two in zip(grads, got):
+        assert torch.equal(one, two)

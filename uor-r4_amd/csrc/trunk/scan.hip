@@ -376,11 +376,15 @@ Scan scan_of(const uor_trunk_scan_args *s, uint32_t size) {
   a.rows = Rows{s->offsets, s->tokens, s->seqs};
   a.heads = s->heads, a.groups = s->groups, a.dim = s->dim, a.state = s->state;
   a.size = size, a.pieces = pieces(s->tokens, s->seqs, size), a.later = s->tokens / size + 1, a.tiles = (s->dim + 31) / 32;
-  a.x_stride = s->x_stride, a.dt_stride = s->dt_stride, a.b_stride = s->b_stride, a.c_stride = s->c_stride, a.y_stride = s->y_stride;
+  // One row has no stride; chunks go by one all the same.
+  const int64_t inner = (int64_t)s->heads * s->dim, shared = (int64_t)s->groups * s->state;
+  const bool one = s->tokens <= 1;
+  a.x_stride = one ? inner : s->x_stride, a.dt_stride = one ? s->heads : s->dt_stride, a.y_stride = one ? inner : s->y_stride;
+  a.b_stride = one ? shared : s->b_stride, a.c_stride = one ? shared : s->c_stride;
   a.x = s->x, a.dt = s->dt, a.B = s->B, a.C = s->C, a.A = s->A, a.D = s->D, a.bias = s->dt_bias;
   a.initial = s->initial, a.y = s->y, a.final = s->final;
-  a.x_wide = wide(s->x, s->x_stride, s->dim), a.b_wide = wide(s->B, s->b_stride, s->state), a.c_wide = wide(s->C, s->c_stride, s->state);
-  a.y_wide = wide(s->y, s->y_stride, s->dim);
+  a.x_wide = wide(s->x, a.x_stride, s->dim), a.b_wide = wide(s->B, a.b_stride, s->state), a.c_wide = wide(s->C, a.c_stride, s->state);
+  a.y_wide = wide(s->y, a.y_stride, s->dim);
   a.state_wide = s->state % 4 == 0 && aligned16(s->initial, 0, 4) && aligned16(s->final, 0, 4);
   return a;
 }

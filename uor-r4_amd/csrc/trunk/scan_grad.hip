@@ -809,7 +809,7 @@ extern "C" int uor_trunk_scan_backward_async(const uor_trunk_scan_args *s, void 
   k.h = (float *)(base + p.h), k.sums = (double *)(base + p.sums);
   k.dBparts = (float *)(base + p.dB), k.dCparts = (float *)(base + p.dC);
   k.dx = s->dx, k.ddt = s->ddt, k.dB = s->dB, k.dC = s->dC, k.dA = s->dA, k.dD = s->dD, k.dbias = s->ddt_bias, k.dinitial = s->dinitial;
-  k.dy_wide = wide_rows(s->dy, s->y_stride, s->dim, size);
+  k.dy_wide = wide_rows(s->dy, k.s.y_stride, s->dim, size);
   k.dx_wide = aligned16(s->dx, 0, size) && s->dim * size % 16 == 0;
   k.shared_wide = aligned16(s->dB, 0, size) && aligned16(s->dC, 0, size) && s->state % 4 == 0;
   k.mid_wide = s->state % 4 == 0;
