@@ -119,3 +119,73 @@ def test_states_reach_the_gradients_in_32_bits():
     assert torch.equal(got.dx[:, 0].cpu(), goal.to(BF16).t())  # B_s is one at place s: dx[s] = D g[:, s]
     got = gradient(one_hot, none, step, none, none, initial=goal.float()[None, None])
     assert torch.equal(got.dC[:, 0].cpu(), goal.to(BF16))      # dy_t is one at value t: dC[t] = h[t, :]
+
+
+# ---------------------------------------------------------------------------------------------
+# The activation's tails. In 32 bits e^-v is off by at most 4 x 2^-24 of itself (the exponential's and its
+# argument's last bits, and their product), the sum and the reciprocal by 2 x 2^-24, and each product
+# after by 2^-24: under 16 x 2^-24 of the value itself, however small it is.
+SIGMOID = 16 * 2.0 ** -24
+
+
+def tails():
+    return torch.cat([torch.linspace(-86, 86, 4001), torch.linspace(-2, 2, 95)]).float()
+
+
+def relative(got, want, unit):
+    off = (got.cpu().double() - want).abs()
+    bad = ~(off <= unit * want.abs())
+    assert not bad.any(), (int(bad.sum()), float((off / want.abs())[bad].max() * 2 ** 24))
+
+
+def test_silu_keeps_its_bits_for_negative_values():
+    """One tap of one: y = v sigmoid(v), as the convolution computes it and its step."""
+    v = tails()
+    want = v.double() / (1 + torch.exp(-v.double()))
+    w = torch.ones(v.numel(), 1)
+    y, _ = trunk.conv(*gpu(v[None], w))
+    relative(y[0], want, SIGMOID)
+    y = trunk.conv_step(*gpu(v[None], w), torch.zeros(1, 0, v.numel()).cuda())
+    relative(y[0], want, SIGMOID)
+
+
+def test_silu_slopes_keep_their_bits_for_negative_values():
+    """sigmoid(v) (1 + v sigmoid(-v)), but where its two terms cancel: there, relative to them."""
+    v = tails()
+    wide = v.double()
+    s = 1 / (1 + torch.exp(-wide))
+    want = s * (1 + wide * (1 - s))
+    size = s * (1 + wide.abs() * (1 - s))
+    got = trunk.conv_backward(*gpu(torch.ones(1, v.numel()), v[None], torch.ones(v.numel(), 1)))
+    off = (got.dx[0].cpu().double() - want).abs()
+    assert not (off > SIGMOID * size).any(), float((off / size).max() * 2 ** 24)
+
+
+def test_gates_keep_their_bits_for_negative_values():
+    """Rows of one value: with a large eps the norm is a factor that is known."""
+    v = tails()
+    rows, one = v[:, None].contiguous(), torch.ones(v.numel(), 1)
+    wide = v.double()
+    gated = wide / (1 + torch.exp(-wide))
+    want = gated / torch.sqrt(gated * gated + 1e12)
+    r, _ = trunk.norms(None, *gpu(one), gate=rows.cuda(), eps=1e12)
+    whole = want.abs() >= 2.0 ** -126  # numbers below have fewer bits, whoever computes them
+    assert whole.sum() > 3500
+    relative(r[:, 0].cpu()[whole], want[whole], 2 * SIGMOID)
+
+
+def test_step_slopes_keep_their_bits_for_negative_steps():
+    """ddt = (x . g B) sigmoid(dt) with a decay of one, for steps down to e^-80."""
+    v = tails()
+    n = v.numel()
+    one = torch.ones(n, 1, 1)
+    got = trunk.scan_backward(*gpu(torch.zeros(n, 1, 1), one, v[:, None].contiguous(), torch.zeros(1), one, torch.zeros(n, 1, 1)),
+                              dfinal=torch.ones(1, 1, 1, 1).cuda())
+    relative(got.ddt[:, 0], 1 / (1 + torch.exp(-v.double())), 2 * SIGMOID)
+
+
+def test_silu_of_infinities():
+    v = torch.tensor([[float("inf"), float("-inf"), float("nan"), 200.0, -200.0, 0.0]])
+    y, _ = trunk.conv(*gpu(v, torch.ones(6, 1)))
+    y = y[0].tolist()
+    assert y[0] == float("inf") and y[2] != y[2] and y[3] == 200.0 and abs(y[4]) < 1e-34 and y[5] == 0.0

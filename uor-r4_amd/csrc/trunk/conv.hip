@@ -119,10 +119,10 @@ __device__ __forceinline__ Some<E> weighted(const Some<E> *rows, const Some<E> (
   for (int k = 0; k < TAPS; k++) v = __builtin_elementwise_fma(rows[k], w[k], v);  // one rounding in every form
   return v;
 }
-template <int E>
+template <class T, int E>
 __device__ __forceinline__ Some<E> silu(Some<E> v) {
 #pragma unroll
-  for (int e = 0; e < E; e++) v[e] *= sigmoid(v[e]);
+  for (int e = 0; e < E; e++) v[e] *= sigmoid_of<T>(v[e]);
   return v;
 }
 
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 3) void conv_rows(Conv a) {
 #pragma unroll
     for (int k = 0; k < kRowBatch; k++) {
       Some<E> v = weighted<TAPS, E>(rows + k, w, bias);
-      if (a.silu) v = silu<E>(v);
+      if (a.silu) v = silu<T, E>(v);
       if (k < (int)left) put_some<T, WIDE, E>((T *)a.y + (first + k) * a.y_stride, c, a.channels, v);
     }
     if (first + kRowBatch < at.end) {
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kGradThreads, 3) void conv_grad_rows(Conv a) {
             const Some<E> v = weighted<TAPS, E>(rows + b, w, bias);
 #pragma unroll
             for (int e = 0; e < E; e++) {
-              const float s = sigmoid(v[e]);
+              const float s = sigmoid_of<T>(v[e]);
               g[e] *= s * fmaf(v[e], 1.0f - s, 1.0f);
             }
           }
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void conv_step(Conv a) {
   rows[TAPS - 1] = row_some<T, WIDE, E>(a.x, row * a.x_stride, c, a.channels);
   taps_of<TAPS, WIDE, E>(a, c, w, bias);
   Some<E> v = weighted<TAPS, E>(rows, w, bias);
-  if (a.silu) v = silu<E>(v);
+  if (a.silu) v = silu<T, E>(v);
   put_some<T, WIDE, E>(y, c, a.channels, v);
 #pragma unroll
   for (int k = 0; k < TAPS - 1; k++) put_some<T, WIDE, E>(state + k * a.channels, c, a.channels, rows[k + 1]);

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_rows(Norms a) {
       if (a.gate) {
         const f32x8 z = values<T>(a.gate, row * a.gate_stride, there, c, a.width);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[i][e] *= z[e] * sigmoid(z[e]);
+        for (int e = 0; e < 8; e++) v[i][e] *= z[e] * sigmoid_of<T>(z[e]);
       }
     }
     if (a.out) {
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
       v[i] = u[i];
       if (a.gate) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[i][e] *= z[i][e] * sigmoid(z[i][e]);
+        for (int e = 0; e < 8; e++) v[i][e] *= z[i][e] * sigmoid_of<T>(z[i][e]);
       }
     }
     if (a.out) {
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norms_grad_rows(Norms a) {
         f32x8 dz;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float s = sigmoid(z[i][e]);
+          const float s = sigmoid_of<T>(z[i][e]);
           dz[e] = dv[e] * u[i][e] * s * (1.0f + z[i][e] * (1.0f - s));
           dv[e] *= z[i][e] * s;
         }
