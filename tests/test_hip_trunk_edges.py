@@ -136,3 +136,38 @@ def test_one_row_has_no_stride(stride, dtype):
     trunk._call("scan_backward", a, 0)
     for one, two in zip(grads, got):
         assert torch.equal(one, two)
+
+
+# ---------------------------------------------------------------------------------------------
+# Gradients of pieces of several chunks: states kept between them, the walk along a piece and back.
+
+
+LONG = [
+    # lengths, heads, groups, dim, state, chunks that the longest piece has
+    ([450, 449, 320, 193, 192, 129, 128, 65, 64, 63, 0, 1, 130] + [45] * 64, 16, 2, 40, 72, 3),
+    ([1300, 640, 641, 577, 576, 449, 193, 129, 128, 0, 1] + [130] * 38, 64, 8, 8, 16, 9),
+    ([250, 0, 193] + [37] * 125, 16, 16, 5, 33, 1),
+]
+
+
+def kept_bytes(x):
+    """What the states of all chunks take in a gradient's scratch memory."""
+    rows, heads, dim = x["x"].shape
+    state = x["B"].shape[2]
+    parts, padded = (1 if dim <= 32 else 2 if dim <= 64 else 4), (32 if state <= 32 else 64 if state <= 64 else 128)
+    return (rows // 64 + 1) * heads * parts * padded * 32 * 4
+
+
+@pytest.mark.parametrize("shape", LONG, ids=["3 chunks, state 72", "9 chunks", "64 rows, a group a head"])
+def test_scan_backward_of_pieces_of_several_chunks(shape, dtype):
+    lengths, heads, groups, dim, state, chunks = shape
+    x, m = scan_case(dtype, lengths, heads, groups, dim, state, initial=True, seed=21)
+    rows, units = sum(lengths), heads * (1 if dim <= 32 else 2)
+    assert len(lengths) * units >= 2048  # sequences enough that only those far over an even share are cut
+    assert -(-4 * -(-rows * units // 4096) // 64) >= chunks
+    args, _ = trunk._scan_args(*(x[k] for k in ("x", "dt", "A", "B", "C", "D", "dt_bias", "offsets", "initial")))
+    got = trunk.lib().uor_trunk_scan_backward_workspace_bytes(args)
+    if chunks >= 9:
+        assert got >= kept_bytes(x)  # more than all else together: pieces are of three chunks or more
+    check_scan(x, dtype)
+    check_scan_backward(x, m, dtype)
