@@ -224,3 +224,24 @@ def test_places_that_are_no_tensors_are_refused():
                  lambda: trunk.conv_step(x, w, bf16(6, 3, 10), slots=list(range(6)))):
         with pytest.raises(trunk.TrunkError, match="slots is no tensor"):
             call()
+
+
+@built
+@pytest.mark.parametrize("seqs,length,heads,dim,state", [(2048, 128, 8, 64, 64), (8192, 128, 8, 64, 64), (2048, 512, 32, 64, 128),
+                                                         (1, 65536, 16, 64, 128), (300, 509, 8, 64, 64)])
+def test_scratch_memory_of_cut_sequences_goes_by_rows_not_by_sequences(seqs, length, heads, dim, state):
+    """Scratch memory for states is that of pieces after a sequence's first: a place for each piece's rows of the
+    call, however many sequences there are, and in a gradient a state for each 64 rows and the sums of B's and C's."""
+    L, rows, inner = trunk.lib(), seqs * length, heads * dim
+    a = trunk.CScan(dtype=0, tokens=rows, seqs=seqs, heads=heads, groups=1, dim=dim, state=state, x_stride=inner, y_stride=inner,
+                    dt_stride=heads, b_stride=state, c_stride=state, x=16, dt=16, B=16, C=16, A=16, offsets=16)
+    one = heads * (dim * state * 4 + 8)  # a piece's states and decays
+    order = (rows // 64 + seqs + 2) * 8
+    # Pieces are as long as an even share of 4,096 wavefronts, and of at least 64 rows.
+    even = -(-rows * heads * (dim // 32) // 4096)
+    places = rows // max(64, even) + 1
+    assert 0 < L.uor_trunk_scan_workspace_bytes(C.byref(a)) <= places * one + order + 256
+    # dA, dD and ddt_bias of each piece; B's and C's gradients in f32 for each of a group's up to 4 x heads wavefronts' turns.
+    sums, kept = (places + seqs) * heads * 24, (rows // 64 + 1) * heads * dim * state * 4
+    parts = max(1, min(-(-512 // seqs), heads))
+    assert L.uor_trunk_scan_backward_workspace_bytes(C.byref(a)) <= 2 * places * one + kept + sums + order + 2 * parts * rows * state * 4 + 4096

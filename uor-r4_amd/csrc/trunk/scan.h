@@ -74,8 +74,8 @@ struct Scan {
   const float *initial;  // [seqs][heads][dim][state], or NULL
   void *y;
   float *final;
-  float *starts;         // [pieces][heads][dim][state]: where a piece begins, if sequences are cut; or NULL
-  double *totals;        // [pieces][heads]: log2 of a piece's whole decay
+  float *starts;         // [later][heads][dim][state]: where a sequence's pieces after its first begin, if any are cut; or NULL
+  double *totals;        // [later][heads]: log2 of a piece's whole decay
   uint32_t *order;       // the pieces, longest first: how many, and from the third on sequence and number; or NULL
   bool x_wide, b_wide, c_wide, y_wide, state_wide;
 };
@@ -102,6 +102,9 @@ __device__ __forceinline__ bool next_piece(const Scan &a, uint32_t &number, Piec
   number = at.start / a.size + at.seq + at.number;
   return true;
 }
+
+// The place of the piece that follows in the sequence; a piece's own is one less.
+__device__ __forceinline__ uint64_t next_place(const Scan &a, const Piece &at) { return (uint64_t)(at.start / a.size) + at.number; }
 
 // A join's blocks: by sequences, or by the places of later pieces, where there are fewer.
 __host__ __device__ inline uint32_t join_places(const Scan &a) { return a.rows.seqs < a.later ? a.rows.seqs : a.later; }

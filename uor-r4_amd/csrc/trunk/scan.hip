@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
   const uint64_t whole = (uint64_t)a.dim * a.state, part = (uint64_t)unit.p0 * a.state;
   f32x4 h[NT][PW];
   get_state<NT, PW>(h,
-                    at.number ? a.starts + ((uint64_t)unit.piece * a.heads + head) * whole + part
+                    at.number ? a.starts + ((next_place(a, at) - 1) * a.heads + head) * whole + part
                               : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + part : nullptr,
                     dim, a.state, a.state_wide);
 
@@ -211,32 +211,36 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
     put_state<NT, PW>(h, a.final + ((uint64_t)at.seq * a.heads + head) * whole + part, dim, a.state, a.state_wide);
 }
 
-// The pieces' end states into their start states, along each sequence that has more than one.
+// The end states of pieces from zeros into the start states of those after them, along each sequence that
+// has more than one.
 __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
   const uint32_t head = blockIdx.x % a.heads;
   uint32_t seq, n;
   if (!joined(a, blockIdx.x / a.heads, seq, n)) return;
-  const uint64_t base = a.rows.at(seq) / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
+  const uint64_t base = a.rows.at(seq) / a.size, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float h = a.initial ? a.initial[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = a.starts + (base * a.heads + head) * whole + e;
     const double *totals = a.totals + base * a.heads + head;
-    float own[kAhead], decay[kAhead];  // of the next pieces: what is read does not wait for the sums
-    const auto read = [&](uint32_t j) {
+    float own[kAhead], decay[kAhead], next[kAhead], next_decay[kAhead];
+    const auto read = [&](uint32_t j) {  // ahead: what is read waits neither for the sums nor for what is written
 #pragma unroll
       for (uint32_t k = 0; k < kAhead; k++) {
-        const uint32_t piece = j + k + 1 < n ? j + k : 0;
-        own[k] = at[piece * step];
-        decay[k] = (float)totals[(uint64_t)piece * a.heads];
+        const uint32_t place = j + k + 1 < n ? j + k : 0;
+        next[k] = at[place * step];
+        next_decay[k] = (float)totals[(uint64_t)place * a.heads];
       }
     };
-    for (uint32_t j = 0; j < n; j += kAhead) {
-      read(j);
+    read(0);
+    for (uint32_t j = 0; j + 1 < n; j += kAhead) {
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; k++) own[k] = next[k], decay[k] = next_decay[k];
+      if (j + kAhead + 1 < n) read(j + kAhead);
 #pragma unroll
       for (uint32_t k = 0; k < kAhead; k++) {
-        if (j + k >= n) break;
-        if (j + k) at[(j + k) * step] = h;
+        if (j + k + 1 >= n) break;
         h = exp2_(decay[k]) * h + own[k];
+        at[(j + k) * step] = h;
       }
     }
   }
@@ -338,8 +342,9 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   // launch looks at 1,024 sequences at a time.
   p.ordered = s->seqs > 1 && s->seqs <= 8192 && waves > 3072 && s->tokens >= 32768;
   if (p.cut) {
-    p.totals = (n * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
-    p.bytes = p.totals + n * s->heads * sizeof(double);
+    const uint64_t later = s->tokens / p.size + 1;
+    p.totals = (later * s->heads * s->dim * s->state * 4 + 15) / 16 * 16;
+    p.bytes = p.totals + later * s->heads * sizeof(double);
   }
   if (p.ordered) {
     p.order = (p.bytes + 15) / 16 * 16;

@@ -40,7 +40,7 @@ struct Grad {
   const float *dfinal;
   uint32_t subs, parts; // a group's wavefronts are taken in so many turns, shared by so many blocks
   float *h;             // [tokens / 64 + 1][heads * tiles][NT * 2][64][4]: states before chunks
-  float *g_starts;      // like s.starts: the gradients at the pieces' ends
+  float *g_starts;      // like s.starts: the gradients at the starts of pieces after their sequence's first
   double *sums;         // [pieces][heads][3]: dA, dD, ddt_bias
   float *dBparts, *dCparts;  // [parts][tokens][groups][state], with more than one turn
   void *dx, *ddt, *dB, *dC;
@@ -188,9 +188,9 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
     const T *x = (const T *)a.x + head * a.dim + p0, *dy = (const T *)k.dy + head * a.dim + p0, *dt = (const T *)a.dt + head;
     const float A = a.A[head], skip = a.D ? a.D[head] : 0.0f, bias = a.bias ? a.bias[head] : 0.0f;
     const uint64_t cell = (uint64_t)p0 * a.state;
-    const float *start = at.number ? a.starts + ((uint64_t)number * a.heads + head) * whole + cell
+    const float *start = at.number ? a.starts + ((next_place(a, at) - 1) * a.heads + head) * whole + cell
                                    : a.initial ? a.initial + ((uint64_t)at.seq * a.heads + head) * whole + cell : nullptr;
-    const float *finish = at.end != at.stop ? k.g_starts + ((uint64_t)number * a.heads + head) * whole + cell
+    const float *finish = at.end != at.stop ? k.g_starts + (next_place(a, at) * a.heads + head) * whole + cell
                                             : k.dfinal ? k.dfinal + ((uint64_t)at.seq * a.heads + head) * whole + cell : nullptr;
     // Where the state before the piece's j-th chunk is kept.
     const auto kept = [&](uint32_t j) {
@@ -660,31 +660,37 @@ __global__ __launch_bounds__(1024) void grad_sums(Grad k) {
   if (k.dbias) k.dbias[head] = (float)part[2][0];
 }
 
-// The gradients at the pieces' starts, of their own y, into those at their ends, from each cut
-// sequence's end.
+// The gradients at the starts of pieces after their sequence's first, from those of their own y, from each
+// cut sequence's end.
 __global__ __launch_bounds__(kThreads) void grad_join(Grad k) {
   const Scan &a = k.s;
   const uint32_t head = blockIdx.x % a.heads;
   uint32_t seq, n;
   if (!joined(a, blockIdx.x / a.heads, seq, n)) return;
-  const uint64_t base = a.rows.at(seq) / a.size + seq, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
+  const uint64_t base = a.rows.at(seq) / a.size, whole = (uint64_t)a.dim * a.state, step = a.heads * whole;
   for (uint64_t e = blockIdx.y * kThreads + threadIdx.x; e < whole; e += (uint64_t)gridDim.y * kThreads) {
     float g = k.dfinal ? k.dfinal[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = k.g_starts + (base * a.heads + head) * whole + e;
     const double *totals = a.totals + base * a.heads + head;
-    for (uint32_t j = 0; j < n; j += kAhead) {  // from the end
-      float own[kAhead], decay[kAhead];
+    float own[kAhead], decay[kAhead], next[kAhead], next_decay[kAhead];
+    const auto read = [&](uint32_t j) {  // ahead, from the end
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; i++) {
-        const uint32_t piece = j + i + 1 < n ? n - 1 - j - i : n - 1;
-        own[i] = at[piece * step];
-        decay[i] = (float)totals[(uint64_t)piece * a.heads];
+        const uint32_t place = j + i + 1 < n ? n - 2 - j - i : n - 2;
+        next[i] = at[place * step];
+        next_decay[i] = (float)totals[(uint64_t)place * a.heads];
       }
+    };
+    read(0);
+    for (uint32_t j = 0; j + 1 < n; j += kAhead) {
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; i++) own[i] = next[i], decay[i] = next_decay[i];
+      if (j + kAhead + 1 < n) read(j + kAhead);
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; i++) {
-        if (j + i >= n) break;
-        if (j + i) at[(n - 1 - j - i) * step] = g;
+        if (j + i + 1 >= n) break;
         g = exp2_(decay[i]) * g + own[i];
+        at[(n - 2 - j - i) * step] = g;
       }
     }
   }
@@ -724,12 +730,12 @@ Plan plan_of(const uor_trunk_scan_args *s) {
     return begin;
   };
   const bool cut = p.size < s->tokens;
-  const uint64_t starts = cut ? (uint64_t)p.pieces * s->heads * s->dim * s->state * 4 : 0;
+  const uint64_t later = cut ? s->tokens / p.size + 1 : 0, starts = later * s->heads * s->dim * s->state * 4;
   p.cut = take(starts), p.back = take(starts);
   // As in the scan; two wavefronts a SIMD, and each chunk takes several times as long.
   p.ordered = s->seqs > 1 && s->seqs <= 8192 && (uint64_t)p.pieces * s->groups * p.parts * p.waves > 2048 && s->tokens >= 16384;
   p.order = take(p.ordered ? ((uint64_t)p.pieces + 1) * 8 : 0);
-  p.totals = take(cut ? (uint64_t)p.pieces * s->heads * 8 : 0);
+  p.totals = take(later * s->heads * 8);
   // States are kept of chunks that have one before them and one after them in their piece.
   p.h = take(p.size > 2 * kChunk && s->tokens > 2 * kChunk ? ((uint64_t)s->tokens / kChunk + 1) * s->heads * tiles * n16 * 32 * 4 : 0);
   p.sums = take((uint64_t)p.pieces * s->heads * 3 * 8);

@@ -364,9 +364,10 @@ __device__ __forceinline__ Unit unit_of(const Scan &a, uint32_t parts) {
   return u;
 }
 
-// A piece's end state from zeros and its whole decay; a sequence's last piece needs neither. BACK: the
-// gradient at the state before a piece from that of y alone, with dy for x and C for B, along the
-// piece from its end: the sum of e^(l_t) dy_t (x) C_t.
+// A piece's end state from zeros and its whole decay, at the place of the piece after it; a sequence's last
+// piece needs neither. BACK, for the pieces after a sequence's first, at their own places: the gradient at
+// the state before a piece from that of y alone, with dy for x and C for B, along the piece from its end:
+// the sum of e^(l_t) dy_t (x) C_t.
 template <class T, int NT, int PW, int W, bool BACK>
 __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
   constexpr int kN = 16 * NT, kP = 16 * PW, kNp = pitch<T>(kN), kPp = pitch<T>(kP);
@@ -376,7 +377,6 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
   uint32_t seq, which, count;
   if (unit.piece >= a.later || !later_piece<true>(a.rows, unit.piece, a.size, seq, which, count)) return;
   const Piece at = piece_of(a.rows, seq, BACK ? which + 1 : which, a.size);
-  const uint32_t number = at.start / a.size + seq + at.number;  // its place among all pieces
   const int wave = threadIdx.x >> 6, lane0 = threadIdx.x & 63;
   const uint32_t head = unit.head;
   const T *x = (const T *)a.x + head * a.dim + unit.p0, *dt = (const T *)a.dt + head, *B = (const T *)a.B + unit.group * a.state;
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
     total += d.total;
   }
   if (unit.idle) return;
-  const uint64_t slot = (uint64_t)number * a.heads + head;
+  const uint64_t slot = (uint64_t)unit.piece * a.heads + head;
   put_state<NT, PW>(h, a.starts + slot * a.dim * a.state + (uint64_t)unit.p0 * a.state, dim, a.state, a.state_wide);
   if (lane0 == 0 && unit.p0 == 0) a.totals[slot] = total;
 }
