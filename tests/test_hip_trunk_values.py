@@ -189,3 +189,11 @@ def test_silu_of_infinities():
     y, _ = trunk.conv(*gpu(v, torch.ones(6, 1)))
     y = y[0].tolist()
     assert y[0] == float("inf") and y[2] != y[2] and y[3] == 200.0 and abs(y[4]) < 1e-34 and y[5] == 0.0
+
+
+def test_a_step_that_is_no_number_has_no_gradient():
+    one = torch.ones(1, 1, 1)
+    for dtype in (torch.float32, BF16):
+        got = trunk.scan_backward(*gpu(one.to(dtype), one.to(dtype), torch.full((1, 1), float("nan"), dtype=dtype), torch.zeros(1), one.to(dtype),
+                                       one.to(dtype)))
+        assert got.ddt.isnan().all() and got.dx.isnan().all() and not got.dC.isfinite().any()

@@ -39,10 +39,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // 1 / (1 + e^-v) to 2^-21 of it: what the rounding of v log2(e) leaves goes into the exponential, which
-// would be |v| 2^-24 of itself off without. Past +-87, where a float holds e^-v no more, as at 87; for no
-// number some number, as every use multiplies by what v is too.
+// would be |v| 2^-24 of itself off without. Past +-87, where a float holds e^-v no more, as at 87.
 __device__ __forceinline__ float sigmoid(float v) {
-  v = __builtin_amdgcn_fmed3f(v, -87.0f, 87.0f);
+  v = v < -87.0f ? -87.0f : v > 87.0f ? 87.0f : v;  // and NaN where v is
   const float t = v * -kLog2e, left = fmaf(v, -1.92596299e-8f, fmaf(v, -kLog2e, -t));
   const float e = exp2_(t);
   return __builtin_amdgcn_rcpf(1.0f + fmaf(e, left * 0.693147181f, e));
