@@ -24,6 +24,9 @@
  * state) are all bf16 or all f32; parameters (A, D, dt_bias, weight, bias, post, scale, pre), the
  * scan's states and the parameters' gradients are f32.
  *
+ * What is infinite or no number reaches the results that depend on it by these formulas and their
+ * gradients, as an infinity or NaN, and no others.
+ *
  * Every call takes device pointers, runs on `stream` (a hipStream_t) of `device` and allocates
  * nothing: where a call needs scratch memory, the caller passes at least *_workspace_bytes of it,
  * aligned to 16 bytes. Results do not depend on the order in which blocks run. The calls can be

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import trunk_cases as oracle
-from test_hip_trunk import CONV_UNIT, check_scan, check_scan_backward, conv_case, dtype, near, scan_case, trunk  # noqa: F401
+from test_hip_trunk import CONV_UNIT, check_scan, check_scan_backward, conv_case, dtype, near, scan_case, trunk, unit_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -171,3 +171,85 @@ def test_scan_backward_of_pieces_of_several_chunks(shape, dtype):
         assert got >= kept_bytes(x)  # more than all else together: pieces are of three chunks or more
     check_scan(x, dtype)
     check_scan_backward(x, m, dtype)
+
+
+# ---------------------------------------------------------------------------------------------
+# Values that are not finite: by the definition they reach some results, and no others.
+
+
+def same_where_finite(name, got, want, size, dtype, unit):
+    """got is finite exactly where the definition is, and near it there."""
+    there = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got).cpu(), there), (name, int((torch.isfinite(got).cpu() != there).sum()), int((~there).sum()))
+    near(name, got.cpu()[there], want[there], size[there], dtype, unit)
+
+
+def check_odd(x, dy, df, dtype):
+    dim, state = x["x"].shape[2], x["B"].shape[2]
+    unit = unit_of(dtype, 64 + state + 32)
+    for name, got, want, size in zip(("y", "final"), trunk.scan(**x), oracle.scan(**x), oracle.scan(**x, magnitude=True)):
+        same_where_finite(name, got, want, size, dtype if name == "y" else torch.float32, unit)
+    got = trunk.scan_backward(dy, **x, dfinal=df)
+    want = oracle.scan_backward(dy, **x, dfinal=df)
+    size = oracle.scan_backward(dy, **x, dfinal=df, magnitude=True)
+    unit = unit_of(dtype, 2 * (64 + dim + state + 32))
+    a = x["A"].cpu().double().abs()
+    later = torch.zeros_like(size["q"])
+    for s, e in oracle.bounds(x["offsets"], x["x"].shape[0]):
+        for t in range(s, e):
+            later[t] = torch.nan_to_num(size["q"][t:min(e, t + 64)], nan=0.0, posinf=0.0).sum(0)
+    size["ddt"] = size["ddt"] + a * later
+    size["dA"] = size["dA"] + (size["step"] * later).sum(0)
+    size["ddt_bias"] = size["ddt_bias"] + (a * later).sum(0)
+    for name in trunk.ScanGrads._fields:
+        if want[name] is None:
+            assert getattr(got, name) is None
+            continue
+        kind = dtype if name in ("dx", "ddt", "dB", "dC") else torch.float32
+        same_where_finite(name, getattr(got, name), want[name], size[name], kind, unit + (0 if kind == dtype == torch.bfloat16 else 64 * 2.0 ** -24))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("name", ["x", "dt", "B", "C", "dy", "initial", "dfinal", "A", "D", "dt_bias"])
+def test_what_is_not_finite_reaches_what_depends_on_it(name, value, dtype):
+    """One value of each input, at the ends and in the middle of chunks and of their tiles; the sequence
+    before and the one after, the other head and the other group have none."""
+    x, m = scan_case(dtype, [30, 150, 40], 4, 2, 40, 20, initial=True, seed=31)
+    dy, df = m(*x["x"].shape), m.f32(3, 4, 40, 20)
+    rows = [30 + t for t in (0, 5, 37, 63, 64, 100, 149)]
+    for row in rows if name in ("x", "dt", "B", "C", "dy") else [1]:
+        bad = {**x, "dy": dy, "dfinal": df}
+        t = bad[name] = bad[name].clone()
+        place = (row, 2, 7, 11)[:t.dim()] if t.dim() > 1 else (2,)
+        if name in ("B", "C"):
+            place = (row, 1, 7)
+        t[place] = value
+        if name == "A":
+            t[2] = -abs(value)
+        check_odd({k: v for k, v in bad.items() if k not in ("dy", "dfinal")}, bad["dy"], bad["dfinal"], dtype)
+
+
+@pytest.mark.parametrize("name", ["x", "dt", "B", "C", "dy"])
+def test_what_is_not_finite_in_long_and_cut_sequences(name, dtype):
+    """Several odd rows, in sequences of several pieces, and without states before and after."""
+    x, m = scan_case(dtype, [3, 700, 64], 8, 1, 32, 33, seed=32)
+    dy = m(*x["x"].shape)
+    bad = {**x, "dy": dy}
+    t = bad[name] = bad[name].clone()
+    for row, value in ((3 + 200, float("nan")), (3 + 201, float("inf")), (3 + 333, -float("inf")), (3 + 699, float("nan"))):
+        t[(row, 0, 3)[:t.dim()] if name != "dt" else (row, 5)] = value
+    dy = bad.pop("dy")
+    check_odd(bad, dy, None, dtype)
+
+
+@pytest.mark.parametrize("name", ["x", "dt", "B", "C", "dy"])
+def test_what_is_not_finite_in_pieces_of_several_chunks(name, dtype):
+    x, m = scan_case(dtype, [450, 320, 130] + [60] * 32, 64, 8, 8, 16, initial=True, seed=33)
+    dy, df = m(*x["x"].shape), m.f32(35, 64, 8, 16)
+    assert 35 * 64 >= 2048 and -(-4 * -(-x["x"].shape[0] * 64 // 4096) // 64) >= 3
+    bad = {**x, "dy": dy}
+    t = bad[name] = bad[name].clone()
+    for row in (70, 450 + 200, 450 + 320 + 129):
+        t[(row, 1, 3)[:t.dim()]] = float("nan")
+    dy = bad.pop("dy")
+    check_odd(bad, dy, df, dtype)

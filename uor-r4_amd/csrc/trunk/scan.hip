@@ -92,7 +92,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_rows(Scan a) {
     nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
     nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
     const bool odd = __any(nextX.put(lane, sX, a.x_stride, dim, a.x_wide));
-    const Decay d = steps_of(lane, s, raw, first + lane < end, A, bias);
+    const Decay d = steps_of(lane, s, row_of(raw, first + lane < end, A, bias));
     __syncthreads();
     if (unit.idle) {
       fetch(end);

@@ -144,11 +144,42 @@ __device__ __forceinline__ void hold(f32x4 (&h)[NT][2]) {
   for (int n = 0; n < NT; n++) asm volatile("" : "+v"(h[n][0]), "+v"(h[n][1]));
 }
 
+// Values that are infinite or no number (odd) meet zeros in the products: of rows that come before or after,
+// of the parts of the unit matrix. What is not finite by the definition then is none here, but more may
+// be: in the chunk, rows on the other side. A piece where that was (some ddt of it is not finite) is taken once more by
+// a second form, whose products leave such values out, and which then writes NaN where they reach:
+//   dx_s: an odd dy_t of the same value or any C_t of t >= s, B_s, a step's NaN after s, D_s;
+//   dB_s: an odd dy_t, the same value of C_t of t >= s, x_s, a step's NaN after s, D_s, the same value of g;
+//   dC_t: an odd x_s or D_s, the same value of B_s of s <= t, dy_t;
+//   da_u: an odd dy_t or C_t of t >= u, x_s, B_s or D_s of s < u, any of g, any step's NaN.
+// Where all is finite that is one launch more: 37 f32 sequences of up to 301 take 72 us where they took 68,
+// 2,048 bf16 sequences of 128 1,087 where they took 1,075.
+template <bool ODD, class V>
+__device__ __forceinline__ V clean(V v) {
+  if constexpr (ODD) {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (!finite((float)v[e])) v[e] = 0.0f;
+  }
+  return v;
+}
+constexpr float kNone = __builtin_nanf("");
+// The odd rows of a wavefront's chunk, a bit a row. `decays`: those whose decay is odd, `steps`: D_t.
+struct Odd {
+  uint64_t dy, x, B, C, steps, decays;
+  bool g;
+};
+__device__ __forceinline__ bool from_row(uint64_t rows, int s) { return rows >> s; }
+__device__ __forceinline__ bool after_row(uint64_t rows, int s) { return rows >> s >> 1; }
+__device__ __forceinline__ bool before_row(uint64_t rows, int s) { return rows & ((1ull << s) - 1); }
+__device__ __forceinline__ bool up_to_row(uint64_t rows, int s) { return rows << (63 - s); }
+__device__ __forceinline__ bool at_row(uint64_t rows, int s) { return rows >> s & 1; }
+
 // Wavefronts that a SIMD is to hold: with states of more than 64 a wavefront needs all its registers.
 template <int NT, int W>
 constexpr int kHeld = NT > 4 || W == 1 ? 1 : 2;
 
-template <class T, int NT, int W>
+template <class T, int NT, int W, bool ODD>
 __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   constexpr int kN = 16 * NT, kP = 32, kNp = pitch<T>(kN), kPp = pitch<T>(kP), G = 2;
   __shared__ __align__(16) T sB[kChunk * kNp], sC[kChunk * kNp], sYs[W][kChunk * kPp];
@@ -160,10 +191,12 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   __shared__ float sDa[W][kChunk], sDirect[W][kChunk], sDiag[W];
   const Scan &a = k.s;
   const uint32_t share = a.heads / a.groups, units = share * a.tiles;
-  clear_unowned(a.rows, (T *)k.dx, (int64_t)a.heads * a.dim, a.heads * a.dim);
-  clear_unowned(a.rows, (T *)k.ddt, a.heads, a.heads);
-  clear_unowned(a.rows, (T *)k.dB, (int64_t)a.groups * a.state, a.groups * a.state);
-  clear_unowned(a.rows, (T *)k.dC, (int64_t)a.groups * a.state, a.groups * a.state);
+  if constexpr (!ODD) {
+    clear_unowned(a.rows, (T *)k.dx, (int64_t)a.heads * a.dim, a.heads * a.dim);
+    clear_unowned(a.rows, (T *)k.ddt, a.heads, a.heads);
+    clear_unowned(a.rows, (T *)k.dB, (int64_t)a.groups * a.state, a.groups * a.state);
+    clear_unowned(a.rows, (T *)k.dC, (int64_t)a.groups * a.state, a.groups * a.state);
+  }
   uint32_t number, block;
   place_of(blockIdx.x, a.groups * k.parts, number, block);
   Piece at;
@@ -176,6 +209,12 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   T *sY = sYs[wave];
   GradSteps &s = steps[wave];
   const uint32_t sub0 = k.subs * part / k.parts, sub1 = k.subs * (part + 1) / k.parts;
+  if constexpr (ODD) {  // of the block's own heads, whose sums the block itself writes anew
+    bool any = false;
+    for (uint32_t unit = sub0 * W; unit < sub1 * W && unit < units; unit += a.tiles)
+      any |= !(fabs(k.sums[((uint64_t)number * a.heads + group * share + unit / a.tiles) * 3 + 2]) < __builtin_inf());
+    if (!any) return;
+  }
 
 #pragma unroll 1
   for (uint32_t sub = sub0; sub < sub1; sub++) {
@@ -218,7 +257,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         __syncthreads();
         nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
         nextX.put(lane, sY, a.x_stride, dim, a.x_wide && dim);
-        const Decay d = steps_of(lane, s, raw, true, A, bias);
+        const Decay d = steps_of(lane, s, row_of(raw, true, A, bias));
         __syncthreads();
         fetch(j + 1);
         if (idle) continue;
@@ -259,12 +298,20 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
       __syncthreads();
       const float raw_now = raw;
       Decay d;
+      Odd odd = {};
       {
         const int lane = anew(lane0), thread = wave * 64 + lane;
         nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
         nextC.put(thread, sC, a.c_stride, a.state, a.c_wide);
         nextY.put(lane, sY, a.y_stride, dim, k.dy_wide && dim);
-        d = steps_of(lane, s, raw, first + lane < end, A, bias);
+        Row row = row_of(raw, first + lane < end, A, bias);
+        if constexpr (ODD) {
+          odd.steps = __ballot(!finite(row.step));
+          odd.decays = __ballot(!(fabs(row.log) < __builtin_inf()));
+          row.step = finite(row.step) ? row.step : 0.0f;
+          row.log = fabs(row.log) < __builtin_inf() ? row.log : 0.0;
+        }
+        d = steps_of(lane, s, row);
         if (!idle && j + 1 < chunks) {
           if (j) {
             const float *from = kept(j) + lane * 4;
@@ -278,6 +325,24 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         }
       }
       __syncthreads();
+      if constexpr (ODD) {
+        const int lane = anew(lane0);
+        bool dy_odd = false, x_odd = false, B_odd = false, C_odd = false, g_odd = false;
+        for (uint32_t p = 0; p < dim; p++) {
+          dy_odd |= !finite((float)sY[lane * kPp + p]);
+          x_odd |= first + lane < end && !finite((float)x[(int64_t)(first + lane) * a.x_stride + p]);
+        }
+        for (uint32_t n = 0; n < a.state; n++) {
+          B_odd |= !finite((float)sB[lane * kNp + n]);
+          C_odd |= !finite((float)sC[lane * kNp + n]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) g_odd |= !finite(g[n][0][r]) || !finite(g[n][1][r]);
+        odd.dy = __ballot(dy_odd), odd.x = __ballot(x_odd), odd.B = __ballot(B_odd), odd.C = __ballot(C_odd);
+        odd.g = __any(has_g && g_odd);
+      }
 
       // Rows s by pairs of tiles, and for each the rows t of the pair after and of its own: (1, 1),
       // (0, 1), (0, 0). accB and dx are the rows s', accC the rows t's. One copy of the code serves all
@@ -304,7 +369,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             const uint32_t pitch = (uint32_t)a.x_stride * sizeof(T), bytes = (end - first - 1) * pitch + dim * (uint32_t)sizeof(T);
             const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(x + (int64_t)first * a.x_stride), 0, (int)bytes, 0x00020000);
 #pragma unroll
-            for (int w = 0; w < 2; w++) X[w] = load_eight<T>(from, (s0 + 16 * w) * pitch + 8 * q * (uint32_t)sizeof(T), 8 * q, dim);
+            for (int w = 0; w < 2; w++) X[w] = clean<ODD>(load_eight<T>(from, (s0 + 16 * w) * pitch + 8 * q * (uint32_t)sizeof(T), 8 * q, dim));
           } else {
             T *rows = (T *)sRed[wave];
 #pragma unroll 1
@@ -313,7 +378,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               *(V8<T> *)(rows + e) = load_some<T, 8>(x + (int64_t)row * a.x_stride, row < end, e % kP, dim);
             }
 #pragma unroll
-            for (int w = 0; w < 2; w++) X[w] = operand(rows + (w * 16 + i16) * kP, 8 * q);
+            for (int w = 0; w < 2; w++) X[w] = clean<ODD>(operand(rows + (w * 16 + i16) * kP, 8 * q));
           }
           if (!idle && has_g) {
             hold(g);
@@ -324,9 +389,14 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               for (int i = 0; i < 2; i++) gp[i] = Fine<T>::of(__builtin_shufflevector(g[2 * kk][i], g[2 * kk + 1][i], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
               for (int w = 0; w < 2; w++) {
-                const V8<T> b = operand(sB + (s0 + 16 * w) * kNp, 32 * kk + 8 * q);
+                const V8<T> b = clean<ODD>(operand(sB + (s0 + 16 * w) * kNp, 32 * kk + 8 * q));
 #pragma unroll
                 for (int i = 0; i < 2; i++) dx[w][i] = mul(gp[i], b, dx[w][i]);
+              }
+              if constexpr (ODD) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                  gp[i] = Fine<T>::of(clean<true>(__builtin_shufflevector(g[2 * kk][i], g[2 * kk + 1][i], 0, 1, 2, 3, 4, 5, 6, 7)));
               }
 #pragma unroll
               for (int half = 0; half < 2; half++) {
@@ -338,6 +408,13 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
                 const auto gt = Fine<T>::of(turned);
 #pragma unroll
                 for (int w = 0; w < 2; w++) accB[w][n] = mul(gt, X[w], accB[w][n]);
+                if constexpr (ODD) {
+#pragma unroll
+                  for (int r = 0; r < 4; r++) {
+                    const float none = row_sum(finite(g[n][0][r]) && finite(g[n][1][r]) ? 0.0f : kNone);
+                    accB[0][n][r] += none, accB[1][n][r] += none;
+                  }
+                }
               }
               __builtin_amdgcn_sched_barrier(0);
             }
@@ -364,7 +441,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             hold(h);
             V8<T> y[2];
 #pragma unroll
-            for (int v = 0; v < 2; v++) y[v] = operand(sY + (t0 + 16 * v) * kPp, 8 * q);
+            for (int v = 0; v < 2; v++) y[v] = clean<ODD>(operand(sY + (t0 + 16 * v) * kPp, 8 * q));
 #pragma unroll
             for (int n = 0; n < NT; n++) {
               const auto hp = Fine<T>::of(__builtin_shufflevector(h[n][0], h[n][1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -377,7 +454,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               float through = 0.0f;
 #pragma unroll
               for (int kk = 0; kk < NT / 2; kk++)
-                through += dot(widen<T>(operand(sC + t * kNp, 32 * kk + 8 * q)),
+                through += dot(widen<T>(clean<ODD>(operand(sC + t * kNp, 32 * kk + 8 * q))),
                                __builtin_shufflevector(accC[v][2 * kk], accC[v][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7));
               through = column_sum(through);
               if (q == 0) sSum[wave][0][t] = through;
@@ -398,7 +475,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             const float step = s.step[mine], to_end = s.w[mine];
             V8<T> b[NT / 2];
 #pragma unroll
-            for (int kk = 0; kk < NT / 2; kk++) b[kk] = operand(sB + mine * kNp, 32 * kk + 8 * q);
+            for (int kk = 0; kk < NT / 2; kk++) b[kk] = clean<ODD>(operand(sB + mine * kNp, 32 * kk + 8 * q));
             f32x4 M[2], z[2];
 #pragma unroll
             for (int v = 0; v < 2; v++) {
@@ -406,8 +483,8 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
               if (v < w && sp == tp) continue;
               f32x4 S = {0, 0, 0, 0};
 #pragma unroll
-              for (int kk = 0; kk < NT / 2; kk++) S = Mma<T>::mul(operand(sC + (t0 + 16 * v) * kNp, 32 * kk + 8 * q), b[kk], S);
-              const f32x4 Wt = Mma<T>::mul(operand(sY + (t0 + 16 * v) * kPp, 8 * q), X[w], f32x4{0, 0, 0, 0});
+              for (int kk = 0; kk < NT / 2; kk++) S = Mma<T>::mul(clean<ODD>(operand(sC + (t0 + 16 * v) * kNp, 32 * kk + 8 * q)), b[kk], S);
+              const f32x4 Wt = Mma<T>::mul(clean<ODD>(operand(sY + (t0 + 16 * v) * kPp, 8 * q)), X[w], f32x4{0, 0, 0, 0});
               const int t4 = 32 * tp + 16 * v + 4 * q;
               if (v > w || sp != tp) {
                 // Tiles 2 and 1 are next to each other, and so are those of one pair.
@@ -448,7 +525,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             }
             const auto m = Fine<T>::of(__builtin_shufflevector(M[0], M[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (int i = 0; i < 2; i++) dx[w][i] = mul(column<T, kPp>(lane, sY, 32 * tp, i), m, dx[w][i]);
+            for (int i = 0; i < 2; i++) dx[w][i] = mul(clean<ODD>(column<T, kPp>(lane, sY, 32 * tp, i)), m, dx[w][i]);
             Z[w] = Fine<T>::of(__builtin_shufflevector(z[0], z[1], 0, 1, 2, 3, 4, 5, 6, 7));
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -462,7 +539,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             }
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            const V8<T> c = column<T, kNp>(lane, sC, 32 * tp, n);
+            const V8<T> c = clean<ODD>(column<T, kNp>(lane, sC, 32 * tp, n));
 #pragma unroll
             for (int w = 0; w < 2; w++) accB[w][n] = mul(c, Z[w], accB[w][n]);
           }
@@ -472,7 +549,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
           for (int v = 0; v < 2; v++) Zt[v] = turn(Z[0], Z[1], ones<T>(lane, v));
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            const V8<T> b = column<T, kNp>(lane, sB, 32 * sp, n);
+            const V8<T> b = clean<ODD>(column<T, kNp>(lane, sB, 32 * sp, n));
 #pragma unroll
             for (int v = 0; v < 2; v++) accC[v][n] = mul(b, Zt[v], accC[v][n]);
           }
@@ -485,8 +562,16 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
             const float below = column_sum(col[w]), in = column_sum(own[w]);
             if (q == 0) sSum[wave][4][mine] = below, sSum[wave][5][mine] = below + in;
             if (first + mine >= end) continue;
-            const f32x8 v = __builtin_shufflevector(dx[w][0], dx[w][1], 0, 1, 2, 3, 4, 5, 6, 7) * s.step[mine] +
-                            widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
+            f32x8 v = __builtin_shufflevector(dx[w][0], dx[w][1], 0, 1, 2, 3, 4, 5, 6, 7) * s.step[mine] +
+                      widen<T>(operand(sY + mine * kPp, 8 * q)) * skip;
+            if constexpr (ODD) {
+              const bool row = from_row(odd.C, mine) || at_row(odd.B | odd.steps, mine) || after_row(odd.decays, mine);
+              for (int e = 0; e < 8; e++) {
+                bool none = row;
+                for (int t = mine; t < kChunk; t++) none |= !finite((float)sY[t * kPp + 8 * q + e]);
+                v[e] = none ? kNone : v[e];
+              }
+            }
             const V8<T> o = __builtin_convertvector(v, V8<T>);
             T *to = (T *)k.dx + ((uint64_t)(first + mine) * a.heads + head) * a.dim + p0 + 8 * q;
             if (k.dx_wide) {  // whole pieces of eight values, or four of 32 bits
@@ -498,6 +583,24 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
                 if (8 * q + e < (int)dim) to[e] = o[e];
             }
           }
+        }
+
+        if constexpr (ODD) {
+          for (int w = 0; w < 2; w++)
+            for (int n = 0; n < NT; n++)
+              for (int r = 0; r < 4; r++) {
+                const int s_ = s0 + 16 * w, t_ = t0 + 16 * w, c = place(n, 4 * q + r);
+                if (!idle && step_ != 1) {  // dB of these rows is whole
+                  bool none = at_row(odd.x | odd.steps, s_) || after_row(odd.decays, s_) || from_row(odd.dy, s_);
+                  for (int t = s_; t < kChunk; t++) none |= !finite((float)sC[t * kNp + c]);
+                  accB[w][n][r] = none ? kNone : accB[w][n][r];
+                }
+                if (!idle && step_ != 0) {  // and dC
+                  bool none = at_row(odd.dy, t_) || up_to_row(odd.x | odd.steps | odd.decays, t_);
+                  for (int s = 0; s <= t_; s++) none |= !finite((float)sB[s * kNp + c]);
+                  accC[w][n][r] = none ? kNone : accC[w][n][r];
+                }
+              }
         }
 
         // dB's and dC's sums over the block's wavefronts, of two tiles of rows, and out: turns after the
@@ -574,6 +677,11 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         sDirect[wave][lane] = there ? (float)r + sum[5][lane] : 0.0f;
         const float all = wave_sum(diag);
         if (lane == 0) sDiag[wave] = all;
+        if constexpr (ODD) {
+          if (from_row(odd.dy | odd.C, lane) || before_row(odd.x | odd.B | odd.steps, lane) || odd.decays || odd.g) sDa[wave][lane] = kNone;
+          if (from_row(odd.dy | odd.C, lane) || at_row(odd.x | odd.B, lane) || after_row(odd.decays, lane)) sDirect[wave][lane] = kNone;
+          if (lane == 0 && (odd.dy | odd.x)) sDiag[wave] = kNone;
+        }
       } else {
         sDa[wave][lane] = sDirect[wave][lane] = 0.0f;
         if (lane == 0) sDiag[wave] = 0.0f;
@@ -589,7 +697,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         if (lane == 0) sumD += (double)all;
         if (first + lane < end) {
           const float dstep = (direct + A * da) * sigmoid(raw_now + bias);
-          sumA += (double)(s.step[lane] * da);
+          sumA += (double)((ODD && at_row(odd.steps, lane) ? kNone : s.step[lane]) * da);
           sumBias += (double)dstep;
           ((T *)k.ddt)[(uint64_t)(first + lane) * a.heads + head] = (T)dstep;
         }
@@ -602,6 +710,10 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
 #pragma unroll
           for (int i = 0; i < 2; i++) ys[kk][i] = column<T, kPp>(lane, sY, 32 * kk, i);
         advance<T, NT, 2>(lane, g, ys, sC, s.u, d.from, d.whole);
+        if (ODD && odd.decays) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) g[n][0] = g[n][1] = f32x4{kNone, kNone, kNone, kNone};
+        }
       }
     }
     if (idle) continue;
@@ -763,7 +875,8 @@ int launch(const Grad &k, hipStream_t stream) {
     hipLaunchKernelGGL(grad_join, join, dim3(kThreads), 0, stream, k);
   }
   if (a.order) hipLaunchKernelGGL(scan_order, dim3(1), dim3(1024), 0, stream, a);
-  hipLaunchKernelGGL((grad_rows<T, NT, W>), dim3(grid_of(a.pieces, a.groups * k.parts)), dim3(64 * W), 0, stream, k);
+  hipLaunchKernelGGL((grad_rows<T, NT, W, false>), dim3(grid_of(a.pieces, a.groups * k.parts)), dim3(64 * W), 0, stream, k);
+  hipLaunchKernelGGL((grad_rows<T, NT, W, true>), dim3(grid_of(a.pieces, a.groups * k.parts)), dim3(64 * W), 0, stream, k);
   if (k.parts > 1 && a.rows.tokens) {
     const uint64_t n = (uint64_t)a.rows.tokens * a.groups * a.state;
     hipLaunchKernelGGL(grad_parts<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, stream, k);

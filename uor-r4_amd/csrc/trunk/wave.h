@@ -236,10 +236,23 @@ struct Decay {
   float c20, c30, c31;  // from the end of tile 0 to tile 2's start, ...
   double total;
 };
+// A row's step and the logarithm of its decay, nothing past the chunk's last row. -1e5 already leaves
+// nothing of what was before, and differences of such sums are numbers, where infinities' are none.
+struct Row {
+  float step;
+  double log;
+};
+__device__ __forceinline__ Row row_of(float raw, bool there, float A, float bias) {
+  Row r;
+  r.step = there ? softplus(raw + bias) : 0.0f;
+  r.log = there ? (double)r.step * (double)A * 1.4426950408889634 : 0.0;
+  r.log = r.log < -1e5 ? -1e5 : r.log;
+  return r;
+}
 template <class S>
-__device__ __forceinline__ Decay steps_of(int lane, S &s, float raw, bool there, float A, float bias) {
-  const float step = there ? softplus(raw + bias) : 0.0f;
-  const double l = running_sum(there ? (double)step * (double)A * 1.4426950408889634 : 0.0);
+__device__ __forceinline__ Decay steps_of(int lane, S &s, Row row) {
+  const float step = row.step;
+  const double l = running_sum(row.log);
   const double r1 = lane_of(l, 15), r2 = lane_of(l, 31), r3 = lane_of(l, 47), r4 = lane_of(l, 63);
   const double start = lane < 16 ? 0.0 : lane < 32 ? r1 : lane < 48 ? r2 : r3, end = lane < 16 ? r1 : lane < 32 ? r2 : lane < 48 ? r3 : r4;
   const float hi = (float)l;
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 2) void scan_ends(Scan a) {
     __syncthreads();
     nextB.put(thread, sB, a.b_stride, a.state, a.b_wide);
     nextX.put(lane, sXs[wave], a.x_stride, dim, a.x_wide);
-    const Decay d = steps_of(lane, steps[wave], raw, first + lane < end, A, bias);
+    const Decay d = steps_of(lane, steps[wave], row_of(raw, first + lane < end, A, bias));
     __syncthreads();
     fetch(i + 1);
     if (unit.idle) continue;
