@@ -10,8 +10,13 @@ one sequence. Rows before the first offset and from the last one on are no seque
 returned is 0 there, and nothing else depends on them. Where the inner axes of a tensor are not dense it is copied first. Errors raise
 ``TrunkError``; there is no fallback: a missing library or device raises.
 
-``*_backward`` computes the gradients from the call's own inputs; nothing is kept between calls.
-Results are the same each time, bit for bit.
+``scan``, ``conv`` and ``norms`` take part in autograd: where an input requires a gradient, the outputs
+have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which
+a program may call by itself (it is not differentiable). The steps update their states in place and have no gradient: going
+back through one raises. Nothing is kept between calls. Results are the same each time, bit for bit.
+
+A training step that is captured into a graph calls ``*_backward`` by itself, or has no eager graph of the
+same leaves alive meanwhile: torch would order their gradients after the other graph's stream.
 """
 
 from __future__ import annotations
@@ -232,6 +237,31 @@ def _make(like):
     return torch.empty_like(like) if like.is_contiguous() else torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
+def _tracked(tensors):
+    """Whether a gradient is wanted at one of them."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+class _Step(torch.autograd.Function):
+    """A step's outputs, of which there is no gradient."""
+
+    @staticmethod
+    def forward(ctx, name, call, *inputs):
+        ctx.name = name
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise TrunkError(f"{ctx.name} has no gradient: its states are updated in place")
+
+
+_changed = torch.autograd.graph.increment_version  # of states in place, for autograd to see
+
+
 # ---------------------------------------------------------------------------------------------
 # The scan.
 
@@ -263,6 +293,8 @@ def scan(x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, initial=None):
     groups, state), the skip D and the steps' bias (heads), from the states ``initial`` (sequences,
     heads, dim, state; zeros without). ``final`` are the states after each sequence's last row."""
     a, keep = _scan_args(x, dt, A, B, C, D, dt_bias, offsets, initial)
+    if _tracked(keep):
+        return _Scan.apply(x, dt, A, B, C, D, dt_bias, offsets, initial)
     index = _one_device(*keep)
     y, final = _make(x), torch.empty((a.seqs, a.heads, a.dim, a.state), dtype=torch.float32, device=x.device)
     a.y, a.final = _ptr(y), _ptr(final)
@@ -285,6 +317,24 @@ def scan_backward(dy, x, dt, A, B, C, *, D=None, dt_bias=None, offsets=None, ini
     return got
 
 
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, offsets, initial):
+        ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, offsets, initial)
+        ctx.set_materialize_grads(False)
+        return scan(x, dt, A, B, C, D=D, dt_bias=dt_bias, offsets=offsets, initial=initial)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal):
+        if dy is None and dfinal is None:
+            return (None,) * 9
+        x, dt, A, B, C, D, dt_bias, offsets, initial = ctx.saved_tensors
+        got = scan_backward(torch.zeros_like(x) if dy is None else dy, x, dt, A, B, C, D=D, dt_bias=dt_bias, offsets=offsets,
+                            initial=initial, dfinal=dfinal)
+        return got.dx, got.ddt, got.dA, got.dB, got.dC, got.dD, got.ddt_bias, None, got.dinitial
+
+
 def scan_step(x, dt, A, B, C, states, *, slots=None, D=None, dt_bias=None):
     """y (rows, heads, dim): one token a session. ``states`` (slots, heads, dim, state) float32 is
     updated in place; ``slots`` (int32) says which state each row has, no two alike. A row whose slot
@@ -293,11 +343,14 @@ def scan_step(x, dt, A, B, C, states, *, slots=None, D=None, dt_bias=None):
     inner = (a.heads, a.dim, a.state)
     _want(isinstance(states, torch.Tensor) and states.dtype == torch.float32 and states.dim() == 4 and states.shape[1:] == inner
           and states.is_contiguous(), "states is no dense float32 tensor of (slots, {}, {}, {})", *inner)
+    if _tracked((states, *keep)):
+        return _Step.apply("scan_step", lambda: scan_step(x, dt, A, B, C, states, slots=slots, D=D, dt_bias=dt_bias), states, *keep)
     slots = _index(slots, a.tokens, states.shape[0])
     index = _one_device(states, slots, *keep)
     y = _make(x)
     a.y, a.index, a.states, a.slots = _ptr(y), _ptr(slots), _ptr(states), states.shape[0]
     _call("scan_step", a, index)
+    _changed((states,))
     return y
 
 
@@ -327,6 +380,8 @@ def conv(x, weight, bias=None, *, offsets=None, initial=None, silu=True):
     rows of x (rows, channels), the rows before it from ``initial`` (sequences, taps - 1, channels;
     zeros without). ``final`` are each sequence's last taps - 1 rows, the next call's ``initial``."""
     a, keep = _conv_args(x, weight, bias, offsets, initial, silu)
+    if _tracked(keep):
+        return _Conv.apply(x, weight, bias, offsets, initial, silu)
     index = _one_device(*keep)
     y, final = _make(x), torch.empty((a.seqs, a.taps - 1, a.channels), dtype=x.dtype, device=x.device)
     a.y, a.final = _ptr(y), _ptr(final)
@@ -348,6 +403,25 @@ def conv_backward(dy, x, weight, bias=None, *, offsets=None, initial=None, dfina
     return got
 
 
+class _Conv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, offsets, initial, silu):
+        ctx.save_for_backward(x, weight, bias, offsets, initial)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return conv(x, weight, bias, offsets=offsets, initial=initial, silu=silu)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal):
+        if dy is None and dfinal is None:
+            return (None,) * 6
+        x, weight, bias, offsets, initial = ctx.saved_tensors
+        got = conv_backward(torch.zeros_like(x) if dy is None else dy, x, weight, bias, offsets=offsets, initial=initial, dfinal=dfinal,
+                            silu=ctx.silu)
+        return got.dx, got.dweight, got.dbias, None, got.dinitial, None
+
+
 def conv_step(x, weight, states, bias=None, *, slots=None, silu=True):
     """y (rows, channels): one token a session; ``states`` (slots, taps - 1, channels) of x's type is
     updated in place, ``slots`` as in ``scan_step``."""
@@ -355,11 +429,14 @@ def conv_step(x, weight, states, bias=None, *, slots=None, silu=True):
     inner = (a.taps - 1, a.channels)
     _want(isinstance(states, torch.Tensor) and states.dtype == x.dtype and states.dim() == 3 and states.shape[1:] == inner
           and states.is_contiguous(), "states is no dense {} tensor of (slots, {}, {})", x.dtype, *inner)
+    if _tracked((states, *keep)):
+        return _Step.apply("conv_step", lambda: conv_step(x, weight, states, bias, slots=slots, silu=silu), states, *keep)
     slots = _index(slots, a.tokens, states.shape[0])
     index = _one_device(states, slots, *keep)
     y = _make(x)
     a.y, a.index, a.states, a.slots = _ptr(y), _ptr(slots), _ptr(states), states.shape[0]
     _call("conv_step", a, index)
+    _changed((states,))
     return y
 
 
@@ -391,6 +468,9 @@ def norms(residual, out=None, *, gate=None, post=None, scale=None, pre=None, eps
     is only normed (residual' is the residual itself); without ``residual`` residual' is the normed
     block alone; without ``pre`` normed is None. ``gate``, ``post`` and ``scale`` are 1 without."""
     a, first, keep = _norms_args(residual, out, gate, post, scale, pre, eps)
+    if _tracked(keep):
+        residual_out, normed = _Norms.apply(residual, out, gate, post, scale, pre, eps)
+        return (residual if out is None else residual_out), normed
     index = _one_device(*keep)
     residual_out = residual if out is None else _make(first)
     normed = None if pre is None else _make(first)
@@ -413,3 +493,21 @@ def norms_backward(dresidual_out, dnormed, residual, out=None, *, gate=None, pos
     a.dresidual, a.dout, a.dgate, a.dpost, a.dscale, a.dpre = map(_ptr, got)
     _call("norms_backward", a, index)
     return got
+
+
+class _Norms(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, out, gate, post, scale, pre, eps):
+        ctx.save_for_backward(residual, out, gate, post, scale, pre)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        residual_out, normed = norms(residual, out, gate=gate, post=post, scale=scale, pre=pre, eps=eps)
+        return (None if out is None else residual_out), normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dresidual_out, dnormed):
+        if dresidual_out is None and dnormed is None:
+            return (None,) * 7
+        residual, out, gate, post, scale, pre = ctx.saved_tensors
+        return (*norms_backward(dresidual_out, dnormed, residual, out, gate=gate, post=post, scale=scale, pre=pre, eps=ctx.eps), None)
