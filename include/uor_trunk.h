@@ -15,10 +15,11 @@
  *             n = r' rsqrt(mean r'^2 + eps) pre.
  *
  * Rows are packed: sequence s owns rows offsets[s] .. offsets[s + 1] - 1 (int32 on the device,
- * ascending; values outside 0 .. tokens are taken as the nearest inside, so that no call reads or
- * writes past its arrays). A sequence may have no rows. Rows before offsets[0] and from offsets[seqs]
- * on are no sequence's: y, dx, ddt, dB and dC are zeros there, and no other output depends on them. Rows of x, dt, B, C and y lie `*_stride` values apart (of one row
- * the stride is not looked at) and are dense inside.
+ * ascending; values outside 0 .. tokens are taken as the nearest inside). Of offsets that do not ascend
+ * the results are not defined, but no call reads or writes past its arrays. A sequence may have no
+ * rows. Rows before offsets[0] and from offsets[seqs] on are no sequence's: y, dx, ddt, dB and dC are
+ * zeros there, and no other output depends on them. Rows of x, dt, B, C and y lie `*_stride` values
+ * apart (of one row the stride is not looked at) and are dense inside.
  *
  * Types: activations (x, dt, B, C, y, out, gate, residual and their gradients, the convolution's
  * state) are all bf16 or all f32; parameters (A, D, dt_bias, weight, bias, post, scale, pre), the

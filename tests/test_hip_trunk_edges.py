@@ -253,3 +253,52 @@ def test_what_is_not_finite_in_pieces_of_several_chunks(name, dtype):
         t[(row, 1, 3)[:t.dim()]] = float("nan")
     dy = bad.pop("dy")
     check_odd(bad, dy, df, dtype)
+
+
+# ---------------------------------------------------------------------------------------------
+# Offsets that do not ascend: no promise is made of the results, but nothing outside the arrays is written.
+
+
+@pytest.fixture
+def fenced(monkeypatch):
+    """Everything that a call allocates lies between two stretches of 64 KB that stay as they are."""
+    fences, edge, make = [], 1 << 16, torch.empty
+
+    def fence(shape, dtype, device):
+        shape = tuple(shape) if isinstance(shape, (tuple, list, torch.Size)) else (shape,)
+        size = 1
+        for s in shape:
+            size *= s
+        n = size * dtype.itemsize
+        whole = make(2 * edge + (n + 255) // 256 * 256, dtype=torch.uint8, device=device).fill_(0x5a)
+        fences.append((whole, n))
+        return whole[edge:edge + n].view(dtype).view(shape)
+
+    monkeypatch.setattr(torch, "empty", lambda *shape, dtype, device: fence(shape[0] if len(shape) == 1 else shape, dtype, device))
+    monkeypatch.setattr(torch, "empty_like", lambda t, memory_format=None: fence(t.shape, t.dtype, t.device))
+    yield lambda: [w for w, n in fences if bool((w[:edge] != 0x5a).any()) or bool((w[edge + n:] != 0x5a).any())]
+
+
+@pytest.mark.parametrize("rows", [130, 1500])
+@pytest.mark.parametrize("offsets", [[0, 50, 20, 90, 10, 130], [130, 0, 130, 0], [1 << 30, -7, 60, -(1 << 31), 1400], [90, 90, 10], [700, 0, 1500, 600, 1500]],
+                         ids=str)
+def test_offsets_that_do_not_ascend_write_nothing_outside(offsets, rows, dtype, fenced):
+    x, m = scan_case(dtype, [rows], 4, 2, 40, 20)
+    n = len(offsets) - 1
+    x["offsets"] = torch.tensor(offsets, dtype=torch.int32).cuda()
+    x["initial"] = m.f32(n, 4, 40, 20)
+    c, _ = conv_case(dtype, [rows], 24, 4, False)
+    c.update(offsets=x["offsets"], initial=m(n, 3, 24))
+    dy, df, dyc, dfc = m(rows, 4, 40), m.f32(n, 4, 40, 20), m(rows, 24), m(n, 3, 24)
+    kept = {k: v.clone() for k, v in (*x.items(), *((f"conv {k}", v) for k, v in c.items()))}
+    trunk.scan(**x)
+    trunk.scan_backward(dy, **x, dfinal=df)
+    trunk.conv(**c)
+    trunk.conv_backward(dyc, **c, dfinal=dfc)
+    torch.cuda.synchronize()
+    assert not fenced()
+    for k, v in kept.items():
+        assert torch.equal(v, c[k[5:]] if k.startswith("conv ") else x[k])
+    # And the next call is as any other.
+    x["offsets"], x["initial"] = oracle.offsets_of([rows]).cuda(), None
+    check_scan(x, dtype)
