@@ -211,9 +211,9 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
   const uint32_t sub0 = k.subs * part / k.parts, sub1 = k.subs * (part + 1) / k.parts;
   if constexpr (ODD) {  // of the block's own heads, whose sums the block itself writes anew
     bool any = false;
-    for (uint32_t unit = sub0 * W; unit < sub1 * W && unit < units; unit += a.tiles)
+    for (uint32_t unit = sub0 * W + lane0 * a.tiles; unit < sub1 * W && unit < units; unit += 64 * a.tiles)
       any |= !(fabs(k.sums[((uint64_t)number * a.heads + group * share + unit / a.tiles) * 3 + 2]) < __builtin_inf());
-    if (!any) return;
+    if (!__any(any)) return;  // each wavefront looks at all of them
   }
 
 #pragma unroll 1
@@ -844,7 +844,10 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   const bool cut = p.size < s->tokens;
   const uint64_t later = cut ? s->tokens / p.size + 1 : 0, starts = later * s->heads * s->dim * s->state * 4;
   p.cut = take(starts), p.back = take(starts);
-  // As in the scan; two wavefronts a SIMD, and each chunk takes several times as long.
+  // As in the scan; two wavefronts a SIMD, and each chunk takes several times as long. Without and with it:
+  // 520 sequences of up to 128 (2,080 wavefronts) 308 and 250 us, 520 of up to 64 (16,710 rows) 180 and 180,
+  // 2,000 of up to 20 303 and 277, 8,000 of up to 20 1,043 and 1,037; below the borders 300 of up to 200 would
+  // gain (292 and 248), 300 of up to 60 not (116 and 117).
   p.ordered = s->seqs > 1 && s->seqs <= 8192 && (uint64_t)p.pieces * s->groups * p.parts * p.waves > 2048 && s->tokens >= 16384;
   p.order = take(p.ordered ? ((uint64_t)p.pieces + 1) * 8 : 0);
   p.totals = take(later * s->heads * 8);
