@@ -7,15 +7,15 @@
 // wavefronts are of one group and share B and C; x is each wavefront's own.
 //
 // Rows are bound by instructions and by time, not by bytes or products: 300 bf16 prompts of up to 509,
-// 8 heads of 64 by a state of 64, take 82 us (91 with the launches around), of which their bytes would
-// take 41, the vector instructions 48 and the products 16. Two pairs of tiles of x a wavefront compute
+// 8 heads of 64 by a state of 64, take 90 us (98 with the launches around), of which their bytes would
+// take 41, the vector instructions 54 and the products 20. Two pairs of tiles of x a wavefront compute
 // scores and decays once for both, but leave half the wavefronts, two a SIMD instead of three: 130 us
 // against 112, before the longest went first.
 //
 // A sequence of many rows and few heads would run on few wavefronts. Such sequences are cut into
 // pieces: a first launch gives every piece its end state from zeros, a second joins them along the
 // sequence, and the main launch runs all pieces at once. One of 65,536 rows, 16 heads of 64 by 128:
-// 98 + 24 + 248 us.
+// 84 + 26 + 230 us.
 #include "wave.h"
 
 namespace trunk {
@@ -222,32 +222,26 @@ __global__ __launch_bounds__(kThreads) void scan_join(Scan a) {
     float h = a.initial ? a.initial[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = a.starts + (base * a.heads + head) * whole + e;
     const double *totals = a.totals + base * a.heads + head;
-    float own[kAhead], decay[kAhead], next[kAhead], next_decay[kAhead];
-    const auto read = [&](uint32_t j) {  // ahead: what is read waits neither for the sums nor for what is written
+    for (uint32_t j = 0; j < n; j += kAhead) {
+      float own[kAhead], decay[kAhead];  // of the next pieces: what is read does not wait for the sums
 #pragma unroll
       for (uint32_t k = 0; k < kAhead; k++) {
         const uint32_t place = j + k + 1 < n ? j + k : 0;
-        next[k] = at[place * step];
-        next_decay[k] = (float)totals[(uint64_t)place * a.heads];
+        own[k] = at[place * step];
+        decay[k] = (float)totals[(uint64_t)place * a.heads];
       }
-    };
-    read(0);
-    for (uint32_t j = 0; j + 1 < n; j += kAhead) {
-#pragma unroll
-      for (uint32_t k = 0; k < kAhead; k++) own[k] = next[k], decay[k] = next_decay[k];
-      if (j + kAhead + 1 < n) read(j + kAhead);
 #pragma unroll
       for (uint32_t k = 0; k < kAhead; k++) {
-        if (j + k + 1 >= n) break;
+        if (j + k >= n) break;
+        if (j + k) at[(j + k - 1) * step] = h;
         h = exp2_(decay[k]) * h + own[k];
-        at[(j + k) * step] = h;
       }
     }
   }
 }
 
 // The pieces by their chunks, the longest first, so that none begins when the others end: 300 prompts of
-// up to 509 take 116 us in their own order and 82 in this, and 5 for the order. Which of two alike comes
+// up to 509 take 129 us in their own order and 95 in this, 5 of them for the order. Which of two alike comes
 // first may differ from call to call; no result depends on it.
 __global__ __launch_bounds__(1024) void scan_order(Scan a) {
   constexpr uint32_t kBuckets = 64;
@@ -290,9 +284,9 @@ __global__ __launch_bounds__(1024) void scan_order(Scan a) {
 
 // How many rows a piece has: sequences are cut where they alone would leave the card idle. The grid
 // then has about 4,096 wavefronts, two for each place; pieces under `least` rows cost more to join
-// than they gain: one head over 9 prompts of 2,580 rows takes 122 us in pieces of 512 and 47 in pieces of
-// 128, gradients of 37 of up to 301 102 us in pieces of 128 and 67 in pieces of 64. Where there are sequences for every place only those are cut that would still run
-// when the others have long ended.
+// than they gain: one head over 9 bf16 prompts of 2,580 rows takes 69 us in pieces of 512 and 31 in pieces
+// of 128, f32 gradients of 37 of up to 301 102 us in pieces of 128 and 70 in pieces of 64. Where there are
+// sequences for every place only those are cut that would still run when the others have long ended.
 uint32_t piece_rows(uint32_t tokens, uint32_t seqs, uint32_t units, uint32_t least) {
   const uint64_t even = ((uint64_t)tokens * units + 4095) / 4096, want = (uint64_t)seqs * units < 2048 ? even : 4 * even;
   const uint64_t size = (want < least ? least : want) + kChunk - 1;
@@ -339,7 +333,11 @@ Plan plan_of(const uor_trunk_scan_args *s) {
   p.cut = p.size < s->tokens;
   const uint64_t n = pieces(s->tokens, s->seqs, p.size), waves = n * s->heads * ((s->dim + 31) / 32);
   // One launch more, where more wavefronts are wanted than the card holds and each has long to go; the
-  // launch looks at 1,024 sequences at a time.
+  // launch looks at 1,024 sequences at a time. Without and with it, bf16, 8 heads of 64 by a state of 64:
+  // 200 prompts of up to 340 (3,200 wavefronts, 35,342 rows) 78 and 59 us, 300 of up to 250 72 and 61, 600
+  // of up to 110 (33,321 rows) 69 and 64, 8,000 of up to 40 491 and 486. Below the borders it gains where
+  // lengths are long (190 of up to 340: 75 and 56) and not where they are short (600 of up to 60: 50 and 52),
+  // and with many sequences it costs more than it gives (20,000 of up to 10: 1,033 and 1,077).
   p.ordered = s->seqs > 1 && s->seqs <= 8192 && waves > 3072 && s->tokens >= 32768;
   if (p.cut) {
     const uint64_t later = s->tokens / p.size + 1;

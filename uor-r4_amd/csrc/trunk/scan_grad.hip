@@ -26,10 +26,10 @@
 // over the block's wavefronts through LDS, in their order. Long sequences are cut into pieces as in
 // the scan; one launch more gives every piece's gradient at its start.
 //
-// Bound by instructions: 2,048 bf16 sequences of 128, 8 heads of 64 by a state of 64, take 980 us, of
-// which the vector instructions alone would take 494, the products 132 and the bytes 184. Two blocks
+// Bound by instructions: 2,048 bf16 sequences of 128, 8 heads of 64 by a state of 64, take 1,041 us,
+// of which the vector instructions alone would take 539, the products 166 and the bytes 184. Two blocks
 // of four wavefronts share a compute unit, two wavefronts a SIMD with 256 registers each; one a SIMD
-// with 512 takes 1,750 us, one block of eight wavefronts 1,027.
+// with 512 took 1,750 us where this took 980, one block of eight wavefronts 1,027.
 #include "wave.h"
 
 namespace trunk {
@@ -784,25 +784,19 @@ __global__ __launch_bounds__(kThreads) void grad_join(Grad k) {
     float g = k.dfinal ? k.dfinal[((uint64_t)seq * a.heads + head) * whole + e] : 0.0f;
     float *at = k.g_starts + (base * a.heads + head) * whole + e;
     const double *totals = a.totals + base * a.heads + head;
-    float own[kAhead], decay[kAhead], next[kAhead], next_decay[kAhead];
-    const auto read = [&](uint32_t j) {  // ahead, from the end
+    for (uint32_t j = 0; j < n; j += kAhead) {  // from the end
+      float own[kAhead], decay[kAhead];
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; i++) {
         const uint32_t place = j + i + 1 < n ? n - 2 - j - i : n - 2;
-        next[i] = at[place * step];
-        next_decay[i] = (float)totals[(uint64_t)place * a.heads];
+        own[i] = at[place * step];
+        decay[i] = (float)totals[(uint64_t)place * a.heads];
       }
-    };
-    read(0);
-    for (uint32_t j = 0; j + 1 < n; j += kAhead) {
-#pragma unroll
-      for (uint32_t i = 0; i < kAhead; i++) own[i] = next[i], decay[i] = next_decay[i];
-      if (j + kAhead + 1 < n) read(j + kAhead);
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; i++) {
-        if (j + i + 1 >= n) break;
+        if (j + i >= n) break;
+        if (j + i) at[(n - 1 - j - i) * step] = g;
         g = exp2_(decay[i]) * g + own[i];
-        at[(n - 2 - j - i) * step] = g;
       }
     }
   }
