@@ -20,7 +20,9 @@ constexpr uint32_t kRun = 16, kGradRun = 32;
 constexpr int kBatch = 4, kRowBatch = 8;  // rows that are read together, in a gradient and without
 // A gradient's registers leave a SIMD three wavefronts, twelve a compute unit: one block of 768 threads,
 // and no more blocks than compute units, so that all begin at once: 258 us; 768 blocks 279, 512 threads
-// (one block still) 299, 384 (two, a sixth of the lanes idle) 379, 1,024 (128 registers a thread) 387.
+// (one block still) 299, 384 (two, a sixth of the lanes idle) 379, 1,024 (128 registers a thread) 387: 2,048
+// bf16 sequences of 128 by 640 channels, the only number of channels that was timed. Others may leave more
+// lanes idle: a third of them at 2,048 channels, 42 of a hundred at 1,792.
 constexpr uint32_t kGradThreads = 768, kMostGradBlocks = 256;
 
 struct Conv {

@@ -6,7 +6,7 @@
 // and their gradients. Bound by the rows, each read once and written once: LANES lanes hold a row,
 // V pieces of eight values each, from its first read to its last write; means are sums of 32 bits.
 // A block goes through many rows with the parameters, and in a gradient their sums, in registers.
-// 152,700 bf16 rows of 256: 76 us, 5.2 TB/s; gradients of 131,072 of 512: 209 us, 5.1 TB/s, 10 of
+// 152,700 bf16 rows of 256: 76 us, 5.2 TB/s; gradients of 131,072 of 512: 209 us, 5.1 TB/s, 9 of
 // them the sums over blocks.
 #include "trunk.h"
 
@@ -236,8 +236,11 @@ __global__ __launch_bounds__(1024) void norms_grad_sums(const float *parts, uint
 
 namespace {
 
-// Blocks of the grid. A gradient's registers leave a compute unit three blocks of 256 threads, so 768
-// of them all begin at once: 209 us, where 1,024 run in two turns and take 259.
+// Blocks of the grid. Up to a width of 512 a gradient's registers leave a compute unit three blocks of 256
+// threads, so 768 of them all begin at once: 65,536 bf16 rows of 512 take 115 us, in 512 blocks 129 and in
+// 1,024, which run in two turns, 142. Wider rows leave it two blocks, and over 4,096 one of 1,024 threads:
+// there 768 are not the best (65,536 x 1,024: 269 us, 222 in 512 blocks; 16,384 x 4,096: 297 and 243;
+// 8,192 x 8,192: 427, 402 in 256), but no rule by width has been made.
 constexpr uint32_t kMostBlocks = 2048, kMostWorkers = 768;
 
 uint32_t lanes_of(uint32_t width) {

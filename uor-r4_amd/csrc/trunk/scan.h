@@ -95,7 +95,7 @@ Scan scan_of(const uor_trunk_scan_args *s, uint32_t size);
 // The block's piece, in the pieces' order or the call's; `number` is then its place among all pieces.
 __device__ __forceinline__ bool next_piece(const Scan &a, uint32_t &number, Piece &at) {
   if (number >= a.pieces) return false;
-  if (!a.order) return wave_piece(a.rows, number, a.size, at);
+  if (!a.order) return piece<true>(a.rows, number, a.size, at);
   if (number >= a.order[0]) return false;
   const uint32_t *place = a.order + 2 + 2 * number;
   at = piece_of(a.rows, place[0], place[1], a.size);

@@ -152,8 +152,6 @@ __device__ __forceinline__ bool piece(const Rows &rows, uint32_t i, uint32_t siz
   return true;
 }
 
-__device__ __forceinline__ bool wave_piece(const Rows &rows, uint32_t i, uint32_t size, Piece &p) { return piece<true>(rows, i, size, p); }
-
 // The i-th of the places that pieces after a sequence's first have, of which there are `size`-long
 // stretches of rows: sequence s has them from offsets[s] / size on. Where several sequences begin in
 // one stretch only the last can have any. `which` is the piece's number less one, `count` how many
