@@ -696,7 +696,7 @@ __global__ __launch_bounds__(64 * W, (kHeld<NT, W>)) void grad_rows(Grad k) {
         }
         if (lane == 0) sumD += (double)all;
         if (first + lane < end) {
-          const float dstep = (direct + A * da) * sigmoid(raw_now + bias);
+          const float dstep = (direct + A * da) * sigmoid<>(raw_now + bias);
           sumA += (double)((ODD && at_row(odd.steps, lane) ? kNone : s.step[lane]) * da);
           sumBias += (double)dstep;
           ((T *)k.ddt)[(uint64_t)(first + lane) * a.heads + head] = (T)dstep;

@@ -39,12 +39,14 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // 1 / (1 + e^-v) to 2^-21 of it: what the rounding of v log2(e) leaves goes into the exponential, which
-// would be |v| 2^-24 of itself off without. Past +-87, where a float holds e^-v no more, as at 87.
+// would be |v| 2^-24 of itself off without. Past +-87, where a float holds e^-v no more, as at 87. NUMBER:
+// for NaN it may be some number, where the result is multiplied by what v is too.
+template <bool NUMBER = false>
 __device__ __forceinline__ float sigmoid(float v) {
-  v = v < -87.0f ? -87.0f : v > 87.0f ? 87.0f : v;  // and NaN where v is
-  const float t = v * -kLog2e, left = fmaf(v, -1.92596299e-8f, fmaf(v, -kLog2e, -t));
-  const float e = exp2_(t);
-  return __builtin_amdgcn_rcpf(1.0f + fmaf(e, left * 0.693147181f, e));
+  const float c = __builtin_amdgcn_fmed3f(v, -87.0f, 87.0f);
+  const float t = c * -kLog2e, left = fmaf(c, -1.92596299e-8f, fmaf(c, -kLog2e, -t));
+  const float e = exp2_(t), s = __builtin_amdgcn_rcpf(1.0f + fmaf(e, left * 0.693147181f, e));
+  return NUMBER || v == v ? s : v;
 }
 // The activation's, for rows of T. Rows of bf16 go without what the rounding leaves: of a negative v the
 // value is |v| 2^-24 of itself off, 2^-20 at -16, where the rows' own rounding is 2^-9. That takes five
@@ -53,7 +55,7 @@ __device__ __forceinline__ float sigmoid(float v) {
 template <class T>
 __device__ __forceinline__ float sigmoid_of(float v) {
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + exp2_(-kLog2e * v));
-  else return sigmoid(v);
+  else return sigmoid<true>(v);
 }
 // e^v of v <= 0, to 2^-22 of it: what the rounding of v log2(e) leaves goes into the result.
 __device__ __forceinline__ float exp_down(float v) {
