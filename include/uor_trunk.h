@@ -1,8 +1,10 @@
 /*
  * uor_trunk.h - C ABI of a float trunk's operators on MI355X (gfx950).
  *
- * The served step of uor_fbs.h is integer. A trunk is trained, and may answer, in floating point
- * before it is exported; these are the parts of its layers in that form:
+ * Beside the served integer step of uor_fbs.h: parts of the layers of recurrent trunks that are trained,
+ * and answer, in floating point. They are neighbours of the served layers and not their float form (the
+ * served recurrence turns quaternions, its gate is a product of them, it has no norm after a block, and
+ * its windows may be longer), and nothing here exports to the served container:
  *
  *   scan    the selective state space scan, one decay a head and position:
  *             D_t = softplus(dt_t + dt_bias),  h_t = exp(D_t A) h_(t-1) + D_t x_t (x) B_t,

@@ -7,13 +7,15 @@ waits for nothing. Activations are bfloat16 or float32; parameters, the scan's s
 parameters' gradients are float32. Rows are packed: ``offsets`` (int32, one more than there are
 sequences, ascending, on the device) says where each sequence's rows begin; without it all rows are
 one sequence. Rows before the first offset and from the last one on are no sequence's: what is
-returned is 0 there, and nothing else depends on them. Where the inner axes of a tensor are not dense it is copied first. Errors raise
-``TrunkError``; there is no fallback: a missing library or device raises.
+returned is 0 there, and nothing else depends on them. Where the inner axes of a tensor are not dense
+it is copied first. Errors raise ``TrunkError``; there is no fallback: a missing library or device
+raises.
 
 ``scan``, ``conv`` and ``norms`` take part in autograd: where an input requires a gradient, the outputs
-have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which
-a program may call by itself (it is not differentiable). The steps update their states in place and have no gradient: going
-back through one raises. Nothing is kept between calls. Results are the same each time, bit for bit.
+have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which a
+program may call by itself (it is not differentiable). The steps update their states in place and have
+no gradient: going back through one raises. Nothing is kept between calls. Results are the same each
+time, bit for bit.
 
 A training step that is captured into a graph calls ``*_backward`` by itself, or has no eager graph of the
 same leaves alive meanwhile: torch would order their gradients after the other graph's stream.
