@@ -245,3 +245,13 @@ def test_scratch_memory_of_cut_sequences_goes_by_rows_not_by_sequences(seqs, len
     sums, kept = (places + seqs) * heads * 24, (rows // 64 + 1) * heads * dim * state * 4
     parts = max(1, min(-(-512 // seqs), heads))
     assert L.uor_trunk_scan_backward_workspace_bytes(C.byref(a)) <= 2 * places * one + kept + sums + order + 2 * parts * rows * state * 4 + 4096
+
+
+def test_a_reply_to_nothing_is_refused():
+    """An empty prompt has no last row: its reply would go on from another prompt's."""
+    from uor_fbs import float_trunk as ft
+    cfg = ft.Config(vocab=8, width=8, layers=1, heads=1, dim=4, state=4)
+    p, state = ft.make_params(cfg, device="cpu"), ft.make_state(cfg, 2, device="cpu")
+    for offsets in ([0, 3, 3], [0, 0, 3]):
+        with pytest.raises(ValueError, match="no tokens"):
+            ft.reply(cfg, p, torch.zeros(3, dtype=torch.long), torch.tensor(offsets, dtype=torch.int32), 2, state, torch.tensor([0, 1], dtype=torch.int32))

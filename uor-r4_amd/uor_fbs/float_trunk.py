@@ -192,7 +192,9 @@ def train(cfg, p, steps, count=64, length=8, rate=3e-3, seed=1, report=None):
 
 
 def reply(cfg, p, tokens, offsets, count, state, slots):
-    """``count`` greedy tokens of each prompt's session, (prompts, count)."""
+    """``count`` greedy tokens of each prompt's session, (prompts, count). A prompt has a token at least."""
+    if bool((offsets[1:] <= offsets[:-1]).any()):
+        raise ValueError("a prompt of no tokens has nothing that a reply could follow")
     logits = prompts(cfg, p, tokens, offsets, state, slots.long())
     now = logits[offsets[1:].long() - 1].argmax(1)
     said = [now]
