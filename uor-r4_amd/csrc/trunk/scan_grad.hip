@@ -152,8 +152,8 @@ __device__ __forceinline__ void hold(f32x4 (&h)[NT][2]) {
 //   dB_s: an odd dy_t, the same value of C_t of t >= s, x_s, a step's NaN after s, D_s, the same value of g;
 //   dC_t: an odd x_s or D_s, the same value of B_s of s <= t, dy_t;
 //   da_u: an odd dy_t or C_t of t >= u, x_s, B_s or D_s of s < u, any of g, any step's NaN.
-// Where all is finite that is one launch more: 37 f32 sequences of up to 301 take 72 us where they took 68,
-// 2,048 bf16 sequences of 128 1,087 where they took 1,075.
+// Where all is finite that is one launch more: 37 f32 sequences of up to 301 take 71 us where they took 68,
+// 2,048 bf16 sequences of 128 1,090 where they took 1,075.
 template <bool ODD, class V>
 __device__ __forceinline__ V clean(V v) {
   if constexpr (ODD) {
