@@ -138,6 +138,70 @@ int uor_trunk_norms_async(const uor_trunk_norms_args *args, void *stream);
 uint64_t uor_trunk_norms_backward_workspace_bytes(const uor_trunk_norms_args *args);
 int uor_trunk_norms_backward_async(const uor_trunk_norms_args *args, void *workspace, uint64_t bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Both ends of a trunk over its vocabulary.
+ *
+ *   embed   y_t = scale E[token_t]; a token outside 0 .. vocab - 1 (padding) has a row of zeros, and no
+ *           part in the gradient dE_v = scale sum of dy_t over the rows whose token is v, which is summed
+ *           in the rows' order.
+ *   loss    z_tv = x_t . W_v,  lse_t = log sum_v e^z_tv,  loss_t = lse_t - z_t,target
+ *           without keeping the logits z. A row whose target is outside 0 .. vocab - 1 takes no part: its
+ *           loss, lse and gradient are 0, and nothing of it is read.
+ *   choose  token_t = argmax_v z_tv, the lowest of equals,  logprob_t = z_t,token - lse_t.
+ *           Of a row with no logit over -inf the token is 0.
+ *
+ * Tokens and targets are int32, or int64 where `wide` is 1. E and W are [vocab][width], dense inside, in
+ * bf16 or f32 (W in the type of x), their rows `*_stride` values apart.
+ */
+#define UOR_TRUNK_MAX_VOCAB 0x1000000u
+#define UOR_TRUNK_MAX_ROWS 0x1000000u
+
+uint64_t uor_trunk_sizeof_embed(void);
+uint64_t uor_trunk_sizeof_head(void);
+
+typedef struct {
+  int32_t device;
+  uint32_t dtype, table_dtype;          /* of the rows y and dy; of E and dE */
+  uint32_t rows, vocab, width, wide;
+  float scale;
+  int64_t table_stride, dy_stride;
+  const void *tokens;                   /* [rows] */
+  const void *table;                    /* E; not read by the gradient */
+  void *y;                              /* [rows][width], dense */
+  /* a gradient's: */
+  const void *dy;                       /* [rows][width] */
+  void *dtable;                         /* [vocab][width], dense: all of it is written */
+} uor_trunk_embed_args;
+
+int uor_trunk_embed_async(const uor_trunk_embed_args *args, void *stream);
+uint64_t uor_trunk_embed_backward_workspace_bytes(const uor_trunk_embed_args *args);
+int uor_trunk_embed_backward_async(const uor_trunk_embed_args *args, void *workspace, uint64_t bytes, void *stream);
+
+/* dlosses and dlse may be NULL for zeros. With G_tv = (dlosses_t + dlse_t) e^(z_tv - lse_t) - dlosses_t
+ * [v is t's target]: dx = G W, dweight = G^T x. `lse` is the call's own. G is rounded to the type of x.
+ * Workspaces are aligned to 256 bytes. */
+typedef struct {
+  int32_t device;
+  uint32_t dtype, dweight_dtype;        /* of x, weight and dx; of dweight */
+  uint32_t rows, vocab, width, wide, reserved;
+  int64_t x_stride, w_stride;
+  const void *x, *weight;               /* [rows][width], [vocab][width] */
+  const void *targets;                  /* [rows] */
+  float *losses, *lse;                  /* [rows]; lse is read by the gradient */
+  int64_t *tokens;                      /* [rows] */
+  float *logprobs;                      /* [rows] */
+  /* a gradient's: */
+  const float *dlosses, *dlse;          /* [rows] */
+  void *dx, *dweight;                   /* [rows][width], [vocab][width], dense; either may be NULL */
+} uor_trunk_head_args;
+
+uint64_t uor_trunk_loss_workspace_bytes(const uor_trunk_head_args *args);
+int uor_trunk_loss_async(const uor_trunk_head_args *args, void *workspace, uint64_t bytes, void *stream);
+uint64_t uor_trunk_loss_backward_workspace_bytes(const uor_trunk_head_args *args);
+int uor_trunk_loss_backward_async(const uor_trunk_head_args *args, void *workspace, uint64_t bytes, void *stream);
+uint64_t uor_trunk_choose_workspace_bytes(const uor_trunk_head_args *args);
+int uor_trunk_choose_async(const uor_trunk_head_args *args, void *workspace, uint64_t bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,275 @@
+// head.hip - the head over a vocabulary without keeping its logits: the rows' softmax cross entropy, and
+// the largest logit's token with its log probability.
+//
+//   z_tv = x_t . W_v,  lse_t = log sum_v e^z_tv,  loss_t = lse_t - z_t,target
+//   token_t = argmax_v z_tv (the lowest of equals),  logprob_t = z_t,token - lse_t
+//
+// A block takes 128 rows through some of the vocabulary, 256 words a tile. The words are the result's rows, so
+// that a lane has 64 logits of one row of x in registers: their largest, and the sum of 2^(z log2 e - most), are
+// kept from tile to tile as a lane's own. Pieces of the vocabulary are joined by a second launch, in their order.
+#include "head_pack.h"
+
+namespace trunk {
+
+struct Scan {
+  Matrix w, x;
+  uint32_t rows, vocab, width;  // width: values of a row, whole 16 bytes
+  uint32_t row_tiles, word_tiles, splits;
+  const uint32_t *count;        // how many rows there are, or NULL: `rows`
+  const int32_t *target;        // [rows up to 256]
+  Sum *parts;                   // [2 splits][128 row_tiles]
+};
+
+// A logit's running softmax in base 2.
+struct Running {
+  float most = -3e38f, sum = 0.0f;
+  __device__ __forceinline__ void join(float most2, float sum2) {
+    const float m = fmaxf(most, most2);
+    sum = sum * exp2_(most - m) + sum2 * exp2_(most2 - m);
+    most = m;
+  }
+};
+
+template <class T, bool PICK>
+struct ScanTiles {
+  const Scan &a;
+  uint32_t tiles, stages, row0, word0;
+  int lane, wave;
+  Running run[2];
+  float value[2];
+  uint32_t place[2];
+  int32_t target[2];
+
+  template <class FA, class FB>
+  __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
+    const uint32_t word = word0 + n * kTileM;
+    fa.start((const T *)((const char *)a.w.at + (int64_t)word * a.w.pitch), a.w.pitch, a.vocab - word, a.width);
+    fb.start((const T *)((const char *)a.x.at + (int64_t)row0 * a.x.pitch), a.x.pitch, a.rows - row0, a.width);
+  }
+  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[4][2]) {
+    const int half = lane >> 5;
+    const uint32_t word = word0 + n * kTileM + 128 * (wave >> 1);
+    if (word + 128 > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // words that are none
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float most = z[0][j][0];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) most = fmaxf(most, z[i][j][r]);
+      if constexpr (PICK) {
+        if (__any(most > value[j])) {  // seldom after the first tiles
+          uint32_t at = 0;
+#pragma unroll
+          for (int i = 3; i >= 0; i--)
+#pragma unroll
+            for (int r = 15; r >= 0; r--) at = z[i][j][r] == most ? 32 * i + row_of(r, 0) : at;
+          if (most > value[j]) value[j] = most, place[j] = word + at + 4 * half;
+        }
+      } else {
+        const uint32_t at = (uint32_t)target[j] - word;
+        if (__any(at < 128)) {
+          const int own = (int)at - 4 * half;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) value[j] = own == 32 * i + row_of(r, 0) ? z[i][j][r] : value[j];
+        }
+      }
+      const float base = fmaxf(run[j].most, most * kLog2e);
+      float sum[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) sum[i] += exp2_(fmaf(z[i][j][r], kLog2e, -base));
+      run[j].sum = fmaf(run[j].sum, exp2_(run[j].most - base), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      run[j].most = base;
+    }
+  }
+};
+
+// `value` and `place` of two parts of a row: the target's logit, which one of them has at most, or the largest.
+template <bool PICK>
+__device__ __forceinline__ void join_value(float &value, uint32_t &place, float value2, uint32_t place2) {
+  if constexpr (PICK) {
+    const bool other = value2 > value || (value2 == value && place2 < place);
+    value = other ? value2 : value;
+    place = other ? place2 : place;
+  } else {
+    value += value2;
+  }
+}
+
+template <class T, bool PICK>
+__global__ __launch_bounds__(256, 2) void head_scan(Scan a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
+  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), split = work / a.row_tiles;
+  const uint32_t row0 = work % a.row_tiles * kTileN;
+  if (a.count && row0 >= *a.count) return;
+  const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  ScanTiles<T, PICK> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, first * kTileM, lane, wave};
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    tiles.value[j] = PICK ? -__builtin_inff() : 0.0f, tiles.place[j] = 0;
+    tiles.target[j] = PICK ? -1 : a.target[row0 + 64 * (wave & 1) + 32 * j + (lane & 31)];
+  }
+  run_tiles<T, true, true>(lds, tiles);
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    Running run = tiles.run[j];
+    run.join(__shfl_xor(run.most, 32), __shfl_xor(run.sum, 32));
+    float value = tiles.value[j];
+    uint32_t place = tiles.place[j];
+    join_value<PICK>(value, place, __shfl_xor(value, 32), __shfl_xor(place, 32));
+    if (lane < 32)
+      a.parts[(uint64_t)(2 * split + (wave >> 1)) * (a.row_tiles * kTileN) + row0 + 64 * (wave & 1) + 32 * j + lane] =
+          Sum{run.most, run.sum, value, place};
+  }
+}
+
+// A wavefront joins a row's parts, which are `across` apart.
+template <bool PICK>
+__global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, uint32_t across, uint32_t rows, const uint32_t *count,
+                                                 const int32_t *order, float *losses, float *lse, int64_t *tokens, float *logprobs) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= (count ? *count : rows)) return;
+  Running run;
+  float value = PICK ? -__builtin_inff() : 0.0f;
+  uint32_t place = PICK ? ~0u : 0;
+  for (uint32_t i = lane; i < n; i += 64) {
+    const Sum p = parts[(uint64_t)i * across + row];
+    run.join(p.most, p.sum);
+    join_value<PICK>(value, place, p.value, p.place);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    run.join(__shfl_xor(run.most, k), __shfl_xor(run.sum, k));
+    join_value<PICK>(value, place, __shfl_xor(value, k), __shfl_xor(place, k));
+  }
+  if (lane) return;
+  const double sum = ((double)run.most + (double)log2f(run.sum)) * kLn2;
+  if constexpr (PICK) {
+    tokens[row] = place == ~0u ? 0 : place;
+    logprobs[row] = (float)((double)value - sum);
+  } else {
+    const uint32_t at = order ? (uint32_t)order[row] : row;
+    lse[at] = (float)sum;
+    losses[at] = (float)(sum - (double)value);
+  }
+}
+
+namespace {
+
+// Parts of the vocabulary that blocks take by themselves: as many as fill the card twice over with blocks of
+// which two share a compute unit.
+uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles) {
+  const uint32_t want = (1024 + row_tiles - 1) / row_tiles;
+  return want < 1 ? 1 : want < word_tiles ? want : word_tiles;
+}
+
+// Where a call's scratch memory has what.
+struct Plan {
+  bool lay;  // the matrix is laid out anew
+  uint32_t width, row_tiles, word_tiles, splits;
+  uint64_t parts, w, x, order, target, counts, count, bytes;
+};
+Plan plan_of(const uor_trunk_head_args *s, bool pick) {
+  Plan p{};
+  const uint32_t size = size_of(s->dtype);
+  p.width = (uint32_t)up(s->width, 16 / size);
+  p.lay = !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
+  p.row_tiles = (s->rows + kTileN - 1) / kTileN;
+  p.word_tiles = (s->vocab + kTileM - 1) / kTileM;
+  p.splits = splits_of(p.row_tiles ? p.row_tiles : 1, p.word_tiles);
+  Scratch at;
+  const uint64_t rows = up(s->rows, kTileM);
+  p.parts = at.take(2ull * p.splits * p.row_tiles * kTileN * sizeof(Sum));
+  p.w = at.take(p.lay ? (uint64_t)s->vocab * p.width * size : 0);
+  p.x = at.take(pick && as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype) ? 0 : rows * p.width * size);
+  p.order = at.take(pick ? 0 : rows * 4);
+  p.target = at.take(pick ? 0 : rows * 4);
+  p.counts = at.take(pick ? 0 : (s->rows + kPackRows - 1) / kPackRows * 4);
+  p.count = at.take(pick ? 0 : 4);
+  p.bytes = at.bytes;
+  return p;
+}
+
+template <class T>
+void lay(const void *from, int64_t stride, uint32_t rows, uint32_t width, uint32_t pitch, void *to, hipStream_t stream) {
+  const uint64_t blocks = ((uint64_t)rows * (pitch / kVec<T>) + 255) / 256;
+  hipLaunchKernelGGL((head_lay<T>), dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (const T *)from, stride, rows, width,
+                     pitch, (T *)to);
+}
+
+template <class T, bool PICK>
+int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
+  const Plan p = plan_of(s, PICK);
+  Scan a{};
+  a.rows = s->rows, a.vocab = s->vocab, a.width = p.width;
+  a.row_tiles = p.row_tiles, a.word_tiles = p.word_tiles, a.splits = p.splits;
+  a.parts = (Sum *)(work + p.parts);
+  a.w = {s->weight, s->w_stride * (int64_t)sizeof(T)};
+  if (p.lay) {
+    lay<T>(s->weight, s->w_stride, s->vocab, s->width, p.width, work + p.w, stream);
+    a.w = {work + p.w, (int64_t)p.width * (int64_t)sizeof(T)};
+  }
+  a.x = {work + p.x, (int64_t)p.width * (int64_t)sizeof(T)};
+  if constexpr (PICK) {
+    if (as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)) a.x = {s->x, s->x_stride * (int64_t)sizeof(T)};
+    else lay<T>(s->x, s->x_stride, s->rows, s->width, p.width, work + p.x, stream);
+  } else {
+    Pack k{};
+    k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.pitch = p.width, k.stride = s->x_stride;
+    k.x = s->x, k.targets = s->targets, k.wide = s->wide != 0;
+    k.to = work + p.x, k.order = (int32_t *)(work + p.order), k.target = (int32_t *)(work + p.target);
+    k.count = (uint32_t *)(work + p.count), k.losses = s->losses, k.lse = s->lse;
+    const uint32_t blocks = (s->rows + kPackRows - 1) / kPackRows;
+    if (s->rows > 4096) {
+      hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, s->targets, k.wide, s->rows, s->vocab, (uint32_t *)(work + p.counts));
+      k.counts = (const uint32_t *)(work + p.counts);
+    }
+    hipLaunchKernelGGL((head_pack<T, false>), dim3(blocks), dim3(256), 0, stream, k);
+    a.count = k.count, a.target = k.target;
+  }
+  hipLaunchKernelGGL((head_scan<T, PICK>), dim3(p.row_tiles * p.splits), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((head_join<PICK>), dim3((s->rows + 3) / 4), dim3(256), 0, stream, a.parts, 2 * p.splits, p.row_tiles * kTileN, s->rows,
+                     a.count, PICK ? nullptr : (const int32_t *)(work + p.order), s->losses, s->lse, s->tokens, s->logprobs);
+  return launched();
+}
+
+template <bool PICK>
+int scan(const uor_trunk_head_args *s, void *workspace, uint64_t bytes, void *stream) {
+  const uint64_t want = plan_of(s, PICK).bytes;
+  if (!workspace || bytes < want || (uintptr_t)workspace % 256)
+    return fail(-1, "a workspace of %llu bytes, aligned to 256, is wanted", (unsigned long long)want);
+  const OnDevice on(s->device);
+  if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
+  return s->dtype == UOR_TRUNK_BF16 ? scan<bf16, PICK>(s, (char *)workspace, (hipStream_t)stream)
+                                    : scan<float, PICK>(s, (char *)workspace, (hipStream_t)stream);
+}
+
+}  // namespace
+}  // namespace trunk
+
+using namespace trunk;
+
+extern "C" uint64_t uor_trunk_sizeof_head(void) { return sizeof(uor_trunk_head_args); }
+
+extern "C" uint64_t uor_trunk_loss_workspace_bytes(const uor_trunk_head_args *s) { return check_head(s) || !s->rows ? 0 : plan_of(s, false).bytes; }
+
+extern "C" int uor_trunk_loss_async(const uor_trunk_head_args *s, void *workspace, uint64_t bytes, void *stream) {
+  if (const int e = check_head(s)) return e;
+  if (!s->rows) return 0;
+  if (!s->targets || !s->losses || !s->lse) return fail(-1, "null targets, losses or lse");
+  return scan<false>(s, workspace, bytes, stream);
+}
+
+extern "C" uint64_t uor_trunk_choose_workspace_bytes(const uor_trunk_head_args *s) { return check_head(s) || !s->rows ? 0 : plan_of(s, true).bytes; }
+
+extern "C" int uor_trunk_choose_async(const uor_trunk_head_args *s, void *workspace, uint64_t bytes, void *stream) {
+  if (const int e = check_head(s)) return e;
+  if (!s->rows) return 0;
+  if (!s->tokens || !s->logprobs) return fail(-1, "null tokens or logprobs");
+  return scan<true>(s, workspace, bytes, stream);
+}

@@ -1,0 +1,390 @@
+// head_grad.hip - the gradients of the head's softmax cross entropy, without keeping its logits:
+//
+//   G_tv = (dloss_t + dlse_t) e^(z_tv - lse_t) - dloss_t [v = target_t],  dx = G W,  dW = G^T x.
+//
+// A piece of the rows by a piece of the vocabulary at a time: one launch computes the piece's logits again
+// and writes its G, in the type of x, to scratch memory that the caches hold; one takes G W and one G^T x from
+// it. dx is summed over the pieces of the vocabulary and dW over those of the rows, in 32 bits. Where a piece has
+// fewer tiles than the card takes at once, its sums are split along their axis and joined at the end.
+//
+// G is rounded to bf16 where x is, half a step (2^-8) of each value, independent of the others. Of the largest,
+// the target's, that would be an error of the whole row: it is left out of G, and its terms G_t,target W_target
+// and G_t,target x_t are added to dx and dW in 32 bits at their ends, dW's by sorted targets.
+#include "head_pack.h"
+#include "sorted.h"
+
+namespace trunk {
+
+struct Logits {
+  Matrix w, x;
+  uint32_t rows, vocab, width;
+  uint32_t row0, row_tiles, word0, word_tiles, splits;  // the piece, in tiles of 128 rows and 256 words
+  const uint32_t *count;
+  const int32_t *target;
+  const float4 *factors;
+  const int32_t *order;
+  float *terms;     // [rows of the call]: the targets' G, where x is bf16
+  void *g;          // [128 row_tiles][pitch]
+  uint32_t pitch;   // values
+};
+
+template <class T>
+struct LogitTiles {
+  const Logits &a;
+  uint32_t tiles, stages, row0, word0;  // row0 in the piece, word0 of the vocabulary
+  int lane, wave;
+  float base[2], all[2], one[2];
+  int32_t target[2], place[2];
+
+  template <class FA, class FB>
+  __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
+    const uint32_t word = word0 + n * kTileM, row = a.row0 + row0;
+    fa.start((const T *)((const char *)a.w.at + (int64_t)word * a.w.pitch), a.w.pitch, a.vocab - word, a.width);
+    fb.start((const T *)((const char *)a.x.at + (int64_t)row * a.x.pitch), a.x.pitch, kTileN, a.width);
+  }
+  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[4][2]) {
+    const int half = lane >> 5;
+    const uint32_t word = word0 + n * kTileM + 128 * (wave >> 1);
+    if (word + 128 > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // their G is 0
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) z[i][j][r] = all[j] * exp2_(fmaf(z[i][j][r], kLog2e, -base[j]));
+      const uint32_t at = (uint32_t)target[j] - word;
+      if (__any(at < 128)) {
+        float term = 0.0f;
+        const int own = (int)at - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const bool here = own == 32 * i + row_of(r, 0);
+            if constexpr (sizeof(T) == 2) term = here ? z[i][j][r] : term, z[i][j][r] = here ? 0.0f : z[i][j][r];
+            else z[i][j][r] -= here ? one[j] : 0.0f;
+          }
+        if (sizeof(T) == 2 && at < 128 && (int)(at >> 2 & 1) == half) a.terms[place[j]] = term - one[j];
+      }
+      T *to = (T *)a.g + (uint64_t)(row0 + 64 * (wave & 1) + 32 * j + (lane & 31)) * a.pitch + (word - a.word0);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 2) {
+          // A lane has four words of every eight, the lane 32 on the other four: they change places, so that
+          // each writes eight next to each other.
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            uint32_t p[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const bf16x2 lo = {(bf16)z[i][j][4 * q + 2 * e], (bf16)z[i][j][4 * q + 2 * e + 1]};
+              const bf16x2 hi = {(bf16)z[i][j][4 * q + 4 + 2 * e], (bf16)z[i][j][4 * q + 5 + 2 * e]};
+              const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi), false, false);
+              p[0][e] = both[0], p[1][e] = both[1];
+            }
+            *(u32x4 *)(to + 32 * i + 8 * (q + half)) = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            *(f32x4 *)(to + 32 * i + 8 * q + 4 * half) = f32x4{z[i][j][4 * q], z[i][j][4 * q + 1], z[i][j][4 * q + 2], z[i][j][4 * q + 3]};
+        }
+      }
+    }
+  }
+};
+
+template <class T>
+__global__ __launch_bounds__(256, 2) void head_logits(Logits a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
+  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), split = work / a.row_tiles, row0 = work % a.row_tiles * kTileN;
+  if (a.row0 + row0 >= *a.count) return;
+  const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  LogitTiles<T> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, a.word0 + first * kTileM, lane, wave};
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const uint32_t row = a.row0 + row0 + 64 * (wave & 1) + 32 * j + (lane & 31);
+    const float4 f = a.factors[row];
+    tiles.base[j] = f.x, tiles.all[j] = f.y, tiles.one[j] = f.z, tiles.target[j] = a.target[row], tiles.place[j] = a.order[row];
+  }
+  run_tiles<T, true, true>(lds, tiles);
+}
+
+// A product of a piece: out[m][n] (+)= sum_k a[m][k] b[k][n] over a share of its k.
+struct Product {
+  Matrix a, b;             // b lies across: rows of k
+  uint32_t m, n, k;        // sums of the piece; k may be fewer, see Limit
+  uint32_t m_tiles, n_tiles, splits;
+  uint32_t row0;           // the piece's first packed row
+  const uint32_t *count;   // how many packed rows there are
+  float *parts;            // [splits][m_rows][n_pitch]: sums so far
+  uint64_t m_rows;
+  uint32_t n_pitch;
+  uint32_t m0;             // the piece's first row of parts
+  bool first;              // nothing has been summed before
+};
+
+// ROWS: the summed axis are the rows of x (dW), else the words (dx).
+template <class T, bool ROWS>
+struct ProductTiles {
+  const Product &p;
+  uint32_t tiles, stages, m0, n0, k0, depth, split;
+  int lane, wave;
+  template <class FA, class FB>
+  __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
+    if constexpr (ROWS) fa.start((const T *)((const char *)p.a.at + (int64_t)k0 * p.a.pitch) + m0, p.a.pitch, p.m - m0, depth);
+    else fa.start((const T *)((const char *)p.a.at + (int64_t)m0 * p.a.pitch) + k0, p.a.pitch, kTileM, depth);
+    fb.start((const T *)((const char *)p.b.at + (int64_t)k0 * p.b.pitch) + n0, p.b.pitch, p.n - n0, depth);
+  }
+  __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[4][2]) {
+    const int half = lane >> 5;
+    float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 128 * (wave >> 1)) * p.n_pitch + n0 + 64 * (wave & 1) + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (n0 + 64 * (wave & 1) + 32 * j + (lane & 31) >= p.n) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float *at = to + (uint64_t)(32 * i + row_of(r, half)) * p.n_pitch + 32 * j;
+          *at = p.first ? sums[i][j][r] : *at + sums[i][j][r];
+        }
+    }
+  }
+};
+
+template <class T, bool ROWS>
+__global__ __launch_bounds__(256, 2) void head_product(Product p) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
+  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), n0 = work % p.n_tiles * kTileN, rest = work / p.n_tiles;
+  const uint32_t m0 = rest % p.m_tiles * kTileM, split = rest / p.m_tiles;
+  const uint32_t count = *p.count, there = count > p.row0 ? count - p.row0 : 0;  // of the piece's rows
+  uint32_t k = p.k;
+  if constexpr (ROWS) k = there < k ? there : k;
+  else if (m0 >= there) return;
+  // The share of the summed axis, in stages.
+  const uint32_t all = (k + kDeep<T> - 1) / kDeep<T>;
+  const uint32_t s0 = (uint32_t)((uint64_t)all * split / p.splits), s1 = (uint32_t)((uint64_t)all * (split + 1) / p.splits);
+  if (s0 == s1 && !p.first) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t k0 = s0 * kDeep<T>, k1 = s1 * kDeep<T> < k ? s1 * kDeep<T> : k;
+  ProductTiles<T, ROWS> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, lane, wave};
+  run_tiles<T, !ROWS, false>(lds, tiles);
+}
+
+// The splits' sums in their order, rounded to the result's type. dx: packed rows go to their own places, with
+// their targets' terms.
+struct Ends {
+  const float *parts;
+  uint32_t splits, rows, n, n_pitch, row0;  // row0: the first's number of all packed rows
+  uint64_t m_rows;
+  const uint32_t *count;   // dx's: how many packed rows there are, or NULL
+  const int32_t *order, *target;
+  const float *terms;      // or NULL
+  Matrix w;
+  void *to;
+};
+template <class R>
+__global__ __launch_bounds__(256) void head_sums(Ends a) {
+  const uint32_t pieces = (a.n + 7) / 8, there = a.count ? (*a.count > a.row0 ? *a.count - a.row0 : 0) : a.rows;
+  const uint32_t limit = there < a.rows ? there : a.rows;
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < (uint64_t)limit * pieces; i += gridDim.x * 256ull) {
+    const uint64_t row = i / pieces;
+    const uint32_t col = (uint32_t)(i % pieces) * 8;
+    f32x8 v = load_some<float, 8>(a.parts + row * a.n_pitch, true, col, a.n);
+    for (uint32_t s = 1; s < a.splits; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
+    const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.row0 + row] : row;
+    if (a.terms)
+      v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)((const char *)a.w.at + a.target[a.row0 + row] * a.w.pitch), true, col, a.n)), f32x8) *
+           a.terms[place];
+    store_some<R, 8>((R *)a.to + place * a.n, col, a.n, __builtin_convertvector(v, V8<R>));
+  }
+}
+
+// The gradient of no rows.
+template <class R>
+__global__ __launch_bounds__(256) void head_nothing(R *to, uint64_t n) {
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) to[i] = (R)0.0f;
+}
+
+namespace {
+
+constexpr uint64_t kPiece = 1ull << 28;  // bytes of G: what the last cache holds
+
+struct GradPlan {
+  bool lay;
+  uint32_t width, rows, words;           // a row's values; rows and words of a piece, whole tiles
+  uint32_t all_rows, all_words;          // of the call, whole tiles
+  uint32_t n_tiles, x_splits, w_splits, n_pitch;
+  uint32_t x_rows, w_rows;               // how many rows' and words' sums are kept at once
+  SortPlan sort;                         // of the targets, where x is bf16
+  uint64_t g, dx, dw, w, x, order, target, factors, terms, sorted, counts, count, bytes;
+};
+uint32_t splits_for(uint32_t tiles, uint32_t stages) {
+  const uint32_t want = 512 / tiles, most = stages / 8;
+  return want < 2 || most < 2 ? 1 : want < most ? want : most;
+}
+GradPlan grad_plan(const uor_trunk_head_args *s) {
+  GradPlan p{};
+  const uint32_t size = size_of(s->dtype), deep = 64 / size;
+  p.width = (uint32_t)up(s->width, 16 / size);
+  p.lay = !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
+  p.all_rows = (uint32_t)up(s->rows, kTileM), p.all_words = (uint32_t)up(s->vocab, kTileM);
+  // A piece of about as many rows as words, whose sums are read and written the least for the G between.
+  const uint64_t values = kPiece / size;
+  uint64_t side = kTileM;
+  while ((side + kTileM) * (side + kTileM) <= values) side += kTileM;
+  p.rows = p.all_rows < side ? p.all_rows : (uint32_t)side;
+  const uint64_t words = values / p.rows / kTileM * kTileM;
+  p.words = p.all_words < words ? p.all_words : (uint32_t)words;
+  const uint64_t rows = values / p.words / kTileM * kTileM;
+  p.rows = p.all_rows < rows ? p.all_rows : (uint32_t)rows;
+  p.n_tiles = (p.width + kTileN - 1) / kTileN;
+  p.n_pitch = p.n_tiles * kTileN;
+  p.x_splits = splits_for(p.rows / kTileM * p.n_tiles, p.words / deep);
+  p.w_splits = splits_for(p.words / kTileM * p.n_tiles, p.rows / deep);
+  // With the rows' pieces outside, the sums of dx are kept of one of them and those of dW of all words; or the
+  // other way round.
+  const bool rows_outside = (uint64_t)p.x_splits * (p.all_rows - p.rows) > (uint64_t)p.w_splits * (p.all_words - p.words);
+  p.x_rows = rows_outside ? p.rows : p.all_rows, p.w_rows = rows_outside ? p.all_words : p.words;
+  Scratch at;
+  p.g = at.take((uint64_t)p.rows * p.words * size);
+  p.dx = at.take(4ull * p.x_splits * p.x_rows * p.n_pitch);
+  p.dw = at.take(4ull * (p.w_splits + (size == 2)) * p.w_rows * p.n_pitch);  // and the targets' terms
+  p.w = at.take(p.lay ? (uint64_t)s->vocab * p.width * size : 0);
+  p.x = at.take((uint64_t)p.all_rows * p.width * size);
+  p.order = at.take(4ull * p.all_rows);
+  p.target = at.take(4ull * p.all_rows);
+  p.factors = at.take(16ull * p.all_rows);
+  if (size == 2) {
+    p.sort = sort_plan(s->rows, s->vocab, s->width);
+    p.sorted = at.take(s->dweight ? p.sort.bytes : 0);
+    p.terms = at.take(4ull * s->rows);
+  }
+  p.counts = at.take((s->rows + kPackRows - 1) / kPackRows * 4);
+  p.count = at.take(4);
+  p.bytes = at.bytes;
+  return p;
+}
+
+template <class R>
+void sums(const Ends &a, hipStream_t stream) {
+  const uint64_t blocks = ((uint64_t)a.rows * ((a.n + 7) / 8) + 255) / 256;
+  hipLaunchKernelGGL((head_sums<R>), dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
+}
+
+template <class T>
+int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
+  const GradPlan p = grad_plan(s);
+  const int64_t pitch = (int64_t)p.width * (int64_t)sizeof(T), g_pitch = (int64_t)p.words * (int64_t)sizeof(T);
+  Matrix w{s->weight, s->w_stride * (int64_t)sizeof(T)}, x{work + p.x, pitch};
+  if (p.lay) {
+    const uint64_t blocks = ((uint64_t)s->vocab * (p.width / kVec<T>) + 255) / 256;
+    hipLaunchKernelGGL((head_lay<T>), dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (const T *)s->weight, s->w_stride,
+                       s->vocab, s->width, p.width, (T *)(work + p.w));
+    w = {work + p.w, pitch};
+  }
+  uint32_t *count = (uint32_t *)(work + p.count);
+  Pack k{};
+  k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.pitch = p.width, k.stride = s->x_stride;
+  k.x = s->x, k.targets = s->targets, k.wide = s->wide != 0;
+  k.to = work + p.x, k.order = (int32_t *)(work + p.order), k.target = (int32_t *)(work + p.target), k.count = count;
+  k.lse_in = s->lse, k.dlosses = s->dlosses, k.dlse = s->dlse, k.factors = (float4 *)(work + p.factors);
+  k.dx = s->dx, k.dx_width = s->dx ? s->width : 0;
+  const uint32_t blocks = (s->rows + kPackRows - 1) / kPackRows;
+  if (s->rows > 4096) {
+    hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, s->targets, k.wide, s->rows, s->vocab, (uint32_t *)(work + p.counts));
+    k.counts = (const uint32_t *)(work + p.counts);
+  }
+  hipLaunchKernelGGL((head_pack<T, true>), dim3(blocks), dim3(256), 0, stream, k);
+  constexpr bool kTerms = sizeof(T) == 2;
+  float *terms = kTerms ? (float *)(work + p.terms) : nullptr;
+  Sums t{};
+  if (kTerms && s->dweight) {
+    t.width = s->width, t.scale = 1.0f, t.stride = s->x_stride, t.pitch = p.n_pitch, t.from = s->x, t.weights = terms;
+    sort_rows(p.sort, s->targets, s->wide != 0, s->rows, s->vocab, work + p.sorted, stream, t);
+  }
+  // Of the two axes' pieces, one's are outside: see grad_plan.
+  const uint32_t row_pieces = (s->rows + p.rows - 1) / p.rows, word_pieces = (s->vocab + p.words - 1) / p.words;
+  const bool rows_outside = p.x_rows < p.all_rows;
+  for (uint32_t i = 0; i < row_pieces * word_pieces; i++) {
+    const uint32_t row_piece = rows_outside ? i / word_pieces : i % row_pieces, word_piece = rows_outside ? i % word_pieces : i / row_pieces;
+    const uint32_t row0 = row_piece * p.rows, word0 = word_piece * p.words;
+    const uint32_t rows = s->rows - row0 < p.rows ? s->rows - row0 : p.rows, words = s->vocab - word0 < p.words ? s->vocab - word0 : p.words;
+    const uint32_t word_tiles = (words + kTileM - 1) / kTileM;
+    Logits l{};
+    l.w = w, l.x = x, l.rows = s->rows, l.vocab = s->vocab, l.width = p.width;
+    l.row0 = row0, l.row_tiles = (rows + kTileN - 1) / kTileN, l.word0 = word0, l.word_tiles = word_tiles;
+    const uint32_t want = (1024 + l.row_tiles - 1) / l.row_tiles;
+    l.splits = want < word_tiles ? want : word_tiles;
+    l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.pitch = p.words;
+    hipLaunchKernelGGL((head_logits<T>), dim3(l.row_tiles * l.splits), dim3(256), 0, stream, l);
+    Product a{};
+    a.a = {work + p.g, g_pitch}, a.row0 = row0, a.count = count, a.n = p.width, a.n_tiles = p.n_tiles, a.n_pitch = p.n_pitch;
+    if (s->dx) {
+      a.b = {(const char *)w.at + (int64_t)word0 * w.pitch, w.pitch};
+      a.m = rows, a.k = words, a.m_tiles = (rows + kTileM - 1) / kTileM, a.splits = p.x_splits;
+      a.parts = (float *)(work + p.dx), a.m_rows = p.x_rows, a.m0 = rows_outside ? 0 : row0, a.first = word0 == 0;
+      hipLaunchKernelGGL((head_product<T, false>), dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a);
+      if (word_piece + 1 == word_pieces) {
+        Ends e{};
+        e.n = s->width, e.n_pitch = p.n_pitch;
+        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.x_splits, e.rows = rows, e.row0 = row0, e.m_rows = p.x_rows;
+        e.count = count, e.order = k.order, e.target = k.target, e.terms = terms, e.w = w, e.to = s->dx;
+        sums<T>(e, stream);
+      }
+    }
+    if (s->dweight) {
+      a.b = {work + p.x + (int64_t)row0 * pitch, pitch};
+      a.m = (uint32_t)up(words, kTileM), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
+      a.parts = (float *)(work + p.dw), a.m_rows = p.w_rows, a.m0 = rows_outside ? word0 : 0, a.first = row0 == 0;
+      hipLaunchKernelGGL((head_product<T, true>), dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a);
+      if (row_piece + 1 == row_pieces) {
+        Ends e{};
+        e.n = s->width, e.n_pitch = p.n_pitch;
+        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.w_splits, e.rows = words, e.m_rows = p.w_rows;
+        if constexpr (kTerms) {
+          t.word0 = word0, t.words = words, t.to = a.parts + ((uint64_t)p.w_splits * p.w_rows + a.m0) * p.n_pitch;
+          sum_rows<float, T>(t, stream);
+          e.splits++;
+        }
+        const uint64_t at = (uint64_t)word0 * s->width;
+        if (s->dweight_dtype == UOR_TRUNK_BF16) e.to = (bf16 *)s->dweight + at, sums<bf16>(e, stream);
+        else e.to = (float *)s->dweight + at, sums<float>(e, stream);
+      }
+    }
+  }
+  return launched();
+}
+
+}  // namespace
+}  // namespace trunk
+
+using namespace trunk;
+
+extern "C" uint64_t uor_trunk_loss_backward_workspace_bytes(const uor_trunk_head_args *s) { return check_head(s) || !s->rows ? 0 : grad_plan(s).bytes; }
+
+extern "C" int uor_trunk_loss_backward_async(const uor_trunk_head_args *s, void *workspace, uint64_t bytes, void *stream) {
+  if (const int e = check_head(s)) return e;
+  if (s->dweight_dtype > UOR_TRUNK_F32) return fail(-1, "dweight_dtype %u is neither bf16 nor f32", s->dweight_dtype);
+  if (s->rows && (!s->targets || !s->lse)) return fail(-1, "null targets or lse");
+  if (!s->dx && !s->dweight) return 0;
+  if (!s->rows) {
+    if (!s->dweight) return 0;
+    const OnDevice on(s->device);
+    if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
+    const uint64_t n = (uint64_t)s->vocab * s->width;
+    if (s->dweight_dtype == UOR_TRUNK_BF16)
+      hipLaunchKernelGGL((head_nothing<bf16>), dim3(2048), dim3(256), 0, (hipStream_t)stream, (bf16 *)s->dweight, n);
+    else
+      hipLaunchKernelGGL((head_nothing<float>), dim3(2048), dim3(256), 0, (hipStream_t)stream, (float *)s->dweight, n);
+    return launched();
+  }
+  const uint64_t want = uor_trunk_loss_backward_workspace_bytes(s);
+  if (!workspace || bytes < want || (uintptr_t)workspace % 256)
+    return fail(-1, "a workspace of %llu bytes, aligned to 256, is wanted", (unsigned long long)want);
+  const OnDevice on(s->device);
+  if (!on.ok) return fail(-2, "hipSetDevice(%d) failed", s->device);
+  return s->dtype == UOR_TRUNK_BF16 ? grad<bf16>(s, (char *)workspace, (hipStream_t)stream) : grad<float>(s, (char *)workspace, (hipStream_t)stream);
+}

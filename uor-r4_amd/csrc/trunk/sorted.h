@@ -1,0 +1,339 @@
+// sorted.h - sums of rows by a number that each has, a word of the vocabulary: what the embedding's gradient and
+// the targets' terms of the head's share.
+//
+// The rows' numbers are sorted by their words, rows of a word staying in their order: up to 4,096 in one block,
+// more by digits of the word in two or three passes. Then pieces of the sorted rows are summed, each by the lanes
+// that hold a row of the result; a word whose rows go over a piece's end leaves its parts to a second launch, which
+// adds them up in their order. So a word that a large share of all rows has is summed by many. Other blocks of the
+// first launch write zeros to the rows of words that do not occur. No sum depends on the order in which blocks run.
+#pragma once
+#include "trunk.h"
+
+#include <type_traits>
+
+namespace trunk {
+
+// A row's word, or `vocab` for none.
+__device__ __forceinline__ uint32_t token_of(const void *tokens, bool wide, uint64_t row, uint32_t vocab) {
+  const int64_t t = wide ? ((const int64_t *)tokens)[row] : ((const int32_t *)tokens)[row];
+  return t >= 0 && t < (int64_t)vocab ? (uint32_t)t : vocab;
+}
+
+// result[word - word0] = scale sum of weight_t rows_t over the rows t of that word, of `words` words from word0 on.
+struct Sums {
+  uint32_t rows, width, word0, words;
+  float scale;
+  int64_t stride, pitch;        // values from row to row of the rows, of the result
+  const void *from;
+  const float *weights;         // [rows], or NULL: 1
+  void *to;
+  const uint32_t *keys, *order; // [rows] sorted: words (the vocabulary's size: none), and their rows
+  uint32_t length, groups;      // rows of a piece, pieces
+  float *parts;                 // [groups][2][width]: a piece's first word's sum and its last one's
+  uint32_t sum_blocks;          // of the first launch, the others write zeros
+};
+
+// ---------------------------------------------------------------------------------------------
+// The sort.
+
+constexpr uint32_t kFew = 4096, kSortBlocks = 512, kMostBins = 1024;
+
+// Up to `n` (a power of two) rows in one block: pairs of a token and a row, all different, by exchanges.
+static __global__ __launch_bounds__(1024) void sort_few(const void *tokens, bool wide, uint32_t rows, uint32_t vocab, uint32_t n, uint32_t *keys,
+                                                       uint32_t *from) {
+  extern __shared__ uint64_t pairs[];
+  for (uint32_t i = threadIdx.x; i < n; i += 1024)
+    pairs[i] = i < rows ? (uint64_t)token_of(tokens, wide, i, vocab) << 32 | i : ~(uint64_t)0;
+  for (uint32_t size = 2; size <= n; size <<= 1)
+    for (uint32_t step = size >> 1; step; step >>= 1) {
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < n / 2; i += 1024) {
+        const uint32_t lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const uint64_t p = pairs[lo], q = pairs[hi];
+        if ((p > q) == !(lo & size)) pairs[lo] = q, pairs[hi] = p;
+      }
+    }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < rows; i += 1024) keys[i] = (uint32_t)(pairs[i] >> 32), from[i] = (uint32_t)pairs[i];
+}
+
+// A pass over one digit of the tokens. A block has `share` rows next to each other, each of its
+// wavefronts a quarter of them.
+struct Digit {
+  uint32_t rows, vocab, share, shift, bins;
+  bool wide;
+  const void *tokens;                // the first pass's, else NULL
+  const uint32_t *keys, *from;       // the pass before's
+  uint32_t *counts;                  // [blocks][bins]
+  uint32_t *keys_out, *from_out;
+  __device__ __forceinline__ uint32_t key(uint64_t i) const { return tokens ? token_of(tokens, wide, i, vocab) : keys[i]; }
+};
+__device__ __forceinline__ void count_digits(const Digit &a, uint32_t *bins, uint64_t first, uint64_t end) {
+  for (uint64_t i = first + (threadIdx.x & 63); i < end; i += 64) atomicAdd(&bins[(a.key(i) >> a.shift) & (a.bins - 1)], 1u);
+}
+__device__ __forceinline__ void share_of(const Digit &a, uint64_t &first, uint64_t &end) {
+  const uint32_t part = a.share / 4;
+  first = (uint64_t)blockIdx.x * a.share + (threadIdx.x >> 6) * part;
+  end = first + part < a.rows ? first + part : a.rows;
+}
+static __global__ __launch_bounds__(256) void sort_count(Digit a) {
+  __shared__ uint32_t bins[kMostBins];
+  for (uint32_t b = threadIdx.x; b < a.bins; b += 256) bins[b] = 0;
+  __syncthreads();
+  uint64_t first, end;
+  share_of(a, first, end);
+  count_digits(a, bins, first, end);
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < a.bins; b += 256) a.counts[(uint64_t)blockIdx.x * a.bins + b] = bins[b];
+}
+// A row goes behind all rows of lower digits, those of its digit in blocks before, in wavefronts
+// before and in its own wavefront before it.
+static __global__ __launch_bounds__(256) void sort_place(Digit a) {
+  __shared__ uint32_t at[4][kMostBins], sums[4];
+  for (uint32_t b = threadIdx.x; b < 4 * kMostBins; b += 256) (&at[0][0])[b] = 0;
+  __syncthreads();
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  uint64_t first, end;
+  share_of(a, first, end);
+  count_digits(a, at[wave], first, end);
+  // A thread's four digits next to each other: their rows in blocks before, and in all.
+  const uint32_t b0 = threadIdx.x * 4;
+  uint32_t before[4] = {}, all[4] = {};
+  for (uint32_t k = 0; k < gridDim.x; k++)
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++)
+      if (b0 + e < a.bins) {
+        const uint32_t n = a.counts[(uint64_t)k * a.bins + b0 + e];
+        before[e] += k < blockIdx.x ? n : 0;
+        all[e] += n;
+      }
+  uint32_t mine = all[0] + all[1] + all[2] + all[3], lower = mine;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const uint32_t v = __shfl_up(lower, k);
+    lower += lane >= (uint32_t)k ? v : 0;
+  }
+  if (lane == 63) sums[wave] = lower;
+  __syncthreads();
+  lower -= mine;
+  for (uint32_t w = 0; w < wave; w++) lower += sums[w];
+#pragma unroll
+  for (uint32_t e = 0; e < 4; e++) {
+    if (b0 + e < a.bins) {
+      uint32_t place = lower + before[e];
+      for (uint32_t w = 0; w < 4; w++) {
+        const uint32_t n = at[w][b0 + e];
+        at[w][b0 + e] = place;
+        place += n;
+      }
+    }
+    lower += all[e];
+  }
+  __syncthreads();
+  for (uint64_t base = first; base < end; base += 64) {
+    const uint64_t i = base + lane;
+    const bool there = i < end;
+    const uint32_t key = there ? a.key(i) : 0, digit = (key >> a.shift) & (a.bins - 1);
+    uint64_t same = __ballot(there);  // the lanes of the same digit
+    for (uint32_t bit = 1; bit < a.bins; bit <<= 1) {
+      const uint64_t set = __ballot(there && (digit & bit));
+      same &= digit & bit ? set : ~set;
+    }
+    if (there) {
+      const uint32_t place = at[wave][digit] + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1));
+      a.keys_out[place] = key;
+      a.from_out[place] = a.tokens ? (uint32_t)i : a.from[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (there && !(same >> lane >> 1)) at[wave][digit] += __builtin_popcountll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The sums.
+
+// LANES lanes take a piece of `length` sorted rows and 8 LANES of their columns.
+template <class R, class T, int LANES>
+__global__ __launch_bounds__(256) void sorted_sums(Sums a) {
+  const uint32_t lane = threadIdx.x % LANES;
+  if (blockIdx.x >= a.sum_blocks) {  // zeros: 64 words a block, those that do not occur
+    const uint64_t word0 = (uint64_t)(blockIdx.x - a.sum_blocks) * 64;
+    const uint32_t word = (uint32_t)word0 + (threadIdx.x & 63), key = a.word0 + word;
+    uint32_t lo = 0, hi = a.rows;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (a.keys[mid] < key) lo = mid + 1;
+      else hi = mid;
+    }
+    const uint64_t none = __ballot(word < a.words && (lo == a.rows || a.keys[lo] != key));
+    for (uint32_t k = threadIdx.x / LANES; k < 64; k += 256 / LANES)
+      if (none >> k & 1)
+        for (uint32_t col = (blockIdx.y * LANES + lane) * 8; col < a.width; col += gridDim.y * LANES * 8)
+          store_some<R, 8>((R *)a.to + (int64_t)(word0 + k) * a.pitch, col, a.width, V8<R>{});
+    return;
+  }
+  const uint32_t group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, col = (blockIdx.y * LANES + lane) * 8;
+  const uint64_t first = (uint64_t)group * a.length;
+  if (group >= a.groups || col >= a.width) return;
+  const uint64_t end = first + a.length < a.rows ? first + a.length : a.rows;
+  uint32_t key = a.keys[first];
+  if (key >= a.word0 + a.words || a.keys[end - 1] < a.word0) return;
+  bool whole = !(first && a.keys[first - 1] == key);  // the word's rows begin in this piece
+  f32x8 sum = {};
+  // Where a sum goes that ends here: the result's row, or a part for the second launch.
+  auto put = [&](bool ends) {
+    const uint32_t word = key - a.word0;
+    if (word >= a.words) return;
+    if (whole && ends) {
+      store_some<R, 8>((R *)a.to + (int64_t)word * a.pitch, col, a.width, __builtin_convertvector(sum * a.scale, V8<R>));
+    } else {
+      store_some<float, 8>(a.parts + ((uint64_t)group * 2 + (whole ? 1 : 0)) * a.width, col, a.width, sum);
+    }
+  };
+  constexpr uint32_t kAhead = 8;
+  for (uint64_t i = first; i < end; i += kAhead) {
+    uint32_t keys[kAhead];
+    f32x8 v[kAhead];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      const bool there = i + k < end;
+      keys[k] = there ? a.keys[i + k] : ~0u;
+      const uint32_t row = there ? a.order[i + k] : 0;
+      const bool wanted = keys[k] - a.word0 < a.words;
+      v[k] = __builtin_convertvector((load_some<T, 8>((const T *)a.from + (int64_t)row * a.stride, wanted, col, a.width)), f32x8);
+      if (a.weights && wanted) v[k] *= a.weights[row];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      if (i + k >= end) break;
+      if (keys[k] != key) {
+        put(true);
+        key = keys[k], sum = f32x8{}, whole = true;
+      }
+      sum += v[k];
+    }
+  }
+  put(end == a.rows || a.keys[end] != key);
+}
+
+// A word whose rows began in a piece and go on in the next: its parts in their order. A block a piece; its lanes'
+// groups take a stretch of the parts each.
+template <class R, int LANES>
+__global__ __launch_bounds__(256) void sorted_join(Sums a) {
+  constexpr uint32_t kGroups = 256 / LANES;
+  __shared__ float joined[kGroups][LANES * 8 + 1];
+  const uint32_t group = blockIdx.x, lane = threadIdx.x % LANES, part = threadIdx.x / LANES, col = (blockIdx.y * LANES + lane) * 8;
+  const uint64_t first = (uint64_t)group * a.length, end = first + a.length;
+  if (end >= a.rows) return;
+  const uint32_t key = a.keys[end - 1];
+  if (key - a.word0 >= a.words || a.keys[end] != key) return;  // no word goes on
+  if (first && a.keys[first - 1] == key) return;               // it began before this piece
+  // The last piece that has it, by halves.
+  uint32_t lo = group + 1, hi = a.groups;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.keys[(uint64_t)mid * a.length] == key) lo = mid;
+    else hi = mid;
+  }
+  // This piece's second part, then the first ones of pieces group + 1 .. lo.
+  const uint32_t n = lo - group + 1, each = (n + kGroups - 1) / kGroups, from = part * each, to = from + each < n ? from + each : n;
+  f32x8 sum = {};
+#pragma unroll 8
+  for (uint32_t i = from; i < to; i++)
+    sum += load_some<float, 8>(a.parts + ((uint64_t)(group + i) * 2 + (i ? 0 : 1)) * a.width, true, col, a.width);
+#pragma unroll
+  for (int e = 0; e < 8; e++) joined[part][lane * 8 + e] = sum[e];
+  __syncthreads();
+  if (part || col >= a.width) return;
+  for (uint32_t p = 1; p < kGroups; p++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum[e] += joined[p][lane * 8 + e];
+  store_some<R, 8>((R *)a.to + (int64_t)(key - a.word0) * a.pitch, col, a.width, __builtin_convertvector(sum * a.scale, V8<R>));
+}
+
+// Lanes of a row: as many as hold it, eight values each, up to a wavefront.
+inline uint32_t lanes_of_row(uint32_t width) {
+  uint32_t lanes = 4;
+  while (lanes * 8 < width && lanes < 64) lanes *= 2;
+  return lanes;
+}
+// f of the number of lanes as a constant.
+template <class F>
+inline void with_lanes(uint32_t width, F f) {
+  switch (lanes_of_row(width)) {
+    case 4: f(std::integral_constant<int, 4>{}); break;
+    case 8: f(std::integral_constant<int, 8>{}); break;
+    case 16: f(std::integral_constant<int, 16>{}); break;
+    case 32: f(std::integral_constant<int, 32>{}); break;
+    default: f(std::integral_constant<int, 64>{});
+  }
+}
+
+// Host side: where a sort and its sums have what, `bytes` in all.
+struct SortPlan {
+  uint32_t passes, bits, blocks, share;  // passes 0: in one block
+  uint32_t length, groups;
+  uint64_t keys[2], order[2], counts, parts, bytes;
+};
+inline SortPlan sort_plan(uint32_t rows, uint32_t vocab, uint32_t width) {
+  SortPlan p{};
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    const uint64_t here = at;
+    at += (n + 255) / 256 * 256;
+    return here;
+  };
+  p.keys[0] = take(4ull * rows), p.order[0] = take(4ull * rows);
+  if (rows > kFew) {
+    uint32_t bits = 1;
+    while (vocab >> bits) bits++;  // of the largest word and of none
+    p.passes = (bits + 9) / 10;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    p.share = 2048;
+    while ((uint64_t)p.share * kSortBlocks < rows) p.share *= 2;
+    p.blocks = (rows + p.share - 1) / p.share;
+    p.keys[1] = take(4ull * rows), p.order[1] = take(4ull * rows);
+    p.counts = take(4ull * p.blocks << p.bits);
+  }
+  p.length = 16;
+  while (p.length < 64 && rows / p.length > 2048) p.length *= 2;
+  p.groups = (rows + p.length - 1) / p.length;
+  p.parts = take(8ull * p.groups * width);
+  p.bytes = at;
+  return p;
+}
+// Sorts the rows by their words; `a` takes what the sums need to know.
+inline void sort_rows(const SortPlan &p, const void *tokens, bool wide, uint32_t rows, uint32_t vocab, char *work, hipStream_t stream, Sums &a) {
+  uint32_t *k[2] = {(uint32_t *)(work + p.keys[0]), (uint32_t *)(work + p.keys[1])};
+  uint32_t *f[2] = {(uint32_t *)(work + p.order[0]), (uint32_t *)(work + p.order[1])};
+  a.rows = rows, a.length = p.length, a.groups = p.groups, a.parts = (float *)(work + p.parts);
+  a.keys = k[0], a.order = f[0];
+  if (!rows) return;
+  if (!p.passes) {
+    uint32_t n = 2;
+    while (n < rows) n *= 2;
+    hipLaunchKernelGGL(sort_few, dim3(1), dim3(1024), n * sizeof(uint64_t), stream, tokens, wide, rows, vocab, n, k[0], f[0]);
+    return;
+  }
+  for (uint32_t i = 0; i < p.passes; i++) {
+    const Digit d{rows, vocab, p.share, i * p.bits, 1u << p.bits, wide, i ? nullptr : tokens, k[(i + 1) & 1], f[(i + 1) & 1],
+                  (uint32_t *)(work + p.counts), k[i & 1], f[i & 1]};
+    hipLaunchKernelGGL(sort_count, dim3(p.blocks), dim3(256), 0, stream, d);
+    hipLaunchKernelGGL(sort_place, dim3(p.blocks), dim3(256), 0, stream, d);
+    a.keys = d.keys_out, a.order = d.from_out;
+  }
+}
+template <class R, class T>
+inline void sum_rows(const Sums &a, hipStream_t stream) {
+  with_lanes(a.width, [&](auto lanes) {
+    constexpr uint32_t kGroups = 256 / lanes();
+    Sums b = a;
+    b.sum_blocks = (a.groups + kGroups - 1) / kGroups;
+    const uint32_t slices = (a.width + lanes() * 8 - 1) / (lanes() * 8);
+    hipLaunchKernelGGL((sorted_sums<R, T, lanes()>), dim3(b.sum_blocks + (a.words + 63) / 64, slices), dim3(256), 0, stream, b);
+    if (a.groups > 1) hipLaunchKernelGGL((sorted_join<R, lanes()>), dim3(a.groups - 1, slices), dim3(256), 0, stream, b);
+  });
+}
+
+}  // namespace trunk

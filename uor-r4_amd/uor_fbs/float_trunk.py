@@ -7,8 +7,10 @@ A layer takes the normed residual n of its rows and computes
     y           = scan(x, dt, A, B, C)
     residual'   = residual + scale rms((y W_out) silu(n W_gate)) post,  n' = rms(residual') pre
 
-with W_* products of torch. ``python -m uor_fbs.float_trunk`` trains one to repeat its prompts and then
-lets sessions go on from them token by token.
+with W_* products of torch. Its rows begin as the embedding's and end at the head over the vocabulary: as logits,
+or (``Config.keep_logits`` false) as a loss, its gradients and a choice of tokens that keep none.
+``python -m uor_fbs.float_trunk`` trains one to repeat its prompts and then lets sessions go on from them
+token by token.
 """
 
 from __future__ import annotations
@@ -30,6 +32,7 @@ class Config(NamedTuple):
     state: int = 32
     taps: int = 4
     dtype: torch.dtype = torch.bfloat16
+    keep_logits: bool = True  # the loss, its gradients and replies from whole logits of the trunk's type
 
     @property
     def inner(self):
@@ -88,10 +91,18 @@ def make_state(cfg, slots, device="cuda"):
                  [torch.zeros(slots, cfg.heads, cfg.dim, cfg.state, device=device) for _ in range(cfg.layers)])
 
 
-def prompts(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
-    """Logits (rows, vocab) of packed prompts. With ``state`` and ``slots`` (int64, one a prompt) the
-    prompts' final states are put into their slots; ``saved`` (a list) takes what the gradients need."""
-    residual = p["embed"].to(cfg.dtype)[tokens]
+def _logits(cfg, p, n):
+    return (n @ p["head"].to(cfg.dtype)).float()
+
+
+def _words(cfg, p):
+    """The head's matrix, a row a word."""
+    return p["head"].t().to(cfg.dtype, memory_format=torch.contiguous_format)
+
+
+def _prompt_rows(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
+    """The rows before the head of packed prompts."""
+    residual = trunk.embed(tokens, p["embed"], dtype=cfg.dtype)
     _, n = trunk.norms(residual, pre=p["first"])
     for i in range(cfg.layers):
         w = _layer(cfg, p, i)
@@ -107,12 +118,18 @@ def prompts(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
         residual, n = trunk.norms(residual, out, gate=gate, post=w["post"], scale=w["scale"], pre=w["pre"])
     if saved is not None:
         saved.append(n)
-    return (n @ p["head"].to(cfg.dtype)).float()
+    return n
 
 
-def step(cfg, p, tokens, state, slots):
-    """Logits (rows, vocab) of one more token of each session; ``slots`` (int32) says where it lives."""
-    residual = p["embed"].to(cfg.dtype)[tokens]
+def prompts(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
+    """Logits (rows, vocab) of packed prompts. With ``state`` and ``slots`` (int64, one a prompt) the
+    prompts' final states are put into their slots; ``saved`` (a list) takes what the gradients need."""
+    return _logits(cfg, p, _prompt_rows(cfg, p, tokens, offsets, state, slots, saved))
+
+
+def _step_rows(cfg, p, tokens, state, slots):
+    """The rows before the head of one more token of each session."""
+    residual = trunk.embed(tokens, p["embed"], dtype=cfg.dtype)
     _, n = trunk.norms(residual, pre=p["first"])
     for i in range(cfg.layers):
         w = _layer(cfg, p, i)
@@ -122,24 +139,36 @@ def step(cfg, p, tokens, state, slots):
         y = trunk.scan_step(x, rows[:, cfg.channels:], w["A"], B, C, state.scan[i], slots=slots, D=w["D"], dt_bias=w["dt_bias"])
         residual, n = trunk.norms(residual, y.flatten(1) @ w["w_out"], gate=n @ w["w_gate"], post=w["post"], scale=w["scale"],
                                   pre=w["pre"])
-    return (n @ p["head"].to(cfg.dtype)).float()
+    return n
+
+
+def step(cfg, p, tokens, state, slots):
+    """Logits (rows, vocab) of one more token of each session; ``slots`` (int32) says where it lives."""
+    return _logits(cfg, p, _step_rows(cfg, p, tokens, state, slots))
 
 
 def gradients(cfg, p, tokens, targets, offsets):
     """(loss, {name: gradient}): the mean cross entropy of the rows' next tokens (target -1: none)."""
     saved = []
-    logits = prompts(cfg, p, tokens, offsets, saved=saved)
+    n = _prompt_rows(cfg, p, tokens, offsets, saved=saved)
     wanted = targets >= 0
     count = wanted.sum().clamp(min=1)
-    log = torch.log_softmax(logits, 1)
-    at = targets.clamp(min=0)[:, None]
-    loss = -(log.gather(1, at)[:, 0] * wanted).sum() / count
-    d_logits = torch.exp(log)
-    d_logits.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float32))
-    d_logits = (d_logits * (wanted / count)[:, None]).to(cfg.dtype)
-
-    grads = {"head": saved[-1].t().float() @ d_logits.float()}
-    d_n, d_residual = d_logits @ p["head"].to(cfg.dtype).t(), None
+    if cfg.keep_logits:
+        log = torch.log_softmax(_logits(cfg, p, n), 1)
+        at = targets.clamp(min=0)[:, None]
+        loss = -(log.gather(1, at)[:, 0] * wanted).sum() / count
+        d_logits = torch.exp(log)
+        d_logits.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float32))
+        d_logits = (d_logits * (wanted / count)[:, None]).to(cfg.dtype)
+        grads = {"head": n.t().float() @ d_logits.float()}
+        d_n = d_logits @ p["head"].to(cfg.dtype).t()
+    else:
+        words = _words(cfg, p)
+        losses, lse = trunk.loss(n, words, targets)
+        loss = losses.sum() / count
+        g = trunk.loss_backward(wanted / count, n, words, targets, lse, dtype=torch.float32)
+        grads, d_n = {"head": g.dweight.t()}, g.dx
+    d_residual = None
     for i in reversed(range(cfg.layers)):
         w = _layer(cfg, p, i)
         residual, n, rows, mixed, y, out, gate = saved[i]
@@ -159,7 +188,7 @@ def gradients(cfg, p, tokens, targets, offsets):
         grads.update({f"{i}.{k}": v for k, v in layer.items()})
     first = trunk.norms_backward(d_residual, d_n, saved[0][0], pre=p["first"])
     grads["first"] = first.dpre
-    grads["embed"] = torch.zeros_like(p["embed"]).index_add_(0, tokens, first.dresidual.float())
+    grads["embed"] = trunk.embed_backward(first.dresidual, tokens, p["embed"])
     return loss, grads
 
 
@@ -195,17 +224,23 @@ def reply(cfg, p, tokens, offsets, count, state, slots):
     """``count`` greedy tokens of each prompt's session, (prompts, count). A prompt has a token at least."""
     if bool((offsets[1:] <= offsets[:-1]).any()):
         raise ValueError("a prompt of no tokens has nothing that a reply could follow")
-    logits = prompts(cfg, p, tokens, offsets, state, slots.long())
-    now = logits[offsets[1:].long() - 1].argmax(1)
+    last = offsets[1:].long() - 1
+    if cfg.keep_logits:
+        now = prompts(cfg, p, tokens, offsets, state, slots.long())[last].argmax(1)
+        next_of = lambda now: step(cfg, p, now, state, slots).argmax(1)  # noqa: E731
+    else:
+        words = _words(cfg, p)
+        now, _ = trunk.choose(_prompt_rows(cfg, p, tokens, offsets, state, slots.long())[last], words)
+        next_of = lambda now: trunk.choose(_step_rows(cfg, p, now, state, slots), words)[0]  # noqa: E731
     said = [now]
     for _ in range(count - 1):
-        now = step(cfg, p, now, state, slots).argmax(1)
+        now = next_of(now)
         said.append(now)
     return torch.stack(said, 1)
 
 
 def main():
-    cfg, length = Config(), 8
+    cfg, length = Config(keep_logits=False), 8
     p = make_params(cfg)
     train(cfg, p, 400, length=length, report=50)
     tokens, _, _ = repeats(cfg, 32, length, torch.Generator().manual_seed(99))

@@ -36,12 +36,16 @@ SYMBOLS = ("uor_trunk_abi_version", "uor_trunk_last_error", "uor_trunk_sizeof_sc
            "uor_trunk_scan_backward_workspace_bytes", "uor_trunk_scan_backward_async", "uor_trunk_scan_step_async",
            "uor_trunk_conv_async", "uor_trunk_conv_backward_workspace_bytes", "uor_trunk_conv_backward_async",
            "uor_trunk_conv_step_async", "uor_trunk_norms_async", "uor_trunk_norms_backward_workspace_bytes",
-           "uor_trunk_norms_backward_async")
+           "uor_trunk_norms_backward_async", "uor_trunk_sizeof_embed", "uor_trunk_sizeof_head", "uor_trunk_embed_async",
+           "uor_trunk_embed_backward_workspace_bytes", "uor_trunk_embed_backward_async", "uor_trunk_loss_workspace_bytes",
+           "uor_trunk_loss_async", "uor_trunk_loss_backward_workspace_bytes", "uor_trunk_loss_backward_async",
+           "uor_trunk_choose_workspace_bytes", "uor_trunk_choose_async")
 ABI_VERSION = 1
 DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 MAX_DIM = MAX_STATE = 128
 MAX_TAPS = 4
 MAX_WIDTH = 8192
+MAX_VOCAB = MAX_ROWS = 1 << 24
 
 P, I64, U32, F32 = C.c_void_p, C.c_int64, C.c_uint32, C.c_float
 
@@ -72,6 +76,17 @@ class CNorms(C.Structure):
                                     "dresidual_out", "dnormed", "dresidual", "dout", "dgate", "dpost", "dscale", "dpre")])
 
 
+class CEmbed(C.Structure):
+    _fields_ = ([("device", C.c_int32)] + [(n, U32) for n in ("dtype", "table_dtype", "rows", "vocab", "width", "wide")] + [("scale", F32)]
+                + [(n, I64) for n in ("table_stride", "dy_stride")] + [(n, P) for n in ("tokens", "table", "y", "dy", "dtable")])
+
+
+class CHead(C.Structure):
+    _fields_ = ([("device", C.c_int32)] + [(n, U32) for n in ("dtype", "dweight_dtype", "rows", "vocab", "width", "wide", "reserved")]
+                + [(n, I64) for n in ("x_stride", "w_stride")]
+                + [(n, P) for n in ("x", "weight", "targets", "losses", "lse", "tokens", "logprobs", "dlosses", "dlse", "dx", "dweight")])
+
+
 class ScanGrads(NamedTuple):
     dx: torch.Tensor
     ddt: torch.Tensor
@@ -99,8 +114,19 @@ class NormGrads(NamedTuple):
     dpre: Optional[torch.Tensor]
 
 
+class LossGrads(NamedTuple):
+    dx: Optional[torch.Tensor]
+    dweight: Optional[torch.Tensor]
+
+
 _Tensor = torch.Tensor
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # none without a HIP device to call it for
+# Arguments and, of each call that takes them, whether it wants scratch memory.
+_FORMS = (("scan", CScan, {"scan": True, "scan_backward": True, "scan_step": False}),
+          ("conv", CConv, {"conv": False, "conv_backward": True, "conv_step": False}),
+          ("norms", CNorms, {"norms": False, "norms_backward": True}),
+          ("embed", CEmbed, {"embed": False, "embed_backward": True}),
+          ("head", CHead, {"loss": True, "loss_backward": True, "choose": True}))
 _lib = None
 _calls = {}  # name: (the call, its workspace's size or None)
 
@@ -113,20 +139,18 @@ def lib():
         L = C.CDLL(LIB_PATH)
         L.uor_trunk_abi_version.restype = U32
         L.uor_trunk_last_error.restype = C.c_char_p
-        for name, struct in (("scan", CScan), ("conv", CConv), ("norms", CNorms)):
+        for name, struct, forms in _FORMS:
             size = getattr(L, f"uor_trunk_sizeof_{name}")
             size.restype = C.c_uint64
             if size() != C.sizeof(struct) or L.uor_trunk_abi_version() != ABI_VERSION:
                 raise TrunkError(f"{LIB_PATH} is of another version: build it again")
-            forms = {"scan": ("", "_backward", "_step"), "conv": ("", "_backward", "_step"), "norms": ("", "_backward")}[name]
-            for form in forms:
-                call, bytes_of = getattr(L, f"uor_trunk_{name}{form}_async"), None
-                needs = form == "_backward" or (name == "scan" and form == "")
+            for form, needs in forms.items():
+                call, bytes_of = getattr(L, f"uor_trunk_{form}_async"), None
                 call.argtypes = [C.POINTER(struct)] + ([P, C.c_uint64] if needs else []) + [P]
                 if needs:
-                    bytes_of = getattr(L, f"uor_trunk_{name}{form}_workspace_bytes")
+                    bytes_of = getattr(L, f"uor_trunk_{form}_workspace_bytes")
                     bytes_of.argtypes, bytes_of.restype = [C.POINTER(struct)], C.c_uint64
-                _calls[name + form] = call, bytes_of
+                _calls[form] = call, bytes_of
         _lib = L
     return _lib
 
@@ -513,3 +537,155 @@ class _Norms(torch.autograd.Function):
             return (None,) * 7
         residual, out, gate, post, scale, pre = ctx.saved_tensors
         return (*norms_backward(dresidual_out, dnormed, residual, out, gate=gate, post=post, scale=scale, pre=pre, eps=ctx.eps), None)
+
+
+# ---------------------------------------------------------------------------------------------
+# The ends: the embedding, and the head's loss and choice.
+
+
+def _places(name, t, rows=None):
+    """A dense vector of tokens or targets, int32 or int64, and whether it is int64."""
+    _want(isinstance(t, _Tensor), "{} is no tensor", name)
+    _want(t.dtype in (torch.int32, torch.int64), "{} is {}, not int32 or int64", name, t.dtype)
+    _want(t.dim() == 1 if rows is None else t.shape == (rows,), "{} has shape {}, not {}", name, tuple(t.shape), ("rows",) if rows is None else (rows,))
+    return (t if t.is_contiguous() else t.contiguous()), int(t.dtype == torch.int64)
+
+
+def _matrix(name, t):
+    """The type, vocabulary and width of a table or a head's matrix."""
+    dtype = _dtype(t, name)
+    _want(t.dim() == 2, "{} has the axes word and value", name)
+    vocab, width = t.shape
+    _want(1 <= vocab <= MAX_VOCAB and 1 <= width <= MAX_WIDTH, "{} of {} words of {} values: at most {} of {}, and one of each", name, vocab, width,
+          MAX_VOCAB, MAX_WIDTH)
+    return dtype, vocab, width
+
+
+def _embed_args(tokens, table, scale, dtype):
+    kind, vocab, width = _matrix("table", table)
+    dtype = kind if dtype is None else dtype
+    _want(dtype in DTYPES, "dtype is {}, not bfloat16 or float32", dtype)
+    tokens, wide = _places("tokens", tokens)
+    rows = tokens.numel()
+    _want(rows <= MAX_ROWS, "{} rows are more than {}", rows, MAX_ROWS)
+    return CEmbed(0, DTYPES[dtype], DTYPES[kind], rows, vocab, width, wide, scale, 0, 0, _ptr(tokens)), tokens, dtype
+
+
+def embed(tokens, table, *, scale=1.0, dtype=None):
+    """y (rows, width) = scale table[tokens], rounded once to ``dtype`` (None: the table's). ``table``
+    (vocab, width) is float32 or bfloat16, ``tokens`` (rows) int32 or int64. A token outside the
+    vocabulary (padding) has a row of zeros and no part in the gradient."""
+    a, tokens, dtype = _embed_args(tokens, table, scale, dtype)
+    if _tracked((table,)):
+        return _Embed.apply(tokens, table, scale, dtype)
+    table, a.table_stride = _rows("table", table, table.dtype, table.shape, a.width)
+    index = _one_device(tokens, table)
+    y = torch.empty((a.rows, a.width), dtype=dtype, device=table.device)
+    a.table, a.y = _ptr(table), _ptr(y)
+    _call("embed", a, index)
+    return y
+
+
+def embed_backward(dy, tokens, table, *, scale=1.0):
+    """The gradient of ``embed`` at its table, of the table's shape and type: scale times the sums of dy's
+    rows by their token, in 32 bits and the rows' order, rounded once. Nothing of ``table`` is read."""
+    _want(dy is not None, "dy is no tensor")
+    a, tokens, dtype = _embed_args(tokens, table, scale, _dtype(dy, "dy"))
+    dy, a.dy_stride = _rows("dy", dy, dtype, (a.rows, a.width), a.width)
+    index = _one_device(dy, tokens, table)
+    got = _make(table)
+    a.dy, a.dtable = _ptr(dy), _ptr(got)
+    _call("embed_backward", a, index)
+    return got
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table, scale, dtype):
+        ctx.save_for_backward(tokens, table)
+        ctx.scale = scale
+        return embed(tokens, table, scale=scale, dtype=dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        tokens, table = ctx.saved_tensors
+        return None, embed_backward(dy, tokens, table, scale=ctx.scale), None, None
+
+
+def _head_args(x, weight, targets):
+    dtype, vocab, width = _matrix("weight", weight)
+    _want(isinstance(x, _Tensor) and x.dim() == 2, "x has the axes row and value")
+    rows = x.shape[0]
+    _want(rows <= MAX_ROWS, "{} rows are more than {}", rows, MAX_ROWS)
+    x, xs = _rows("x", x, dtype, (rows, width), width)
+    weight, ws = _rows("weight", weight, dtype, (vocab, width), width)
+    targets, wide = (None, 0) if targets is None else _places("targets", targets, rows)
+    return CHead(0, DTYPES[dtype], DTYPES[dtype], rows, vocab, width, wide, 0, xs, ws, _ptr(x), _ptr(weight), _ptr(targets)), (x, weight, targets)
+
+
+def loss(x, weight, targets):
+    """(losses, lse), float32 (rows): the softmax cross entropy of each row of x (rows, width) over the words of
+    ``weight`` (vocab, width; x's type), and the logarithm of its sum, without keeping the logits. ``targets``
+    (rows; int32 or int64) says each row's word; a row whose target is outside the vocabulary takes no part, and
+    both are 0 there. What is wanted of the losses (their mean over the rows with a target) is the caller's."""
+    _want(targets is not None, "targets is no tensor")
+    a, keep = _head_args(x, weight, targets)
+    if _tracked((x, weight)):
+        return _Loss.apply(x, weight, targets)
+    index = _one_device(*keep)
+    losses, lse = (torch.empty(a.rows, dtype=torch.float32, device=x.device) for _ in range(2))
+    a.losses, a.lse = _ptr(losses), _ptr(lse)
+    _call("loss", a, index)
+    return losses, lse
+
+
+def loss_backward(dlosses, x, weight, targets, lse, *, dlse=None, dtype=None):
+    """(dx, dweight): the gradients of ``loss`` at x and weight from those of its outputs (either may be None
+    for zeros) and the call's own ``lse``. The logits are computed again, a piece of the vocabulary and of the rows
+    at a time; their gradient is rounded to x's type before its products with x and weight, which are summed in
+    32 bits. ``dtype``: dweight's type, weight's own without (float32 for a program that adds up
+    gradients of bfloat16 calls)."""
+    _want(targets is not None, "targets is no tensor")
+    a, keep = _head_args(x, weight, targets)
+    _want(lse is not None, "lse is no tensor")
+    lse, dlosses, dlse = (_dense(n, t, torch.float32, (a.rows,)) for n, t in (("lse", lse), ("dlosses", dlosses), ("dlse", dlse)))
+    dtype = weight.dtype if dtype is None else dtype
+    _want(dtype in DTYPES, "dtype is {}, not bfloat16 or float32", dtype)
+    index = _one_device(lse, dlosses, dlse, *keep)
+    got = LossGrads(_make(x), torch.empty(weight.shape, dtype=dtype, device=weight.device))
+    a.lse, a.dlosses, a.dlse, a.dweight_dtype = _ptr(lse), _ptr(dlosses), _ptr(dlse), DTYPES[dtype]
+    a.dx, a.dweight = map(_ptr, got)
+    _call("loss_backward", a, index)
+    return got
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets):
+        losses, lse = loss(x, weight, targets)
+        ctx.save_for_backward(x, weight, targets, lse)
+        ctx.set_materialize_grads(False)
+        return losses, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlosses, dlse):
+        if dlosses is None and dlse is None:
+            return None, None, None
+        x, weight, targets, lse = ctx.saved_tensors
+        got = loss_backward(dlosses, x, weight, targets, lse, dlse=dlse)
+        return got.dx, got.dweight, None
+
+
+def choose(x, weight):
+    """(tokens, logprobs): of each row of x (rows, width) the word of ``weight`` (vocab, width; x's type) with the
+    largest logit, the lowest of equals (int64), and its log probability (float32), without keeping the
+    logits. They have no gradient. Of a row with no logit over -inf the token is 0; logits that are no number are not chosen."""
+    a, keep = _head_args(x, weight, None)
+    index = _one_device(*keep)
+    tokens = torch.empty(a.rows, dtype=torch.int64, device=x.device)
+    logprobs = torch.empty(a.rows, dtype=torch.float32, device=x.device)
+    a.tokens, a.logprobs = _ptr(tokens), _ptr(logprobs)
+    _call("choose", a, index)
+    return tokens, logprobs
