@@ -153,7 +153,7 @@ int uor_trunk_norms_backward_async(const uor_trunk_norms_args *args, void *works
  * Tokens and targets are int32, or int64 where `wide` is 1. E and W are [vocab][width], dense inside, in
  * bf16 or f32 (W in the type of x), their rows `*_stride` values apart.
  */
-#define UOR_TRUNK_MAX_VOCAB 0x1000000u
+#define UOR_TRUNK_MAX_VOCAB 0x800000u
 #define UOR_TRUNK_MAX_ROWS 0x1000000u
 
 uint64_t uor_trunk_sizeof_embed(void);

@@ -132,7 +132,7 @@ def test_c_entries_refuse_before_they_reach_a_device():
 
     calls = (L.uor_trunk_loss_async, L.uor_trunk_loss_backward_async, L.uor_trunk_choose_async)
     for change, text in [(dict(dtype=2), "dtype"), (dict(width=0), "width"), (dict(width=8193), "width"), (dict(vocab=0), "vocabulary"),
-                         (dict(vocab=(1 << 24) + 1), "vocabulary"), (dict(rows=(1 << 24) + 1), "rows"), (dict(x_stride=7), "overlap"),
+                         (dict(vocab=(1 << 23) + 1), "vocabulary"), (dict(rows=(1 << 24) + 1), "rows"), (dict(x_stride=7), "overlap"),
                          (dict(w_stride=7), "overlap"), (dict(x=None), "null x"), (dict(weight=None), "null x or weight")]:
         for call in calls:
             assert call(C.byref(head(**change)), None, 0, None) == -1 and text in last(), (change, last())
@@ -164,16 +164,19 @@ def test_c_entries_refuse_before_they_reach_a_device():
 
 
 @built
-@pytest.mark.parametrize("rows,vocab,width", [(32768, 32768, 256), (262144, 32768, 256), (8192, 131072, 1024), (1 << 20, 131072, 512)])
+@pytest.mark.parametrize("rows,vocab,width", [(32768, 32768, 256), (262144, 32768, 256), (8192, 131072, 1024), (1 << 20, 131072, 512), (1 << 20, 1 << 23, 64)])
 def test_scratch_memory_does_not_grow_with_the_logits(rows, vocab, width):
-    """A piece of the logits' gradient is of 2^28 bytes at most; the rest goes by rows x width and by words x width."""
+    """A piece of the logits' gradient is of 2^30 bytes at most; the rest goes by rows x width and by words x width."""
     L = trunk.lib()
     a = trunk.CHead(dtype=0, rows=rows, vocab=vocab, width=width, x_stride=width, w_stride=width, x=16, weight=16)
-    # Sums so far of 32 bits: dx's of all rows and dW's of a piece, in up to 512 tiles' worth of splits; packed rows; the sort and its parts.
-    most = (1 << 28) + 4 * 2 * max(rows * width, 512 * 256 * 128) + 4 * 2 * max(vocab * width, 512 * 256 * 128) + 4 * vocab * width
-    most += rows * width * 3 + rows * 64 + (1 << 22)
+    # Sums so far of 32 bits: dx's and dW's in up to 512 tiles' worth of splits, or of one piece of the one and all of the other,
+    # and the targets' terms; the matrix and the rows laid out; the sort and its parts.
+    laid = 2 * width * (vocab + 2 * rows)
+    most = (1 << 30) + 4 * 2 * max(rows * width, 512 * 256 * 128) + 4 * 3 * max(vocab * width, 512 * 256 * 128) + laid
+    most += rows * width // 8 + rows * 64 + (1 << 22)
     assert 0 < L.uor_trunk_loss_backward_workspace_bytes(C.byref(a)) <= most
-    assert 0 < L.uor_trunk_loss_workspace_bytes(C.byref(a)) <= rows * width * 2 + rows * 16 + 32 * max(rows * 2, 1024 * 128 * 2) + (1 << 20)
+    # Two sums of a row for each part of the words: 2,048 blocks' worth, or one part.
+    assert 0 < L.uor_trunk_loss_workspace_bytes(C.byref(a)) <= laid + rows * 16 + 32 * (max(rows, 2048 * 128) + (1 << 16))
 
 
 def test_the_struct_sizes_are_the_librarys():

@@ -6,8 +6,8 @@ namespace trunk {
 
 // A call's matrices as the kernels read them: rows 16 bytes aligned, whole numbers of 16 bytes wide.
 struct Matrix {
-  const void *at;
-  int64_t pitch;  // bytes from row to row
+  const char *at;
+  int64_t pitch;  // bytes from row to row, or from panel to panel
 };
 // What is known of a row's softmax in base 2: its largest logit, the sum of 2^(logit - largest), and the
 // target's logit, or the largest one's value and place.
@@ -27,6 +27,14 @@ __device__ __forceinline__ uint32_t by_xcd(uint32_t block, uint32_t n) {
   return xcd * each + (xcd < more ? xcd : more) + (block >> 3);
 }
 
+// A block's row tile and share of the words. Blocks of an XCD go through eight row tiles by all shares before
+// the next eight, so that what runs at once reads few rows and few words.
+__device__ __forceinline__ void by_eights(uint32_t work, uint32_t row_tiles, uint32_t splits, uint32_t &row_tile, uint32_t &split) {
+  const uint32_t group = work / (8 * splits), left = work - group * 8 * splits, rows = min(8u, row_tiles - group * 8);
+  row_tile = group * 8 + left % rows;
+  split = left / rows;
+}
+
 // Scratch memory, a stretch at a time.
 struct Scratch {
   uint64_t bytes = 0;
@@ -44,6 +52,12 @@ inline bool as_it_lies(const void *p, int64_t stride, uint32_t rows, uint32_t wi
   return (uint64_t)width * size % 16 == 0 && ((uintptr_t)p & 15) == 0 &&
          (rows <= 1 || (stride * size % 16 == 0 && stride * (int64_t)size < (1 << 23)));
 }
+// From how many rows on a matrix is laid out by panels, whose rows could be read as they lie: it is then read
+// by many row tiles. XXX
+constexpr uint32_t kLayRows = 1024;
+inline bool laid_out(const uor_trunk_head_args *s) { return s->rows >= kLayRows || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype); }
+// Whether small tiles fill the card better: the large ones would leave some of its compute units idle. XXX
+inline bool small_tiles(uint64_t rows, uint64_t words) { return up(rows, Large::kN) / Large::kN * (up(words, Large::kM) / Large::kM) < 256; }
 inline int check_head(const uor_trunk_head_args *s) {
   if (!s) return fail(-1, "null argument");
   if (s->dtype > UOR_TRUNK_F32) return fail(-1, "dtype %u is neither bf16 nor f32", s->dtype);

@@ -14,10 +14,10 @@ namespace trunk {
 struct Scan {
   Matrix w, x;
   uint32_t rows, vocab, width;  // width: values of a row, whole 16 bytes
-  uint32_t row_tiles, word_tiles, splits;
+  uint32_t row_tiles, word_tiles, splits;  // in the shape's tiles
   const uint32_t *count;        // how many rows there are, or NULL: `rows`
   const int32_t *target;        // [rows up to 256]
-  Sum *parts;                   // [2 splits][128 row_tiles]
+  Sum *parts;                   // [2 splits][rows of row_tiles]
 };
 
 // A logit's running softmax in base 2.
@@ -30,59 +30,61 @@ struct Running {
   }
 };
 
-template <class T, bool PICK>
+template <class T, class S, bool PICK, Lies W>
 struct ScanTiles {
+  static constexpr Lies kX = PICK ? W : PANELS;
+  static constexpr int kStores = 0;
   const Scan &a;
   uint32_t tiles, stages, row0, word0;
   int lane, wave;
-  Running run[2];
-  float value[2];
-  uint32_t place[2];
-  int32_t target[2];
+  Running run[S::N];
+  float value[S::N];
+  uint32_t place[S::N];
+  int32_t target[S::N];
 
   template <class FA, class FB>
   __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
-    const uint32_t word = word0 + n * kTileM;
-    fa.start((const T *)((const char *)a.w.at + (int64_t)word * a.w.pitch), a.w.pitch, a.vocab - word, a.width);
-    fb.start((const T *)((const char *)a.x.at + (int64_t)row0 * a.x.pitch), a.x.pitch, a.rows - row0, a.width);
+    const uint32_t word = word0 + n * S::kM;
+    fa.start(a.w.at + (int64_t)word * (W == ROWS ? a.w.pitch : 64), a.w.pitch, a.vocab - word, a.width);
+    fb.start(a.x.at + (int64_t)row0 * (kX == ROWS ? a.x.pitch : 64), a.x.pitch, a.rows - row0, a.width);
   }
-  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[4][2]) {
+  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[S::M][S::N]) {
     const int half = lane >> 5;
-    const uint32_t word = word0 + n * kTileM + 128 * (wave >> 1);
-    if (word + 128 > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // words that are none
+    const uint32_t word = word0 + n * S::kM + 32 * S::M * (wave >> 1);
+    if (word + 32 * S::M > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // words that are none
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < S::N; j++) {
       float most = z[0][j][0];
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) most = fmaxf(most, z[i][j][r]);
       if constexpr (PICK) {
         if (__any(most > value[j])) {  // seldom after the first tiles
           uint32_t at = 0;
 #pragma unroll
-          for (int i = 3; i >= 0; i--)
+          for (int i = S::M - 1; i >= 0; i--)
 #pragma unroll
             for (int r = 15; r >= 0; r--) at = z[i][j][r] == most ? 32 * i + row_of(r, 0) : at;
           if (most > value[j]) value[j] = most, place[j] = word + at + 4 * half;
         }
       } else {
         const uint32_t at = (uint32_t)target[j] - word;
-        if (__any(at < 128)) {
+        if (__any(at < 32 * S::M)) {
           const int own = (int)at - 4 * half;
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+          for (int i = 0; i < S::M; i++)
 #pragma unroll
             for (int r = 0; r < 16; r++) value[j] = own == 32 * i + row_of(r, 0) ? z[i][j][r] : value[j];
         }
       }
       const float base = fmaxf(run[j].most, most * kLog2e);
-      float sum[4] = {};
+      float sum[S::M] = {};
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) sum[i] += exp2_(fmaf(z[i][j][r], kLog2e, -base));
-      run[j].sum = fmaf(run[j].sum, exp2_(run[j].most - base), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      run[j].sum = fmaf(run[j].sum, exp2_(run[j].most - base), S::M > 2 ? (sum[0] + sum[1]) + (sum[2] + sum[S::M - 1]) : sum[0] + sum[1]);
       run[j].most = base;
     }
   }
@@ -100,44 +102,47 @@ __device__ __forceinline__ void join_value(float &value, uint32_t &place, float 
   }
 }
 
-template <class T, bool PICK>
-__global__ __launch_bounds__(256, 2) void head_scan(Scan a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
-  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), split = work / a.row_tiles;
-  const uint32_t row0 = work % a.row_tiles * kTileN;
+template <class T, class S, bool PICK, Lies W>
+__global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+  uint32_t row_tile, split;
+  by_eights(by_xcd(blockIdx.x, gridDim.x), a.row_tiles, a.splits, row_tile, split);
+  const uint32_t row0 = row_tile * S::kN;
   if (a.count && row0 >= *a.count) return;
   const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  ScanTiles<T, PICK> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, first * kTileM, lane, wave};
+  ScanTiles<T, S, PICK, W> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, first * S::kM, lane, wave};
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+  for (int j = 0; j < S::N; j++) {
     tiles.value[j] = PICK ? -__builtin_inff() : 0.0f, tiles.place[j] = 0;
-    tiles.target[j] = PICK ? -1 : a.target[row0 + 64 * (wave & 1) + 32 * j + (lane & 31)];
+    tiles.target[j] = PICK ? -1 : a.target[row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)];
   }
-  run_tiles<T, true, true>(lds, tiles);
+  run_tiles<T, S, true, W, true, tiles.kX>(lds, tiles);
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+  for (int j = 0; j < S::N; j++) {
     Running run = tiles.run[j];
     run.join(__shfl_xor(run.most, 32), __shfl_xor(run.sum, 32));
     float value = tiles.value[j];
     uint32_t place = tiles.place[j];
     join_value<PICK>(value, place, __shfl_xor(value, 32), __shfl_xor(place, 32));
     if (lane < 32)
-      a.parts[(uint64_t)(2 * split + (wave >> 1)) * (a.row_tiles * kTileN) + row0 + 64 * (wave & 1) + 32 * j + lane] =
+      a.parts[(uint64_t)(2 * split + (wave >> 1)) * (a.row_tiles * S::kN) + row0 + 32 * S::N * (wave & 1) + 32 * j + lane] =
           Sum{run.most, run.sum, value, place};
   }
 }
 
-// A wavefront joins a row's parts, which are `across` apart.
-template <bool PICK>
+// WAVES wavefronts join a row's parts, which are `across` apart.
+template <bool PICK, int WAVES>
 __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, uint32_t across, uint32_t rows, const uint32_t *count,
                                                  const int32_t *order, float *losses, float *lse, int64_t *tokens, float *logprobs) {
-  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= (count ? *count : rows)) return;
+  __shared__ Sum joined[4];
+  const uint32_t row = blockIdx.x * (4 / WAVES) + threadIdx.x / (64 * WAVES), lane = threadIdx.x % (64 * WAVES);
+  if (row >= (count ? *count : rows)) return;  // with WAVES of 4: all of the block
   Running run;
   float value = PICK ? -__builtin_inff() : 0.0f;
   uint32_t place = PICK ? ~0u : 0;
-  for (uint32_t i = lane; i < n; i += 64) {
+#pragma unroll 4
+  for (uint32_t i = lane; i < n; i += 64 * WAVES) {
     const Sum p = parts[(uint64_t)i * across + row];
     run.join(p.most, p.sum);
     join_value<PICK>(value, place, p.value, p.place);
@@ -146,6 +151,14 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, u
   for (int k = 1; k < 64; k <<= 1) {
     run.join(__shfl_xor(run.most, k), __shfl_xor(run.sum, k));
     join_value<PICK>(value, place, __shfl_xor(value, k), __shfl_xor(place, k));
+  }
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) joined[threadIdx.x >> 6] = Sum{run.most, run.sum, value, place};
+    __syncthreads();
+    for (int w = 1; w < WAVES; w++) {
+      run.join(joined[w].most, joined[w].sum);
+      join_value<PICK>(value, place, joined[w].value, joined[w].place);
+    }
   }
   if (lane) return;
   const double sum = ((double)run.most + (double)log2f(run.sum)) * kLn2;
@@ -161,16 +174,18 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, u
 
 namespace {
 
-// Parts of the vocabulary that blocks take by themselves: as many as fill the card twice over with blocks of
-// which two share a compute unit.
-uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles) {
-  const uint32_t want = (1024 + row_tiles - 1) / row_tiles;
-  return want < 1 ? 1 : want < word_tiles ? want : word_tiles;
+// Parts of the vocabulary that blocks take by themselves. The card takes 512 blocks of large tiles at once (1,024 of
+// small ones). Four times as many even out; but a block of few tiles spends its time on its first loads, so a part
+// has four tiles at least where that leaves no compute unit idle.
+uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
+  const uint32_t even = (4 * at_once + row_tiles - 1) / row_tiles, fill = (at_once + row_tiles - 1) / row_tiles;
+  const uint32_t most = fill > word_tiles / 4 ? fill : word_tiles / 4, n = even < most ? even : most;
+  return n < 1 ? 1 : n < word_tiles ? n : word_tiles;
 }
 
 // Where a call's scratch memory has what.
 struct Plan {
-  bool lay;  // the matrix is laid out anew
+  bool lay, small;  // the matrix is laid out anew; small tiles
   uint32_t width, row_tiles, word_tiles, splits;
   uint64_t parts, w, x, order, target, counts, count, bytes;
 };
@@ -178,28 +193,25 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
   Plan p{};
   const uint32_t size = size_of(s->dtype);
   p.width = (uint32_t)up(s->width, 16 / size);
-  p.lay = !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
-  p.row_tiles = (s->rows + kTileN - 1) / kTileN;
-  p.word_tiles = (s->vocab + kTileM - 1) / kTileM;
-  p.splits = splits_of(p.row_tiles ? p.row_tiles : 1, p.word_tiles);
+  p.lay = pick ? !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype) ||
+                     !as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)
+               : laid_out(s);
+  p.small = small_tiles(s->rows, s->vocab);
+  const uint32_t n = p.small ? Small::kN : Large::kN, m = p.small ? Small::kM : Large::kM;
+  p.row_tiles = (s->rows + n - 1) / n;
+  p.word_tiles = (s->vocab + m - 1) / m;
+  p.splits = splits_of(p.row_tiles, p.word_tiles, p.small ? 1024 : 512);
   Scratch at;
-  const uint64_t rows = up(s->rows, kTileM);
-  p.parts = at.take(2ull * p.splits * p.row_tiles * kTileN * sizeof(Sum));
-  p.w = at.take(p.lay ? (uint64_t)s->vocab * p.width * size : 0);
-  p.x = at.take(pick && as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype) ? 0 : rows * p.width * size);
+  const uint64_t rows = up(s->rows, kRound);
+  p.parts = at.take(2ull * p.splits * p.row_tiles * n * sizeof(Sum));
+  p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
+  p.x = at.take(pick && !p.lay ? 0 : rows * up(s->width * size, 64));
   p.order = at.take(pick ? 0 : rows * 4);
   p.target = at.take(pick ? 0 : rows * 4);
   p.counts = at.take(pick ? 0 : (s->rows + kPackRows - 1) / kPackRows * 4);
   p.count = at.take(pick ? 0 : 4);
   p.bytes = at.bytes;
   return p;
-}
-
-template <class T>
-void lay(const void *from, int64_t stride, uint32_t rows, uint32_t width, uint32_t pitch, void *to, hipStream_t stream) {
-  const uint64_t blocks = ((uint64_t)rows * (pitch / kVec<T>) + 255) / 256;
-  hipLaunchKernelGGL((head_lay<T>), dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (const T *)from, stride, rows, width,
-                     pitch, (T *)to);
 }
 
 template <class T, bool PICK>
@@ -209,32 +221,33 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   a.rows = s->rows, a.vocab = s->vocab, a.width = p.width;
   a.row_tiles = p.row_tiles, a.word_tiles = p.word_tiles, a.splits = p.splits;
   a.parts = (Sum *)(work + p.parts);
-  a.w = {s->weight, s->w_stride * (int64_t)sizeof(T)};
-  if (p.lay) {
-    lay<T>(s->weight, s->w_stride, s->vocab, s->width, p.width, work + p.w, stream);
-    a.w = {work + p.w, (int64_t)p.width * (int64_t)sizeof(T)};
-  }
-  a.x = {work + p.x, (int64_t)p.width * (int64_t)sizeof(T)};
+  a.w = {(const char *)s->weight, s->w_stride * (int64_t)sizeof(T)};
+  if (p.lay) a.w = lay<T>(s->weight, s->w_stride, s->vocab, s->width, work + p.w, stream);
   if constexpr (PICK) {
-    if (as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)) a.x = {s->x, s->x_stride * (int64_t)sizeof(T)};
-    else lay<T>(s->x, s->x_stride, s->rows, s->width, p.width, work + p.x, stream);
+    if (p.lay) a.x = lay<T>(s->x, s->x_stride, s->rows, s->width, work + p.x, stream);
+    else a.x = {(const char *)s->x, s->x_stride * (int64_t)sizeof(T)};
   } else {
     Pack k{};
-    k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.pitch = p.width, k.stride = s->x_stride;
+    k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.piece = (uint32_t)up(s->rows, kRound), k.stride = s->x_stride;
+    a.x = {work + p.x, (int64_t)k.piece * 64};
     k.x = s->x, k.targets = s->targets, k.wide = s->wide != 0;
     k.to = work + p.x, k.order = (int32_t *)(work + p.order), k.target = (int32_t *)(work + p.target);
     k.count = (uint32_t *)(work + p.count), k.losses = s->losses, k.lse = s->lse;
-    const uint32_t blocks = (s->rows + kPackRows - 1) / kPackRows;
-    if (s->rows > 4096) {
-      hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, s->targets, k.wide, s->rows, s->vocab, (uint32_t *)(work + p.counts));
-      k.counts = (const uint32_t *)(work + p.counts);
-    }
-    hipLaunchKernelGGL((head_pack<T, false>), dim3(blocks), dim3(256), 0, stream, k);
+    pack<T, false>(k, (uint32_t *)(work + p.counts), stream);
     a.count = k.count, a.target = k.target;
   }
-  hipLaunchKernelGGL((head_scan<T, PICK>), dim3(p.row_tiles * p.splits), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL((head_join<PICK>), dim3((s->rows + 3) / 4), dim3(256), 0, stream, a.parts, 2 * p.splits, p.row_tiles * kTileN, s->rows,
-                     a.count, PICK ? nullptr : (const int32_t *)(work + p.order), s->losses, s->lse, s->tokens, s->logprobs);
+  const dim3 grid(p.row_tiles * p.splits);
+  const uint32_t across = p.row_tiles * (p.small ? Small::kN : Large::kN);
+  if (p.small && p.lay) hipLaunchKernelGGL((head_scan<T, Small, PICK, PANELS>), grid, dim3(256), 0, stream, a);
+  else if (p.small) hipLaunchKernelGGL((head_scan<T, Small, PICK, ROWS>), grid, dim3(256), 0, stream, a);
+  else if (p.lay) hipLaunchKernelGGL((head_scan<T, Large, PICK, PANELS>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((head_scan<T, Large, PICK, ROWS>), grid, dim3(256), 0, stream, a);
+  const auto join = [&](auto kernel, uint32_t each) {
+    hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, a.parts, 2 * p.splits, across, s->rows, a.count,
+                       PICK ? nullptr : (const int32_t *)(work + p.order), s->losses, s->lse, s->tokens, s->logprobs);
+  };
+  if (p.splits > 64) join(head_join<PICK, 4>, 1);
+  else join(head_join<PICK, 1>, 4);
   return launched();
 }
 

@@ -3,8 +3,7 @@
 //   G_tv = (dloss_t + dlse_t) e^(z_tv - lse_t) - dloss_t [v = target_t],  dx = G W,  dW = G^T x.
 //
 // A piece of the rows by a piece of the vocabulary at a time: one launch computes the piece's logits again
-// and writes its G, in the type of x, to scratch memory that the caches hold; one takes G W and one G^T x from
-// it. dx is summed over the pieces of the vocabulary and dW over those of the rows, in 32 bits. Where a piece has
+// and writes its G, in the type of x, to scratch memory; one takes G W and one G^T x from it. dx is summed over the pieces of the vocabulary and dW over those of the rows, in 32 bits. Where a piece has
 // fewer tiles than the card takes at once, its sums are split along their axis and joined at the end.
 //
 // G is rounded to bf16 where x is, half a step (2^-8) of each value, independent of the others. Of the largest,
@@ -16,59 +15,61 @@
 namespace trunk {
 
 struct Logits {
-  Matrix w, x;
+  Matrix w, x;      // x: the piece's panels
   uint32_t rows, vocab, width;
-  uint32_t row0, row_tiles, word0, word_tiles, splits;  // the piece, in tiles of 128 rows and 256 words
+  uint32_t row0, row_tiles, word0, word_tiles, splits;  // the piece, in the shape's tiles
   const uint32_t *count;
   const int32_t *target;
   const float4 *factors;
   const int32_t *order;
   float *terms;     // [rows of the call]: the targets' G, where x is bf16
-  void *g;          // [128 row_tiles][pitch]
-  uint32_t pitch;   // values
+  char *g;          // [words / a panel's][g_rows][64 bytes]
+  uint32_t g_rows;
 };
 
-template <class T>
+template <class T, class S, Lies W>
 struct LogitTiles {
+  static constexpr int kStores = S::M * S::N * (sizeof(T) == 2 ? 2 : 4);
   const Logits &a;
   uint32_t tiles, stages, row0, word0;  // row0 in the piece, word0 of the vocabulary
   int lane, wave;
-  float base[2], all[2], one[2];
-  int32_t target[2], place[2];
+  float base[S::N], all[S::N], one[S::N];
+  int32_t target[S::N], place[S::N];
 
   template <class FA, class FB>
   __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
-    const uint32_t word = word0 + n * kTileM, row = a.row0 + row0;
-    fa.start((const T *)((const char *)a.w.at + (int64_t)word * a.w.pitch), a.w.pitch, a.vocab - word, a.width);
-    fb.start((const T *)((const char *)a.x.at + (int64_t)row * a.x.pitch), a.x.pitch, kTileN, a.width);
+    const uint32_t word = word0 + n * S::kM;
+    fa.start(a.w.at + (int64_t)word * (W == ROWS ? a.w.pitch : 64), a.w.pitch, a.vocab - word, a.width);
+    fb.start(a.x.at + row0 * 64, a.x.pitch, S::kN, a.width);
   }
-  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[4][2]) {
+  __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[S::M][S::N]) {
     const int half = lane >> 5;
-    const uint32_t word = word0 + n * kTileM + 128 * (wave >> 1);
-    if (word + 128 > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // their G is 0
+    const uint32_t word = word0 + n * S::kM + 32 * S::M * (wave >> 1);
+    if (word + 32 * S::M > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // their G is 0
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < S::N; j++) {
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) z[i][j][r] = all[j] * exp2_(fmaf(z[i][j][r], kLog2e, -base[j]));
       const uint32_t at = (uint32_t)target[j] - word;
-      if (__any(at < 128)) {
+      if (__any(at < 32 * S::M)) {
         float term = 0.0f;
         const int own = (int)at - 4 * half;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < S::M; i++)
 #pragma unroll
           for (int r = 0; r < 16; r++) {
             const bool here = own == 32 * i + row_of(r, 0);
             if constexpr (sizeof(T) == 2) term = here ? z[i][j][r] : term, z[i][j][r] = here ? 0.0f : z[i][j][r];
             else z[i][j][r] -= here ? one[j] : 0.0f;
           }
-        if (sizeof(T) == 2 && at < 128 && (int)(at >> 2 & 1) == half) a.terms[place[j]] = term - one[j];
+        if (sizeof(T) == 2 && at < 32 * S::M && (int)(at >> 2 & 1) == half) a.terms[place[j]] = term - one[j];
       }
-      T *to = (T *)a.g + (uint64_t)(row0 + 64 * (wave & 1) + 32 * j + (lane & 31)) * a.pitch + (word - a.word0);
+      const uint64_t panel = (uint64_t)a.g_rows * 64;
+      char *to = a.g + (word - a.word0) / kDeep<T> * panel + (row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)) * 64;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < S::M; i++) {
         if constexpr (sizeof(T) == 2) {
           // A lane has four words of every eight, the lane 32 on the other four: they change places, so that
           // each writes eight next to each other.
@@ -82,38 +83,40 @@ struct LogitTiles {
               const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi), false, false);
               p[0][e] = both[0], p[1][e] = both[1];
             }
-            *(u32x4 *)(to + 32 * i + 8 * (q + half)) = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
+            *(u32x4 *)(to + i * panel + 16 * (q + half)) = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
           }
         } else {
 #pragma unroll
           for (int q = 0; q < 4; q++)
-            *(f32x4 *)(to + 32 * i + 8 * q + 4 * half) = f32x4{z[i][j][4 * q], z[i][j][4 * q + 1], z[i][j][4 * q + 2], z[i][j][4 * q + 3]};
+            *(f32x4 *)(to + (2 * i + q / 2) * panel + 32 * (q & 1) + 16 * half) = f32x4{z[i][j][4 * q], z[i][j][4 * q + 1], z[i][j][4 * q + 2], z[i][j][4 * q + 3]};
         }
       }
     }
   }
 };
 
-template <class T>
-__global__ __launch_bounds__(256, 2) void head_logits(Logits a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
-  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), split = work / a.row_tiles, row0 = work % a.row_tiles * kTileN;
+template <class T, class S, Lies W>
+__global__ __launch_bounds__(256, S::kBlocks) void head_logits(Logits a) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+  uint32_t row_tile, split;
+  by_eights(by_xcd(blockIdx.x, gridDim.x), a.row_tiles, a.splits, row_tile, split);
+  const uint32_t row0 = row_tile * S::kN;
   if (a.row0 + row0 >= *a.count) return;
   const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  LogitTiles<T> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, a.word0 + first * kTileM, lane, wave};
+  LogitTiles<T, S, W> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, a.word0 + first * S::kM, lane, wave};
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const uint32_t row = a.row0 + row0 + 64 * (wave & 1) + 32 * j + (lane & 31);
+  for (int j = 0; j < S::N; j++) {
+    const uint32_t row = a.row0 + row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31);
     const float4 f = a.factors[row];
     tiles.base[j] = f.x, tiles.all[j] = f.y, tiles.one[j] = f.z, tiles.target[j] = a.target[row], tiles.place[j] = a.order[row];
   }
-  run_tiles<T, true, true>(lds, tiles);
+  run_tiles<T, S, true, W, true, PANELS>(lds, tiles);
 }
 
 // A product of a piece: out[m][n] (+)= sum_k a[m][k] b[k][n] over a share of its k.
 struct Product {
-  Matrix a, b;             // b lies across: rows of k
+  Matrix a, b;             // a: panels of G
   uint32_t m, n, k;        // sums of the piece; k may be fewer, see Limit
   uint32_t m_tiles, n_tiles, splits;
   uint32_t row0;           // the piece's first packed row
@@ -125,26 +128,32 @@ struct Product {
   bool first;              // nothing has been summed before
 };
 
-// ROWS: the summed axis are the rows of x (dW), else the words (dx).
-template <class T, bool ROWS>
+// DW: the summed axis are the rows of x, else the words. B: how x or the matrix lies.
+template <class T, class S, bool DW, Lies B>
 struct ProductTiles {
+  static constexpr int kStores = 0;
   const Product &p;
   uint32_t tiles, stages, m0, n0, k0, depth, split;
   int lane, wave;
   template <class FA, class FB>
   __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
-    if constexpr (ROWS) fa.start((const T *)((const char *)p.a.at + (int64_t)k0 * p.a.pitch) + m0, p.a.pitch, p.m - m0, depth);
-    else fa.start((const T *)((const char *)p.a.at + (int64_t)m0 * p.a.pitch) + k0, p.a.pitch, kTileM, depth);
-    fb.start((const T *)((const char *)p.b.at + (int64_t)k0 * p.b.pitch) + n0, p.b.pitch, p.n - n0, depth);
+    // k0, m0 and n0 are whole panels.
+    if constexpr (DW) {
+      fa.start(p.a.at + m0 / kDeep<T> * p.a.pitch + (uint64_t)k0 * 64, p.a.pitch, p.m - m0, depth);
+    } else {
+      fa.start(p.a.at + k0 / kDeep<T> * p.a.pitch + (uint64_t)m0 * 64, p.a.pitch, S::kM, depth);
+    }
+    if constexpr (B == PANELS) fb.start(p.b.at + n0 / kDeep<T> * p.b.pitch + (uint64_t)k0 * 64, p.b.pitch, p.n - n0, depth);
+    else fb.start(p.b.at + (int64_t)k0 * p.b.pitch + n0 * sizeof(T), p.b.pitch, p.n - n0, depth);
   }
-  __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[4][2]) {
+  __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[S::M][S::N]) {
     const int half = lane >> 5;
-    float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 128 * (wave >> 1)) * p.n_pitch + n0 + 64 * (wave & 1) + (lane & 31);
+    float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 32 * S::M * (wave >> 1)) * p.n_pitch + n0 + 32 * S::N * (wave & 1) + (lane & 31);
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      if (n0 + 64 * (wave & 1) + 32 * j + (lane & 31) >= p.n) continue;
+    for (int j = 0; j < S::N; j++) {
+      if (n0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31) >= p.n) continue;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           float *at = to + (uint64_t)(32 * i + row_of(r, half)) * p.n_pitch + 32 * j;
@@ -154,14 +163,14 @@ struct ProductTiles {
   }
 };
 
-template <class T, bool ROWS>
-__global__ __launch_bounds__(256, 2) void head_product(Product p) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
-  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), n0 = work % p.n_tiles * kTileN, rest = work / p.n_tiles;
-  const uint32_t m0 = rest % p.m_tiles * kTileM, split = rest / p.m_tiles;
+template <class T, class S, bool DW, Lies B>
+__global__ __launch_bounds__(256, S::kBlocks) void head_product(Product p) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), n0 = work % p.n_tiles * S::kN, rest = work / p.n_tiles;
+  const uint32_t m0 = rest % p.m_tiles * S::kM, split = rest / p.m_tiles;
   const uint32_t count = *p.count, there = count > p.row0 ? count - p.row0 : 0;  // of the piece's rows
   uint32_t k = p.k;
-  if constexpr (ROWS) k = there < k ? there : k;
+  if constexpr (DW) k = there < k ? there : k;
   else if (m0 >= there) return;
   // The share of the summed axis, in stages.
   const uint32_t all = (k + kDeep<T> - 1) / kDeep<T>;
@@ -169,8 +178,8 @@ __global__ __launch_bounds__(256, 2) void head_product(Product p) {
   if (s0 == s1 && !p.first) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t k0 = s0 * kDeep<T>, k1 = s1 * kDeep<T> < k ? s1 * kDeep<T> : k;
-  ProductTiles<T, ROWS> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, lane, wave};
-  run_tiles<T, !ROWS, false>(lds, tiles);
+  ProductTiles<T, S, DW, B> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, lane, wave};
+  run_tiles<T, S, !DW, PANELS, false, B>(lds, tiles);
 }
 
 // The splits' sums in their order, rounded to the result's type. dx: packed rows go to their own places, with
@@ -182,7 +191,8 @@ struct Ends {
   const uint32_t *count;   // dx's: how many packed rows there are, or NULL
   const int32_t *order, *target;
   const float *terms;      // or NULL
-  Matrix w;
+  const void *w;           // the matrix as the caller has it
+  int64_t w_stride;
   void *to;
 };
 template <class R>
@@ -193,10 +203,11 @@ __global__ __launch_bounds__(256) void head_sums(Ends a) {
     const uint64_t row = i / pieces;
     const uint32_t col = (uint32_t)(i % pieces) * 8;
     f32x8 v = load_some<float, 8>(a.parts + row * a.n_pitch, true, col, a.n);
+#pragma unroll 8
     for (uint32_t s = 1; s < a.splits; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
     const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.row0 + row] : row;
     if (a.terms)
-      v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)((const char *)a.w.at + a.target[a.row0 + row] * a.w.pitch), true, col, a.n)), f32x8) *
+      v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)a.w + a.target[a.row0 + row] * a.w_stride, true, col, a.n)), f32x8) *
            a.terms[place];
     store_some<R, 8>((R *)a.to + place * a.n, col, a.n, __builtin_convertvector(v, V8<R>));
   }
@@ -210,40 +221,49 @@ __global__ __launch_bounds__(256) void head_nothing(R *to, uint64_t n) {
 
 namespace {
 
-constexpr uint64_t kPiece = 1ull << 28;  // bytes of G: what the last cache holds
+// Bytes of a piece's G. Larger pieces read and write the sums so far less often; this much is a small part of
+// the memory of the card. Loss and gradients of 32,768 rows (a quarter without a target) at width 256 and 32,768
+// words: 256 MB 3,447 us, 512 MB 2,827, 1 GB 2,612, 2 GB 2,591; 8,192 rows at width 1,024 and 131,072 words: 9,019,
+// 8,796, 8,674 and 8,758.
+constexpr uint64_t kPiece = 1ull << 30;
 
 struct GradPlan {
-  bool lay;
-  uint32_t width, rows, words;           // a row's values; rows and words of a piece, whole tiles
+  bool lay, small;
+  uint32_t width, rows, words;  // a row's values; rows and words of a piece, whole tiles
   uint32_t all_rows, all_words;          // of the call, whole tiles
   uint32_t n_tiles, x_splits, w_splits, n_pitch;
   uint32_t x_rows, w_rows;               // how many rows' and words' sums are kept at once
   SortPlan sort;                         // of the targets, where x is bf16
   uint64_t g, dx, dw, w, x, order, target, factors, terms, sorted, counts, count, bytes;
 };
-uint32_t splits_for(uint32_t tiles, uint32_t stages) {
-  const uint32_t want = 512 / tiles, most = stages / 8;
+uint32_t splits_for(uint32_t at_once, uint32_t tiles, uint32_t stages) {
+  const uint32_t want = at_once / tiles, most = stages / 8;
   return want < 2 || most < 2 ? 1 : want < most ? want : most;
+}
+// The size of even pieces of `all` that are `most` at most, in whole large tiles.
+uint32_t even_pieces(uint64_t all, uint64_t most) {
+  const uint64_t n = (all + most - 1) / most;
+  return (uint32_t)up((all + n - 1) / n, kRound);
 }
 GradPlan grad_plan(const uor_trunk_head_args *s) {
   GradPlan p{};
   const uint32_t size = size_of(s->dtype), deep = 64 / size;
   p.width = (uint32_t)up(s->width, 16 / size);
-  p.lay = !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
-  p.all_rows = (uint32_t)up(s->rows, kTileM), p.all_words = (uint32_t)up(s->vocab, kTileM);
+  p.lay = laid_out(s);
+  p.small = small_tiles(s->rows, s->vocab);
+  const uint32_t tile_m = p.small ? Small::kM : Large::kM, tile_n = p.small ? Small::kN : Large::kN, at_once = p.small ? 1024 : 512;
+  p.all_rows = (uint32_t)up(s->rows, kRound), p.all_words = (uint32_t)up(s->vocab, kRound);
   // A piece of about as many rows as words, whose sums are read and written the least for the G between.
   const uint64_t values = kPiece / size;
-  uint64_t side = kTileM;
-  while ((side + kTileM) * (side + kTileM) <= values) side += kTileM;
-  p.rows = p.all_rows < side ? p.all_rows : (uint32_t)side;
-  const uint64_t words = values / p.rows / kTileM * kTileM;
-  p.words = p.all_words < words ? p.all_words : (uint32_t)words;
-  const uint64_t rows = values / p.words / kTileM * kTileM;
-  p.rows = p.all_rows < rows ? p.all_rows : (uint32_t)rows;
-  p.n_tiles = (p.width + kTileN - 1) / kTileN;
-  p.n_pitch = p.n_tiles * kTileN;
-  p.x_splits = splits_for(p.rows / kTileM * p.n_tiles, p.words / deep);
-  p.w_splits = splits_for(p.words / kTileM * p.n_tiles, p.rows / deep);
+  uint64_t side = kRound;
+  while ((side + kRound) * (side + kRound) <= values) side += kRound;
+  p.rows = even_pieces(p.all_rows, side);
+  p.words = even_pieces(p.all_words, values / p.rows / kRound * kRound);
+  p.rows = even_pieces(p.all_rows, values / p.words / kRound * kRound);
+  p.n_tiles = (p.width + tile_n - 1) / tile_n;
+  p.n_pitch = p.n_tiles * tile_n;
+  p.x_splits = splits_for(at_once, p.rows / tile_m * p.n_tiles, p.words / deep);
+  p.w_splits = splits_for(at_once, p.words / tile_m * p.n_tiles, p.rows / deep);
   // With the rows' pieces outside, the sums of dx are kept of one of them and those of dW of all words; or the
   // other way round.
   const bool rows_outside = (uint64_t)p.x_splits * (p.all_rows - p.rows) > (uint64_t)p.w_splits * (p.all_words - p.words);
@@ -252,8 +272,8 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   p.g = at.take((uint64_t)p.rows * p.words * size);
   p.dx = at.take(4ull * p.x_splits * p.x_rows * p.n_pitch);
   p.dw = at.take(4ull * (p.w_splits + (size == 2)) * p.w_rows * p.n_pitch);  // and the targets' terms
-  p.w = at.take(p.lay ? (uint64_t)s->vocab * p.width * size : 0);
-  p.x = at.take((uint64_t)p.all_rows * p.width * size);
+  p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
+  p.x = at.take(up(p.all_rows, p.rows) * up(s->width * size, 64));
   p.order = at.take(4ull * p.all_rows);
   p.target = at.take(4ull * p.all_rows);
   p.factors = at.take(16ull * p.all_rows);
@@ -277,27 +297,18 @@ void sums(const Ends &a, hipStream_t stream) {
 template <class T>
 int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const GradPlan p = grad_plan(s);
-  const int64_t pitch = (int64_t)p.width * (int64_t)sizeof(T), g_pitch = (int64_t)p.words * (int64_t)sizeof(T);
-  Matrix w{s->weight, s->w_stride * (int64_t)sizeof(T)}, x{work + p.x, pitch};
-  if (p.lay) {
-    const uint64_t blocks = ((uint64_t)s->vocab * (p.width / kVec<T>) + 255) / 256;
-    hipLaunchKernelGGL((head_lay<T>), dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (const T *)s->weight, s->w_stride,
-                       s->vocab, s->width, p.width, (T *)(work + p.w));
-    w = {work + p.w, pitch};
-  }
+  const int64_t panel = (int64_t)p.rows * 64;  // of G and of a piece of x
+  const uint32_t tile_m = p.small ? Small::kM : Large::kM, tile_n = p.small ? Small::kN : Large::kN, at_once = p.small ? 1024 : 512;
+  Matrix w{(const char *)s->weight, s->w_stride * (int64_t)sizeof(T)};
+  if (p.lay) w = lay<T>(s->weight, s->w_stride, s->vocab, s->width, work + p.w, stream);
   uint32_t *count = (uint32_t *)(work + p.count);
   Pack k{};
-  k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.pitch = p.width, k.stride = s->x_stride;
+  k.rows = s->rows, k.width = s->width, k.vocab = s->vocab, k.piece = p.rows, k.stride = s->x_stride;
   k.x = s->x, k.targets = s->targets, k.wide = s->wide != 0;
   k.to = work + p.x, k.order = (int32_t *)(work + p.order), k.target = (int32_t *)(work + p.target), k.count = count;
   k.lse_in = s->lse, k.dlosses = s->dlosses, k.dlse = s->dlse, k.factors = (float4 *)(work + p.factors);
-  k.dx = s->dx, k.dx_width = s->dx ? s->width : 0;
-  const uint32_t blocks = (s->rows + kPackRows - 1) / kPackRows;
-  if (s->rows > 4096) {
-    hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, s->targets, k.wide, s->rows, s->vocab, (uint32_t *)(work + p.counts));
-    k.counts = (const uint32_t *)(work + p.counts);
-  }
-  hipLaunchKernelGGL((head_pack<T, true>), dim3(blocks), dim3(256), 0, stream, k);
+  k.dx = s->dx;
+  pack<T, true>(k, (uint32_t *)(work + p.counts), stream);
   constexpr bool kTerms = sizeof(T) == 2;
   float *terms = kTerms ? (float *)(work + p.terms) : nullptr;
   Sums t{};
@@ -312,34 +323,45 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     const uint32_t row_piece = rows_outside ? i / word_pieces : i % row_pieces, word_piece = rows_outside ? i % word_pieces : i / row_pieces;
     const uint32_t row0 = row_piece * p.rows, word0 = word_piece * p.words;
     const uint32_t rows = s->rows - row0 < p.rows ? s->rows - row0 : p.rows, words = s->vocab - word0 < p.words ? s->vocab - word0 : p.words;
-    const uint32_t word_tiles = (words + kTileM - 1) / kTileM;
+    const uint32_t word_tiles = (words + tile_m - 1) / tile_m;
     Logits l{};
+    const Matrix x{work + p.x + (uint64_t)row0 * up(s->width * sizeof(T), 64), panel};
     l.w = w, l.x = x, l.rows = s->rows, l.vocab = s->vocab, l.width = p.width;
-    l.row0 = row0, l.row_tiles = (rows + kTileN - 1) / kTileN, l.word0 = word0, l.word_tiles = word_tiles;
-    const uint32_t want = (1024 + l.row_tiles - 1) / l.row_tiles;
+    l.row0 = row0, l.row_tiles = (rows + tile_n - 1) / tile_n, l.word0 = word0, l.word_tiles = word_tiles;
+    const uint32_t want = (2 * at_once + l.row_tiles - 1) / l.row_tiles;
     l.splits = want < word_tiles ? want : word_tiles;
-    l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.pitch = p.words;
-    hipLaunchKernelGGL((head_logits<T>), dim3(l.row_tiles * l.splits), dim3(256), 0, stream, l);
+    l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.g_rows = p.rows;
+    const dim3 logits(l.row_tiles * l.splits);
+    if (p.small && p.lay) hipLaunchKernelGGL((head_logits<T, Small, PANELS>), logits, dim3(256), 0, stream, l);
+    else if (p.small) hipLaunchKernelGGL((head_logits<T, Small, ROWS>), logits, dim3(256), 0, stream, l);
+    else if (p.lay) hipLaunchKernelGGL((head_logits<T, Large, PANELS>), logits, dim3(256), 0, stream, l);
+    else hipLaunchKernelGGL((head_logits<T, Large, ROWS>), logits, dim3(256), 0, stream, l);
     Product a{};
-    a.a = {work + p.g, g_pitch}, a.row0 = row0, a.count = count, a.n = p.width, a.n_tiles = p.n_tiles, a.n_pitch = p.n_pitch;
+    a.a = {work + p.g, panel}, a.row0 = row0, a.count = count, a.n = p.width, a.n_tiles = p.n_tiles, a.n_pitch = p.n_pitch;
     if (s->dx) {
-      a.b = {(const char *)w.at + (int64_t)word0 * w.pitch, w.pitch};
-      a.m = rows, a.k = words, a.m_tiles = (rows + kTileM - 1) / kTileM, a.splits = p.x_splits;
+      a.b = {w.at + (int64_t)word0 * (p.lay ? 64 : w.pitch), w.pitch};
+      a.m = rows, a.k = words, a.m_tiles = (rows + tile_m - 1) / tile_m, a.splits = p.x_splits;
       a.parts = (float *)(work + p.dx), a.m_rows = p.x_rows, a.m0 = rows_outside ? 0 : row0, a.first = word0 == 0;
-      hipLaunchKernelGGL((head_product<T, false>), dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a);
+      const dim3 grid(a.m_tiles * a.n_tiles * a.splits);
+      if (p.small && p.lay) hipLaunchKernelGGL((head_product<T, Small, false, PANELS>), grid, dim3(256), 0, stream, a);
+      else if (p.small) hipLaunchKernelGGL((head_product<T, Small, false, ROWS>), grid, dim3(256), 0, stream, a);
+      else if (p.lay) hipLaunchKernelGGL((head_product<T, Large, false, PANELS>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((head_product<T, Large, false, ROWS>), grid, dim3(256), 0, stream, a);
       if (word_piece + 1 == word_pieces) {
         Ends e{};
         e.n = s->width, e.n_pitch = p.n_pitch;
         e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.x_splits, e.rows = rows, e.row0 = row0, e.m_rows = p.x_rows;
-        e.count = count, e.order = k.order, e.target = k.target, e.terms = terms, e.w = w, e.to = s->dx;
+        e.count = count, e.order = k.order, e.target = k.target, e.terms = terms, e.w = s->weight, e.w_stride = s->w_stride, e.to = s->dx;
         sums<T>(e, stream);
       }
     }
     if (s->dweight) {
-      a.b = {work + p.x + (int64_t)row0 * pitch, pitch};
-      a.m = (uint32_t)up(words, kTileM), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
+      a.b = x;
+      a.m = (uint32_t)up(words, kRound), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
       a.parts = (float *)(work + p.dw), a.m_rows = p.w_rows, a.m0 = rows_outside ? word0 : 0, a.first = row0 == 0;
-      hipLaunchKernelGGL((head_product<T, true>), dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a);
+      const dim3 grid(a.m_tiles * a.n_tiles * a.splits);
+      if (p.small) hipLaunchKernelGGL((head_product<T, Small, true, PANELS>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((head_product<T, Large, true, PANELS>), grid, dim3(256), 0, stream, a);
       if (row_piece + 1 == row_pieces) {
         Ends e{};
         e.n = s->width, e.n_pitch = p.n_pitch;

@@ -4,25 +4,25 @@
 
 namespace trunk {
 
-constexpr uint32_t kPackRows = 64;  // rows of a block of the packing kernels
+constexpr uint32_t kPackRows = 64, kPackPieces = 32;  // rows of a block of the packing kernels, and 16-byte pieces of each
 
 // The rows of a call, and where those with a target go. Rows without one (a target outside 0 .. vocab - 1)
 // take no part: nothing of them is read, whatever it is, and no product is spent on them.
 struct Pack {
-  uint32_t rows, width, vocab, pitch;  // pitch: values of a packed row, the width up to whole 16 bytes
+  uint32_t rows, width, vocab;
+  uint32_t piece;         // packed rows of a piece, whose panels lie behind the piece's before
   int64_t stride;
   const void *x, *targets;
   bool wide;              // targets are of 64 bits
   const uint32_t *counts; // rows with a target in each block's share, or NULL: each block counts for itself
-  void *to;               // [rows up to 256][pitch]
+  char *to;               // [pieces][panels][piece][64 bytes]
   int32_t *order, *target;  // [rows up to 256]: a packed row's own row and target (-1: none)
   uint32_t *count;          // how many rows are packed
   float *losses, *lse;      // a loss: 0 for the rows without a target
   // a gradient's:
   const float *lse_in, *dlosses, *dlse;
   float4 *factors;          // [rows up to 256], see Factors
-  void *dx;                 // zeros for the rows without a target
-  uint32_t dx_width;
+  void *dx;                 // zeros for the rows without a target, or NULL
 };
 
 __device__ __forceinline__ int32_t target_of(const void *targets, bool wide, uint32_t row, uint32_t vocab) {
@@ -58,9 +58,15 @@ __device__ __forceinline__ float4 factors_of(float lse, float dloss, float dlse)
   return {hi, all * fmaf(left, 0.693147181f, 1.0f), dloss, 0.0f};
 }
 
+// Where 16 bytes of a packed row lie: the c-th of it.
+__device__ __forceinline__ uint64_t packed_at(const Pack &a, uint32_t panels, uint32_t row, uint32_t c) {
+  const uint32_t piece = row / a.piece;
+  return (((uint64_t)piece * panels + (c >> 2)) * a.piece + (row - piece * a.piece)) * 64 + (c & 3) * 16;
+}
+
 template <class T, bool GRAD>
 __global__ __launch_bounds__(256) void head_pack(Pack a) {
-  __shared__ uint32_t scratch[4], from[kPackRows];
+  __shared__ uint32_t scratch[4], from[kPackRows], none[kPackRows];
   const uint32_t first = blockIdx.x * kPackRows;
   uint32_t before = 0;
   if (a.counts) {
@@ -70,60 +76,89 @@ __global__ __launch_bounds__(256) void head_pack(Pack a) {
   }
   before = block_sum(before, scratch);
   const uint32_t row = first + threadIdx.x;
-  bool none = false;
+  // The block's pieces of each row; the first block of a share writes what there is one of a row.
+  const uint32_t panels = (a.width + kDeep<T> - 1) / kDeep<T>, piece0 = blockIdx.y * kPackPieces;
+  const uint32_t pieces = min(kPackPieces, panels * 4 - piece0);
+  const bool leads = blockIdx.y == 0;
   if (threadIdx.x < kPackRows) {
     const int32_t t = row < a.rows ? target_of(a.targets, a.wide, row, a.vocab) : -1;
-    const uint64_t which = __ballot(t >= 0);
+    const uint64_t which = __ballot(t >= 0), below = ((uint64_t)1 << threadIdx.x) - 1;
+    const uint32_t place = __builtin_popcountll(which & below);
     if (threadIdx.x == 0) scratch[0] = __builtin_popcountll(which);
-    none = row < a.rows && t < 0;
     if (t >= 0) {
-      const uint32_t place = __builtin_popcountll(which & (((uint64_t)1 << threadIdx.x) - 1));
       from[place] = row;
-      a.order[before + place] = (int32_t)row;
-      a.target[before + place] = t;
-      if constexpr (GRAD)
-        a.factors[before + place] = factors_of(a.lse_in[row], a.dlosses ? a.dlosses[row] : 0.0f, a.dlse ? a.dlse[row] : 0.0f);
-    } else if (row < a.rows) {
-      if (a.losses) a.losses[row] = 0.0f;
-      if (a.lse) a.lse[row] = 0.0f;
+      if (leads) {
+        a.order[before + place] = (int32_t)row;
+        a.target[before + place] = t;
+        if constexpr (GRAD)
+          a.factors[before + place] = factors_of(a.lse_in[row], a.dlosses ? a.dlosses[row] : 0.0f, a.dlse ? a.dlse[row] : 0.0f);
+      }
+    } else {
+      none[threadIdx.x - place] = row;
+      if (leads && row < a.rows) {
+        if (a.losses) a.losses[row] = 0.0f;
+        if (a.lse) a.lse[row] = 0.0f;
+      }
     }
   }
   __syncthreads();
-  const uint32_t n = scratch[0], pieces = a.pitch / kVec<T>;
+  const uint32_t n = scratch[0];
+#pragma unroll 4
   for (uint32_t i = threadIdx.x; i < n * pieces; i += 256) {
-    const uint32_t r = i / pieces, col = i % pieces * kVec<T>;
-    const auto v = load_some<T, kVec<T>>((const T *)a.x + (int64_t)from[r] * a.stride, true, col, a.width);
-    *(Part<T> *)((T *)a.to + (uint64_t)(before + r) * a.pitch + col) = v;
+    const uint32_t r = i / pieces, c = piece0 + i % pieces;
+    const auto v = load_some<T, kVec<T>>((const T *)a.x + (int64_t)from[r] * a.stride, true, c * kVec<T>, a.width);
+    *(Part<T> *)(a.to + packed_at(a, panels, before + r, c)) = v;
   }
   if constexpr (GRAD) {  // the share's rows without a target
-    for (uint32_t k = 0; k < kPackRows; k++) {
-      const uint32_t other = first + k;
-      if (other < a.rows && target_of(a.targets, a.wide, other, a.vocab) < 0)
-        for (uint32_t c = threadIdx.x; c < a.dx_width; c += 256) ((T *)a.dx)[(uint64_t)other * a.dx_width + c] = (T)0.0f;
-    }
+    if (a.dx)
+      for (uint32_t i = threadIdx.x; i < (kPackRows - n) * pieces; i += 256) {
+        const uint32_t r = none[i / pieces], col = (piece0 + i % pieces) * kVec<T>;
+        if (r < a.rows && col < a.width) store_some<T, kVec<T>>((T *)a.dx + (uint64_t)r * a.width, col, a.width, Part<T>{});
+      }
   }
-  (void)none;
   if (blockIdx.x + 1 < gridDim.x) return;
   // The last block: how many rows there are, and rows of nothing up to a tile's end.
-  const uint32_t all = before + n, end = (all + kTileM - 1) / kTileM * kTileM;
-  if (threadIdx.x == 0) *a.count = all;
-  for (uint32_t i = all + threadIdx.x; i < end; i += 256) {
-    a.order[i] = -1, a.target[i] = -1;
-    if constexpr (GRAD) a.factors[i] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t all = before + n, end = (all + kRound - 1) / kRound * kRound;
+  if (leads) {
+    if (threadIdx.x == 0) *a.count = all;
+    for (uint32_t i = all + threadIdx.x; i < end; i += 256) {
+      a.order[i] = -1, a.target[i] = -1;
+      if constexpr (GRAD) a.factors[i] = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
   }
-  for (uint64_t i = threadIdx.x; i < (uint64_t)(end - all) * pieces; i += 256)
-    *(Part<T> *)((T *)a.to + (uint64_t)(all + i / pieces) * a.pitch + i % pieces * kVec<T>) = Part<T>{};
+  for (uint32_t i = threadIdx.x; i < (end - all) * pieces; i += 256)
+    *(Part<T> *)(a.to + packed_at(a, panels, all + i / pieces, piece0 + i % pieces)) = Part<T>{};
 }
 
-// A matrix's rows as the tiles read them: `pitch` values, zeros past the width.
+// A matrix by panels, zeros past its width.
 template <class T>
-__global__ __launch_bounds__(256) void head_lay(const T *from, int64_t stride, uint32_t rows, uint32_t width, uint32_t pitch, T *to) {
-  const uint32_t pieces = pitch / kVec<T>;
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < (uint64_t)rows * pieces; i += gridDim.x * 256ull) {
-    const uint32_t col = (uint32_t)(i % pieces) * kVec<T>;
-    const uint64_t row = i / pieces;
-    *(Part<T> *)(to + row * pitch + col) = load_some<T, kVec<T>>(from + (int64_t)row * stride, true, col, width);
+__global__ __launch_bounds__(256) void head_lay(const T *from, int64_t stride, uint32_t rows, uint32_t width, uint32_t panels, uint32_t all, char *to) {
+  // A block takes 16 rows of four panels: 256 bytes of each are read, and 1 KB of each panel is written.
+  const uint32_t quads = (panels + 3) / 4;
+  for (uint64_t i = blockIdx.x; i < (uint64_t)((rows + 15) / 16) * quads; i += gridDim.x) {
+    const uint32_t row = (uint32_t)(i / quads) * 16 + threadIdx.x / 16, c = (uint32_t)(i % quads) * 16 + threadIdx.x % 16;
+    if (row < rows && c < panels * 4)
+      *(Part<T> *)(to + ((uint64_t)(c >> 2) * all + row) * 64 + (c & 3) * 16) = load_some<T, kVec<T>>(from + (int64_t)row * stride, true, c * kVec<T>, width);
   }
+}
+
+// Packs a call's rows; `counts` is scratch memory for a number a block.
+template <class T, bool GRAD>
+inline void pack(Pack k, uint32_t *counts, hipStream_t stream) {
+  const uint32_t blocks = (k.rows + kPackRows - 1) / kPackRows, panels = (k.width + kDeep<T> - 1) / kDeep<T>;
+  if (k.rows > 4096) {  // else each block counts the rows before its own by itself
+    hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, k.targets, k.wide, k.rows, k.vocab, counts);
+    k.counts = counts;
+  }
+  hipLaunchKernelGGL((head_pack<T, GRAD>), dim3(blocks, (panels * 4 + kPackPieces - 1) / kPackPieces), dim3(256), 0, stream, k);
+}
+template <class T>
+inline Matrix lay(const void *from, int64_t stride, uint32_t rows, uint32_t width, char *to, hipStream_t stream) {
+  const uint32_t panels = (width + kDeep<T> - 1) / kDeep<T>;
+  const uint64_t blocks = (uint64_t)((rows + 15) / 16) * ((panels + 3) / 4);
+  hipLaunchKernelGGL((head_lay<T>), dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (const T *)from, stride, rows, width,
+                     panels, rows, to);
+  return {to, (int64_t)rows * 64};
 }
 
 }  // namespace trunk

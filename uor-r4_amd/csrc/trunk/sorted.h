@@ -1,7 +1,7 @@
 // sorted.h - sums of rows by a number that each has, a word of the vocabulary: what the embedding's gradient and
 // the targets' terms of the head's share.
 //
-// The rows' numbers are sorted by their words, rows of a word staying in their order: up to 4,096 in one block,
+// The rows' numbers are sorted by their words, rows of a word staying in their order: up to 16,384 by counting,
 // more by digits of the word in two or three passes. Then pieces of the sorted rows are summed, each by the lanes
 // that hold a row of the result; a word whose rows go over a piece's end leaves its parts to a second launch, which
 // adds them up in their order. So a word that a large share of all rows has is summed by many. Other blocks of the
@@ -36,78 +36,102 @@ struct Sums {
 // ---------------------------------------------------------------------------------------------
 // The sort.
 
-constexpr uint32_t kFew = 4096, kSortBlocks = 512, kMostBins = 1024;
+// Up to kFew rows are sorted by counting: a row's place is how many words before its own there are. That reads
+// every word for every row, but in one launch, all from LDS: 16,384 rows take XXX us, by digits XXX.
+constexpr uint32_t kFew = 8192, kSortBlocks = 256, kMostBins = 1024, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 
-// Up to `n` (a power of two) rows in one block: pairs of a token and a row, all different, by exchanges.
-static __global__ __launch_bounds__(1024) void sort_few(const void *tokens, bool wide, uint32_t rows, uint32_t vocab, uint32_t n, uint32_t *keys,
-                                                       uint32_t *from) {
-  extern __shared__ uint64_t pairs[];
-  for (uint32_t i = threadIdx.x; i < n; i += 1024)
-    pairs[i] = i < rows ? (uint64_t)token_of(tokens, wide, i, vocab) << 32 | i : ~(uint64_t)0;
-  for (uint32_t size = 2; size <= n; size <<= 1)
-    for (uint32_t step = size >> 1; step; step >>= 1) {
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < n / 2; i += 1024) {
-        const uint32_t lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const uint64_t p = pairs[lo], q = pairs[hi];
-        if ((p > q) == !(lo & size)) pairs[lo] = q, pairs[hi] = p;
-      }
-    }
+// 64 rows a block, each of its eight wavefronts an eighth of all words; `all` is the rows up to whole 32.
+static __global__ __launch_bounds__(512) void sort_few(const void *tokens, bool wide, uint32_t rows, uint32_t vocab, uint32_t all, uint32_t *keys,
+                                                       uint32_t *order) {
+  extern __shared__ uint32_t words[];
+  __shared__ uint32_t counts[8][64];
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < all; i += 512) words[i] = i < rows ? token_of(tokens, wide, i, vocab) : ~0u;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < rows; i += 1024) keys[i] = (uint32_t)(pairs[i] >> 32), from[i] = (uint32_t)pairs[i];
+  const uint32_t lane = threadIdx.x & 63, part = threadIdx.x >> 6, row = blockIdx.x * 64 + lane, key = row < rows ? words[row] : 0;
+  const uint32_t each = all / 8, first = part * each;
+  // Rows before this one count with its own word too, rows behind it do not.
+  uint32_t n = 0;
+  using Four = __attribute__((ext_vector_type(4))) uint32_t;
+  if (first + each <= blockIdx.x * 64) {
+    for (uint32_t i = first; i < first + each; i += 4) {
+      const Four w = *(const Four *)(words + i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) n += w[e] <= key;
+    }
+  } else if (first >= blockIdx.x * 64 + 64) {
+    for (uint32_t i = first; i < first + each; i += 4) {
+      const Four w = *(const Four *)(words + i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) n += w[e] < key;
+    }
+  } else {
+    for (uint32_t i = first; i < first + each; i++) n += words[i] < key + (i < row);
+  }
+  counts[part][lane] = n;
+  __syncthreads();
+  if (part || row >= rows) return;
+  for (int k = 1; k < 8; k++) n += counts[k][lane];
+  keys[n] = key, order[n] = row;
 }
 
-// A pass over one digit of the tokens. A block has `share` rows next to each other, each of its
-// wavefronts a quarter of them.
+// A pass over one digit of the words. A block has `share` rows next to each other, each of its
+// wavefronts an even part of them.
 struct Digit {
   uint32_t rows, vocab, share, shift, bins;
   bool wide;
   const void *tokens;                // the first pass's, else NULL
-  const uint32_t *keys, *from;       // the pass before's
+  const uint32_t *keys, *order;      // the pass before's
   uint32_t *counts;                  // [blocks][bins]
-  uint32_t *keys_out, *from_out;
+  uint32_t *keys_out, *order_out;
   __device__ __forceinline__ uint32_t key(uint64_t i) const { return tokens ? token_of(tokens, wide, i, vocab) : keys[i]; }
 };
 __device__ __forceinline__ void count_digits(const Digit &a, uint32_t *bins, uint64_t first, uint64_t end) {
+#pragma unroll 4
   for (uint64_t i = first + (threadIdx.x & 63); i < end; i += 64) atomicAdd(&bins[(a.key(i) >> a.shift) & (a.bins - 1)], 1u);
 }
 __device__ __forceinline__ void share_of(const Digit &a, uint64_t &first, uint64_t &end) {
-  const uint32_t part = a.share / 4;
+  const uint32_t part = a.share / kSortWaves;
   first = (uint64_t)blockIdx.x * a.share + (threadIdx.x >> 6) * part;
   end = first + part < a.rows ? first + part : a.rows;
 }
-static __global__ __launch_bounds__(256) void sort_count(Digit a) {
+static __global__ __launch_bounds__(kSortThreads) void sort_count(Digit a) {
   __shared__ uint32_t bins[kMostBins];
-  for (uint32_t b = threadIdx.x; b < a.bins; b += 256) bins[b] = 0;
+  for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) bins[b] = 0;
   __syncthreads();
   uint64_t first, end;
   share_of(a, first, end);
   count_digits(a, bins, first, end);
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < a.bins; b += 256) a.counts[(uint64_t)blockIdx.x * a.bins + b] = bins[b];
+  for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) a.counts[(uint64_t)blockIdx.x * a.bins + b] = bins[b];
 }
 // A row goes behind all rows of lower digits, those of its digit in blocks before, in wavefronts
 // before and in its own wavefront before it.
-static __global__ __launch_bounds__(256) void sort_place(Digit a) {
-  __shared__ uint32_t at[4][kMostBins], sums[4];
-  for (uint32_t b = threadIdx.x; b < 4 * kMostBins; b += 256) (&at[0][0])[b] = 0;
+static __global__ __launch_bounds__(kSortThreads) void sort_place(Digit a) {
+  __shared__ uint32_t at[kSortWaves][kMostBins], before[kMostBins], all[kMostBins], sums[kSortWaves];
+  for (uint32_t b = threadIdx.x; b < kSortWaves * a.bins; b += kSortThreads) at[b / a.bins][b % a.bins] = 0;
+  for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) before[b] = all[b] = 0;
   __syncthreads();
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   uint64_t first, end;
   share_of(a, first, end);
   count_digits(a, at[wave], first, end);
-  // A thread's four digits next to each other: their rows in blocks before, and in all.
-  const uint32_t b0 = threadIdx.x * 4;
-  uint32_t before[4] = {}, all[4] = {};
-  for (uint32_t k = 0; k < gridDim.x; k++)
-#pragma unroll
-    for (uint32_t e = 0; e < 4; e++)
-      if (b0 + e < a.bins) {
-        const uint32_t n = a.counts[(uint64_t)k * a.bins + b0 + e];
-        before[e] += k < blockIdx.x ? n : 0;
-        all[e] += n;
-      }
-  uint32_t mine = all[0] + all[1] + all[2] + all[3], lower = mine;
+  // A digit's rows in blocks before and in all: a thread takes a digit and an even part of the blocks. The sums of
+  // whole numbers do not depend on their order.
+  {
+    const uint32_t parts = kSortThreads / a.bins, b = threadIdx.x % a.bins, part = threadIdx.x / a.bins;
+    const uint32_t from = part * gridDim.x / parts, to = (part + 1) * gridDim.x / parts;
+    uint32_t earlier = 0, sum = 0;
+#pragma unroll 16
+    for (uint32_t k = from; k < to; k++) {
+      const uint32_t n = a.counts[(uint64_t)k * a.bins + b];
+      earlier += k < blockIdx.x ? n : 0, sum += n;
+    }
+    atomicAdd(&before[b], earlier), atomicAdd(&all[b], sum);
+  }
+  __syncthreads();
+  const uint32_t b = threadIdx.x, mine = b < a.bins ? all[b] : 0;
+  uint32_t lower = mine;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
     const uint32_t v = __shfl_up(lower, k);
@@ -115,43 +139,54 @@ static __global__ __launch_bounds__(256) void sort_place(Digit a) {
   }
   if (lane == 63) sums[wave] = lower;
   __syncthreads();
-  lower -= mine;
-  for (uint32_t w = 0; w < wave; w++) lower += sums[w];
-#pragma unroll
-  for (uint32_t e = 0; e < 4; e++) {
-    if (b0 + e < a.bins) {
-      uint32_t place = lower + before[e];
-      for (uint32_t w = 0; w < 4; w++) {
-        const uint32_t n = at[w][b0 + e];
-        at[w][b0 + e] = place;
-        place += n;
-      }
+  if (b < a.bins) {
+    uint32_t place = lower - mine + before[b];
+    for (uint32_t w = 0; w < wave; w++) place += sums[w];
+    for (uint32_t w = 0; w < kSortWaves; w++) {
+      const uint32_t n = at[w][b];
+      at[w][b] = place;
+      place += n;
     }
-    lower += all[e];
   }
   __syncthreads();
-  for (uint64_t base = first; base < end; base += 64) {
-    const uint64_t i = base + lane;
-    const bool there = i < end;
-    const uint32_t key = there ? a.key(i) : 0, digit = (key >> a.shift) & (a.bins - 1);
-    uint64_t same = __ballot(there);  // the lanes of the same digit
-    for (uint32_t bit = 1; bit < a.bins; bit <<= 1) {
-      const uint64_t set = __ballot(there && (digit & bit));
-      same &= digit & bit ? set : ~set;
+  constexpr uint32_t kAhead = 4;
+  for (uint64_t base = first; base < end; base += 64 * kAhead) {
+    uint32_t keys[kAhead], rows[kAhead];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      const uint64_t i = base + 64 * k + lane;
+      keys[k] = i < end ? a.key(i) : 0;
+      rows[k] = i < end ? (a.tokens ? (uint32_t)i : a.order[i]) : 0;
     }
-    if (there) {
-      const uint32_t place = at[wave][digit] + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1));
-      a.keys_out[place] = key;
-      a.from_out[place] = a.tokens ? (uint32_t)i : a.from[i];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      const bool there = base + 64 * k + lane < end;
+      const uint32_t digit = (keys[k] >> a.shift) & (a.bins - 1);
+      uint64_t same = __ballot(there);  // the lanes of the same digit
+      for (uint32_t bit = 1; bit < a.bins; bit <<= 1) {
+        const uint64_t set = __ballot(there && (digit & bit));
+        same &= digit & bit ? set : ~set;
+      }
+      if (there) {
+        const uint32_t place = at[wave][digit] + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1));
+        a.keys_out[place] = keys[k];
+        a.order_out[place] = rows[k];
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (there && !(same >> lane >> 1)) at[wave][digit] += __builtin_popcountll(same);
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
-    if (there && !(same >> lane >> 1)) at[wave][digit] += __builtin_popcountll(same);
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // The sums.
+
+// The first of the sorted rows whose word is not before `key`, looked for by a whole wavefront.
+__device__ __forceinline__ uint32_t first_of(const uint32_t *keys, uint32_t rows, uint32_t key) {
+  if (!rows || keys[0] >= key) return 0;
+  return last_before<true>(rows, [&](uint32_t i) { return keys[i] < key; }) + 1;
+}
 
 // LANES lanes take a piece of `length` sorted rows and 8 LANES of their columns.
 template <class R, class T, int LANES>
@@ -160,7 +195,8 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
   if (blockIdx.x >= a.sum_blocks) {  // zeros: 64 words a block, those that do not occur
     const uint64_t word0 = (uint64_t)(blockIdx.x - a.sum_blocks) * 64;
     const uint32_t word = (uint32_t)word0 + (threadIdx.x & 63), key = a.word0 + word;
-    uint32_t lo = 0, hi = a.rows;
+    // The sorted rows of the 64 words: whole wavefronts look for their ends, and each lane for its word's between.
+    uint32_t lo = first_of(a.keys, a.rows, a.word0 + (uint32_t)word0), hi = first_of(a.keys, a.rows, a.word0 + (uint32_t)word0 + 64);
     while (lo < hi) {
       const uint32_t mid = (lo + hi) / 2;
       if (a.keys[mid] < key) lo = mid + 1;
@@ -191,25 +227,34 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
       store_some<float, 8>(a.parts + ((uint64_t)group * 2 + (whole ? 1 : 0)) * a.width, col, a.width, sum);
     }
   };
+  // Eight rows on their way at a time, and their words and numbers eight before.
   constexpr uint32_t kAhead = 8;
+  uint32_t keys[kAhead], rows[kAhead];
+  auto look = [&](uint64_t i) {
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      const uint64_t at = i + k < end ? i + k : end - 1;
+      keys[k] = a.keys[at], rows[k] = a.order[at];
+    }
+  };
+  look(first);
   for (uint64_t i = first; i < end; i += kAhead) {
-    uint32_t keys[kAhead];
+    uint32_t now[kAhead];
     f32x8 v[kAhead];
 #pragma unroll
     for (uint32_t k = 0; k < kAhead; k++) {
-      const bool there = i + k < end;
-      keys[k] = there ? a.keys[i + k] : ~0u;
-      const uint32_t row = there ? a.order[i + k] : 0;
-      const bool wanted = keys[k] - a.word0 < a.words;
-      v[k] = __builtin_convertvector((load_some<T, 8>((const T *)a.from + (int64_t)row * a.stride, wanted, col, a.width)), f32x8);
-      if (a.weights && wanted) v[k] *= a.weights[row];
+      now[k] = keys[k];
+      const bool wanted = i + k < end && keys[k] - a.word0 < a.words;
+      v[k] = __builtin_convertvector((load_some<T, 8>((const T *)a.from + (int64_t)rows[k] * a.stride, wanted, col, a.width)), f32x8);
+      if (a.weights && wanted) v[k] *= a.weights[rows[k]];
     }
+    look(i + kAhead);
 #pragma unroll
     for (uint32_t k = 0; k < kAhead; k++) {
       if (i + k >= end) break;
-      if (keys[k] != key) {
+      if (now[k] != key) {
         put(true);
-        key = keys[k], sum = f32x8{}, whole = true;
+        key = now[k], sum = f32x8{}, whole = true;
       }
       sum += v[k];
     }
@@ -229,13 +274,8 @@ __global__ __launch_bounds__(256) void sorted_join(Sums a) {
   const uint32_t key = a.keys[end - 1];
   if (key - a.word0 >= a.words || a.keys[end] != key) return;  // no word goes on
   if (first && a.keys[first - 1] == key) return;               // it began before this piece
-  // The last piece that has it, by halves.
-  uint32_t lo = group + 1, hi = a.groups;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.keys[(uint64_t)mid * a.length] == key) lo = mid;
-    else hi = mid;
-  }
+  // The last piece that has it.
+  const uint32_t lo = last_before<true>(a.groups, [&](uint32_t i) { return a.keys[(uint64_t)i * a.length] <= key; });
   // This piece's second part, then the first ones of pieces group + 1 .. lo.
   const uint32_t n = lo - group + 1, each = (n + kGroups - 1) / kGroups, from = part * each, to = from + each < n ? from + each : n;
   f32x8 sum = {};
@@ -289,8 +329,8 @@ inline SortPlan sort_plan(uint32_t rows, uint32_t vocab, uint32_t width) {
     uint32_t bits = 1;
     while (vocab >> bits) bits++;  // of the largest word and of none
     p.passes = (bits + 9) / 10;
-    p.bits = (bits + p.passes - 1) / p.passes;
-    p.share = 2048;
+    p.bits = (bits + p.passes - 1) / p.passes;  // 2^bits divides a block's threads
+    p.share = 4096;
     while ((uint64_t)p.share * kSortBlocks < rows) p.share *= 2;
     p.blocks = (rows + p.share - 1) / p.share;
     p.keys[1] = take(4ull * rows), p.order[1] = take(4ull * rows);
@@ -311,17 +351,16 @@ inline void sort_rows(const SortPlan &p, const void *tokens, bool wide, uint32_t
   a.keys = k[0], a.order = f[0];
   if (!rows) return;
   if (!p.passes) {
-    uint32_t n = 2;
-    while (n < rows) n *= 2;
-    hipLaunchKernelGGL(sort_few, dim3(1), dim3(1024), n * sizeof(uint64_t), stream, tokens, wide, rows, vocab, n, k[0], f[0]);
+    const uint32_t all = (rows + 31) / 32 * 32;
+    hipLaunchKernelGGL(sort_few, dim3((rows + 63) / 64), dim3(512), all * sizeof(uint32_t), stream, tokens, wide, rows, vocab, all, k[0], f[0]);
     return;
   }
   for (uint32_t i = 0; i < p.passes; i++) {
     const Digit d{rows, vocab, p.share, i * p.bits, 1u << p.bits, wide, i ? nullptr : tokens, k[(i + 1) & 1], f[(i + 1) & 1],
                   (uint32_t *)(work + p.counts), k[i & 1], f[i & 1]};
-    hipLaunchKernelGGL(sort_count, dim3(p.blocks), dim3(256), 0, stream, d);
-    hipLaunchKernelGGL(sort_place, dim3(p.blocks), dim3(256), 0, stream, d);
-    a.keys = d.keys_out, a.order = d.from_out;
+    hipLaunchKernelGGL(sort_count, dim3(p.blocks), dim3(kSortThreads), 0, stream, d);
+    hipLaunchKernelGGL(sort_place, dim3(p.blocks), dim3(kSortThreads), 0, stream, d);
+    a.keys = d.keys_out, a.order = d.order_out;
   }
 }
 template <class R, class T>

@@ -6,6 +6,10 @@
 // them, written by loads that go past the registers, so that two blocks share a compute unit and
 // one's matrix instructions run through the other's epilogue and barriers.
 //
+// Matrices that the kernels lay out themselves lie by panels: 64 bytes of each row, row after row, and then the rows'
+// next 64 bytes. A stage's part of 256 rows is then 16 KB in one piece along the summed axis, and 2 KB pieces across.
+// XXX
+//
 // An operand lies along the summed axis (its values for one row or column of the result next to each
 // other) or across it (a row apart). Along, a stage's rows are 64 bytes, and a lane reads the 16 bytes
 // that the matrix instruction wants of it; across, they come out of LDS by transposing reads (bf16) or
@@ -22,8 +26,18 @@ namespace trunk {
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
-constexpr int kTileM = 256, kTileN = 128, kStages = 3;
-constexpr int kStageBytes = (kTileM + kTileN) * 64, kLdsBytes = kStages * kStageBytes;
+constexpr int kStages = 3;
+// A block's tile: 2 x 2 wavefronts of M x N results of 32 x 32.
+template <int M_, int N_>
+struct Shape {
+  static constexpr int M = M_, N = N_, kM = 64 * M, kN = 64 * N, kLoads = M + N;
+  static constexpr int kStageBytes = (kM + kN) * 64, kLdsBytes = kStages * kStageBytes;
+  static constexpr int kBlocks = M * N > 4 ? 2 : 4;  // that share a compute unit
+};
+using Large = Shape<4, 2>;
+// XXX small
+using Small = Shape<2, 1>;
+constexpr int kRound = 256;  // rows and words are rounded up to whole large tiles
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset that no buffer has: the load gives zeros
 template <class T>
 constexpr int kVec = 16 / sizeof(T);  // values of 16 bytes
@@ -53,49 +67,59 @@ __device__ __forceinline__ f32x16 mma32(f32x4 a, f32x4 b, f32x16 c) {
 // The row of a 32 x 32 result that a lane's r-th value has; its column is lane % 32.
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 // -inf in the place of sums whose row is `limit` or more from the wavefront's first.
-__device__ __forceinline__ void cut_rows(f32x16 (&z)[4][2], uint32_t limit, int half) {
+template <int M, int N>
+__device__ __forceinline__ void cut_rows(f32x16 (&z)[M][N], uint32_t limit, int half) {
   const int own = (int)limit - 4 * half;
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < M; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const bool there = 32 * i + row_of(r, 0) < own;
-      z[i][0][r] = there ? z[i][0][r] : -__builtin_inff(), z[i][1][r] = there ? z[i][1][r] : -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < N; j++) z[i][j][r] = there ? z[i][j][r] : -__builtin_inff();
     }
 }
 
-// The places of 16-byte pieces in a row of a stage: piece c lies at c ^ twist(row).
-template <class T, bool ALONG>
+// The places of 16-byte pieces in a row of a stage: piece c lies at c ^ twist(row). R: the operand's rows (columns).
+template <class T, bool ALONG, int R>
 __device__ __forceinline__ uint32_t twist(uint32_t row) {
-  if constexpr (ALONG) return (row >> 2) & 3;          // 16 rows of 64 bytes cover the banks four times
-  else if constexpr (sizeof(T) == 2) return (row & 3) << 2;  // four rows are read at once, 64 bytes each
-  else return ((row >> 2) & 1) << 3;                   // two rows four apart, 128 bytes each
+  if constexpr (ALONG) return (row >> 2) & 3;                           // 16 rows of 64 bytes cover the banks four times
+  else if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) << 3;      // two rows four apart are read at once, 128 bytes each
+  else if constexpr (R >= 128) return (row & 3) << 2;                   // four rows, 64 bytes each, that lie 256 bytes or more apart
+  else return ((row >> 1) & 1) << 2;                                    // or 128
 }
 
-// A stage of both operands to LDS at `to` (the wavefront's own place of it), past the registers: the 256 rows'
-// four loads, the 128 rows' two, each 4 KB of the block. The wait for them is the caller's. The first wait is
+// A stage of both operands to LDS at `to` (the wavefront's own place of it), past the registers: the first one's
+// loads, then the second one's, each 4 KB of the block. The wait for them is the caller's. The first wait is
 // between what may have written the buffers' scalar registers and the loads that read them, the others
 // between m0 and the loads that take it.
+#define LOAD(at, buffer) "buffer_load_dwordx4 " at ", " buffer ", 0 offen lds\n\t"
+#define NEXT "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\t"
 __device__ __forceinline__ void to_lds(uint32_t to, u32x4 a, const uint32_t (&at)[4], u32x4 b, const uint32_t (&bt)[2]) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %7, 0 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %7, 0 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %7, 0 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %7, 0 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %8, 0 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tbuffer_load_dwordx4 %6, %8, 0 offen lds"
-      ::"s"(to), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(bt[0]), "v"(bt[1]), "s"(a), "s"(b)
-      : "memory", "scc");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" LOAD("%1", "%7") NEXT LOAD("%2", "%7") NEXT LOAD("%3", "%7") NEXT LOAD("%4", "%7") NEXT LOAD(
+                   "%5", "%8") NEXT LOAD("%6", "%8")
+               ::"s"(to), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(bt[0]), "v"(bt[1]), "s"(a), "s"(b)
+               : "memory", "scc");
 }
+__device__ __forceinline__ void to_lds(uint32_t to, u32x4 a, const uint32_t (&at)[2], u32x4 b, const uint32_t (&bt)[1]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" LOAD("%1", "%4") NEXT LOAD("%2", "%4") NEXT LOAD("%3", "%5")
+               ::"s"(to), "v"(at[0]), "v"(at[1]), "v"(bt[0]), "s"(a), "s"(b)
+               : "memory", "scc");
+}
+#undef LOAD
+#undef NEXT
 __device__ __forceinline__ u32x4 buffer_at(const char *base) {
   const uint64_t at = (uint64_t)base;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
   return u32x4{lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u};
 }
 
+// How a matrix lies in memory: row after row, `pitch` bytes apart, or by panels, which are `pitch` bytes apart.
+enum Lies { ROWS, PANELS };
+
 // One operand's way into LDS. Its R rows (columns of the result's, for the second operand) times the
 // stage's depth; what is past `there` of them or past the summed axis's `depth` is read as zeros.
-template <class T, bool ALONG, int R>
+template <class T, bool ALONG, Lies LIES, int R>
 struct Feed {
   static constexpr int kJobs = R * 4 / 256;  // loads a lane and stage
   static constexpr int kRow = ALONG ? 4 : R * (int)sizeof(T) / 16, kRows = 256 / kRow;  // pieces of a row, rows a load of the block
@@ -103,16 +127,18 @@ struct Feed {
   int64_t step;
   uint32_t off[kJobs];
   int left;
-  // `pitch` bytes from row to row in memory; 256 of them are under 2^31. `base` is aligned to 16.
-  __device__ __forceinline__ void start(const T *from, int64_t pitch, uint32_t there, uint32_t depth) {
-    base = (const char *)from;
-    step = ALONG ? 64 : kDeep<T> * pitch;
+  // `from` is the operand's first value, aligned to 16 bytes (to a panel's row where panels are read across).
+  // What an operand's rows (256 of them), or its panels, cover in memory is under 2^31 bytes.
+  __device__ __forceinline__ void start(const char *from, int64_t pitch, uint32_t there, uint32_t depth) {
+    base = from;
+    step = ALONG ? (LIES == ROWS ? 64 : pitch) : kDeep<T> * (LIES == ROWS ? pitch : 64);
     const uint32_t row = threadIdx.x / kRow, place = threadIdx.x % kRow;
-    left = (int)depth - (int)(ALONG ? (place ^ twist<T, true>(row)) * kVec<T> : row);
+    left = (int)depth - (int)(ALONG ? (place ^ twist<T, true, R>(row)) * kVec<T> : row);
 #pragma unroll
     for (int i = 0; i < kJobs; i++) {
-      const uint32_t r = row + i * kRows, c = place ^ twist<T, ALONG>(r);  // along: the same in all of them
-      off[i] = (ALONG ? r : c * kVec<T>) < there ? r * (uint32_t)pitch + c * 16 : kNowhere;
+      const uint32_t r = row + i * kRows, c = place ^ twist<T, ALONG, R>(r);  // along: the same in all of them
+      const uint32_t at = LIES == ROWS ? r * (uint32_t)pitch + c * 16 : r * 64 + (c & 3) * 16 + (ALONG ? 0 : (c >> 2) * (uint32_t)pitch);
+      off[i] = (ALONG ? r : c * kVec<T>) < there ? at : kNowhere;
     }
   }
   __device__ __forceinline__ void nothing() { left = -(1 << 30); }
@@ -136,15 +162,15 @@ struct Reader {
     const uint32_t half = lane >> 5, i32 = lane & 31, j = lane & 15;
     if constexpr (ALONG) {
 #pragma unroll
-      for (uint32_t s = 0; s < 2; s++) at[s] = (first * 32 + i32) * 64 + (((2 * s + half) ^ twist<T, true>(i32)) * 16);
+      for (uint32_t s = 0; s < 2; s++) at[s] = (first * 32 + i32) * 64 + (((2 * s + half) ^ twist<T, true, R>(i32)) * 16);
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++) {
         if constexpr (sizeof(T) == 2) {
-          const uint32_t row = 8 * half + (j >> 2), c = (4 * (first + i) + (i32 >> 4) * 2 + ((j & 3) >> 1)) ^ twist<T, false>(row);
+          const uint32_t row = 8 * half + (j >> 2), c = (4 * (first + i) + (i32 >> 4) * 2 + ((j & 3) >> 1)) ^ twist<T, false, R>(row);
           at[i] = row * kPitch + c * 16 + 8 * (j & 1);
         } else {
-          const uint32_t c = (8 * (first + i) + (i32 >> 2)) ^ twist<T, false>(4 * half);
+          const uint32_t c = (8 * (first + i) + (i32 >> 2)) ^ twist<T, false, R>(4 * half);
           at[i] = 4 * half * kPitch + c * 16 + (i32 & 3) * 4;
         }
       }
@@ -171,21 +197,23 @@ struct Reader {
 };
 
 // A block's tiles one after another. `work` says how many there are and of how many stages each
-// (tiles, stages), gives the feeds of the n-th (feed(n, a, b)) and takes its sums (take(n, sums)). The loads
-// run two stages ahead, over a tile's end into the next.
-template <class T, bool A_ALONG, bool B_ALONG, class Work>
+// (tiles, stages), gives the feeds of the n-th (feed(n, a, b)) and takes its sums (take(n, sums), with kStores
+// stores at least to memory). The loads run two stages ahead, over a tile's end into the next. Loads and stores end in
+// their order, so that behind a tile's stores the next two stages wait for loads alone: with a wait for the stores
+// too, 8,192 x 16,384 logits of width 1,024 took 372 us where they take XXX.
+template <class T, class S, bool A_ALONG, Lies A_LIES, bool B_ALONG, Lies B_LIES, class Work>
 __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
-  Feed<T, A_ALONG, kTileM> fa;
-  Feed<T, B_ALONG, kTileN> fb;
-  Reader<T, A_ALONG, kTileM, 4> ra;
-  Reader<T, B_ALONG, kTileN, 2> rb;
+  Feed<T, A_ALONG, A_LIES, S::kM> fa;
+  Feed<T, B_ALONG, B_LIES, S::kN> fb;
+  Reader<T, A_ALONG, S::kM, S::M> ra;
+  Reader<T, B_ALONG, S::kN, S::N> rb;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  ra.start(lane, 4 * (wave >> 1));
-  rb.start(lane, 2 * (wave & 1));
+  ra.start(lane, S::M * (wave >> 1));
+  rb.start(lane, S::N * (wave & 1));
   const uint32_t tiles = work.tiles, stages = work.stages;
   if (!stages) {  // sums over nothing
     for (uint32_t n = 0; n < tiles; n++) {
-      f32x16 sums[4][2] = {};
+      f32x16 sums[S::M][S::N] = {};
       work.take(n, sums);
     }
     return;
@@ -194,10 +222,10 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   uint32_t ahead_tile = 0, ahead = 0, put = 0;
   work.feed(0, fa, fb);
   auto issue = [&]() {
-    uint32_t at[4], bt[2];
+    uint32_t at[S::M], bt[S::N];
     const u32x4 a = fa.next(at), b = fb.next(bt);
     to_lds(lds0 + put + wave * 1024, a, at, b, bt);
-    put = put == (kStages - 1) * kStageBytes ? 0 : put + kStageBytes;
+    put = put == (kStages - 1) * S::kStageBytes ? 0 : put + S::kStageBytes;
     if (++ahead == stages) {
       ahead = 0;
       if (++ahead_tile < tiles) work.feed(ahead_tile, fa, fb);
@@ -206,29 +234,35 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   };
   issue();
   issue();
-  uint32_t from = 0;
+  uint32_t from = 0, stored = 0;
   for (uint32_t n = 0; n < tiles; n++) {
-    f32x16 sums[4][2] = {};
+    f32x16 sums[S::M][S::N] = {};
     for (uint32_t k = 0; k < stages; k++) {
-      // This stage's loads are all but the last six; everyone has read the stage that is written next.
-      asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      // This stage's loads are all but the last stage's; everyone has read the stage that is written next.
+      if (Work::kStores && stored) {
+        stored--;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads + Work::kStores) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads) : "memory");
+      }
       issue();
       const char *stage = lds + from;
-      from = from == (kStages - 1) * kStageBytes ? 0 : from + kStageBytes;
+      from = from == (kStages - 1) * S::kStageBytes ? 0 : from + S::kStageBytes;
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        Part<T> a[4], b[2];
+        Part<T> a[S::M], b[S::N];
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = ra.get(stage, s, i);
+        for (int i = 0; i < S::M; i++) a[i] = ra.get(stage, s, i);
 #pragma unroll
-        for (int i = 0; i < 2; i++) b[i] = rb.get(stage + kTileM * 64, s, i);
+        for (int i = 0; i < S::N; i++) b[i] = rb.get(stage + S::kM * 64, s, i);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < S::M; i++)
 #pragma unroll
-          for (int j = 0; j < 2; j++) sums[i][j] = mma32(a[i], b[j], sums[i][j]);
+          for (int j = 0; j < S::N; j++) sums[i][j] = mma32(a[i], b[j], sums[i][j]);
       }
     }
     work.take(n, sums);
+    stored = 2;
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the loads that run ahead of the last tile
 }

@@ -45,7 +45,7 @@ DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 MAX_DIM = MAX_STATE = 128
 MAX_TAPS = 4
 MAX_WIDTH = 8192
-MAX_VOCAB = MAX_ROWS = 1 << 24
+MAX_VOCAB, MAX_ROWS = 1 << 23, 1 << 24
 
 P, I64, U32, F32 = C.c_void_p, C.c_int64, C.c_uint32, C.c_float
 
