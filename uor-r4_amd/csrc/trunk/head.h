@@ -9,8 +9,10 @@ struct Matrix {
   const char *at;
   int64_t pitch;  // bytes from row to row, or from panel to panel
 };
-// What is known of a row's softmax in base 2: its largest logit, the sum of 2^(logit - largest), and the
-// target's logit, or the largest one's value and place.
+// What is known of a row's softmax: its largest logit, the sum of e^(logit - largest), and the target's logit,
+// or the largest one's value and place. The largest one is in base 2 (times log2 e, rounded) where exponents are formed in
+// one instruction, fma(z, log2 e, -most); otherwise, in 32 bits and for few rows, the logits are subtracted first, so that
+// the largest one's share is 1 exactly and the loss of a sure row is right to its own size.
 struct Sum {
   float most, sum, value;
   uint32_t place;
@@ -56,8 +58,11 @@ inline bool as_it_lies(const void *p, int64_t stride, uint32_t rows, uint32_t wi
 // by many row tiles. XXX
 constexpr uint32_t kLayRows = 1024;
 inline bool laid_out(const uor_trunk_head_args *s) { return s->rows >= kLayRows || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype); }
-// Whether small tiles fill the card better: the large ones would leave some of its compute units idle. XXX
-inline bool small_tiles(uint64_t rows, uint64_t words) { return up(rows, Large::kN) / Large::kN * (up(words, Large::kM) / Large::kM) < 256; }
+// Whether small tiles are taken: in 32 bits, where there are registers for two sets of sums of them, and where the large
+// ones would leave some compute units idle. XXX
+inline bool small_tiles(const uor_trunk_head_args *s) {
+  return s->dtype == UOR_TRUNK_F32 || up(s->rows, Large::kN) / Large::kN * (up(s->vocab, Large::kM) / Large::kM) < 256;
+}
 inline int check_head(const uor_trunk_head_args *s) {
   if (!s) return fail(-1, "null argument");
   if (s->dtype > UOR_TRUNK_F32) return fail(-1, "dtype %u is neither bf16 nor f32", s->dtype);

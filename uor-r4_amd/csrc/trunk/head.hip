@@ -20,12 +20,16 @@ struct Scan {
   Sum *parts;                   // [2 splits][rows of row_tiles]
 };
 
-// A logit's running softmax in base 2.
+// Logits' running softmax; BASE2: `most` is in base 2, see Sum.
+template <bool BASE2>
 struct Running {
   float most = -3e38f, sum = 0.0f;
+  static __device__ __forceinline__ float power(float v) { return exp2_(BASE2 ? v : v * kLog2e); }
+  static __device__ __forceinline__ float term(float z, float most) { return BASE2 ? exp2_(fmaf(z, kLog2e, -most)) : power(z - most); }
+  static __device__ __forceinline__ float scaled(float z) { return BASE2 ? z * kLog2e : z; }
   __device__ __forceinline__ void join(float most2, float sum2) {
     const float m = fmaxf(most, most2);
-    sum = sum * exp2_(most - m) + sum2 * exp2_(most2 - m);
+    sum = sum * power(most - m) + sum2 * power(most2 - m);
     most = m;
   }
 };
@@ -33,11 +37,12 @@ struct Running {
 template <class T, class S, bool PICK, Lies W>
 struct ScanTiles {
   static constexpr Lies kX = PICK ? W : PANELS;
+  using Run = Running<sizeof(T) == 2>;
   static constexpr int kStores = 0;
   const Scan &a;
   uint32_t tiles, stages, row0, word0;
   int lane, wave;
-  Running run[S::N];
+  Run run[S::N];
   float value[S::N];
   uint32_t place[S::N];
   int32_t target[S::N];
@@ -78,13 +83,13 @@ struct ScanTiles {
             for (int r = 0; r < 16; r++) value[j] = own == 32 * i + row_of(r, 0) ? z[i][j][r] : value[j];
         }
       }
-      const float base = fmaxf(run[j].most, most * kLog2e);
+      const float base = fmaxf(run[j].most, Run::scaled(most));
       float sum[S::M] = {};
 #pragma unroll
       for (int i = 0; i < S::M; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) sum[i] += exp2_(fmaf(z[i][j][r], kLog2e, -base));
-      run[j].sum = fmaf(run[j].sum, exp2_(run[j].most - base), S::M > 2 ? (sum[0] + sum[1]) + (sum[2] + sum[S::M - 1]) : sum[0] + sum[1]);
+        for (int r = 0; r < 16; r++) sum[i] += Run::term(z[i][j][r], base);
+      run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), S::M > 2 ? (sum[0] + sum[1]) + (sum[2] + sum[S::M - 1]) : sum[0] + sum[1]);
       run[j].most = base;
     }
   }
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
   run_tiles<T, S, true, W, true, tiles.kX>(lds, tiles);
 #pragma unroll
   for (int j = 0; j < S::N; j++) {
-    Running run = tiles.run[j];
+    auto run = tiles.run[j];
     run.join(__shfl_xor(run.most, 32), __shfl_xor(run.sum, 32));
     float value = tiles.value[j];
     uint32_t place = tiles.place[j];
@@ -131,14 +136,135 @@ __global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
   }
 }
 
+// Few rows: bound by the matrix, which is read once, past LDS. A block takes 16 words at a time, its four wavefronts a
+// quarter of their values each (every fourth 64 bytes), so that a narrow vocabulary's long rows are not one
+// wavefront's chain; the rows of x lie in LDS. The quarters meet in LDS, and a thread then has the logit of one
+// word for one row of each tile of 16 rows.
+struct Few {
+  const void *w, *x;
+  int64_t w_stride, x_stride;   // values
+  uint32_t rows, vocab, width, pitch;  // pitch: bytes of a row of x in LDS
+  const void *targets;
+  bool wide;
+  Sum *parts;                   // [blocks][rows]
+};
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+constexpr uint32_t kFewPad = 17;  // floats between words of a quarter's sums
+
+template <class T, bool PICK, int TILES>
+__global__ __launch_bounds__(256) void head_few(Few a) {
+  extern __shared__ char x[];
+  __shared__ float quarters[2][4][TILES][16 * kFewPad];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t pieces = (a.width + kDeep<T> - 1) / kDeep<T> * 4;
+  for (uint32_t i = threadIdx.x; i < a.rows * pieces; i += 256)
+    *(Part<T> *)(x + i / pieces * a.pitch + i % pieces * 16) =
+        load_some<T, kVec<T>>((const T *)a.x + (int64_t)(i / pieces) * a.x_stride, true, i % pieces * kVec<T>, a.width);
+  __syncthreads();
+  const uint32_t i16 = lane & 15, chunk = lane >> 4, full = a.width / kDeep<T>;  // stretches of 64 bytes that a row has whole
+  const char *xs[TILES];
+#pragma unroll
+  for (int j = 0; j < TILES; j++) xs[j] = x + (16 * j + i16 < a.rows ? 16 * j + i16 : 0) * a.pitch + chunk * 16;
+  using Run = Running<false>;
+  Run run[TILES];
+  float value[TILES];
+  uint32_t place[TILES];
+  int64_t target[TILES];
+#pragma unroll
+  for (int j = 0; j < TILES; j++) {
+    const uint32_t row = 16 * j + threadIdx.x % 16;
+    value[j] = PICK ? -__builtin_inff() : 0.0f, place[j] = ~0u;
+    target[j] = !PICK && row < a.rows ? target_of(a.targets, a.wide, row, a.vocab) : -1;
+  }
+  uint32_t buffer = 0;
+  for (uint32_t g = blockIdx.x; g * 16 < a.vocab; g += gridDim.x, buffer ^= 1) {
+    const uint32_t mine = g * 16 + i16 < a.vocab ? g * 16 + i16 : a.vocab - 1;
+    const T *row = (const T *)a.w + (int64_t)mine * a.w_stride;
+    f32x4 sums[TILES] = {};
+    auto add = [&](Part<T> w, uint32_t s) {
+#pragma unroll
+      for (int j = 0; j < TILES; j++) sums[j] = mma16(w, *(const Part<T> *)(xs[j] + s * 64), sums[j]);
+    };
+    // Eight stretches on their way while the eight before are multiplied.
+    constexpr uint32_t kAhead = 8;
+    Part<T> now[kAhead], next[kAhead];
+    auto look = [&](Part<T> (&to)[kAhead], uint32_t s) {
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; k++) {
+        const uint32_t at = s + 4 * k < full ? s + 4 * k : wave < full ? wave : 0;  // one too many is read again
+        to[k] = loose<T, kVec<T>>(row + (full ? at * kDeep<T> + chunk * kVec<T> : 0));
+      }
+    };
+    if (full) {
+      look(now, wave);
+      for (uint32_t s = wave; s < full; s += 4 * kAhead) {
+        if (s + 4 * kAhead < full) look(next, s + 4 * kAhead);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++)
+          if (s + 4 * k < full) add(now[k], s + 4 * k);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) now[k] = next[k];
+      }
+    }
+    if (full * kDeep<T> < a.width && wave == (full & 3))
+      add(load_some<T, kVec<T>>(row, true, full * kDeep<T> + chunk * kVec<T>, a.width), full);
+#pragma unroll
+    for (int j = 0; j < TILES; j++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) quarters[buffer][wave][j][(4 * chunk + r) * kFewPad + i16] = sums[j][r];
+    __syncthreads();
+    const uint32_t at = threadIdx.x / 16 * kFewPad + threadIdx.x % 16, word = g * 16 + threadIdx.x / 16;
+#pragma unroll
+    for (int j = 0; j < TILES; j++) {
+      float z = (quarters[buffer][0][j][at] + quarters[buffer][1][j][at]) + (quarters[buffer][2][j][at] + quarters[buffer][3][j][at]);
+      if (word >= a.vocab) z = -__builtin_inff();
+      if constexpr (PICK) {
+        if (z > value[j]) value[j] = z, place[j] = word;
+      } else {
+        if ((int64_t)word == target[j]) value[j] = z;
+      }
+      const float base = fmaxf(run[j].most, z);
+      run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), Run::term(z, base));
+      run[j].most = base;
+    }
+  }
+  __shared__ Sum joined[4][16];
+#pragma unroll
+  for (int j = 0; j < TILES; j++) {
+#pragma unroll
+    for (int k = 16; k < 64; k <<= 1) {
+      run[j].join(__shfl_xor(run[j].most, k), __shfl_xor(run[j].sum, k));
+      join_value<PICK>(value[j], place[j], __shfl_xor(value[j], k), __shfl_xor(place[j], k));
+    }
+    __syncthreads();
+    if (lane < 16) joined[wave][lane] = Sum{run[j].most, run[j].sum, value[j], place[j]};
+    __syncthreads();
+    if (threadIdx.x < 16 && 16 * j + threadIdx.x < a.rows) {
+      for (int w = 1; w < 4; w++) {
+        const Sum p = joined[w][threadIdx.x];
+        run[j].join(p.most, p.sum);
+        join_value<PICK>(value[j], place[j], p.value, p.place);
+      }
+      a.parts[(uint64_t)blockIdx.x * a.rows + 16 * j + threadIdx.x] = Sum{run[j].most, run[j].sum, value[j], place[j]};
+    }
+  }
+}
+
 // WAVES wavefronts join a row's parts, which are `across` apart.
-template <bool PICK, int WAVES>
+template <bool PICK, int WAVES, bool BASE2>
 __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, uint32_t across, uint32_t rows, const uint32_t *count,
-                                                 const int32_t *order, float *losses, float *lse, int64_t *tokens, float *logprobs) {
+                                                 const int32_t *order, const void *targets, bool wide, uint32_t vocab, float *losses, float *lse,
+                                                 int64_t *tokens, float *logprobs) {
   __shared__ Sum joined[4];
   const uint32_t row = blockIdx.x * (4 / WAVES) + threadIdx.x / (64 * WAVES), lane = threadIdx.x % (64 * WAVES);
   if (row >= (count ? *count : rows)) return;  // with WAVES of 4: all of the block
-  Running run;
+  Running<BASE2> run;
   float value = PICK ? -__builtin_inff() : 0.0f;
   uint32_t place = PICK ? ~0u : 0;
 #pragma unroll 4
@@ -161,18 +287,21 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, u
     }
   }
   if (lane) return;
-  const double sum = ((double)run.most + (double)log2f(run.sum)) * kLn2;
+  const double most = BASE2 ? (double)run.most * kLn2 : (double)run.most, rest = log((double)run.sum);
   if constexpr (PICK) {
     tokens[row] = place == ~0u ? 0 : place;
-    logprobs[row] = (float)((double)value - sum);
+    logprobs[row] = (float)((double)value - most - rest);
   } else {
+    // Packed rows have a target; others may have none.
     const uint32_t at = order ? (uint32_t)order[row] : row;
-    lse[at] = (float)sum;
-    losses[at] = (float)(sum - (double)value);
+    const bool there = order || target_of(targets, wide, row, vocab) >= 0;
+    lse[at] = there ? (float)(most + rest) : 0.0f;
+    losses[at] = there ? (float)(most - (double)value + rest) : 0.0f;
   }
 }
 
 namespace {
+
 
 // Parts of the vocabulary that blocks take by themselves. The card takes 512 blocks of large tiles at once (1,024 of
 // small ones). Four times as many even out; but a block of few tiles spends its time on its first loads, so a part
@@ -183,20 +312,38 @@ uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
   return n < 1 ? 1 : n < word_tiles ? n : word_tiles;
 }
 
+// Bytes of a row of x in LDS: 16 more than its stretches, so that 16 rows' pieces lie in different banks.
+uint32_t few_pitch(const uor_trunk_head_args *s) { return (uint32_t)up(s->width * size_of(s->dtype), 64) + 16; }
+// Whether a call's rows are few. In 32 bits they are up to 64 that fit into LDS: tiles of 64 rows spend their matrix
+// instructions on rows that are none (1 row over 131,072 words of 512: 57 us, in tiles 135). In bf16 tiles read the matrix
+// as fast (16 rows over 131,072 words of 512: 35 us, 39 here), unless they leave compute units idle (over 4,550 of
+// 1,536: 18 and 15) or have to lay it out first (over 5,000 of 100: 20 and 14).
+bool few_rows(const uor_trunk_head_args *s) {
+  if (s->rows > 64 || s->rows * few_pitch(s) > 122880) return false;
+  return s->dtype == UOR_TRUNK_F32 || s->vocab <= 16384 || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
+}
+
 // Where a call's scratch memory has what.
 struct Plan {
   bool lay, small;  // the matrix is laid out anew; small tiles
+  uint32_t few;  // blocks of the few rows' kernel, or 0
   uint32_t width, row_tiles, word_tiles, splits;
   uint64_t parts, w, x, order, target, counts, count, bytes;
 };
 Plan plan_of(const uor_trunk_head_args *s, bool pick) {
   Plan p{};
   const uint32_t size = size_of(s->dtype);
+  if (few_rows(s)) {
+    const uint32_t groups = (s->vocab + 15) / 16;
+    p.few = groups < 1024 ? groups : 1024;
+    p.bytes = up((uint64_t)p.few * s->rows * sizeof(Sum), 256);
+    return p;
+  }
   p.width = (uint32_t)up(s->width, 16 / size);
   p.lay = pick ? !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype) ||
                      !as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)
                : laid_out(s);
-  p.small = small_tiles(s->rows, s->vocab);
+  p.small = small_tiles(s);
   const uint32_t n = p.small ? Small::kN : Large::kN, m = p.small ? Small::kM : Large::kM;
   p.row_tiles = (s->rows + n - 1) / n;
   p.word_tiles = (s->vocab + m - 1) / m;
@@ -217,6 +364,20 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
 template <class T, bool PICK>
 int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const Plan p = plan_of(s, PICK);
+  const auto join = [&](auto kernel, uint32_t each, const Sum *parts, uint32_t n, uint32_t across, const uint32_t *count) {
+    hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, parts, n, across, s->rows, count,
+                       PICK || p.few ? nullptr : (const int32_t *)(work + p.order), s->targets, s->wide != 0, s->vocab, s->losses, s->lse, s->tokens,
+                       s->logprobs);
+  };
+  if (p.few) {
+    const Few f{s->weight, s->x, s->w_stride, s->x_stride, s->rows, s->vocab, s->width, few_pitch(s), s->targets, s->wide != 0, (Sum *)work};
+    const uint32_t lds = s->rows * f.pitch;
+    if (s->rows <= 16) hipLaunchKernelGGL((head_few<T, PICK, 1>), dim3(p.few), dim3(256), lds, stream, f);
+    else if (s->rows <= 32) hipLaunchKernelGGL((head_few<T, PICK, 2>), dim3(p.few), dim3(256), lds, stream, f);
+    else hipLaunchKernelGGL((head_few<T, PICK, 4>), dim3(p.few), dim3(256), lds, stream, f);
+    join(head_join<PICK, 4, false>, 1, f.parts, p.few, s->rows, nullptr);
+    return launched();
+  }
   Scan a{};
   a.rows = s->rows, a.vocab = s->vocab, a.width = p.width;
   a.row_tiles = p.row_tiles, a.word_tiles = p.word_tiles, a.splits = p.splits;
@@ -238,16 +399,12 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   }
   const dim3 grid(p.row_tiles * p.splits);
   const uint32_t across = p.row_tiles * (p.small ? Small::kN : Large::kN);
-  if (p.small && p.lay) hipLaunchKernelGGL((head_scan<T, Small, PICK, PANELS>), grid, dim3(256), 0, stream, a);
-  else if (p.small) hipLaunchKernelGGL((head_scan<T, Small, PICK, ROWS>), grid, dim3(256), 0, stream, a);
-  else if (p.lay) hipLaunchKernelGGL((head_scan<T, Large, PICK, PANELS>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((head_scan<T, Large, PICK, ROWS>), grid, dim3(256), 0, stream, a);
-  const auto join = [&](auto kernel, uint32_t each) {
-    hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, a.parts, 2 * p.splits, across, s->rows, a.count,
-                       PICK ? nullptr : (const int32_t *)(work + p.order), s->losses, s->lse, s->tokens, s->logprobs);
-  };
-  if (p.splits > 64) join(head_join<PICK, 4>, 1);
-  else join(head_join<PICK, 1>, 4);
+  const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
+  if (p.small) p.lay ? run(head_scan<T, Small, PICK, PANELS>) : run(head_scan<T, Small, PICK, ROWS>);
+  else if constexpr (sizeof(T) == 2) p.lay ? run(head_scan<T, Large, PICK, PANELS>) : run(head_scan<T, Large, PICK, ROWS>);
+  constexpr bool kBase2 = sizeof(T) == 2;
+  if (p.splits > 64) join(head_join<PICK, 4, kBase2>, 1, a.parts, 2 * p.splits, across, a.count);
+  else join(head_join<PICK, 1, kBase2>, 4, a.parts, 2 * p.splits, across, a.count);
   return launched();
 }
 

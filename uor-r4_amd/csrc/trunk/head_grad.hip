@@ -126,7 +126,19 @@ struct Product {
   uint32_t n_pitch;
   uint32_t m0;             // the piece's first row of parts
   bool first;              // nothing has been summed before
+  // dW that is whole with this launch is rounded and written, with the targets' terms.
+  void *to;                // [words][n_to], the piece's first, or NULL
+  uint32_t words, n_to;
+  bool f32;                // its type
+  const uint8_t *present;  // which words have terms
+  const float *terms;      // [words][n_pitch], or NULL
 };
+
+// v of the lane next to an even one, or before an odd one.
+__device__ __forceinline__ float neighbour(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, false));
+}
+
 
 // DW: the summed axis are the rows of x, else the words. B: how x or the matrix lies.
 template <class T, class S, bool DW, Lies B>
@@ -146,8 +158,48 @@ struct ProductTiles {
     if constexpr (B == PANELS) fb.start(p.b.at + n0 / kDeep<T> * p.b.pitch + (uint64_t)k0 * 64, p.b.pitch, p.n - n0, depth);
     else fb.start(p.b.at + (int64_t)k0 * p.b.pitch + n0 * sizeof(T), p.b.pitch, p.n - n0, depth);
   }
+  // bf16 results go out two columns a lane: two rows of a pair of lanes change places.
+  __device__ __forceinline__ void put(f32x16 (&sums)[S::M][S::N]) {
+    const int half = lane >> 5;
+    const uint32_t word0 = m0 + 32 * S::M * (wave >> 1), col0 = n0 + 32 * S::N * (wave & 1) + (lane & 31);
+    const bool pairs = !p.f32 && p.n_to % 2 == 0 && ((uintptr_t)p.to & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < S::M; i++) {
+      const uint32_t word = word0 + 32 * i + (lane & 31);
+      const uint32_t has = p.terms ? (uint32_t)__ballot(word < p.words && p.present[word]) : 0;
+#pragma unroll
+      for (int j = 0; j < S::N; j++) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) put(word0 + 32 * i, row_of(r, half), col0 + 32 * j, has, pairs, sums[i][j][r], sums[i][j][r + 1]);
+        asm volatile("" ::: "memory");  // else all the words' terms are read, and kept, before any is used
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint32_t first, uint32_t row, uint32_t col, uint32_t has, bool pairs, float a, float b) {
+    const uint32_t word = first + row;
+    if (has) {
+      if (has >> row & 1 && col < p.n_to) a += p.terms[(uint64_t)word * p.n_pitch + col];
+      if (has >> (row + 1) & 1 && col < p.n_to) b += p.terms[(uint64_t)(word + 1) * p.n_pitch + col];
+    }
+    if (pairs) {
+      const float other = neighbour(lane & 1 ? a : b);
+      const bf16x2 v = {(bf16)(lane & 1 ? other : a), (bf16)(lane & 1 ? b : other)};
+      const uint32_t to = word + (lane & 1), at = col & ~1u;
+      if (to < p.words && at < p.n_to) *(bf16x2 *)((bf16 *)p.to + (uint64_t)to * p.n_to + at) = v;
+    } else if (col < p.n_to) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (word + e >= p.words) continue;
+        const uint64_t at = (uint64_t)(word + e) * p.n_to + col;
+        if (p.f32) ((float *)p.to)[at] = e ? b : a;
+        else ((bf16 *)p.to)[at] = (bf16)(e ? b : a);
+      }
+    }
+  }
   __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[S::M][S::N]) {
     const int half = lane >> 5;
+    if constexpr (DW)
+      if (p.to) return put(sums);
     float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 32 * S::M * (wave >> 1)) * p.n_pitch + n0 + 32 * S::N * (wave & 1) + (lane & 31);
 #pragma unroll
     for (int j = 0; j < S::N; j++) {
@@ -190,7 +242,8 @@ struct Ends {
   uint64_t m_rows;
   const uint32_t *count;   // dx's: how many packed rows there are, or NULL
   const int32_t *order, *target;
-  const float *terms;      // or NULL
+  const float *terms;      // dx's, or NULL
+  const uint8_t *present;  // dW's words with terms, which are the last of the splits; or NULL
   const void *w;           // the matrix as the caller has it
   int64_t w_stride;
   void *to;
@@ -203,8 +256,9 @@ __global__ __launch_bounds__(256) void head_sums(Ends a) {
     const uint64_t row = i / pieces;
     const uint32_t col = (uint32_t)(i % pieces) * 8;
     f32x8 v = load_some<float, 8>(a.parts + row * a.n_pitch, true, col, a.n);
+    const uint32_t splits = a.splits + (a.present && a.present[row]);
 #pragma unroll 8
-    for (uint32_t s = 1; s < a.splits; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
+    for (uint32_t s = 1; s < splits; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
     const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.row0 + row] : row;
     if (a.terms)
       v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)a.w + a.target[a.row0 + row] * a.w_stride, true, col, a.n)), f32x8) *
@@ -234,7 +288,7 @@ struct GradPlan {
   uint32_t n_tiles, x_splits, w_splits, n_pitch;
   uint32_t x_rows, w_rows;               // how many rows' and words' sums are kept at once
   SortPlan sort;                         // of the targets, where x is bf16
-  uint64_t g, dx, dw, w, x, order, target, factors, terms, sorted, counts, count, bytes;
+  uint64_t g, dx, dw, w, x, order, target, factors, terms, sorted, present, counts, count, bytes;
 };
 uint32_t splits_for(uint32_t at_once, uint32_t tiles, uint32_t stages) {
   const uint32_t want = at_once / tiles, most = stages / 8;
@@ -250,7 +304,7 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   const uint32_t size = size_of(s->dtype), deep = 64 / size;
   p.width = (uint32_t)up(s->width, 16 / size);
   p.lay = laid_out(s);
-  p.small = small_tiles(s->rows, s->vocab);
+  p.small = small_tiles(s);
   const uint32_t tile_m = p.small ? Small::kM : Large::kM, tile_n = p.small ? Small::kN : Large::kN, at_once = p.small ? 1024 : 512;
   p.all_rows = (uint32_t)up(s->rows, kRound), p.all_words = (uint32_t)up(s->vocab, kRound);
   // A piece of about as many rows as words, whose sums are read and written the least for the G between.
@@ -281,6 +335,7 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
     p.sort = sort_plan(s->rows, s->vocab, s->width);
     p.sorted = at.take(s->dweight ? p.sort.bytes : 0);
     p.terms = at.take(4ull * s->rows);
+    p.present = at.take(s->dweight ? s->vocab : 0);
   }
   p.counts = at.take((s->rows + kPackRows - 1) / kPackRows * 4);
   p.count = at.take(4);
@@ -307,13 +362,13 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   k.x = s->x, k.targets = s->targets, k.wide = s->wide != 0;
   k.to = work + p.x, k.order = (int32_t *)(work + p.order), k.target = (int32_t *)(work + p.target), k.count = count;
   k.lse_in = s->lse, k.dlosses = s->dlosses, k.dlse = s->dlse, k.factors = (float4 *)(work + p.factors);
-  k.dx = s->dx;
+  k.dx = s->dx, k.present = sizeof(T) == 2 && s->dweight ? (uint8_t *)(work + p.present) : nullptr;
   pack<T, true>(k, (uint32_t *)(work + p.counts), stream);
   constexpr bool kTerms = sizeof(T) == 2;
   float *terms = kTerms ? (float *)(work + p.terms) : nullptr;
   Sums t{};
   if (kTerms && s->dweight) {
-    t.width = s->width, t.scale = 1.0f, t.stride = s->x_stride, t.pitch = p.n_pitch, t.from = s->x, t.weights = terms;
+    t.width = s->width, t.scale = 1.0f, t.stride = s->x_stride, t.pitch = p.n_pitch, t.from = s->x, t.weights = terms, t.present = k.present;
     sort_rows(p.sort, s->targets, s->wide != 0, s->rows, s->vocab, work + p.sorted, stream, t);
   }
   // Of the two axes' pieces, one's are outside: see grad_plan.
@@ -331,22 +386,18 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     const uint32_t want = (2 * at_once + l.row_tiles - 1) / l.row_tiles;
     l.splits = want < word_tiles ? want : word_tiles;
     l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.g_rows = p.rows;
-    const dim3 logits(l.row_tiles * l.splits);
-    if (p.small && p.lay) hipLaunchKernelGGL((head_logits<T, Small, PANELS>), logits, dim3(256), 0, stream, l);
-    else if (p.small) hipLaunchKernelGGL((head_logits<T, Small, ROWS>), logits, dim3(256), 0, stream, l);
-    else if (p.lay) hipLaunchKernelGGL((head_logits<T, Large, PANELS>), logits, dim3(256), 0, stream, l);
-    else hipLaunchKernelGGL((head_logits<T, Large, ROWS>), logits, dim3(256), 0, stream, l);
+    const auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.row_tiles * l.splits), dim3(256), 0, stream, l); };
+    if (p.small) p.lay ? logits(head_logits<T, Small, PANELS>) : logits(head_logits<T, Small, ROWS>);
+    else if constexpr (sizeof(T) == 2) p.lay ? logits(head_logits<T, Large, PANELS>) : logits(head_logits<T, Large, ROWS>);
     Product a{};
+    const auto product = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a); };
     a.a = {work + p.g, panel}, a.row0 = row0, a.count = count, a.n = p.width, a.n_tiles = p.n_tiles, a.n_pitch = p.n_pitch;
     if (s->dx) {
       a.b = {w.at + (int64_t)word0 * (p.lay ? 64 : w.pitch), w.pitch};
       a.m = rows, a.k = words, a.m_tiles = (rows + tile_m - 1) / tile_m, a.splits = p.x_splits;
       a.parts = (float *)(work + p.dx), a.m_rows = p.x_rows, a.m0 = rows_outside ? 0 : row0, a.first = word0 == 0;
-      const dim3 grid(a.m_tiles * a.n_tiles * a.splits);
-      if (p.small && p.lay) hipLaunchKernelGGL((head_product<T, Small, false, PANELS>), grid, dim3(256), 0, stream, a);
-      else if (p.small) hipLaunchKernelGGL((head_product<T, Small, false, ROWS>), grid, dim3(256), 0, stream, a);
-      else if (p.lay) hipLaunchKernelGGL((head_product<T, Large, false, PANELS>), grid, dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((head_product<T, Large, false, ROWS>), grid, dim3(256), 0, stream, a);
+      if (p.small) p.lay ? product(head_product<T, Small, false, PANELS>) : product(head_product<T, Small, false, ROWS>);
+      else if constexpr (sizeof(T) == 2) p.lay ? product(head_product<T, Large, false, PANELS>) : product(head_product<T, Large, false, ROWS>);
       if (word_piece + 1 == word_pieces) {
         Ends e{};
         e.n = s->width, e.n_pitch = p.n_pitch;
@@ -359,21 +410,26 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       a.b = x;
       a.m = (uint32_t)up(words, kRound), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
       a.parts = (float *)(work + p.dw), a.m_rows = p.w_rows, a.m0 = rows_outside ? word0 : 0, a.first = row0 == 0;
-      const dim3 grid(a.m_tiles * a.n_tiles * a.splits);
-      if (p.small) hipLaunchKernelGGL((head_product<T, Small, true, PANELS>), grid, dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((head_product<T, Large, true, PANELS>), grid, dim3(256), 0, stream, a);
-      if (row_piece + 1 == row_pieces) {
+      const bool last = row_piece + 1 == row_pieces, direct = last && a.first && p.w_splits == 1;
+      const bool f32 = s->dweight_dtype == UOR_TRUNK_F32;
+      void *to = (char *)s->dweight + (uint64_t)word0 * s->width * size_of(s->dweight_dtype);
+      if (kTerms && last) {
+        t.word0 = word0, t.words = words, t.to = a.parts + ((uint64_t)p.w_splits * p.w_rows + a.m0) * p.n_pitch, t.present = k.present + word0;
+        sum_rows<float, T>(t, stream);
+      }
+      if (direct) {
+        a.to = to, a.words = words, a.n_to = s->width, a.f32 = f32;
+        if (kTerms) a.present = t.present, a.terms = (const float *)t.to;
+      }
+      if (p.small) product(head_product<T, Small, true, PANELS>);
+      else if constexpr (sizeof(T) == 2) product(head_product<T, Large, true, PANELS>);
+      if (last && !direct) {
         Ends e{};
         e.n = s->width, e.n_pitch = p.n_pitch;
-        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.w_splits, e.rows = words, e.m_rows = p.w_rows;
-        if constexpr (kTerms) {
-          t.word0 = word0, t.words = words, t.to = a.parts + ((uint64_t)p.w_splits * p.w_rows + a.m0) * p.n_pitch;
-          sum_rows<float, T>(t, stream);
-          e.splits++;
-        }
-        const uint64_t at = (uint64_t)word0 * s->width;
-        if (s->dweight_dtype == UOR_TRUNK_BF16) e.to = (bf16 *)s->dweight + at, sums<bf16>(e, stream);
-        else e.to = (float *)s->dweight + at, sums<float>(e, stream);
+        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.w_splits, e.rows = words, e.m_rows = p.w_rows, e.to = to;
+        if (kTerms) e.present = t.present;
+        if (f32) sums<float>(e, stream);
+        else sums<bf16>(e, stream);
       }
     }
   }

@@ -23,6 +23,7 @@ struct Pack {
   const float *lse_in, *dlosses, *dlse;
   float4 *factors;          // [rows up to 256], see Factors
   void *dx;                 // zeros for the rows without a target, or NULL
+  uint8_t *present;         // [vocab up to 16] zeros, or NULL
 };
 
 __device__ __forceinline__ int32_t target_of(const void *targets, bool wide, uint32_t row, uint32_t vocab) {
@@ -109,7 +110,12 @@ __global__ __launch_bounds__(256) void head_pack(Pack a) {
     const auto v = load_some<T, kVec<T>>((const T *)a.x + (int64_t)from[r] * a.stride, true, c * kVec<T>, a.width);
     *(Part<T> *)(a.to + packed_at(a, panels, before + r, c)) = v;
   }
-  if constexpr (GRAD) {  // the share's rows without a target
+  if constexpr (GRAD) {
+    if (a.present) {
+      const uint64_t blocks = (uint64_t)gridDim.x * gridDim.y, block = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
+      for (uint64_t i = block * 256 + threadIdx.x; i < (a.vocab + 15) / 16; i += blocks * 256) *(u32x4 *)(a.present + i * 16) = u32x4{};
+    }
+    // The share's rows without a target.
     if (a.dx)
       for (uint32_t i = threadIdx.x; i < (kPackRows - n) * pieces; i += 256) {
         const uint32_t r = none[i / pieces], col = (piece0 + i % pieces) * kVec<T>;

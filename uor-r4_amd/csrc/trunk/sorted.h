@@ -31,6 +31,7 @@ struct Sums {
   uint32_t length, groups;      // rows of a piece, pieces
   float *parts;                 // [groups][2][width]: a piece's first word's sum and its last one's
   uint32_t sum_blocks;          // of the first launch, the others write zeros
+  uint8_t *present;             // [words] or NULL: set to 1 for words that occur, and no zeros are written for others
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -221,6 +222,7 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
   auto put = [&](bool ends) {
     const uint32_t word = key - a.word0;
     if (word >= a.words) return;
+    if (a.present && lane == 0 && blockIdx.y == 0) a.present[word] = 1;
     if (whole && ends) {
       store_some<R, 8>((R *)a.to + (int64_t)word * a.pitch, col, a.width, __builtin_convertvector(sum * a.scale, V8<R>));
     } else {
@@ -370,7 +372,7 @@ inline void sum_rows(const Sums &a, hipStream_t stream) {
     Sums b = a;
     b.sum_blocks = (a.groups + kGroups - 1) / kGroups;
     const uint32_t slices = (a.width + lanes() * 8 - 1) / (lanes() * 8);
-    hipLaunchKernelGGL((sorted_sums<R, T, lanes()>), dim3(b.sum_blocks + (a.words + 63) / 64, slices), dim3(256), 0, stream, b);
+    hipLaunchKernelGGL((sorted_sums<R, T, lanes()>), dim3(b.sum_blocks + (a.present ? 0 : (a.words + 63) / 64), slices), dim3(256), 0, stream, b);
     if (a.groups > 1) hipLaunchKernelGGL((sorted_join<R, lanes()>), dim3(a.groups - 1, slices), dim3(256), 0, stream, b);
   });
 }

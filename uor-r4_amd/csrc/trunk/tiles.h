@@ -16,6 +16,9 @@
 // a value at a time (f32). 16-byte pieces of a row are dealt over its places by an exclusive or with
 // the row's number, so that no two of the lanes that read at once meet in a bank.
 //
+// In 32 bits the sums of 128 values at a time are added to a second set of sums, so that the errors of long sums are those
+// of their 128ths.
+//
 // Any order of the summed axis is right that both operands share: an f32 lane's 16 bytes are four
 // values of four matrix instructions of two.
 #pragma once
@@ -235,9 +238,17 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   issue();
   issue();
   uint32_t from = 0, stored = 0;
+  constexpr bool kFold = sizeof(T) == 4;
+  static_assert(!kFold || S::M * S::N <= 4, "no registers for two sets of sums");
   for (uint32_t n = 0; n < tiles; n++) {
-    f32x16 sums[S::M][S::N] = {};
+    f32x16 sums[S::M][S::N] = {}, folded[kFold ? S::M : 1][kFold ? S::N : 1] = {};
     for (uint32_t k = 0; k < stages; k++) {
+      if (kFold && k && k % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < S::M; i++)
+#pragma unroll
+          for (int j = 0; j < S::N; j++) folded[kFold ? i : 0][kFold ? j : 0] += sums[i][j], sums[i][j] = f32x16{};
+      }
       // This stage's loads are all but the last stage's; everyone has read the stage that is written next.
       if (Work::kStores && stored) {
         stored--;
@@ -260,6 +271,12 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
 #pragma unroll
           for (int j = 0; j < S::N; j++) sums[i][j] = mma32(a[i], b[j], sums[i][j]);
       }
+    }
+    if constexpr (kFold) {
+#pragma unroll
+      for (int i = 0; i < S::M; i++)
+#pragma unroll
+        for (int j = 0; j < S::N; j++) sums[i][j] += folded[i][j];
     }
     work.take(n, sums);
     stored = 2;
