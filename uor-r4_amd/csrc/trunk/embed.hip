@@ -29,7 +29,8 @@ __global__ __launch_bounds__(256) void embed_rows(Embed a) {
       const uint64_t row = base + k * kRows;
       token[k] = row < a.rows ? token_of(a.tokens, a.wide, row, a.vocab) : a.vocab;
     }
-    for (uint32_t col = lane * 8; col < a.width; col += LANES * 8) {
+    for (uint32_t eight = lane; eight * 8 < a.width; eight += LANES) {
+      const uint32_t col = eight_of(eight, a.width);
       f32x8 v[kAhead];
 #pragma unroll
       for (uint32_t k = 0; k < kAhead; k++)
@@ -39,7 +40,12 @@ __global__ __launch_bounds__(256) void embed_rows(Embed a) {
         const uint64_t row = base + k * kRows;
         if (row >= a.rows) break;
         v[k] = token[k] < a.vocab ? v[k] * a.scale : f32x8{};
-        store_some<T, 8>((T *)a.y + row * a.width, col, a.width, __builtin_convertvector(v[k], V8<T>));
+        // Past the caches, which hold the table meanwhile: 262,144 rows of 256 33.6 us, through them 36.4; 131,072 of 512 from
+        // 131,072 words 29.8 and 35.5.
+        const auto out = __builtin_convertvector(v[k], V8<T>);
+        T *to = (T *)a.y + row * a.width;
+        if (col + 8 <= a.width) __builtin_nontemporal_store(out, (typename Loose<T, 8>::At *)(to + col));
+        else store_some<T, 8>(to, col, a.width, out);
       }
     }
   }

@@ -7,7 +7,7 @@
 // A block takes 128 rows through some of the vocabulary, 256 words a tile. The words are the result's rows, so
 // that a lane has 64 logits of one row of x in registers: their largest, and the sum of 2^(z log2 e - most), are
 // kept from tile to tile as a lane's own. Pieces of the vocabulary are joined by a second launch, in their order.
-#include "head_pack.h"
+#include "few.h"
 
 namespace trunk {
 
@@ -89,7 +89,9 @@ struct ScanTiles {
       for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) sum[i] += Run::term(z[i][j][r], base);
-      run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), S::M > 2 ? (sum[0] + sum[1]) + (sum[2] + sum[S::M - 1]) : sum[0] + sum[1]);
+      float total = sum[0] + sum[1];
+      if constexpr (S::M == 4) total += sum[2] + sum[3];
+      run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), total);
       run[j].most = base;
     }
   }
@@ -136,41 +138,8 @@ __global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
   }
 }
 
-// Few rows: bound by the matrix, which is read once, past LDS. A block takes 16 words at a time, its four wavefronts a
-// quarter of their values each (every fourth 64 bytes), so that a narrow vocabulary's long rows are not one
-// wavefront's chain; the rows of x lie in LDS. The quarters meet in LDS, and a thread then has the logit of one
-// word for one row of each tile of 16 rows.
-struct Few {
-  const void *w, *x;
-  int64_t w_stride, x_stride;   // values
-  uint32_t rows, vocab, width, pitch;  // pitch: bytes of a row of x in LDS
-  const void *targets;
-  bool wide;
-  Sum *parts;                   // [blocks][rows]
-};
-__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma16(f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-  return c;
-}
-
-constexpr uint32_t kFewPad = 17;  // floats between words of a quarter's sums
-
 template <class T, bool PICK, int TILES>
 __global__ __launch_bounds__(256) void head_few(Few a) {
-  extern __shared__ char x[];
-  __shared__ float quarters[2][4][TILES][16 * kFewPad];
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t pieces = (a.width + kDeep<T> - 1) / kDeep<T> * 4;
-  for (uint32_t i = threadIdx.x; i < a.rows * pieces; i += 256)
-    *(Part<T> *)(x + i / pieces * a.pitch + i % pieces * 16) =
-        load_some<T, kVec<T>>((const T *)a.x + (int64_t)(i / pieces) * a.x_stride, true, i % pieces * kVec<T>, a.width);
-  __syncthreads();
-  const uint32_t i16 = lane & 15, chunk = lane >> 4, full = a.width / kDeep<T>;  // stretches of 64 bytes that a row has whole
-  const char *xs[TILES];
-#pragma unroll
-  for (int j = 0; j < TILES; j++) xs[j] = x + (16 * j + i16 < a.rows ? 16 * j + i16 : 0) * a.pitch + chunk * 16;
   using Run = Running<false>;
   Run run[TILES];
   float value[TILES];
@@ -182,59 +151,19 @@ __global__ __launch_bounds__(256) void head_few(Few a) {
     value[j] = PICK ? -__builtin_inff() : 0.0f, place[j] = ~0u;
     target[j] = !PICK && row < a.rows ? target_of(a.targets, a.wide, row, a.vocab) : -1;
   }
-  uint32_t buffer = 0;
-  for (uint32_t g = blockIdx.x; g * 16 < a.vocab; g += gridDim.x, buffer ^= 1) {
-    const uint32_t mine = g * 16 + i16 < a.vocab ? g * 16 + i16 : a.vocab - 1;
-    const T *row = (const T *)a.w + (int64_t)mine * a.w_stride;
-    f32x4 sums[TILES] = {};
-    auto add = [&](Part<T> w, uint32_t s) {
-#pragma unroll
-      for (int j = 0; j < TILES; j++) sums[j] = mma16(w, *(const Part<T> *)(xs[j] + s * 64), sums[j]);
-    };
-    // Eight stretches on their way while the eight before are multiplied.
-    constexpr uint32_t kAhead = 8;
-    Part<T> now[kAhead], next[kAhead];
-    auto look = [&](Part<T> (&to)[kAhead], uint32_t s) {
-#pragma unroll
-      for (uint32_t k = 0; k < kAhead; k++) {
-        const uint32_t at = s + 4 * k < full ? s + 4 * k : wave < full ? wave : 0;  // one too many is read again
-        to[k] = loose<T, kVec<T>>(row + (full ? at * kDeep<T> + chunk * kVec<T> : 0));
-      }
-    };
-    if (full) {
-      look(now, wave);
-      for (uint32_t s = wave; s < full; s += 4 * kAhead) {
-        if (s + 4 * kAhead < full) look(next, s + 4 * kAhead);
-#pragma unroll
-        for (uint32_t k = 0; k < kAhead; k++)
-          if (s + 4 * k < full) add(now[k], s + 4 * k);
-#pragma unroll
-        for (uint32_t k = 0; k < kAhead; k++) now[k] = next[k];
-      }
+  few_logits<T, TILES>(a, a.rows, nullptr, [&](int j, uint32_t word, float z) {
+    if (word >= a.vocab) z = -__builtin_inff();
+    if constexpr (PICK) {
+      if (z > value[j]) value[j] = z, place[j] = word;
+    } else {
+      if ((int64_t)word == target[j]) value[j] = z;
     }
-    if (full * kDeep<T> < a.width && wave == (full & 3))
-      add(load_some<T, kVec<T>>(row, true, full * kDeep<T> + chunk * kVec<T>, a.width), full);
-#pragma unroll
-    for (int j = 0; j < TILES; j++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) quarters[buffer][wave][j][(4 * chunk + r) * kFewPad + i16] = sums[j][r];
-    __syncthreads();
-    const uint32_t at = threadIdx.x / 16 * kFewPad + threadIdx.x % 16, word = g * 16 + threadIdx.x / 16;
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-      float z = (quarters[buffer][0][j][at] + quarters[buffer][1][j][at]) + (quarters[buffer][2][j][at] + quarters[buffer][3][j][at]);
-      if (word >= a.vocab) z = -__builtin_inff();
-      if constexpr (PICK) {
-        if (z > value[j]) value[j] = z, place[j] = word;
-      } else {
-        if ((int64_t)word == target[j]) value[j] = z;
-      }
-      const float base = fmaxf(run[j].most, z);
-      run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), Run::term(z, base));
-      run[j].most = base;
-    }
-  }
+    const float base = fmaxf(run[j].most, z);
+    run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), Run::term(z, base));
+    run[j].most = base;
+  });
   __shared__ Sum joined[4][16];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < TILES; j++) {
 #pragma unroll
@@ -312,17 +241,6 @@ uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
   return n < 1 ? 1 : n < word_tiles ? n : word_tiles;
 }
 
-// Bytes of a row of x in LDS: 16 more than its stretches, so that 16 rows' pieces lie in different banks.
-uint32_t few_pitch(const uor_trunk_head_args *s) { return (uint32_t)up(s->width * size_of(s->dtype), 64) + 16; }
-// Whether a call's rows are few. In 32 bits they are up to 64 that fit into LDS: tiles of 64 rows spend their matrix
-// instructions on rows that are none (1 row over 131,072 words of 512: 57 us, in tiles 135). In bf16 tiles read the matrix
-// as fast (16 rows over 131,072 words of 512: 35 us, 39 here), unless they leave compute units idle (over 4,550 of
-// 1,536: 18 and 15) or have to lay it out first (over 5,000 of 100: 20 and 14).
-bool few_rows(const uor_trunk_head_args *s) {
-  if (s->rows > 64 || s->rows * few_pitch(s) > 122880) return false;
-  return s->dtype == UOR_TRUNK_F32 || s->vocab <= 16384 || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype);
-}
-
 // Where a call's scratch memory has what.
 struct Plan {
   bool lay, small;  // the matrix is laid out anew; small tiles
@@ -370,7 +288,7 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
                        s->logprobs);
   };
   if (p.few) {
-    const Few f{s->weight, s->x, s->w_stride, s->x_stride, s->rows, s->vocab, s->width, few_pitch(s), s->targets, s->wide != 0, (Sum *)work};
+    const Few f{s->weight, s->x, s->w_stride, s->x_stride, s->rows, s->vocab, s->width, few_pitch(s), 0, s->vocab, s->targets, s->wide != 0, (Sum *)work};
     const uint32_t lds = s->rows * f.pitch;
     if (s->rows <= 16) hipLaunchKernelGGL((head_few<T, PICK, 1>), dim3(p.few), dim3(256), lds, stream, f);
     else if (s->rows <= 32) hipLaunchKernelGGL((head_few<T, PICK, 2>), dim3(p.few), dim3(256), lds, stream, f);

@@ -9,7 +9,7 @@
 // G is rounded to bf16 where x is, half a step (2^-8) of each value, independent of the others. Of the largest,
 // the target's, that would be an error of the whole row: it is left out of G, and its terms G_t,target W_target
 // and G_t,target x_t are added to dx and dW in 32 bits at their ends, dW's by sorted targets.
-#include "head_pack.h"
+#include "few.h"
 #include "sorted.h"
 
 namespace trunk {
@@ -36,6 +36,13 @@ struct LogitTiles {
   float base[S::N], all[S::N], one[S::N];
   int32_t target[S::N], place[S::N];
 
+  // A logit's share of its row; in 32 bits with what the rounding of its exponent leaves.
+  static __device__ __forceinline__ float share(float z, float base) {
+    if constexpr (sizeof(T) == 2) return exp2_(fmaf(z, kLog2e, -base));
+    const float v = z - base < -120.0f ? -120.0f : z - base, t = v * kLog2e;
+    const float left = fmaf(v, 1.92596299e-8f, fmaf(v, kLog2e, -t)), e = exp2_(t);
+    return fmaf(e, left * 0.693147181f, e);
+  }
   template <class FA, class FB>
   __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
     const uint32_t word = word0 + n * S::kM;
@@ -51,7 +58,7 @@ struct LogitTiles {
 #pragma unroll
       for (int i = 0; i < S::M; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) z[i][j][r] = all[j] * exp2_(fmaf(z[i][j][r], kLog2e, -base[j]));
+        for (int r = 0; r < 16; r++) z[i][j][r] = all[j] * share(z[i][j][r], base[j]);
       const uint32_t at = (uint32_t)target[j] - word;
       if (__any(at < 32 * S::M)) {
         float term = 0.0f;
@@ -112,6 +119,34 @@ __global__ __launch_bounds__(256, S::kBlocks) void head_logits(Logits a) {
     tiles.base[j] = f.x, tiles.all[j] = f.y, tiles.one[j] = f.z, tiles.target[j] = a.target[row], tiles.place[j] = a.order[row];
   }
   run_tiles<T, S, true, W, true, PANELS>(lds, tiles);
+}
+
+// The same for few rows of 32 bits. A block's 16 words are a panel of G.
+struct FewLogits {
+  Few f;
+  const uint32_t *count;
+  const int32_t *order, *target;
+  const float4 *factors;
+  char *g;          // [words / 16][g_rows][64 bytes]
+  uint32_t g_rows;
+};
+template <int TILES>
+__global__ __launch_bounds__(256) void head_few_logits(FewLogits a) {
+  using Tiles = LogitTiles<float, Small, ROWS>;
+  const uint32_t rows = *a.count;
+  float4 factor[TILES];
+  int32_t target[TILES];
+#pragma unroll
+  for (int j = 0; j < TILES; j++) {
+    const uint32_t row = 16 * j + threadIdx.x % 16;
+    factor[j] = a.factors[row], target[j] = a.target[row];
+  }
+  few_logits<float, TILES>(a.f, rows, a.order, [&](int j, uint32_t word, float z) {
+    const uint32_t row = 16 * j + threadIdx.x % 16, at = word - a.f.word0;
+    if (row >= rows) return;
+    const float g = word < a.f.vocab ? factor[j].y * Tiles::share(z, factor[j].x) - ((int32_t)word == target[j] ? factor[j].z : 0.0f) : 0.0f;
+    *(float *)(a.g + ((uint64_t)(at / 16) * a.g_rows + row) * 64 + at % 16 * 4) = g;
+  });
 }
 
 // A product of a piece: out[m][n] (+)= sum_k a[m][k] b[k][n] over a share of its k.
@@ -270,7 +305,7 @@ __global__ __launch_bounds__(256) void head_sums(Ends a) {
   const uint32_t limit = there < a.rows ? there : a.rows, share = threadIdx.x / kEach;
   for (uint64_t base = (uint64_t)blockIdx.x * kEach; base < (uint64_t)limit * pieces; base += (uint64_t)gridDim.x * kEach) {
     const uint64_t i = base + threadIdx.x % kEach, row = i / pieces;
-    const uint32_t col = (uint32_t)(i % pieces) * 8;
+    const uint32_t col = eight_of((uint32_t)(i % pieces), a.n);
     const bool mine = row < limit;
     const uint32_t splits = a.splits + (mine && a.present && a.present[row]);
     f32x8 v = {};
@@ -303,7 +338,7 @@ __global__ __launch_bounds__(256) void head_sums(Ends a) {
 constexpr uint32_t kFewTerms = 256;
 template <class T>
 __global__ __launch_bounds__(64) void head_terms(Sums a, const void *targets, bool wide, uint32_t vocab) {
-  const uint32_t row = blockIdx.x, col = (blockIdx.y * 64 + threadIdx.x) * 8;
+  const uint32_t row = blockIdx.x, eight = blockIdx.y * 64 + threadIdx.x, col = eight_of(eight, a.width);
   const int32_t mine = target_of(targets, wide, row, vocab);
   if (mine < 0 || (uint32_t)mine - a.word0 >= a.words) return;
   uint64_t same[kFewTerms / 64];
@@ -318,13 +353,13 @@ __global__ __launch_bounds__(64) void head_terms(Sums a, const void *targets, bo
   f32x8 sum = {};
 #pragma unroll
   for (uint32_t k = 0; k < kFewTerms / 64; k++)
-    for (uint64_t left = same[k]; left; left &= left - 1) {
+    for (uint64_t left = eight * 8 < a.width ? same[k] : 0; left; left &= left - 1) {
       const uint32_t other = 64 * k + __builtin_ctzll(left);
       sum += __builtin_convertvector((load_some<T, 8>((const T *)a.from + (int64_t)other * a.stride, true, col, a.width)), f32x8) * a.weights[other];
     }
   const uint32_t word = (uint32_t)mine - a.word0;
   if (threadIdx.x == 0 && blockIdx.y == 0) a.present[word] = 1;
-  store_some<float, 8>((float *)a.to + (int64_t)word * a.pitch, col, a.width, sum);
+  if (eight * 8 < a.width) store_some<float, 8>((float *)a.to + (int64_t)word * a.pitch, col, a.width, sum);
 }
 
 // The gradient of no rows.
@@ -452,7 +487,15 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     l.splits = want < word_tiles ? want : word_tiles;
     l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.g_rows = p.rows;
     const auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.row_tiles * l.splits), dim3(256), 0, stream, l); };
-    if (p.small) p.lay ? logits(head_logits<T, Small, PANELS>) : logits(head_logits<T, Small, ROWS>);
+    bool few = false;
+    if constexpr (sizeof(T) == 4) few = few_rows(s);
+    if (few) {
+      const Few f{s->weight, s->x, s->w_stride, s->x_stride, s->rows, s->vocab, s->width, few_pitch(s), word0, words, nullptr, false, nullptr};
+      const FewLogits v{f, count, k.order, k.target, k.factors, work + p.g, p.rows};
+      const uint32_t groups = (words + 15) / 16;
+      const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups < 1024 ? groups : 1024), dim3(256), s->rows * f.pitch, stream, v); };
+      if constexpr (sizeof(T) == 4) s->rows <= 16 ? run(head_few_logits<1>) : s->rows <= 32 ? run(head_few_logits<2>) : run(head_few_logits<4>);
+    } else if (p.small) p.lay ? logits(head_logits<T, Small, PANELS>) : logits(head_logits<T, Small, ROWS>);
     else if constexpr (sizeof(T) == 2) p.lay ? logits(head_logits<T, Large, PANELS>) : logits(head_logits<T, Large, ROWS>);
     Product a{};
     const auto product = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a); };

@@ -50,9 +50,11 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *scratch) {
   return v;
 }
 
-// A gradient's factors of a packed row: G = e2 2^(z log2 e - base) for e2 = (dloss + dlse) 2^(what the
-// rounding of base = lse log2 e left), less dloss at the target.
+// A gradient's factors of a packed row. In bf16 G = e2 2^(z log2 e - base) for e2 = (dloss + dlse) 2^(what the
+// rounding of base = lse log2 e left); in 32 bits G = e2 e^(z - base) for base = lse. Less dloss at the target.
+template <class T>
 __device__ __forceinline__ float4 factors_of(float lse, float dloss, float dlse) {
+  if constexpr (sizeof(T) == 4) return {lse, dloss + dlse, dloss, 0.0f};
   const double base = (double)lse * 1.4426950408889634;
   const float hi = (float)base, all = dloss + dlse;
   const float left = hi - hi == 0.0f ? (float)(hi - base) : 0.0f;
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(256) void head_pack(Pack a) {
         a.order[before + place] = (int32_t)row;
         a.target[before + place] = t;
         if constexpr (GRAD)
-          a.factors[before + place] = factors_of(a.lse_in[row], a.dlosses ? a.dlosses[row] : 0.0f, a.dlse ? a.dlse[row] : 0.0f);
+          a.factors[before + place] = factors_of<T>(a.lse_in[row], a.dlosses ? a.dlosses[row] : 0.0f, a.dlse ? a.dlse[row] : 0.0f);
       }
     } else {
       none[threadIdx.x - place] = row;

@@ -186,6 +186,10 @@ static __global__ __launch_bounds__(kSortThreads) void sort_place(Digit a) {
 // ---------------------------------------------------------------------------------------------
 // The sums.
 
+// The first of a lane's eight columns. The last lane of a row takes its last eight, some of them also the
+// lane's before it, which writes the same: rows of any width are read and written eight values at a time.
+__device__ __forceinline__ uint32_t eight_of(uint32_t i, uint32_t width) { return width < 8 ? 8 * i : min(8 * i, width - 8); }
+
 // The first of the sorted rows whose word is not before `key`, looked for by a whole wavefront.
 __device__ __forceinline__ uint32_t first_of(const uint32_t *keys, uint32_t rows, uint32_t key) {
   if (!rows || keys[0] >= key) return 0;
@@ -209,13 +213,13 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
     const uint64_t none = __ballot(word < a.words && (lo == a.rows || a.keys[lo] != key));
     for (uint32_t k = threadIdx.x / LANES; k < 64; k += 256 / LANES)
       if (none >> k & 1)
-        for (uint32_t col = (blockIdx.y * LANES + lane) * 8; col < a.width; col += gridDim.y * LANES * 8)
-          store_some<R, 8>((R *)a.to + (int64_t)(word0 + k) * a.pitch, col, a.width, V8<R>{});
+        if ((blockIdx.y * LANES + lane) * 8 < a.width)
+          store_some<R, 8>((R *)a.to + (int64_t)(word0 + k) * a.pitch, eight_of(blockIdx.y * LANES + lane, a.width), a.width, V8<R>{});
     return;
   }
-  const uint32_t group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, col = (blockIdx.y * LANES + lane) * 8;
+  const uint32_t group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, eight = blockIdx.y * LANES + lane, col = eight_of(eight, a.width);
   const uint64_t first = (uint64_t)group * a.length;
-  if (group >= a.groups || col >= a.width) return;
+  if (group >= a.groups || eight * 8 >= a.width) return;
   const uint64_t end = first + a.length < a.rows ? first + a.length : a.rows;
   uint32_t key = a.keys[first];
   if (key >= a.word0 + a.words || a.keys[end - 1] < a.word0) return;
@@ -273,7 +277,8 @@ template <class R, int LANES>
 __global__ __launch_bounds__(256) void sorted_join(Sums a) {
   constexpr uint32_t kGroups = 256 / LANES;
   __shared__ float joined[kGroups][LANES * 8 + 1];
-  const uint32_t group = blockIdx.x, lane = threadIdx.x % LANES, part = threadIdx.x / LANES, col = (blockIdx.y * LANES + lane) * 8;
+  const uint32_t group = blockIdx.x, lane = threadIdx.x % LANES, part = threadIdx.x / LANES, eight = blockIdx.y * LANES + lane;
+  const uint32_t col = eight_of(eight, a.width);
   const uint64_t first = (uint64_t)group * a.length, end = first + a.length;
   if (end >= a.rows) return;
   const uint32_t key = a.keys[end - 1];
@@ -284,13 +289,14 @@ __global__ __launch_bounds__(256) void sorted_join(Sums a) {
   // This piece's second part, then the first ones of pieces group + 1 .. lo.
   const uint32_t n = lo - group + 1, each = (n + kGroups - 1) / kGroups, from = part * each, to = from + each < n ? from + each : n;
   f32x8 sum = {};
+  if (eight * 8 < a.width)
 #pragma unroll 8
-  for (uint32_t i = from; i < to; i++)
-    sum += load_some<float, 8>(a.parts + ((uint64_t)(group + i) * 2 + (i ? 0 : 1)) * a.width, true, col, a.width);
+    for (uint32_t i = from; i < to; i++)
+      sum += load_some<float, 8>(a.parts + ((uint64_t)(group + i) * 2 + (i ? 0 : 1)) * a.width, true, col, a.width);
 #pragma unroll
   for (int e = 0; e < 8; e++) joined[part][lane * 8 + e] = sum[e];
   __syncthreads();
-  if (part || col >= a.width) return;
+  if (part || eight * 8 >= a.width) return;
   for (uint32_t p = 1; p < kGroups; p++)
 #pragma unroll
     for (int e = 0; e < 8; e++) sum[e] += joined[p][lane * 8 + e];

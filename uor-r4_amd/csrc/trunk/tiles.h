@@ -8,7 +8,8 @@
 //
 // Matrices that the kernels lay out themselves lie by panels: 64 bytes of each row, row after row, and then the rows'
 // next 64 bytes. A stage's part of 256 rows is then 16 KB in one piece along the summed axis, and 2 KB pieces across.
-// XXX
+// Rows that lie 2 KB apart are read by half lines of the caches, every line twice: 8,192 x 131,072 logits of width
+// 1,024 took 333 M requests to the L2 caches as rows and 201 M as panels (2.15 and 2.05 ms).
 //
 // An operand lies along the summed axis (its values for one row or column of the result next to each
 // other) or across it (a row apart). Along, a stage's rows are 64 bytes, and a lane reads the 16 bytes
@@ -17,7 +18,8 @@
 // the row's number, so that no two of the lanes that read at once meet in a bank.
 //
 // In 32 bits the sums of 128 values at a time are added to a second set of sums, so that the errors of long sums are those
-// of their 128ths.
+// of their 128ths. Operands of 32 bits as three planes of bf16 and six products of them ran 1.4 times as fast for 4,096
+// rows of 512, half as fast for up to 100, and up to 6 times further from 64 bits; they are not used.
 //
 // Any order of the summed axis is right that both operands share: an f32 lane's 16 bytes are four
 // values of four matrix instructions of two.
@@ -38,7 +40,6 @@ struct Shape {
   static constexpr int kBlocks = M * N > 4 ? 2 : 4;  // that share a compute unit
 };
 using Large = Shape<4, 2>;
-// XXX small
 using Small = Shape<2, 1>;
 constexpr int kRound = 256;  // rows and words are rounded up to whole large tiles
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset that no buffer has: the load gives zeros
@@ -203,7 +204,7 @@ struct Reader {
 // (tiles, stages), gives the feeds of the n-th (feed(n, a, b)) and takes its sums (take(n, sums), with kStores
 // stores at least to memory). The loads run two stages ahead, over a tile's end into the next. Loads and stores end in
 // their order, so that behind a tile's stores the next two stages wait for loads alone: with a wait for the stores
-// too, 8,192 x 16,384 logits of width 1,024 took 372 us where they take XXX.
+// too, 8,192 x 16,384 logits of width 1,024 and their G took 372 us, without 348.
 template <class T, class S, bool A_ALONG, Lies A_LIES, bool B_ALONG, Lies B_LIES, class Work>
 __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   Feed<T, A_ALONG, A_LIES, S::kM> fa;
