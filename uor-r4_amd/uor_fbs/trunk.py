@@ -640,9 +640,9 @@ def loss(x, weight, targets):
     return losses, lse
 
 
-def loss_backward(dlosses, x, weight, targets, lse, *, dlse=None, dtype=None):
+def loss_backward(dlosses, x, weight, targets, lse, *, dlse=None, dtype=None, dx=True, dweight=True):
     """(dx, dweight): the gradients of ``loss`` at x and weight from those of its outputs (either may be None
-    for zeros) and the call's own ``lse``. The logits are computed again, a piece of the vocabulary and of the rows
+    for zeros) and the call's own ``lse``; with ``dx`` or ``dweight`` false that one is None and not computed. The logits are computed again, a piece of the vocabulary and of the rows
     at a time; their gradient is rounded to x's type before its products with x and weight, which are summed in
     32 bits. ``dtype``: dweight's type, weight's own without (float32 for a program that adds up
     gradients of bfloat16 calls)."""
@@ -653,7 +653,7 @@ def loss_backward(dlosses, x, weight, targets, lse, *, dlse=None, dtype=None):
     dtype = weight.dtype if dtype is None else dtype
     _want(dtype in DTYPES, "dtype is {}, not bfloat16 or float32", dtype)
     index = _one_device(lse, dlosses, dlse, *keep)
-    got = LossGrads(_make(x), torch.empty(weight.shape, dtype=dtype, device=weight.device))
+    got = LossGrads(_make(x) if dx else None, torch.empty(weight.shape, dtype=dtype, device=weight.device) if dweight else None)
     a.lse, a.dlosses, a.dlse, a.dweight_dtype = _ptr(lse), _ptr(dlosses), _ptr(dlse), DTYPES[dtype]
     a.dx, a.dweight = map(_ptr, got)
     _call("loss_backward", a, index)
@@ -674,7 +674,8 @@ class _Loss(torch.autograd.Function):
         if dlosses is None and dlse is None:
             return None, None, None
         x, weight, targets, lse = ctx.saved_tensors
-        got = loss_backward(dlosses, x, weight, targets, lse, dlse=dlse)
+        dx, dweight, _ = ctx.needs_input_grad
+        got = loss_backward(dlosses, x, weight, targets, lse, dlse=dlse, dx=dx, dweight=dweight)
         return got.dx, got.dweight, None
 
 
