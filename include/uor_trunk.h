@@ -14,7 +14,8 @@
  *   conv    the short causal convolution of each channel over its last `taps` rows;
  *   norms   the norms before and after a block fused with its gate and residual scale:
  *             v = out silu(gate),  r' = residual + scale v rsqrt(mean v^2 + eps) post,
- *             n = r' rsqrt(mean r'^2 + eps) pre.
+ *             n = r' rsqrt(mean r'^2 + eps) pre;
+ *   embed, loss, choose  the trunk's ends over its vocabulary, see below.
  *
  * Rows are packed: sequence s owns rows offsets[s] .. offsets[s + 1] - 1 (int32 on the device,
  * ascending; values outside 0 .. tokens are taken as the nearest inside). Of offsets that do not ascend

@@ -1,17 +1,20 @@
 """The float trunk's operators on the GPU (include/uor_trunk.h): the selective state space scan and
 its short causal convolution (packed sequences, their gradients, single tokens over device slots),
-and the norms before and after a block fused with its gate and residual scale (and their gradients).
+the norms before and after a block fused with its gate and residual scale (and their gradients), and the
+trunk's ends over its vocabulary: the embedding's lookup and gradient, the head's cross entropy with its
+gradients and its greedy choice, without keeping the logits.
 
 Every function takes and returns torch tensors on one HIP device, runs on torch's current stream and
 waits for nothing. Activations are bfloat16 or float32; parameters, the scan's states and the
-parameters' gradients are float32. Rows are packed: ``offsets`` (int32, one more than there are
+parameters' gradients are float32. The embedding's table and the head's matrix are of either type, and
+their gradients of theirs. Rows are packed: ``offsets`` (int32, one more than there are
 sequences, ascending, on the device) says where each sequence's rows begin; without it all rows are
 one sequence. Rows before the first offset and from the last one on are no sequence's: what is
 returned is 0 there, and nothing else depends on them. Where the inner axes of a tensor are not dense
 it is copied first. Errors raise ``TrunkError``; there is no fallback: a missing library or device
 raises.
 
-``scan``, ``conv`` and ``norms`` take part in autograd: where an input requires a gradient, the outputs
+``scan``, ``conv``, ``norms``, ``embed`` and ``loss`` take part in autograd: where an input requires a gradient, the outputs
 have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which a
 program may call by itself (it is not differentiable). The steps update their states in place and have
 no gradient: going back through one raises. Nothing is kept between calls. Results are the same each
