@@ -28,6 +28,18 @@ def test_gradients_against_64_bits():
         close(grads[k], v.grad, k)
 
 
+def test_a_target_outside_the_vocabulary_is_none():
+    cfg = config(keep_logits=False)
+    p = ft.make_params(cfg, 3)
+    tokens, offsets = ragged([5, 20], cfg.vocab)
+    targets = tokens.roll(-1)
+    targets[[3, 11]] = -1
+    want = ft.gradients(cfg, p, tokens, targets, offsets)
+    targets[11] = cfg.vocab
+    got = ft.gradients(cfg, p, tokens, targets, offsets)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(got[1][k], v) for k, v in want[1].items())
+
+
 def test_replies_are_those_of_the_logits():
     cfg = config()
     p = ft.make_params(cfg, 4)

@@ -8,7 +8,8 @@ A layer takes the normed residual n of its rows and computes
     residual'   = residual + scale rms((y W_out) silu(n W_gate)) post,  n' = rms(residual') pre
 
 with W_* products of torch. Its rows begin as the embedding's and end at the head over the vocabulary: as logits,
-or (``Config.keep_logits`` false) as a loss, its gradients and a choice of tokens that keep none.
+or (``Config.keep_logits`` false) as a loss, its gradients and a choice of tokens that keep none. A token or target
+outside the vocabulary (not the last words by negative numbers) is none: its row begins as zeros.
 ``python -m uor_fbs.float_trunk`` trains one to repeat its prompts and then lets sessions go on from them
 token by token.
 """
@@ -151,7 +152,7 @@ def gradients(cfg, p, tokens, targets, offsets):
     """(loss, {name: gradient}): the mean cross entropy of the rows' next tokens (target -1: none)."""
     saved = []
     n = _prompt_rows(cfg, p, tokens, offsets, saved=saved)
-    wanted = targets >= 0
+    wanted = (targets >= 0) & (targets < cfg.vocab)
     count = wanted.sum().clamp(min=1)
     if cfg.keep_logits:
         log = torch.log_softmax(_logits(cfg, p, n), 1)
