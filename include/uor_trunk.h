@@ -179,7 +179,8 @@ uint64_t uor_trunk_embed_backward_workspace_bytes(const uor_trunk_embed_args *ar
 int uor_trunk_embed_backward_async(const uor_trunk_embed_args *args, void *workspace, uint64_t bytes, void *stream);
 
 /* dlosses and dlse may be NULL for zeros. With G_tv = (dlosses_t + dlse_t) e^(z_tv - lse_t) - dlosses_t
- * [v is t's target]: dx = G W, dweight = G^T x. `lse` is the call's own. G is rounded to the type of x.
+ * [v is t's target]: dx = G W, dweight = G^T x. `lse` is the call's own. G is rounded to the type of x but for
+ * the targets'.
  * Workspaces are aligned to 256 bytes. */
 typedef struct {
   int32_t device;

@@ -645,9 +645,10 @@ def loss(x, weight, targets):
 
 def loss_backward(dlosses, x, weight, targets, lse, *, dlse=None, dtype=None, dx=True, dweight=True):
     """(dx, dweight): the gradients of ``loss`` at x and weight from those of its outputs (either may be None
-    for zeros) and the call's own ``lse``; with ``dx`` or ``dweight`` false that one is None and not computed. The logits are computed again, a piece of the vocabulary and of the rows
-    at a time; their gradient is rounded to x's type before its products with x and weight, which are summed in
-    32 bits. ``dtype``: dweight's type, weight's own without (float32 for a program that adds up
+    for zeros) and the call's own ``lse``; with ``dx`` or ``dweight`` false that one is None and not computed. The
+    logits are computed again, a piece of the vocabulary and of the rows at a time; their gradient, but for the
+    targets', is rounded to x's type before its products with x and weight, which are summed in 32 bits.
+    ``dtype``: dweight's type, weight's own without (float32 for a program that adds up
     gradients of bfloat16 calls)."""
     _want(targets is not None, "targets is no tensor")
     a, keep = _head_args(x, weight, targets)
@@ -684,8 +685,8 @@ class _Loss(torch.autograd.Function):
 
 def choose(x, weight):
     """(tokens, logprobs): of each row of x (rows, width) the word of ``weight`` (vocab, width; x's type) with the
-    largest logit, the lowest of equals (int64), and its log probability (float32), without keeping the
-    logits. They have no gradient. Of a row with no logit over -inf the token is 0; logits that are no number are not chosen."""
+    largest logit, the lowest of equals (int64), and its log probability (float32), without keeping the logits. They
+    have no gradient. Of a row with no logit over -inf the token is 0; logits that are no number are not chosen."""
     a, keep = _head_args(x, weight, None)
     index = _one_device(*keep)
     tokens = torch.empty(a.rows, dtype=torch.int64, device=x.device)
