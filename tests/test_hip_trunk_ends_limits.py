@@ -33,6 +33,16 @@ def test_shared_memory_and_one_word(dtype, rows, vocab, width):  # noqa: F811
     check_choice(x, weight)
 
 
+@pytest.mark.parametrize("masked", [0.0, 0.45, 0.97])
+@pytest.mark.parametrize("rows,vocab,width", [(3800, 3900, 330), (5000, 2500, 609), (1000, 9000, 100), (2100, 700, 1300)])
+def test_uneven_shares(dtype, rows, vocab, width, masked):  # noqa: F811
+    """Tiles that no whole number of turns of the card takes, and fewer rows with a target than there are."""
+    x, weight, targets, m = loss_case(dtype, rows, vocab, width, masked=masked)
+    lse = check_loss(x, weight, targets)
+    check_gradients(x, weight, targets, lse, m(rows, dtype=torch.float32), None)
+    check_choice(x, weight)
+
+
 def on_gpu(seed, dtype, *shape):  # noqa: F811
     return torch.randn(shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda", dtype=dtype)
 

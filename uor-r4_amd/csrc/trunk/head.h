@@ -29,13 +29,73 @@ __device__ __forceinline__ uint32_t by_xcd(uint32_t block, uint32_t n) {
   return xcd * each + (xcd < more ? xcd : more) + (block >> 3);
 }
 
-// A block's row tile and share of the words. Blocks of an XCD go through eight row tiles by all shares before
-// the next eight, so that what runs at once reads few rows and few words.
-__device__ __forceinline__ void by_eights(uint32_t work, uint32_t row_tiles, uint32_t splits, uint32_t &row_tile, uint32_t &split) {
-  const uint32_t group = work / (8 * splits), left = work - group * 8 * splits, rows = min(8u, row_tiles - group * 8);
-  row_tile = group * 8 + left % rows;
-  split = left / rows;
+// a / b, by 32 bits where they are, as they nearly always are: divisions of 64 are some hundred instructions.
+__device__ __forceinline__ uint64_t ratio(uint64_t a, uint64_t b) { return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b; }
+// Row tiles by word tiles, in even shares for groups of blocks: a group takes up to eight row tiles abreast through its share of
+// the words, so that what runs at once reads few rows and few words. A unit is a word tile of a set of row tiles. Where the card takes
+// all tiles at once, a block takes one, and all row tiles are abreast.
+// `blocks`: how many there may be, eighths of them an XCD; `at_once`: how many the card takes.
+struct RowShares {
+  uint64_t units;
+  uint32_t groups, tiles, sets, abreast;
+  bool single, resident;  // a block has one tile; all blocks run at once
+  __device__ __forceinline__ RowShares(uint32_t rows, uint32_t tile, uint32_t word_tiles, uint32_t blocks, uint32_t at_once) {
+    tiles = (rows + tile - 1) / tile;
+    single = (uint64_t)tiles * word_tiles <= at_once, resident = blocks <= at_once;
+    sets = single ? 1 : (tiles + 7) / 8, abreast = single ? tiles : (tiles + sets - 1) / sets;
+    units = (uint64_t)sets * word_tiles;
+    groups = single ? word_tiles : (uint32_t)min((uint64_t)(8 * (blocks / 8 / abreast)), units);
+  }
+  __device__ __forceinline__ uint64_t first(uint32_t group) const { return ratio(units * group, groups); }
+  __device__ __forceinline__ uint32_t of(uint64_t unit) const { return (uint32_t)ratio((unit + 1) * groups - 1, units); }
+};
+// Blocks for them: as many as the card takes at once (two a compute unit of large tiles, four of small ones), and up to four
+// times as many of 16 tiles or more, as compute units are not equally fast: 32,768 rows of 256 over 32,768 words 600 us, in 512
+// blocks 619; but 1,024 rows in 512 blocks 30, in all of the 1,024 that there is work for 37.
+inline uint32_t scan_blocks(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
+  const uint64_t even = row_tiles * (uint64_t)word_tiles / 16 / 8 * 8;
+  return (uint32_t)(even < at_once ? at_once : even < 4 * at_once ? even : 4 * at_once);
 }
+inline uint32_t scan_grid(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
+  const uint64_t all = row_tiles * (uint64_t)word_tiles;
+  return all < at_once ? (uint32_t)all : scan_blocks(row_tiles, word_tiles, at_once);
+}
+// A block's: `tiles` word tiles of row tiles, from the word tile `word` of the row tile `row` on. With the last word tile of
+// a row tile it goes on with the row tile `abreast` further.
+struct Walk {
+  uint32_t group, tiles, row, word, abreast, word_tiles;
+  __device__ __forceinline__ Walk(const RowShares &s, uint32_t words, uint32_t block) {
+    tiles = 0, abreast = s.abreast, word_tiles = words;
+    if (s.single) {
+      // Eight row tiles by all words, before the next eight.
+      const uint32_t all = s.tiles * words;
+      if (block >= all) return;
+      const uint32_t work = by_xcd(block, all), set = work / (8 * words), left = work - set * 8 * words, rows = min(8u, s.tiles - 8 * set);
+      group = word = left / rows, row = 8 * set + left % rows, tiles = 1;
+      return;
+    }
+    // An XCD (every eighth block) has groups next to each other.
+    const uint32_t xcd = block & 7, j = block >> 3, own = s.groups / 8 + (xcd < s.groups % 8), all = own * abreast;
+    if (j >= all) return;
+    // Of blocks that run at once, every 32nd of an XCD's shares a compute unit (measured). Its blocks take groups next to
+    // each other, whose shares are even together where each is a tile more or less.
+    const uint32_t unit = j & 31, q = unit * (all >> 5) + min(unit, all & 31) + (j >> 5);
+    const uint32_t first = s.resident ? q / own : j % abreast;
+    group = xcd * (s.groups / 8) + min(xcd, s.groups % 8) + (s.resident ? q % own : j / abreast);
+    const uint64_t from = s.first(group);
+    uint64_t to = s.first(group + 1);
+    if ((s.sets - 1) * s.abreast + first >= s.tiles) to = min(to, (uint64_t)(s.sets - 1) * words);  // the last set has fewer
+    if (from >= to) return;
+    const uint32_t set = (uint32_t)ratio(from, words);
+    tiles = (uint32_t)(to - from), row = set * s.abreast + first, word = (uint32_t)(from - (uint64_t)set * words);
+  }
+  // One tile on; whether it is another row tile.
+  __device__ __forceinline__ bool next() {
+    if (++word < word_tiles) return false;
+    word = 0, row += abreast;
+    return true;
+  }
+};
 
 // Scratch memory, a stretch at a time.
 struct Scratch {

@@ -4,9 +4,11 @@
 //   z_tv = x_t . W_v,  lse_t = log sum_v e^z_tv,  loss_t = lse_t - z_t,target
 //   token_t = argmax_v z_tv (the lowest of equals),  logprob_t = z_t,token - lse_t
 //
-// A block takes 128 rows through some of the vocabulary, 256 words a tile. The words are the result's rows, so
+// A block takes 128 rows through some of the vocabulary, 256 words a tile, and then the next rows. The words are the result's rows, so
 // that a lane has 64 logits of one row of x in registers: their largest, and the sum of 2^(z log2 e - most), are
-// kept from tile to tile as a lane's own. Pieces of the vocabulary are joined by a second launch, in their order.
+// kept from tile to tile as a lane's own. Parts of a row are joined by a second launch, in their order.
+// Shares of blocks are even to a tile: 11,917 of 17,024 rows of 1,609 over 2,479 words 130 us, with shares of rows by shares of
+// words, which left the card's last turn two thirds empty, 204.
 #include "few.h"
 
 namespace trunk {
@@ -14,10 +16,11 @@ namespace trunk {
 struct Scan {
   Matrix w, x;
   uint32_t rows, vocab, width;  // width: values of a row, whole 16 bytes
-  uint32_t row_tiles, word_tiles, splits;  // in the shape's tiles
+  uint32_t word_tiles;          // in the shape's tiles
+  uint32_t blocks, at_once;     // see RowShares
   const uint32_t *count;        // how many rows there are, or NULL: `rows`
   const int32_t *target;        // [rows up to 256]
-  Sum *parts;                   // [2 splits][rows of row_tiles]
+  Sum *parts;                   // [group + set][abreast][2][a tile's rows], see RowShares: groups and sets go on together
 };
 
 // Logits' running softmax; BASE2: `most` is in base 2, see Sum.
@@ -34,28 +37,60 @@ struct Running {
   }
 };
 
+// `value` and `place` of two parts of a row: the target's logit, which one of them has at most, or the largest.
+template <bool PICK>
+__device__ __forceinline__ void join_value(float &value, uint32_t &place, float value2, uint32_t place2) {
+  if constexpr (PICK) {
+    const bool other = value2 > value || (value2 == value && place2 < place);
+    value = other ? value2 : value;
+    place = other ? place2 : place;
+  } else {
+    value += value2;
+  }
+}
+
 template <class T, class S, bool PICK, Lies W>
 struct ScanTiles {
   static constexpr Lies kX = PICK ? W : PANELS;
   using Run = Running<sizeof(T) == 2>;
   static constexpr int kStores = 0;
   const Scan &a;
-  uint32_t tiles, stages, row0, word0;
+  uint32_t tiles;
+  Walk ahead, at;
   int lane, wave;
   Run run[S::N];
   float value[S::N];
   uint32_t place[S::N];
   int32_t target[S::N];
 
+  // A row tile's beginning and end.
+  __device__ __forceinline__ void open() {
+#pragma unroll
+    for (int j = 0; j < S::N; j++) {
+      run[j] = Run{}, value[j] = PICK ? -__builtin_inff() : 0.0f, place[j] = 0;
+      target[j] = PICK ? -1 : a.target[at.row * S::kN + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)];
+    }
+  }
+  __device__ __forceinline__ void close() {
+    Sum *to = a.parts + ((uint64_t)(2 * (at.group * at.abreast + at.row) + (wave >> 1))) * S::kN + 32 * S::N * (wave & 1);
+#pragma unroll
+    for (int j = 0; j < S::N; j++) {
+      run[j].join(__shfl_xor(run[j].most, 32), __shfl_xor(run[j].sum, 32));
+      join_value<PICK>(value[j], place[j], __shfl_xor(value[j], 32), __shfl_xor(place[j], 32));
+      if (lane < 32) to[32 * j + lane] = Sum{run[j].most, run[j].sum, value[j], place[j]};
+    }
+  }
+  __device__ __forceinline__ uint32_t stages(uint32_t) const { return (a.width + kDeep<T> - 1) / kDeep<T>; }
   template <class FA, class FB>
-  __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
-    const uint32_t word = word0 + n * S::kM;
+  __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
+    const uint32_t word = ahead.word * S::kM, row0 = ahead.row * S::kN;
+    ahead.next();
     fa.start(a.w.at + (int64_t)word * (W == ROWS ? a.w.pitch : 64), a.w.pitch, a.vocab - word, a.width);
     fb.start(a.x.at + (int64_t)row0 * (kX == ROWS ? a.x.pitch : 64), a.x.pitch, a.rows - row0, a.width);
   }
   __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[S::M][S::N]) {
     const int half = lane >> 5;
-    const uint32_t word = word0 + n * S::kM + 32 * S::M * (wave >> 1);
+    const uint32_t word = at.word * S::kM + 32 * S::M * (wave >> 1);
     if (word + 32 * S::M > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // words that are none
 #pragma unroll
     for (int j = 0; j < S::N; j++) {
@@ -94,48 +129,21 @@ struct ScanTiles {
       run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), total);
       run[j].most = base;
     }
+    if (at.word + 1 == at.word_tiles || n + 1 == tiles) close();
+    if (at.next() && n + 1 < tiles) open();
   }
 };
-
-// `value` and `place` of two parts of a row: the target's logit, which one of them has at most, or the largest.
-template <bool PICK>
-__device__ __forceinline__ void join_value(float &value, uint32_t &place, float value2, uint32_t place2) {
-  if constexpr (PICK) {
-    const bool other = value2 > value || (value2 == value && place2 < place);
-    value = other ? value2 : value;
-    place = other ? place2 : place;
-  } else {
-    value += value2;
-  }
-}
 
 template <class T, class S, bool PICK, Lies W>
 __global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-  uint32_t row_tile, split;
-  by_eights(by_xcd(blockIdx.x, gridDim.x), a.row_tiles, a.splits, row_tile, split);
-  const uint32_t row0 = row_tile * S::kN;
-  if (a.count && row0 >= *a.count) return;
-  const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
+  const uint32_t rows = a.count ? *a.count : a.rows;
+  const Walk walk(RowShares(rows, S::kN, a.word_tiles, a.blocks, a.at_once), a.word_tiles, blockIdx.x);
+  if (!walk.tiles) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  ScanTiles<T, S, PICK, W> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, first * S::kM, lane, wave};
-#pragma unroll
-  for (int j = 0; j < S::N; j++) {
-    tiles.value[j] = PICK ? -__builtin_inff() : 0.0f, tiles.place[j] = 0;
-    tiles.target[j] = PICK ? -1 : a.target[row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)];
-  }
+  ScanTiles<T, S, PICK, W> tiles{a, walk.tiles, walk, walk, lane, wave};
+  tiles.open();
   run_tiles<T, S, true, W, true, tiles.kX>(lds, tiles);
-#pragma unroll
-  for (int j = 0; j < S::N; j++) {
-    auto run = tiles.run[j];
-    run.join(__shfl_xor(run.most, 32), __shfl_xor(run.sum, 32));
-    float value = tiles.value[j];
-    uint32_t place = tiles.place[j];
-    join_value<PICK>(value, place, __shfl_xor(value, 32), __shfl_xor(place, 32));
-    if (lane < 32)
-      a.parts[(uint64_t)(2 * split + (wave >> 1)) * (a.row_tiles * S::kN) + row0 + 32 * S::N * (wave & 1) + 32 * j + lane] =
-          Sum{run.most, run.sum, value, place};
-  }
 }
 
 template <class T, bool PICK, int TILES>
@@ -185,20 +193,31 @@ __global__ __launch_bounds__(256) void head_few(Few a) {
   }
 }
 
-// WAVES wavefronts join a row's parts, which are `across` apart.
+// WAVES wavefronts join a row's parts: of tiles of `tile` rows, see Scan, or (0) of few rows, one a block.
 template <bool PICK, int WAVES, bool BASE2>
-__global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, uint32_t across, uint32_t rows, const uint32_t *count,
-                                                 const int32_t *order, const void *targets, bool wide, uint32_t vocab, float *losses, float *lse,
-                                                 int64_t *tokens, float *logprobs) {
+__global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t tile, uint32_t word_tiles, uint32_t blocks, uint32_t at_once,
+                                                 uint32_t rows,
+                                                 const uint32_t *count, const int32_t *order, const void *targets, bool wide, uint32_t vocab,
+                                                 float *losses, float *lse, int64_t *tokens, float *logprobs) {
   __shared__ Sum joined[4];
   const uint32_t row = blockIdx.x * (4 / WAVES) + threadIdx.x / (64 * WAVES), lane = threadIdx.x % (64 * WAVES);
-  if (row >= (count ? *count : rows)) return;  // with WAVES of 4: all of the block
+  const uint32_t all = count ? *count : rows;
+  if (row >= all) return;  // with WAVES of 4: all of the block
+  uint32_t n = blocks, across = rows, two = 2 * rows;  // parts, and from one to the next and to the one after
+  const Sum *from = parts + row;
+  if (tile) {
+    const RowShares s(all, tile, word_tiles, blocks, at_once);
+    const uint32_t at = row / tile, set = at / s.abreast;
+    const uint32_t first = s.of((uint64_t)set * word_tiles), last = s.of((uint64_t)(set + 1) * word_tiles - 1);
+    n = 2 * (last - first + 1), across = tile, two = 2 * s.abreast * tile;
+    from = parts + (uint64_t)2 * (first * s.abreast + at) * tile + row % tile;
+  }
   Running<BASE2> run;
   float value = PICK ? -__builtin_inff() : 0.0f;
   uint32_t place = PICK ? ~0u : 0;
 #pragma unroll 4
   for (uint32_t i = lane; i < n; i += 64 * WAVES) {
-    const Sum p = parts[(uint64_t)i * across + row];
+    const Sum p = from[(uint64_t)(i >> 1) * two + (i & 1) * across];
     run.join(p.most, p.sum);
     join_value<PICK>(value, place, p.value, p.place);
   }
@@ -231,21 +250,11 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t n, u
 
 namespace {
 
-
-// Parts of the vocabulary that blocks take by themselves. The card takes 512 blocks of large tiles at once (1,024 of
-// small ones). Four times as many even out; but a block of few tiles spends its time on its first loads, so a part
-// has four tiles at least where that leaves no compute unit idle.
-uint32_t splits_of(uint32_t row_tiles, uint32_t word_tiles, uint32_t at_once) {
-  const uint32_t even = (4 * at_once + row_tiles - 1) / row_tiles, fill = (at_once + row_tiles - 1) / row_tiles;
-  const uint32_t most = fill > word_tiles / 4 ? fill : word_tiles / 4, n = even < most ? even : most;
-  return n < 1 ? 1 : n < word_tiles ? n : word_tiles;
-}
-
 // Where a call's scratch memory has what.
 struct Plan {
   bool lay, small;  // the matrix is laid out anew; small tiles
   uint32_t few;  // blocks of the few rows' kernel, or 0
-  uint32_t width, row_tiles, word_tiles, splits;
+  uint32_t width, tile, word_tiles, at_once, blocks, grid;
   uint64_t parts, w, x, order, target, counts, count, bytes;
 };
 Plan plan_of(const uor_trunk_head_args *s, bool pick) {
@@ -262,13 +271,14 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
                      !as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)
                : laid_out(s);
   p.small = small_tiles(s);
-  const uint32_t n = p.small ? Small::kN : Large::kN, m = p.small ? Small::kM : Large::kM;
-  p.row_tiles = (s->rows + n - 1) / n;
+  p.tile = p.small ? Small::kN : Large::kN;
+  const uint32_t m = p.small ? Small::kM : Large::kM, row_tiles = (s->rows + p.tile - 1) / p.tile;
   p.word_tiles = (s->vocab + m - 1) / m;
-  p.splits = splits_of(p.row_tiles, p.word_tiles, p.small ? 1024 : 512);
+  p.at_once = p.small ? 1024 : 512;
+  p.blocks = scan_blocks(row_tiles, p.word_tiles, p.at_once), p.grid = scan_grid(row_tiles, p.word_tiles, p.at_once);
   Scratch at;
   const uint64_t rows = up(s->rows, kRound);
-  p.parts = at.take(2ull * p.splits * p.row_tiles * n * sizeof(Sum));
+  p.parts = at.take(2ull * (p.grid + row_tiles) * p.tile * sizeof(Sum));
   p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
   p.x = at.take(pick && !p.lay ? 0 : rows * up(s->width * size, 64));
   p.order = at.take(pick ? 0 : rows * 4);
@@ -282,8 +292,8 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
 template <class T, bool PICK>
 int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const Plan p = plan_of(s, PICK);
-  const auto join = [&](auto kernel, uint32_t each, const Sum *parts, uint32_t n, uint32_t across, const uint32_t *count) {
-    hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, parts, n, across, s->rows, count,
+  const auto join = [&](auto kernel, uint32_t each, const Sum *parts, uint32_t blocks, const uint32_t *count) {
+    hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, parts, p.tile, p.word_tiles, blocks, p.at_once, s->rows, count,
                        PICK || p.few ? nullptr : (const int32_t *)(work + p.order), s->targets, s->wide != 0, s->vocab, s->losses, s->lse, s->tokens,
                        s->logprobs);
   };
@@ -293,12 +303,12 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     if (s->rows <= 16) hipLaunchKernelGGL((head_few<T, PICK, 1>), dim3(p.few), dim3(256), lds, stream, f);
     else if (s->rows <= 32) hipLaunchKernelGGL((head_few<T, PICK, 2>), dim3(p.few), dim3(256), lds, stream, f);
     else hipLaunchKernelGGL((head_few<T, PICK, 4>), dim3(p.few), dim3(256), lds, stream, f);
-    join(head_join<PICK, 4, false>, 1, f.parts, p.few, s->rows, nullptr);
+    join(head_join<PICK, 4, false>, 1, f.parts, p.few, nullptr);
     return launched();
   }
   Scan a{};
   a.rows = s->rows, a.vocab = s->vocab, a.width = p.width;
-  a.row_tiles = p.row_tiles, a.word_tiles = p.word_tiles, a.splits = p.splits;
+  a.word_tiles = p.word_tiles, a.blocks = p.blocks, a.at_once = p.at_once;
   a.parts = (Sum *)(work + p.parts);
   a.w = {(const char *)s->weight, s->w_stride * (int64_t)sizeof(T)};
   if (p.lay) a.w = lay<T>(s->weight, s->w_stride, s->vocab, s->width, work + p.w, stream);
@@ -315,14 +325,15 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     pack<T, false>(k, (uint32_t *)(work + p.counts), stream);
     a.count = k.count, a.target = k.target;
   }
-  const dim3 grid(p.row_tiles * p.splits);
-  const uint32_t across = p.row_tiles * (p.small ? Small::kN : Large::kN);
+  const dim3 grid(p.grid);
   const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
   if (p.small) p.lay ? run(head_scan<T, Small, PICK, PANELS>) : run(head_scan<T, Small, PICK, ROWS>);
   else if constexpr (sizeof(T) == 2) p.lay ? run(head_scan<T, Large, PICK, PANELS>) : run(head_scan<T, Large, PICK, ROWS>);
   constexpr bool kBase2 = sizeof(T) == 2;
-  if (p.splits > 64) join(head_join<PICK, 4, kBase2>, 1, a.parts, 2 * p.splits, across, a.count);
-  else join(head_join<PICK, 1, kBase2>, 4, a.parts, 2 * p.splits, across, a.count);
+  // More than 128 parts a row: by a block.
+  const uint32_t row_tiles = (s->rows + p.tile - 1) / p.tile;
+  if (min((uint64_t)p.word_tiles, (uint64_t)p.blocks / row_tiles) > 64) join(head_join<PICK, 4, kBase2>, 1, a.parts, p.blocks, a.count);
+  else join(head_join<PICK, 1, kBase2>, 4, a.parts, p.blocks, a.count);
   return launched();
 }
 

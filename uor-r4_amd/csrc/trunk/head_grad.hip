@@ -3,8 +3,10 @@
 //   G_tv = (dloss_t + dlse_t) e^(z_tv - lse_t) - dloss_t [v = target_t],  dx = G W,  dW = G^T x.
 //
 // A piece of the rows by a piece of the vocabulary at a time: one launch computes the piece's logits again
-// and writes its G, in the type of x, to scratch memory; one takes G W and one G^T x from it. dx is summed over the pieces of the vocabulary and dW over those of the rows, in 32 bits. Where a piece has
-// fewer tiles than the card takes at once, its sums are split along their axis and joined at the end.
+// and writes its G, in the type of x, to scratch memory; one takes G W and one G^T x from it. dx is summed over the pieces of the
+// vocabulary and dW over those of the rows, in 32 bits. Where a product's tiles leave compute units idle in the card's last turn, the
+// summed axis is shared out evenly instead, and the shares of a tile are joined by a launch behind. How many rows are packed is known
+// on the card alone, so that what a block does is worked out there, of the rows that there are.
 //
 // G is rounded to bf16 where x is, half a step (2^-8) of each value, independent of the others. Of the largest,
 // the target's, that would be an error of the whole row: it is left out of G, and its terms G_t,target W_target
@@ -17,7 +19,8 @@ namespace trunk {
 struct Logits {
   Matrix w, x;      // x: the piece's panels
   uint32_t rows, vocab, width;
-  uint32_t row0, row_tiles, word0, word_tiles, splits;  // the piece, in the shape's tiles
+  uint32_t row0, piece_rows, word0, word_tiles;  // the piece, in the shape's tiles
+  uint32_t blocks, at_once;  // see RowShares
   const uint32_t *count;
   const int32_t *target;
   const float4 *factors;
@@ -31,10 +34,22 @@ template <class T, class S, Lies W>
 struct LogitTiles {
   static constexpr int kStores = S::M * S::N * (sizeof(T) == 2 ? 2 : 4);
   const Logits &a;
-  uint32_t tiles, stages, row0, word0;  // row0 in the piece, word0 of the vocabulary
+  uint32_t tiles;
+  Walk ahead, at;   // in the piece
   int lane, wave;
   float base[S::N], all[S::N], one[S::N];
   int32_t target[S::N], place[S::N];
+
+  // A row tile's beginning.
+  __device__ __forceinline__ void open() {
+#pragma unroll
+    for (int j = 0; j < S::N; j++) {
+      const uint32_t row = a.row0 + at.row * S::kN + 32 * S::N * (wave & 1) + 32 * j + (lane & 31);
+      const float4 f = a.factors[row];
+      base[j] = f.x, all[j] = f.y, one[j] = f.z, target[j] = a.target[row], place[j] = a.order[row];
+    }
+  }
+  __device__ __forceinline__ uint32_t stages(uint32_t) const { return (a.width + kDeep<T> - 1) / kDeep<T>; }
 
   // A logit's share of its row; in 32 bits with what the rounding of its exponent leaves.
   static __device__ __forceinline__ float share(float z, float base) {
@@ -44,14 +59,15 @@ struct LogitTiles {
     return fmaf(e, left * 0.693147181f, e);
   }
   template <class FA, class FB>
-  __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
-    const uint32_t word = word0 + n * S::kM;
+  __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
+    const uint32_t word = a.word0 + ahead.word * S::kM, row0 = ahead.row * S::kN;
+    ahead.next();
     fa.start(a.w.at + (int64_t)word * (W == ROWS ? a.w.pitch : 64), a.w.pitch, a.vocab - word, a.width);
     fb.start(a.x.at + row0 * 64, a.x.pitch, S::kN, a.width);
   }
   __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[S::M][S::N]) {
     const int half = lane >> 5;
-    const uint32_t word = word0 + n * S::kM + 32 * S::M * (wave >> 1);
+    const uint32_t word = a.word0 + at.word * S::kM + 32 * S::M * (wave >> 1), row0 = at.row * S::kN;
     if (word + 32 * S::M > a.vocab) cut_rows(z, a.vocab > word ? a.vocab - word : 0, half);  // their G is 0
 #pragma unroll
     for (int j = 0; j < S::N; j++) {
@@ -59,10 +75,10 @@ struct LogitTiles {
       for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) z[i][j][r] = all[j] * share(z[i][j][r], base[j]);
-      const uint32_t at = (uint32_t)target[j] - word;
-      if (__any(at < 32 * S::M)) {
+      const uint32_t own_word = (uint32_t)target[j] - word;
+      if (__any(own_word < 32 * S::M)) {
         float term = 0.0f;
-        const int own = (int)at - 4 * half;
+        const int own = (int)own_word - 4 * half;
 #pragma unroll
         for (int i = 0; i < S::M; i++)
 #pragma unroll
@@ -71,7 +87,7 @@ struct LogitTiles {
             if constexpr (sizeof(T) == 2) term = here ? z[i][j][r] : term, z[i][j][r] = here ? 0.0f : z[i][j][r];
             else z[i][j][r] -= here ? one[j] : 0.0f;
           }
-        if (sizeof(T) == 2 && at < 32 * S::M && (int)(at >> 2 & 1) == half) a.terms[place[j]] = term - one[j];
+        if (sizeof(T) == 2 && own_word < 32 * S::M && (int)(own_word >> 2 & 1) == half) a.terms[place[j]] = term - one[j];
       }
       const uint64_t panel = (uint64_t)a.g_rows * 64;
       char *to = a.g + (word - a.word0) / kDeep<T> * panel + (row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)) * 64;
@@ -99,25 +115,19 @@ struct LogitTiles {
         }
       }
     }
+    if (at.next() && n + 1 < tiles) open();
   }
 };
 
 template <class T, class S, Lies W>
 __global__ __launch_bounds__(256, S::kBlocks) void head_logits(Logits a) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-  uint32_t row_tile, split;
-  by_eights(by_xcd(blockIdx.x, gridDim.x), a.row_tiles, a.splits, row_tile, split);
-  const uint32_t row0 = row_tile * S::kN;
-  if (a.row0 + row0 >= *a.count) return;
-  const uint32_t first = (uint32_t)((uint64_t)a.word_tiles * split / a.splits), end = (uint32_t)((uint64_t)a.word_tiles * (split + 1) / a.splits);
+  const uint32_t count = *a.count, rows = count > a.row0 ? min(count - a.row0, a.piece_rows) : 0;
+  const Walk walk(RowShares(rows, S::kN, a.word_tiles, a.blocks, a.at_once), a.word_tiles, blockIdx.x);
+  if (!walk.tiles) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  LogitTiles<T, S, W> tiles{a, end - first, (a.width + kDeep<T> - 1) / kDeep<T>, row0, a.word0 + first * S::kM, lane, wave};
-#pragma unroll
-  for (int j = 0; j < S::N; j++) {
-    const uint32_t row = a.row0 + row0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31);
-    const float4 f = a.factors[row];
-    tiles.base[j] = f.x, tiles.all[j] = f.y, tiles.one[j] = f.z, tiles.target[j] = a.target[row], tiles.place[j] = a.order[row];
-  }
+  LogitTiles<T, S, W> tiles{a, walk.tiles, walk, walk, lane, wave};
+  tiles.open();
   run_tiles<T, S, true, W, true, PANELS>(lds, tiles);
 }
 
@@ -149,19 +159,57 @@ __global__ __launch_bounds__(256) void head_few_logits(FewLogits a) {
   });
 }
 
-// A product of a piece: out[m][n] (+)= sum_k a[m][k] b[k][n] over a share of its k.
-struct Product {
-  Matrix a, b;             // a: panels of G
-  uint32_t m, n, k;        // sums of the piece; k may be fewer, see Limit
-  uint32_t m_tiles, n_tiles, splits;
+// How a product's blocks share it. A group of blocks takes all columns' tiles abreast through its share of the row tiles'
+// stages, so that it reads its rows of G once. A tile that is whole in a group's share ends there; of others every group leaves its
+// sums in a slot, two of which a block has: of a tile that begins in its share, and of one that does not.
+struct Split {
+  uint32_t m, k;           // the piece's rows of the result and its summed axis; of dx or dW fewer, where fewer rows are packed
   uint32_t row0;           // the piece's first packed row
   const uint32_t *count;   // how many packed rows there are
-  float *parts;            // [splits][m_rows][n_pitch]: sums so far
-  uint64_t m_rows;
+  uint32_t tile_m, tile_n, n_tiles;
+  uint32_t groups;         // or 0: a group has one row tile
+  bool dw;
+};
+// Values between slots, so that blocks that write theirs in step do not meet in a memory channel.
+constexpr uint32_t kSlotPad = 64;
+struct SplitShares {
+  uint32_t there, k, stages;  // rows of the piece; the summed axis; its stages
+  uint32_t units, groups;     // row tiles by stages: under 2^18, so that their product with the groups is of 32 bits
+  uint32_t m_tiles, of_tile;  // groups of a row tile, where all have as many: then no group has two, and those of all tiles go abreast
+  __device__ __forceinline__ SplitShares(const Split &a, uint32_t deep) {
+    there = *a.count > a.row0 ? *a.count - a.row0 : 0;
+    k = a.dw && there < a.k ? there : a.k;
+    m_tiles = ((!a.dw && there < a.m ? there : a.m) + a.tile_m - 1) / a.tile_m;
+    stages = (k + deep - 1) / deep;
+    units = m_tiles * stages;
+    groups = m_tiles;
+    of_tile = 1;
+    if (!a.groups) return;
+    of_tile = 0;
+    if (!units) {
+      groups = 0;
+      return;
+    }
+    groups = min(a.groups, units < 8 ? 1u : units / 8);  // eight stages at least, or four
+    const uint32_t more = (groups + m_tiles - 1) / m_tiles, fewer = more * m_tiles == groups ? more : more - 1;
+    if (more * m_tiles <= a.groups && more * m_tiles * 4 <= units) of_tile = more;
+    else if (fewer && (groups - fewer * m_tiles) * 16 <= groups) of_tile = fewer;
+    if (of_tile) groups = of_tile * m_tiles;
+  }
+  __device__ __forceinline__ uint32_t first(uint32_t group) const { return units * group / groups; }
+  __device__ __forceinline__ uint32_t of(uint32_t unit) const { return ((unit + 1) * groups - 1) / units; }
+};
+
+// A product of a piece: out[m][n] (+)= sum_k a[m][k] b[k][n].
+struct Product {
+  Split split;
+  Matrix a, b;             // a: panels of G
+  uint32_t n;              // columns, whole 16 bytes of values
+  float *slots;            // [blocks][2][a tile's rows][a tile's columns], kSlotPad apart
+  float *sums;             // [rows of the result][n_pitch]: the pieces' so far
   uint32_t n_pitch;
-  uint32_t m0;             // the piece's first row of parts
   bool first;              // nothing has been summed before
-  // A result that is whole with this launch is rounded and written, with the targets' terms.
+  // A result that is whole with a tile is rounded and written, with the targets' terms.
   void *to;                // [words][n_to], the piece's first (dx: [rows of the call][n_to]), or NULL
   uint32_t words, n_to;    // words: of the piece (dx: not looked at)
   bool f32;                // its type
@@ -181,16 +229,22 @@ __device__ __forceinline__ float neighbour(float v) {
 // DW: the summed axis are the rows of x, else the words. B: how x or the matrix lies.
 template <class T, class S, bool DW, Lies B>
 struct ProductTiles {
-  static constexpr bool kPuts = DW || S::M * S::N <= 4;  // large tiles of dx have their splits' sums to join anyway
+  static constexpr bool kPuts = DW || S::M * S::N <= 4;  // large tiles of dx have sums of pieces to join anyway
   static constexpr int kStores = 0;
   const Product &p;
-  uint32_t tiles, stages, m0, n0, k0, depth, split, there;  // there: rows of the piece
+  const SplitShares &share;
+  uint32_t tiles, slot, m_tile, n0, from, to, there;  // from, to: the block's units; m_tile: its first
   int lane, wave;
+  // The n-th tile's part of the summed axis, in stages.
+  __device__ __forceinline__ uint32_t begin(uint32_t n) const { return n ? 0 : from - m_tile * share.stages; }
+  __device__ __forceinline__ uint32_t end(uint32_t n) const { return n + 1 < tiles ? share.stages : to - (m_tile + n) * share.stages; }
+  __device__ __forceinline__ uint32_t stages(uint32_t n) const { return end(n) - begin(n); }
   template <class FA, class FB>
-  __device__ __forceinline__ void feed(uint32_t, FA &fa, FB &fb) {
+  __device__ __forceinline__ void feed(uint32_t n, FA &fa, FB &fb) {
+    const uint32_t m0 = (m_tile + n) * S::kM, k0 = begin(n) * kDeep<T>, k1 = end(n) * kDeep<T>, depth = min(k1, share.k) - k0;
     // k0, m0 and n0 are whole panels.
     if constexpr (DW) {
-      fa.start(p.a.at + m0 / kDeep<T> * p.a.pitch + (uint64_t)k0 * 64, p.a.pitch, p.m - m0, depth);
+      fa.start(p.a.at + m0 / kDeep<T> * p.a.pitch + (uint64_t)k0 * 64, p.a.pitch, S::kM, depth);
     } else {
       fa.start(p.a.at + k0 / kDeep<T> * p.a.pitch + (uint64_t)m0 * 64, p.a.pitch, S::kM, depth);
     }
@@ -198,7 +252,7 @@ struct ProductTiles {
     else fb.start(p.b.at + (int64_t)k0 * p.b.pitch + n0 * sizeof(T), p.b.pitch, p.n - n0, depth);
   }
   // bf16 results go out two columns a lane: two rows of a pair of lanes change places.
-  __device__ __forceinline__ void put(f32x16 (&sums)[S::M][S::N]) {
+  __device__ __forceinline__ void put(uint32_t m0, f32x16 (&sums)[S::M][S::N]) {
     const int half = lane >> 5;
     const uint32_t word0 = m0 + 32 * S::M * (wave >> 1), col0 = n0 + 32 * S::N * (wave & 1) + (lane & 31);
     const bool pairs = !p.f32 && p.n_to % 2 == 0 && ((uintptr_t)p.to & 3) == 0;
@@ -216,14 +270,14 @@ struct ProductTiles {
   }
   __device__ __forceinline__ float term(uint32_t word, uint64_t place, uint32_t col) const {
     if constexpr (DW) return p.terms[(uint64_t)word * p.n_pitch + col];
-    else return p.terms[place] * (float)((const bf16 *)p.w)[p.target[p.row0 + word] * p.w_stride + col];
+    else return p.terms[place] * (float)((const bf16 *)p.w)[p.target[p.split.row0 + word] * p.w_stride + col];
   }
   __device__ __forceinline__ void put(uint32_t first, uint32_t row, uint32_t col, uint32_t has, bool pairs, float a, float b) {
     const uint32_t word = first + row, most = DW ? p.words : there;
     uint64_t places[2] = {word, word + 1};
     if constexpr (!DW) {
 #pragma unroll
-      for (int e = 0; e < 2; e++) places[e] = word + e < there ? (uint32_t)p.order[p.row0 + word + e] : 0;
+      for (int e = 0; e < 2; e++) places[e] = word + e < there ? (uint32_t)p.order[p.split.row0 + word + e] : 0;
     }
     if (has) {
       if (has >> row & 1 && col < p.n_to) a += term(word, places[0], col);
@@ -244,93 +298,131 @@ struct ProductTiles {
       }
     }
   }
-  __device__ __forceinline__ void take(uint32_t, f32x16 (&sums)[S::M][S::N]) {
+  __device__ __forceinline__ void take(uint32_t n, f32x16 (&sums)[S::M][S::N]) {
     const int half = lane >> 5;
+    const uint32_t m0 = (m_tile + n) * S::kM;
+    const bool whole = begin(n) == 0 && end(n) == share.stages;
     if constexpr (kPuts)
-      if (p.to) return put(sums);
-    float *to = p.parts + (split * p.m_rows + p.m0 + m0 + 32 * S::M * (wave >> 1)) * p.n_pitch + n0 + 32 * S::N * (wave & 1) + (lane & 31);
-#pragma unroll
-    for (int j = 0; j < S::N; j++) {
-      if (n0 + 32 * S::N * (wave & 1) + 32 * j + (lane & 31) >= p.n) continue;
+      if (whole && p.to) return put(m0, sums);
+    const uint32_t row = 32 * S::M * (wave >> 1) + 4 * half, col = 32 * S::N * (wave & 1) + (lane & 31);
+    if (!whole) {
+      float *to = p.slots + (uint64_t)(2 * slot + (begin(n) == 0)) * (S::kM * S::kN + kSlotPad) + row * S::kN + col;
 #pragma unroll
       for (int i = 0; i < S::M; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          float *at = to + (uint64_t)(32 * i + row_of(r, half)) * p.n_pitch + 32 * j;
-          *at = p.first ? sums[i][j][r] : *at + sums[i][j][r];
-        }
+        for (int r = 0; r < 16; r++)
+#pragma unroll
+          for (int j = 0; j < S::N; j++) to[(32 * i + row_of(r, 0)) * S::kN + 32 * j] = sums[i][j][r];
+      return;
     }
+    float *to = p.sums + (uint64_t)(m0 + row) * p.n_pitch + n0 + col;
+#pragma unroll
+    for (int i = 0; i < S::M; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        float *at = to + (uint64_t)((32 * i + row_of(r, 0)) * p.n_pitch);
+#pragma unroll
+        for (int j = 0; j < S::N; j++) at[32 * j] = p.first ? sums[i][j][r] : at[32 * j] + sums[i][j][r];
+      }
   }
 };
 
 template <class T, class S, bool DW, Lies B>
 __global__ __launch_bounds__(256, S::kBlocks) void head_product(Product p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-  const uint32_t work = by_xcd(blockIdx.x, gridDim.x), n0 = work % p.n_tiles * S::kN, rest = work / p.n_tiles;
-  const uint32_t m0 = rest % p.m_tiles * S::kM, split = rest / p.m_tiles;
-  const uint32_t count = *p.count, there = count > p.row0 ? count - p.row0 : 0;  // of the piece's rows
-  uint32_t k = p.k;
-  if constexpr (DW) k = there < k ? there : k;
-  else if (m0 >= there) return;
-  // The share of the summed axis, in stages.
-  const uint32_t all = (k + kDeep<T> - 1) / kDeep<T>;
-  const uint32_t s0 = (uint32_t)((uint64_t)all * split / p.splits), s1 = (uint32_t)((uint64_t)all * (split + 1) / p.splits);
-  if (s0 == s1 && !p.first) return;
+  const SplitShares share(p.split, kDeep<T>);
+  const uint32_t blocks = share.groups * p.split.n_tiles;
+  if (blockIdx.x >= blocks) return;
+  const uint32_t work = by_xcd(blockIdx.x, blocks), n_tile = work % p.split.n_tiles, n0 = n_tile * S::kN;
+  uint32_t group = work / p.split.n_tiles;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t k0 = s0 * kDeep<T>, k1 = s1 * kDeep<T> < k ? s1 * kDeep<T> : k;
-  ProductTiles<T, S, DW, B> tiles{p, 1, s1 - s0, m0, n0, k0, k1 - k0, split, there, lane, wave};
+  if (!share.stages) {  // sums over nothing, a tile a group
+    ProductTiles<T, S, DW, B> tiles{p, share, 1, 0, group, n0, 0, 0, share.there, lane, wave};
+    f32x16 sums[S::M][S::N] = {};
+    return tiles.take(0, sums);
+  }
+  uint32_t from, to, m_tile, n = 1;
+  if (share.of_tile) {
+    const uint32_t part = group / share.m_tiles;
+    m_tile = group - part * share.m_tiles, group = m_tile * share.of_tile + part;
+    const uint32_t each = share.stages / share.of_tile, one = share.stages - each * share.of_tile;  // so many have one more
+    from = m_tile * share.stages + part * each + min(part, one), to = from + each + (part < one);
+  } else {
+    from = share.first(group), to = share.first(group + 1), m_tile = from / share.stages, n = (to - 1) / share.stages - m_tile + 1;
+  }
+  ProductTiles<T, S, DW, B> tiles{p, share, n, group * p.split.n_tiles + n_tile, m_tile, n0, from, to, share.there, lane, wave};
   run_tiles<T, S, !DW, PANELS, false, B>(lds, tiles);
 }
 
-// The splits' sums in their order, rounded to the result's type. dx: packed rows go to their own places, with
-// their targets' terms.
+// A product's tiles that no group has whole (or, where the product has not written them to their places, all tiles): the groups'
+// sums in their order, added to those of the pieces before; with the last piece rounded to the result's type. dx: packed
+// rows go to their own places, with their targets' terms.
 struct Ends {
-  const float *parts;
-  uint32_t splits, rows, n, n_pitch, row0;  // row0: the first's number of all packed rows
-  uint64_t m_rows;
-  const uint32_t *count;   // dx's: how many packed rows there are, or NULL
+  Split split;
+  uint32_t deep;           // values of a stage
+  const float *slots;
+  float *sums;             // the piece's
+  uint32_t n, n_pitch;
+  bool first, last;        // piece
+  bool put;                // the product has written whole tiles to their places
+  uint32_t rows;           // of the result's that are wanted; of dx as many as are packed
   const int32_t *order, *target;
-  const float *terms;      // dx's, or NULL
-  const uint8_t *present;  // dW's words with terms, which are the last of the splits; or NULL
+  const float *terms;      // dx: [rows of the call], or NULL
+  const float *word_terms; // dW: [words][n_pitch], or NULL
+  const uint8_t *present;  // dW's words with terms
   const void *w;           // the matrix as the caller has it
   int64_t w_stride;
   void *to;
 };
-// SHARES threads take eight values of a row, a stretch of the splits each.
+// SHARES threads take eight values of a row, a stretch of the slots each.
 template <class R, int SHARES>
 __global__ __launch_bounds__(256) void head_sums(Ends a) {
   constexpr uint32_t kEach = 256 / SHARES;
   __shared__ float joined[SHARES > 1 ? 256 : 1][9];
-  const uint32_t pieces = (a.n + 7) / 8, there = a.count ? (*a.count > a.row0 ? *a.count - a.row0 : 0) : a.rows;
-  const uint32_t limit = there < a.rows ? there : a.rows, share = threadIdx.x / kEach;
-  for (uint64_t base = (uint64_t)blockIdx.x * kEach; base < (uint64_t)limit * pieces; base += (uint64_t)gridDim.x * kEach) {
-    const uint64_t i = base + threadIdx.x % kEach, row = i / pieces;
-    const uint32_t col = eight_of((uint32_t)(i % pieces), a.n);
-    const bool mine = row < limit;
-    const uint32_t splits = a.splits + (mine && a.present && a.present[row]);
-    f32x8 v = {};
-    if (mine) {
-      const uint32_t from = splits * share / SHARES, to = splits * (share + 1) / SHARES;
+  const SplitShares share(a.split, a.deep);
+  // A block has some rows of a tile.
+  const uint32_t m_tile = blockIdx.x / a.split.n_tiles, n_tile = blockIdx.x % a.split.n_tiles;
+  const uint32_t mine = threadIdx.x / kEach, i = blockIdx.y * kEach + threadIdx.x % kEach, pieces = a.split.tile_n / 8;
+  const uint32_t row_in = i / pieces, col_in = i % pieces * 8, row = m_tile * a.split.tile_m + row_in, col = n_tile * a.split.tile_n + col_in;
+  const uint32_t limit = !a.split.dw && share.there < a.rows ? share.there : a.rows;
+  // The groups that have some of the tile.
+  uint32_t first = 0, n = 0;
+  if (m_tile * a.split.tile_m >= limit) return;
+  const uint32_t unit = m_tile * share.stages;
+  if (share.of_tile) first = m_tile * share.of_tile, n = share.of_tile;
+  else if (share.stages) first = share.of(unit), n = share.of(unit + share.stages - 1) - first + 1;
+  const bool whole = n == 1;
+  if (whole && (a.put || !a.last)) return;
+  const bool wanted = row < limit && col < a.n;
+  f32x8 v = {};
+  if (wanted && !whole) {
+    const uint32_t from = n * mine / SHARES, to = n * (mine + 1) / SHARES, tile = a.split.tile_m * a.split.tile_n + kSlotPad;
 #pragma unroll 8
-      for (uint32_t s = from; s < to; s++) v += load_some<float, 8>(a.parts + (s * a.m_rows + row) * a.n_pitch, true, col, a.n);
-    }
-    if constexpr (SHARES > 1) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) joined[threadIdx.x][e] = v[e];
-      __syncthreads();
-      if (share == 0)
-        for (int k = 1; k < SHARES; k++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[e] += joined[k * kEach + threadIdx.x][e];
-      __syncthreads();
-    }
-    if (!mine || share) continue;
-    const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.row0 + row] : row;
-    if (a.terms)
-      v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)a.w + a.target[a.row0 + row] * a.w_stride, true, col, a.n)), f32x8) *
-           a.terms[place];
-    store_some<R, 8>((R *)a.to + place * a.n, col, a.n, __builtin_convertvector(v, V8<R>));
+    for (uint32_t g = from; g < to; g++)
+      v += loose<float, 8>(a.slots + (uint64_t)(2 * ((first + g) * a.split.n_tiles + n_tile) + (g == 0)) * tile + row_in * a.split.tile_n + col_in);
   }
+  if constexpr (SHARES > 1) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) joined[threadIdx.x][e] = v[e];
+    __syncthreads();
+    if (mine == 0)
+      for (int k = 1; k < SHARES; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += joined[k * kEach + threadIdx.x][e];
+  }
+  if (!wanted || mine) return;
+  float *sums = a.sums + (uint64_t)row * a.n_pitch + col;
+  if (whole || !a.first) v += loose<float, 8>(sums);
+  if (!a.last) {
+    loose<float, 8>(sums, v);
+    return;
+  }
+  const uint64_t place = a.order ? (uint64_t)(uint32_t)a.order[a.split.row0 + row] : row;
+  if (a.present && a.present[row]) v += loose<float, 8>(a.word_terms + (uint64_t)row * a.n_pitch + col);
+  if (a.terms)
+    v += __builtin_convertvector((load_some<bf16, 8>((const bf16 *)a.w + a.target[a.split.row0 + row] * a.w_stride, true, col, a.n)), f32x8) *
+         a.terms[place];
+  store_some<R, 8>((R *)a.to + place * a.n, col, a.n, __builtin_convertvector(v, V8<R>));
 }
 
 // The targets' terms of dW for few rows, without a sort: a wavefront a row and 512 columns. The first row of
@@ -380,14 +472,20 @@ struct GradPlan {
   bool lay, small;
   uint32_t width, rows, words;  // a row's values; rows and words of a piece, whole tiles
   uint32_t all_rows, all_words;          // of the call, whole tiles
-  uint32_t n_tiles, x_splits, w_splits, n_pitch;
+  uint32_t tile_m, tile_n, at_once, n_tiles, n_pitch;
   uint32_t x_rows, w_rows;               // how many rows' and words' sums are kept at once
+  bool puts_x, puts_w;                   // products write whole tiles to their places: there are no pieces to be summed
   SortPlan sort;                         // of the targets, where x is bf16
-  uint64_t g, dx, dw, w, x, order, target, factors, terms, sorted, present, counts, count, bytes;
+  uint64_t g, dx, dw, slots, word_terms, w, x, order, target, factors, terms, sorted, present, counts, count, bytes;
 };
-uint32_t splits_for(uint32_t at_once, uint32_t tiles, uint32_t stages) {
-  const uint32_t want = at_once / tiles, most = stages / 8;
-  return want < 2 || most < 2 ? 1 : want < most ? want : most;
+// Groups that share a product's stages, or 0 where each takes a row tile. Tiles that do not fill the card's last turn leave it idle
+// for so many stages (of 0.9 us in large bf16 tiles and of 2.1 us in 32 bits); the tiles' sums in slots cost up to 40 us and 20.
+// 7,260 rows of 609 over 2,562 words in 32 bits 848 us, without shares 1,017; 24,576 of 32,768 rows of 256 over 32,768 words 2,199 and
+// 2,511; 1,322 rows of 1,838 over 11,168 words, whose dW would gain 30 stages, 425 with them and 366 without.
+uint32_t groups_for(const GradPlan &p, uint32_t m, uint32_t k, uint32_t deep) {
+  const uint64_t tiles = (uint64_t)((m + p.tile_m - 1) / p.tile_m) * p.n_tiles, stages = (k + deep - 1) / deep;
+  const uint64_t idle = (tiles + p.at_once - 1) / p.at_once * stages - tiles * stages / p.at_once;
+  return stages < 16 || (2 * tiles > p.at_once && idle < (deep == 32 ? 48 : 12)) ? 0 : p.at_once / p.n_tiles;
 }
 // The size of even pieces of `all` that are `most` at most, in whole large tiles.
 uint32_t even_pieces(uint64_t all, uint64_t most) {
@@ -400,7 +498,7 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   p.width = (uint32_t)up(s->width, 16 / size);
   p.lay = laid_out(s);
   p.small = small_tiles(s);
-  const uint32_t tile_m = p.small ? Small::kM : Large::kM, tile_n = p.small ? Small::kN : Large::kN, at_once = p.small ? 1024 : 512;
+  p.tile_m = p.small ? Small::kM : Large::kM, p.tile_n = p.small ? Small::kN : Large::kN, p.at_once = p.small ? 1024 : 512;
   p.all_rows = (uint32_t)up(s->rows, kRound), p.all_words = (uint32_t)up(s->vocab, kRound);
   // A piece of about as many rows as words, whose sums are read and written the least for the G between.
   const uint64_t values = kPiece / size;
@@ -409,18 +507,21 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   p.rows = even_pieces(p.all_rows, side);
   p.words = even_pieces(p.all_words, values / p.rows / kRound * kRound);
   p.rows = even_pieces(p.all_rows, values / p.words / kRound * kRound);
-  p.n_tiles = (p.width + tile_n - 1) / tile_n;
-  p.n_pitch = p.n_tiles * tile_n;
-  p.x_splits = splits_for(at_once, p.rows / tile_m * p.n_tiles, p.words / deep);
-  p.w_splits = splits_for(at_once, p.words / tile_m * p.n_tiles, p.rows / deep);
+  p.n_tiles = (p.width + p.tile_n - 1) / p.tile_n;
+  p.n_pitch = p.n_tiles * p.tile_n;
   // With the rows' pieces outside, the sums of dx are kept of one of them and those of dW of all words; or the
   // other way round.
-  const bool rows_outside = (uint64_t)p.x_splits * (p.all_rows - p.rows) > (uint64_t)p.w_splits * (p.all_words - p.words);
+  const bool rows_outside = p.all_rows - p.rows > p.all_words - p.words;
   p.x_rows = rows_outside ? p.rows : p.all_rows, p.w_rows = rows_outside ? p.all_words : p.words;
+  p.puts_x = p.small && p.words >= p.all_words, p.puts_w = p.rows >= p.all_rows;
+  const uint64_t x_units = (uint64_t)p.rows / p.tile_m * (p.words / deep), w_units = (uint64_t)p.words / p.tile_m * (p.rows / deep);
+  const uint64_t units = x_units > w_units ? x_units : w_units, groups = p.at_once / p.n_tiles, most = units < 8 ? 1 : units / 4;  // see SplitShares
   Scratch at;
   p.g = at.take((uint64_t)p.rows * p.words * size);
-  p.dx = at.take(4ull * p.x_splits * p.x_rows * p.n_pitch);
-  p.dw = at.take(4ull * (p.w_splits + (size == 2)) * p.w_rows * p.n_pitch);  // and the targets' terms
+  p.dx = at.take(p.puts_x ? 0 : 4ull * p.x_rows * p.n_pitch);
+  p.dw = at.take(p.puts_w ? 0 : 4ull * p.w_rows * p.n_pitch);
+  p.slots = at.take(8ull * (groups < most ? groups : most) * p.n_tiles * (p.tile_m * p.tile_n + kSlotPad));
+  p.word_terms = at.take(size == 2 ? 4ull * p.words * p.n_pitch : 0);
   p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
   p.x = at.take(up(p.all_rows, p.rows) * up(s->width * size, 64));
   p.order = at.take(4ull * p.all_rows);
@@ -440,11 +541,11 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
 
 template <class R>
 void sums(const Ends &a, hipStream_t stream) {
+  const uint32_t m_tiles = (a.rows + a.split.tile_m - 1) / a.split.tile_m;
   const auto run = [&](auto kernel, uint32_t each) {
-    const uint64_t blocks = ((uint64_t)a.rows * ((a.n + 7) / 8) + each - 1) / each;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(m_tiles * a.split.n_tiles, a.split.tile_m * a.split.tile_n / 8 / each), dim3(256), 0, stream, a);
   };
-  if (a.splits >= 16) run(head_sums<R, 8>, 32);
+  if (a.split.groups >= 16 * m_tiles) run(head_sums<R, 8>, 32);
   else run(head_sums<R, 1>, 256);
 }
 
@@ -452,7 +553,6 @@ template <class T>
 int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const GradPlan p = grad_plan(s);
   const int64_t panel = (int64_t)p.rows * 64;  // of G and of a piece of x
-  const uint32_t tile_m = p.small ? Small::kM : Large::kM, tile_n = p.small ? Small::kN : Large::kN, at_once = p.small ? 1024 : 512;
   Matrix w{(const char *)s->weight, s->w_stride * (int64_t)sizeof(T)};
   if (p.lay) w = lay<T>(s->weight, s->w_stride, s->vocab, s->width, work + p.w, stream);
   uint32_t *count = (uint32_t *)(work + p.count);
@@ -478,15 +578,15 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     const uint32_t row_piece = rows_outside ? i / word_pieces : i % row_pieces, word_piece = rows_outside ? i % word_pieces : i / row_pieces;
     const uint32_t row0 = row_piece * p.rows, word0 = word_piece * p.words;
     const uint32_t rows = s->rows - row0 < p.rows ? s->rows - row0 : p.rows, words = s->vocab - word0 < p.words ? s->vocab - word0 : p.words;
-    const uint32_t word_tiles = (words + tile_m - 1) / tile_m;
+    const uint32_t word_tiles = (words + p.tile_m - 1) / p.tile_m;
     Logits l{};
     const Matrix x{work + p.x + (uint64_t)row0 * up(s->width * sizeof(T), 64), panel};
     l.w = w, l.x = x, l.rows = s->rows, l.vocab = s->vocab, l.width = p.width;
-    l.row0 = row0, l.row_tiles = (rows + tile_n - 1) / tile_n, l.word0 = word0, l.word_tiles = word_tiles;
-    const uint32_t want = (2 * at_once + l.row_tiles - 1) / l.row_tiles;
-    l.splits = want < word_tiles ? want : word_tiles;
+    l.row0 = row0, l.piece_rows = rows, l.word0 = word0, l.word_tiles = word_tiles;
     l.count = count, l.target = k.target, l.factors = k.factors, l.order = k.order, l.terms = terms, l.g = work + p.g, l.g_rows = p.rows;
-    const auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.row_tiles * l.splits), dim3(256), 0, stream, l); };
+    const uint32_t row_tiles = (rows + p.tile_n - 1) / p.tile_n;
+    l.blocks = scan_blocks(row_tiles, word_tiles, p.at_once), l.at_once = p.at_once;
+    const auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(scan_grid(row_tiles, word_tiles, p.at_once)), dim3(256), 0, stream, l); };
     bool few = false;
     if constexpr (sizeof(T) == 4) few = few_rows(s);
     if (few) {
@@ -497,56 +597,53 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       if constexpr (sizeof(T) == 4) s->rows <= 16 ? run(head_few_logits<1>) : s->rows <= 32 ? run(head_few_logits<2>) : run(head_few_logits<4>);
     } else if (p.small) p.lay ? logits(head_logits<T, Small, PANELS>) : logits(head_logits<T, Small, ROWS>);
     else if constexpr (sizeof(T) == 2) p.lay ? logits(head_logits<T, Large, PANELS>) : logits(head_logits<T, Large, ROWS>);
+    constexpr uint32_t deep = kDeep<T>;
     Product a{};
-    const auto product = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.m_tiles * a.n_tiles * a.splits), dim3(256), 0, stream, a); };
-    a.a = {work + p.g, panel}, a.row0 = row0, a.count = count, a.n = p.width, a.n_tiles = p.n_tiles, a.n_pitch = p.n_pitch;
+    const auto product = [&](auto kernel) {
+      const uint32_t groups = a.split.groups ? a.split.groups : (a.split.m + p.tile_m - 1) / p.tile_m;
+      hipLaunchKernelGGL(kernel, dim3(groups * p.n_tiles), dim3(256), 0, stream, a);
+    };
+    a.split = {0, 0, row0, count, p.tile_m, p.tile_n, p.n_tiles, 0, false};
+    a.a = {work + p.g, panel}, a.n = p.width, a.n_pitch = p.n_pitch, a.slots = (float *)(work + p.slots);
+    Ends e{};
+    e.deep = deep, e.slots = a.slots, e.n = s->width, e.n_pitch = p.n_pitch;
     if (s->dx) {
+      a.split.m = rows, a.split.k = words, a.split.groups = groups_for(p, rows, words, deep);
       a.b = {w.at + (int64_t)word0 * (p.lay ? 64 : w.pitch), w.pitch};
-      a.m = rows, a.k = words, a.m_tiles = (rows + tile_m - 1) / tile_m, a.splits = p.x_splits;
-      a.parts = (float *)(work + p.dx), a.m_rows = p.x_rows, a.m0 = rows_outside ? 0 : row0, a.first = word0 == 0;
-      const bool direct = p.small && p.x_splits == 1 && word_pieces == 1;
-      if (direct) {
+      a.sums = (float *)(work + p.dx) + (uint64_t)(rows_outside ? 0 : row0) * p.n_pitch, a.first = word0 == 0;
+      if (p.puts_x) {
         a.to = s->dx, a.n_to = s->width, a.f32 = sizeof(T) == 4;
         a.terms = terms, a.order = k.order, a.target = k.target, a.w = s->weight, a.w_stride = s->w_stride;
       }
       if (p.small) p.lay ? product(head_product<T, Small, false, PANELS>) : product(head_product<T, Small, false, ROWS>);
       else if constexpr (sizeof(T) == 2) p.lay ? product(head_product<T, Large, false, PANELS>) : product(head_product<T, Large, false, ROWS>);
-      if (!direct && word_piece + 1 == word_pieces) {
-        Ends e{};
-        e.n = s->width, e.n_pitch = p.n_pitch;
-        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.x_splits, e.rows = rows, e.row0 = row0, e.m_rows = p.x_rows;
-        e.count = count, e.order = k.order, e.target = k.target, e.terms = terms, e.w = s->weight, e.w_stride = s->w_stride, e.to = s->dx;
-        sums<T>(e, stream);
-      }
+      e.split = a.split, e.sums = a.sums, e.first = a.first, e.last = word_piece + 1 == word_pieces, e.put = p.puts_x, e.rows = rows;
+      e.order = k.order, e.target = k.target, e.terms = terms, e.w = s->weight, e.w_stride = s->w_stride, e.to = s->dx;
+      if (a.split.groups || (e.last && !e.put)) sums<T>(e, stream);
     }
     if (s->dweight) {
-      a.to = nullptr, a.terms = nullptr;
+      a.split.m = words, a.split.k = rows, a.split.groups = groups_for(p, words, rows, deep), a.split.dw = true;
       a.b = x;
-      a.m = (uint32_t)up(words, kRound), a.k = rows, a.m_tiles = word_tiles, a.splits = p.w_splits;
-      a.parts = (float *)(work + p.dw), a.m_rows = p.w_rows, a.m0 = rows_outside ? word0 : 0, a.first = row0 == 0;
-      const bool last = row_piece + 1 == row_pieces, direct = last && a.first && p.w_splits == 1;
-      const bool f32 = s->dweight_dtype == UOR_TRUNK_F32;
+      a.sums = (float *)(work + p.dw) + (uint64_t)(rows_outside ? word0 : 0) * p.n_pitch, a.first = row0 == 0;
+      a.to = nullptr, a.terms = nullptr;
+      const bool last = row_piece + 1 == row_pieces, f32 = s->dweight_dtype == UOR_TRUNK_F32;
       void *to = (char *)s->dweight + (uint64_t)word0 * s->width * size_of(s->dweight_dtype);
       if (kTerms && last) {
-        t.word0 = word0, t.words = words, t.to = a.parts + ((uint64_t)p.w_splits * p.w_rows + a.m0) * p.n_pitch, t.present = k.present + word0;
+        t.word0 = word0, t.words = words, t.to = work + p.word_terms, t.present = k.present + word0;
         if (s->rows <= kFewTerms)
           hipLaunchKernelGGL((head_terms<T>), dim3(s->rows, (s->width + 511) / 512), dim3(64), 0, stream, t, s->targets, s->wide != 0, s->vocab);
         else sum_rows<float, T>(t, stream);
       }
-      if (direct) {
+      if (p.puts_w) {
         a.to = to, a.words = words, a.n_to = s->width, a.f32 = f32;
         if (kTerms) a.present = t.present, a.terms = (const float *)t.to;
       }
       if (p.small) product(head_product<T, Small, true, PANELS>);
       else if constexpr (sizeof(T) == 2) product(head_product<T, Large, true, PANELS>);
-      if (last && !direct) {
-        Ends e{};
-        e.n = s->width, e.n_pitch = p.n_pitch;
-        e.parts = a.parts + (uint64_t)a.m0 * p.n_pitch, e.splits = p.w_splits, e.rows = words, e.m_rows = p.w_rows, e.to = to;
-        if (kTerms) e.present = t.present;
-        if (f32) sums<float>(e, stream);
-        else sums<bf16>(e, stream);
-      }
+      e.split = a.split, e.sums = a.sums, e.first = a.first, e.last = last, e.put = p.puts_w, e.rows = words;
+      e.order = nullptr, e.terms = nullptr, e.to = to;
+      if (kTerms && last) e.present = t.present, e.word_terms = (const float *)t.to;
+      if (a.split.groups || (last && !e.put)) f32 ? sums<float>(e, stream) : sums<bf16>(e, stream);
     }
   }
   return launched();

@@ -200,8 +200,8 @@ struct Reader {
   }
 };
 
-// A block's tiles one after another. `work` says how many there are and of how many stages each
-// (tiles, stages), gives the feeds of the n-th (feed(n, a, b)) and takes its sums (take(n, sums), with kStores
+// A block's tiles one after another. `work` says how many there are (tiles) and of how many stages each (stages(n)), gives the
+// feeds of the n-th (feed(n, a, b)) and takes its sums (take(n, sums), with kStores
 // stores at least to memory). The loads run two stages ahead, over a tile's end into the next. Loads and stores end in
 // their order, so that behind a tile's stores the next two stages wait for loads alone: with a wait for the stores
 // too, 8,192 x 16,384 logits of width 1,024 and their G took 372 us, without 348.
@@ -214,25 +214,18 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   ra.start(lane, S::M * (wave >> 1));
   rb.start(lane, S::N * (wave & 1));
-  const uint32_t tiles = work.tiles, stages = work.stages;
-  if (!stages) {  // sums over nothing
-    for (uint32_t n = 0; n < tiles; n++) {
-      f32x16 sums[S::M][S::N] = {};
-      work.take(n, sums);
-    }
-    return;
-  }
+  const uint32_t tiles = work.tiles;
+  if (!tiles) return;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-  uint32_t ahead_tile = 0, ahead = 0, put = 0;
+  uint32_t ahead_tile = 0, ahead = work.stages(0), put = 0;
   work.feed(0, fa, fb);
   auto issue = [&]() {
     uint32_t at[S::M], bt[S::N];
     const u32x4 a = fa.next(at), b = fb.next(bt);
     to_lds(lds0 + put + wave * 1024, a, at, b, bt);
     put = put == (kStages - 1) * S::kStageBytes ? 0 : put + S::kStageBytes;
-    if (++ahead == stages) {
-      ahead = 0;
-      if (++ahead_tile < tiles) work.feed(ahead_tile, fa, fb);
+    if (!--ahead) {
+      if (++ahead_tile < tiles) ahead = work.stages(ahead_tile), work.feed(ahead_tile, fa, fb);
       else fa.nothing(), fb.nothing();
     }
   };
@@ -243,6 +236,7 @@ __device__ __forceinline__ void run_tiles(char *lds, Work &work) {
   static_assert(!kFold || S::M * S::N <= 4, "no registers for two sets of sums");
   for (uint32_t n = 0; n < tiles; n++) {
     f32x16 sums[S::M][S::N] = {}, folded[kFold ? S::M : 1][kFold ? S::N : 1] = {};
+    const uint32_t stages = work.stages(n);
     for (uint32_t k = 0; k < stages; k++) {
       if (kFold && k && k % 8 == 0) {
 #pragma unroll
