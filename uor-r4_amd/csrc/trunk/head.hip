@@ -19,7 +19,9 @@ struct Scan {
   uint32_t word_tiles;          // in the shape's tiles
   uint32_t blocks, at_once;     // see RowShares
   const uint32_t *count;        // how many rows there are, or NULL: `rows`
-  const int32_t *target;        // [rows up to 256]
+  const int32_t *target;        // [rows up to 256] of packed rows
+  const void *targets;          // the caller's, of rows that are not
+  bool wide;
   Sum *parts;                   // [group + set][abreast][2][a tile's rows], see RowShares: groups and sets go on together
 };
 
@@ -49,9 +51,8 @@ __device__ __forceinline__ void join_value(float &value, uint32_t &place, float 
   }
 }
 
-template <class T, class S, bool PICK, Lies W>
+template <class T, class S, bool PICK, Lies W, Lies X>
 struct ScanTiles {
-  static constexpr Lies kX = PICK ? W : PANELS;
   using Run = Running<sizeof(T) == 2>;
   static constexpr int kStores = 0;
   const Scan &a;
@@ -68,7 +69,10 @@ struct ScanTiles {
 #pragma unroll
     for (int j = 0; j < S::N; j++) {
       run[j] = Run{}, value[j] = PICK ? -__builtin_inff() : 0.0f, place[j] = 0;
-      target[j] = PICK ? -1 : a.target[at.row * S::kN + 32 * S::N * (wave & 1) + 32 * j + (lane & 31)];
+      const uint32_t row = at.row * S::kN + 32 * S::N * (wave & 1) + 32 * j + (lane & 31);
+      if constexpr (PICK) target[j] = -1;
+      else if constexpr (X == PANELS) target[j] = a.target[row];
+      else target[j] = row < a.rows ? target_of(a.targets, a.wide, row, a.vocab) : -1;
     }
   }
   __device__ __forceinline__ void close() {
@@ -86,7 +90,7 @@ struct ScanTiles {
     const uint32_t word = ahead.word * S::kM, row0 = ahead.row * S::kN;
     ahead.next();
     fa.start(a.w.at + (int64_t)word * (W == ROWS ? a.w.pitch : 64), a.w.pitch, a.vocab - word, a.width);
-    fb.start(a.x.at + (int64_t)row0 * (kX == ROWS ? a.x.pitch : 64), a.x.pitch, a.rows - row0, a.width);
+    fb.start(a.x.at + (int64_t)row0 * (X == ROWS ? a.x.pitch : 64), a.x.pitch, a.rows - row0, a.width);
   }
   __device__ __forceinline__ void take(uint32_t n, f32x16 (&z)[S::M][S::N]) {
     const int half = lane >> 5;
@@ -134,16 +138,16 @@ struct ScanTiles {
   }
 };
 
-template <class T, class S, bool PICK, Lies W>
+template <class T, class S, bool PICK, Lies W, Lies X>
 __global__ __launch_bounds__(256, S::kBlocks) void head_scan(Scan a) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
   const uint32_t rows = a.count ? *a.count : a.rows;
   const Walk walk(RowShares(rows, S::kN, a.word_tiles, a.blocks, a.at_once), a.word_tiles, blockIdx.x);
   if (!walk.tiles) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  ScanTiles<T, S, PICK, W> tiles{a, walk.tiles, walk, walk, lane, wave};
+  ScanTiles<T, S, PICK, W, X> tiles{a, walk.tiles, walk, walk, lane, wave};
   tiles.open();
-  run_tiles<T, S, true, W, true, tiles.kX>(lds, tiles);
+  run_tiles<T, S, true, W, true, X>(lds, tiles);
 }
 
 template <class T, bool PICK, int TILES>
@@ -250,9 +254,17 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t tile
 
 namespace {
 
+// Whether a loss takes its rows as they lie, those without a target too, whose results are then dropped: where one tile a block is
+// all there is, and its products are too little to be worth the rows' packing. 333 rows of 200 over 4,100 words in 32 bits 16 us,
+// packed 19; of 512 over 8,000 43 and, seven in ten without a target, 32; 800 rows of 512 over 8,000 in bf16 20 and 27, or 21 and 17.
+bool as_they_are(const uor_trunk_head_args *s, uint64_t tiles, uint32_t at_once) {
+  return tiles <= at_once && 2.0 * s->rows * s->vocab * s->width <= (s->dtype == UOR_TRUNK_F32 ? 1.2e9 : 7e9) &&
+         as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype);
+}
 // Where a call's scratch memory has what.
 struct Plan {
   bool lay, small;  // the matrix is laid out anew; small tiles
+  bool packed;      // a loss: the rows with a target next to each other
   uint32_t few;  // blocks of the few rows' kernel, or 0
   uint32_t width, tile, word_tiles, at_once, blocks, grid;
   uint64_t parts, w, x, order, target, counts, count, bytes;
@@ -278,13 +290,14 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
   p.blocks = scan_blocks(row_tiles, p.word_tiles, p.at_once), p.grid = scan_grid(row_tiles, p.word_tiles, p.at_once);
   Scratch at;
   const uint64_t rows = up(s->rows, kRound);
+  p.packed = !pick && (p.lay || !as_they_are(s, (uint64_t)row_tiles * p.word_tiles, p.at_once));
   p.parts = at.take(2ull * (p.grid + row_tiles) * p.tile * sizeof(Sum));
   p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
-  p.x = at.take(pick && !p.lay ? 0 : rows * up(s->width * size, 64));
-  p.order = at.take(pick ? 0 : rows * 4);
-  p.target = at.take(pick ? 0 : rows * 4);
-  p.counts = at.take(pick ? 0 : (s->rows + kPackRows - 1) / kPackRows * 4);
-  p.count = at.take(pick ? 0 : 4);
+  p.x = at.take(p.lay || p.packed ? rows * up(s->width * size, 64) : 0);
+  p.order = at.take(p.packed ? rows * 4 : 0);
+  p.target = at.take(p.packed ? rows * 4 : 0);
+  p.counts = at.take(p.packed ? (s->rows + kPackRows - 1) / kPackRows * 4 : 0);
+  p.count = at.take(p.packed ? 4 : 0);
   p.bytes = at.bytes;
   return p;
 }
@@ -294,7 +307,7 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const Plan p = plan_of(s, PICK);
   const auto join = [&](auto kernel, uint32_t each, const Sum *parts, uint32_t blocks, const uint32_t *count) {
     hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, parts, p.tile, p.word_tiles, blocks, p.at_once, s->rows, count,
-                       PICK || p.few ? nullptr : (const int32_t *)(work + p.order), s->targets, s->wide != 0, s->vocab, s->losses, s->lse, s->tokens,
+                       p.packed ? (const int32_t *)(work + p.order) : nullptr, s->targets, s->wide != 0, s->vocab, s->losses, s->lse, s->tokens,
                        s->logprobs);
   };
   if (p.few) {
@@ -312,7 +325,8 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   a.parts = (Sum *)(work + p.parts);
   a.w = {(const char *)s->weight, s->w_stride * (int64_t)sizeof(T)};
   if (p.lay) a.w = lay<T>(s->weight, s->w_stride, s->vocab, s->width, work + p.w, stream);
-  if constexpr (PICK) {
+  a.targets = s->targets, a.wide = s->wide != 0;
+  if (!p.packed) {
     if (p.lay) a.x = lay<T>(s->x, s->x_stride, s->rows, s->width, work + p.x, stream);
     else a.x = {(const char *)s->x, s->x_stride * (int64_t)sizeof(T)};
   } else {
@@ -327,8 +341,15 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   }
   const dim3 grid(p.grid);
   const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
-  if (p.small) p.lay ? run(head_scan<T, Small, PICK, PANELS>) : run(head_scan<T, Small, PICK, ROWS>);
-  else if constexpr (sizeof(T) == 2) p.lay ? run(head_scan<T, Large, PICK, PANELS>) : run(head_scan<T, Large, PICK, ROWS>);
+  const auto tiles = [&](auto shape) {
+    using S = decltype(shape);
+    constexpr Lies kOther = PICK ? ROWS : PANELS;
+    if (p.lay) run(head_scan<T, S, PICK, PANELS, PANELS>);
+    else if (PICK || !p.packed) run(head_scan<T, S, PICK, ROWS, ROWS>);
+    else run(head_scan<T, S, PICK, ROWS, kOther>);
+  };
+  if (p.small) tiles(Small{});
+  else if constexpr (sizeof(T) == 2) tiles(Large{});
   constexpr bool kBase2 = sizeof(T) == 2;
   // More than 128 parts a row: by a block.
   const uint32_t row_tiles = (s->rows + p.tile - 1) / p.tile;
