@@ -119,11 +119,33 @@ inline bool as_it_lies(const void *p, int64_t stride, uint32_t rows, uint32_t wi
 // and 9,579.
 constexpr uint32_t kLayRows = 1024;
 inline bool laid_out(const uor_trunk_head_args *s) { return s->rows >= kLayRows || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype); }
-// Whether small tiles are taken: in 32 bits, where there are registers for two sets of sums of them, and where the large
-// ones would leave some compute units idle (333 rows over 4,099 words of 100 in 32 bits: 18 us, 26 in large tiles; 501 over
-// 5,003 of 200 and their gradients 103 and 143).
-inline bool small_tiles(const uor_trunk_head_args *s) {
-  return s->dtype == UOR_TRUNK_F32 || up(s->rows, Large::kN) / Large::kN * (up(s->vocab, Large::kM) / Large::kM) < 256;
+// A call's tiles. Small ones where large ones would leave some compute units idle (333 rows over 4,099 words of 100 in 32 bits: 18 us, 26
+// in large tiles; 501 over 5,003 of 200 and their gradients 103 and 143), and in 32 bits, where there are no registers for two sets of
+// sums of large ones. Tiny ones where small ones would leave half of the units idle (loss and gradients of 500 rows of 512 over 1,500
+// words in 32 bits 87 us, in small tiles 95; but of 333 of 100 over 4,099 59 and 56).
+struct Tiling {
+  uint32_t m, n, at_once;  // at_once: that the card takes
+};
+template <class S>
+constexpr Tiling kTiling = {S::kM, S::kN, 256 * S::kBlocks};
+template <class S>
+inline bool fewer_than(const uor_trunk_head_args *s, uint64_t tiles) {
+  return up(s->rows, S::kN) / S::kN * (up(s->vocab, S::kM) / S::kM) < tiles;
+}
+// f of the call's shape of tiles, as an object of it; and what they are.
+template <class T, class F>
+inline void with_tiles(const uor_trunk_head_args *s, F f) {
+  if (fewer_than<Small>(s, 128)) f(Tiny{});
+  else if constexpr (sizeof(T) == 4) f(Small{});
+  else if (fewer_than<Large>(s, 256)) f(Small{});
+  else f(Large{});
+}
+inline Tiling tiling(const uor_trunk_head_args *s) {
+  Tiling t;
+  const auto set = [&](auto shape) { t = kTiling<decltype(shape)>; };
+  if (s->dtype == UOR_TRUNK_F32) with_tiles<float>(s, set);
+  else with_tiles<bf16>(s, set);
+  return t;
 }
 inline int check_head(const uor_trunk_head_args *s) {
   if (!s) return fail(-1, "null argument");

@@ -128,7 +128,8 @@ struct ScanTiles {
       for (int i = 0; i < S::M; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) sum[i] += Run::term(z[i][j][r], base);
-      float total = sum[0] + sum[1];
+      float total = sum[0];
+      if constexpr (S::M >= 2) total += sum[1];
       if constexpr (S::M == 4) total += sum[2] + sum[3];
       run[j].sum = fmaf(run[j].sum, Run::power(run[j].most - base), total);
       run[j].most = base;
@@ -263,8 +264,8 @@ bool as_they_are(const uor_trunk_head_args *s, uint64_t tiles, uint32_t at_once)
 }
 // Where a call's scratch memory has what.
 struct Plan {
-  bool lay, small;  // the matrix is laid out anew; small tiles
-  bool packed;      // a loss: the rows with a target next to each other
+  bool lay;     // the matrix is laid out anew
+  bool packed;  // a loss: the rows with a target next to each other
   uint32_t few;  // blocks of the few rows' kernel, or 0
   uint32_t width, tile, word_tiles, at_once, blocks, grid;
   uint64_t parts, w, x, order, target, counts, count, bytes;
@@ -282,11 +283,9 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
   p.lay = pick ? !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype) ||
                      !as_it_lies(s->x, s->x_stride, s->rows, s->width, s->dtype)
                : laid_out(s);
-  p.small = small_tiles(s);
-  p.tile = p.small ? Small::kN : Large::kN;
-  const uint32_t m = p.small ? Small::kM : Large::kM, row_tiles = (s->rows + p.tile - 1) / p.tile;
-  p.word_tiles = (s->vocab + m - 1) / m;
-  p.at_once = p.small ? 1024 : 512;
+  const Tiling t = tiling(s);
+  p.tile = t.n, p.at_once = t.at_once, p.word_tiles = (s->vocab + t.m - 1) / t.m;
+  const uint32_t row_tiles = (s->rows + t.n - 1) / t.n;
   p.blocks = scan_blocks(row_tiles, p.word_tiles, p.at_once), p.grid = scan_grid(row_tiles, p.word_tiles, p.at_once);
   Scratch at;
   const uint64_t rows = up(s->rows, kRound);
@@ -341,15 +340,13 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   }
   const dim3 grid(p.grid);
   const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
-  const auto tiles = [&](auto shape) {
+  with_tiles<T>(s, [&](auto shape) {
     using S = decltype(shape);
     constexpr Lies kOther = PICK ? ROWS : PANELS;
     if (p.lay) run(head_scan<T, S, PICK, PANELS, PANELS>);
     else if (PICK || !p.packed) run(head_scan<T, S, PICK, ROWS, ROWS>);
     else run(head_scan<T, S, PICK, ROWS, kOther>);
-  };
-  if (p.small) tiles(Small{});
-  else if constexpr (sizeof(T) == 2) tiles(Large{});
+  });
   constexpr bool kBase2 = sizeof(T) == 2;
   // More than 128 parts a row: by a block.
   const uint32_t row_tiles = (s->rows + p.tile - 1) / p.tile;

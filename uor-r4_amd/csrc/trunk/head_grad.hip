@@ -491,7 +491,7 @@ namespace {
 constexpr uint64_t kPiece = 1ull << 30;
 
 struct GradPlan {
-  bool lay, small;
+  bool lay;
   uint32_t width, rows, words;  // a row's values; rows and words of a piece, whole tiles
   uint32_t all_rows, all_words;          // of the call, whole tiles
   uint32_t tile_m, tile_n, at_once, n_tiles, n_pitch;
@@ -519,8 +519,8 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   const uint32_t size = size_of(s->dtype), deep = 64 / size;
   p.width = (uint32_t)up(s->width, 16 / size);
   p.lay = laid_out(s);
-  p.small = small_tiles(s);
-  p.tile_m = p.small ? Small::kM : Large::kM, p.tile_n = p.small ? Small::kN : Large::kN, p.at_once = p.small ? 1024 : 512;
+  const Tiling t = tiling(s);
+  p.tile_m = t.m, p.tile_n = t.n, p.at_once = t.at_once;
   p.all_rows = (uint32_t)up(s->rows, kRound), p.all_words = (uint32_t)up(s->vocab, kRound);
   // A piece of about as many rows as words, whose sums are read and written the least for the G between.
   const uint64_t values = kPiece / size;
@@ -535,7 +535,7 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   // other way round.
   const bool rows_outside = p.all_rows - p.rows > p.all_words - p.words;
   p.x_rows = rows_outside ? p.rows : p.all_rows, p.w_rows = rows_outside ? p.all_words : p.words;
-  p.puts_x = p.small && p.words >= p.all_words, p.puts_w = p.rows >= p.all_rows;
+  p.puts_x = p.tile_m < Large::kM && p.words >= p.all_words, p.puts_w = p.rows >= p.all_rows;
   const uint64_t x_units = (uint64_t)p.rows / p.tile_m * (p.words / deep), w_units = (uint64_t)p.words / p.tile_m * (p.rows / deep);
   const uint64_t units = x_units > w_units ? x_units : w_units, groups = p.at_once / p.n_tiles, most = units < 8 ? 1 : units / 4;  // see SplitShares
   Scratch at;
@@ -617,8 +617,12 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
       const uint32_t groups = (words + 15) / 16;
       const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups < 1024 ? groups : 1024), dim3(256), s->rows * f.pitch, stream, v); };
       if constexpr (sizeof(T) == 4) s->rows <= 16 ? run(head_few_logits<1>) : s->rows <= 32 ? run(head_few_logits<2>) : run(head_few_logits<4>);
-    } else if (p.small) p.lay ? logits(head_logits<T, Small, PANELS>) : logits(head_logits<T, Small, ROWS>);
-    else if constexpr (sizeof(T) == 2) p.lay ? logits(head_logits<T, Large, PANELS>) : logits(head_logits<T, Large, ROWS>);
+    } else {
+      with_tiles<T>(s, [&](auto shape) {
+        using S = decltype(shape);
+        p.lay ? logits(head_logits<T, S, PANELS>) : logits(head_logits<T, S, ROWS>);
+      });
+    }
     constexpr uint32_t deep = kDeep<T>;
     Product a{};
     const auto product = [&](auto kernel) {
@@ -637,8 +641,10 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
         a.to = s->dx, a.n_to = s->width, a.f32 = sizeof(T) == 4;
         a.terms = terms, a.order = k.order, a.target = k.target, a.w = s->weight, a.w_stride = s->w_stride;
       }
-      if (p.small) p.lay ? product(head_product<T, Small, false, PANELS>) : product(head_product<T, Small, false, ROWS>);
-      else if constexpr (sizeof(T) == 2) p.lay ? product(head_product<T, Large, false, PANELS>) : product(head_product<T, Large, false, ROWS>);
+      with_tiles<T>(s, [&](auto shape) {
+        using S = decltype(shape);
+        p.lay ? product(head_product<T, S, false, PANELS>) : product(head_product<T, S, false, ROWS>);
+      });
       e.split = a.split, e.sums = a.sums, e.first = a.first, e.last = word_piece + 1 == word_pieces, e.put = p.puts_x, e.rows = rows;
       e.order = k.order, e.target = k.target, e.terms = terms, e.w = s->weight, e.w_stride = s->w_stride, e.to = s->dx;
       if (a.split.groups || (e.last && !e.put)) sums<T>(e, stream);
@@ -660,8 +666,7 @@ int grad(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
         a.to = to, a.words = words, a.n_to = s->width, a.f32 = f32;
         if (kTerms) a.present = t.present, a.terms = (const float *)t.to;
       }
-      if (p.small) product(head_product<T, Small, true, PANELS>);
-      else if constexpr (sizeof(T) == 2) product(head_product<T, Large, true, PANELS>);
+      with_tiles<T>(s, [&](auto shape) { product(head_product<T, decltype(shape), true, PANELS>); });
       e.split = a.split, e.sums = a.sums, e.first = a.first, e.last = last, e.put = p.puts_w, e.rows = words;
       e.order = nullptr, e.terms = nullptr, e.to = to;
       if (kTerms && last) e.present = t.present, e.word_terms = (const float *)t.to;

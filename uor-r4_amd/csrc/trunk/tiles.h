@@ -1,4 +1,4 @@
-// tiles.h - products of two matrices by tiles of 256 x 128: what the head's kernels share.
+// tiles.h - products of two matrices by tiles of 256 x 128 (or 128 x 64, or 64 x 64): what the head's kernels share.
 //
 // A block of four wavefronts takes a tile of 256 x 128 sums, each wavefront 128 x 64 of it in 128
 // registers a lane, as 4 x 2 results of 32 x 32 of the matrix instruction. Both operands come by
@@ -41,6 +41,7 @@ struct Shape {
 };
 using Large = Shape<4, 2>;
 using Small = Shape<2, 1>;
+using Tiny = Shape<1, 1>;
 constexpr int kRound = 256;  // rows and words are rounded up to whole large tiles
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset that no buffer has: the load gives zeros
 template <class T>
@@ -108,6 +109,11 @@ __device__ __forceinline__ void to_lds(uint32_t to, u32x4 a, const uint32_t (&at
 __device__ __forceinline__ void to_lds(uint32_t to, u32x4 a, const uint32_t (&at)[2], u32x4 b, const uint32_t (&bt)[1]) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" LOAD("%1", "%4") NEXT LOAD("%2", "%4") NEXT LOAD("%3", "%5")
                ::"s"(to), "v"(at[0]), "v"(at[1]), "v"(bt[0]), "s"(a), "s"(b)
+               : "memory", "scc");
+}
+__device__ __forceinline__ void to_lds(uint32_t to, u32x4 a, const uint32_t (&at)[1], u32x4 b, const uint32_t (&bt)[1]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" LOAD("%1", "%3") NEXT LOAD("%2", "%4")
+               ::"s"(to), "v"(at[0]), "v"(bt[0]), "s"(a), "s"(b)
                : "memory", "scc");
 }
 #undef LOAD
