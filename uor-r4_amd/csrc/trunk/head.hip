@@ -198,16 +198,15 @@ __global__ __launch_bounds__(256) void head_few(Few a) {
   }
 }
 
-// WAVES wavefronts join a row's parts: of tiles of `tile` rows, see Scan, or (0) of few rows, one a block.
-template <bool PICK, int WAVES, bool BASE2>
+// LANES threads join a row's parts: of tiles of `tile` rows, see Scan, or (0) of few rows, one a block.
+template <bool PICK, int LANES, bool BASE2>
 __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t tile, uint32_t word_tiles, uint32_t blocks, uint32_t at_once,
-                                                 uint32_t rows,
-                                                 const uint32_t *count, const int32_t *order, const void *targets, bool wide, uint32_t vocab,
-                                                 float *losses, float *lse, int64_t *tokens, float *logprobs) {
+                                                 uint32_t rows, const uint32_t *count, const int32_t *order, const void *targets, bool wide,
+                                                 uint32_t vocab, float *losses, float *lse, int64_t *tokens, float *logprobs) {
   __shared__ Sum joined[4];
-  const uint32_t row = blockIdx.x * (4 / WAVES) + threadIdx.x / (64 * WAVES), lane = threadIdx.x % (64 * WAVES);
+  const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
   const uint32_t all = count ? *count : rows;
-  if (row >= all) return;  // with WAVES of 4: all of the block
+  if (row >= all) return;  // with 256 lanes: all of the block
   uint32_t n = blocks, across = rows, two = 2 * rows;  // parts, and from one to the next and to the one after
   const Sum *from = parts + row;
   if (tile) {
@@ -221,20 +220,20 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t tile
   float value = PICK ? -__builtin_inff() : 0.0f;
   uint32_t place = PICK ? ~0u : 0;
 #pragma unroll 4
-  for (uint32_t i = lane; i < n; i += 64 * WAVES) {
+  for (uint32_t i = lane; i < n; i += LANES) {
     const Sum p = from[(uint64_t)(i >> 1) * two + (i & 1) * across];
     run.join(p.most, p.sum);
     join_value<PICK>(value, place, p.value, p.place);
   }
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
+  for (int k = 1; k < (LANES < 64 ? LANES : 64); k <<= 1) {
     run.join(__shfl_xor(run.most, k), __shfl_xor(run.sum, k));
     join_value<PICK>(value, place, __shfl_xor(value, k), __shfl_xor(place, k));
   }
-  if constexpr (WAVES > 1) {
+  if constexpr (LANES > 64) {
     if ((threadIdx.x & 63) == 0) joined[threadIdx.x >> 6] = Sum{run.most, run.sum, value, place};
     __syncthreads();
-    for (int w = 1; w < WAVES; w++) {
+    for (int w = 1; w < LANES / 64; w++) {
       run.join(joined[w].most, joined[w].sum);
       join_value<PICK>(value, place, joined[w].value, joined[w].place);
     }
@@ -304,7 +303,8 @@ Plan plan_of(const uor_trunk_head_args *s, bool pick) {
 template <class T, bool PICK>
 int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
   const Plan p = plan_of(s, PICK);
-  const auto join = [&](auto kernel, uint32_t each, const Sum *parts, uint32_t blocks, const uint32_t *count) {
+  const auto join = [&](auto kernel, uint32_t lanes, const Sum *parts, uint32_t blocks, const uint32_t *count) {
+    const uint32_t each = 256 / lanes;
     hipLaunchKernelGGL(kernel, dim3((s->rows + each - 1) / each), dim3(256), 0, stream, parts, p.tile, p.word_tiles, blocks, p.at_once, s->rows, count,
                        p.packed ? (const int32_t *)(work + p.order) : nullptr, s->targets, s->wide != 0, s->vocab, s->losses, s->lse, s->tokens,
                        s->logprobs);
@@ -315,7 +315,7 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     if (s->rows <= 16) hipLaunchKernelGGL((head_few<T, PICK, 1>), dim3(p.few), dim3(256), lds, stream, f);
     else if (s->rows <= 32) hipLaunchKernelGGL((head_few<T, PICK, 2>), dim3(p.few), dim3(256), lds, stream, f);
     else hipLaunchKernelGGL((head_few<T, PICK, 4>), dim3(p.few), dim3(256), lds, stream, f);
-    join(head_join<PICK, 4, false>, 1, f.parts, p.few, nullptr);
+    join(head_join<PICK, 256, false>, 256, f.parts, p.few, nullptr);
     return launched();
   }
   Scan a{};
@@ -348,10 +348,13 @@ int scan(const uor_trunk_head_args *s, char *work, hipStream_t stream) {
     else run(head_scan<T, S, PICK, ROWS, kOther>);
   });
   constexpr bool kBase2 = sizeof(T) == 2;
-  // More than 128 parts a row: by a block.
+  // More than 128 parts a row: by a block. Many rows of few parts: by four threads, which read those of many rows side by side
+  // (32,768 rows of 16 to 18 parts: 5 us, by a wavefront 20 to 24).
   const uint32_t row_tiles = (s->rows + p.tile - 1) / p.tile;
-  if (min((uint64_t)p.word_tiles, (uint64_t)p.blocks / row_tiles) > 64) join(head_join<PICK, 4, kBase2>, 1, a.parts, p.blocks, a.count);
-  else join(head_join<PICK, 1, kBase2>, 4, a.parts, p.blocks, a.count);
+  const uint64_t groups = min((uint64_t)p.word_tiles, (uint64_t)p.blocks / row_tiles);
+  if (groups > 64) join(head_join<PICK, 256, kBase2>, 256, a.parts, p.blocks, a.count);
+  else if (groups > 16 || s->rows < 4096) join(head_join<PICK, 64, kBase2>, 64, a.parts, p.blocks, a.count);
+  else join(head_join<PICK, 4, kBase2>, 4, a.parts, p.blocks, a.count);
   return launched();
 }
 
