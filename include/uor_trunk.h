@@ -147,7 +147,7 @@ int uor_trunk_norms_backward_async(const uor_trunk_norms_args *args, void *works
  *           in the rows' order.
  *   loss    z_tv = x_t . W_v,  lse_t = log sum_v e^z_tv,  loss_t = lse_t - z_t,target
  *           without keeping the logits z. A row whose target is outside 0 .. vocab - 1 takes no part: its
- *           loss, lse and gradient are 0, and nothing of it is read.
+ *           loss, lse and gradient are 0, and nothing that it holds reaches any result.
  *   choose  token_t = argmax_v z_tv, the lowest of equals,  logprob_t = z_t,token - lse_t.
  *           Of a row with no logit over -inf the token is 0.
  *
