@@ -149,14 +149,14 @@ def step(cfg, p, tokens, state, slots):
 
 
 def gradients(cfg, p, tokens, targets, offsets):
-    """(loss, {name: gradient}): the mean cross entropy of the rows' next tokens (target -1: none)."""
+    """(loss, {name: gradient}): the mean cross entropy of the rows' next tokens (a target outside the vocabulary: none)."""
     saved = []
     n = _prompt_rows(cfg, p, tokens, offsets, saved=saved)
     wanted = (targets >= 0) & (targets < cfg.vocab)
     count = wanted.sum().clamp(min=1)
     if cfg.keep_logits:
         log = torch.log_softmax(_logits(cfg, p, n), 1)
-        at = targets.clamp(min=0)[:, None]
+        at = torch.where(wanted, targets, 0)[:, None]
         loss = -(log.gather(1, at)[:, 0] * wanted).sum() / count
         d_logits = torch.exp(log)
         d_logits.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float32))
