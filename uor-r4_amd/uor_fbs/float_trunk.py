@@ -101,9 +101,31 @@ def _words(cfg, p):
     return p["head"].t().to(cfg.dtype, memory_format=torch.contiguous_format)
 
 
+def _embed(cfg, p, tokens):
+    """The tokens' rows. The table may be of any floating type, the tokens on another device, and both of more words and rows
+    than one lookup takes: a word is none for the other parts of the table, whose rows are zeros then."""
+    table = p["embed"] if p["embed"].dtype in trunk.DTYPES else p["embed"].to(cfg.dtype)
+    tokens = tokens.to(table.device)
+    if tokens.numel() <= trunk.MAX_ROWS and len(table) <= trunk.MAX_VOCAB:
+        return trunk.embed(tokens, table, dtype=cfg.dtype)
+    words = range(0, len(table), trunk.MAX_VOCAB)
+    return torch.cat([sum(trunk.embed(some - at, table[at:at + trunk.MAX_VOCAB], dtype=cfg.dtype) for at in words)
+                      for some in tokens.long().split(trunk.MAX_ROWS)])
+
+
+def _embed_backward(p, d_rows, tokens):
+    """The table's gradient."""
+    table, tokens = p["embed"], tokens.to(p["embed"].device)
+    if tokens.numel() <= trunk.MAX_ROWS and len(table) <= trunk.MAX_VOCAB:
+        return trunk.embed_backward(d_rows, tokens, table)
+    parts = list(zip(d_rows.split(trunk.MAX_ROWS), tokens.long().split(trunk.MAX_ROWS)))
+    return torch.cat([sum(trunk.embed_backward(d, some - at, table[at:at + trunk.MAX_VOCAB]) for d, some in parts)
+                      for at in range(0, len(table), trunk.MAX_VOCAB)])
+
+
 def _prompt_rows(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
     """The rows before the head of packed prompts."""
-    residual = trunk.embed(tokens, p["embed"], dtype=cfg.dtype)
+    residual = _embed(cfg, p, tokens)
     _, n = trunk.norms(residual, pre=p["first"])
     for i in range(cfg.layers):
         w = _layer(cfg, p, i)
@@ -130,7 +152,7 @@ def prompts(cfg, p, tokens, offsets, state=None, slots=None, saved=None):
 
 def _step_rows(cfg, p, tokens, state, slots):
     """The rows before the head of one more token of each session."""
-    residual = trunk.embed(tokens, p["embed"], dtype=cfg.dtype)
+    residual = _embed(cfg, p, tokens)
     _, n = trunk.norms(residual, pre=p["first"])
     for i in range(cfg.layers):
         w = _layer(cfg, p, i)
@@ -189,7 +211,7 @@ def gradients(cfg, p, tokens, targets, offsets):
         grads.update({f"{i}.{k}": v for k, v in layer.items()})
     first = trunk.norms_backward(d_residual, d_n, saved[0][0], pre=p["first"])
     grads["first"] = first.dpre
-    grads["embed"] = trunk.embed_backward(first.dresidual, tokens, p["embed"])
+    grads["embed"] = _embed_backward(p, first.dresidual, tokens)
     return loss, grads
 
 
