@@ -605,15 +605,17 @@ def embed_backward(dy, tokens, table, *, scale=1.0):
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, table, scale, dtype):
-        ctx.save_for_backward(tokens, table)
-        ctx.scale = scale
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.table = scale, (table.shape, table.dtype, table.device)  # the table itself may change before the gradient
         return embed(tokens, table, scale=scale, dtype=dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        tokens, table = ctx.saved_tensors
-        return None, embed_backward(dy, tokens, table, scale=ctx.scale), None, None
+        tokens, = ctx.saved_tensors
+        shape, dtype, device = ctx.table
+        like = torch.empty((), dtype=dtype, device=device).expand(shape)
+        return None, embed_backward(dy, tokens, like, scale=ctx.scale), None, None
 
 
 def _head_args(x, weight, targets):
