@@ -140,22 +140,30 @@ def lib():
         if not os.path.exists(LIB_PATH):
             raise TrunkError(f"{LIB_PATH} is not built (make -C uor-r4_amd/csrc)")
         L = C.CDLL(LIB_PATH)
-        L.uor_trunk_abi_version.restype = U32
-        L.uor_trunk_last_error.restype = C.c_char_p
-        for name, struct, forms in _FORMS:
-            size = getattr(L, f"uor_trunk_sizeof_{name}")
-            size.restype = C.c_uint64
-            if size() != C.sizeof(struct) or L.uor_trunk_abi_version() != ABI_VERSION:
-                raise TrunkError(f"{LIB_PATH} is of another version: build it again")
-            for form, needs in forms.items():
-                call, bytes_of = getattr(L, f"uor_trunk_{form}_async"), None
-                call.argtypes = [C.POINTER(struct)] + ([P, C.c_uint64] if needs else []) + [P]
-                if needs:
-                    bytes_of = getattr(L, f"uor_trunk_{form}_workspace_bytes")
-                    bytes_of.argtypes, bytes_of.restype = [C.POINTER(struct)], C.c_uint64
-                _calls[form] = call, bytes_of
+        try:
+            _bind(L)
+        except AttributeError:  # a call that it does not have
+            raise TrunkError(f"{LIB_PATH} is of another version: build it again") from None
         _lib = L
     return _lib
+
+
+def _bind(L):
+    """The library's calls and what they take."""
+    L.uor_trunk_abi_version.restype = U32
+    L.uor_trunk_last_error.restype = C.c_char_p
+    for name, struct, forms in _FORMS:
+        size = getattr(L, f"uor_trunk_sizeof_{name}")
+        size.restype = C.c_uint64
+        if size() != C.sizeof(struct) or L.uor_trunk_abi_version() != ABI_VERSION:
+            raise TrunkError(f"{LIB_PATH} is of another version: build it again")
+        for form, needs in forms.items():
+            call, bytes_of = getattr(L, f"uor_trunk_{form}_async"), None
+            call.argtypes = [C.POINTER(struct)] + ([P, C.c_uint64] if needs else []) + [P]
+            if needs:
+                bytes_of = getattr(L, f"uor_trunk_{form}_workspace_bytes")
+                bytes_of.argtypes, bytes_of.restype = [C.POINTER(struct)], C.c_uint64
+            _calls[form] = call, bytes_of
 
 
 def _call(name, args, index):
