@@ -17,7 +17,7 @@ raises.
 ``scan``, ``conv``, ``norms``, ``embed`` and ``loss`` take part in autograd: where an input requires a gradient, the outputs
 have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which a
 program may call by itself (it is not differentiable). The steps update their states in place and have
-no gradient: going back through one raises. Nothing is kept between calls. Results are the same each
+no gradient: going back through one raises, and so does a forward-mode derivative of any call. Nothing is kept between calls. Results are the same each
 time, bit for bit.
 
 A training step that is captured into a graph calls ``*_backward`` by itself, or has no eager graph of the
@@ -123,6 +123,7 @@ class LossGrads(NamedTuple):
 
 
 _Tensor = torch.Tensor
+_forward = torch.autograd.forward_ad
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # none without a HIP device to call it for
 # Arguments and, of each call that takes them, whether it wants scratch memory.
 _FORMS = (("scan", CScan, {"scan": True, "scan_backward": True, "scan_step": False}),
@@ -218,8 +219,16 @@ def _dense(name, t, dtype, shape):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _no_tangents(tensors):
+    """No call has a forward-mode derivative: one that is asked for would be lost."""
+    if _forward._current_level >= 0:
+        for t in tensors:
+            _want(t is None or _forward.unpack_dual(t).tangent is None, "forward-mode derivatives are not computed")
+
+
 def _one_device(*tensors):
     """The index of the tensors' device: one HIP device for all of them."""
+    _no_tangents(tensors)
     index = None
     for t in tensors:
         if t is not None:
@@ -279,6 +288,7 @@ def _tracked(tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
+                _no_tangents(tensors)
                 return True
     return False
 
