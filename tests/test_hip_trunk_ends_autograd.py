@@ -19,3 +19,20 @@ def test_a_table_may_change_before_its_gradient(strided, dtype):  # noqa: F811
         table.mul_(2.0)
     y.backward(dy)
     assert table.grad.dtype == dtype and torch.equal(table.grad, trunk.embed_backward(dy, tokens, table.detach(), scale=1.5))
+
+
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_the_choice_has_no_gradient_and_says_so(which, dtype):  # noqa: F811
+    x, weight, _, _ = loss_case(dtype, 20, 90, 16)
+    want = trunk.choose(x, weight)
+    (x if which == "x" else weight).requires_grad_()
+    tokens, logprobs = trunk.choose(x, weight)
+    assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1]) and not tokens.requires_grad
+    with pytest.raises(trunk.TrunkError, match="choose has no gradient"):
+        (logprobs.sum() + x.float().sum()).backward()
+    with torch.no_grad():
+        assert not trunk.choose(x, weight)[1].requires_grad
+    # What the refusal names instead.
+    losses, _ = trunk.loss(x, weight, tokens)
+    losses.sum().backward()
+    assert (x if which == "x" else weight).grad.abs().sum() > 0

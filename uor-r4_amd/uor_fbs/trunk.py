@@ -17,8 +17,8 @@ raises.
 ``scan``, ``conv``, ``norms``, ``embed`` and ``loss`` take part in autograd: where an input requires a gradient, the outputs
 have ``*_backward`` as theirs, which computes the gradients from the call's own inputs, and which a
 program may call by itself (it is not differentiable). The steps update their states in place and have
-no gradient: going back through one raises, and so does a forward-mode derivative of any call. Nothing is kept between calls. Results are the same each
-time, bit for bit.
+no gradient, nor has ``choose``: going back through one raises, and so does a forward-mode derivative of
+any call. Nothing is kept between calls. Results are the same each time, bit for bit.
 
 A training step that is captured into a graph calls ``*_backward`` by itself, or has no eager graph of the
 same leaves alive meanwhile: torch would order their gradients after the other graph's stream.
@@ -293,17 +293,20 @@ def _tracked(tensors):
     return False
 
 
-class _Step(torch.autograd.Function):
-    """A step's outputs, of which there is no gradient."""
+_IN_PLACE = "its states are updated in place"
+
+
+class _NoGradient(torch.autograd.Function):
+    """The outputs of a call that has no gradient, and why."""
 
     @staticmethod
-    def forward(ctx, name, call, *inputs):
-        ctx.name = name
+    def forward(ctx, name, why, call, *inputs):
+        ctx.text = f"{name} has no gradient: {why}"
         return call()
 
     @staticmethod
     def backward(ctx, *grads):
-        raise TrunkError(f"{ctx.name} has no gradient: its states are updated in place")
+        raise TrunkError(ctx.text)
 
 
 _changed = torch.autograd.graph.increment_version  # of states in place, for autograd to see
@@ -391,7 +394,7 @@ def scan_step(x, dt, A, B, C, states, *, slots=None, D=None, dt_bias=None):
     _want(isinstance(states, torch.Tensor) and states.dtype == torch.float32 and states.dim() == 4 and states.shape[1:] == inner
           and states.is_contiguous(), "states is no dense float32 tensor of (slots, {}, {}, {})", *inner)
     if _tracked((states, *keep)):
-        return _Step.apply("scan_step", lambda: scan_step(x, dt, A, B, C, states, slots=slots, D=D, dt_bias=dt_bias), states, *keep)
+        return _NoGradient.apply("scan_step", _IN_PLACE, lambda: scan_step(x, dt, A, B, C, states, slots=slots, D=D, dt_bias=dt_bias), states, *keep)
     slots = _index(slots, a.tokens, states.shape[0])
     index = _one_device(states, slots, *keep)
     y = _make(x)
@@ -477,7 +480,7 @@ def conv_step(x, weight, states, bias=None, *, slots=None, silu=True):
     _want(isinstance(states, torch.Tensor) and states.dtype == x.dtype and states.dim() == 3 and states.shape[1:] == inner
           and states.is_contiguous(), "states is no dense {} tensor of (slots, {}, {})", x.dtype, *inner)
     if _tracked((states, *keep)):
-        return _Step.apply("conv_step", lambda: conv_step(x, weight, states, bias, slots=slots, silu=silu), states, *keep)
+        return _NoGradient.apply("conv_step", _IN_PLACE, lambda: conv_step(x, weight, states, bias, slots=slots, silu=silu), states, *keep)
     slots = _index(slots, a.tokens, states.shape[0])
     index = _one_device(states, slots, *keep)
     y = _make(x)
@@ -705,9 +708,12 @@ class _Loss(torch.autograd.Function):
 
 def choose(x, weight):
     """(tokens, logprobs): of each row of x (rows, width) the word of ``weight`` (vocab, width; x's type) with the
-    largest logit, the lowest of equals (int64), and its log probability (float32), without keeping the logits. They
-    have no gradient. Of a row with no logit over -inf the token is 0; logits that are no number are not chosen."""
+    largest logit, the lowest of equals (int64), and its log probability (float32), without keeping the logits. The
+    log probability has no gradient: going back through it raises (``loss`` of the tokens has one). Of a row with no
+    logit over -inf the token is 0; logits that are no number are not chosen."""
     a, keep = _head_args(x, weight, None)
+    if _tracked((x, weight)):
+        return _NoGradient.apply("choose", "loss gives a token's log probability with one", lambda: choose(x, weight), x, weight)
     index = _one_device(*keep)
     tokens = torch.empty(a.rows, dtype=torch.int64, device=x.device)
     logprobs = torch.empty(a.rows, dtype=torch.float32, device=x.device)
