@@ -181,7 +181,8 @@ int uor_trunk_embed_backward_async(const uor_trunk_embed_args *args, void *works
 /* dlosses and dlse may be NULL for zeros. With G_tv = (dlosses_t + dlse_t) e^(z_tv - lse_t) - dlosses_t
  * [v is t's target]: dx = G W, dweight = G^T x. `lse` is the call's own. G is rounded to the type of x but for
  * the targets'.
- * Workspaces are aligned to 256 bytes. */
+ * Workspaces are aligned to 256 bytes. Their sizes are those of the very call: they go by the types, sizes and strides,
+ * by the alignment of x and weight, and by which of dx and dweight are wanted. */
 typedef struct {
   int32_t device;
   uint32_t dtype, dweight_dtype;        /* of x, weight and dx; of dweight */

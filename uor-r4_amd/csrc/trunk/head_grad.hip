@@ -536,14 +536,15 @@ GradPlan grad_plan(const uor_trunk_head_args *s) {
   const bool rows_outside = p.all_rows - p.rows > p.all_words - p.words;
   p.x_rows = rows_outside ? p.rows : p.all_rows, p.w_rows = rows_outside ? p.all_words : p.words;
   p.puts_x = p.tile_m < Large::kM && p.words >= p.all_words, p.puts_w = p.rows >= p.all_rows;
-  const uint64_t x_units = (uint64_t)p.rows / p.tile_m * (p.words / deep), w_units = (uint64_t)p.words / p.tile_m * (p.rows / deep);
+  const uint64_t x_units = s->dx ? (uint64_t)p.rows / p.tile_m * (p.words / deep) : 0;
+  const uint64_t w_units = s->dweight ? (uint64_t)p.words / p.tile_m * (p.rows / deep) : 0;
   const uint64_t units = x_units > w_units ? x_units : w_units, groups = p.at_once / p.n_tiles, most = units < 8 ? 1 : units / 4;  // see SplitShares
   Scratch at;
   p.g = at.take((uint64_t)p.rows * p.words * size);
-  p.dx = at.take(p.puts_x ? 0 : 4ull * p.x_rows * p.n_pitch);
-  p.dw = at.take(p.puts_w ? 0 : 4ull * p.w_rows * p.n_pitch);
+  p.dx = at.take(!s->dx || p.puts_x ? 0 : 4ull * p.x_rows * p.n_pitch);
+  p.dw = at.take(!s->dweight || p.puts_w ? 0 : 4ull * p.w_rows * p.n_pitch);
   p.slots = at.take(8ull * (groups < most ? groups : most) * p.n_tiles * (p.tile_m * p.tile_n + kSlotPad));
-  p.word_terms = at.take(size == 2 ? 4ull * p.words * p.n_pitch : 0);
+  p.word_terms = at.take(size == 2 && s->dweight ? 4ull * p.words * p.n_pitch : 0);
   p.w = at.take(p.lay ? s->vocab * up(s->width * size, 64) : 0);
   p.x = at.take(up(p.all_rows, p.rows) * up(s->width * size, 64));
   p.order = at.take(4ull * p.all_rows);
