@@ -12,13 +12,13 @@ struct Matrix {
 // What is known of a row's softmax: its largest logit, the sum of e^(logit - largest), and the target's logit,
 // or the largest one's value and place. The largest one is in base 2 (times log2 e, rounded) where exponents are formed in
 // one instruction, fma(z, log2 e, -most); otherwise, in 32 bits and for few rows, the logits are subtracted first, so that
-// the largest one's share is 1 exactly and the loss of a sure row is right to its own size.
+// the largest one's share is 1 exactly and the loss of a sure row is right to its own size. In base 2 that share is what the
+// rounding of `most` left, which the loss takes back, as it divides by the same log2 e: of 32 bits, 1.3e-8 of itself off. The
+// true one's inverse left 1.3e-8 of the logit: losses of sure rows were -4e-5 at a logit of 3,000.
 struct Sum {
   float most, sum, value;
   uint32_t place;
 };
-
-constexpr double kLn2 = 0.6931471805599453;
 
 __host__ __device__ constexpr uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 

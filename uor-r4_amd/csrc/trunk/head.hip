@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void head_join(const Sum *parts, uint32_t tile
     }
   }
   if (lane) return;
-  const double most = BASE2 ? (double)run.most * kLn2 : (double)run.most, rest = log((double)run.sum);
+  const double most = BASE2 ? (double)run.most / (double)kLog2e : (double)run.most, rest = log((double)run.sum);
   if constexpr (PICK) {
     tokens[row] = place == ~0u ? 0 : place;
     logprobs[row] = (float)((double)value - most - rest);

@@ -53,11 +53,11 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *scratch) {
 }
 
 // A gradient's factors of a packed row. In bf16 G = e2 2^(z log2 e - base) for e2 = (dloss + dlse) 2^(what the
-// rounding of base = lse log2 e left); in 32 bits G = e2 e^(z - base) for base = lse. Less dloss at the target.
+// rounding of base = lse log2 e left, with log2 e of 32 bits as the exponents have it); in 32 bits G = e2 e^(z - base) for base = lse. Less dloss at the target.
 template <class T>
 __device__ __forceinline__ float4 factors_of(float lse, float dloss, float dlse) {
   if constexpr (sizeof(T) == 4) return {lse, dloss + dlse, dloss, 0.0f};
-  const double base = (double)lse * 1.4426950408889634;
+  const double base = (double)lse * (double)kLog2e;
   const float hi = (float)base, all = dloss + dlse;
   const float left = hi - hi == 0.0f ? (float)(hi - base) : 0.0f;
   return {hi, all * fmaf(left, 0.693147181f, 1.0f), dloss, 0.0f};
