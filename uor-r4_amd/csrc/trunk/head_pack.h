@@ -17,6 +17,7 @@ struct Pack {
   const void *x, *targets;
   bool wide;              // targets are of 64 bits
   const uint32_t *counts; // rows with a target in each block's share, or NULL: each block counts for itself
+  bool summed;            // of the shares before it instead
   char *to;               // [pieces][panels][piece][64 bytes]
   int32_t *order, *target;  // [rows up to 256]: a packed row's own row and target (-1: none)
   uint32_t *count;          // how many rows are packed
@@ -39,6 +40,38 @@ static __global__ __launch_bounds__(64) void head_count(const void *targets, boo
   const bool there = row < rows && target_of(targets, wide, row, vocab) >= 0;
   const uint64_t which = __ballot(there);
   if (threadIdx.x == 0) counts[blockIdx.x] = __builtin_popcountll(which);
+}
+
+// Of many blocks none adds up all those before it, which would go by their square: one block puts the sums so far in the counts'
+// places, each of its threads those of a stretch of them. Of few that is a launch more for nothing. Losses over 100 words in bf16: 65,536
+// rows of 64 26 us, each block adding up for itself 24; 131,072 of 64 35 and 35, of 512 83 and 88; 262,144 of 512 157 and 198; 2^20 of
+// 256 320 and 540; 2^24 of 64 2,260 and 9,800.
+constexpr uint32_t kManyShares = 2048;
+static __global__ __launch_bounds__(1024) void head_starts(uint32_t *counts, uint32_t blocks) {
+  __shared__ uint32_t sums[16];
+  const uint32_t each = (blocks + 4095) / 4096 * 4, first = threadIdx.x * each, end = min(first + each, blocks);  // the array has whole fours
+  uint32_t mine = 0;
+#pragma unroll 8
+  for (uint32_t i = first; i < end; i += 4) {
+    const u32x4 v = *(const u32x4 *)(counts + i);
+    mine += v[0] + v[1] + v[2] + v[3];
+  }
+  uint32_t before = mine;
+#pragma unroll
+  for (uint32_t k = 1; k < 64; k <<= 1) {
+    const uint32_t v = __shfl_up(before, k);
+    before += (threadIdx.x & 63) >= k ? v : 0;
+  }
+  if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6] = before;
+  __syncthreads();
+  before -= mine;
+  for (uint32_t w = 0; w < threadIdx.x >> 6; w++) before += sums[w];
+#pragma unroll 8
+  for (uint32_t i = first; i < end; i += 4) {
+    const u32x4 v = *(const u32x4 *)(counts + i);
+    *(u32x4 *)(counts + i) = u32x4{before, before + v[0], before + v[0] + v[1], before + v[0] + v[1] + v[2]};
+    before += v[0] + v[1] + v[2] + v[3];
+  }
 }
 
 // The sum over a block of 256 threads, to all of them.
@@ -74,12 +107,16 @@ __global__ __launch_bounds__(256) void head_pack(Pack a) {
   __shared__ uint32_t scratch[4], from[kPackRows], none[kPackRows];
   const uint32_t first = blockIdx.x * kPackRows;
   uint32_t before = 0;
-  if (a.counts) {
-    for (uint32_t i = threadIdx.x; i < blockIdx.x; i += 256) before += a.counts[i];
+  if (a.summed) {
+    before = a.counts[blockIdx.x];
   } else {
-    for (uint32_t i = threadIdx.x; i < first; i += 256) before += target_of(a.targets, a.wide, i, a.vocab) >= 0;
+    if (a.counts) {
+      for (uint32_t i = threadIdx.x; i < blockIdx.x; i += 256) before += a.counts[i];
+    } else {
+      for (uint32_t i = threadIdx.x; i < first; i += 256) before += target_of(a.targets, a.wide, i, a.vocab) >= 0;
+    }
+    before = block_sum(before, scratch);
   }
-  before = block_sum(before, scratch);
   const uint32_t row = first + threadIdx.x;
   // The block's pieces of each row; the first block of a share writes what there is one of a row.
   const uint32_t panels = (a.width + kDeep<T> - 1) / kDeep<T>, piece0 = blockIdx.y * kPackPieces;
@@ -159,6 +196,10 @@ inline void pack(Pack k, uint32_t *counts, hipStream_t stream) {
   if (k.rows > 4096) {  // else each block counts the rows before its own by itself
     hipLaunchKernelGGL(head_count, dim3(blocks), dim3(64), 0, stream, k.targets, k.wide, k.rows, k.vocab, counts);
     k.counts = counts;
+    if (blocks >= kManyShares) {
+      hipLaunchKernelGGL(head_starts, dim3(1), dim3(1024), 0, stream, counts, blocks);
+      k.summed = true;
+    }
   }
   hipLaunchKernelGGL((head_pack<T, GRAD>), dim3(blocks, (panels * 4 + kPackPieces - 1) / kPackPieces), dim3(256), 0, stream, k);
 }
