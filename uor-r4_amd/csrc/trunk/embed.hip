@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void embed_rows(Embed a) {
         const uint64_t row = base + k * kRows;
         if (row >= a.rows) break;
         v[k] = token[k] < a.vocab ? v[k] * a.scale : f32x8{};
-        // Past the caches, which hold the table meanwhile: 262,144 rows of 256 33.6 us, through them 36.4; 131,072 of 512 from
+        // In bf16 past the caches, which hold the table meanwhile: 262,144 rows of 256 33.6 us, through them 36.4; 131,072 of 512 from
         // 131,072 words 29.8 and 35.5.
         store_past<T>((T *)a.y + row * a.width, col, a.width, __builtin_convertvector(v[k], V8<T>));
       }

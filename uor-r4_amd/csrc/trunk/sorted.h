@@ -190,12 +190,35 @@ static __global__ __launch_bounds__(kSortThreads) void sort_place(Digit a) {
 // lane's before it, which writes the same: rows of any width are read and written eight values at a time.
 __device__ __forceinline__ uint32_t eight_of(uint32_t i, uint32_t width) { return width < 8 ? 8 * i : min(8 * i, width - 8); }
 
-// Eight values of a row to memory past the caches, which hold what is read meanwhile. Zeros of a gradient of 131,072 words
-// of 1,024, most of which do not occur, written so: 82 us, through the caches 107.
+// Eight values of a row to memory, in bf16 past the caches, which hold what is read meanwhile. In f32 a lane's values are two
+// stores, each of which has every other 16 bytes of its lines, so that they go through the caches, where lines become whole: lookups of
+// 262,144 rows of 256 80 us, past them 99; of 32,768 13.6 and 12.0.
 template <class T>
 __device__ __forceinline__ void store_past(T *row, uint32_t col, uint32_t cols, V8<T> v) {
-  if (col + 8 <= cols) __builtin_nontemporal_store(v, (typename Loose<T, 8>::At *)(row + col));
+  if (sizeof(T) == 2 && col + 8 <= cols) __builtin_nontemporal_store(v, (typename Loose<T, 8>::At *)(row + col));
   else store_some<T, 8>(row, col, cols, v);
+}
+// Zeros of a row's 8 LANES columns, the lanes' 16 bytes next to each other; the last ones are some of those before too. In bf16 past the
+// caches: of 131,072 words of 1,024, most of which do not occur, 82 us, through them 107. In f32 through them, as whole rows past
+// them gain where rows are whole lines (131,072 of 1,024 for 777 rows 139 us, through them 143; for 16,384 161 and 199) and lose where they
+// are not or are short (60,000 of 1,001 79 and 50; 262,144 of 256 88 and 77). With the lanes' 16 bytes 32 apart the first took 323
+// past the caches and 148 through them.
+template <class T, int LANES>
+__device__ __forceinline__ void write_zeros(T *row, uint32_t cols, uint32_t lane) {
+  constexpr uint32_t kEach = 16 / sizeof(T), kSlice = 8 * LANES;
+  const uint32_t first = blockIdx.y * kSlice;
+#pragma unroll
+  for (uint32_t c = 0; c < kSlice; c += kEach * LANES) {
+    const uint32_t col = first + c + lane * kEach;
+    if (col >= cols) continue;
+    if (cols < kEach) {
+      store_some<T, kEach>(row, col, cols, {});
+      continue;
+    }
+    T *at = row + min(col, cols - kEach);
+    if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(typename Loose<T, kEach>::Values{}, (typename Loose<T, kEach>::At *)at);
+    else loose<T, kEach>(at, {});
+  }
 }
 
 // The first of the sorted rows whose word is not before `key`, looked for by a whole wavefront.
@@ -220,9 +243,7 @@ __global__ __launch_bounds__(256) void sorted_sums(Sums a) {
     }
     const uint64_t none = __ballot(word < a.words && (lo == a.rows || a.keys[lo] != key));
     for (uint32_t k = threadIdx.x / LANES; k < 64; k += 256 / LANES)
-      if (none >> k & 1)
-        if ((blockIdx.y * LANES + lane) * 8 < a.width)
-          store_past<R>((R *)a.to + (int64_t)(word0 + k) * a.pitch, eight_of(blockIdx.y * LANES + lane, a.width), a.width, V8<R>{});
+      if (none >> k & 1) write_zeros<R, LANES>((R *)a.to + (int64_t)(word0 + k) * a.pitch, a.width, lane);
     return;
   }
   const uint32_t group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, eight = blockIdx.y * LANES + lane, col = eight_of(eight, a.width);
