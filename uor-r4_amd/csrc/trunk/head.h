@@ -115,8 +115,8 @@ inline bool as_it_lies(const void *p, int64_t stride, uint32_t rows, uint32_t wi
          (rows <= 1 || (stride * size % 16 == 0 && stride * (int64_t)size < (1 << 23)));
 }
 // From how many rows on a matrix is laid out by panels, whose rows could be read as they lie: it is then read
-// by many row tiles. 8,192 rows at width 1,024 and 131,072 words: 2,103 us, as it lies 2,152; loss and gradients 9,489
-// and 9,579.
+// by many row tiles. 8,192 rows at width 1,024 and 131,072 words: 1,920 us, as it lies 2,010; loss and gradients 8,475
+// and 8,550.
 constexpr uint32_t kLayRows = 1024;
 inline bool laid_out(const uor_trunk_head_args *s) { return s->rows >= kLayRows || !as_it_lies(s->weight, s->w_stride, s->vocab, s->width, s->dtype); }
 // A call's tiles. Small ones where large ones would leave some compute units idle (333 rows over 4,099 words of 100 in 32 bits: 18 us, 26

@@ -486,8 +486,8 @@ namespace {
 
 // Bytes of a piece's G. Larger pieces read and write the sums so far less often; this much is a small part of
 // the memory of the card. Loss and gradients of 32,768 rows (a quarter without a target) at width 256 and 32,768
-// words: 256 MB 3,447 us, 512 MB 2,827, 1 GB 2,612, 2 GB 2,591; 8,192 rows at width 1,024 and 131,072 words: 9,019,
-// 8,796, 8,674 and 8,758.
+// words: 256 MB 2,615 us, 512 MB 2,350, 1 GB 2,150 to 2,205, 2 GB 2,205 to 2,260; 8,192 rows at width 1,024 and 131,072
+// words: 8,490, 8,555, 8,475 and 8,450.
 constexpr uint64_t kPiece = 1ull << 30;
 
 struct GradPlan {

@@ -352,7 +352,7 @@ inline void with_lanes(uint32_t width, F f) {
 
 // Host side: where a sort and its sums have what, `bytes` in all.
 struct SortPlan {
-  uint32_t passes, bits, blocks, share;  // passes 0: in one block
+  uint32_t passes, bits, blocks, share;  // passes 0: by counting, in one launch
   uint32_t length, groups;
   uint64_t keys[2], order[2], counts, parts, bytes;
 };

@@ -9,7 +9,7 @@
 // Matrices that the kernels lay out themselves lie by panels: 64 bytes of each row, row after row, and then the rows'
 // next 64 bytes. A stage's part of 256 rows is then 16 KB in one piece along the summed axis, and 2 KB pieces across.
 // Rows that lie 2 KB apart are read by half lines of the caches, every line twice: 8,192 x 131,072 logits of width
-// 1,024 took 333 M requests to the L2 caches as rows and 201 M as panels (2.15 and 2.05 ms).
+// 1,024 took 333 M requests to the L2 caches as rows and 201 M as panels (2.01 and 1.92 ms).
 //
 // An operand lies along the summed axis (its values for one row or column of the result next to each
 // other) or across it (a row apart). Along, a stage's rows are 64 bytes, and a lane reads the 16 bytes
